@@ -37,6 +37,12 @@ EXPORTS = (
     "bs_silu_mul",
     "bs_kernel_launches",
     "bs_argmax_rows",
+    "bs_window_attention_batched",
+    "bs_window_attention_batched_workspace_bytes",
+    "bs_window_prefill_attention",
+    "bs_window_prefill_attention_workspace_bytes",
+    "bs_rotary_append",
+    "bs_copy_blocks",
 )
 
 _i32, _i64, _u64, _p, _dbl = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_double
@@ -109,6 +115,33 @@ _SIGNATURES = {
     "bs_silu_mul": ([_p, _i64, _i64, _i64, _i32, _p, _p], ctypes.c_int),
     "bs_kernel_launches": ([], ctypes.c_uint64),
     "bs_argmax_rows": ([_p, _i64, _i64, _i64, _i32, _p, _p], ctypes.c_int),
+    "bs_window_attention_batched": (
+        [_p, _i64, _p, _p, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _i32, _dbl, _i64, _i64, _p, _i64, _p, _u64, _p, _p],
+        ctypes.c_int,
+    ),
+    "bs_window_attention_batched_workspace_bytes": (
+        [_i64, _i64, _i64, _i64, _i64, _i64, _i32, _i64, _i64, ctypes.POINTER(_u64)],
+        ctypes.c_int,
+    ),
+    "bs_window_prefill_attention": (
+        [_p, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i64, _i32, _dbl, _i64, _i64, _p, _i64, _p, _u64, _p, _p],
+        ctypes.c_int,
+    ),
+    "bs_window_prefill_attention_workspace_bytes": (
+        [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i64, _i64,
+         ctypes.POINTER(_u64)],
+        ctypes.c_int,
+    ),
+    "bs_rotary_append": (
+        [_p, _i64, _i32, _p, _i64, _i32, _dbl, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _i32,
+         _i64, _i64, _p, _p],
+        ctypes.c_int,
+    ),
+    "bs_copy_blocks": (
+        [_p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _p, _p], ctypes.c_int,
+    ),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -106,6 +106,32 @@ class PagedBackend:
         self._sequences[seq_id] = _Sequence(cache, deque(prompt_tokens))
         return seq_id
 
+    def fork_sequence(self, seq_id: int, prompt_tokens: list[int]) -> int:
+        """Starts a sequence that continues seq_id's tokens so far with
+        ``prompt_tokens`` (a shared prompt, another turn of a conversation): what
+        is cached for seq_id is shared, not computed again.  Without
+        ``prompt_tokens`` the new sequence generates what seq_id would.  A step
+        that seq_id still runs in must be finished first."""
+        parent = self._sequences[seq_id]
+        if parent.feeds is not None:
+            raise RuntimeError(f"sequence {seq_id} has an unfinished step")
+        if parent.finished and not prompt_tokens:
+            raise RuntimeError(f"sequence {seq_id} has finished: a fork needs new tokens")
+        child_id = next(self._ids)
+        child = _Sequence(self._pool.fork(parent.cache, child_id), deque(parent.pending))
+        if parent.next_token is not None:
+            if prompt_tokens:
+                child.pending.append(parent.next_token)
+            else:
+                child.next_token = parent.next_token
+        child.pending.extend(prompt_tokens)
+        self._sequences[child_id] = child
+        return child_id
+
+    def compact(self) -> int:
+        """Moves the cache blocks in use to the lowest ids; returns how many moved."""
+        return self._pool.compact()
+
     def step(self) -> dict[int, StepOutput]:
         launched = self.launch()
         return self.finish(launched) if launched is not None else {}

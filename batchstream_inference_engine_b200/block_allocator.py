@@ -9,11 +9,21 @@ every table into an int32 tensor ``[max_seqs, max_blocks_per_seq]`` on the GPU
 (one row per live sequence), so kernels read block tables and context lengths
 from device memory; only new table entries cross PCIe, batched into one copy per
 ``sync_device()``.
+
+Three operations go beyond the reference: ``fork`` starts a sequence from the
+cached tokens of another (whole blocks are shared and reference-counted, the last
+partial one is copied), ``trim`` frees the blocks that a sliding window has left
+behind, and ``compact`` renumbers the blocks in use to the lowest ids.  ``fork``
+and ``compact`` return the (source, destination) block copies that the caller owes
+the pool (``ops.copy_blocks``) before the next step.
 """
 
 from __future__ import annotations
 
 import torch
+
+
+EMPTY_BLOCK = -1  # table entry of a trimmed block
 
 
 class OutOfBlocks(RuntimeError):
@@ -27,6 +37,8 @@ class BlockAllocator:
         self._block_size = block_size
         self._free = list(range(num_blocks))
         self._tables: dict[int, list[int]] = {}
+        self._refs: dict[int, int] = {}  # tables that hold a block, where more than one does
+        self._trimmed: dict[int, int] = {}  # entries below this were looked at by trim
         self.num_blocks = num_blocks
         # Device mirror (optional).
         self._device = torch.device(device) if device is not None else None
@@ -84,11 +96,98 @@ class BlockAllocator:
         return self._tables[seq_id][block_index], offset
 
     def free(self, seq_id: int) -> None:
-        self._free.extend(self._tables.pop(seq_id))
+        for block in self._tables.pop(seq_id):
+            self._release(block)
+        self._trimmed.pop(seq_id, None)
         row = self._rows.pop(seq_id, None)
         if row is not None:
             self._synced.pop(seq_id, None)
             self._free_rows.append(row)
+
+    # ---------------------------------------------------------------- forks, windows, compaction
+
+    def _release(self, block: int) -> int:
+        """Drops one table's hold on a block; 1 when that freed it."""
+        if block == EMPTY_BLOCK:
+            return 0
+        refs = self._refs.get(block, 1)
+        if refs > 1:
+            if refs == 2:
+                del self._refs[block]
+            else:
+                self._refs[block] = refs - 1
+            return 0
+        self._free.append(block)
+        return 1
+
+    def fork(self, seq_id: int, child_id: int, tokens: int) -> list[tuple[int, int]]:
+        """Starts child_id with the first `tokens` tokens of seq_id: its whole
+        blocks are shared (neither sequence writes them again), and a last
+        partial block is taken from the free list for the child.  Returns that
+        block's (source, destination) copy, if any.  Takes nothing and raises
+        OutOfBlocks when no block or device table row is free."""
+        table = self._tables[seq_id]
+        if child_id in self._tables:
+            raise ValueError(f"sequence {child_id} already exists")
+        whole, tail = divmod(tokens, self._block_size)
+        if tokens < 0 or whole + (tail > 0) > len(table):
+            raise ValueError(f"sequence {seq_id} has no blocks for {tokens} tokens")
+        copied = tail > 0 and table[whole] != EMPTY_BLOCK
+        if copied and not self._free:
+            raise OutOfBlocks(f"forking sequence {seq_id} needs a block but none is free")
+        if self.device_tables is not None:
+            if not self._free_rows:
+                raise OutOfBlocks(f"all {self.max_seqs} device table rows are in use")
+            self._rows[child_id] = self._free_rows.pop()
+            self._synced[child_id] = 0
+        child = table[:whole]
+        for block in child:
+            if block != EMPTY_BLOCK:
+                self._refs[block] = self._refs.get(block, 1) + 1
+        if seq_id in self._trimmed:
+            self._trimmed[child_id] = min(self._trimmed[seq_id], whole)
+        pairs = []
+        if copied:
+            child.append(self._free.pop())
+            pairs.append((table[whole], child[-1]))
+        elif tail:
+            child.append(EMPTY_BLOCK)
+        self._tables[child_id] = child
+        return pairs
+
+    def trim(self, seq_id: int, first_token: int, keep_first: int = 0) -> int:
+        """Gives up the blocks of seq_id whose tokens all lie before first_token
+        and at or past keep_first (the tokens between the sinks and the window);
+        their table entries become EMPTY_BLOCK.  Returns how many blocks that
+        freed (a block that a fork still holds stays in use)."""
+        table = self._tables[seq_id]
+        end = min(first_token // self._block_size, len(table))
+        begin = max(self._trimmed.get(seq_id, 0), -(-keep_first // self._block_size))
+        freed = 0
+        for i in range(begin, end):
+            freed += self._release(table[i])
+            table[i] = EMPTY_BLOCK
+        if end > begin:
+            self._trimmed[seq_id] = end
+        return freed
+
+    def compact(self) -> list[tuple[int, int]]:
+        """Renumbers the blocks in use to ids below their count: each block above
+        takes the place of a free one below, the lowest first.  Returns the
+        (source, destination) copies; no block is both."""
+        used = sorted({b for table in self._tables.values() for b in table} - {EMPTY_BLOCK})
+        count = len(used)
+        sources = [b for b in used if b >= count]
+        moved = dict(zip(sources, sorted(b for b in self._free if b < count)))
+        for seq_id, table in self._tables.items():
+            if any(b in moved for b in table):
+                self._tables[seq_id][:] = [moved.get(b, b) for b in table]
+                if seq_id in self._synced:
+                    self._synced[seq_id] = 0
+        self._refs = {moved.get(b, b): n for b, n in self._refs.items()}
+        if moved:
+            self._free = list(range(count, self.num_blocks))
+        return list(moved.items())
 
     # ---------------------------------------------------------------- device mirror
 
@@ -115,7 +214,9 @@ class BlockAllocator:
                 value.extend(table[done:])
                 self._synced[seq_id] = len(table)
         if index:
-            packed = torch.tensor([index, value], dtype=torch.int64).pin_memory()
+            packed = torch.tensor([index, value], dtype=torch.int64)
+            if self._device.type == "cuda":
+                packed = packed.pin_memory()
             packed = packed.to(self._device, non_blocking=True)
             flat = self.device_tables.view(-1)
             flat.index_copy_(0, packed[0], packed[1].to(torch.int32))

@@ -1045,6 +1045,7 @@ int bs_take_status(void* workspace, void* stream, uint32_t* status_out) {
   if (bits & BS_STATUS_BAD_ROW) msg += " sequence row outside the block tables;";
   if (bits & BS_STATUS_BAD_POSITION) msg += " position outside the rotary tables;";
   if (bits & BS_STATUS_BAD_INDEX) msg += " gathered row index out of range;";
+  if (bits & BS_STATUS_BAD_COPY) msg += " block copied to is named by another pair;";
   g_error = msg;
   return BS_ERR_DEVICE;
 }
@@ -1087,4 +1088,11 @@ int32_t decode_record_stride(int64_t groups, int64_t head_dim) {
   return record_stride(groups, head_dim);
 }
 void add_kernel_launches(int n) { count_launches(n); }
+
+int sm_count(int* sms) {
+  DeviceInfo* d = nullptr;
+  if (int rc = current_device_info(&d)) return rc;
+  *sms = d->sms;
+  return BS_OK;
+}
 }  // namespace bsb

@@ -1,0 +1,357 @@
+// C ABI of the operators that keep a conversation's cache bounded: attention over
+// a sliding window with sink tokens, rotary embedding with the K/V append from
+// frequencies, and block copies (declared in include/batchstream_b200.h).
+//
+// Validation, messages and launch rules as in capi.cu: a malformed call is an
+// error code plus a message, launches go on the caller's stream, nothing here
+// allocates device memory.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+
+#include "../../include/batchstream_b200.h"
+#include "window.cuh"
+
+namespace bsb {
+// capi.cu: messages, launch count, SMs of the current device.
+void set_last_error(const char* message);
+void add_kernel_launches(int n);
+int sm_count(int* sms);
+int launch_rotary_append(const void* qkv, int64_t qkv_stride, bool bf16, const double* freq,
+                         int32_t rotary_dim, bool interleaved, double amp, const int32_t* pos,
+                         const int32_t* slots, int32_t ntok, int32_t H, int32_t Hkv, int32_t D,
+                         void* q_out, void* k_pool, void* v_pool, bool pool_bf16,
+                         int64_t pool_slots, uint32_t* status, cudaStream_t stream);
+int launch_copy_blocks(void* k_pool, void* v_pool, const int32_t* src, const int32_t* dst,
+                       int32_t n, int32_t num_blocks, int64_t rows, int64_t block_bytes, bool vec,
+                       int sms, uint32_t* status, cudaStream_t stream);
+}  // namespace bsb
+
+namespace {
+
+int fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  bsb::set_last_error(buf);
+  return code;
+}
+
+int cuda_fail(int e, const char* what) {
+  return fail(BS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(static_cast<cudaError_t>(e)));
+}
+
+#define BS_CHECK(cond, ...)                                \
+  do {                                                     \
+    if (!(cond)) return fail(BS_ERR_INVALID, __VA_ARGS__); \
+  } while (0)
+
+constexpr int64_t kInt32Max = 2147483647ll;
+constexpr int64_t kMaxHeadDim = 256;
+constexpr int64_t kMaxGroups = 16;
+// Context lengths, windows and sink counts: sums of two stay within int32.
+constexpr int64_t kMaxContext = 1ll << 30;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+int dtype_size(int32_t dtype) { return dtype == BS_BF16 ? 2 : 4; }
+
+// a * b, or -1 when it does not fit (both non-negative).
+int64_t product(int64_t a, int64_t b) {
+  int64_t out = 0;
+  return __builtin_mul_overflow(a, b, &out) ? -1 : out;
+}
+
+// The sizes of a window attention call.
+struct WindowShape {
+  int64_t rows, tokens, max_query_len;  // sequences; query tokens
+  bool chunks;                          // chunks of tokens (else one token per row)
+  int64_t heads, kv_heads, head_dim, block_size, max_blocks, window, sinks;
+  int32_t dtype;
+};
+
+int check_window_shape(const WindowShape& s) {
+  BS_CHECK(s.dtype == BS_BF16 || s.dtype == BS_F32, "dtype must be bfloat16 or float32");
+  BS_CHECK(s.rows >= 0 && s.rows <= kInt32Max && s.tokens >= 0 && s.tokens <= kInt32Max,
+           "row or token count out of range");
+  BS_CHECK(s.max_query_len >= 0 && s.max_query_len <= kInt32Max, "max_query_len out of range");
+  BS_CHECK(s.kv_heads > 0 && s.heads > 0 && s.heads % s.kv_heads == 0,
+           "heads must equal kv_heads * groups");
+  BS_CHECK(s.head_dim > 0 && s.block_size > 0 && s.max_blocks > 0, "sizes must be positive");
+  BS_CHECK(s.window >= 1, "window must be at least 1");
+  BS_CHECK(s.sinks >= 0, "sinks must be non-negative");
+  if (s.head_dim > kMaxHeadDim || s.heads / s.kv_heads > kMaxGroups || s.kv_heads > kInt32Max) {
+    return fail(BS_ERR_UNSUPPORTED, "head_dim <= %lld and groups <= %lld are supported",
+                static_cast<long long>(kMaxHeadDim), static_cast<long long>(kMaxGroups));
+  }
+  const int64_t context = product(s.max_blocks, s.block_size);
+  if (context < 0 || context > kMaxContext) {
+    return fail(BS_ERR_UNSUPPORTED, "a table row covers more than 2^30 tokens");
+  }
+  return BS_OK;
+}
+
+// Key ranges of the CUDA-core kernel: about four CTAs per SM in all, none of
+// fewer than 256 keys.
+constexpr int64_t kMaxSimtSplits = 64;
+constexpr int64_t kMinSimtKeys = 256;
+
+// How the CUDA-core kernel runs a call.
+struct SimtPlan {
+  int64_t tile_tokens, qtiles, items, splits, rec_stride, bytes;
+};
+
+int plan_simt(const WindowShape& s, SimtPlan* p) {
+  int sms = 0;
+  if (int rc = bsb::sm_count(&sms)) return rc;
+  const int64_t groups = s.heads / s.kv_heads;
+  p->tile_tokens = s.chunks ? std::max<int64_t>(1, bsb::kWindowSimtRows / groups) : 1;
+  p->qtiles = s.chunks ? (s.max_query_len + p->tile_tokens - 1) / p->tile_tokens : 1;
+  p->items = product(product(s.rows, p->qtiles), s.kv_heads);
+  if (p->items < 0 || p->items > kInt32Max) {
+    return fail(BS_ERR_UNSUPPORTED, "too many query tiles");
+  }
+  const int64_t keys = std::min(s.max_blocks * s.block_size,
+                                std::min(s.window, kMaxContext) + std::min(s.sinks, kMaxContext) +
+                                    p->tile_tokens);
+  const int64_t want = p->items > 0 ? (4ll * sms + p->items - 1) / p->items : 1;
+  p->splits = std::max<int64_t>(
+      1, std::min(std::min(want, kMaxSimtSplits), keys / kMinSimtKeys));
+  if (p->items * p->splits > kInt32Max) p->splits = 1;
+  const int64_t gm = p->tile_tokens * groups <= 8 ? 8 : bsb::kWindowSimtRows;
+  p->rec_stride = gm * s.head_dim + 2 * gm;
+  p->bytes = p->splits > 1 ? p->items * p->splits * p->rec_stride * 4 : 0;
+  return BS_OK;
+}
+
+int window_workspace(const WindowShape& s, uint64_t* bytes_out) {
+  BS_CHECK(bytes_out != nullptr, "bytes_out is null");
+  if (int rc = check_window_shape(s)) return rc;
+  SimtPlan p;
+  if (int rc = plan_simt(s, &p)) return rc;
+  *bytes_out = static_cast<uint64_t>(p.bytes);
+  return BS_OK;
+}
+
+// Everything of a call but its shape.
+struct WindowCall {
+  const void* query;
+  int64_t q_stride;
+  const int32_t* cu_q;
+  const int32_t* context_lens;
+  const int32_t* seq_rows;
+  const void* key_pool;
+  const void* value_pool;
+  const int32_t* block_tables;
+  int64_t table_stride, table_rows, num_blocks;
+  double scaling;
+  void* output;
+  int64_t o_stride;
+  void* workspace;
+  uint64_t workspace_bytes;
+  uint32_t* status;
+  void* stream;
+};
+
+int run_window(const WindowShape& s, const WindowCall& c) {
+  if (int rc = check_window_shape(s)) return rc;
+  BS_CHECK(s.max_blocks <= c.table_stride, "max_blocks_per_seq must be in [1, table_stride]");
+  BS_CHECK(c.table_rows > 0 && c.table_rows <= kInt32Max, "table_rows out of range");
+  BS_CHECK(c.num_blocks > 0, "sizes must be positive");
+  BS_CHECK(c.q_stride >= s.heads * s.head_dim && c.o_stride >= s.heads * s.head_dim,
+           "token strides must cover heads * head_dim");
+  const int64_t pool_rows = product(product(s.kv_heads, c.num_blocks), s.block_size);
+  if (pool_rows < 0 || pool_rows > kInt32Max) {
+    return fail(BS_ERR_UNSUPPORTED, "pool has more than 2^31 rows");
+  }
+  if (s.rows == 0 || s.tokens == 0) return BS_OK;
+  BS_CHECK(!s.chunks || s.max_query_len > 0, "max_query_len must be positive");
+  BS_CHECK(c.query && c.key_pool && c.value_pool && c.block_tables && c.context_lens &&
+               c.output && (!s.chunks || c.cu_q),
+           "null pointer argument");
+  bsb::WindowArgs a{};
+  a.q = c.query;
+  a.q_stride = c.q_stride;
+  a.out = c.output;
+  a.o_stride = c.o_stride;
+  a.k_pool = c.key_pool;
+  a.v_pool = c.value_pool;
+  a.block_tables = c.block_tables;
+  a.bt_stride = c.table_stride;
+  a.bt_rows = static_cast<int32_t>(c.table_rows);
+  a.max_blocks = static_cast<int32_t>(s.max_blocks);
+  a.seq_rows = c.seq_rows;
+  a.context_lens = c.context_lens;
+  a.cu_q = s.chunks ? c.cu_q : nullptr;
+  a.num_rows = static_cast<int32_t>(s.rows);
+  a.num_tokens = static_cast<int32_t>(s.tokens);
+  a.max_query_len = static_cast<int32_t>(s.max_query_len);
+  a.num_heads = static_cast<int32_t>(s.heads);
+  a.num_kv_heads = static_cast<int32_t>(s.kv_heads);
+  a.groups = static_cast<int32_t>(s.heads / s.kv_heads);
+  a.head_dim = static_cast<int32_t>(s.head_dim);
+  a.block_size = static_cast<int32_t>(s.block_size);
+  a.num_blocks = static_cast<int32_t>(c.num_blocks);
+  a.window = static_cast<int32_t>(std::min(s.window, kMaxContext));
+  a.sinks = static_cast<int32_t>(std::min(s.sinks, kMaxContext));
+  a.scale = static_cast<float>(c.scaling);
+  a.status = c.status;
+
+  SimtPlan p;
+  if (int rc = plan_simt(s, &p)) return rc;
+  if (p.bytes > 0 &&
+      (c.workspace == nullptr || c.workspace_bytes < static_cast<uint64_t>(p.bytes))) {
+    return fail(BS_ERR_WORKSPACE, "workspace of %llu bytes is smaller than the %lld needed",
+                static_cast<unsigned long long>(c.workspace_bytes),
+                static_cast<long long>(p.bytes));
+  }
+  BS_CHECK(aligned16(c.workspace), "workspace must be 16-byte aligned");
+  a.tile_tokens = static_cast<int32_t>(p.tile_tokens);
+  a.qtiles = static_cast<int32_t>(p.qtiles);
+  a.splits = static_cast<int32_t>(p.splits);
+  a.records = static_cast<float*>(c.workspace);
+  a.rec_stride = static_cast<int32_t>(p.rec_stride);
+  const bool vec = (s.head_dim * dtype_size(s.dtype)) % 16 == 0 && aligned16(c.key_pool);
+  const int rc = bsb::launch_window_simt(a, s.dtype == BS_BF16, vec,
+                                         static_cast<cudaStream_t>(c.stream));
+  if (rc != 0) return cuda_fail(rc, "window attention launch");
+  bsb::add_kernel_launches(p.splits > 1 ? 2 : 1);
+  return BS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int bs_window_attention_batched_workspace_bytes(int64_t num_seqs, int64_t num_heads,
+                                                int64_t num_kv_heads, int64_t head_dim,
+                                                int64_t block_size, int64_t max_blocks_per_seq,
+                                                int32_t dtype, int64_t window, int64_t sinks,
+                                                uint64_t* bytes_out) {
+  const WindowShape s{num_seqs, num_seqs,   1,          false,
+                      num_heads, num_kv_heads, head_dim, block_size,
+                      max_blocks_per_seq, window, sinks, dtype};
+  return window_workspace(s, bytes_out);
+}
+
+int bs_window_prefill_attention_workspace_bytes(int64_t num_tokens, int64_t num_rows,
+                                                int64_t max_query_len, int64_t num_heads,
+                                                int64_t num_kv_heads, int64_t head_dim,
+                                                int64_t block_size, int64_t max_blocks_per_seq,
+                                                int32_t dtype, int64_t window, int64_t sinks,
+                                                uint64_t* bytes_out) {
+  const WindowShape s{num_rows, num_tokens,   max_query_len, true,
+                      num_heads, num_kv_heads, head_dim, block_size,
+                      max_blocks_per_seq, window, sinks, dtype};
+  return window_workspace(s, bytes_out);
+}
+
+int bs_window_attention_batched(const void* query, int64_t query_seq_stride, const void* key_pool,
+                                const void* value_pool, const int32_t* block_tables,
+                                int64_t table_stride, int64_t table_rows, const int32_t* seq_rows,
+                                const int32_t* context_lens, int64_t num_seqs, int64_t num_heads,
+                                int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                                int64_t num_blocks, int64_t max_blocks_per_seq, int32_t dtype,
+                                double scaling, int64_t window, int64_t sinks, void* output,
+                                int64_t output_seq_stride, void* workspace,
+                                uint64_t workspace_bytes, uint32_t* status, void* stream) {
+  const WindowShape s{num_seqs, num_seqs,   1,          false,
+                      num_heads, num_kv_heads, head_dim, block_size,
+                      max_blocks_per_seq, window, sinks, dtype};
+  const WindowCall c{query,        query_seq_stride, nullptr,    context_lens, seq_rows,
+                     key_pool,     value_pool,       block_tables, table_stride, table_rows,
+                     num_blocks,   scaling,          output,     output_seq_stride, workspace,
+                     workspace_bytes, status,        stream};
+  return run_window(s, c);
+}
+
+int bs_window_prefill_attention(const void* query, int64_t query_token_stride, const int32_t* cu_q,
+                                int64_t num_rows, int64_t num_tokens, int64_t max_query_len,
+                                const int32_t* context_lens, const int32_t* seq_rows,
+                                const void* key_pool, const void* value_pool,
+                                const int32_t* block_tables, int64_t table_stride,
+                                int64_t table_rows, int64_t max_blocks_per_seq, int64_t num_heads,
+                                int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                                int64_t num_blocks, int32_t dtype, double scaling, int64_t window,
+                                int64_t sinks, void* output, int64_t output_token_stride,
+                                void* workspace, uint64_t workspace_bytes, uint32_t* status,
+                                void* stream) {
+  const WindowShape s{num_rows, num_tokens,   max_query_len, true,
+                      num_heads, num_kv_heads, head_dim, block_size,
+                      max_blocks_per_seq, window, sinks, dtype};
+  const WindowCall c{query,        query_token_stride, cu_q,      context_lens, seq_rows,
+                     key_pool,     value_pool,       block_tables, table_stride, table_rows,
+                     num_blocks,   scaling,          output,     output_token_stride, workspace,
+                     workspace_bytes, status,        stream};
+  return run_window(s, c);
+}
+
+int bs_rotary_append(const void* qkv, int64_t qkv_row_stride, int32_t dtype,
+                     const double* frequencies, int64_t rotary_dim, int32_t interleaved,
+                     double amplitude, const int32_t* positions, const int32_t* slot_mapping,
+                     int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                     void* query_out, void* key_pool, void* value_pool, int32_t pool_dtype,
+                     int64_t num_blocks, int64_t block_size, uint32_t* status, void* stream) {
+  BS_CHECK(dtype == BS_BF16 || dtype == BS_F32, "dtype must be bfloat16 or float32");
+  BS_CHECK(pool_dtype == BS_BF16 || pool_dtype == BS_F32, "pool dtype must be bf16 or fp32");
+  BS_CHECK(num_tokens >= 0 && num_tokens <= kInt32Max, "num_tokens out of range");
+  BS_CHECK(num_heads > 0 && num_kv_heads > 0 && head_dim > 0, "sizes must be positive");
+  BS_CHECK(rotary_dim >= 2 && rotary_dim % 2 == 0 && rotary_dim <= head_dim,
+           "rotary_dim must be even and in [2, head_dim]");
+  BS_CHECK(std::isfinite(amplitude), "amplitude must be finite");
+  BS_CHECK(num_blocks > 0 && block_size > 0, "sizes must be positive");
+  if (head_dim > 1024 || num_heads > 65536 || num_kv_heads > 65536) {
+    return fail(BS_ERR_UNSUPPORTED, "head_dim <= 1024 and at most 65536 heads are supported");
+  }
+  BS_CHECK(qkv_row_stride >= (num_heads + 2 * num_kv_heads) * head_dim,
+           "qkv rows must hold q, k and v");
+  const int64_t slots = product(num_blocks, block_size);
+  if (slots < 0 || slots > kInt32Max) return fail(BS_ERR_UNSUPPORTED, "pool too large");
+  if (num_tokens == 0) return BS_OK;
+  BS_CHECK(qkv && frequencies && positions && slot_mapping && query_out && key_pool && value_pool,
+           "null pointer argument");
+  const int rc = bsb::launch_rotary_append(
+      qkv, qkv_row_stride, dtype == BS_BF16, frequencies, static_cast<int32_t>(rotary_dim),
+      interleaved != 0, amplitude, positions, slot_mapping, static_cast<int32_t>(num_tokens),
+      static_cast<int32_t>(num_heads), static_cast<int32_t>(num_kv_heads),
+      static_cast<int32_t>(head_dim), query_out, key_pool, value_pool, pool_dtype == BS_BF16,
+      slots, status, static_cast<cudaStream_t>(stream));
+  if (rc != 0) return cuda_fail(rc, "rotary_append launch");
+  bsb::add_kernel_launches(1);
+  return BS_OK;
+}
+
+int bs_copy_blocks(void* key_pool, void* value_pool, int32_t pool_dtype, int64_t num_layers,
+                   int64_t num_kv_heads, int64_t num_blocks, int64_t block_size, int64_t head_dim,
+                   const int32_t* src, const int32_t* dst, int64_t num_pairs, uint32_t* status,
+                   void* stream) {
+  BS_CHECK(pool_dtype == BS_BF16 || pool_dtype == BS_F32, "pool dtype must be bf16 or fp32");
+  BS_CHECK(num_layers > 0 && num_kv_heads > 0 && num_blocks > 0 && block_size > 0 && head_dim > 0,
+           "sizes must be positive");
+  BS_CHECK(num_blocks <= kInt32Max, "num_blocks out of range");
+  BS_CHECK(num_pairs >= 0 && num_pairs <= kInt32Max, "num_pairs out of range");
+  const int64_t rows = product(num_layers, num_kv_heads);
+  const int64_t block_bytes = product(product(block_size, head_dim), dtype_size(pool_dtype));
+  if (rows < 0 || block_bytes < 0 || product(product(rows, num_blocks), block_bytes) < 0) {
+    return fail(BS_ERR_UNSUPPORTED, "pool too large");
+  }
+  if (num_pairs == 0) return BS_OK;
+  BS_CHECK(key_pool && value_pool && src && dst, "null pointer argument");
+  int sms = 0;
+  if (int rc = bsb::sm_count(&sms)) return rc;
+  const bool vec = block_bytes % 16 == 0 && aligned16(key_pool) && aligned16(value_pool);
+  const int rc = bsb::launch_copy_blocks(key_pool, value_pool, src, dst,
+                                         static_cast<int32_t>(num_pairs),
+                                         static_cast<int32_t>(num_blocks), rows, block_bytes, vec,
+                                         sms, status, static_cast<cudaStream_t>(stream));
+  if (rc != 0) return cuda_fail(rc, "copy_blocks launch");
+  bsb::add_kernel_launches(1);
+  return BS_OK;
+}
+
+}  // extern "C"

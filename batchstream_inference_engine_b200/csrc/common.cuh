@@ -27,6 +27,7 @@ enum : uint32_t {
   kStatusBadRow = 1u << 4,       // sequence row outside the block-table tensor
   kStatusBadPosition = 1u << 5,  // position outside the rotary tables
   kStatusBadIndex = 1u << 6,     // gathered row index outside its tensor
+  kStatusBadCopy = 1u << 7,      // block copy whose destination another pair names
 };
 
 constexpr uint32_t kSpinLimit = 1u << 26;

@@ -1,0 +1,364 @@
+// Sliding-window paged attention on the CUDA cores: fp32 pools and every shape
+// the tensor-core kernels do not take (any block size, head_dim <= 256, up to 16
+// query heads per kv head), for single tokens and for prompt chunks.
+//
+// One CTA per (query tile, kv head, key range); the tile is one token, or as many
+// tokens of a chunk as fill 16 rows with their query heads, so each key row is
+// read once for all of them.  Each warp takes every fourth group of 32 keys: lane
+// j looks up key j of the group, the warp copies the group's K rows to shared
+// memory (16-byte loads), lane j computes key j's scores against the query rows
+// (fp32 in shared memory, read as broadcasts), the running softmax of a row comes
+// from warp reductions, and the weighted V rows are read straight from the pool
+// with lanes along head_dim (coalesced).  No barrier until the four warps' states
+// are combined at the end.
+//
+// A weight of zero skips its V row, so NaN or infinities in a key that a row does
+// not see never reach that row.
+#include "window.cuh"
+
+namespace bsb {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr float kLog2eW = 1.4426950408889634f;
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v);
+template <>
+__device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
+template <typename T>
+__device__ __forceinline__ T of_float(float v);
+template <>
+__device__ __forceinline__ float of_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 of_float<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// 16 bytes of a row as floats.
+__device__ __forceinline__ void widen16(const float* p, float* out) {
+  *reinterpret_cast<float4*>(out) = *reinterpret_cast<const float4*>(p);
+}
+__device__ __forceinline__ void widen16(const __nv_bfloat16* p, float* out) {
+  float v[8];
+  load8(p, v);
+  reinterpret_cast<float4*>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+// Floats of one K row in shared memory: lanes read the rows in parallel, so the
+// pad moves consecutive rows to different banks (four floats keep 16-byte reads
+// aligned).
+__host__ __device__ constexpr int row_floats(int head_dim, bool vec) {
+  return head_dim + (vec ? 4 : 1);
+}
+
+__host__ __device__ inline size_t simt_smem(int head_dim, int gm, bool vec) {
+  return sizeof(float) * (static_cast<size_t>(gm) * head_dim +
+                          kWarps * 32 * row_floats(head_dim, vec) + kWarps * 32 * gm +
+                          2 * kWarps * gm);
+}
+
+// Linear CTA index -> (sequence, query tile, kv head).
+__device__ __forceinline__ void window_item(const WindowArgs& a, int64_t item, int32_t& r,
+                                            int32_t& tile, int32_t& h) {
+  h = static_cast<int32_t>(item % a.num_kv_heads);
+  item /= a.num_kv_heads;
+  tile = static_cast<int32_t>(item % a.qtiles);
+  r = static_cast<int32_t>(item / a.qtiles);
+}
+
+// GM: query rows held per CTA; DPL: head dims per lane; VEC: 16-byte K rows.
+template <typename T, int GM, int DPL, bool VEC>
+__global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs a) {
+  extern __shared__ __align__(16) float wsm[];
+  pdl_wait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int32_t split = blockIdx.x % a.splits;
+  const int64_t item = blockIdx.x / a.splits;
+  int32_t r, tile, h;
+  window_item(a, item, r, tile, h);
+  WindowTile w;
+  if (!window_tile(a, r, tile, w, tid == 0 && tile == 0 && h == 0 && split == 0)) return;
+  const int32_t per = window_range(w.count, a.splits);
+  if (static_cast<int64_t>(split) * per >= w.count) return;
+  const int32_t begin = split * per;
+  const int32_t end = w.count - begin < per ? w.count : begin + per;
+
+  const int G = a.groups, D = a.head_dim, bs = a.block_size;
+  const int rows = w.ntok * G;  // <= GM (host)
+  const int rf = row_floats(D, VEC);
+  float* sQ = wsm;
+  float* sK = sQ + GM * D + warp * 32 * rf;
+  float* sP = wsm + GM * D + kWarps * 32 * rf + warp * 32 * GM;
+  float* sM = wsm + GM * D + kWarps * 32 * rf + kWarps * 32 * GM;
+  float* sL = sM + kWarps * GM;
+
+  // Query rows: row t * G + g is head g of the kv head's group, token t.
+  const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(w.tok0) * a.q_stride +
+               static_cast<int64_t>(h) * G * D;
+  for (int e = tid; e < rows * D; e += kThreads) {
+    const int t = e / (G * D);
+    sQ[e] = to_float<T>(q[static_cast<int64_t>(t) * a.q_stride + (e - t * G * D)]);
+  }
+  __syncthreads();
+
+  const int64_t head_off = static_cast<int64_t>(h) * a.num_blocks * bs * D;
+  const T* kh = static_cast<const T*>(a.k_pool) + head_off;
+  const T* vh = static_cast<const T*>(a.v_pool) + head_off;
+  const int32_t* table = a.block_tables + static_cast<int64_t>(w.row) * a.bt_stride;
+  const float zscale = a.scale * kLog2eW;
+
+  float m[GM], l[GM], o[GM][DPL];
+#pragma unroll
+  for (int i = 0; i < GM; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < DPL; ++k) o[i][k] = 0.f;
+  }
+
+  for (int32_t base = begin + warp * 32; base < end; base += kThreads) {
+    // Lane j's key of the group: its position and its row's offset (-1: none).
+    const int32_t v = base + lane;
+    int32_t pos = 0;
+    int64_t off = -1;
+    if (v < end) {
+      pos = window_key(w, v);
+      const int32_t blk = __ldg(table + pos / bs);
+      if (blk >= 0 && blk < a.num_blocks) {
+        off = (static_cast<int64_t>(blk) * bs + pos % bs) * D;
+      } else {
+        set_status(a.status, kStatusBadBlock);
+      }
+    }
+    if constexpr (VEC) {
+      constexpr int kElems = 16 / sizeof(T);
+      const int per_row = D / kElems;
+      for (int it = 0; it < per_row; ++it) {
+        const int idx = it * 32 + lane;
+        const int key = idx / per_row, c = (idx - key * per_row) * kElems;
+        const int64_t ko = __shfl_sync(0xffffffffu, off, key);
+        float* dst = sK + key * rf + c;
+        if (ko >= 0) {
+          widen16(kh + ko + c, dst);
+        } else {
+#pragma unroll
+          for (int x = 0; x < kElems; ++x) dst[x] = 0.f;
+        }
+      }
+    } else {
+      for (int key = 0; key < 32; ++key) {
+        const int64_t ko = __shfl_sync(0xffffffffu, off, key);
+        for (int d = lane; d < D; d += 32) sK[key * rf + d] = ko >= 0 ? to_float<T>(kh[ko + d]) : 0.f;
+      }
+    }
+    __syncwarp();
+    float s[GM];
+#pragma unroll
+    for (int i = 0; i < GM; ++i) s[i] = 0.f;
+    const float* krow = sK + lane * rf;
+    if constexpr (VEC) {
+      for (int d = 0; d < D; d += 4) {
+        const float4 k4 = *reinterpret_cast<const float4*>(krow + d);
+#pragma unroll
+        for (int i = 0; i < GM; ++i) {
+          if (i < rows) {
+            const float4 q4 = *reinterpret_cast<const float4*>(sQ + i * D + d);
+            s[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[i]))));
+          }
+        }
+      }
+    } else {
+      for (int d = 0; d < D; ++d) {
+        const float kv = krow[d];
+#pragma unroll
+        for (int i = 0; i < GM; ++i) {
+          if (i < rows) s[i] = fmaf(sQ[i * D + d], kv, s[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < GM; ++i) {
+      if (i >= rows) continue;
+      const int32_t qpos = w.pos0 + i / G;
+      const bool seen = off >= 0 && pos <= qpos && (pos < a.sinks || pos > qpos - a.window);
+      const float z = seen ? s[i] * zscale : -INFINITY;
+      float mx = z;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      const float mnew = fmaxf(m[i], mx);
+      const float mb = mnew == -INFINITY ? 0.f : mnew;  // no key of this row yet
+      const float corr = fast_exp2(m[i] - mb);
+      const float p = seen ? fast_exp2(z - mb) : 0.f;
+      m[i] = mnew;
+      l[i] = l[i] * corr + p;  // this lane's part of the sum
+#pragma unroll
+      for (int k = 0; k < DPL; ++k) o[i][k] *= corr;
+      sP[lane * GM + i] = p;
+    }
+    __syncwarp();
+    const int nkeys = min(32, end - base);
+#pragma unroll 4
+    for (int j = 0; j < nkeys; ++j) {
+      const int64_t vo = __shfl_sync(0xffffffffu, off, j);
+      if (vo < 0) continue;
+      float vv[DPL];
+#pragma unroll
+      for (int k = 0; k < DPL; ++k) {
+        const int d = lane + 32 * k;
+        vv[k] = d < D ? to_float<T>(vh[vo + d]) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < GM; ++i) {
+        if (i >= rows) continue;
+        const float p = sP[j * GM + i];
+        if (p != 0.f) {
+#pragma unroll
+          for (int k = 0; k < DPL; ++k) o[i][k] = fmaf(p, vv[k], o[i][k]);
+        }
+      }
+    }
+    __syncwarp();  // the next group overwrites sK and sP
+  }
+
+  // Each warp's state over its own K rows (32 * rf >= rows * D floats).
+#pragma unroll
+  for (int i = 0; i < GM; ++i) {
+    if (i >= rows) continue;
+    float lr = l[i];
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) lr += __shfl_xor_sync(0xffffffffu, lr, x);
+    if (lane == 0) {
+      sM[warp * GM + i] = m[i];
+      sL[warp * GM + i] = lr;
+    }
+#pragma unroll
+    for (int k = 0; k < DPL; ++k) {
+      const int d = lane + 32 * k;
+      if (d < D) sK[i * D + d] = o[i][k];
+    }
+  }
+  __syncthreads();
+  const float* states = wsm + GM * D;
+  T* out = static_cast<T*>(a.out) + static_cast<int64_t>(w.tok0) * a.o_stride +
+           static_cast<int64_t>(h) * G * D;
+  float* rec = a.splits > 1 ? a.records + static_cast<int64_t>(blockIdx.x) * a.rec_stride : nullptr;
+  for (int e = tid; e < rows * D; e += kThreads) {
+    const int i = e / D;
+    float M = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kWarps; ++x) M = fmaxf(M, sM[x * GM + i]);
+    const float mb = M == -INFINITY ? 0.f : M;
+    float L = 0.f, O = 0.f;
+#pragma unroll
+    for (int x = 0; x < kWarps; ++x) {
+      const float f = fast_exp2(sM[x * GM + i] - mb);
+      L += sL[x * GM + i] * f;
+      O += states[x * 32 * rf + e] * f;
+    }
+    if (rec != nullptr) {
+      rec[e] = O;
+      if (e - i * D == 0) {
+        rec[GM * D + i] = M;
+        rec[GM * D + GM + i] = L;
+      }
+    } else {
+      const int t = e / (G * D);
+      out[static_cast<int64_t>(t) * a.o_stride + (e - t * G * D)] = of_float<T>(O / L);
+    }
+  }
+}
+
+// Joins the records of a tile's key ranges, in range order.
+template <typename T, int GM>
+__global__ void __launch_bounds__(kThreads) window_simt_merge_kernel(const WindowArgs a) {
+  pdl_wait();
+  int32_t r, tile, h;
+  window_item(a, blockIdx.x, r, tile, h);
+  WindowTile w;
+  if (!window_tile(a, r, tile, w, false)) return;
+  const int G = a.groups, D = a.head_dim;
+  const int32_t per = window_range(w.count, a.splits);
+  const int n = (w.count + per - 1) / per;
+  const float* rec = a.records + static_cast<int64_t>(blockIdx.x) * a.splits * a.rec_stride;
+  T* out = static_cast<T*>(a.out) + static_cast<int64_t>(w.tok0) * a.o_stride +
+           static_cast<int64_t>(h) * G * D;
+  for (int e = threadIdx.x; e < w.ntok * G * D; e += kThreads) {
+    const int i = e / D;
+    float M = -INFINITY;
+    for (int s = 0; s < n; ++s) {
+      M = fmaxf(M, rec[static_cast<int64_t>(s) * a.rec_stride + GM * D + i]);
+    }
+    const float mb = M == -INFINITY ? 0.f : M;
+    float L = 0.f, O = 0.f;
+    for (int s = 0; s < n; ++s) {
+      const float* p = rec + static_cast<int64_t>(s) * a.rec_stride;
+      const float f = fast_exp2(p[GM * D + i] - mb);
+      L += p[GM * D + GM + i] * f;
+      O += p[e] * f;
+    }
+    const int t = e / (G * D);
+    out[static_cast<int64_t>(t) * a.o_stride + (e - t * G * D)] = of_float<T>(O / L);
+  }
+}
+
+template <typename T, int GM, int DPL, bool VEC>
+int launch_one(const WindowArgs& a, cudaStream_t stream) {
+  const size_t smem = simt_smem(a.head_dim, GM, VEC);
+  auto kernel = window_simt_kernel<T, GM, DPL, VEC>;
+  if (smem > 48 * 1024) {
+    static unsigned long long configured = 0;  // one bit per device
+    const cudaError_t e = once_per_device(&configured, [&] {
+      return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  static_cast<int>(simt_smem(DPL * 32, GM, VEC)));
+    });
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  const int64_t items = static_cast<int64_t>(a.num_rows) * a.qtiles * a.num_kv_heads;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(items * a.splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const int rc = static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, a));
+  if (rc != 0 || a.splits == 1) return rc;
+  cfg.gridDim = dim3(static_cast<unsigned>(items));
+  cfg.dynamicSmemBytes = 0;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, window_simt_merge_kernel<T, GM>, a));
+}
+
+template <typename T, int GM, bool VEC>
+int launch_dims(const WindowArgs& a, cudaStream_t stream) {
+  if (a.head_dim <= 32) return launch_one<T, GM, 1, VEC>(a, stream);
+  if (a.head_dim <= 64) return launch_one<T, GM, 2, VEC>(a, stream);
+  if (a.head_dim <= 128) return launch_one<T, GM, 4, VEC>(a, stream);
+  return launch_one<T, GM, 8, VEC>(a, stream);
+}
+
+template <typename T>
+int launch_rows(const WindowArgs& a, bool vec, cudaStream_t stream) {
+  if (a.tile_tokens * a.groups <= 8) {
+    return vec ? launch_dims<T, 8, true>(a, stream) : launch_dims<T, 8, false>(a, stream);
+  }
+  return vec ? launch_dims<T, kWindowSimtRows, true>(a, stream)
+             : launch_dims<T, kWindowSimtRows, false>(a, stream);
+}
+
+}  // namespace
+
+int launch_window_simt(const WindowArgs& a, bool bf16, bool vec, cudaStream_t stream) {
+  return bf16 ? launch_rows<__nv_bfloat16>(a, vec, stream) : launch_rows<float>(a, vec, stream);
+}
+
+}  // namespace bsb

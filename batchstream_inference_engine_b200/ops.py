@@ -9,6 +9,7 @@ surface as ``RuntimeError``, as the reference op raises them through
 from __future__ import annotations
 
 import ctypes
+import math
 import threading
 
 import torch
@@ -568,6 +569,11 @@ __all__ = [
     "rope_append",
     "silu_mul",
     "argmax_rows",
+    "window_attention_batched",
+    "window_prefill_attention",
+    "rope_frequencies",
+    "rotary_append",
+    "copy_blocks",
     "take_status",
     "kernel_launches",
     "decode_workspace_bytes",
@@ -645,3 +651,277 @@ def prefill_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: t
             float(scaling), BS_PREFILL_PER_TOKEN if per_token else 0, out.data_ptr(),
             out.stride(0), ws.data_ptr(), ws.numel(), stream))
     return out
+
+
+# ------------------------------------------------------------------ bounded caches
+
+
+def _int32_list(name: str, t: torch.Tensor, count: int) -> torch.Tensor:
+    """`t` as int32 entries one after the other, at least `count` of them."""
+    if t.dtype != torch.int32:
+        raise RuntimeError(f"{name} must be int32")
+    if t.dim() != 1 or t.numel() < count:
+        raise RuntimeError(f"{name} must be one-dimensional with at least {count} entries")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _window_inputs(name: str, query, key_pool, value_pool, block_tables, out, max_blocks_per_seq):
+    """The checks that both window attentions share; returns query, block_tables,
+    out and max_blocks as the C call takes them."""
+    if query.dim() != 3 or key_pool.dim() != 4 or value_pool.shape != key_pool.shape:
+        raise RuntimeError(f"{name}: query must be [T, H, D] and the pools [Hkv, NB, bs, D]")
+    if query.dtype != key_pool.dtype or value_pool.dtype != key_pool.dtype:
+        raise RuntimeError(f"{name}: query and pools must share a dtype")
+    if not (key_pool.is_contiguous() and value_pool.is_contiguous()):
+        raise RuntimeError(f"{name}: pools must be contiguous")
+    if query.size(2) != key_pool.size(3):
+        raise RuntimeError(f"{name}: query and pools disagree on head_dim")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2:
+        raise RuntimeError(f"{name}: block_tables must be int32 [rows, max_blocks]")
+    T, H, D = query.shape
+    if query.stride(2) != 1 or query.stride(1) != D or query.stride(0) < H * D:
+        query = query.contiguous()
+    if block_tables.stride(1) != 1 or block_tables.stride(0) < block_tables.size(1):
+        block_tables = block_tables.contiguous()
+    if out is None:
+        out = torch.empty((T, H, D), dtype=query.dtype, device=query.device)
+    elif (out.shape != (T, H, D) or out.dtype != query.dtype or out.stride(2) != 1
+          or out.stride(1) != D or (T > 1 and out.stride(0) < H * D)):
+        raise RuntimeError(f"{name}: out must be {[T, H, D]} with contiguous heads in the query's "
+                           "dtype")
+    mb = block_tables.size(1) if max_blocks_per_seq is None else int(max_blocks_per_seq)
+    return query, block_tables, out, mb
+
+
+def _token_stride(t: torch.Tensor) -> int:
+    """Elements between tokens of [T, H, D] (any stride of a single token will do)."""
+    return max(t.stride(0), t.size(1) * t.size(2))
+
+
+def _scratch(nbytes: int, device: torch.device) -> torch.Tensor | None:
+    """Scratch of one call, from the stream-ordered allocator (inside a capture:
+    from the graph's own pool, so two graphs never share it)."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def window_attention_batched(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
+                             block_tables: torch.Tensor, context_lens: torch.Tensor,
+                             scaling: float, window: int, sinks: int = 0,
+                             seq_rows: torch.Tensor | None = None,
+                             out: torch.Tensor | None = None,
+                             max_blocks_per_seq: int | None = None) -> torch.Tensor:
+    """Decode attention of a ragged batch over a sliding window and sink tokens.
+
+    As ``paged_attention_batched``, except that sequence b's query (position
+    p = context_lens[b] - 1) sees key j only if j < sinks or j > p - window.
+    Blocks outside are never read and may have been freed
+    (``BlockAllocator.trim``).  A length of 0 marks a padding row, whose output
+    row is left as it was.  Scores stay in fp32.
+    """
+    device = _require_cuda("window_attention_batched", query, key_pool, value_pool, block_tables,
+                           context_lens, seq_rows, out)
+    query, block_tables, out, mb = _window_inputs("window_attention_batched", query, key_pool,
+                                                  value_pool, block_tables, out,
+                                                  max_blocks_per_seq)
+    B, H, D = query.shape
+    Hkv, NB, bs, _ = key_pool.shape
+    context_lens = _int32_list("context_lens", context_lens, B)
+    if seq_rows is not None:
+        seq_rows = _int32_list("seq_rows", seq_rows, B)
+    code = dtype_code(query.dtype)
+    with torch.cuda.device(device):
+        stream = torch.cuda.current_stream(device).cuda_stream
+        need = ctypes.c_uint64(0)
+        check(lib().bs_window_attention_batched_workspace_bytes(
+            B, H, Hkv, D, bs, mb, code, int(window), int(sinks), ctypes.byref(need)))
+        scratch = _scratch(need.value, device)
+        check(lib().bs_window_attention_batched(
+            query.data_ptr(), _token_stride(query), key_pool.data_ptr(), value_pool.data_ptr(),
+            block_tables.data_ptr(), block_tables.stride(0), block_tables.size(0),
+            seq_rows.data_ptr() if seq_rows is not None else None, context_lens.data_ptr(), B, H,
+            Hkv, D, bs, NB, mb, code, float(scaling), int(window), int(sinks), out.data_ptr(),
+            _token_stride(out), scratch.data_ptr() if scratch is not None else None, need.value,
+            workspace_for(device, 0).data_ptr(), stream))
+    return out
+
+
+def window_prefill_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
+                             block_tables: torch.Tensor, cu_q: torch.Tensor,
+                             context_lens: torch.Tensor, scaling: float, max_query_len: int,
+                             window: int, sinks: int = 0, seq_rows: torch.Tensor | None = None,
+                             out: torch.Tensor | None = None,
+                             max_blocks_per_seq: int | None = None) -> torch.Tensor:
+    """Attention of prompt chunks over a sliding window and sink tokens.
+
+    As ``prefill_attention``, except that the query token at position p sees key
+    j <= p only if j < sinks or j > p - window.  Blocks that no token of a chunk
+    sees are never read.  A context length of 0 marks a padding chunk; rows of
+    ``out`` past the last chunk are left as they were.  A chunk longer than
+    ``max_query_len`` or than its context, or outside the T rows, is reported
+    (``take_status``) and skipped.
+    """
+    device = _require_cuda("window_prefill_attention", query, key_pool, value_pool, block_tables,
+                           cu_q, context_lens, seq_rows, out)
+    query, block_tables, out, mb = _window_inputs("window_prefill_attention", query, key_pool,
+                                                  value_pool, block_tables, out,
+                                                  max_blocks_per_seq)
+    T, H, D = query.shape
+    Hkv, NB, bs, _ = key_pool.shape
+    context_lens = _int32_list("context_lens", context_lens, 0)
+    R = context_lens.numel()
+    cu_q = _int32_list("cu_q", cu_q, R + 1)
+    if seq_rows is not None:
+        seq_rows = _int32_list("seq_rows", seq_rows, R)
+    code = dtype_code(query.dtype)
+    with torch.cuda.device(device):
+        stream = torch.cuda.current_stream(device).cuda_stream
+        need = ctypes.c_uint64(0)
+        check(lib().bs_window_prefill_attention_workspace_bytes(
+            T, R, int(max_query_len), H, Hkv, D, bs, mb, code, int(window), int(sinks),
+            ctypes.byref(need)))
+        scratch = _scratch(need.value, device)
+        check(lib().bs_window_prefill_attention(
+            query.data_ptr(), _token_stride(query), cu_q.data_ptr(), R, T, int(max_query_len),
+            context_lens.data_ptr(), seq_rows.data_ptr() if seq_rows is not None else None,
+            key_pool.data_ptr(), value_pool.data_ptr(), block_tables.data_ptr(),
+            block_tables.stride(0), block_tables.size(0), mb, H, Hkv, D, bs, NB, code,
+            float(scaling), int(window), int(sinks), out.data_ptr(), _token_stride(out),
+            scratch.data_ptr() if scratch is not None else None, need.value,
+            workspace_for(device, 0).data_ptr(), stream))
+    return out
+
+
+def rope_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None,
+                     device: torch.device | str = "cuda") -> tuple[torch.Tensor, float]:
+    """Rotary frequencies for ``rotary_append``: fp64 [rotary_dim / 2] on `device`,
+    and the amplitude.
+
+    f_i = theta^(-2 i / rotary_dim), changed for contexts `factor` times longer by
+    ``scaling["type"]``:
+
+    * "linear": f_i / factor (positions interpolated);
+    * "ntk": theta grows by factor^(d / (d - 2)), so the slowest pair turns factor
+      times slower and the fastest as before;
+    * "yarn": f_i where pair i turns more than ``beta_fast`` (32) times within
+      ``original_max_position``, f_i / factor below ``beta_slow`` (1) turns, and a
+      linear ramp over the pairs between; amplitude 0.1 ln(factor) + 1, or
+      ``attention_factor``;
+    * "banded": by wavelength: f_i below original_max_position /
+      ``high_freq_factor``, f_i / factor above original_max_position /
+      ``low_freq_factor``, blended between.
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise RuntimeError("rotary_dim must be even and at least 2")
+    if not theta > 0:
+        raise RuntimeError("theta must be positive")
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    amplitude = 1.0
+    base = math.log(theta)
+    kind = "none" if scaling is None else scaling.get("type")
+    if kind != "none":
+        factor = float(scaling["factor"])
+        if not (factor >= 1.0 and math.isfinite(factor)):
+            raise RuntimeError("the scaling factor must be finite and at least 1")
+    if kind == "ntk" and rotary_dim > 2:
+        base += math.log(factor) * rotary_dim / (rotary_dim - 2)
+    freq = torch.exp(-2.0 * i / rotary_dim * base)
+    if kind == "linear":
+        freq = freq / factor
+    elif kind == "yarn":
+        length = float(scaling["original_max_position"])
+
+        def pair_of(turns):  # the (fractional) pair that turns this often in `length`
+            return rotary_dim * math.log(length / (2 * math.pi * turns)) / (2 * base)
+
+        low = max(math.floor(pair_of(float(scaling.get("beta_fast", 32.0)))), 0)
+        high = min(math.ceil(pair_of(float(scaling.get("beta_slow", 1.0)))), rotary_dim - 1)
+        slow = ((i - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        freq = freq * (1.0 - slow) + freq / factor * slow
+        amplitude = scaling.get("attention_factor")
+        amplitude = 0.1 * math.log(factor) + 1.0 if amplitude is None else float(amplitude)
+    elif kind == "banded":
+        length = float(scaling["original_max_position"])
+        few, many = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        if not many > few:
+            raise RuntimeError("high_freq_factor must be above low_freq_factor")
+        keep = ((length * freq / (2 * math.pi) - few) / (many - few)).clamp(0.0, 1.0)
+        freq = freq * keep + freq / factor * (1.0 - keep)
+    elif kind not in ("none", "ntk"):
+        raise RuntimeError(f"unknown rotary scaling type {kind!r}")
+    return freq.to(device), amplitude
+
+
+def rotary_append(qkv: torch.Tensor, frequencies: torch.Tensor, positions: torch.Tensor,
+                  slot_mapping: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
+                  num_heads: int, interleaved: bool = False, amplitude: float = 1.0,
+                  query_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary embedding and K/V append from frequencies, in one launch.
+
+    As ``rope_append``, without tables: pair i of the first
+    2 * len(frequencies) dims of every q and k head turns by
+    position * frequencies[i] (fp64, ``rope_frequencies``) and is multiplied by
+    ``amplitude``; the other dims are copied.  Pairs are dims (i, i + half) or,
+    ``interleaved``, (2i, 2i + 1).  Computed in fp32 and rounded once.  A
+    negative slot skips the row's K/V write; two rows must not share a slot.
+    Returns q as [T, H, D].
+    """
+    device = _require_cuda("rotary_append", qkv, frequencies, positions, slot_mapping, key_pool,
+                           value_pool, query_out)
+    if key_pool.dim() != 4 or value_pool.shape != key_pool.shape \
+            or value_pool.dtype != key_pool.dtype:
+        raise RuntimeError("the pools must be [Hkv, NB, bs, D] of one shape and dtype")
+    if not (key_pool.is_contiguous() and value_pool.is_contiguous()):
+        raise RuntimeError("pools must be contiguous")
+    Hkv, NB, bs, D = key_pool.shape
+    T = positions.numel()
+    positions = _int32_list("positions", positions, T)
+    slot_mapping = _int32_list("slot_mapping", slot_mapping, T)
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1:
+        raise RuntimeError("frequencies must be one-dimensional float64")
+    if qkv.dim() < 2 or qkv.size(0) < T:
+        raise RuntimeError("qkv needs a row per position")
+    width = (num_heads + 2 * Hkv) * D
+    q2 = _rows_2d("qkv", qkv, width)
+    if q2.stride(0) < width:
+        q2 = q2.contiguous()
+    q_out = query_out if query_out is not None else torch.empty(
+        (T, num_heads, D), dtype=qkv.dtype, device=device)
+    if not q_out.is_contiguous() or q_out.dtype != qkv.dtype or q_out.numel() < T * num_heads * D:
+        raise RuntimeError("query_out must be contiguous [T, heads, head_dim] in the qkv dtype")
+    with torch.cuda.device(device):
+        stream = torch.cuda.current_stream(device).cuda_stream
+        check(lib().bs_rotary_append(
+            q2.data_ptr(), q2.stride(0), dtype_code(qkv.dtype),
+            frequencies.contiguous().data_ptr(), 2 * frequencies.numel(), 1 if interleaved else 0,
+            float(amplitude), positions.data_ptr(), slot_mapping.data_ptr(), T, num_heads, Hkv, D,
+            q_out.data_ptr(), key_pool.data_ptr(), value_pool.data_ptr(),
+            dtype_code(key_pool.dtype), NB, bs, workspace_for(device, 0).data_ptr(), stream))
+    return q_out
+
+
+def copy_blocks(key_pool: torch.Tensor, value_pool: torch.Tensor, src: torch.Tensor,
+                dst: torch.Tensor) -> None:
+    """Copies block src[i] to block dst[i], K and V, in every layer and kv head.
+
+    Pools [L, Hkv, NB, bs, D] (or one layer's [Hkv, NB, bs, D]); src and dst int32
+    on the device.  All pairs happen at once: a pair whose destination another
+    pair names too, as source or destination, is reported (``take_status``) and
+    skipped, and so is one outside the pool.  Negative ends are padding.
+    """
+    device = _require_cuda("copy_blocks", key_pool, value_pool, src, dst)
+    if key_pool.dim() not in (4, 5) or value_pool.shape != key_pool.shape \
+            or value_pool.dtype != key_pool.dtype:
+        raise RuntimeError("the pools must be [L, Hkv, NB, bs, D] of one shape and dtype")
+    if not (key_pool.is_contiguous() and value_pool.is_contiguous()):
+        raise RuntimeError("pools must be contiguous")
+    if src.numel() != dst.numel():
+        raise RuntimeError("src and dst must have one entry per pair")
+    n = src.numel()
+    src, dst = _int32_list("src", src, n), _int32_list("dst", dst, n)
+    layers = key_pool.size(0) if key_pool.dim() == 5 else 1
+    Hkv, NB, bs, D = key_pool.shape[-4:]
+    with torch.cuda.device(device):
+        stream = torch.cuda.current_stream(device).cuda_stream
+        check(lib().bs_copy_blocks(
+            key_pool.data_ptr(), value_pool.data_ptr(), dtype_code(key_pool.dtype), layers, Hkv, NB,
+            bs, D, src.data_ptr(), dst.data_ptr(), n, workspace_for(device, 0).data_ptr(), stream))

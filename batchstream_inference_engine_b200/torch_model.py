@@ -31,7 +31,7 @@ from __future__ import annotations
 
 import json
 import struct
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from pathlib import Path
 
 import torch
@@ -51,6 +51,16 @@ class ModelConfig:
     num_kv_heads: int
     rope_theta: float
     rms_norm_eps: float
+    # Forms that the reference has no counterpart for; the defaults are its model.
+    # attention_window > 0: a token sees the last attention_window tokens (itself
+    # included) and the first attention_sinks ones, and the cache keeps only those.
+    attention_window: int = 0
+    attention_sinks: int = 0
+    # Rotary embedding over the first rotary_dim dims of a head (0: all), in
+    # interleaved pairs, with frequencies scaled as ops.rope_frequencies has it.
+    rotary_dim: int = 0
+    rope_interleaved: bool = False
+    rope_scaling: dict | None = field(default=None, hash=False)
 
     @classmethod
     def from_file(cls, path: Path) -> "ModelConfig":
@@ -67,6 +77,13 @@ class ModelConfig:
     @property
     def head_dim(self) -> int:
         return self.hidden_size // self.num_heads
+
+    @property
+    def rotary_from_tables(self) -> bool:
+        """The reference's rotary embedding: half layout over the whole head,
+        from bf16 cos/sin tables."""
+        return (self.rotary_dim in (0, self.head_dim) and not self.rope_interleaved
+                and self.rope_scaling is None)
 
 
 # The Qwen2.5-0.5B shape (24 layers, hidden 896, 14 / 2 heads, head_dim 64).
@@ -181,6 +198,32 @@ class PagedKVPool:
     def release(self, cache: "PagedKVCache") -> None:
         self.allocator.free(cache.seq_id)
 
+    def fork(self, cache: "PagedKVCache", seq_id: int) -> "PagedKVCache":
+        """A new sequence that starts with the tokens cached for `cache`: whole
+        blocks are shared, a last partial one is copied (all layers, one launch)."""
+        self._copy(self.allocator.fork(cache.seq_id, seq_id, cache.length))
+        child = self.new_cache(seq_id)
+        child.length = cache.length
+        return child
+
+    def trim(self, cache: "PagedKVCache", window: int, sinks: int) -> int:
+        """Frees the blocks that no token after the cached ones sees through a
+        window of `window` tokens and `sinks` first ones; returns how many."""
+        return self.allocator.trim(cache.seq_id, cache.length - window + 1, keep_first=sinks)
+
+    def compact(self) -> int:
+        """Moves the blocks in use to the lowest ids (all layers, one launch);
+        returns how many moved."""
+        pairs = self.allocator.compact()
+        self._copy(pairs)
+        return len(pairs)
+
+    def _copy(self, pairs: list[tuple[int, int]]) -> None:
+        if pairs:
+            ends = torch.tensor(pairs, dtype=torch.int32).t().contiguous().pin_memory()
+            src, dst = ends.to(self.device, non_blocking=True)
+            ops.copy_blocks(self.keys, self.values, src, dst)
+
 
 class PagedKVCache:
     """One sequence's view of the pool (src/server/torch_model.py:140-170).  The
@@ -265,13 +308,19 @@ class TorchModel:
         # Rotary tables exactly as the reference makes them (fp32 angles on the
         # CPU, cos/sin rounded to bf16, torch_model.py:199-200, 289-292), built
         # once for every position and gathered per step on the device.
-        steps = torch.arange(0, config.head_dim, 2, dtype=torch.float)
-        inverse_frequencies = 1.0 / (config.rope_theta ** (steps / config.head_dim))
-        positions = torch.arange(max_position)
-        frequencies = positions[:, None].float() * inverse_frequencies
-        angles = torch.cat((frequencies, frequencies), dim=-1)
-        self.cos = angles.cos().to(torch.bfloat16).to(device=self.device, dtype=dtype)
-        self.sin = angles.sin().to(torch.bfloat16).to(device=self.device, dtype=dtype)
+        # Other rotary forms go from frequencies instead (ops.rotary_append).
+        if config.rotary_from_tables:
+            steps = torch.arange(0, config.head_dim, 2, dtype=torch.float)
+            inverse_frequencies = 1.0 / (config.rope_theta ** (steps / config.head_dim))
+            positions = torch.arange(max_position)
+            frequencies = positions[:, None].float() * inverse_frequencies
+            angles = torch.cat((frequencies, frequencies), dim=-1)
+            self.cos = angles.cos().to(torch.bfloat16).to(device=self.device, dtype=dtype)
+            self.sin = angles.sin().to(torch.bfloat16).to(device=self.device, dtype=dtype)
+        else:
+            self.rope_frequencies, self.rope_amplitude = ops.rope_frequencies(
+                config.rotary_dim or config.head_dim, config.rope_theta, config.rope_scaling,
+                device=self.device)
         self.max_position = max_position
         # Per-step accounting for benchmarks: forwards, tokens and rows
         # processed, attention FLOPs (QK^T + PV over visible keys), launches of
@@ -428,27 +477,66 @@ class TorchModel:
 
         def attend(q, kp, vp, attended):
             if n_dec:
-                ops.paged_attention_batched(q[:n_dec], kp, vp, alloc.device_tables, ctx_d[:n_dec],
-                                            config.head_dim ** -0.5, seq_rows=rows_d[:n_dec],
-                                            out=attended[:n_dec], lens_ready=True,
-                                            after_append=True)
+                self._attend_tokens(q[:n_dec], kp, vp, alloc.device_tables, ctx_d[:n_dec],
+                                    rows_d[:n_dec], attended[:n_dec])
             if n_dec < R:
-                ops.prefill_attention(q[n_dec:], kp, vp, alloc.device_tables, pre_cu,
-                                      ctx[n_dec:], config.head_dim ** -0.5,
-                                      max_query_len=max_chunk, seq_rows=rows_d[n_dec:],
-                                      out=attended[n_dec:])
+                self._attend_chunks(q[n_dec:], kp, vp, alloc.device_tables, pre_cu, ctx[n_dec:],
+                                    max_chunk, rows_d[n_dec:], attended[n_dec:])
 
         last = self._layers(pool, self._resolve(pool, tokens_d), positions, slots, ends_d, attend)
-        for (tokens, cache) in groups:
-            cache.advance(len(tokens))
+        self._advance(pool, groups)
         st = self.stats
         st["steps"] += 1
         st["tokens"] += T
         st["rows"] += R
-        st["attn_flops"] += config.num_layers * 4 * config.num_heads * config.head_dim * sum(
-            n * s + n * (n + 1) // 2 for s, n in zip(starts, lengths))
+        st["attn_flops"] += self._attention_flops(starts, lengths)
         st["launches"] += ops.kernel_launches() - launches
         return last
+
+    def _attend_tokens(self, q, kp, vp, tables, lens, rows, out) -> None:
+        """One layer's attention of the rows that hold one new token each."""
+        c = self.config
+        if c.attention_window:
+            ops.window_attention_batched(q, kp, vp, tables, lens, c.head_dim ** -0.5,
+                                         c.attention_window, c.attention_sinks, seq_rows=rows,
+                                         out=out)
+        else:
+            ops.paged_attention_batched(q, kp, vp, tables, lens, c.head_dim ** -0.5,
+                                        seq_rows=rows, out=out, lens_ready=True,
+                                        after_append=True)
+
+    def _attend_chunks(self, q, kp, vp, tables, cu_q, lens, max_query_len, rows, out) -> None:
+        """One layer's attention of the prompt chunks."""
+        c = self.config
+        if c.attention_window:
+            ops.window_prefill_attention(q, kp, vp, tables, cu_q, lens, c.head_dim ** -0.5,
+                                         max_query_len, c.attention_window, c.attention_sinks,
+                                         seq_rows=rows, out=out)
+        else:
+            ops.prefill_attention(q, kp, vp, tables, cu_q, lens, c.head_dim ** -0.5,
+                                  max_query_len=max_query_len, seq_rows=rows, out=out)
+
+    def _advance(self, pool: PagedKVPool, groups) -> None:
+        """Counts a launched step's tokens as cached and frees the blocks behind
+        the window (a later step that takes them runs after this one)."""
+        for tokens, cache in groups:
+            cache.advance(len(tokens))
+            if self.config.attention_window:
+                pool.trim(cache, self.config.attention_window, self.config.attention_sinks)
+
+    def _attention_flops(self, starts, lengths) -> int:
+        """QK^T and PV FLOPs of a step, over the keys its tokens see."""
+        c = self.config
+        seen = sum(n * s + n * (n + 1) // 2 for s, n in zip(starts, lengths))
+        if c.attention_window:
+            # Token p does not see p + 1 - both keys (if any), those between the
+            # sinks and its window.
+            both = c.attention_window + c.attention_sinks
+            for s, n in zip(starts, lengths):
+                last = max(0, s + n - both)
+                hiding = min(n, last)  # the chunk's tokens that miss any
+                seen -= hiding * last - hiding * (hiding - 1) // 2
+        return c.num_layers * 4 * c.num_heads * c.head_dim * seen
 
     @staticmethod
     def _resolve(pool: PagedKVPool, tokens: torch.Tensor) -> torch.Tensor:
@@ -478,7 +566,12 @@ class TorchModel:
                 normed = ops.rms_norm(hidden, lw["ln1"], eps, add=delta, sum_out=hidden)
             qkv = F.linear(normed, lw["qkv_w"], lw["qkv_b"])
             kp, vp = pool.keys[layer], pool.values[layer]
-            ops.rope_append(qkv, self.cos, self.sin, positions, slots, kp, vp, H, query_out=q)
+            if config.rotary_from_tables:
+                ops.rope_append(qkv, self.cos, self.sin, positions, slots, kp, vp, H, query_out=q)
+            else:
+                ops.rotary_append(qkv, self.rope_frequencies, positions, slots, kp, vp, H,
+                                  interleaved=config.rope_interleaved,
+                                  amplitude=self.rope_amplitude, query_out=q)
             attend(q, kp, vp, attended)
             delta = F.linear(attended.view(T, H * D), lw["o_w"])
             normed = ops.rms_norm(hidden, lw["ln2"], eps, add=delta, sum_out=hidden)
@@ -525,7 +618,6 @@ class TorchModel:
         decode rows then P prompt-chunk rows holding up to Q tokens, described
         by the int32 ``inputs`` (see ``_graph_inputs``).  Launches only (no host
         synchronisation), so it can be captured."""
-        config = self.config
         B, P, Q = key
         R, T = B + P, B + Q
         alloc = pool.allocator
@@ -534,16 +626,14 @@ class TorchModel:
             alloc.device_tables, start, n_new, T, pool.block_size, pool.num_blocks,
             seq_rows=rows)
         pre_cu = cu_q[B:] - B if P else None
-        scale = config.head_dim ** -0.5
 
         def attend(q, kp, vp, attended):
             if B:
-                ops.paged_attention_batched(q[:B], kp, vp, alloc.device_tables, after, scale,
-                                            seq_rows=rows[:B], out=attended[:B], lens_ready=True,
-                                            after_append=True)
+                self._attend_tokens(q[:B], kp, vp, alloc.device_tables, after, rows[:B],
+                                    attended[:B])
             if P:
-                ops.prefill_attention(q[B:], kp, vp, alloc.device_tables, pre_cu, ctx[B:], scale,
-                                      max_query_len=Q, seq_rows=rows[B:], out=attended[B:])
+                self._attend_chunks(q[B:], kp, vp, alloc.device_tables, pre_cu, ctx[B:], Q,
+                                    rows[B:], attended[B:])
 
         last = self._layers(pool, self._resolve(pool, tokens), positions, slots, ends, attend)
         ids = ops.argmax_rows(F.linear(last, self.embed))
@@ -657,14 +747,12 @@ class TorchModel:
         inputs.copy_(self._stage(values))
         graph.replay()
         B = key[0]
-        for tokens, cache in groups:
-            cache.advance(len(tokens))
+        self._advance(pool, groups)
         st = self.stats
         st["steps"] += 1
         st["tokens"] += sum(lengths)
         st["rows"] += len(groups)
-        st["attn_flops"] += config.num_layers * 4 * config.num_heads * config.head_dim * sum(
-            n * s + n * (n + 1) // 2 for s, n in zip(starts, lengths))
+        st["attn_flops"] += self._attention_flops(starts, lengths)
         st["launches"] += graph_launches
         index = list(range(n_dec)) + list(range(B, B + len(groups) - n_dec))
         return self._pending(ids, index)

@@ -53,6 +53,7 @@ enum bs_error {
 #define BS_STATUS_BAD_ROW 0x10u
 #define BS_STATUS_BAD_POSITION 0x20u
 #define BS_STATUS_BAD_INDEX 0x40u
+#define BS_STATUS_BAD_COPY 0x80u
 
 /* Message of the last failing call on this thread ("" if none). */
 const char* bs_last_error(void);
@@ -315,6 +316,97 @@ int bs_silu_mul(const void* gate_up, int64_t row_stride, int64_t num_tokens, int
  */
 int bs_argmax_rows(const void* logits, int64_t row_stride, int64_t rows, int64_t cols,
                    int32_t dtype, int32_t* out, void* stream);
+
+/*
+ * Sliding-window attention with sink tokens over the paged cache (no counterpart
+ * in the reference, which attends over every cached token).  The query token at
+ * position p of a sequence sees key j when
+ *     j <= p  and  (j < sinks  or  j > p - window).
+ * Blocks that no query token of the call sees are never read, so their table
+ * entries may hold anything (freed blocks: BS_EMPTY_BLOCK by convention).
+ *
+ * bs_window_attention_batched: one new token per sequence, as
+ * bs_paged_attention_batched; sequence b's token is at position
+ * context_lens[b] - 1.  bs_window_prefill_attention: chunks of new tokens, as
+ * bs_prefill_attention; a chunk that is longer than max_query_len, that lies
+ * outside the num_tokens rows, or whose context is shorter than itself is
+ * reported and skipped.  A context length of 0 marks a padding row in both:
+ * nothing is read for it and its output rows are left as they were.
+ *
+ * window >= 1 and sinks >= 0 (values past 2^30 mean all); a table row covers at
+ * most 2^30 tokens.  Scores, softmax statistics and sums are fp32; the
+ * tensor-core kernels (bf16, head_dim 64 or 128, block sizes that are multiples
+ * of 16) round the probabilities to bf16 before they weight V, the others keep
+ * them in fp32.
+ *
+ * `workspace` is scratch of the size that the matching query gives: 16-byte
+ * aligned, its contents irrelevant before and after, one per call in flight (it
+ * may be NULL when that size is 0).  `status` is a device word (may be NULL)
+ * that gets the status bits.
+ */
+#define BS_EMPTY_BLOCK (-1)
+int bs_window_attention_batched(const void* query, int64_t query_seq_stride, const void* key_pool,
+                                const void* value_pool, const int32_t* block_tables,
+                                int64_t table_stride, int64_t table_rows, const int32_t* seq_rows,
+                                const int32_t* context_lens, int64_t num_seqs, int64_t num_heads,
+                                int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                                int64_t num_blocks, int64_t max_blocks_per_seq, int32_t dtype,
+                                double scaling, int64_t window, int64_t sinks, void* output,
+                                int64_t output_seq_stride, void* workspace,
+                                uint64_t workspace_bytes, uint32_t* status, void* stream);
+int bs_window_attention_batched_workspace_bytes(int64_t num_seqs, int64_t num_heads,
+                                                int64_t num_kv_heads, int64_t head_dim,
+                                                int64_t block_size, int64_t max_blocks_per_seq,
+                                                int32_t dtype, int64_t window, int64_t sinks,
+                                                uint64_t* bytes_out);
+int bs_window_prefill_attention(const void* query, int64_t query_token_stride, const int32_t* cu_q,
+                                int64_t num_rows, int64_t num_tokens, int64_t max_query_len,
+                                const int32_t* context_lens, const int32_t* seq_rows,
+                                const void* key_pool, const void* value_pool,
+                                const int32_t* block_tables, int64_t table_stride,
+                                int64_t table_rows, int64_t max_blocks_per_seq, int64_t num_heads,
+                                int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                                int64_t num_blocks, int32_t dtype, double scaling, int64_t window,
+                                int64_t sinks, void* output, int64_t output_token_stride,
+                                void* workspace, uint64_t workspace_bytes, uint32_t* status,
+                                void* stream);
+int bs_window_prefill_attention_workspace_bytes(int64_t num_tokens, int64_t num_rows,
+                                                int64_t max_query_len, int64_t num_heads,
+                                                int64_t num_kv_heads, int64_t head_dim,
+                                                int64_t block_size, int64_t max_blocks_per_seq,
+                                                int32_t dtype, int64_t window, int64_t sinks,
+                                                uint64_t* bytes_out);
+
+/*
+ * Rotary embedding and K/V append as bs_rope_append, from frequencies instead of
+ * tables: pair i of the first rotary_dim dims of every q and k head turns by
+ * position * frequencies[i] (rotary_dim / 2 fp64 values in device memory; angles
+ * are formed in fp64, so positions up to 2^31 keep fp32 accuracy), its result
+ * multiplied by `amplitude`; the other dims are copied.  Pairs are dims
+ * (i, i + rotary_dim / 2), or (2i, 2i + 1) with `interleaved`.  One rounding, to
+ * the output's dtype.  A negative slot skips the row's pool writes; a negative
+ * position skips its q and k, a slot past the pool its pool writes, and each
+ * sets a bit in *status.  Two rows must not name the same slot.
+ */
+int bs_rotary_append(const void* qkv, int64_t qkv_row_stride, int32_t dtype,
+                     const double* frequencies, int64_t rotary_dim, int32_t interleaved,
+                     double amplitude, const int32_t* positions, const int32_t* slot_mapping,
+                     int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                     void* query_out, void* key_pool, void* value_pool, int32_t pool_dtype,
+                     int64_t num_blocks, int64_t block_size, uint32_t* status, void* stream);
+
+/*
+ * Copies block src[i] of every layer and kv head to block dst[i], K and V
+ * (pools [num_layers, num_kv_heads, num_blocks, block_size, head_dim],
+ * contiguous), all pairs at once.  A pair with a negative end is padding, a pair
+ * onto itself does nothing.  A block outside the pool (BS_STATUS_BAD_BLOCK) or a
+ * destination that another pair also names, as source or destination
+ * (BS_STATUS_BAD_COPY), sets the bit in *status and skips the pair.
+ */
+int bs_copy_blocks(void* key_pool, void* value_pool, int32_t pool_dtype, int64_t num_layers,
+                   int64_t num_kv_heads, int64_t num_blocks, int64_t block_size, int64_t head_dim,
+                   const int32_t* src, const int32_t* dst, int64_t num_pairs, uint32_t* status,
+                   void* stream);
 
 /*
  * Waits for `stream`, then reads and clears the status word at the start of a
