@@ -1089,6 +1089,11 @@ int32_t decode_record_stride(int64_t groups, int64_t head_dim) {
 }
 void add_kernel_launches(int n) { count_launches(n); }
 
+// Tensor map of a pool's [rows, head_dim] view for 16 x 64 boxes (see encode_pool_map).
+int pool_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int64_t head_dim) {
+  return encode_pool_map(map, base, rows, head_dim);
+}
+
 int sm_count(int* sms) {
   DeviceInfo* d = nullptr;
   if (int rc = current_device_info(&d)) return rc;

@@ -9,18 +9,23 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
 
 #include "../../include/batchstream_b200.h"
+#include "decode.cuh"
 #include "window.cuh"
 
 namespace bsb {
-// capi.cu: messages, launch count, SMs of the current device.
+// capi.cu: messages, launch count, SMs of the current device, tensor maps and
+// record sizes of the decode kernels.
 void set_last_error(const char* message);
 void add_kernel_launches(int n);
 int sm_count(int* sms);
+int pool_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int64_t head_dim);
+int32_t decode_record_stride(int64_t groups, int64_t head_dim);
 int launch_rotary_append(const void* qkv, int64_t qkv_stride, bool bf16, const double* freq,
                          int32_t rotary_dim, bool interleaved, double amp, const int32_t* pos,
                          const int32_t* slots, int32_t ntok, int32_t H, int32_t Hkv, int32_t D,
@@ -129,12 +134,61 @@ int plan_simt(const WindowShape& s, SimtPlan* p) {
   return BS_OK;
 }
 
+// Shapes the tensor-core kernels take (with 16-byte aligned pools and queries, and
+// outputs that their stores can address; see mma_pointers).
+bool mma_shape(const WindowShape& s) {
+  return s.dtype == BS_BF16 && s.block_size % 16 == 0 && (s.head_dim == 64 || s.head_dim == 128);
+}
+
+// How the tensor-core decode runs a call: persistent CTAs over the batch's units,
+// two partial records and one merge task each.
+struct MmaDecodePlan {
+  int64_t grid, rec_stride, tasks_offset, bytes;
+};
+
+int plan_mma_decode(const WindowShape& s, MmaDecodePlan* p) {
+  int sms = 0, dev = 0;
+  if (int rc = bsb::sm_count(&sms)) return rc;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  const int64_t groups = s.heads / s.kv_heads;
+  // Resident CTAs per SM by device, [head_dim 128][more than 8 heads a group].
+  static std::atomic<int> resident[64][2][2];
+  std::atomic<int>* known = dev < 64 ? &resident[dev][s.head_dim == 128][groups > 8] : nullptr;
+  int ctas = known != nullptr ? known->load() : 0;
+  if (ctas == 0) {
+    ctas = bsb::window_decode_mma_ctas_per_sm(static_cast<int>(s.head_dim),
+                                              static_cast<int>(groups));
+    if (ctas <= 0) return fail(BS_ERR_CUDA, "occupancy query for window decode failed (%d)", ctas);
+    if (known != nullptr) known->store(ctas);
+  }
+  // Units the batch can hold: a window of n tokens touches n / 16 + 1 of them.
+  // Fewer than one unit a warp would only add records to merge.
+  const int64_t unit = bsb::kWindowUnit;
+  const int64_t seen = (std::min(s.window, kMaxContext) + unit - 1) / unit + 1 +
+                       (std::min(s.sinks, kMaxContext) + unit - 1) / unit;
+  const int64_t units = s.rows * s.kv_heads * std::min(seen, s.max_blocks * s.block_size / unit);
+  p->grid = std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(sms) * ctas,
+                                                   (units + 3) / 4));
+  p->rec_stride = bsb::decode_record_stride(groups, s.head_dim);
+  p->tasks_offset = (2 * p->grid * p->rec_stride * 4 + 255) / 256 * 256;
+  p->bytes = p->tasks_offset + p->grid * static_cast<int64_t>(sizeof(bsb::MergeTask));
+  return BS_OK;
+}
+
+// Scratch of a call: the largest of the kernels its shape may run on.
 int window_workspace(const WindowShape& s, uint64_t* bytes_out) {
   BS_CHECK(bytes_out != nullptr, "bytes_out is null");
   if (int rc = check_window_shape(s)) return rc;
   SimtPlan p;
   if (int rc = plan_simt(s, &p)) return rc;
-  *bytes_out = static_cast<uint64_t>(p.bytes);
+  int64_t need = p.bytes;
+  if (mma_shape(s) && !s.chunks) {
+    MmaDecodePlan m;
+    if (int rc = plan_mma_decode(s, &m)) return rc;
+    need = std::max(need, m.bytes);
+  }
+  *bytes_out = static_cast<uint64_t>(need);
   return BS_OK;
 }
 
@@ -158,6 +212,67 @@ struct WindowCall {
   void* stream;
 };
 
+int check_workspace(const WindowCall& c, int64_t need) {
+  if (need > 0 && (c.workspace == nullptr || c.workspace_bytes < static_cast<uint64_t>(need))) {
+    return fail(BS_ERR_WORKSPACE, "workspace of %llu bytes is smaller than the %lld needed",
+                static_cast<unsigned long long>(c.workspace_bytes), static_cast<long long>(need));
+  }
+  BS_CHECK(aligned16(c.workspace), "workspace must be 16-byte aligned");
+  return BS_OK;
+}
+
+// Pointers and strides the tensor-core kernels can take: TMA and bulk copies of
+// pools and query rows, 16-byte output rows.
+bool mma_pointers(const WindowCall& c) {
+  return aligned16(c.query) && aligned16(c.key_pool) && aligned16(c.value_pool) &&
+         aligned16(c.output) && c.q_stride % 8 == 0 && c.o_stride % 8 == 0;
+}
+
+int run_mma_decode(const WindowShape& s, const WindowCall& c) {
+  MmaDecodePlan p;
+  if (int rc = plan_mma_decode(s, &p)) return rc;
+  if (int rc = check_workspace(c, p.bytes)) return rc;
+  CUtensorMap kmap, vmap;
+  const int64_t rows = s.kv_heads * c.num_blocks * s.block_size;
+  if (int rc = bsb::pool_tensor_map(&kmap, c.key_pool, rows, s.head_dim)) return rc;
+  if (int rc = bsb::pool_tensor_map(&vmap, c.value_pool, rows, s.head_dim)) return rc;
+  bsb::DecodeArgs a{};
+  a.q = c.query;
+  a.q_stride_seq = c.q_stride;
+  a.out = c.output;
+  a.o_stride_seq = c.o_stride;
+  a.k_pool = c.key_pool;
+  a.v_pool = c.value_pool;
+  a.block_tables = c.block_tables;
+  a.bt_stride = c.table_stride;
+  a.bt_rows = static_cast<int32_t>(c.table_rows);
+  a.seq_rows = c.seq_rows;
+  a.context_lens = c.context_lens;
+  a.num_seqs = static_cast<int32_t>(s.rows);
+  a.num_heads = static_cast<int32_t>(s.heads);
+  a.num_kv_heads = static_cast<int32_t>(s.kv_heads);
+  a.groups = static_cast<int32_t>(s.heads / s.kv_heads);
+  a.head_dim = static_cast<int32_t>(s.head_dim);
+  a.block_size = static_cast<int32_t>(s.block_size);
+  a.num_blocks = static_cast<int32_t>(c.num_blocks);
+  a.max_blocks = static_cast<int32_t>(s.max_blocks);
+  a.scale = static_cast<float>(c.scaling);
+  uint8_t* ws = static_cast<uint8_t*>(c.workspace);
+  a.partials = reinterpret_cast<float*>(ws);
+  a.rec_stride = static_cast<int32_t>(p.rec_stride);
+  a.tasks = reinterpret_cast<bsb::MergeTask*>(ws + p.tasks_offset);
+  a.status = c.status;
+  a.window = static_cast<int32_t>(std::min(s.window, kMaxContext));
+  a.sinks = static_cast<int32_t>(std::min(s.sinks, kMaxContext));
+  a.block_units = static_cast<int32_t>(s.block_size / bsb::kWindowUnit);
+  bsb::apply_wait_probe(a);
+  const int rc = bsb::launch_window_decode_mma(a, kmap, vmap, static_cast<int>(p.grid),
+                                               static_cast<cudaStream_t>(c.stream));
+  if (rc != 0) return cuda_fail(rc, "window decode launch");
+  bsb::add_kernel_launches(2);  // the decode and its merge pass
+  return BS_OK;
+}
+
 int run_window(const WindowShape& s, const WindowCall& c) {
   if (int rc = check_window_shape(s)) return rc;
   BS_CHECK(s.max_blocks <= c.table_stride, "max_blocks_per_seq must be in [1, table_stride]");
@@ -174,6 +289,7 @@ int run_window(const WindowShape& s, const WindowCall& c) {
   BS_CHECK(c.query && c.key_pool && c.value_pool && c.block_tables && c.context_lens &&
                c.output && (!s.chunks || c.cu_q),
            "null pointer argument");
+  if (mma_shape(s) && !s.chunks && mma_pointers(c)) return run_mma_decode(s, c);
   bsb::WindowArgs a{};
   a.q = c.query;
   a.q_stride = c.q_stride;
@@ -204,13 +320,7 @@ int run_window(const WindowShape& s, const WindowCall& c) {
 
   SimtPlan p;
   if (int rc = plan_simt(s, &p)) return rc;
-  if (p.bytes > 0 &&
-      (c.workspace == nullptr || c.workspace_bytes < static_cast<uint64_t>(p.bytes))) {
-    return fail(BS_ERR_WORKSPACE, "workspace of %llu bytes is smaller than the %lld needed",
-                static_cast<unsigned long long>(c.workspace_bytes),
-                static_cast<long long>(p.bytes));
-  }
-  BS_CHECK(aligned16(c.workspace), "workspace must be 16-byte aligned");
+  if (int rc = check_workspace(c, p.bytes)) return rc;
   a.tile_tokens = static_cast<int32_t>(p.tile_tokens);
   a.qtiles = static_cast<int32_t>(p.qtiles);
   a.splits = static_cast<int32_t>(p.splits);

@@ -70,14 +70,46 @@ struct DecodeArgs {
   // warp 0 of CTA 0 never arms or fills its stages, so its first wait runs
   // out with no copy in flight.  Zero in every production call.
   int32_t probe_unarmed;
+  // Sliding-window calls only (the WIN variants below): keys j < sinks or
+  // j >= len - window are seen; a unit is then 16 tokens, `block_units` of them to
+  // a block.
+  int32_t window, sinks, block_units;
 };
+
+// Tokens per unit of the sliding-window variant (one tile of the tensor cores).
+constexpr int32_t kWindowUnit = 16;
+
+// Units of a sequence of `len` tokens seen through the window: the sink_units
+// first ones, then those from the window's first unit on.
+struct WindowUnits {
+  int32_t sink_units, first_unit, units;
+};
+
+__device__ __forceinline__ WindowUnits window_units(const DecodeArgs& a, int32_t len) {
+  WindowUnits w;
+  w.first_unit = max(0, len - a.window) / kWindowUnit;
+  w.sink_units = min((a.sinks + kWindowUnit - 1) / kWindowUnit, w.first_unit);
+  w.units = w.sink_units + (len + kWindowUnit - 1) / kWindowUnit - w.first_unit;
+  return w;
+}
 
 // Applies the process-wide wait settings of bs_set_wait_probe (capi.cu) to a
 // launch.
 void apply_wait_probe(DecodeArgs& a);
 
+// Units of a valid length.
+template <bool WIN>
+__device__ __forceinline__ int32_t length_units(const DecodeArgs& a, int32_t len) {
+  if constexpr (WIN) {
+    return window_units(a, len).units;
+  } else {
+    return (len + a.block_size - 1) / a.block_size;
+  }
+}
+
 // Units of a sequence from its raw length and table row (already loaded);
 // invalid ones count as 0 units with len = 0.
+template <bool WIN = false>
 __device__ __forceinline__ int32_t units_of(const DecodeArgs& a, int32_t raw_len, int32_t raw_row,
                                             int32_t& len, int32_t& row) {
   len = raw_len;
@@ -87,11 +119,12 @@ __device__ __forceinline__ int32_t units_of(const DecodeArgs& a, int32_t raw_len
     len = 0;
     return 0;
   }
-  return (len + a.block_size - 1) / a.block_size;
+  return length_units<WIN>(a, len);
 }
 
 // Units of a sequence with raw length `raw_len` and table row `raw_row` after
 // validation; also returns the clamped length.
+template <bool WIN = false>
 __device__ __forceinline__ int32_t seq_units_raw(const DecodeArgs& a, int32_t raw_len,
                                                  int32_t raw_row, int32_t& len, int32_t& row,
                                                  bool report) {
@@ -109,13 +142,14 @@ __device__ __forceinline__ int32_t seq_units_raw(const DecodeArgs& a, int32_t ra
     len = 0;
     return 0;
   }
-  return (len + a.block_size - 1) / a.block_size;
+  return length_units<WIN>(a, len);
 }
 
 // Units of sequence i after validation; also returns the clamped length.
+template <bool WIN = false>
 __device__ __forceinline__ int32_t seq_units(const DecodeArgs& a, int32_t i, int32_t& len,
                                              int32_t& row, bool report) {
-  return seq_units_raw(a, __ldg(a.context_lens + i),
+  return seq_units_raw<WIN>(a, __ldg(a.context_lens + i),
                        a.seq_rows != nullptr ? __ldg(a.seq_rows + i) : i, len, row, report);
 }
 
@@ -162,6 +196,7 @@ __device__ __forceinline__ int64_t warp_inclusive_scan(int64_t v) {
 
 // All threads of the CTA call this.  Computes W and this CTA's span, and (when
 // find_start) finds the sequence holding the span's first unit.
+template <bool WIN = false>
 __device__ __forceinline__ Span compute_span(const DecodeArgs& a, ScanSmem& sm,
                                              bool find_start = true) {
   const int tid = threadIdx.x, nthr = blockDim.x, lane = tid & 31, warp = tid >> 5;
@@ -174,7 +209,7 @@ __device__ __forceinline__ Span compute_span(const DecodeArgs& a, ScanSmem& sm,
   int64_t local = 0;
   for (int32_t i = tid; i < B; i += nthr) {
     int32_t len, row;
-    local += seq_units(a, i, len, row, c == 0);
+    local += seq_units<WIN>(a, i, len, row, c == 0);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) local += __shfl_xor_sync(0xffffffffu, local, o);
@@ -204,7 +239,7 @@ __device__ __forceinline__ Span compute_span(const DecodeArgs& a, ScanSmem& sm,
     int64_t nb = 0;
     if (i < B) {
       int32_t len, row;
-      nb = seq_units(a, i, len, row, false);
+      nb = seq_units<WIN>(a, i, len, row, false);
     }
     int64_t incl = warp_inclusive_scan(nb);
     __syncthreads();  // warp_tot reuse
@@ -337,11 +372,11 @@ struct WarpStarts {
 
 // Like compute_span, then splits the CTA span into NW contiguous warp spans and
 // locates the sequence holding each warp's first unit.  All threads call it.
-template <int NW>
+template <int NW, bool WIN = false>
 __device__ __forceinline__ Span compute_warp_spans(const DecodeArgs& a, ScanSmem& sm,
                                                    WarpStarts& ws) {
   static_assert(NW <= 8, "at most 8 warp spans");
-  Span sp = compute_span(a, sm, false);  // warp 0's start is the CTA's start
+  Span sp = compute_span<WIN>(a, sm, false);  // warp 0's start is the CTA's start
   const int tid = threadIdx.x, nthr = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int nwarps = (nthr + 31) >> 5;
   const int32_t B = a.num_seqs;
@@ -355,7 +390,7 @@ __device__ __forceinline__ Span compute_warp_spans(const DecodeArgs& a, ScanSmem
     int64_t nb = 0;
     if (i < B) {
       int32_t len, row;
-      nb = seq_units(a, i, len, row, false);
+      nb = seq_units<WIN>(a, i, len, row, false);
     }
     int64_t incl = warp_inclusive_scan(nb);
     __syncthreads();
@@ -402,7 +437,7 @@ __device__ __forceinline__ Span compute_warp_spans(const DecodeArgs& a, ScanSmem
 // until this returns), one inclusive scan of the per-thread unit counts gives
 // every thread its prefix and everyone the total, and each thread then looks for
 // the warp start units among its own sequences.  All threads call it.
-template <int NW>
+template <int NW, bool WIN = false>
 __device__ __forceinline__ Span compute_warp_spans_smem(const DecodeArgs& a, ScanSmem& sm,
                                                         WarpStarts& ws, int32_t* scratch) {
   static_assert(NW <= 8, "at most 8 warp spans");
@@ -424,7 +459,7 @@ __device__ __forceinline__ Span compute_warp_spans_smem(const DecodeArgs& a, Sca
     lens[i] = len;
     rows[i] = row;
     int32_t l2, r2;
-    local += seq_units_raw(a, len, row, l2, r2, c == 0);  // CTA 0 reports bad input once
+    local += seq_units_raw<WIN>(a, len, row, l2, r2, c == 0);  // CTA 0 reports bad input once
   }
   const int64_t incl = warp_inclusive_scan(local);
   if (lane == 31) sm.warp_tot[warp] = incl;
@@ -449,7 +484,7 @@ __device__ __forceinline__ Span compute_warp_spans_smem(const DecodeArgs& a, Sca
       const int32_t i = i0 + k;
       if (i >= B) break;
       int32_t len, row;
-      const int64_t nb = seq_units_raw(a, lens[i], rows[i], len, row, false);
+      const int64_t nb = seq_units_raw<WIN>(a, lens[i], rows[i], len, row, false);
       if (nb > 0) {
 #pragma unroll
         for (int t = 0; t < NW; ++t) {
@@ -618,6 +653,10 @@ __device__ void cta_merge_records(const DecodeArgs& a, const Span& sp, int32_t s
 int launch_decode_mma(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap& vmap,
                       int grid, cudaStream_t stream);
 int decode_mma_ctas_per_sm(int head_dim, int groups);
+// The sliding-window variant (block sizes that are multiples of 16; needs tasks).
+int launch_window_decode_mma(const DecodeArgs& a, const CUtensorMap& kmap,
+                             const CUtensorMap& vmap, int grid, cudaStream_t stream);
+int window_decode_mma_ctas_per_sm(int head_dim, int groups);
 int launch_decode_simt(const DecodeArgs& a, int dtype_is_bf16, int grid, cudaStream_t stream);
 int decode_simt_ctas_per_sm(int head_dim, int groups, int dtype_is_bf16);
 

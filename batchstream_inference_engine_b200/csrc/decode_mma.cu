@@ -21,6 +21,11 @@
 // registers.  Cut segments go to per-warp slots in shared memory; after one CTA
 // barrier the warp holding the end of each chain merges it and writes the output
 // or, for a segment that crosses CTAs, the CTA's partial record (decode.cuh).
+//
+// WIN selects the sliding-window form (window attention with sink tokens): a unit
+// is 16 tokens of the sequence's visible range (its sink units, then the window's),
+// masked by a 16-bit map, the block size any multiple of 16, and the scores are not
+// rounded to bf16 (the reference's rounding points belong to the full form only).
 #include "decode.cuh"
 
 namespace bsb {
@@ -33,8 +38,8 @@ enum : int32_t { kFirst = 1, kLast = 2, kWhole = 4, kSlot1 = 8 };
 struct TileMeta {
   int32_t seq;
   int32_t kvh;
-  int32_t blk;  // block index within the sequence
-  int32_t len;  // context length of the sequence
+  int32_t blk;  // block index within the sequence (WIN: unused)
+  int32_t len;  // context length of the sequence (WIN: map of the unit's visible tokens)
   int32_t flags;
   int32_t nb;   // units of the segment
   int64_t seg_unit;
@@ -66,7 +71,7 @@ struct Cfg {
   static_assert(SLOT_FLOATS * 4 <= S * STAGE_BYTES, "slot 1 must fit in the stages");
 };
 
-template <int D, bool G16>
+template <int D, bool G16, bool WIN>
 __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
     decode_mma_kernel(const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap, const DecodeArgs a) {
@@ -117,8 +122,8 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
   constexpr int kScratchInts = W * S * C::STAGE_BYTES / 4;
   const Span sp =
       2 * a.num_seqs <= kScratchInts
-          ? compute_warp_spans_smem<W>(a, scan, starts, reinterpret_cast<int32_t*>(smem))
-          : compute_warp_spans<W>(a, scan, starts);  // both sync the inits
+          ? compute_warp_spans_smem<W, WIN>(a, scan, starts, reinterpret_cast<int32_t*>(smem))
+          : compute_warp_spans<W, WIN>(a, scan, starts);  // both sync the inits
   if (a.lens_ready && !early_loads) pdl_wait();  // query, pools from here on
   if (sp.r0 >= sp.r1) {
     if (a.tasks != nullptr && tid == 0) a.tasks[blockIdx.x].valid = 0;
@@ -145,8 +150,10 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
   // (its latency then hides behind the blocks the current window still holds).
   int32_t pre_row = -1, pre0 = 0, pre_val = 0;
   int64_t cu = wr0;
+  WindowUnits cw{};  // WIN: the current sequence's visible range
   if (ntiles > 0) {
-    cnb = units_of(a, starts.len[warp], starts.row[warp], clen, crow);
+    cnb = units_of<WIN>(a, starts.len[warp], starts.row[warp], clen, crow);
+    if constexpr (WIN) cw = window_units(a, clen);
     const int64_t rel = wr0 - cprefix * Hkv;
     ch = static_cast<int32_t>(rel / cnb);
     cb = static_cast<int32_t>(rel % cnb);
@@ -169,21 +176,43 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
     // The window caches up to 32 entries of one table row, filled to the row's
     // width rather than this sequence's block count: sequences that share a row
     // (the tokens of a prefill chunk) have different lengths and reuse it.
-    if (win_row != crow || cb < win0 || cb >= win0 + 32) {
-      if (pre_row == crow && cb >= pre0 && cb < pre0 + 32) {
+    // WIN: the unit's place in the sequence; `ent` is its table entry.
+    const int32_t tu = !WIN || cb < cw.sink_units ? cb : cb - cw.sink_units + cw.first_unit;
+    const int32_t ent = !WIN || a.block_units == 1 ? tu : tu / a.block_units;
+    if (win_row != crow || ent < win0 || ent >= win0 + 32) {
+      if (pre_row == crow && ent >= pre0 && ent < pre0 + 32) {
         win_row = pre_row;
         win0 = pre0;
         win_val = pre_val;
       } else {
         win_row = crow;
-        win0 = cb;
-        win_val = window(crow, cb);
+        win0 = ent;
+        win_val = window(crow, ent);
       }
       // Prefetch the window the cursor needs next: the rest of this segment,
       // else this sequence's other kv heads (the same row from entry 0), else
       // the next sequence's row.
       int32_t next_row = -1, next0 = 0;
-      if (win0 + 32 < cnb) {
+      if constexpr (WIN) {
+        // From the sinks to the window's first entry (when it lies outside), then
+        // along the window, then to where the next segment starts.
+        const int32_t first = cw.first_unit / a.block_units;
+        const int32_t end = ((clen + kWindowUnit - 1) / kWindowUnit - 1) / a.block_units;
+        if (cb < cw.sink_units && first >= win0 + 32) {
+          next_row = crow;
+          next0 = first;
+        } else if (win0 + 32 <= end) {
+          next_row = crow;
+          next0 = win0 + 32;
+        } else if (ch + 1 < a.num_kv_heads) {
+          next_row = crow;
+          next0 = cw.sink_units > 0 ? 0 : first;
+        } else if (ci + 1 < a.num_seqs && nxt_row >= 0 && nxt_row < a.bt_rows) {
+          next_row = nxt_row;
+          const WindowUnits nw = window_units(a, max(nxt_len, 0));
+          next0 = nw.sink_units > 0 ? 0 : nw.first_unit / a.block_units;
+        }
+      } else if (win0 + 32 < cnb) {
         next_row = crow;
         next0 = win0 + 32;
       } else if (ch + 1 < a.num_kv_heads) {
@@ -197,7 +226,7 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
         pre_val = window(next_row, next0);
       }
     }
-    const int32_t blk = __shfl_sync(0xffffffffu, win_val, cb - win0);
+    const int32_t blk = __shfl_sync(0xffffffffu, win_val, ent - win0);
     const bool valid = blk >= 0 && blk < a.num_blocks;
     const int64_t seg_unit = cprefix * Hkv + static_cast<int64_t>(ch) * cnb;
     const bool first = (cu == wr0) || (cb == 0);
@@ -208,8 +237,16 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
       TileMeta& m = meta[warp][stage];
       m.seq = ci;
       m.kvh = ch;
-      m.blk = cb;
-      m.len = clen;
+      if constexpr (WIN) {
+        const int32_t tok0 = tu * kWindowUnit, lo = clen - a.window;
+        auto below = [](int32_t n) {  // map of a unit's first n tokens
+          return n >= kWindowUnit ? 0xffff : n <= 0 ? 0 : (1 << n) - 1;
+        };
+        m.len = valid ? below(clen - tok0) & (~below(lo - tok0) | below(a.sinks - tok0)) : 0;
+      } else {
+        m.blk = cb;
+        m.len = clen;
+      }
       m.flags = (first ? kFirst : 0) | (last ? kLast : 0) | (whole ? kWhole : 0) |
                 (seg_unit > wr0 ? kSlot1 : 0);
       m.nb = cnb;
@@ -222,7 +259,9 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
       if (valid) {
         // Row of the block in the [Hkv * NB * bs, D] view; the host checks that
         // Hkv * NB * bs fits in int32.
-        const int32_t y = (ch * a.num_blocks + blk) * kBS;
+        const int32_t y = WIN ? (ch * a.num_blocks + blk) * a.block_size +
+                                    (tu - ent * a.block_units) * kBS
+                              : (ch * a.num_blocks + blk) * kBS;
 #pragma unroll
         for (int hf = 0; hf < C::HALVES; ++hf) {
           tma_load_2d_hint(st + hf * 2048, &kmap, &full_bar[warp][stage], hf * 64, y, policy);
@@ -246,11 +285,12 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
         ch = 0;
         cprefix += cnb;
         ++ci;
-        cnb = (ci < a.num_seqs) ? units_of(a, nxt_len, nxt_row, clen, crow) : 1;
+        cnb = (ci < a.num_seqs) ? units_of<WIN>(a, nxt_len, nxt_row, clen, crow) : 1;
         while (cnb == 0) {  // empty or invalid sequences own no units
           ++ci;
-          cnb = (ci < a.num_seqs) ? seq_units(a, ci, clen, crow, false) : 1;
+          cnb = (ci < a.num_seqs) ? seq_units<WIN>(a, ci, clen, crow, false) : 1;
         }
+        if constexpr (WIN) cw = window_units(a, max(clen, 0));
         if (ci + 1 < a.num_seqs) {
           nxt_len = __ldg(a.context_lens + ci + 1);
           nxt_row = a.seq_rows != nullptr ? __ldg(a.seq_rows + ci + 1) : ci + 1;
@@ -276,6 +316,7 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
   float o[NTILES][4];
   float m2[2] = {-INFINITY, -INFINITY}, lsum[2] = {0.f, 0.f};
   const float scale = a.scale;
+  const float zscale = a.scale * kLog2e;
   const uint64_t limit = a.wait_limit_ns != 0 ? a.wait_limit_ns : kWaitLimitNs;
   // After a wait gave up the warp walks the rest of its span without data: it
   // still parks (empty) portions, so the CTA merge and the per-segment counters
@@ -323,8 +364,7 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
       }
     }
     if (!dry) {
-      const int tok0 = mt.blk * kBS;
-      const int valid = min(kBS, mt.len - tok0);
+      const int valid = WIN ? kBS : min(kBS, mt.len - mt.blk * kBS);
       const uint32_t kbase = smem_u32(st);
       const uint32_t vbase = kbase + C::BLOCK_BYTES;
       float s[2][4];
@@ -350,8 +390,13 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int tok = 8 * j + 2 * t + (e & 1);
-          float v = round_bf16(round_bf16(s[j][e]) * scale) * kLog2e;
-          v = (tok < valid) ? v : -INFINITY;
+          float v;
+          if constexpr (WIN) {
+            v = ((mt.len >> tok) & 1) ? s[j][e] * zscale : -INFINITY;
+          } else {
+            v = round_bf16(round_bf16(s[j][e]) * scale) * kLog2e;
+            v = (tok < valid) ? v : -INFINITY;
+          }
           s[j][e] = v;
           mx[e >> 1] = fmaxf(mx[e >> 1], v);
         }
@@ -362,9 +407,12 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
         float m = mx[hr];
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const float mnew = fmaxf(m2[hr], m);
+        const float mtop = fmaxf(m2[hr], m);
+        // WIN: a unit in an invalid block shows no token, so the maximum may still
+        // be -inf (no -inf - -inf).
+        const float mnew = WIN && mtop == -INFINITY ? 0.f : mtop;
         corr[hr] = fast_exp2(m2[hr] - mnew);
-        m2[hr] = mnew;
+        m2[hr] = mtop;
         float ps = 0.f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -396,7 +444,16 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
         // 2t+8, 2t+9 (regs 1/3); zero the ones past the context (they may hold
         // stale or NaN data, and 0 * NaN would poison the sum).
         uint32_t keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;
-        if (valid < kBS) {
+        if constexpr (WIN) {
+          if (mt.len != 0xffff) {
+            auto pair = [&](int tok) {
+              return (((mt.len >> tok) & 1) ? 0x0000ffffu : 0u) |
+                     (((mt.len >> (tok + 1)) & 1) ? 0xffff0000u : 0u);
+            };
+            keep_lo = pair(2 * t);
+            keep_hi = pair(2 * t + 8);
+          }
+        } else if (valid < kBS) {
           keep_lo = ((2 * t < valid) ? 0x0000ffffu : 0u) | ((2 * t + 1 < valid) ? 0xffff0000u : 0u);
           keep_hi = ((2 * t + 8 < valid) ? 0x0000ffffu : 0u) |
                     ((2 * t + 9 < valid) ? 0xffff0000u : 0u);
@@ -583,13 +640,13 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
   }
 }
 
-template <int D, bool G16>
+template <int D, bool G16, bool WIN>
 int launch_one(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap& vmap, int grid,
                cudaStream_t stream) {
   using C = Cfg<D, G16>;
   static unsigned long long configured = 0;  // one bit per device
   cudaError_t e = once_per_device(&configured, [] {
-    return cudaFuncSetAttribute(decode_mma_kernel<D, G16>,
+    return cudaFuncSetAttribute(decode_mma_kernel<D, G16, WIN>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   });
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -603,7 +660,7 @@ int launch_one(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap& 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_mma_kernel<D, G16>, kmap, vmap, a));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_mma_kernel<D, G16, WIN>, kmap, vmap, a));
 }
 
 // Merges, after the decode kernel, the cut segments its CTAs listed: one CTA
@@ -620,14 +677,14 @@ __global__ void __launch_bounds__(128, 3) decode_merge_kernel(const DecodeArgs a
   cta_merge_records<__nv_bfloat16>(a, sp, t.seq, t.kvh, t.seg_unit, t.nb, merge_scratch);
 }
 
-template <int D, bool G16>
+template <int D, bool G16, bool WIN>
 int occupancy_one() {
   using C = Cfg<D, G16>;
-  cudaError_t e = cudaFuncSetAttribute(decode_mma_kernel<D, G16>,
+  cudaError_t e = cudaFuncSetAttribute(decode_mma_kernel<D, G16, WIN>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   if (e != cudaSuccess) return -static_cast<int>(e);
   int n = 0;
-  e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_mma_kernel<D, G16>, C::W * 32,
+  e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_mma_kernel<D, G16, WIN>, C::W * 32,
                                                     C::SMEM_BYTES);
   if (e != cudaSuccess) return -static_cast<int>(e);
   return n;
@@ -635,16 +692,19 @@ int occupancy_one() {
 
 }  // namespace
 
-int launch_decode_mma(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap& vmap,
-                      int grid, cudaStream_t stream) {
+namespace {
+
+template <bool WIN>
+int launch_both(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap& vmap, int grid,
+                cudaStream_t stream) {
   const bool g16 = a.groups > 8;
   int rc;
   if (a.head_dim == 64)
-    rc = g16 ? launch_one<64, true>(a, kmap, vmap, grid, stream)
-             : launch_one<64, false>(a, kmap, vmap, grid, stream);
+    rc = g16 ? launch_one<64, true, WIN>(a, kmap, vmap, grid, stream)
+             : launch_one<64, false, WIN>(a, kmap, vmap, grid, stream);
   else
-    rc = g16 ? launch_one<128, true>(a, kmap, vmap, grid, stream)
-             : launch_one<128, false>(a, kmap, vmap, grid, stream);
+    rc = g16 ? launch_one<128, true, WIN>(a, kmap, vmap, grid, stream)
+             : launch_one<128, false, WIN>(a, kmap, vmap, grid, stream);
   if (rc != 0 || a.tasks == nullptr) return rc;
   // Merge pass: at most `grid` records per segment.
   const int smem = static_cast<int>((2 * static_cast<int64_t>(grid) * a.groups + 2 * a.groups) *
@@ -674,10 +734,31 @@ int launch_decode_mma(const DecodeArgs& a, const CUtensorMap& kmap, const CUtens
   return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_merge_kernel, a));
 }
 
-int decode_mma_ctas_per_sm(int head_dim, int groups) {
+template <bool WIN>
+int ctas_per_sm(int head_dim, int groups) {
   const bool g16 = groups > 8;
-  if (head_dim == 64) return g16 ? occupancy_one<64, true>() : occupancy_one<64, false>();
-  return g16 ? occupancy_one<128, true>() : occupancy_one<128, false>();
+  if (head_dim == 64) return g16 ? occupancy_one<64, true, WIN>() : occupancy_one<64, false, WIN>();
+  return g16 ? occupancy_one<128, true, WIN>() : occupancy_one<128, false, WIN>();
+}
+
+}  // namespace
+
+int launch_decode_mma(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                      int grid, cudaStream_t stream) {
+  return launch_both<false>(a, kmap, vmap, grid, stream);
+}
+
+int decode_mma_ctas_per_sm(int head_dim, int groups) {
+  return ctas_per_sm<false>(head_dim, groups);
+}
+
+int launch_window_decode_mma(const DecodeArgs& a, const CUtensorMap& kmap,
+                             const CUtensorMap& vmap, int grid, cudaStream_t stream) {
+  return launch_both<true>(a, kmap, vmap, grid, stream);
+}
+
+int window_decode_mma_ctas_per_sm(int head_dim, int groups) {
+  return ctas_per_sm<true>(head_dim, groups);
 }
 
 }  // namespace bsb
