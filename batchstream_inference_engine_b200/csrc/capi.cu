@@ -1094,6 +1094,26 @@ int pool_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int64_t he
   return encode_pool_map(map, base, rows, head_dim);
 }
 
+// Tensor map of a query's [tokens, heads, head_dim] view (token stride in elements),
+// boxes of 64 dims, box_heads heads and box_tokens tokens: the packed query rows of
+// the sliding-window prefill.  128-byte swizzle.
+int query_tensor_map(CUtensorMap* map, const void* base, int64_t tokens, int64_t token_stride,
+                     int64_t heads, int64_t head_dim, int64_t box_heads, int64_t box_tokens) {
+  EncodeTiledFn fn = nullptr;
+  if (int rc = get_encode_fn(&fn)) return rc;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(heads),
+                        static_cast<cuuint64_t>(tokens)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_dim * 2),
+                           static_cast<cuuint64_t>(token_stride * 2)};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides,
+                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(BS_ERR_CUDA, "cuTensorMapEncodeTiled (packed query) failed (%d)", static_cast<int>(r));
+  return BS_OK;
+}
+
 int sm_count(int* sms) {
   DeviceInfo* d = nullptr;
   if (int rc = current_device_info(&d)) return rc;

@@ -25,6 +25,8 @@ void set_last_error(const char* message);
 void add_kernel_launches(int n);
 int sm_count(int* sms);
 int pool_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int64_t head_dim);
+int query_tensor_map(CUtensorMap* map, const void* base, int64_t tokens, int64_t token_stride,
+                     int64_t heads, int64_t head_dim, int64_t box_heads, int64_t box_tokens);
 int32_t decode_record_stride(int64_t groups, int64_t head_dim);
 int launch_rotary_append(const void* qkv, int64_t qkv_stride, bool bf16, const double* freq,
                          int32_t rotary_dim, bool interleaved, double amp, const int32_t* pos,
@@ -176,6 +178,42 @@ int plan_mma_decode(const WindowShape& s, MmaDecodePlan* p) {
   return BS_OK;
 }
 
+// How the tensor-core prefill runs a call: one CTA per pair of 128-row query tiles,
+// kv head and range of key steps.
+struct MmaChunkPlan {
+  int64_t tile_tokens, qtiles, items, splits, ml_offset, bytes;
+};
+
+constexpr int64_t kMaxRecordBytes = 64ll << 20;
+
+int plan_mma_chunks(const WindowShape& s, MmaChunkPlan* p) {
+  int sms = 0;
+  if (int rc = bsb::sm_count(&sms)) return rc;
+  const int64_t groups = s.heads / s.kv_heads;
+  p->tile_tokens = 2 * (bsb::kWindowPairRows / 2 / groups);
+  p->qtiles = (s.max_query_len + p->tile_tokens - 1) / p->tile_tokens;
+  p->items = product(product(s.rows, p->qtiles), s.kv_heads);
+  if (p->items < 0 || p->items > kInt32Max / bsb::kMaxWindowRanges / 8) {
+    return fail(BS_ERR_UNSUPPORTED, "too many query tiles");
+  }
+  // Pairs that can hold tokens (the others of a padded launch exit at once); one CTA
+  // runs per SM, so ranges are cut only as far as one wave of them goes.
+  const int64_t busy = std::max<int64_t>(
+      1, std::min(s.rows * p->qtiles,
+                  (s.tokens + p->tile_tokens - 1) / p->tile_tokens + s.rows) * s.kv_heads);
+  const int64_t keys = std::min(s.max_blocks * s.block_size,
+                                std::min(s.window, kMaxContext) + std::min(s.sinks, kMaxContext) +
+                                    p->tile_tokens + 32);
+  const int64_t most = (keys + 127) / 128 / bsb::kMinWindowSteps;
+  const int64_t record = bsb::kWindowPairRows * (s.head_dim + 2) * 4;
+  p->splits = std::max<int64_t>(
+      1, std::min(std::min<int64_t>(sms / busy, bsb::kMaxWindowRanges), most));
+  while (p->splits > 1 && p->items * p->splits * record > kMaxRecordBytes) --p->splits;
+  p->ml_offset = p->items * p->splits * bsb::kWindowPairRows * s.head_dim;
+  p->bytes = p->splits > 1 ? p->items * p->splits * record : 0;
+  return BS_OK;
+}
+
 // Scratch of a call: the largest of the kernels its shape may run on.
 int window_workspace(const WindowShape& s, uint64_t* bytes_out) {
   BS_CHECK(bytes_out != nullptr, "bytes_out is null");
@@ -183,7 +221,11 @@ int window_workspace(const WindowShape& s, uint64_t* bytes_out) {
   SimtPlan p;
   if (int rc = plan_simt(s, &p)) return rc;
   int64_t need = p.bytes;
-  if (mma_shape(s) && !s.chunks) {
+  if (mma_shape(s) && s.chunks) {
+    MmaChunkPlan m;
+    if (int rc = plan_mma_chunks(s, &m)) return rc;
+    need = std::max(need, m.bytes);
+  } else if (mma_shape(s)) {
     MmaDecodePlan m;
     if (int rc = plan_mma_decode(s, &m)) return rc;
     need = std::max(need, m.bytes);
@@ -273,6 +315,31 @@ int run_mma_decode(const WindowShape& s, const WindowCall& c) {
   return BS_OK;
 }
 
+int run_mma_chunks(const WindowShape& s, const WindowCall& c, bsb::WindowArgs& a) {
+  MmaChunkPlan p;
+  if (int rc = plan_mma_chunks(s, &p)) return rc;
+  if (int rc = check_workspace(c, p.bytes)) return rc;
+  CUtensorMap qmap, kmap, vmap;
+  const int64_t rows = s.kv_heads * c.num_blocks * s.block_size;
+  const int64_t groups = s.heads / s.kv_heads;
+  if (int rc = bsb::query_tensor_map(&qmap, c.query, s.tokens, c.q_stride, s.heads, s.head_dim,
+                                     groups, p.tile_tokens / 2)) {
+    return rc;
+  }
+  if (int rc = bsb::pool_tensor_map(&kmap, c.key_pool, rows, s.head_dim)) return rc;
+  if (int rc = bsb::pool_tensor_map(&vmap, c.value_pool, rows, s.head_dim)) return rc;
+  a.tile_tokens = static_cast<int32_t>(p.tile_tokens);
+  a.qtiles = static_cast<int32_t>(p.qtiles);
+  a.splits = static_cast<int32_t>(p.splits);
+  a.records = static_cast<float*>(c.workspace);
+  a.rec_stride_ml = p.ml_offset;
+  const int rc = bsb::launch_window_prefill(a, qmap, kmap, vmap,
+                                            static_cast<cudaStream_t>(c.stream));
+  if (rc != 0) return cuda_fail(rc, "window prefill launch");
+  bsb::add_kernel_launches(p.splits > 1 ? 2 : 1);
+  return BS_OK;
+}
+
 int run_window(const WindowShape& s, const WindowCall& c) {
   if (int rc = check_window_shape(s)) return rc;
   BS_CHECK(s.max_blocks <= c.table_stride, "max_blocks_per_seq must be in [1, table_stride]");
@@ -289,7 +356,8 @@ int run_window(const WindowShape& s, const WindowCall& c) {
   BS_CHECK(c.query && c.key_pool && c.value_pool && c.block_tables && c.context_lens &&
                c.output && (!s.chunks || c.cu_q),
            "null pointer argument");
-  if (mma_shape(s) && !s.chunks && mma_pointers(c)) return run_mma_decode(s, c);
+  const bool mma = mma_shape(s) && mma_pointers(c);
+  if (mma && !s.chunks) return run_mma_decode(s, c);
   bsb::WindowArgs a{};
   a.q = c.query;
   a.q_stride = c.q_stride;
@@ -317,6 +385,9 @@ int run_window(const WindowShape& s, const WindowCall& c) {
   a.sinks = static_cast<int32_t>(std::min(s.sinks, kMaxContext));
   a.scale = static_cast<float>(c.scaling);
   a.status = c.status;
+  // The tensor-core prefill compares scores before it scales them: it needs a
+  // magnitude to scale by.
+  if (mma && a.scale != 0.f && std::isfinite(a.scale)) return run_mma_chunks(s, c, a);
 
   SimtPlan p;
   if (int rc = plan_simt(s, &p)) return rc;

@@ -41,6 +41,9 @@ struct WindowArgs {
   int32_t splits;
   float* records;
   int32_t rec_stride;
+  // Tensor-core chunks: the (maximum, sum) pairs of every record row start this
+  // many floats after the O rows.
+  int64_t rec_stride_ml;
   uint32_t* status;
 };
 
@@ -103,6 +106,14 @@ __host__ __device__ __forceinline__ int32_t window_range(int32_t count, int32_t 
 // Query rows (tokens x heads of one kv head) of a tile of the CUDA-core kernel.
 constexpr int kWindowSimtRows = 16;
 
+// Tensor-core chunks: rows of a record (two query tiles), the fewest steps of 128
+// keys in a range and the most ranges.
+constexpr int kWindowPairRows = 256;
+constexpr int kMinWindowSteps = 2;
+constexpr int kMaxWindowRanges = 8;
+
+int launch_window_prefill(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& kmap,
+                          const CUtensorMap& vmap, cudaStream_t stream);
 int launch_window_simt(const WindowArgs& a, bool bf16, bool vec, cudaStream_t stream);
 
 }  // namespace bsb

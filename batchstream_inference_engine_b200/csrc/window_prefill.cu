@@ -1,0 +1,691 @@
+// Sliding-window paged attention of prompt chunks on the 5th-generation tensor
+// cores (tcgen05 + TMEM): bf16, head_dim 64 or 128, block sizes that are multiples
+// of 16, up to 16 query heads per kv head.
+//
+// Query rows are packed: a tile's 128 rows are 128 / G consecutive tokens times the
+// G query heads of one kv head, so every K and V row that a CTA loads serves the
+// whole group, and the keys a tile reads beyond its window are those of a few
+// tokens (18 at G = 7) instead of 128.  One CTA takes two such tiles (A and B, the
+// tokens next to each other) over the same keys, in steps of 128 keys.
+//
+// The keys a CTA reads are 16-token units: the sink units, then the window's from
+// the first token any row sees to the last row's own.  A step is 8 units, each one
+// TMA box per K, V and 64 dims through the block table, so sink units and window
+// units share a step and nothing between them is touched.
+//
+// Roles (11 warps, one CTA per SM):
+//   * softmax A (warps 0-3) and B (warps 4-7), one thread per query row: S from
+//     TMEM, mask on border steps only, base-2 online softmax in fp32 whose maximum
+//     moves only when it grows by more than 2^8 (then O is rescaled in TMEM), P
+//     rounded to bf16 (the tensor cores' input) over the first half of S's columns;
+//   * MMA (warp 8, one thread): per step, for A then B: O += P V of the step before
+//     (P from TMEM), S = Q K^T of this one over P's columns (the products of one
+//     thread execute in order), one commit.  While one tile's softmax runs, the
+//     tensor core works for the other;
+//   * loader (warp 9);
+//   * guard (warp 10): on border steps it zeroes the V rows that no row of the CTA
+//     sees (never-loaded or stale memory, which 0 * NaN would let through), and the
+//     non-finite elements of the others, whose keys it lists: rows that do see such a
+//     key get its non-finite values added at the end, rows that do not stay clean.
+//
+// Bound: the exponentials (16 a clock and SM against 8192 tensor FLOP: a step of
+// 2 x 128 x 128 scores costs 2048 clocks of the special-function units, the
+// products 1024 at head_dim 64 and 2048 at 128).
+//
+// A call with fewer CTAs than SMs cuts each tile pair's steps into ranges, whose
+// records window_prefill_merge_kernel joins in range order.
+//
+// Waits are bounded and their outcome made warp-uniform before warp-collective
+// instructions; the loader and the MMA warp drain what they started before TMEM is
+// freed, also on the error path.
+#include "tcgen05.cuh"
+#include "window.cuh"
+
+namespace bsb {
+namespace {
+
+constexpr int kRows = 128;  // query rows of a tile (TMEM lanes)
+constexpr int kKeys = 128;  // keys of a step
+constexpr int kUnit = 16;   // tokens per unit (one TMA box)
+constexpr int kUnits = kKeys / kUnit;
+constexpr int kThreads = 352;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kGuardWarp = 10;
+constexpr int kRing = 4;  // step barriers per tile (> K stages, > V stages + 1)
+constexpr uint32_t kTmemCols = 512;  // S/P of A, S/P of B, O of A, O of B
+constexpr float kLog2eP = 1.4426950408889634f;
+constexpr float kRescaleSlack = 8.f;
+constexpr int kMaxBad = 64;  // listed keys with non-finite V (more: all are looked at)
+
+template <int D>
+struct Cfg {
+  static constexpr int HALVES = D / 64;
+  static constexpr int KS = D == 64 ? 4 : 3;  // K stages
+  static constexpr int VS = D == 64 ? 3 : 2;  // V stages
+  static constexpr int HALF_BYTES = kKeys * 128;  // 64 dims of 128 rows
+  static constexpr int TILE_BYTES = HALVES * HALF_BYTES;
+  static constexpr int SMEM_BYTES = 1024 + (2 + KS + VS) * TILE_BYTES;
+  static constexpr uint32_t O_COL = 256;
+  static_assert(KS <= kRing && VS + 1 <= kRing, "a step waiter could fall a whole ring behind");
+};
+
+// The steps of a CTA's key range and which of them each tile needs.
+struct Steps {
+  int32_t sink_units, first_unit, units;
+  int32_t pos0[2], pos1[2];  // first and last position of the tiles' tokens
+  int32_t last[2], first[2];  // their last and first step with window keys
+  int32_t tiles;             // tiles with tokens (1 or 2)
+};
+
+__device__ __forceinline__ Steps steps_of(const WindowArgs& a, const WindowTile& w, int32_t tt) {
+  Steps s;
+  s.first_unit = w.lo / kUnit;
+  s.sink_units = min((a.sinks + kUnit - 1) / kUnit, s.first_unit);
+  const int32_t end = w.pos0 + w.ntok - 1;
+  s.units = s.sink_units + end / kUnit - s.first_unit + 1;
+  s.tiles = w.ntok > tt ? 2 : 1;
+  s.pos0[0] = w.pos0;
+  s.pos1[0] = min(end, w.pos0 + tt - 1);
+  s.pos0[1] = w.pos0 + tt;
+  s.pos1[1] = end;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int32_t lo = max(0, s.pos0[x] - a.window + 1);
+    s.first[x] = (s.sink_units + lo / kUnit - s.first_unit) / kUnits;
+    s.last[x] = (s.sink_units + s.pos1[x] / kUnit - s.first_unit) / kUnits;
+  }
+  return s;
+}
+
+__device__ __forceinline__ int32_t step_count(const Steps& s) {
+  return (s.units + kUnits - 1) / kUnits;
+}
+
+// First position of unit x of the range.
+__device__ __forceinline__ int32_t unit_pos(const Steps& s, int32_t x) {
+  return (x < s.sink_units ? x : x - s.sink_units + s.first_unit) * kUnit;
+}
+
+// Whether tile x has keys in step j.
+__device__ __forceinline__ bool step_active(const Steps& s, int x, int32_t j) {
+  return x < s.tiles && j <= s.last[x] && (j >= s.first[x] || j * kUnits < s.sink_units);
+}
+
+// Whether some row of tile x does not see some key of step j.
+__device__ __forceinline__ bool step_masked(const WindowArgs& a, const Steps& s, int x,
+                                            int32_t j) {
+  const int32_t u0 = j * kUnits, u1 = u0 + kUnits - 1;
+  if (u1 >= s.units || unit_pos(s, u1) + kUnit - 1 > s.pos0[x]) return true;
+  if (u0 < s.sink_units && a.sinks < min(u1 + 1, s.sink_units) * kUnit) return true;
+  // The step's first window unit against the last row's window.
+  return u1 >= s.sink_units && unit_pos(s, max(u0, s.sink_units)) <= s.pos1[x] - a.window;
+}
+
+__device__ __forceinline__ bool sees(const WindowArgs& a, int32_t qpos, int32_t pos) {
+  return pos <= qpos && (pos < a.sinks || pos > qpos - a.window);
+}
+
+// Ranges a tile pair with `steps` steps is cut into.
+__device__ __forceinline__ int32_t step_ranges(int32_t steps, int32_t splits) {
+  const int32_t most = (steps + kMinWindowSteps - 1) / kMinWindowSteps;
+  return most < splits ? most : splits;
+}
+
+// Linear item -> (sequence, tile pair, kv head): a chunk's last tiles, which see the
+// most keys, come first.
+__device__ __forceinline__ void pair_of(const WindowArgs& a, int32_t item, int32_t& r,
+                                        int32_t& tile, int32_t& h) {
+  h = item % a.num_kv_heads;
+  item /= a.num_kv_heads;
+  r = item % a.num_rows;
+  tile = a.qtiles - 1 - item / a.num_rows;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    window_prefill_kernel(const __grid_constant__ CUtensorMap qmap,
+                          const __grid_constant__ CUtensorMap kmap,
+                          const __grid_constant__ CUtensorMap vmap, const WindowArgs a) {
+  using C = Cfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t q_full, k_full[C::KS], v_full[C::VS], v_ok[C::VS], step_done[2][kRing],
+      p_full[2], mma_done;
+  __shared__ uint32_t tmem_base;
+  __shared__ int32_t bad_count, bad_pos[kMaxBad];
+
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  auto sQ = [&](int x) { return smem + x * C::TILE_BYTES; };
+  auto sK = [&](int st) { return smem + (2 + st) * C::TILE_BYTES; };
+  auto sV = [&](int st) { return smem + (2 + C::KS + st) * C::TILE_BYTES; };
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  pdl_wait();
+  const int32_t tt = a.tile_tokens / 2;  // tokens of one tile
+  const int32_t split = blockIdx.x % a.splits;
+  const int32_t item = blockIdx.x / a.splits;
+  int32_t r, tile, h;
+  pair_of(a, item, r, tile, h);
+  WindowTile w;
+  if (!window_tile(a, r, tile, w, tid == 0 && tile == 0 && h == 0 && split == 0)) return;
+  const Steps sd = steps_of(a, w, tt);
+  const int32_t all = step_count(sd);
+  const int32_t ranges = step_ranges(all, a.splits);
+  if (split >= ranges) return;
+  const int32_t j0 = split * all / ranges;
+  const int32_t n = (split + 1) * all / ranges - j0;  // steps of this CTA
+
+  if (tid == 0) {
+    mbar_init(&q_full, 1);
+    for (int s = 0; s < C::KS; ++s) mbar_init(&k_full[s], 1);
+    for (int s = 0; s < C::VS; ++s) {
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_ok[s], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      for (int s = 0; s < kRing; ++s) mbar_init(&step_done[x][s], 1);
+      mbar_init(&p_full[x], kRows);
+    }
+    mbar_init(&mma_done, 1);
+    fence_barrier_init();
+    bad_count = 0;
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tmem_base)),
+                 "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+
+  auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
+  };
+  // Step u of tile x is done: P V of step u - 1 and S of step u.  Waiters take the
+  // steps in order and are never kRing behind (see the ring sizes).
+  auto wait_step = [&](int x, int u) {
+    return wait_all(&step_done[x][u % kRing], (u / kRing) & 1);
+  };
+
+  if (warp == kLoadWarp) {
+    // ---------------------------------------------------------------- loader
+    const int32_t* table = a.block_tables + static_cast<int64_t>(w.row) * a.bt_stride;
+    const int32_t block_units = a.block_size / kUnit;
+    const int unit = lane & (kUnits - 1), half = lane >> 3;  // this lane's box of a step
+    // Pool row of this lane's unit of step j (-1: past the range or invalid).
+    auto fetch = [&](int32_t j) -> int32_t {
+      const int32_t x = (j0 + j) * kUnits + unit;
+      if (j >= n || x >= sd.units) return -1;
+      const int32_t tu = unit_pos(sd, x) / kUnit;
+      const int32_t ent = tu / block_units;
+      const int32_t blk = __ldg(table + ent);
+      if (blk < 0 || blk >= a.num_blocks) {
+        if (half == 0) set_status(a.status, kStatusBadBlock);
+        return -1;
+      }
+      return (h * a.num_blocks + blk) * a.block_size + (tu - ent * block_units) * kUnit;
+    };
+    int32_t y = fetch(0), y_next = fetch(1);
+    if (lane == 0) {
+      const uint32_t rows = static_cast<uint32_t>(tt * a.groups);
+      mbar_arrive_expect_tx(&q_full, sd.tiles * C::HALVES * rows * 128u);
+      for (int x = 0; x < sd.tiles; ++x) {
+        for (int hf = 0; hf < C::HALVES; ++hf) {
+          tma_load_3d(sQ(x) + hf * C::HALF_BYTES, &qmap, &q_full, hf * 64, h * a.groups,
+                      w.tok0 + x * tt);
+        }
+      }
+    }
+    __syncwarp();
+    auto load = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* full, int32_t row) {
+      const bool mine = row >= 0 && half < C::HALVES;
+      const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
+      if (lane == 0) mbar_arrive_expect_tx(full, boxes * 2048u);
+      __syncwarp();
+      if (mine) {
+        tma_load_2d(dst + half * C::HALF_BYTES + unit * 2048, map, full, half * 64, row);
+      }
+    };
+    bool ok = true;
+    int32_t k_loads = 0, v_loads = 0;
+    for (int32_t j = 0; j < n; ++j) {
+      // Step j - KS has read the K stage, step j - VS + 1 the V stage (of both tiles:
+      // B's commit follows A's products).
+      if (j >= C::KS) ok = wait_step(1, j - C::KS);
+      if (!ok) break;
+      load(&kmap, sK(j % C::KS), &k_full[j % C::KS], y);
+      k_loads = j + 1;
+      if (j >= C::VS) ok = wait_step(1, j - C::VS + 1);
+      if (!ok) break;
+      load(&vmap, sV(j % C::VS), &v_full[j % C::VS], y);
+      v_loads = j + 1;
+      y = y_next;
+      y_next = fetch(j + 2);
+    }
+    // Drain: every load has landed before the CTA leaves its shared memory.
+    bool drained = wait_all(&q_full, 0);
+    for (int32_t j = max(0, k_loads - C::KS); j < k_loads; ++j) {
+      drained = wait_all(&k_full[j % C::KS], (j / C::KS) & 1) && drained;
+    }
+    for (int32_t j = max(0, v_loads - C::VS); j < v_loads; ++j) {
+      drained = wait_all(&v_full[j % C::VS], (j / C::VS) & 1) && drained;
+    }
+    if ((!ok || !drained) && lane == 0) set_status(a.status, kStatusWaitTimeout);
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------------- MMA issuer
+    constexpr uint32_t kIdescS = umma_idesc(128, kKeys, 0, 0);
+    constexpr uint32_t kIdescO = umma_idesc(128, D, 0, 1);
+    constexpr uint64_t kTileStep = C::TILE_BYTES >> 4, kHalfStep = C::HALF_BYTES >> 4;
+    const uint64_t desc_q = umma_desc(smem_u32(sQ(0)), 16, 1024);
+    const uint64_t desc_k = umma_desc(smem_u32(sK(0)), 16, 1024);
+    // V: dims contiguous (MN-major): 64-dim halves HALF_BYTES apart, 8 keys 1024.
+    const uint64_t desc_v = umma_desc(smem_u32(sV(0)), C::HALF_BYTES, 1024);
+    bool ok = wait_all(&q_full, 0);
+    int32_t done[2] = {0, 0};  // P tiles consumed, by tile
+    for (int32_t u = 0; u <= n && ok; ++u) {
+      for (int x = 0; x < 2 && ok; ++x) {
+        const bool pv = u > 0 && step_active(sd, x, j0 + u - 1);
+        const bool qk = u < n && step_active(sd, x, j0 + u);
+        const int32_t vs = (u - 1) % C::VS, ks = u % C::KS;
+        if (pv) {
+          ok = wait_all(&p_full[x], done[x] & 1) &&
+               wait_all(&v_ok[vs], ((u - 1) / C::VS) & 1);
+        }
+        if (ok && qk) ok = wait_all(&k_full[ks], (u / C::KS) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t s_col = tmem + x * kKeys;
+          if (pv) {
+            const uint64_t v0 = desc_v + vs * kTileStep;
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k) {
+              umma_f16_ts(tmem + C::O_COL + x * D, s_col + 8 * k, v0 + 128 * k, kIdescO,
+                          (done[x] > 0 || k > 0) ? 1u : 0u);
+            }
+          }
+          if (qk) {
+            const uint64_t q0 = desc_q + x * kTileStep, k0 = desc_k + ks * kTileStep;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint64_t off = (k / 4) * kHalfStep + 2 * (k % 4);
+              umma_f16(s_col, q0 + off, k0 + off, kIdescS, k > 0 ? 1u : 0u);
+            }
+          }
+          umma_commit(&step_done[x][u % kRing]);
+        }
+        if (pv) ++done[x];
+        __syncwarp();
+      }
+    }
+    if (lane == 0) umma_commit(&mma_done);
+    __syncwarp();
+    const bool drained = wait_all(&mma_done, 0);
+    if ((!ok || !drained) && lane == 0) set_status(a.status, kStatusWaitTimeout);
+  } else if (warp == kGuardWarp) {
+    // ---------------------------------------------------------------- guard
+    const int32_t end = w.pos0 + w.ntok - 1;
+    bool ok = true;
+    for (int32_t j = 0; j < n; ++j) {
+      const int vs = j % C::VS;
+      ok = wait_all(&v_full[vs], (j / C::VS) & 1);
+      if (!ok) break;
+      bool border = false;
+      for (int x = 0; x < sd.tiles; ++x) {
+        border |= step_active(sd, x, j0 + j) && step_masked(a, sd, x, j0 + j);
+      }
+      if (border) {
+        // Lane = (row of a group of 4, 16-byte column of a 128-byte row).
+        for (int g = 0; g < kKeys / 4; ++g) {
+          const int row = g * 4 + (lane >> 3), col = lane & 7;
+          const int32_t x = (j0 + j) * kUnits + row / kUnit;
+          const int32_t pos = unit_pos(sd, x) + row % kUnit;
+          const bool live = x < sd.units && pos <= end && (pos < a.sinks || pos >= w.lo);
+          bool bad = false;
+#pragma unroll
+          for (int hf = 0; hf < C::HALVES; ++hf) {
+            uint4* p = reinterpret_cast<uint4*>(sV(vs) + hf * C::HALF_BYTES + row * 128 + col * 16);
+            if (!live) {
+              *p = make_uint4(0u, 0u, 0u, 0u);
+              continue;
+            }
+            uint4 v = *p;
+            uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+            bool hit = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              // All exponent bits set: infinity or NaN.
+              uint32_t keep = 0xffffffffu;
+              if ((e[i] & 0x7f80u) == 0x7f80u) keep &= 0xffff0000u;
+              if ((e[i] & 0x7f800000u) == 0x7f800000u) keep &= 0x0000ffffu;
+              hit |= keep != 0xffffffffu;
+              e[i] &= keep;
+            }
+            if (hit) *p = v;
+            bad |= hit;
+          }
+          const uint32_t any = __ballot_sync(0xffffffffu, bad);
+          if (any != 0 && col == 0 && ((any >> (lane & ~7)) & 0xffu) != 0) {
+            const int32_t at = atomicAdd(&bad_count, 1);
+            if (at < kMaxBad) bad_pos[at] = pos;
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_ok[vs]);
+      __syncwarp();
+    }
+    if (!ok && lane == 0) set_status(a.status, kStatusWaitTimeout);
+  } else {
+    // ---------------------------------------------------------------- softmax
+    const int x = warp >> 2;
+    const int row = tid & (kRows - 1);
+    const int32_t tok = row / a.groups, g = row - tok * a.groups;
+    const bool live = x * tt + tok < w.ntok && tok < tt;
+    const int32_t qpos = w.pos0 + x * tt + tok;
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lane_base + x * kKeys;
+    const uint32_t o_addr = tmem + lane_base + C::O_COL + x * D;
+    const float zscale = fabsf(a.scale) * kLog2eP;
+    float m_used = -INFINITY, l_run = 0.f;
+    int32_t done = 0;
+    bool ok = true;
+    for (int32_t u = 0; u < n; ++u) {
+      ok = wait_step(x, u);
+      if (!ok) break;
+      if (!step_active(sd, x, j0 + u)) continue;
+      tc_fence_after();
+      // Visible tokens of the step's units, 16 bits each (border steps only).
+      const bool border = step_masked(a, sd, x, j0 + u);
+      uint32_t maps[kUnits / 2];
+      if (border) {
+        auto below = [](int32_t c) -> uint32_t {  // map of the first c tokens
+          return c >= kUnit ? 0xffffu : c <= 0 ? 0u : (1u << c) - 1u;
+        };
+#pragma unroll
+        for (int un = 0; un < kUnits; ++un) {
+          const int32_t ux = (j0 + u) * kUnits + un;
+          const int32_t p0 = unit_pos(sd, ux);
+          uint32_t map = below(qpos - p0 + 1) &
+                         (~below(qpos - a.window + 1 - p0) | below(a.sinks - p0));
+          if (ux >= sd.units || !live) map = 0;
+          maps[un / 2] = un % 2 ? maps[un / 2] | (map << 16) : map;
+        }
+      }
+      // Scores of columns 32 c .. 32 c + 31: a negative scale turns them around (the
+      // rest works with its magnitude), unseen keys become -inf.
+      auto scores = [&](int c, uint32_t (&v)[32]) {
+        if (a.scale < 0.f) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] ^= 0x80000000u;
+        }
+        if (border) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (!((maps[c] >> i) & 1u)) v[i] = 0xff800000u;
+          }
+        }
+      };
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      auto maximum = [&](const uint32_t (&v)[32]) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i]));
+      };
+      // 128 scores, their map and the packed P do not fit in the 168 registers a
+      // thread has: columns 0 .. 63 are read for the maximum, then again.
+      uint32_t v0[32], v1[32];
+      tmem_ld32(s_addr, v0);
+      tmem_ld32(s_addr + 32, v1);
+      tmem_wait_ld();
+      scores(0, v0);
+      maximum(v0);
+      scores(1, v1);
+      maximum(v1);
+      tmem_ld32(s_addr + 64, v0);
+      tmem_ld32(s_addr + 96, v1);
+      tmem_wait_ld();
+      scores(2, v0);
+      maximum(v0);
+      scores(3, v1);
+      maximum(v1);
+      const float m_step = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * zscale;
+      const bool grow = live && m_step > m_used + kRescaleSlack;
+      if (done == 0) {
+        m_used = m_step;
+      } else if (__any_sync(0xffffffffu, grow)) {
+        // P V of the step before is done (wait_step), so O may be rescaled; rows
+        // that did not grow keep theirs (factor 1).
+        const float m_new = grow ? m_step : m_used;
+        const float corr = grow ? fast_exp2(m_used - m_new) : 1.f;
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + c0, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
+          tmem_st32(o_addr + c0, o);
+        }
+        l_run *= corr;
+        m_used = m_new;
+      }
+      const float m_base = m_used == -INFINITY ? 0.f : m_used;  // no -inf - -inf
+      const float2 zs2 = make_float2(zscale, zscale), mm = make_float2(-m_base, -m_base);
+      float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
+                       make_float2(0.f, 0.f)};
+      // Probabilities of 32 columns, packed into 16.
+      auto weights = [&](const uint32_t (&v)[32], uint32_t* p) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 e = __ffma2_rn(
+              make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), zs2, mm);
+          const float2 pe = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+          sum[i & 3] = __fadd2_rn(sum[i & 3], pe);
+          p[i] = pack_bf16x2(pe.x, pe.y);
+        }
+      };
+      uint32_t p[32];
+      weights(v0, p);
+      weights(v1, p + 16);
+      tmem_ld32(s_addr, v0);
+      tmem_ld32(s_addr + 32, v1);
+      tmem_wait_ld();  // before P takes the place of columns 32 .. 63
+      tmem_st32(s_addr + 32, p);
+      scores(0, v0);
+      scores(1, v1);
+      weights(v0, p);
+      weights(v1, p + 16);
+      tmem_st32(s_addr, p);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[x]);
+      l_run += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) +
+               ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
+      ++done;
+    }
+    if (ok) ok = wait_step(x, n);  // the last P V is done
+    if (!ok) {
+      if (lane == 0) set_status(a.status, kStatusWaitTimeout);
+    } else if (x < sd.tiles) {
+      tc_fence_after();
+      const bool split_up = ranges > 1;
+      // Listed keys are complete: the guard arrived for every V that was used.
+      const int32_t bad = bad_count;
+      const float scale = split_up || done == 0 ? 1.f : 1.f / l_run;
+      const int32_t* table = a.block_tables + static_cast<int64_t>(w.row) * a.bt_stride;
+      const int64_t rec_row = (static_cast<int64_t>(item) * a.splits + split) * 2 * kRows +
+                              x * kRows + row;
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t v[32];
+        if (done > 0) {
+          tmem_ld32(o_addr + c0, v);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) v[c] = 0u;
+        }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * scale);
+        if (bad > 0 && live) {
+          const int32_t count = bad <= kMaxBad ? bad : n * kKeys;
+          for (int32_t b = 0; b < count; ++b) {
+            int32_t pos;
+            if (bad <= kMaxBad) {
+              pos = bad_pos[b];
+            } else {
+              const int32_t ux = j0 * kUnits + b / kUnit;
+              if (ux >= sd.units) break;
+              pos = unit_pos(sd, ux) + b % kUnit;
+            }
+            if (!sees(a, qpos, pos)) continue;
+            const int32_t blk = __ldg(table + pos / a.block_size);
+            if (blk < 0 || blk >= a.num_blocks) continue;
+            const __nv_bfloat16* src =
+                static_cast<const __nv_bfloat16*>(a.v_pool) +
+                ((static_cast<int64_t>(h) * a.num_blocks + blk) * a.block_size +
+                 pos % a.block_size) * D + c0;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              const float e = __bfloat162float(src[c]);
+              if (!isfinite(e)) v[c] = __float_as_uint(__uint_as_float(v[c]) + e);
+            }
+          }
+        }
+        if (!live) continue;
+        if (split_up) {
+          float* dst = a.records + rec_row * D + c0;
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            *reinterpret_cast<uint4*>(dst + c) = make_uint4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+          }
+        } else {
+          __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) +
+                               static_cast<int64_t>(w.tok0 + x * tt + tok) * a.o_stride +
+                               static_cast<int64_t>(h * a.groups + g) * D + c0;
+#pragma unroll
+          for (int c = 0; c < 32; c += 8) {
+            uint4 o;
+            o.x = pack_bf16x2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+            o.y = pack_bf16x2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
+            o.z = pack_bf16x2(__uint_as_float(v[c + 4]), __uint_as_float(v[c + 5]));
+            o.w = pack_bf16x2(__uint_as_float(v[c + 6]), __uint_as_float(v[c + 7]));
+            *reinterpret_cast<uint4*>(dst + c) = o;
+          }
+        }
+      }
+      if (split_up && live) {
+        float* ml = a.records + a.rec_stride_ml + rec_row * 2;
+        *reinterpret_cast<float2*>(ml) = make_float2(m_used, l_run);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(kTmemCols));
+  }
+}
+
+// Joins the records of a tile pair's step ranges, in range order: eight threads a
+// row, D / 8 columns each.
+constexpr int kMergeThreads = 256;
+constexpr int kMergeRows = kMergeThreads / 8;
+
+template <int D>
+__global__ void __launch_bounds__(kMergeThreads) window_prefill_merge_kernel(const WindowArgs a) {
+  pdl_wait();
+  constexpr int kParts = 2 * kRows / kMergeRows;  // CTAs per tile pair
+  const int32_t item = blockIdx.x / kParts;
+  int32_t r, tile, h;
+  pair_of(a, item, r, tile, h);
+  WindowTile w;
+  if (!window_tile(a, r, tile, w, false)) return;
+  const int32_t tt = a.tile_tokens / 2;
+  const int32_t prow = (blockIdx.x % kParts) * kMergeRows + threadIdx.x / 8;
+  const int32_t x = prow / kRows, row = prow % kRows;
+  const int32_t tok = row / a.groups, g = row - tok * a.groups;
+  if (tok >= tt || x * tt + tok >= w.ntok) return;
+  const Steps sd = steps_of(a, w, tt);
+  const int32_t ranges = step_ranges(step_count(sd), a.splits);
+  if (ranges <= 1) return;  // written by the kernel itself
+  const int32_t c = (threadIdx.x % 8) * (D / 8);
+  const int64_t rec0 = static_cast<int64_t>(item) * a.splits * 2 * kRows + prow;
+  const float* ml = a.records + a.rec_stride_ml;
+  float M = -INFINITY;
+  for (int32_t s = 0; s < ranges; ++s) M = fmaxf(M, ml[(rec0 + s * 2 * kRows) * 2]);
+  float L = 0.f, acc[D / 8];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) acc[i] = 0.f;
+#pragma unroll 4
+  for (int32_t s = 0; s < ranges; ++s) {
+    const float2 p = *reinterpret_cast<const float2*>(ml + (rec0 + s * 2 * kRows) * 2);
+    if (p.x == -INFINITY) continue;  // no key of this row in the range
+    const float f = fast_exp2(p.x - M);
+    L += f * p.y;
+    const float4* o = reinterpret_cast<const float4*>(a.records + (rec0 + s * 2 * kRows) * D + c);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const float4 v = o[i];
+      acc[4 * i] += f * v.x;
+      acc[4 * i + 1] += f * v.y;
+      acc[4 * i + 2] += f * v.z;
+      acc[4 * i + 3] += f * v.w;
+    }
+  }
+  const float inv = 1.f / L;
+  __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) +
+                       static_cast<int64_t>(w.tok0 + x * tt + tok) * a.o_stride +
+                       static_cast<int64_t>(h * a.groups + g) * D + c;
+#pragma unroll
+  for (int i = 0; i < D / 8; i += 8) {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = acc[i + k] * inv;
+    store8(dst + i, v);
+  }
+}
+
+template <int D>
+int launch_d(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& kmap,
+             const CUtensorMap& vmap, cudaStream_t stream) {
+  using C = Cfg<D>;
+  static unsigned long long configured = 0;  // one bit per device
+  cudaError_t e = once_per_device(&configured, [] {
+    return cudaFuncSetAttribute(window_prefill_kernel<D>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+  });
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const int64_t items = static_cast<int64_t>(a.num_rows) * a.qtiles * a.num_kv_heads;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(items * a.splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, window_prefill_kernel<D>, qmap, kmap, vmap, a);
+  if (e != cudaSuccess || a.splits == 1) return static_cast<int>(e);
+  cfg.gridDim = dim3(static_cast<unsigned>(items * (2 * kRows / kMergeRows)));
+  cfg.blockDim = dim3(kMergeThreads);
+  cfg.dynamicSmemBytes = 0;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, window_prefill_merge_kernel<D>, a));
+}
+
+}  // namespace
+
+int launch_window_prefill(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& kmap,
+                          const CUtensorMap& vmap, cudaStream_t stream) {
+  return a.head_dim == 64 ? launch_d<64>(a, qmap, kmap, vmap, stream)
+                          : launch_d<128>(a, qmap, kmap, vmap, stream);
+}
+
+}  // namespace bsb

@@ -654,6 +654,10 @@ def prefill_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: t
 
 
 # ------------------------------------------------------------------ bounded caches
+#
+# These calls last microseconds on the device, so their host side counts: the
+# workspace size of a shape is asked for once, the stream comes as its raw handle,
+# and the device is switched only when it is not the current one.
 
 
 def _int32_list(name: str, t: torch.Tensor, count: int) -> torch.Tensor:
@@ -665,30 +669,68 @@ def _int32_list(name: str, t: torch.Tensor, count: int) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+_null_context = _NullContext()
+
+
+def _on(device: torch.device):
+    """Context in which `device` is current."""
+    if torch.cuda.current_device() == device.index:
+        return _null_context
+    return torch.cuda.device(device)
+
+
+def _stream_and_status(device: torch.device) -> tuple[int, int]:
+    """The current stream of `device` and the address of its status word."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    return stream, _workspaces.get(device, stream, 0).data_ptr()
+
+
+_window_ws_bytes: dict[tuple, int] = {}
+
+
+def _window_scratch(query_fn, device: torch.device, sizes: tuple) -> torch.Tensor | None:
+    """Scratch of one window attention call, from the stream-ordered allocator
+    (inside a capture: from the graph's own pool, so two graphs never share it)."""
+    key = (query_fn, device.index, sizes)
+    need = _window_ws_bytes.get(key)
+    if need is None:
+        got = ctypes.c_uint64(0)
+        check(getattr(lib(), query_fn)(*sizes, ctypes.byref(got)))
+        need = _window_ws_bytes[key] = got.value
+    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+
+
 def _window_inputs(name: str, query, key_pool, value_pool, block_tables, out, max_blocks_per_seq):
     """The checks that both window attentions share; returns query, block_tables,
     out and max_blocks as the C call takes them."""
     if query.dim() != 3 or key_pool.dim() != 4 or value_pool.shape != key_pool.shape:
         raise RuntimeError(f"{name}: query must be [T, H, D] and the pools [Hkv, NB, bs, D]")
-    if query.dtype != key_pool.dtype or value_pool.dtype != key_pool.dtype:
+    dtype = query.dtype
+    if dtype != key_pool.dtype or value_pool.dtype != dtype:
         raise RuntimeError(f"{name}: query and pools must share a dtype")
     if not (key_pool.is_contiguous() and value_pool.is_contiguous()):
         raise RuntimeError(f"{name}: pools must be contiguous")
-    if query.size(2) != key_pool.size(3):
+    shape = query.shape
+    T, H, D = shape
+    if D != key_pool.size(3):
         raise RuntimeError(f"{name}: query and pools disagree on head_dim")
     if block_tables.dtype != torch.int32 or block_tables.dim() != 2:
         raise RuntimeError(f"{name}: block_tables must be int32 [rows, max_blocks]")
-    T, H, D = query.shape
-    if query.stride(2) != 1 or query.stride(1) != D or query.stride(0) < H * D:
-        query = query.contiguous()
-    if block_tables.stride(1) != 1 or block_tables.stride(0) < block_tables.size(1):
-        block_tables = block_tables.contiguous()
+    if not query.is_contiguous():
+        stride = query.stride()
+        if stride[2] != 1 or stride[1] != D or stride[0] < H * D:
+            query = query.contiguous()
+    if not block_tables.is_contiguous():
+        stride = block_tables.stride()
+        if stride[1] != 1 or stride[0] < block_tables.size(1):
+            block_tables = block_tables.contiguous()
     if out is None:
-        out = torch.empty((T, H, D), dtype=query.dtype, device=query.device)
-    elif (out.shape != (T, H, D) or out.dtype != query.dtype or out.stride(2) != 1
-          or out.stride(1) != D or (T > 1 and out.stride(0) < H * D)):
-        raise RuntimeError(f"{name}: out must be {[T, H, D]} with contiguous heads in the query's "
-                           "dtype")
+        out = torch.empty(shape, dtype=dtype, device=query.device)
+    elif out.shape != shape or out.dtype != dtype or not (
+            out.is_contiguous() or (out.stride(2) == 1 and out.stride(1) == D
+                                    and out.stride(0) >= H * D)):
+        raise RuntimeError(f"{name}: out must be {list(shape)} with contiguous heads in the "
+                           "query's dtype")
     mb = block_tables.size(1) if max_blocks_per_seq is None else int(max_blocks_per_seq)
     return query, block_tables, out, mb
 
@@ -696,12 +738,6 @@ def _window_inputs(name: str, query, key_pool, value_pool, block_tables, out, ma
 def _token_stride(t: torch.Tensor) -> int:
     """Elements between tokens of [T, H, D] (any stride of a single token will do)."""
     return max(t.stride(0), t.size(1) * t.size(2))
-
-
-def _scratch(nbytes: int, device: torch.device) -> torch.Tensor | None:
-    """Scratch of one call, from the stream-ordered allocator (inside a capture:
-    from the graph's own pool, so two graphs never share it)."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def window_attention_batched(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
@@ -728,20 +764,18 @@ def window_attention_batched(query: torch.Tensor, key_pool: torch.Tensor, value_
     context_lens = _int32_list("context_lens", context_lens, B)
     if seq_rows is not None:
         seq_rows = _int32_list("seq_rows", seq_rows, B)
-    code = dtype_code(query.dtype)
-    with torch.cuda.device(device):
-        stream = torch.cuda.current_stream(device).cuda_stream
-        need = ctypes.c_uint64(0)
-        check(lib().bs_window_attention_batched_workspace_bytes(
-            B, H, Hkv, D, bs, mb, code, int(window), int(sinks), ctypes.byref(need)))
-        scratch = _scratch(need.value, device)
+    code, window, sinks = dtype_code(query.dtype), int(window), int(sinks)
+    with _on(device):
+        stream, status = _stream_and_status(device)
+        scratch = _window_scratch("bs_window_attention_batched_workspace_bytes", device,
+                                  (B, H, Hkv, D, bs, mb, code, window, sinks))
         check(lib().bs_window_attention_batched(
             query.data_ptr(), _token_stride(query), key_pool.data_ptr(), value_pool.data_ptr(),
             block_tables.data_ptr(), block_tables.stride(0), block_tables.size(0),
             seq_rows.data_ptr() if seq_rows is not None else None, context_lens.data_ptr(), B, H,
-            Hkv, D, bs, NB, mb, code, float(scaling), int(window), int(sinks), out.data_ptr(),
-            _token_stride(out), scratch.data_ptr() if scratch is not None else None, need.value,
-            workspace_for(device, 0).data_ptr(), stream))
+            Hkv, D, bs, NB, mb, code, float(scaling), window, sinks, out.data_ptr(),
+            _token_stride(out), scratch.data_ptr() if scratch is not None else None,
+            scratch.numel() if scratch is not None else 0, status, stream))
     return out
 
 
@@ -772,22 +806,20 @@ def window_prefill_attention(query: torch.Tensor, key_pool: torch.Tensor, value_
     cu_q = _int32_list("cu_q", cu_q, R + 1)
     if seq_rows is not None:
         seq_rows = _int32_list("seq_rows", seq_rows, R)
-    code = dtype_code(query.dtype)
-    with torch.cuda.device(device):
-        stream = torch.cuda.current_stream(device).cuda_stream
-        need = ctypes.c_uint64(0)
-        check(lib().bs_window_prefill_attention_workspace_bytes(
-            T, R, int(max_query_len), H, Hkv, D, bs, mb, code, int(window), int(sinks),
-            ctypes.byref(need)))
-        scratch = _scratch(need.value, device)
+    code, window, sinks = dtype_code(query.dtype), int(window), int(sinks)
+    max_query_len = int(max_query_len)
+    with _on(device):
+        stream, status = _stream_and_status(device)
+        scratch = _window_scratch("bs_window_prefill_attention_workspace_bytes", device,
+                                  (T, R, max_query_len, H, Hkv, D, bs, mb, code, window, sinks))
         check(lib().bs_window_prefill_attention(
-            query.data_ptr(), _token_stride(query), cu_q.data_ptr(), R, T, int(max_query_len),
+            query.data_ptr(), _token_stride(query), cu_q.data_ptr(), R, T, max_query_len,
             context_lens.data_ptr(), seq_rows.data_ptr() if seq_rows is not None else None,
             key_pool.data_ptr(), value_pool.data_ptr(), block_tables.data_ptr(),
             block_tables.stride(0), block_tables.size(0), mb, H, Hkv, D, bs, NB, code,
-            float(scaling), int(window), int(sinks), out.data_ptr(), _token_stride(out),
-            scratch.data_ptr() if scratch is not None else None, need.value,
-            workspace_for(device, 0).data_ptr(), stream))
+            float(scaling), window, sinks, out.data_ptr(), _token_stride(out),
+            scratch.data_ptr() if scratch is not None else None,
+            scratch.numel() if scratch is not None else 0, status, stream))
     return out
 
 
@@ -888,14 +920,14 @@ def rotary_append(qkv: torch.Tensor, frequencies: torch.Tensor, positions: torch
         (T, num_heads, D), dtype=qkv.dtype, device=device)
     if not q_out.is_contiguous() or q_out.dtype != qkv.dtype or q_out.numel() < T * num_heads * D:
         raise RuntimeError("query_out must be contiguous [T, heads, head_dim] in the qkv dtype")
-    with torch.cuda.device(device):
-        stream = torch.cuda.current_stream(device).cuda_stream
+    with _on(device):
+        stream, status = _stream_and_status(device)
         check(lib().bs_rotary_append(
             q2.data_ptr(), q2.stride(0), dtype_code(qkv.dtype),
             frequencies.contiguous().data_ptr(), 2 * frequencies.numel(), 1 if interleaved else 0,
             float(amplitude), positions.data_ptr(), slot_mapping.data_ptr(), T, num_heads, Hkv, D,
             q_out.data_ptr(), key_pool.data_ptr(), value_pool.data_ptr(),
-            dtype_code(key_pool.dtype), NB, bs, workspace_for(device, 0).data_ptr(), stream))
+            dtype_code(key_pool.dtype), NB, bs, status, stream))
     return q_out
 
 
@@ -920,8 +952,8 @@ def copy_blocks(key_pool: torch.Tensor, value_pool: torch.Tensor, src: torch.Ten
     src, dst = _int32_list("src", src, n), _int32_list("dst", dst, n)
     layers = key_pool.size(0) if key_pool.dim() == 5 else 1
     Hkv, NB, bs, D = key_pool.shape[-4:]
-    with torch.cuda.device(device):
-        stream = torch.cuda.current_stream(device).cuda_stream
+    with _on(device):
+        stream, status = _stream_and_status(device)
         check(lib().bs_copy_blocks(
             key_pool.data_ptr(), value_pool.data_ptr(), dtype_code(key_pool.dtype), layers, Hkv, NB,
-            bs, D, src.data_ptr(), dst.data_ptr(), n, workspace_for(device, 0).data_ptr(), stream))
+            bs, D, src.data_ptr(), dst.data_ptr(), n, status, stream))
