@@ -32,9 +32,9 @@ int launch_rotary_append(const void* qkv, int64_t qkv_stride, bool bf16, const d
                          int32_t rotary_dim, bool interleaved, double amp, const int32_t* pos,
                          const int32_t* slots, int32_t ntok, int32_t H, int32_t Hkv, int32_t D,
                          void* q_out, void* k_pool, void* v_pool, bool pool_bf16,
-                         int64_t pool_slots, uint32_t* status, cudaStream_t stream);
+                         int64_t pool_slots, bool vec, uint32_t* status, cudaStream_t stream);
 int launch_copy_blocks(void* k_pool, void* v_pool, const int32_t* src, const int32_t* dst,
-                       int32_t n, int32_t num_blocks, int64_t rows, int64_t block_bytes, bool vec,
+                       int32_t n, int32_t num_blocks, int64_t rows, int64_t block_bytes, int align,
                        int sms, uint32_t* status, cudaStream_t stream);
 }  // namespace bsb
 
@@ -496,12 +496,15 @@ int bs_rotary_append(const void* qkv, int64_t qkv_row_stride, int32_t dtype,
   if (num_tokens == 0) return BS_OK;
   BS_CHECK(qkv && frequencies && positions && slot_mapping && query_out && key_pool && value_pool,
            "null pointer argument");
+  const bool vec = head_dim % 8 == 0 && rotary_dim % (interleaved ? 8 : 16) == 0 &&
+                   qkv_row_stride % 8 == 0 && aligned16(qkv) && aligned16(query_out) &&
+                   aligned16(key_pool) && aligned16(value_pool);
   const int rc = bsb::launch_rotary_append(
       qkv, qkv_row_stride, dtype == BS_BF16, frequencies, static_cast<int32_t>(rotary_dim),
       interleaved != 0, amplitude, positions, slot_mapping, static_cast<int32_t>(num_tokens),
       static_cast<int32_t>(num_heads), static_cast<int32_t>(num_kv_heads),
       static_cast<int32_t>(head_dim), query_out, key_pool, value_pool, pool_dtype == BS_BF16,
-      slots, status, static_cast<cudaStream_t>(stream));
+      slots, vec, status, static_cast<cudaStream_t>(stream));
   if (rc != 0) return cuda_fail(rc, "rotary_append launch");
   bsb::add_kernel_launches(1);
   return BS_OK;
@@ -525,10 +528,13 @@ int bs_copy_blocks(void* key_pool, void* value_pool, int32_t pool_dtype, int64_t
   BS_CHECK(key_pool && value_pool && src && dst, "null pointer argument");
   int sms = 0;
   if (int rc = bsb::sm_count(&sms)) return rc;
-  const bool vec = block_bytes % 16 == 0 && aligned16(key_pool) && aligned16(value_pool);
+  const uint64_t bits = reinterpret_cast<uintptr_t>(key_pool) |
+                        reinterpret_cast<uintptr_t>(value_pool) |
+                        static_cast<uint64_t>(block_bytes);
+  const int align = bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : 2;
   const int rc = bsb::launch_copy_blocks(key_pool, value_pool, src, dst,
                                          static_cast<int32_t>(num_pairs),
-                                         static_cast<int32_t>(num_blocks), rows, block_bytes, vec,
+                                         static_cast<int32_t>(num_blocks), rows, block_bytes, align,
                                          sms, status, static_cast<cudaStream_t>(stream));
   if (rc != 0) return cuda_fail(rc, "copy_blocks launch");
   bsb::add_kernel_launches(1);

@@ -6,6 +6,12 @@
 // pair, would make the result depend on their order, so such a pair is skipped and
 // reported.  Every CTA looks its own destination up in the pair list (n entries
 // from L2, against the 2 * layers * kv heads blocks it copies).
+//
+// Bandwidth bound (each byte read and written once).  A warp copies segments of 32
+// lanes x 32 bytes (the widest access of sm_100), four at a time: all loads of a
+// round are issued before its stores, which keeps enough of them in flight.
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace bsb {
@@ -21,9 +27,38 @@ struct CopyArgs {
   int32_t n, num_blocks;
   int64_t rows;  // layers * kv heads
   int64_t block_bytes;
+  int32_t parts;   // segments of 32 accesses per block
   int32_t slices;  // CTAs per pair
   uint32_t* status;
 };
+
+struct __align__(32) Vec32 {
+  uint32_t w[8];
+};
+
+template <typename V>
+__device__ __forceinline__ V load_vec(const V* p) { return *p; }
+template <>
+__device__ __forceinline__ Vec32 load_vec<Vec32>(const Vec32* p) {
+  Vec32 v;
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]),
+                 "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
+               : "l"(p));
+  return v;
+}
+template <typename V>
+__device__ __forceinline__ void store_vec(V* p, const V& v) { *p = v; }
+template <>
+__device__ __forceinline__ void store_vec<Vec32>(Vec32* p, const Vec32& v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v.w[0]),
+               "r"(v.w[1]), "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]),
+               "r"(v.w[7])
+               : "memory");
+}
+
+constexpr int kWarps = kThreads / 32;
+constexpr int kRound = 4;  // segments a warp copies at a time
 
 template <typename V>
 __global__ void __launch_bounds__(kThreads) copy_blocks_kernel(const CopyArgs a) {
@@ -47,38 +82,70 @@ __global__ void __launch_bounds__(kThreads) copy_blocks_kernel(const CopyArgs a)
     if (threadIdx.x == 0) set_status(a.status, kStatusBadCopy);
     return;
   }
+  // Segment g: part g % parts of the block of (K or V, layer, head) g / parts.
+  const int lane = threadIdx.x & 31;
   const int64_t vecs = a.block_bytes / static_cast<int64_t>(sizeof(V));
-  for (int64_t row = slice; row < 2 * a.rows; row += a.slices) {
-    uint8_t* pool = row < a.rows ? a.k_pool : a.v_pool;
-    const int64_t base = (row < a.rows ? row : row - a.rows) * a.num_blocks;
-    const V* from = reinterpret_cast<const V*>(pool + (base + s) * a.block_bytes);
-    V* to = reinterpret_cast<V*>(pool + (base + d) * a.block_bytes);
-    for (int64_t x = threadIdx.x; x < vecs; x += kThreads) to[x] = from[x];
+  const int64_t segments = 2 * a.rows * a.parts;
+  const int64_t step = static_cast<int64_t>(a.slices) * kWarps;
+  for (int64_t g0 = slice * kWarps + (threadIdx.x >> 5); g0 < segments; g0 += step * kRound) {
+    V v[kRound];
+    V* to[kRound];
+#pragma unroll
+    for (int k = 0; k < kRound; ++k) {
+      const int64_t g = g0 + k * step;
+      to[k] = nullptr;
+      if (g >= segments) continue;
+      const int64_t row = g / a.parts;
+      const int64_t x = (g - row * a.parts) * 32 + lane;
+      if (x >= vecs) continue;
+      uint8_t* pool = row < a.rows ? a.k_pool : a.v_pool;
+      const int64_t base = (row < a.rows ? row : row - a.rows) * a.num_blocks;
+      to[k] = reinterpret_cast<V*>(pool + (base + d) * a.block_bytes) + x;
+      v[k] = load_vec(reinterpret_cast<const V*>(pool + (base + s) * a.block_bytes) + x);
+    }
+#pragma unroll
+    for (int k = 0; k < kRound; ++k) {
+      if (to[k] != nullptr) store_vec(to[k], v[k]);
+    }
   }
 }
 
-}  // namespace
-
-int launch_copy_blocks(void* k_pool, void* v_pool, const int32_t* src, const int32_t* dst,
-                       int32_t n, int32_t num_blocks, int64_t rows, int64_t block_bytes, bool vec,
-                       int sms, uint32_t* status, cudaStream_t stream) {
-  // About eight CTAs per SM over all pairs, at most one per (K or V, layer, head).
-  int64_t slices = (static_cast<int64_t>(sms) * 8 + n - 1) / n;
-  if (slices > 2 * rows) slices = 2 * rows;
-  if (slices * n > 0x7fffffff) return static_cast<int>(cudaErrorInvalidConfiguration);
-  const CopyArgs a{static_cast<uint8_t*>(k_pool), static_cast<uint8_t*>(v_pool), src, dst, n,
-                   num_blocks, rows, block_bytes, static_cast<int32_t>(slices), status};
+template <typename V>
+int launch_copy(CopyArgs a, int sms, cudaStream_t stream) {
+  const int64_t vecs = a.block_bytes / static_cast<int64_t>(sizeof(V));
+  const int64_t parts = (vecs + 31) / 32;
+  const int64_t segments = 2 * a.rows * parts;
+  // About eight CTAs per SM over all pairs, at most one segment per warp.
+  const int64_t slices = std::max<int64_t>(
+      1, std::min((static_cast<int64_t>(sms) * 8 + a.n - 1) / a.n, (segments + kWarps - 1) / kWarps));
+  if (slices * a.n > 0x7fffffff || parts > 0x7fffffff) {
+    return static_cast<int>(cudaErrorInvalidConfiguration);
+  }
+  a.parts = static_cast<int32_t>(parts);
+  a.slices = static_cast<int32_t>(slices);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(slices * n));
+  cfg.gridDim = dim3(static_cast<unsigned>(slices * a.n));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  auto kernel = vec ? copy_blocks_kernel<uint4> : copy_blocks_kernel<uint16_t>;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, a));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, copy_blocks_kernel<V>, a));
+}
+
+}  // namespace
+
+// align: bytes that every block's address is a multiple of.
+int launch_copy_blocks(void* k_pool, void* v_pool, const int32_t* src, const int32_t* dst,
+                       int32_t n, int32_t num_blocks, int64_t rows, int64_t block_bytes, int align,
+                       int sms, uint32_t* status, cudaStream_t stream) {
+  const CopyArgs a{static_cast<uint8_t*>(k_pool), static_cast<uint8_t*>(v_pool), src, dst, n,
+                   num_blocks, rows, block_bytes, 0, 0, status};
+  if (align >= 32) return launch_copy<Vec32>(a, sms, stream);
+  if (align >= 16) return launch_copy<uint4>(a, sms, stream);
+  return launch_copy<uint16_t>(a, sms, stream);
 }
 
 }  // namespace bsb
