@@ -142,11 +142,23 @@ bool mma_shape(const WindowShape& s) {
   return s.dtype == BS_BF16 && s.block_size % 16 == 0 && (s.head_dim == 64 || s.head_dim == 128);
 }
 
-// How the tensor-core decode runs a call: persistent CTAs over the batch's units,
-// two partial records and one merge task each.
+// How the tensor-core decode runs a call: a cluster of segment_ctas CTAs per
+// (sequence, kv head); or (segment_ctas 0) persistent CTAs over the batch's units,
+// with two partial records and one merge task each.
 struct MmaDecodePlan {
-  int64_t grid, rec_stride, tasks_offset, bytes;
+  int64_t segment_ctas, grid, rec_stride, tasks_offset, bytes;
 };
+
+constexpr int64_t kMaxSegmentCtas = 8;
+
+// Whether clusters of c CTAs take the segments, the longest of `most` units, instead
+// of spans over the batch.  Clusters start and end sooner (no scan of the batch, no
+// merge launch), spans share ragged work out evenly.  Measured, clusters / spans in
+// us, d64, two kv heads, one sequence with a window of 64: 7.0 / 10.1, 4096: 14.8 /
+// 19.9; 64 sequences (c = 3), log-uniform lengths up to 4 windows of 1024 (6 units a
+// warp): 13.9 / 15.4, of 2048 (11): 19.2 / 16.7; 200 (c = 1), 256 (5): 11.6 / 14.7,
+// 1024 (17): 24.4 / 17.6; d128, 16 sequences (c = 4), 4096 (16): 18.1 / 24.4.
+bool clusters_win(int64_t c, int64_t most) { return most <= c * 4 * (c >= 4 ? 16 : 8); }
 
 int plan_mma_decode(const WindowShape& s, MmaDecodePlan* p) {
   int sms = 0, dev = 0;
@@ -155,8 +167,8 @@ int plan_mma_decode(const WindowShape& s, MmaDecodePlan* p) {
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   const int64_t groups = s.heads / s.kv_heads;
   // Resident CTAs per SM by device, [head_dim 128][more than 8 heads a group].
-  static std::atomic<int> resident[64][2][2];
-  std::atomic<int>* known = dev < 64 ? &resident[dev][s.head_dim == 128][groups > 8] : nullptr;
+  static std::atomic<int> per_sm[64][2][2];
+  std::atomic<int>* known = dev < 64 ? &per_sm[dev][s.head_dim == 128][groups > 8] : nullptr;
   int ctas = known != nullptr ? known->load() : 0;
   if (ctas == 0) {
     ctas = bsb::window_decode_mma_ctas_per_sm(static_cast<int>(s.head_dim),
@@ -169,9 +181,21 @@ int plan_mma_decode(const WindowShape& s, MmaDecodePlan* p) {
   const int64_t unit = bsb::kWindowUnit;
   const int64_t seen = (std::min(s.window, kMaxContext) + unit - 1) / unit + 1 +
                        (std::min(s.sinks, kMaxContext) + unit - 1) / unit;
-  const int64_t units = s.rows * s.kv_heads * std::min(seen, s.max_blocks * s.block_size / unit);
-  p->grid = std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(sms) * ctas,
-                                                   (units + 3) / 4));
+  const int64_t most = std::min(seen, s.max_blocks * s.block_size / unit);
+  const int64_t resident = static_cast<int64_t>(sms) * ctas, segments = s.rows * s.kv_heads;
+  p->segment_ctas = 0;
+  if (segments > 0 && segments <= resident) {
+    const int64_t c = std::min({kMaxSegmentCtas, std::max<int64_t>(resident / segments, 1),
+                                std::max<int64_t>((most + 3) / 4, 1)});
+    if (clusters_win(c, most)) {
+      p->segment_ctas = c;
+      p->grid = segments * c;
+      p->rec_stride = p->tasks_offset = p->bytes = 0;
+      return BS_OK;
+    }
+  }
+  const int64_t units = s.rows * s.kv_heads * most;
+  p->grid = std::max<int64_t>(1, std::min(resident, (units + 3) / 4));
   p->rec_stride = bsb::decode_record_stride(groups, s.head_dim);
   p->tasks_offset = (2 * p->grid * p->rec_stride * 4 + 255) / 256 * 256;
   p->bytes = p->tasks_offset + p->grid * static_cast<int64_t>(sizeof(bsb::MergeTask));
@@ -302,7 +326,9 @@ int run_mma_decode(const WindowShape& s, const WindowCall& c) {
   uint8_t* ws = static_cast<uint8_t*>(c.workspace);
   a.partials = reinterpret_cast<float*>(ws);
   a.rec_stride = static_cast<int32_t>(p.rec_stride);
-  a.tasks = reinterpret_cast<bsb::MergeTask*>(ws + p.tasks_offset);
+  a.tasks = p.segment_ctas > 0 ? nullptr
+                               : reinterpret_cast<bsb::MergeTask*>(ws + p.tasks_offset);
+  a.segment_ctas = static_cast<int32_t>(p.segment_ctas);
   a.status = c.status;
   a.window = static_cast<int32_t>(std::min(s.window, kMaxContext));
   a.sinks = static_cast<int32_t>(std::min(s.sinks, kMaxContext));
@@ -311,7 +337,7 @@ int run_mma_decode(const WindowShape& s, const WindowCall& c) {
   const int rc = bsb::launch_window_decode_mma(a, kmap, vmap, static_cast<int>(p.grid),
                                                static_cast<cudaStream_t>(c.stream));
   if (rc != 0) return cuda_fail(rc, "window decode launch");
-  bsb::add_kernel_launches(2);  // the decode and its merge pass
+  bsb::add_kernel_launches(p.segment_ctas > 0 ? 1 : 2);  // the decode and its merge pass
   return BS_OK;
 }
 

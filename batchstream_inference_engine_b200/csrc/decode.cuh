@@ -74,7 +74,28 @@ struct DecodeArgs {
   // j >= len - window are seen; a unit is then 16 tokens, `block_units` of them to
   // a block.
   int32_t window, sinks, block_units;
+  // Non-zero: every segment has its own cluster of segment_ctas CTAs (cluster b /
+  // segment_ctas: sequence and kv head as b / Hkv, b % Hkv), which join their parts
+  // through distributed shared memory: no spans over the batch, no merge pass.
+  int32_t segment_ctas;
 };
+
+// Barrier of a cluster's CTAs (all their threads), ordering their shared memory.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Float `index` of shared array `p` in CTA `rank` of the cluster.
+__device__ __forceinline__ float cluster_load(const float* p, int index, uint32_t rank) {
+  uint32_t addr;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(addr)
+               : "r"(smem_u32(p + index)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
 
 // Tokens per unit of the sliding-window variant (one tile of the tensor cores).
 constexpr int32_t kWindowUnit = 16;
@@ -507,6 +528,35 @@ __device__ __forceinline__ Span compute_warp_spans_smem(const DecodeArgs& a, Sca
   sp.seq = ws.seq[0];
   sp.prefix = ws.prefix[0];
   if (sp.seq < 0) sp.r1 = sp.r0;  // cannot happen when r0 < W; never walk from nowhere
+  return sp;
+}
+
+// The span of a CTA of a segment's cluster (DecodeArgs::segment_ctas), in unit numbers
+// of its sequence alone.  All threads call it.
+template <int NW>
+__device__ __forceinline__ Span segment_span(const DecodeArgs& a, WarpStarts& ws, int32_t& seq,
+                                             int32_t& h, int32_t& nb) {
+  const int32_t seg = blockIdx.x / a.segment_ctas, rank = blockIdx.x % a.segment_ctas;
+  seq = seg / a.num_kv_heads;
+  h = seg % a.num_kv_heads;
+  int32_t len, row;
+  nb = seq_units<true>(a, seq, len, row, h == 0 && rank == 0 && threadIdx.x == 0);
+  if (threadIdx.x < NW) {
+    const int k = threadIdx.x;
+    ws.seq[k] = seq;
+    ws.prefix[k] = 0;
+    ws.len[k] = len;
+    ws.row[k] = row;
+    ws.nlen[k] = 0;
+    ws.nrow[k] = -1;
+  }
+  __syncthreads();
+  Span sp{};
+  const int64_t first = static_cast<int64_t>(h) * nb;
+  sp.q = nb;
+  sp.r0 = first + static_cast<int64_t>(nb) * rank / a.segment_ctas;
+  sp.r1 = first + static_cast<int64_t>(nb) * (rank + 1) / a.segment_ctas;
+  sp.seq = seq;
   return sp;
 }
 

@@ -120,12 +120,16 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
   // The stages are free until the first copy: they hold the lengths and rows
   // for the span scan when they fit (one round of global loads).
   constexpr int kScratchInts = W * S * C::STAGE_BYTES / 4;
+  int32_t own_seq = 0, own_kvh = 0, own_units = 0;  // WIN: the cluster's segment
+  const bool clustered = WIN && a.segment_ctas > 0;
   const Span sp =
-      2 * a.num_seqs <= kScratchInts
+      clustered ? segment_span<W>(a, starts, own_seq, own_kvh, own_units)
+      : 2 * a.num_seqs <= kScratchInts
           ? compute_warp_spans_smem<W, WIN>(a, scan, starts, reinterpret_cast<int32_t*>(smem))
           : compute_warp_spans<W, WIN>(a, scan, starts);  // both sync the inits
   if (a.lens_ready && !early_loads) pdl_wait();  // query, pools from here on
-  if (sp.r0 >= sp.r1) {
+  if (clustered && own_units == 0) return;  // the whole cluster: nothing to read or write
+  if (sp.r0 >= sp.r1 && !clustered) {
     if (a.tasks != nullptr && tid == 0) a.tasks[blockIdx.x].valid = 0;
     return;
   }
@@ -231,7 +235,8 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
     const int64_t seg_unit = cprefix * Hkv + static_cast<int64_t>(ch) * cnb;
     const bool first = (cu == wr0) || (cb == 0);
     const bool last = (cu == wr1 - 1) || (cb == cnb - 1);
-    const bool whole = seg_unit >= wr0 && seg_unit + cnb <= wr1;
+    const bool whole = seg_unit >= wr0 && seg_unit + cnb <= wr1 &&
+                       !(clustered && a.segment_ctas > 1);
     if (lane == 0) {
       if (!valid && !dry) set_status(a.status, kStatusBadBlock);
       TileMeta& m = meta[warp][stage];
@@ -532,6 +537,17 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
     }
   }
 
+  // Clusters: the CTA's joined part (O, maxima, sums), read by the other CTAs; empty
+  // until its last warp fills it.  (Slot 0 of warp 0 is folded before that.)
+  __shared__ float part_ml[WIN ? 2 * C::GROWS : 1];
+  const bool joined = clustered && a.segment_ctas > 1;
+  if (joined && tid < C::GROWS) {
+    part_ml[tid] = -INFINITY;
+    part_ml[C::GROWS + tid] = 0.f;
+  }
+  __shared__ int32_t part_slot;
+  if (WIN && tid == 0) part_slot = 0;
+
   // ---------------------------------------------------------------- CTA merge
   // A segment cut between warps is a chain: the last portion of the warp where
   // it starts, the only portion of warps inside it, the first portion of the
@@ -589,7 +605,13 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
     }
     const int64_t seg_unit = slot_unit[warp][k];
     const int32_t nb = slot_nb[warp][k];
-    if (seg_unit >= sp.r0 && seg_unit + nb <= sp.r1) {
+    if (joined) {
+      if (lane < G) {
+        part_ml[lane] = mine[G * D + lane];
+        part_ml[C::GROWS + lane] = mine[G * D + G + lane];
+      }
+      if (lane == 0) part_slot = static_cast<int32_t>(mine - reinterpret_cast<float*>(smem));
+    } else if (seg_unit >= sp.r0 && seg_unit + nb <= sp.r1) {
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
                            static_cast<int64_t>(seq) * a.o_stride_seq +
                            static_cast<int64_t>(kvh) * G * D;
@@ -626,6 +648,36 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
       }
     }
   }
+  if (joined) {
+    // Each CTA of the cluster joins its share of the segment's elements from all
+    // parts, in rank order.  A part's place differs from CTA to CTA.
+    cluster_sync();
+    const uint32_t ranks = a.segment_ctas, rank = blockIdx.x % a.segment_ctas;
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
+                         static_cast<int64_t>(own_seq) * a.o_stride_seq +
+                         static_cast<int64_t>(own_kvh) * G * D;
+    for (int e = rank * (W * 32) + tid; e < G * D; e += ranks * (W * 32)) {
+      const int r = e / D;
+      float M = -INFINITY, m[8];
+#pragma unroll
+      for (uint32_t k = 0; k < 8; ++k) {
+        m[k] = k < ranks ? cluster_load(part_ml, r, k) : -INFINITY;
+        M = fmaxf(M, m[k]);
+      }
+      float L = 0.f, O = 0.f;
+#pragma unroll
+      for (uint32_t k = 0; k < 8; ++k) {
+        if (m[k] == -INFINITY) continue;  // an empty part
+        const float f = fast_exp2(m[k] - M);
+        const int at = __float_as_int(cluster_load(reinterpret_cast<float*>(&part_slot), 0, k));
+        L += f * cluster_load(part_ml, C::GROWS + r, k);
+        O += f * cluster_load(reinterpret_cast<float*>(smem), at + e, k);
+      }
+      out[e] = __float2bfloat16_rn(O / L);
+    }
+    cluster_sync();  // the others may still read this CTA's shared memory
+    return;
+  }
   // Segments crossing CTAs for which this CTA came last: merge with all threads.
   // The stages and slots are free now and serve as scratch.
   __syncthreads();
@@ -655,11 +707,17 @@ int launch_one(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap& 
   cfg.blockDim = dim3(C::W * 32);
   cfg.dynamicSmemBytes = C::SMEM_BYTES;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (WIN && a.segment_ctas > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.segment_ctas;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
   return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_mma_kernel<D, G16, WIN>, kmap, vmap, a));
 }
 

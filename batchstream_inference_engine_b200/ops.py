@@ -694,6 +694,8 @@ def _window_scratch(query_fn, device: torch.device, sizes: tuple) -> torch.Tenso
     key = (query_fn, device.index, sizes)
     need = _window_ws_bytes.get(key)
     if need is None:
+        if len(_window_ws_bytes) >= 4096:  # ragged steps bring ever new sizes
+            _window_ws_bytes.clear()
         got = ctypes.c_uint64(0)
         check(getattr(lib(), query_fn)(*sizes, ctypes.byref(got)))
         need = _window_ws_bytes[key] = got.value
@@ -725,7 +727,7 @@ def _window_inputs(name: str, query, key_pool, value_pool, block_tables, out, ma
         if stride[1] != 1 or stride[0] < block_tables.size(1):
             block_tables = block_tables.contiguous()
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=query.device)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype != dtype or not (
             out.is_contiguous() or (out.stride(2) == 1 and out.stride(1) == D
                                     and out.stride(0) >= H * D)):
@@ -916,8 +918,7 @@ def rotary_append(qkv: torch.Tensor, frequencies: torch.Tensor, positions: torch
     q2 = _rows_2d("qkv", qkv, width)
     if q2.stride(0) < width:
         q2 = q2.contiguous()
-    q_out = query_out if query_out is not None else torch.empty(
-        (T, num_heads, D), dtype=qkv.dtype, device=device)
+    q_out = query_out if query_out is not None else qkv.new_empty((T, num_heads, D))
     if not q_out.is_contiguous() or q_out.dtype != qkv.dtype or q_out.numel() < T * num_heads * D:
         raise RuntimeError("query_out must be contiguous [T, heads, head_dim] in the qkv dtype")
     with _on(device):
