@@ -8,6 +8,10 @@ statically and its symbols are kept local to the library, so the library does
 not depend on (or interfere with) the runtime that PyTorch loads; the driver is
 reached at run time through the runtime's entry-point query, so the library
 also loads on a machine without a GPU driver.
+
+``csrc/binding.cpp`` becomes ``_native.so``, the Python entry points of the
+bounded-cache operators: a C++ extension over torch's headers, linked against
+``libbatchstream_b200.so`` (found next to it) and the libraries torch has loaded.
 """
 
 from __future__ import annotations
@@ -16,6 +20,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -23,6 +28,7 @@ PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE / "csrc"
 BUILD = PACKAGE / "_build"
 LIBRARY = PACKAGE / "libbatchstream_b200.so"
+BINDING = PACKAGE / "_native.so"
 INCLUDE = PACKAGE.parent / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -77,7 +83,37 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         if proc.returncode != 0:
             raise RuntimeError(f"linking libbatchstream_b200.so failed:\n{proc.stderr}")
         tmp.replace(LIBRARY)
+    build_binding(force)
     return LIBRARY
+
+
+def build_binding(force: bool = False) -> Path:
+    """Compile (if stale) and return the path of the Python extension."""
+    source = CSRC / "binding.cpp"
+    if not (force or _stale(BINDING, [source, INCLUDE / "batchstream_b200.h"])):
+        return BINDING
+    compiler = shutil.which("g++")
+    if compiler is None:
+        raise RuntimeError("g++ not found: it is needed to build the Python extension")
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [
+        compiler, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        f"-I{INCLUDE}", f"-I{root / 'include'}",
+        f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+        f"-I{sysconfig.get_paths()['include']}", f"-I{cuda / 'include'}",
+        str(source), "-o", str(tmp), f"-L{PACKAGE}", "-lbatchstream_b200", f"-L{root / 'lib'}",
+        "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN",
+    ]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"building {BINDING.name} failed:\n{proc.stderr}")
+    tmp.replace(BINDING)
+    return BINDING
 
 
 if __name__ == "__main__":

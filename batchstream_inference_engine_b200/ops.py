@@ -17,6 +17,12 @@ import torch
 from . import _lib
 from ._lib import BS_BF16, BS_F32, check, i64_array, lib
 
+try:
+    from . import _native
+except ImportError as e:
+    raise ImportError("the _native extension is not built or does not load; run "
+                      "`python -m batchstream_inference_engine_b200.build`") from e
+
 _DTYPES = {torch.bfloat16: BS_BF16, torch.float32: BS_F32}
 
 
@@ -69,10 +75,13 @@ class _Workspaces:
                     fresh[:4].copy_(buf[:4])
                 buf = fresh
                 self._buffers[key] = buf
+                _native.forget_status()  # it may hold the old buffer's address
             return buf
 
 
 _workspaces = _Workspaces()
+_native.set_status_source(lambda index, stream: _workspaces.get(
+    torch.device("cuda", index), stream, 0).data_ptr())
 
 
 def workspace_for(device: torch.device, nbytes: int) -> torch.Tensor:
@@ -655,91 +664,8 @@ def prefill_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: t
 
 # ------------------------------------------------------------------ bounded caches
 #
-# These calls last microseconds on the device, so their host side counts: the
-# workspace size of a shape is asked for once, the stream comes as its raw handle,
-# and the device is switched only when it is not the current one.
-
-
-def _int32_list(name: str, t: torch.Tensor, count: int) -> torch.Tensor:
-    """`t` as int32 entries one after the other, at least `count` of them."""
-    if t.dtype != torch.int32:
-        raise RuntimeError(f"{name} must be int32")
-    if t.dim() != 1 or t.numel() < count:
-        raise RuntimeError(f"{name} must be one-dimensional with at least {count} entries")
-    return t if t.is_contiguous() else t.contiguous()
-
-
-_null_context = _NullContext()
-
-
-def _on(device: torch.device):
-    """Context in which `device` is current."""
-    if torch.cuda.current_device() == device.index:
-        return _null_context
-    return torch.cuda.device(device)
-
-
-def _stream_and_status(device: torch.device) -> tuple[int, int]:
-    """The current stream of `device` and the address of its status word."""
-    stream = torch._C._cuda_getCurrentRawStream(device.index)
-    return stream, _workspaces.get(device, stream, 0).data_ptr()
-
-
-_window_ws_bytes: dict[tuple, int] = {}
-
-
-def _window_scratch(query_fn, device: torch.device, sizes: tuple) -> torch.Tensor | None:
-    """Scratch of one window attention call, from the stream-ordered allocator
-    (inside a capture: from the graph's own pool, so two graphs never share it)."""
-    key = (query_fn, device.index, sizes)
-    need = _window_ws_bytes.get(key)
-    if need is None:
-        if len(_window_ws_bytes) >= 4096:  # ragged steps bring ever new sizes
-            _window_ws_bytes.clear()
-        got = ctypes.c_uint64(0)
-        check(getattr(lib(), query_fn)(*sizes, ctypes.byref(got)))
-        need = _window_ws_bytes[key] = got.value
-    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
-
-
-def _window_inputs(name: str, query, key_pool, value_pool, block_tables, out, max_blocks_per_seq):
-    """The checks that both window attentions share; returns query, block_tables,
-    out and max_blocks as the C call takes them."""
-    if query.dim() != 3 or key_pool.dim() != 4 or value_pool.shape != key_pool.shape:
-        raise RuntimeError(f"{name}: query must be [T, H, D] and the pools [Hkv, NB, bs, D]")
-    dtype = query.dtype
-    if dtype != key_pool.dtype or value_pool.dtype != dtype:
-        raise RuntimeError(f"{name}: query and pools must share a dtype")
-    if not (key_pool.is_contiguous() and value_pool.is_contiguous()):
-        raise RuntimeError(f"{name}: pools must be contiguous")
-    shape = query.shape
-    T, H, D = shape
-    if D != key_pool.size(3):
-        raise RuntimeError(f"{name}: query and pools disagree on head_dim")
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2:
-        raise RuntimeError(f"{name}: block_tables must be int32 [rows, max_blocks]")
-    if not query.is_contiguous():
-        stride = query.stride()
-        if stride[2] != 1 or stride[1] != D or stride[0] < H * D:
-            query = query.contiguous()
-    if not block_tables.is_contiguous():
-        stride = block_tables.stride()
-        if stride[1] != 1 or stride[0] < block_tables.size(1):
-            block_tables = block_tables.contiguous()
-    if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    elif out.shape != shape or out.dtype != dtype or not (
-            out.is_contiguous() or (out.stride(2) == 1 and out.stride(1) == D
-                                    and out.stride(0) >= H * D)):
-        raise RuntimeError(f"{name}: out must be {list(shape)} with contiguous heads in the "
-                           "query's dtype")
-    mb = block_tables.size(1) if max_blocks_per_seq is None else int(max_blocks_per_seq)
-    return query, block_tables, out, mb
-
-
-def _token_stride(t: torch.Tensor) -> int:
-    """Elements between tokens of [T, H, D] (any stride of a single token will do)."""
-    return max(t.stride(0), t.size(1) * t.size(2))
+# The checks and calls of these are in C++ (csrc/binding.cpp): they last microseconds
+# on the device.
 
 
 def window_attention_batched(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
@@ -756,29 +682,9 @@ def window_attention_batched(query: torch.Tensor, key_pool: torch.Tensor, value_
     (``BlockAllocator.trim``).  A length of 0 marks a padding row, whose output
     row is left as it was.  Scores stay in fp32.
     """
-    device = _require_cuda("window_attention_batched", query, key_pool, value_pool, block_tables,
-                           context_lens, seq_rows, out)
-    query, block_tables, out, mb = _window_inputs("window_attention_batched", query, key_pool,
-                                                  value_pool, block_tables, out,
-                                                  max_blocks_per_seq)
-    B, H, D = query.shape
-    Hkv, NB, bs, _ = key_pool.shape
-    context_lens = _int32_list("context_lens", context_lens, B)
-    if seq_rows is not None:
-        seq_rows = _int32_list("seq_rows", seq_rows, B)
-    code, window, sinks = dtype_code(query.dtype), int(window), int(sinks)
-    with _on(device):
-        stream, status = _stream_and_status(device)
-        scratch = _window_scratch("bs_window_attention_batched_workspace_bytes", device,
-                                  (B, H, Hkv, D, bs, mb, code, window, sinks))
-        check(lib().bs_window_attention_batched(
-            query.data_ptr(), _token_stride(query), key_pool.data_ptr(), value_pool.data_ptr(),
-            block_tables.data_ptr(), block_tables.stride(0), block_tables.size(0),
-            seq_rows.data_ptr() if seq_rows is not None else None, context_lens.data_ptr(), B, H,
-            Hkv, D, bs, NB, mb, code, float(scaling), window, sinks, out.data_ptr(),
-            _token_stride(out), scratch.data_ptr() if scratch is not None else None,
-            scratch.numel() if scratch is not None else 0, status, stream))
-    return out
+    return _native.window_attention_batched(query, key_pool, value_pool, block_tables,
+                                            context_lens, scaling, window, sinks, seq_rows, out,
+                                            max_blocks_per_seq)
 
 
 def window_prefill_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
@@ -796,33 +702,9 @@ def window_prefill_attention(query: torch.Tensor, key_pool: torch.Tensor, value_
     ``max_query_len`` or than its context, or outside the T rows, is reported
     (``take_status``) and skipped.
     """
-    device = _require_cuda("window_prefill_attention", query, key_pool, value_pool, block_tables,
-                           cu_q, context_lens, seq_rows, out)
-    query, block_tables, out, mb = _window_inputs("window_prefill_attention", query, key_pool,
-                                                  value_pool, block_tables, out,
-                                                  max_blocks_per_seq)
-    T, H, D = query.shape
-    Hkv, NB, bs, _ = key_pool.shape
-    context_lens = _int32_list("context_lens", context_lens, 0)
-    R = context_lens.numel()
-    cu_q = _int32_list("cu_q", cu_q, R + 1)
-    if seq_rows is not None:
-        seq_rows = _int32_list("seq_rows", seq_rows, R)
-    code, window, sinks = dtype_code(query.dtype), int(window), int(sinks)
-    max_query_len = int(max_query_len)
-    with _on(device):
-        stream, status = _stream_and_status(device)
-        scratch = _window_scratch("bs_window_prefill_attention_workspace_bytes", device,
-                                  (T, R, max_query_len, H, Hkv, D, bs, mb, code, window, sinks))
-        check(lib().bs_window_prefill_attention(
-            query.data_ptr(), _token_stride(query), cu_q.data_ptr(), R, T, max_query_len,
-            context_lens.data_ptr(), seq_rows.data_ptr() if seq_rows is not None else None,
-            key_pool.data_ptr(), value_pool.data_ptr(), block_tables.data_ptr(),
-            block_tables.stride(0), block_tables.size(0), mb, H, Hkv, D, bs, NB, code,
-            float(scaling), window, sinks, out.data_ptr(), _token_stride(out),
-            scratch.data_ptr() if scratch is not None else None,
-            scratch.numel() if scratch is not None else 0, status, stream))
-    return out
+    return _native.window_prefill_attention(query, key_pool, value_pool, block_tables, cu_q,
+                                            context_lens, scaling, max_query_len, window, sinks,
+                                            seq_rows, out, max_blocks_per_seq)
 
 
 def rope_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None,
@@ -899,37 +781,8 @@ def rotary_append(qkv: torch.Tensor, frequencies: torch.Tensor, positions: torch
     negative slot skips the row's K/V write; two rows must not share a slot.
     Returns q as [T, H, D].
     """
-    device = _require_cuda("rotary_append", qkv, frequencies, positions, slot_mapping, key_pool,
-                           value_pool, query_out)
-    if key_pool.dim() != 4 or value_pool.shape != key_pool.shape \
-            or value_pool.dtype != key_pool.dtype:
-        raise RuntimeError("the pools must be [Hkv, NB, bs, D] of one shape and dtype")
-    if not (key_pool.is_contiguous() and value_pool.is_contiguous()):
-        raise RuntimeError("pools must be contiguous")
-    Hkv, NB, bs, D = key_pool.shape
-    T = positions.numel()
-    positions = _int32_list("positions", positions, T)
-    slot_mapping = _int32_list("slot_mapping", slot_mapping, T)
-    if frequencies.dtype != torch.float64 or frequencies.dim() != 1:
-        raise RuntimeError("frequencies must be one-dimensional float64")
-    if qkv.dim() < 2 or qkv.size(0) < T:
-        raise RuntimeError("qkv needs a row per position")
-    width = (num_heads + 2 * Hkv) * D
-    q2 = _rows_2d("qkv", qkv, width)
-    if q2.stride(0) < width:
-        q2 = q2.contiguous()
-    q_out = query_out if query_out is not None else qkv.new_empty((T, num_heads, D))
-    if not q_out.is_contiguous() or q_out.dtype != qkv.dtype or q_out.numel() < T * num_heads * D:
-        raise RuntimeError("query_out must be contiguous [T, heads, head_dim] in the qkv dtype")
-    with _on(device):
-        stream, status = _stream_and_status(device)
-        check(lib().bs_rotary_append(
-            q2.data_ptr(), q2.stride(0), dtype_code(qkv.dtype),
-            frequencies.contiguous().data_ptr(), 2 * frequencies.numel(), 1 if interleaved else 0,
-            float(amplitude), positions.data_ptr(), slot_mapping.data_ptr(), T, num_heads, Hkv, D,
-            q_out.data_ptr(), key_pool.data_ptr(), value_pool.data_ptr(),
-            dtype_code(key_pool.dtype), NB, bs, status, stream))
-    return q_out
+    return _native.rotary_append(qkv, frequencies, positions, slot_mapping, key_pool, value_pool,
+                                 num_heads, interleaved, amplitude, query_out)
 
 
 def copy_blocks(key_pool: torch.Tensor, value_pool: torch.Tensor, src: torch.Tensor,
@@ -941,20 +794,4 @@ def copy_blocks(key_pool: torch.Tensor, value_pool: torch.Tensor, src: torch.Ten
     pair names too, as source or destination, is reported (``take_status``) and
     skipped, and so is one outside the pool.  Negative ends are padding.
     """
-    device = _require_cuda("copy_blocks", key_pool, value_pool, src, dst)
-    if key_pool.dim() not in (4, 5) or value_pool.shape != key_pool.shape \
-            or value_pool.dtype != key_pool.dtype:
-        raise RuntimeError("the pools must be [L, Hkv, NB, bs, D] of one shape and dtype")
-    if not (key_pool.is_contiguous() and value_pool.is_contiguous()):
-        raise RuntimeError("pools must be contiguous")
-    if src.numel() != dst.numel():
-        raise RuntimeError("src and dst must have one entry per pair")
-    n = src.numel()
-    src, dst = _int32_list("src", src, n), _int32_list("dst", dst, n)
-    layers = key_pool.size(0) if key_pool.dim() == 5 else 1
-    Hkv, NB, bs, D = key_pool.shape[-4:]
-    with _on(device):
-        stream, status = _stream_and_status(device)
-        check(lib().bs_copy_blocks(
-            key_pool.data_ptr(), value_pool.data_ptr(), dtype_code(key_pool.dtype), layers, Hkv, NB,
-            bs, D, src.data_ptr(), dst.data_ptr(), n, status, stream))
+    _native.copy_blocks(key_pool, value_pool, src, dst)
