@@ -104,9 +104,9 @@ int check_window_shape(const WindowShape& s) {
 }
 
 // Key ranges of the CUDA-core kernel: about four CTAs per SM in all, none of
-// fewer than 256 keys.
+// fewer than 128 keys (one group a warp).
 constexpr int64_t kMaxSimtSplits = 64;
-constexpr int64_t kMinSimtKeys = 256;
+constexpr int64_t kMinSimtKeys = 128;
 
 // How the CUDA-core kernel runs a call.
 struct SimtPlan {
@@ -128,7 +128,7 @@ int plan_simt(const WindowShape& s, SimtPlan* p) {
                                     p->tile_tokens);
   const int64_t want = p->items > 0 ? (4ll * sms + p->items - 1) / p->items : 1;
   p->splits = std::max<int64_t>(
-      1, std::min(std::min(want, kMaxSimtSplits), keys / kMinSimtKeys));
+      1, std::min(std::min(want, kMaxSimtSplits), (keys + kMinSimtKeys - 1) / kMinSimtKeys));
   if (p->items * p->splits > kInt32Max) p->splits = 1;
   const int64_t gm = p->tile_tokens * groups <= 8 ? 8 : bsb::kWindowSimtRows;
   p->rec_stride = gm * s.head_dim + 2 * gm;
@@ -423,7 +423,8 @@ int run_window(const WindowShape& s, const WindowCall& c) {
   a.splits = static_cast<int32_t>(p.splits);
   a.records = static_cast<float*>(c.workspace);
   a.rec_stride = static_cast<int32_t>(p.rec_stride);
-  const bool vec = (s.head_dim * dtype_size(s.dtype)) % 16 == 0 && aligned16(c.key_pool);
+  const bool vec = (s.head_dim * dtype_size(s.dtype)) % 16 == 0 && aligned16(c.key_pool) &&
+                   aligned16(c.value_pool);
   const int rc = bsb::launch_window_simt(a, s.dtype == BS_BF16, vec,
                                          static_cast<cudaStream_t>(c.stream));
   if (rc != 0) return cuda_fail(rc, "window attention launch");

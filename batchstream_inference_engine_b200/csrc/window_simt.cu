@@ -5,12 +5,15 @@
 // One CTA per (query tile, kv head, key range); the tile is one token, or as many
 // tokens of a chunk as fill 16 rows with their query heads, so each key row is
 // read once for all of them.  Each warp takes every fourth group of 32 keys: lane
-// j looks up key j of the group, the warp copies the group's K rows to shared
-// memory (16-byte loads), lane j computes key j's scores against the query rows
-// (fp32 in shared memory, read as broadcasts), the running softmax of a row comes
-// from warp reductions, and the weighted V rows are read straight from the pool
-// with lanes along head_dim (coalesced).  No barrier until the four warps' states
-// are combined at the end.
+// j looks up key j of the group, the warp starts asynchronous 16-byte copies of the
+// group's K rows, then of its V rows, into shared memory (so a group costs the
+// latency of its table entries and one of its rows, whatever their number), lane j
+// computes key j's scores against the query rows (fp32 in shared memory, read as
+// broadcasts), the running softmax of a row comes from warp reductions, and the V
+// rows are weighted with lanes along head_dim.  No barrier until the four warps'
+// states are combined at the end.  Rows of more than 512 bytes leave V in the pool
+// (its copy would not fit), and rows that are not whole 16-byte pieces are read one
+// element at a time.
 //
 // A weight of zero skips its V row, so NaN or infinities in a key that a row does
 // not see never reach that row.
@@ -41,28 +44,45 @@ __device__ __forceinline__ __nv_bfloat16 of_float<__nv_bfloat16>(float v) {
 }
 
 // 16 bytes of a row as floats.
-__device__ __forceinline__ void widen16(const float* p, float* out) {
-  *reinterpret_cast<float4*>(out) = *reinterpret_cast<const float4*>(p);
+__device__ __forceinline__ void widen16(const float* p, float (&out)[4]) {
+  const float4 v = *reinterpret_cast<const float4*>(p);
+  out[0] = v.x; out[1] = v.y; out[2] = v.z; out[3] = v.w;
 }
-__device__ __forceinline__ void widen16(const __nv_bfloat16* p, float* out) {
-  float v[8];
-  load8(p, v);
-  reinterpret_cast<float4*>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
+__device__ __forceinline__ void widen16(const __nv_bfloat16* p, float (&out)[8]) { load8(p, out); }
+
+__device__ __forceinline__ void copy16_async(void* smem_dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem_dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Floats of one K row in shared memory: lanes read the rows in parallel, so the
-// pad moves consecutive rows to different banks (four floats keep 16-byte reads
-// aligned).
-__host__ __device__ constexpr int row_floats(int head_dim, bool vec) {
-  return head_dim + (vec ? 4 : 1);
-}
-
-__host__ __device__ inline size_t simt_smem(int head_dim, int gm, bool vec) {
-  return sizeof(float) * (static_cast<size_t>(gm) * head_dim +
-                          kWarps * 32 * row_floats(head_dim, vec) + kWarps * 32 * gm +
-                          2 * kWarps * gm);
-}
+// Shared memory of one warp: 32 K rows, then 32 V rows where they fit; at the end its
+// state, GM rows of head_dim floats.  Lanes read K rows in parallel, so a pad of 16
+// bytes (one float in the element-wise form, which holds floats) moves consecutive
+// rows to different banks.
+template <typename T, int GM, int DPL, bool VEC>
+struct Layout {
+  static constexpr bool kStageV = VEC && DPL * 32 * sizeof(T) <= 512;
+  __host__ __device__ static int k_row(int D) {
+    return VEC ? D * static_cast<int>(sizeof(T)) + 16 : (D + 1) * 4;
+  }
+  __host__ __device__ static int v_row(int D) {
+    return kStageV ? D * static_cast<int>(sizeof(T)) : 0;
+  }
+  __host__ __device__ static int warp_bytes(int D) {
+    const int rows = 32 * (k_row(D) + v_row(D)), state = GM * D * 4;
+    return ((rows > state ? rows : state) + 15) / 16 * 16;
+  }
+  __host__ __device__ static int q_bytes(int D) { return (GM * D * 4 + 15) / 16 * 16; }
+  // Query rows | warps | probabilities [warp][32][GM] | maxima, sums [warp][GM].
+  __host__ __device__ static int total(int D) {
+    return q_bytes(D) + kWarps * (warp_bytes(D) + 32 * GM * 4 + 2 * GM * 4);
+  }
+};
 
 // Linear CTA index -> (sequence, query tile, kv head).
 __device__ __forceinline__ void window_item(const WindowArgs& a, int64_t item, int32_t& r,
@@ -73,10 +93,12 @@ __device__ __forceinline__ void window_item(const WindowArgs& a, int64_t item, i
   r = static_cast<int32_t>(item / a.qtiles);
 }
 
-// GM: query rows held per CTA; DPL: head dims per lane; VEC: 16-byte K rows.
-template <typename T, int GM, int DPL, bool VEC>
+// GM: query rows held per CTA; DPL: head dims per lane; VEC: 16-byte K rows; FULL:
+// head_dim is exactly 32 DPL (its loops then have compile-time bounds).
+template <typename T, int GM, int DPL, bool VEC, bool FULL>
 __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs a) {
-  extern __shared__ __align__(16) float wsm[];
+  using L_ = Layout<T, GM, DPL, VEC>;
+  extern __shared__ __align__(16) uint8_t wsm[];
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int32_t split = blockIdx.x % a.splits;
@@ -90,13 +112,16 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
   const int32_t begin = split * per;
   const int32_t end = w.count - begin < per ? w.count : begin + per;
 
-  const int G = a.groups, D = a.head_dim, bs = a.block_size;
+  const int G = a.groups, D = FULL ? 32 * DPL : a.head_dim, bs = a.block_size;
   const int rows = w.ntok * G;  // <= GM (host)
-  const int rf = row_floats(D, VEC);
-  float* sQ = wsm;
-  float* sK = sQ + GM * D + warp * 32 * rf;
-  float* sP = wsm + GM * D + kWarps * 32 * rf + warp * 32 * GM;
-  float* sM = wsm + GM * D + kWarps * 32 * rf + kWarps * 32 * GM;
+  float* sQ = reinterpret_cast<float*>(wsm);
+  uint8_t* states = wsm + L_::q_bytes(D);
+  const int warp_bytes = L_::warp_bytes(D), k_row = L_::k_row(D), v_row = L_::v_row(D);
+  uint8_t* sK = states + warp * warp_bytes;
+  uint8_t* sV = sK + 32 * k_row;
+  float* probs = reinterpret_cast<float*>(states + kWarps * warp_bytes);
+  float* sP = probs + warp * 32 * GM;
+  float* sM = probs + kWarps * 32 * GM;
   float* sL = sM + kWarps * GM;
 
   // Query rows: row t * G + g is head g of the kv head's group, token t.
@@ -137,44 +162,57 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
         set_status(a.status, kStatusBadBlock);
       }
     }
+    constexpr int kElems = 16 / sizeof(T);
     if constexpr (VEC) {
-      constexpr int kElems = 16 / sizeof(T);
+      // Copies of 16 bytes, consecutive lanes along a row; rows of no key stay as
+      // they are (their scores and weights are never used).
       const int per_row = D / kElems;
-      for (int it = 0; it < per_row; ++it) {
-        const int idx = it * 32 + lane;
-        const int key = idx / per_row, c = (idx - key * per_row) * kElems;
-        const int64_t ko = __shfl_sync(0xffffffffu, off, key);
-        float* dst = sK + key * rf + c;
-        if (ko >= 0) {
-          widen16(kh + ko + c, dst);
-        } else {
-#pragma unroll
-          for (int x = 0; x < kElems; ++x) dst[x] = 0.f;
+      for (int part = 0; part < (L_::kStageV ? 2 : 1); ++part) {
+        const T* from = part == 0 ? kh : vh;
+        uint8_t* to = part == 0 ? sK : sV;
+        const int stride = part == 0 ? k_row : v_row;
+#pragma unroll 4
+        for (int it = 0; it < per_row; ++it) {
+          const int idx = it * 32 + lane;
+          const int key = idx / per_row, c = idx - key * per_row;
+          const int64_t ko = __shfl_sync(0xffffffffu, off, key);
+          if (ko >= 0) copy16_async(to + key * stride + c * 16, from + ko + c * kElems);
         }
+        copy_commit();
       }
+      copy_wait<L_::kStageV ? 1 : 0>();
     } else {
       for (int key = 0; key < 32; ++key) {
         const int64_t ko = __shfl_sync(0xffffffffu, off, key);
-        for (int d = lane; d < D; d += 32) sK[key * rf + d] = ko >= 0 ? to_float<T>(kh[ko + d]) : 0.f;
+        if (ko < 0) continue;
+        float* dst = reinterpret_cast<float*>(sK + key * k_row);
+        for (int d = lane; d < D; d += 32) dst[d] = to_float<T>(kh[ko + d]);
       }
     }
     __syncwarp();
     float s[GM];
 #pragma unroll
     for (int i = 0; i < GM; ++i) s[i] = 0.f;
-    const float* krow = sK + lane * rf;
     if constexpr (VEC) {
-      for (int d = 0; d < D; d += 4) {
-        const float4 k4 = *reinterpret_cast<const float4*>(krow + d);
+      const T* krow = reinterpret_cast<const T*>(sK + lane * k_row);
+#pragma unroll 4
+      for (int d = 0; d < D; d += kElems) {
+        float k[kElems];
+        widen16(krow + d, k);
 #pragma unroll
         for (int i = 0; i < GM; ++i) {
           if (i < rows) {
-            const float4 q4 = *reinterpret_cast<const float4*>(sQ + i * D + d);
-            s[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[i]))));
+#pragma unroll
+            for (int x = 0; x < kElems; x += 4) {
+              const float4 q4 = *reinterpret_cast<const float4*>(sQ + i * D + d + x);
+              s[i] = fmaf(q4.x, k[x], fmaf(q4.y, k[x + 1],
+                                           fmaf(q4.z, k[x + 2], fmaf(q4.w, k[x + 3], s[i]))));
+            }
           }
         }
       }
     } else {
+      const float* krow = reinterpret_cast<const float*>(sK + lane * k_row);
       for (int d = 0; d < D; ++d) {
         const float kv = krow[d];
 #pragma unroll
@@ -185,7 +223,10 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
     }
 #pragma unroll
     for (int i = 0; i < GM; ++i) {
-      if (i >= rows) continue;
+      if (i >= rows) {
+        sP[lane * GM + i] = 0.f;
+        continue;
+      }
       const int32_t qpos = w.pos0 + i / G;
       const bool seen = off >= 0 && pos <= qpos && (pos < a.sinks || pos > qpos - a.window);
       const float z = seen ? s[i] * zscale : -INFINITY;
@@ -202,32 +243,44 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
       for (int k = 0; k < DPL; ++k) o[i][k] *= corr;
       sP[lane * GM + i] = p;
     }
+    if constexpr (L_::kStageV) copy_wait<0>();
     __syncwarp();
+    const uint32_t held = __ballot_sync(0xffffffffu, off >= 0);  // keys with a row
     const int nkeys = min(32, end - base);
 #pragma unroll 4
     for (int j = 0; j < nkeys; ++j) {
-      const int64_t vo = __shfl_sync(0xffffffffu, off, j);
-      if (vo < 0) continue;
+      if (!((held >> j) & 1u)) continue;
+      const int64_t vo = L_::kStageV ? 0 : __shfl_sync(0xffffffffu, off, j);
       float vv[DPL];
 #pragma unroll
       for (int k = 0; k < DPL; ++k) {
         const int d = lane + 32 * k;
-        vv[k] = d < D ? to_float<T>(vh[vo + d]) : 0.f;
+        if constexpr (L_::kStageV) {
+          vv[k] = FULL || d < D ? to_float<T>(reinterpret_cast<const T*>(sV + j * v_row)[d]) : 0.f;
+        } else {
+          vv[k] = FULL || d < D ? to_float<T>(vh[vo + d]) : 0.f;
+        }
       }
 #pragma unroll
-      for (int i = 0; i < GM; ++i) {
+      for (int i = 0; i < GM; i += 4) {
         if (i >= rows) continue;
-        const float p = sP[j * GM + i];
-        if (p != 0.f) {
+        // Rows past the tile's hold zeros.
+        const float4 p4 = *reinterpret_cast<const float4*>(sP + j * GM + i);
+        const float p[4] = {p4.x, p4.y, p4.z, p4.w};
 #pragma unroll
-          for (int k = 0; k < DPL; ++k) o[i][k] = fmaf(p, vv[k], o[i][k]);
+        for (int x = 0; x < 4; ++x) {
+          if (p[x] != 0.f) {
+#pragma unroll
+            for (int k = 0; k < DPL; ++k) o[i + x][k] = fmaf(p[x], vv[k], o[i + x][k]);
+          }
         }
       }
     }
     __syncwarp();  // the next group overwrites sK and sP
   }
 
-  // Each warp's state over its own K rows (32 * rf >= rows * D floats).
+  // Each warp's state over its own K and V rows.
+  float* state = reinterpret_cast<float*>(sK);
 #pragma unroll
   for (int i = 0; i < GM; ++i) {
     if (i >= rows) continue;
@@ -241,11 +294,10 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
 #pragma unroll
     for (int k = 0; k < DPL; ++k) {
       const int d = lane + 32 * k;
-      if (d < D) sK[i * D + d] = o[i][k];
+      if (d < D) state[i * D + d] = o[i][k];
     }
   }
   __syncthreads();
-  const float* states = wsm + GM * D;
   T* out = static_cast<T*>(a.out) + static_cast<int64_t>(w.tok0) * a.o_stride +
            static_cast<int64_t>(h) * G * D;
   float* rec = a.splits > 1 ? a.records + static_cast<int64_t>(blockIdx.x) * a.rec_stride : nullptr;
@@ -260,7 +312,7 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
     for (int x = 0; x < kWarps; ++x) {
       const float f = fast_exp2(sM[x * GM + i] - mb);
       L += sL[x * GM + i] * f;
-      O += states[x * 32 * rf + e] * f;
+      O += reinterpret_cast<const float*>(states + x * warp_bytes)[e] * f;
     }
     if (rec != nullptr) {
       rec[e] = O;
@@ -308,15 +360,16 @@ __global__ void __launch_bounds__(kThreads) window_simt_merge_kernel(const Windo
   }
 }
 
-template <typename T, int GM, int DPL, bool VEC>
+template <typename T, int GM, int DPL, bool VEC, bool FULL>
 int launch_one(const WindowArgs& a, cudaStream_t stream) {
-  const size_t smem = simt_smem(a.head_dim, GM, VEC);
-  auto kernel = window_simt_kernel<T, GM, DPL, VEC>;
+  using L_ = Layout<T, GM, DPL, VEC>;
+  const int smem = L_::total(a.head_dim);
+  auto kernel = window_simt_kernel<T, GM, DPL, VEC, FULL>;
   if (smem > 48 * 1024) {
     static unsigned long long configured = 0;  // one bit per device
     const cudaError_t e = once_per_device(&configured, [&] {
       return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  static_cast<int>(simt_smem(DPL * 32, GM, VEC)));
+                                  L_::total(DPL * 32));
     });
     if (e != cudaSuccess) return static_cast<int>(e);
   }
@@ -338,12 +391,18 @@ int launch_one(const WindowArgs& a, cudaStream_t stream) {
   return static_cast<int>(cudaLaunchKernelEx(&cfg, window_simt_merge_kernel<T, GM>, a));
 }
 
+template <typename T, int GM, int DPL, bool VEC>
+int launch_full(const WindowArgs& a, cudaStream_t stream) {
+  if (VEC && a.head_dim == 32 * DPL) return launch_one<T, GM, DPL, VEC, VEC>(a, stream);
+  return launch_one<T, GM, DPL, VEC, false>(a, stream);
+}
+
 template <typename T, int GM, bool VEC>
 int launch_dims(const WindowArgs& a, cudaStream_t stream) {
-  if (a.head_dim <= 32) return launch_one<T, GM, 1, VEC>(a, stream);
-  if (a.head_dim <= 64) return launch_one<T, GM, 2, VEC>(a, stream);
-  if (a.head_dim <= 128) return launch_one<T, GM, 4, VEC>(a, stream);
-  return launch_one<T, GM, 8, VEC>(a, stream);
+  if (a.head_dim <= 32) return launch_full<T, GM, 1, VEC>(a, stream);
+  if (a.head_dim <= 64) return launch_full<T, GM, 2, VEC>(a, stream);
+  if (a.head_dim <= 128) return launch_full<T, GM, 4, VEC>(a, stream);
+  return launch_full<T, GM, 8, VEC>(a, stream);
 }
 
 template <typename T>
