@@ -3,6 +3,8 @@
 // instruction each.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace bsb {
@@ -71,6 +73,28 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
       "r"(r[29]), "r"(r[30]), "r"(r[31]));
 }
 
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                 "=r"(r[6]), "=r"(r[7])
+               : "r"(addr));
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
+               "r"(r[7]));
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15]));
+}
+
 __device__ __forceinline__ void tmem_wait_ld() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -88,14 +112,64 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
-// A from TMEM (packed pairs along K, lane = row), B from shared memory.
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b,
-                                            uint32_t idesc, uint32_t accumulate) {
+// One lane of a converged warp (the same one each time).
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t mine;
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(
-          tmem_d),
-      "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0));
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(mine));
+  return mine;
+}
+
+// The products below are executed by the lanes with `mine` set, but called by the
+// whole warp: their operands are then warp-uniform values in uniform registers, where
+// the instruction takes them.  Inside an `if (lane == 0)` each operand has to be moved
+// there first, which made an issue take about 65 cycles.  Descriptors come as their
+// low word (start address and leading offset), to which the slice's offset is added
+// here (so that no loop keeps them all in registers), and the high word they share.
+template <uint32_t kOffA, uint32_t kOffB>
+__device__ __forceinline__ void umma_f16_elect(uint32_t mine, uint32_t tmem_d, uint32_t a_lo,
+                                               uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .b32 x, y;\n .reg .b64 a, b;\n"
+      " setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %6, 0;\n"
+      " add.u32 x, %1, %7;\n add.u32 y, %2, %8;\n mov.b64 a, {x, %3};\n mov.b64 b, {y, %3};\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}\n" ::"r"(tmem_d),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(mine), "n"(kOffA),
+      "n"(kOffB));
+}
+
+// A from TMEM (packed pairs along K, lane = row), B from shared memory.
+template <uint32_t kOffA, uint32_t kOffB>
+__device__ __forceinline__ void umma_f16_ts_elect(uint32_t mine, uint32_t tmem_d, uint32_t tmem_a,
+                                                  uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                                  uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .b32 x, y;\n .reg .b64 b;\n"
+      " setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %6, 0;\n"
+      " add.u32 x, %1, %7;\n add.u32 y, %2, %8;\n mov.b64 b, {y, %3};\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %4, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(mine), "n"(kOffA),
+      "n"(kOffB));
+}
+
+// Calls fn(std::integral_constant) for 0 .. N - 1.
+template <int N, typename Fn, int I = 0>
+__device__ __forceinline__ void unroll(Fn&& fn) {
+  if constexpr (I < N) {
+    fn(std::integral_constant<int, I>());
+    unroll<N, Fn, I + 1>(static_cast<Fn&&>(fn));
+  }
+}
+
+__device__ __forceinline__ void umma_commit_elect(uint32_t mine, uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(
+          smem_u32(bar)),
+      "r"(mine)
+      : "memory");
 }
 
 }  // namespace bsb

@@ -13,17 +13,19 @@
 // TMA box per K, V and 64 dims through the block table, so sink units and window
 // units share a step and nothing between them is touched.
 //
-// Roles (11 warps, one CTA per SM):
-//   * softmax A (warps 0-3) and B (warps 4-7), one thread per query row: S from
-//     TMEM, mask on border steps only, base-2 online softmax in fp32 whose maximum
-//     moves only when it grows by more than 2^8 (then O is rescaled in TMEM), P
-//     rounded to bf16 (the tensor cores' input) over the first half of S's columns;
-//   * MMA (warp 8, one thread): per step, for A then B: O += P V of the step before
+// Roles (19 warps, one CTA per SM):
+//   * softmax A (warps 0-7) and B (warps 8-15), two threads per query row, 64 of a
+//     step's keys each (four warps a tile spend half of a step waiting for their own
+//     loads and exponentials): S from TMEM, mask on border steps only, the row's
+//     maximum exchanged through shared memory, base-2 online softmax in fp32 whose
+//     maximum moves only when it grows by more than 2^8 (then O is rescaled in TMEM),
+//     P rounded to bf16 (the tensor cores' input) over the first half of S's columns;
+//   * MMA (warp 16, one thread): per step, for A then B: O += P V of the step before
 //     (P from TMEM), S = Q K^T of this one over P's columns (the products of one
 //     thread execute in order), one commit.  While one tile's softmax runs, the
 //     tensor core works for the other;
-//   * loader (warp 9);
-//   * guard (warp 10): on border steps it zeroes the V rows that no row of the CTA
+//   * loader (warp 17);
+//   * guard (warp 18): on border steps it zeroes the V rows that no row of the CTA
 //     sees (never-loaded or stale memory, which 0 * NaN would let through), and the
 //     non-finite elements of the others, whose keys it lists: rows that do see such a
 //     key get its non-finite values added at the end, rows that do not stay clean.
@@ -48,8 +50,10 @@ constexpr int kRows = 128;  // query rows of a tile (TMEM lanes)
 constexpr int kKeys = 128;  // keys of a step
 constexpr int kUnit = 16;   // tokens per unit (one TMA box)
 constexpr int kUnits = kKeys / kUnit;
-constexpr int kThreads = 352;
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kGuardWarp = 10;
+constexpr int kSoftWarps = 8;            // softmax warps of a tile
+constexpr int kTileThreads = kSoftWarps * 32;
+constexpr int kThreads = 2 * kTileThreads + 96;
+constexpr int kMmaWarp = 16, kLoadWarp = 17, kGuardWarp = 18;
 constexpr int kRing = 4;  // step barriers per tile (> K stages, > V stages + 1)
 constexpr uint32_t kTmemCols = 512;  // S/P of A, S/P of B, O of A, O of B
 constexpr float kLog2eP = 1.4426950408889634f;
@@ -63,17 +67,27 @@ struct Cfg {
   static constexpr int VS = D == 64 ? 3 : 2;  // V stages
   static constexpr int HALF_BYTES = kKeys * 128;  // 64 dims of 128 rows
   static constexpr int TILE_BYTES = HALVES * HALF_BYTES;
-  static constexpr int SMEM_BYTES = 1024 + (2 + KS + VS) * TILE_BYTES;
+  // With the barriers and exchange buffers (3 KiB) all of the 227 KiB at 128.
+  static constexpr int SMEM_BYTES = (2 + KS + VS) * TILE_BYTES;
   static constexpr uint32_t O_COL = 256;
   static_assert(KS <= kRing && VS + 1 <= kRing, "a step waiter could fall a whole ring behind");
 };
 
-// The steps of a CTA's key range and which of them each tile needs.
+// One tile's tokens and the steps that hold keys of its windows.  (Plain members and
+// selects: an array indexed by the tile would live in local memory, which this
+// kernel's shared memory leaves no L1 cache for.)
+struct TileSteps {
+  int32_t used;        // it holds tokens
+  int32_t pos0, pos1;  // first and last position of its tokens
+  int32_t first, last;
+};
+
+// The steps of a CTA's key range.
 struct Steps {
   int32_t sink_units, first_unit, units;
-  int32_t pos0[2], pos1[2];  // first and last position of the tiles' tokens
-  int32_t last[2], first[2];  // their last and first step with window keys
-  int32_t tiles;             // tiles with tokens (1 or 2)
+  TileSteps a, b;
+  __device__ __forceinline__ TileSteps tile(int x) const { return x == 0 ? a : b; }
+  __device__ __forceinline__ int32_t tiles() const { return b.used ? 2 : 1; }
 };
 
 __device__ __forceinline__ Steps steps_of(const WindowArgs& a, const WindowTile& w, int32_t tt) {
@@ -82,17 +96,13 @@ __device__ __forceinline__ Steps steps_of(const WindowArgs& a, const WindowTile&
   s.sink_units = min((a.sinks + kUnit - 1) / kUnit, s.first_unit);
   const int32_t end = w.pos0 + w.ntok - 1;
   s.units = s.sink_units + end / kUnit - s.first_unit + 1;
-  s.tiles = w.ntok > tt ? 2 : 1;
-  s.pos0[0] = w.pos0;
-  s.pos1[0] = min(end, w.pos0 + tt - 1);
-  s.pos0[1] = w.pos0 + tt;
-  s.pos1[1] = end;
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int32_t lo = max(0, s.pos0[x] - a.window + 1);
-    s.first[x] = (s.sink_units + lo / kUnit - s.first_unit) / kUnits;
-    s.last[x] = (s.sink_units + s.pos1[x] / kUnit - s.first_unit) / kUnits;
-  }
+  auto tile = [&](int32_t used, int32_t pos0, int32_t pos1) {
+    const int32_t lo = max(0, pos0 - a.window + 1);
+    return TileSteps{used, pos0, pos1, (s.sink_units + lo / kUnit - s.first_unit) / kUnits,
+                     (s.sink_units + pos1 / kUnit - s.first_unit) / kUnits};
+  };
+  s.a = tile(1, w.pos0, min(end, w.pos0 + tt - 1));
+  s.b = tile(w.ntok > tt ? 1 : 0, w.pos0 + tt, end);
   return s;
 }
 
@@ -105,19 +115,34 @@ __device__ __forceinline__ int32_t unit_pos(const Steps& s, int32_t x) {
   return (x < s.sink_units ? x : x - s.sink_units + s.first_unit) * kUnit;
 }
 
-// Whether tile x has keys in step j.
-__device__ __forceinline__ bool step_active(const Steps& s, int x, int32_t j) {
-  return x < s.tiles && j <= s.last[x] && (j >= s.first[x] || j * kUnits < s.sink_units);
+// Whether a tile has keys in step j.
+__device__ __forceinline__ bool step_active(const Steps& s, const TileSteps& t, int32_t j) {
+  return t.used && j <= t.last && (j >= t.first || j * kUnits < s.sink_units);
 }
 
-// Whether some row of tile x does not see some key of step j.
-__device__ __forceinline__ bool step_masked(const WindowArgs& a, const Steps& s, int x,
-                                            int32_t j) {
+// Whether some row of a tile does not see some key of step j.
+__device__ __forceinline__ bool step_masked(const WindowArgs& a, const Steps& s,
+                                            const TileSteps& t, int32_t j) {
   const int32_t u0 = j * kUnits, u1 = u0 + kUnits - 1;
-  if (u1 >= s.units || unit_pos(s, u1) + kUnit - 1 > s.pos0[x]) return true;
+  if (u1 >= s.units || unit_pos(s, u1) + kUnit - 1 > t.pos0) return true;
   if (u0 < s.sink_units && a.sinks < min(u1 + 1, s.sink_units) * kUnit) return true;
   // The step's first window unit against the last row's window.
-  return u1 >= s.sink_units && unit_pos(s, max(u0, s.sink_units)) <= s.pos1[x] - a.window;
+  return u1 >= s.sink_units && unit_pos(s, max(u0, s.sink_units)) <= t.pos1 - a.window;
+}
+
+// A shared copy of a value, read anew (the softmax threads keep 64 scores in their 96
+// registers: what they need once a step stays in shared memory).
+template <typename T>
+__device__ __forceinline__ T reread(const T& shared) {
+  static_assert(sizeof(T) % 4 == 0, "words");
+  T v;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T) / 4); ++i) {
+    asm volatile("ld.shared.u32 %0, [%1];"
+                 : "=r"(reinterpret_cast<uint32_t*>(&v)[i])
+                 : "r"(smem_u32(&shared) + 4 * i));
+  }
+  return v;
 }
 
 __device__ __forceinline__ bool sees(const WindowArgs& a, int32_t qpos, int32_t pos) {
@@ -140,20 +165,28 @@ __device__ __forceinline__ void pair_of(const WindowArgs& a, int32_t item, int32
   tile = a.qtiles - 1 - item / a.num_rows;
 }
 
+// a * 0 + c on bf16 pairs.
+__device__ __forceinline__ uint32_t fma_zero_bf16x2(uint32_t a, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(0u), "r"(c));
+  return d;
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
     window_prefill_kernel(const __grid_constant__ CUtensorMap qmap,
                           const __grid_constant__ CUtensorMap kmap,
                           const __grid_constant__ CUtensorMap vmap, const WindowArgs a) {
   using C = Cfg<D>;
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem[];  // 128-byte swizzle atoms
   __shared__ uint64_t q_full, k_full[C::KS], v_full[C::VS], v_ok[C::VS], step_done[2][kRing],
       p_full[2], mma_done;
   __shared__ uint32_t tmem_base;
   __shared__ int32_t bad_count, bad_pos[kMaxBad];
+  // The halves' row maxima of a step, and at the end their row sums.
+  __shared__ float exchange[2][2][kRows];
+  __shared__ Steps shared_steps;
 
-  const uint32_t raw = smem_u32(smem_raw);
-  uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   auto sQ = [&](int x) { return smem + x * C::TILE_BYTES; };
   auto sK = [&](int st) { return smem + (2 + st) * C::TILE_BYTES; };
   auto sV = [&](int st) { return smem + (2 + C::KS + st) * C::TILE_BYTES; };
@@ -183,11 +216,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int x = 0; x < 2; ++x) {
       for (int s = 0; s < kRing; ++s) mbar_init(&step_done[x][s], 1);
-      mbar_init(&p_full[x], kRows);
+      mbar_init(&p_full[x], kTileThreads);
     }
     mbar_init(&mma_done, 1);
     fence_barrier_init();
     bad_count = 0;
+    shared_steps = sd;
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -230,8 +264,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int32_t y = fetch(0), y_next = fetch(1);
     if (lane == 0) {
       const uint32_t rows = static_cast<uint32_t>(tt * a.groups);
-      mbar_arrive_expect_tx(&q_full, sd.tiles * C::HALVES * rows * 128u);
-      for (int x = 0; x < sd.tiles; ++x) {
+      mbar_arrive_expect_tx(&q_full, sd.tiles() * C::HALVES * rows * 128u);
+      for (int x = 0; x < sd.tiles(); ++x) {
         for (int hf = 0; hf < C::HALVES; ++hf) {
           tma_load_3d(sQ(x) + hf * C::HALF_BYTES, &qmap, &q_full, hf * 64, h * a.groups,
                       w.tok0 + x * tt);
@@ -277,51 +311,54 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------------------------------------------------------- MMA issuer
     constexpr uint32_t kIdescS = umma_idesc(128, kKeys, 0, 0);
     constexpr uint32_t kIdescO = umma_idesc(128, D, 0, 1);
-    constexpr uint64_t kTileStep = C::TILE_BYTES >> 4, kHalfStep = C::HALF_BYTES >> 4;
+    constexpr uint32_t kTileStep = C::TILE_BYTES >> 4, kHalfStep = C::HALF_BYTES >> 4;
     const uint64_t desc_q = umma_desc(smem_u32(sQ(0)), 16, 1024);
-    const uint64_t desc_k = umma_desc(smem_u32(sK(0)), 16, 1024);
+    const uint32_t hi = static_cast<uint32_t>(desc_q >> 32);  // of every operand
+    const uint32_t q_lo = static_cast<uint32_t>(desc_q);
+    const uint32_t k_lo = static_cast<uint32_t>(umma_desc(smem_u32(sK(0)), 16, 1024));
     // V: dims contiguous (MN-major): 64-dim halves HALF_BYTES apart, 8 keys 1024.
-    const uint64_t desc_v = umma_desc(smem_u32(sV(0)), C::HALF_BYTES, 1024);
+    const uint32_t v_lo =
+        static_cast<uint32_t>(umma_desc(smem_u32(sV(0)), C::HALF_BYTES, 1024));
+    const uint32_t mine = elect_lane();  // issues every product
     bool ok = wait_all(&q_full, 0);
-    int32_t done[2] = {0, 0};  // P tiles consumed, by tile
+    int32_t done_a = 0, done_b = 0;  // P tiles consumed
     for (int32_t u = 0; u <= n && ok; ++u) {
-      for (int x = 0; x < 2 && ok; ++x) {
-        const bool pv = u > 0 && step_active(sd, x, j0 + u - 1);
-        const bool qk = u < n && step_active(sd, x, j0 + u);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const TileSteps& ts = x == 0 ? sd.a : sd.b;
+        int32_t& done = x == 0 ? done_a : done_b;
+        const bool pv = u > 0 && step_active(sd, ts, j0 + u - 1);
+        const bool qk = u < n && step_active(sd, ts, j0 + u);
         const int32_t vs = (u - 1) % C::VS, ks = u % C::KS;
         if (pv) {
-          ok = wait_all(&p_full[x], done[x] & 1) &&
+          ok = wait_all(&p_full[x], done & 1) &&
                wait_all(&v_ok[vs], ((u - 1) / C::VS) & 1);
         }
         if (ok && qk) ok = wait_all(&k_full[ks], (u / C::KS) & 1);
         if (!ok) break;
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t s_col = tmem + x * kKeys;
-          if (pv) {
-            const uint64_t v0 = desc_v + vs * kTileStep;
-#pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k) {
-              umma_f16_ts(tmem + C::O_COL + x * D, s_col + 8 * k, v0 + 128 * k, kIdescO,
-                          (done[x] > 0 || k > 0) ? 1u : 0u);
-            }
-          }
-          if (qk) {
-            const uint64_t q0 = desc_q + x * kTileStep, k0 = desc_k + ks * kTileStep;
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint64_t off = (k / 4) * kHalfStep + 2 * (k % 4);
-              umma_f16(s_col, q0 + off, k0 + off, kIdescS, k > 0 ? 1u : 0u);
-            }
-          }
-          umma_commit(&step_done[x][u % kRing]);
+        const uint32_t s_col = tmem + x * kKeys;
+        if (pv) {
+          const uint32_t v0 = v_lo + vs * kTileStep;
+          unroll<kKeys / 16>([&](auto k) {
+            // P: 8 columns per 16 keys; V: 16 rows of 128 bytes.
+            umma_f16_ts_elect<8 * k, 128 * k>(mine, tmem + C::O_COL + x * D, s_col, v0, hi,
+                                              kIdescO, (done > 0 || k > 0) ? 1u : 0u);
+          });
         }
-        if (pv) ++done[x];
+        if (qk) {
+          const uint32_t q0 = q_lo + x * kTileStep, k0 = k_lo + ks * kTileStep;
+          unroll<D / 16>([&](auto k) {
+            constexpr uint32_t off = (k / 4) * kHalfStep + 2 * (k % 4);  // 32 bytes a slice
+            umma_f16_elect<off, off>(mine, s_col, q0, k0, hi, kIdescS, k > 0 ? 1u : 0u);
+          });
+        }
+        umma_commit_elect(mine, &step_done[x][u % kRing]);
+        if (pv) ++done;
         __syncwarp();
       }
     }
-    if (lane == 0) umma_commit(&mma_done);
-    __syncwarp();
+    umma_commit_elect(mine, &mma_done);
     const bool drained = wait_all(&mma_done, 0);
     if ((!ok || !drained) && lane == 0) set_status(a.status, kStatusWaitTimeout);
   } else if (warp == kGuardWarp) {
@@ -332,44 +369,65 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int vs = j % C::VS;
       ok = wait_all(&v_full[vs], (j / C::VS) & 1);
       if (!ok) break;
-      bool border = false;
-      for (int x = 0; x < sd.tiles; ++x) {
-        border |= step_active(sd, x, j0 + j) && step_masked(a, sd, x, j0 + j);
-      }
+      const bool border =
+          (step_active(sd, sd.a, j0 + j) && step_masked(a, sd, sd.a, j0 + j)) ||
+          (step_active(sd, sd.b, j0 + j) && step_masked(a, sd, sd.b, j0 + j));
       if (border) {
-        // Lane = (row of a group of 4, 16-byte column of a 128-byte row).
-        for (int g = 0; g < kKeys / 4; ++g) {
-          const int row = g * 4 + (lane >> 3), col = lane & 7;
-          const int32_t x = (j0 + j) * kUnits + row / kUnit;
-          const int32_t pos = unit_pos(sd, x) + row % kUnit;
-          const bool live = x < sd.units && pos <= end && (pos < a.sinks || pos >= w.lo);
-          bool bad = false;
-#pragma unroll
-          for (int hf = 0; hf < C::HALVES; ++hf) {
-            uint4* p = reinterpret_cast<uint4*>(sV(vs) + hf * C::HALF_BYTES + row * 128 + col * 16);
-            if (!live) {
-              *p = make_uint4(0u, 0u, 0u, 0u);
-              continue;
+        auto position = [&](int row) {  // of the key of a V row
+          return unit_pos(sd, (j0 + j) * kUnits + row / kUnit) + row % kUnit;
+        };
+        // Rows that no query row sees become zero, lane = row.
+        for (int g = 0; g < kKeys / 32; ++g) {
+          const int row = g * 32 + lane;
+          const int32_t pos = position(row);
+          const bool live = (j0 + j) * kUnits + row / kUnit < sd.units && pos <= end &&
+                            (pos < a.sinks || pos >= w.lo);
+          if (!live) {
+            for (int c = 0; c < 8 * C::HALVES; ++c) {
+              *reinterpret_cast<uint4*>(sV(vs) + (c / 8) * C::HALF_BYTES + row * 128 +
+                                        (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
-            uint4 v = *p;
-            uint32_t* e = reinterpret_cast<uint32_t*>(&v);
-            bool hit = false;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              // All exponent bits set: infinity or NaN.
-              uint32_t keep = 0xffffffffu;
-              if ((e[i] & 0x7f80u) == 0x7f80u) keep &= 0xffff0000u;
-              if ((e[i] & 0x7f800000u) == 0x7f800000u) keep &= 0x0000ffffu;
-              hit |= keep != 0xffffffffu;
-              e[i] &= keep;
-            }
-            if (hit) *p = v;
-            bad |= hit;
           }
-          const uint32_t any = __ballot_sync(0xffffffffu, bad);
-          if (any != 0 && col == 0 && ((any >> (lane & ~7)) & 0xffu) != 0) {
-            const int32_t at = atomicAdd(&bad_count, 1);
-            if (at < kMaxBad) bad_pos[at] = pos;
+        }
+        __syncwarp();
+        // x * 0 is 0 or, for infinities and NaN, NaN, and stays NaN in the sum.
+        uint32_t sum = 0;
+#pragma unroll 8
+        for (int c = 0; c < C::TILE_BYTES / 512; ++c) {
+          const uint4 v = *reinterpret_cast<const uint4*>(sV(vs) + (c * 32 + lane) * 16);
+          sum = fma_zero_bf16x2(v.x, sum);
+          sum = fma_zero_bf16x2(v.y, sum);
+          sum = fma_zero_bf16x2(v.z, sum);
+          sum = fma_zero_bf16x2(v.w, sum);
+        }
+        if (__any_sync(0xffffffffu, sum != 0u)) {
+          // Lane = (row of a group of 4, 16-byte column of a 128-byte row).
+          for (int g = 0; g < kKeys / 4; ++g) {
+            const int row = g * 4 + (lane >> 3), col = lane & 7;
+            bool bad = false;
+            for (int hf = 0; hf < C::HALVES; ++hf) {
+              uint4* p =
+                  reinterpret_cast<uint4*>(sV(vs) + hf * C::HALF_BYTES + row * 128 + col * 16);
+              uint4 v = *p;
+              uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+              bool hit = false;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                // All exponent bits set: infinity or NaN.
+                uint32_t keep = 0xffffffffu;
+                if ((e[i] & 0x7f80u) == 0x7f80u) keep &= 0xffff0000u;
+                if ((e[i] & 0x7f800000u) == 0x7f800000u) keep &= 0x0000ffffu;
+                hit |= keep != 0xffffffffu;
+                e[i] &= keep;
+              }
+              if (hit) *p = v;
+              bad |= hit;
+            }
+            const uint32_t any = __ballot_sync(0xffffffffu, bad);
+            if (col == 0 && ((any >> (lane & ~7)) & 0xffu) != 0) {
+              const int32_t at = atomicAdd(&bad_count, 1);
+              if (at < kMaxBad) bad_pos[at] = position(row);
+            }
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -381,77 +439,80 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok && lane == 0) set_status(a.status, kStatusWaitTimeout);
   } else {
     // ---------------------------------------------------------------- softmax
-    const int x = warp >> 2;
+    const int x = warp / kSoftWarps, hf = (warp >> 2) & 1;  // tile, half of the keys
     const int row = tid & (kRows - 1);
     const int32_t tok = row / a.groups, g = row - tok * a.groups;
     const bool live = x * tt + tok < w.ntok && tok < tt;
     const int32_t qpos = w.pos0 + x * tt + tok;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lane_base + x * kKeys;
-    const uint32_t o_addr = tmem + lane_base + C::O_COL + x * D;
+    const uint32_t o_addr = tmem + lane_base + C::O_COL + x * D + hf * (D / 2);  // its half
+    // Barrier of the tile's warps; true when it is for all of them.  A wait that gave
+    // up in one warp ends the loop in all at once: none is left at a barrier.
+    auto tile_all = [&](bool mine) {
+      uint32_t all;
+      asm volatile(
+          "{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n"
+          " barrier.cta.red.and.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+          : "=r"(all)
+          : "r"(1 + x), "r"(kTileThreads), "r"(mine ? 1u : 0u)
+          : "memory");
+      return all != 0;
+    };
     const float zscale = fabsf(a.scale) * kLog2eP;
     float m_used = -INFINITY, l_run = 0.f;
     int32_t done = 0;
     bool ok = true;
     for (int32_t u = 0; u < n; ++u) {
-      ok = wait_step(x, u);
-      if (!ok) break;
-      if (!step_active(sd, x, j0 + u)) continue;
+      bool border;
+      {
+        const Steps st = reread(shared_steps);
+        const TileSteps ts = st.tile(x);
+        const bool active = step_active(st, ts, j0 + u);
+        border = step_masked(a, st, ts, j0 + u);
+        ok = ok && wait_step(x, u);
+        if (!active) continue;
+      }
       tc_fence_after();
       // Visible tokens of the step's units, 16 bits each (border steps only).
-      const bool border = step_masked(a, sd, x, j0 + u);
-      uint32_t maps[kUnits / 2];
+      uint32_t maps[2];
       if (border) {
         auto below = [](int32_t c) -> uint32_t {  // map of the first c tokens
           return c >= kUnit ? 0xffffu : c <= 0 ? 0u : (1u << c) - 1u;
         };
+        const Steps st = reread(shared_steps);
 #pragma unroll
-        for (int un = 0; un < kUnits; ++un) {
-          const int32_t ux = (j0 + u) * kUnits + un;
-          const int32_t p0 = unit_pos(sd, ux);
+        for (int un = 0; un < kUnits / 2; ++un) {
+          const int32_t ux = (j0 + u) * kUnits + hf * (kUnits / 2) + un;
+          const int32_t p0 = unit_pos(st, ux);
           uint32_t map = below(qpos - p0 + 1) &
                          (~below(qpos - a.window + 1 - p0) | below(a.sinks - p0));
-          if (ux >= sd.units || !live) map = 0;
+          if (ux >= st.units || !live) map = 0;
           maps[un / 2] = un % 2 ? maps[un / 2] | (map << 16) : map;
         }
       }
-      // Scores of columns 32 c .. 32 c + 31: a negative scale turns them around (the
-      // rest works with its magnitude), unseen keys become -inf.
-      auto scores = [&](int c, uint32_t (&v)[32]) {
-        if (a.scale < 0.f) {
+      uint32_t v[2][32];
+      tmem_ld32(s_addr + hf * 64, v[0]);
+      tmem_ld32(s_addr + hf * 64 + 32, v[1]);
+      tmem_wait_ld();
+      if (a.scale < 0.f) {  // turned around: the rest works with the scale's magnitude
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] ^= 0x80000000u;
-        }
-        if (border) {
+        for (int i = 0; i < 64; ++i) v[i / 32][i % 32] ^= 0x80000000u;
+      }
+      if (border) {  // unseen keys become -inf
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (!((maps[c] >> i) & 1u)) v[i] = 0xff800000u;
-          }
+        for (int i = 0; i < 64; ++i) {
+          if (!((maps[i / 32] >> (i % 32)) & 1u)) v[i / 32][i % 32] = 0xff800000u;
         }
-      };
+      }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      auto maximum = [&](const uint32_t (&v)[32]) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i]));
-      };
-      // 128 scores, their map and the packed P do not fit in the 168 registers a
-      // thread has: columns 0 .. 63 are read for the maximum, then again.
-      uint32_t v0[32], v1[32];
-      tmem_ld32(s_addr, v0);
-      tmem_ld32(s_addr + 32, v1);
-      tmem_wait_ld();
-      scores(0, v0);
-      maximum(v0);
-      scores(1, v1);
-      maximum(v1);
-      tmem_ld32(s_addr + 64, v0);
-      tmem_ld32(s_addr + 96, v1);
-      tmem_wait_ld();
-      scores(2, v0);
-      maximum(v0);
-      scores(3, v1);
-      maximum(v1);
-      const float m_step = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * zscale;
+      for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i / 32][i % 32]));
+      const float m_half = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      exchange[x][hf][row] = m_half;
+      ok = tile_all(ok);  // also: every score is read before P takes columns 0 .. 63
+      if (!ok) break;
+      const float m_step = fmaxf(m_half, exchange[x][hf ^ 1][row]) * zscale;
       const bool grow = live && m_step > m_used + kRescaleSlack;
       if (done == 0) {
         m_used = m_step;
@@ -460,56 +521,47 @@ __global__ void __launch_bounds__(kThreads, 1)
         // that did not grow keep theirs (factor 1).
         const float m_new = grow ? m_step : m_used;
         const float corr = grow ? fast_exp2(m_used - m_new) : 1.f;
-#pragma unroll
-        for (int c0 = 0; c0 < D; c0 += 32) {
-          uint32_t o[32];
-          tmem_ld32(o_addr + c0, o);
+#pragma unroll 1
+        for (int c0 = 0; c0 < D / 2; c0 += 8) {  // few columns: the scores stay in registers
+          uint32_t o[8];
+          tmem_ld8(o_addr + c0, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
-          tmem_st32(o_addr + c0, o);
+          for (int c = 0; c < 8; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
+          tmem_st8(o_addr + c0, o);
         }
         l_run *= corr;
         m_used = m_new;
       }
       const float m_base = m_used == -INFINITY ? 0.f : m_used;  // no -inf - -inf
       const float2 zs2 = make_float2(zscale, zscale), mm = make_float2(-m_base, -m_base);
-      float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
-                       make_float2(0.f, 0.f)};
-      // Probabilities of 32 columns, packed into 16.
-      auto weights = [&](const uint32_t (&v)[32], uint32_t* p) {
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t p[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float2 e = __ffma2_rn(
-              make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), zs2, mm);
+              make_float2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), zs2, mm);
           const float2 pe = make_float2(fast_exp2(e.x), fast_exp2(e.y));
-          sum[i & 3] = __fadd2_rn(sum[i & 3], pe);
+          sum[i & 1] = __fadd2_rn(sum[i & 1], pe);
           p[i] = pack_bf16x2(pe.x, pe.y);
         }
-      };
-      uint32_t p[32];
-      weights(v0, p);
-      weights(v1, p + 16);
-      tmem_ld32(s_addr, v0);
-      tmem_ld32(s_addr + 32, v1);
-      tmem_wait_ld();  // before P takes the place of columns 32 .. 63
-      tmem_st32(s_addr + 32, p);
-      scores(0, v0);
-      scores(1, v1);
-      weights(v0, p);
-      weights(v1, p + 16);
-      tmem_st32(s_addr, p);
+        tmem_st16(s_addr + hf * 32 + c * 16, p);
+      }
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&p_full[x]);
-      l_run += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) +
-               ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
+      l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       ++done;
     }
-    if (ok) ok = wait_step(x, n);  // the last P V is done
+    ok = ok && wait_step(x, n);  // the last P V is done
+    exchange[x][hf][row] = l_run;
+    ok = tile_all(ok);
+    l_run += exchange[x][hf ^ 1][row];
     if (!ok) {
       if (lane == 0) set_status(a.status, kStatusWaitTimeout);
-    } else if (x < sd.tiles) {
+    } else if (sd.tile(x).used) {
       tc_fence_after();
       const bool split_up = ranges > 1;
       // Listed keys are complete: the guard arrived for every V that was used.
@@ -519,10 +571,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t rec_row = (static_cast<int64_t>(item) * a.splits + split) * 2 * kRows +
                               x * kRows + row;
 #pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 32) {
+      for (int cc = 0; cc < D / 2; cc += 32) {
+        const int c0 = hf * (D / 2) + cc;  // this thread's columns of the head
         uint32_t v[32];
         if (done > 0) {
-          tmem_ld32(o_addr + c0, v);
+          tmem_ld32(o_addr + cc, v);
           tmem_wait_ld();
         } else {
 #pragma unroll
@@ -577,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (split_up && live) {
+      if (split_up && live && hf == 0) {
         float* ml = a.records + a.rec_stride_ml + rec_row * 2;
         *reinterpret_cast<float2*>(ml) = make_float2(m_used, l_run);
       }
