@@ -228,7 +228,7 @@ int plan_mma_chunks(const WindowShape& s, MmaChunkPlan* p) {
   const int64_t keys = std::min(s.max_blocks * s.block_size,
                                 std::min(s.window, kMaxContext) + std::min(s.sinks, kMaxContext) +
                                     p->tile_tokens + 32);
-  const int64_t most = (keys + 127) / 128 / bsb::kMinWindowSteps;
+  const int64_t most = keys / (bsb::kWindowStepKeys * bsb::kMinWindowSteps);
   const int64_t record = bsb::kWindowPairRows * (s.head_dim + 2) * 4;
   p->splits = std::max<int64_t>(
       1, std::min(std::min<int64_t>(sms / busy, bsb::kMaxWindowRanges), most));

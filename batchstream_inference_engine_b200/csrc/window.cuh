@@ -106,10 +106,11 @@ __host__ __device__ __forceinline__ int32_t window_range(int32_t count, int32_t 
 // Query rows (tokens x heads of one kv head) of a tile of the CUDA-core kernel.
 constexpr int kWindowSimtRows = 16;
 
-// Tensor-core chunks: rows of a record (two query tiles), the fewest steps of 128
+// Tensor-core chunks: rows of a record (two query tiles), the fewest steps of 64
 // keys in a range and the most ranges.
 constexpr int kWindowPairRows = 256;
-constexpr int kMinWindowSteps = 2;
+constexpr int kWindowStepKeys = 64;
+constexpr int kMinWindowSteps = 4;
 constexpr int kMaxWindowRanges = 8;
 
 int launch_window_prefill(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& kmap,

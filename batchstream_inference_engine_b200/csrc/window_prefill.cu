@@ -6,33 +6,32 @@
 // G query heads of one kv head, so every K and V row that a CTA loads serves the
 // whole group, and the keys a tile reads beyond its window are those of a few
 // tokens (18 at G = 7) instead of 128.  One CTA takes two such tiles (A and B, the
-// tokens next to each other) over the same keys, in steps of 128 keys.
+// tokens next to each other) over the same keys, in steps of 64 keys.
 //
 // The keys a CTA reads are 16-token units: the sink units, then the window's from
-// the first token any row sees to the last row's own.  A step is 8 units, each one
+// the first token any row sees to the last row's own.  A step is 4 units, each one
 // TMA box per K, V and 64 dims through the block table, so sink units and window
 // units share a step and nothing between them is touched.
 //
-// Roles (19 warps, one CTA per SM):
-//   * softmax A (warps 0-7) and B (warps 8-15), two threads per query row, 64 of a
-//     step's keys each (four warps a tile spend half of a step waiting for their own
-//     loads and exponentials): S from TMEM, mask on border steps only, the row's
-//     maximum exchanged through shared memory, base-2 online softmax in fp32 whose
-//     maximum moves only when it grows by more than 2^8 (then O is rescaled in TMEM),
-//     P rounded to bf16 (the tensor cores' input) over the first half of S's columns;
-//   * MMA (warp 16, one thread): per step, for A then B: O += P V of the step before
-//     (P from TMEM), S = Q K^T of this one over P's columns (the products of one
-//     thread execute in order), one commit.  While one tile's softmax runs, the
-//     tensor core works for the other;
-//   * loader (warp 17);
-//   * guard (warp 18): on border steps it zeroes the V rows that no row of the CTA
+// Roles (11 warps, one CTA per SM):
+//   * softmax A (warps 0-3) and B (warps 4-7), one thread per query row: S from
+//     TMEM, mask on border steps only, base-2 online softmax in fp32 whose maximum
+//     moves only when it grows by more than 2^8 (then O is rescaled in TMEM), P
+//     rounded to bf16 (the tensor cores' input) over the first half of S's columns;
+//   * MMA (warp 8): step t of a tile is O += P V of step t - 2 (P from TMEM), then
+//     S = Q K^T of step t over that P's columns (one thread's products execute in
+//     order), then one commit.  S has two buffers, so the scores of the next step are
+//     there when the softmax of this one ends: with one buffer of 128 keys it waited
+//     for both products, a third of each step;
+//   * loader (warp 9);
+//   * guard (warp 10): on border steps it zeroes the V rows that no row of the CTA
 //     sees (never-loaded or stale memory, which 0 * NaN would let through), and the
 //     non-finite elements of the others, whose keys it lists: rows that do see such a
 //     key get its non-finite values added at the end, rows that do not stay clean.
 //
-// Bound: the exponentials (16 a clock and SM against 8192 tensor FLOP: a step of
-// 2 x 128 x 128 scores costs 2048 clocks of the special-function units, the
-// products 1024 at head_dim 64 and 2048 at 128).
+// Bound: the exponentials (16 a clock and SM against 8192 tensor FLOP: 128 keys of
+// both tiles cost 2048 clocks of the special-function units, the products 1024 at
+// head_dim 64 and 2048 at 128).
 //
 // A call with fewer CTAs than SMs cuts each tile pair's steps into ranges, whose
 // records window_prefill_merge_kernel joins in range order.
@@ -47,15 +46,13 @@ namespace bsb {
 namespace {
 
 constexpr int kRows = 128;  // query rows of a tile (TMEM lanes)
-constexpr int kKeys = 128;  // keys of a step
+constexpr int kKeys = 64;   // keys of a step
 constexpr int kUnit = 16;   // tokens per unit (one TMA box)
 constexpr int kUnits = kKeys / kUnit;
-constexpr int kSoftWarps = 8;            // softmax warps of a tile
-constexpr int kTileThreads = kSoftWarps * 32;
-constexpr int kThreads = 2 * kTileThreads + 96;
-constexpr int kMmaWarp = 16, kLoadWarp = 17, kGuardWarp = 18;
-constexpr int kRing = 4;  // step barriers per tile (> K stages, > V stages + 1)
-constexpr uint32_t kTmemCols = 512;  // S/P of A, S/P of B, O of A, O of B
+constexpr int kThreads = 352;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kGuardWarp = 10;
+constexpr int kRing = 8;  // step barriers per tile (>= K stages, >= V stages)
+constexpr uint32_t kTmemCols = 512;  // S/P of A (two buffers), of B, O of A, O of B
 constexpr float kLog2eP = 1.4426950408889634f;
 constexpr float kRescaleSlack = 8.f;
 constexpr int kMaxBad = 64;  // listed keys with non-finite V (more: all are looked at)
@@ -63,14 +60,15 @@ constexpr int kMaxBad = 64;  // listed keys with non-finite V (more: all are loo
 template <int D>
 struct Cfg {
   static constexpr int HALVES = D / 64;
-  static constexpr int KS = D == 64 ? 4 : 3;  // K stages
-  static constexpr int VS = D == 64 ? 3 : 2;  // V stages
-  static constexpr int HALF_BYTES = kKeys * 128;  // 64 dims of 128 rows
-  static constexpr int TILE_BYTES = HALVES * HALF_BYTES;
-  // With the barriers and exchange buffers (3 KiB) all of the 227 KiB at 128.
-  static constexpr int SMEM_BYTES = (2 + KS + VS) * TILE_BYTES;
+  static constexpr int KS = D == 64 ? 6 : 5;  // K stages
+  static constexpr int VS = D == 64 ? 6 : 4;  // V stages
+  static constexpr int Q_HALF_BYTES = kRows * 128;  // 64 dims of 128 rows
+  static constexpr int Q_BYTES = HALVES * Q_HALF_BYTES;
+  static constexpr int HALF_BYTES = kKeys * 128;
+  static constexpr int STAGE_BYTES = HALVES * HALF_BYTES;
+  static constexpr int SMEM_BYTES = 2 * Q_BYTES + (KS + VS) * STAGE_BYTES;
   static constexpr uint32_t O_COL = 256;
-  static_assert(KS <= kRing && VS + 1 <= kRing, "a step waiter could fall a whole ring behind");
+  static_assert(KS <= kRing && VS <= kRing, "a step waiter could fall a whole ring behind");
 };
 
 // One tile's tokens and the steps that hold keys of its windows.  (Plain members and
@@ -130,21 +128,6 @@ __device__ __forceinline__ bool step_masked(const WindowArgs& a, const Steps& s,
   return u1 >= s.sink_units && unit_pos(s, max(u0, s.sink_units)) <= t.pos1 - a.window;
 }
 
-// A shared copy of a value, read anew (the softmax threads keep 64 scores in their 96
-// registers: what they need once a step stays in shared memory).
-template <typename T>
-__device__ __forceinline__ T reread(const T& shared) {
-  static_assert(sizeof(T) % 4 == 0, "words");
-  T v;
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T) / 4); ++i) {
-    asm volatile("ld.shared.u32 %0, [%1];"
-                 : "=r"(reinterpret_cast<uint32_t*>(&v)[i])
-                 : "r"(smem_u32(&shared) + 4 * i));
-  }
-  return v;
-}
-
 __device__ __forceinline__ bool sees(const WindowArgs& a, int32_t qpos, int32_t pos) {
   return pos <= qpos && (pos < a.sinks || pos > qpos - a.window);
 }
@@ -180,16 +163,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<D>;
   extern __shared__ __align__(1024) uint8_t smem[];  // 128-byte swizzle atoms
   __shared__ uint64_t q_full, k_full[C::KS], v_full[C::VS], v_ok[C::VS], step_done[2][kRing],
-      p_full[2], mma_done;
+      p_full[2][2], a_ahead, mma_done;
   __shared__ uint32_t tmem_base;
   __shared__ int32_t bad_count, bad_pos[kMaxBad];
-  // The halves' row maxima of a step, and at the end their row sums.
-  __shared__ float exchange[2][2][kRows];
-  __shared__ Steps shared_steps;
 
-  auto sQ = [&](int x) { return smem + x * C::TILE_BYTES; };
-  auto sK = [&](int st) { return smem + (2 + st) * C::TILE_BYTES; };
-  auto sV = [&](int st) { return smem + (2 + C::KS + st) * C::TILE_BYTES; };
+  auto sQ = [&](int x) { return smem + x * C::Q_BYTES; };
+  auto sK = [&](int st) { return smem + 2 * C::Q_BYTES + st * C::STAGE_BYTES; };
+  auto sV = [&](int st) { return smem + 2 * C::Q_BYTES + (C::KS + st) * C::STAGE_BYTES; };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   pdl_wait();
@@ -216,12 +196,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int x = 0; x < 2; ++x) {
       for (int s = 0; s < kRing; ++s) mbar_init(&step_done[x][s], 1);
-      mbar_init(&p_full[x], kTileThreads);
+      for (int b = 0; b < 2; ++b) mbar_init(&p_full[x][b], kRows);
     }
+    mbar_init(&a_ahead, kRows);
     mbar_init(&mma_done, 1);
     fence_barrier_init();
     bad_count = 0;
-    shared_steps = sd;
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -237,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto wait_all = [&](uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
   };
-  // Step u of tile x is done: P V of step u - 1 and S of step u.  Waiters take the
+  // Step u of tile x is done: P V of step u - 2 and S of step u.  Waiters take the
   // steps in order and are never kRing behind (see the ring sizes).
   auto wait_step = [&](int x, int u) {
     return wait_all(&step_done[x][u % kRing], (u / kRing) & 1);
@@ -247,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------------------------------------------------------- loader
     const int32_t* table = a.block_tables + static_cast<int64_t>(w.row) * a.bt_stride;
     const int32_t block_units = a.block_size / kUnit;
-    const int unit = lane & (kUnits - 1), half = lane >> 3;  // this lane's box of a step
+    const int unit = lane % kUnits, half = lane / kUnits;  // this lane's box of a step
     // Pool row of this lane's unit of step j (-1: past the range or invalid).
     auto fetch = [&](int32_t j) -> int32_t {
       const int32_t x = (j0 + j) * kUnits + unit;
@@ -267,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive_expect_tx(&q_full, sd.tiles() * C::HALVES * rows * 128u);
       for (int x = 0; x < sd.tiles(); ++x) {
         for (int hf = 0; hf < C::HALVES; ++hf) {
-          tma_load_3d(sQ(x) + hf * C::HALF_BYTES, &qmap, &q_full, hf * 64, h * a.groups,
+          tma_load_3d(sQ(x) + hf * C::Q_HALF_BYTES, &qmap, &q_full, hf * 64, h * a.groups,
                       w.tok0 + x * tt);
         }
       }
@@ -285,13 +265,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     int32_t k_loads = 0, v_loads = 0;
     for (int32_t j = 0; j < n; ++j) {
-      // Step j - KS has read the K stage, step j - VS + 1 the V stage (of both tiles:
+      // Step j - KS has read the K stage, step j - VS + 2 the V stage (of both tiles:
       // B's commit follows A's products).
       if (j >= C::KS) ok = wait_step(1, j - C::KS);
       if (!ok) break;
       load(&kmap, sK(j % C::KS), &k_full[j % C::KS], y);
       k_loads = j + 1;
-      if (j >= C::VS) ok = wait_step(1, j - C::VS + 1);
+      if (j >= C::VS) ok = wait_step(1, j - C::VS + 2);
       if (!ok) break;
       load(&vmap, sV(j % C::VS), &v_full[j % C::VS], y);
       v_loads = j + 1;
@@ -311,7 +291,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------------------------------------------------------- MMA issuer
     constexpr uint32_t kIdescS = umma_idesc(128, kKeys, 0, 0);
     constexpr uint32_t kIdescO = umma_idesc(128, D, 0, 1);
-    constexpr uint32_t kTileStep = C::TILE_BYTES >> 4, kHalfStep = C::HALF_BYTES >> 4;
+    constexpr uint32_t kQStep = C::Q_BYTES >> 4, kQHalf = C::Q_HALF_BYTES >> 4;
+    constexpr uint32_t kStageStep = C::STAGE_BYTES >> 4, kHalf = C::HALF_BYTES >> 4;
     const uint64_t desc_q = umma_desc(smem_u32(sQ(0)), 16, 1024);
     const uint32_t hi = static_cast<uint32_t>(desc_q >> 32);  // of every operand
     const uint32_t q_lo = static_cast<uint32_t>(desc_q);
@@ -321,40 +302,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         static_cast<uint32_t>(umma_desc(smem_u32(sV(0)), C::HALF_BYTES, 1024));
     const uint32_t mine = elect_lane();  // issues every product
     bool ok = wait_all(&q_full, 0);
-    int32_t done_a = 0, done_b = 0;  // P tiles consumed
-    for (int32_t u = 0; u <= n && ok; ++u) {
+    // By tile: whether it has a P V product yet, and the phase of each P buffer (bit).
+    uint32_t started[2] = {0, 0}, phases[2] = {0, 0};
+    for (int32_t u = 0; u < n + 2 && ok; ++u) {
+      const int b = u & 1;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const TileSteps& ts = x == 0 ? sd.a : sd.b;
-        int32_t& done = x == 0 ? done_a : done_b;
-        const bool pv = u > 0 && step_active(sd, ts, j0 + u - 1);
+        const bool pv = u > 1 && step_active(sd, ts, j0 + u - 2);
         const bool qk = u < n && step_active(sd, ts, j0 + u);
-        const int32_t vs = (u - 1) % C::VS, ks = u % C::KS;
+        const int32_t vs = (u - 2) % C::VS, ks = u % C::KS;
         if (pv) {
-          ok = wait_all(&p_full[x], done & 1) &&
-               wait_all(&v_ok[vs], ((u - 1) / C::VS) & 1);
+          ok = wait_all(&p_full[x][b], (phases[x] >> b) & 1u) &&
+               wait_all(&v_ok[vs], ((u - 2) / C::VS) & 1);
         }
         if (ok && qk) ok = wait_all(&k_full[ks], (u / C::KS) & 1);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t s_col = tmem + x * kKeys;
+        const uint32_t s_col = tmem + (2 * x + b) * kKeys;
         if (pv) {
-          const uint32_t v0 = v_lo + vs * kTileStep;
+          const uint32_t v0 = v_lo + vs * kStageStep;
           unroll<kKeys / 16>([&](auto k) {
             // P: 8 columns per 16 keys; V: 16 rows of 128 bytes.
             umma_f16_ts_elect<8 * k, 128 * k>(mine, tmem + C::O_COL + x * D, s_col, v0, hi,
-                                              kIdescO, (done > 0 || k > 0) ? 1u : 0u);
+                                              kIdescO, k > 0 ? 1u : started[x]);
           });
+          started[x] = 1u;
+          phases[x] ^= 1u << b;
         }
         if (qk) {
-          const uint32_t q0 = q_lo + x * kTileStep, k0 = k_lo + ks * kTileStep;
+          const uint32_t q0 = q_lo + x * kQStep, k0 = k_lo + ks * kStageStep;
           unroll<D / 16>([&](auto k) {
-            constexpr uint32_t off = (k / 4) * kHalfStep + 2 * (k % 4);  // 32 bytes a slice
-            umma_f16_elect<off, off>(mine, s_col, q0, k0, hi, kIdescS, k > 0 ? 1u : 0u);
+            // 32 bytes a slice of 16 dims.
+            umma_f16_elect<(k / 4) * kQHalf + 2 * (k % 4), (k / 4) * kHalf + 2 * (k % 4)>(
+                mine, s_col, q0, k0, hi, kIdescS, k > 0 ? 1u : 0u);
           });
         }
         umma_commit_elect(mine, &step_done[x][u % kRing]);
-        if (pv) ++done;
         __syncwarp();
       }
     }
@@ -376,24 +360,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto position = [&](int row) {  // of the key of a V row
           return unit_pos(sd, (j0 + j) * kUnits + row / kUnit) + row % kUnit;
         };
-        // Rows that no query row sees become zero, lane = row.
+        // Rows that no query row sees become zero (lane = row, then four rows at a
+        // time, eight lanes along each).
         for (int g = 0; g < kKeys / 32; ++g) {
           const int row = g * 32 + lane;
           const int32_t pos = position(row);
           const bool live = (j0 + j) * kUnits + row / kUnit < sd.units && pos <= end &&
                             (pos < a.sinks || pos >= w.lo);
-          if (!live) {
-            for (int c = 0; c < 8 * C::HALVES; ++c) {
-              *reinterpret_cast<uint4*>(sV(vs) + (c / 8) * C::HALF_BYTES + row * 128 +
-                                        (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t dead = __ballot_sync(0xffffffffu, !live);
+          for (int q = 0; q < 8; ++q) {
+            if (!((dead >> (4 * q + (lane >> 3))) & 1u)) continue;
+            uint8_t* p = sV(vs) + (g * 32 + 4 * q + (lane >> 3)) * 128 + (lane & 7) * 16;
+            for (int hf = 0; hf < C::HALVES; ++hf) {
+              *reinterpret_cast<uint4*>(p + hf * C::HALF_BYTES) = make_uint4(0u, 0u, 0u, 0u);
             }
           }
+          __syncwarp();
         }
-        __syncwarp();
         // x * 0 is 0 or, for infinities and NaN, NaN, and stays NaN in the sum.
         uint32_t sum = 0;
 #pragma unroll 8
-        for (int c = 0; c < C::TILE_BYTES / 512; ++c) {
+        for (int c = 0; c < C::STAGE_BYTES / 512; ++c) {
           const uint4 v = *reinterpret_cast<const uint4*>(sV(vs) + (c * 32 + lane) * 16);
           sum = fma_zero_bf16x2(v.x, sum);
           sum = fma_zero_bf16x2(v.y, sum);
@@ -439,61 +426,45 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok && lane == 0) set_status(a.status, kStatusWaitTimeout);
   } else {
     // ---------------------------------------------------------------- softmax
-    const int x = warp / kSoftWarps, hf = (warp >> 2) & 1;  // tile, half of the keys
+    const int x = warp >> 2;
+    const TileSteps ts = sd.tile(x);
     const int row = tid & (kRows - 1);
     const int32_t tok = row / a.groups, g = row - tok * a.groups;
     const bool live = x * tt + tok < w.ntok && tok < tt;
     const int32_t qpos = w.pos0 + x * tt + tok;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lane_base + x * kKeys;
-    const uint32_t o_addr = tmem + lane_base + C::O_COL + x * D + hf * (D / 2);  // its half
-    // Barrier of the tile's warps; true when it is for all of them.  A wait that gave
-    // up in one warp ends the loop in all at once: none is left at a barrier.
-    auto tile_all = [&](bool mine) {
-      uint32_t all;
-      asm volatile(
-          "{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n"
-          " barrier.cta.red.and.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
-          : "=r"(all)
-          : "r"(1 + x), "r"(kTileThreads), "r"(mine ? 1u : 0u)
-          : "memory");
-      return all != 0;
-    };
+    const uint32_t o_addr = tmem + lane_base + C::O_COL + x * D;
     const float zscale = fabsf(a.scale) * kLog2eP;
     float m_used = -INFINITY, l_run = 0.f;
     int32_t done = 0;
+    const bool a_first = step_active(sd, sd.a, j0);  // A has a step here, the first one
     bool ok = true;
     for (int32_t u = 0; u < n; ++u) {
-      bool border;
-      {
-        const Steps st = reread(shared_steps);
-        const TileSteps ts = st.tile(x);
-        const bool active = step_active(st, ts, j0 + u);
-        border = step_masked(a, st, ts, j0 + u);
-        ok = ok && wait_step(x, u);
-        if (!active) continue;
-      }
+      ok = wait_step(x, u);
+      if (!ok) break;
+      if (!step_active(sd, ts, j0 + u)) continue;
       tc_fence_after();
+      const uint32_t s_addr = tmem + lane_base + (2 * x + (u & 1)) * kKeys;
       // Visible tokens of the step's units, 16 bits each (border steps only).
+      const bool border = step_masked(a, sd, ts, j0 + u);
       uint32_t maps[2];
       if (border) {
         auto below = [](int32_t c) -> uint32_t {  // map of the first c tokens
           return c >= kUnit ? 0xffffu : c <= 0 ? 0u : (1u << c) - 1u;
         };
-        const Steps st = reread(shared_steps);
 #pragma unroll
-        for (int un = 0; un < kUnits / 2; ++un) {
-          const int32_t ux = (j0 + u) * kUnits + hf * (kUnits / 2) + un;
-          const int32_t p0 = unit_pos(st, ux);
+        for (int un = 0; un < kUnits; ++un) {
+          const int32_t ux = (j0 + u) * kUnits + un;
+          const int32_t p0 = unit_pos(sd, ux);
           uint32_t map = below(qpos - p0 + 1) &
                          (~below(qpos - a.window + 1 - p0) | below(a.sinks - p0));
-          if (ux >= st.units || !live) map = 0;
+          if (ux >= sd.units || !live) map = 0;
           maps[un / 2] = un % 2 ? maps[un / 2] | (map << 16) : map;
         }
       }
       uint32_t v[2][32];
-      tmem_ld32(s_addr + hf * 64, v[0]);
-      tmem_ld32(s_addr + hf * 64 + 32, v[1]);
+      tmem_ld32(s_addr, v[0]);
+      tmem_ld32(s_addr + 32, v[1]);
       tmem_wait_ld();
       if (a.scale < 0.f) {  // turned around: the rest works with the scale's magnitude
 #pragma unroll
@@ -507,61 +478,67 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i / 32][i % 32]));
-      const float m_half = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      exchange[x][hf][row] = m_half;
-      ok = tile_all(ok);  // also: every score is read before P takes columns 0 .. 63
-      if (!ok) break;
-      const float m_step = fmaxf(m_half, exchange[x][hf ^ 1][row]) * zscale;
+      for (int i = 0; i < 32; ++i) {  // three-input maxima
+        mx[i & 3] = fmaxf(fmaxf(mx[i & 3], __uint_as_float(v[0][i])), __uint_as_float(v[1][i]));
+      }
+      const float m_step = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * zscale;
       const bool grow = live && m_step > m_used + kRescaleSlack;
       if (done == 0) {
         m_used = m_step;
       } else if (__any_sync(0xffffffffu, grow)) {
-        // P V of the step before is done (wait_step), so O may be rescaled; rows
-        // that did not grow keep theirs (factor 1).
+        // O may be rescaled once P V of the step before is done; rows that did not
+        // grow keep theirs (factor 1).
+        ok = wait_step(x, u + 1);
+        if (!ok) break;
+        tc_fence_after();
         const float m_new = grow ? m_step : m_used;
         const float corr = grow ? fast_exp2(m_used - m_new) : 1.f;
 #pragma unroll 1
-        for (int c0 = 0; c0 < D / 2; c0 += 8) {  // few columns: the scores stay in registers
-          uint32_t o[8];
-          tmem_ld8(o_addr + c0, o);
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + c0, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 8; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
-          tmem_st8(o_addr + c0, o);
+          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
+          tmem_st32(o_addr + c0, o);
         }
         l_run *= corr;
         m_used = m_new;
       }
+      // B's first exponentials wait for A's, once: from then on one tile uses the
+      // special-function units while the other loads, reduces and stores.
+      if (x == 1 && done == 0 && a_first) {
+        ok = wait_all(&a_ahead, 0);
+        if (!ok) break;
+      }
       const float m_base = m_used == -INFINITY ? 0.f : m_used;  // no -inf - -inf
       const float2 zs2 = make_float2(zscale, zscale), mm = make_float2(-m_base, -m_base);
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
+                       make_float2(0.f, 0.f)};
+      uint32_t p[32];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t p[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 e = __ffma2_rn(
-              make_float2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), zs2, mm);
-          const float2 pe = make_float2(fast_exp2(e.x), fast_exp2(e.y));
-          sum[i & 1] = __fadd2_rn(sum[i & 1], pe);
-          p[i] = pack_bf16x2(pe.x, pe.y);
-        }
-        tmem_st16(s_addr + hf * 32 + c * 16, p);
+      for (int i = 0; i < 32; ++i) {
+        const float2 e = __ffma2_rn(make_float2(__uint_as_float(v[i / 16][2 * (i % 16)]),
+                                                __uint_as_float(v[i / 16][2 * (i % 16) + 1])),
+                                    zs2, mm);
+        const float2 pe = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+        sum[i & 3] = __fadd2_rn(sum[i & 3], pe);
+        p[i] = pack_bf16x2(pe.x, pe.y);
       }
+      tmem_st32(s_addr, p);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&p_full[x]);
-      l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      mbar_arrive(&p_full[x][u & 1]);
+      if (x == 0 && done == 0) mbar_arrive(&a_ahead);
+      l_run += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) +
+               ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
       ++done;
     }
-    ok = ok && wait_step(x, n);  // the last P V is done
-    exchange[x][hf][row] = l_run;
-    ok = tile_all(ok);
-    l_run += exchange[x][hf ^ 1][row];
+    // The last P V is done (the steps in order, as everywhere).
+    if (ok) ok = wait_step(x, n) && wait_step(x, n + 1);
     if (!ok) {
       if (lane == 0) set_status(a.status, kStatusWaitTimeout);
-    } else if (sd.tile(x).used) {
+    } else if (ts.used) {
       tc_fence_after();
       const bool split_up = ranges > 1;
       // Listed keys are complete: the guard arrived for every V that was used.
@@ -571,11 +548,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t rec_row = (static_cast<int64_t>(item) * a.splits + split) * 2 * kRows +
                               x * kRows + row;
 #pragma unroll
-      for (int cc = 0; cc < D / 2; cc += 32) {
-        const int c0 = hf * (D / 2) + cc;  // this thread's columns of the head
+      for (int c0 = 0; c0 < D; c0 += 32) {
         uint32_t v[32];
         if (done > 0) {
-          tmem_ld32(o_addr + cc, v);
+          tmem_ld32(o_addr + c0, v);
           tmem_wait_ld();
         } else {
 #pragma unroll
@@ -630,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (split_up && live && hf == 0) {
+      if (split_up && live) {
         float* ml = a.records + a.rec_stride_ml + rec_row * 2;
         *reinterpret_cast<float2*>(ml) = make_float2(m_used, l_run);
       }
