@@ -13,7 +13,7 @@
 // TMA box per K, V and 64 dims through the block table, so sink units and window
 // units share a step and nothing between them is touched.
 //
-// Roles (11 warps, one CTA per SM):
+// Roles (12 warps, one CTA per SM):
 //   * softmax A (warps 0-3) and B (warps 4-7), one thread per query row: S from
 //     TMEM, mask on border steps only, base-2 online softmax in fp32 whose maximum
 //     moves only when it grows by more than 2^8 (then O is rescaled in TMEM), P
@@ -23,8 +23,10 @@
 //     order), then one commit.  S has two buffers, so the scores of the next step are
 //     there when the softmax of this one ends: with one buffer of 128 keys it waited
 //     for both products, a third of each step;
-//   * loader (warp 9);
-//   * guard (warp 10): on border steps it zeroes the V rows that no row of the CTA
+//   * loaders, of Q and K (warp 9) and of V (warp 10): a TMA box is only 16 rows, and
+//     issuing one takes a warp some 35 cycles, so one warp for both (16 boxes a step
+//     at head_dim 128) was what the steps waited for;
+//   * guard (warp 11): on border steps it zeroes the V rows that no row of the CTA
 //     sees (never-loaded or stale memory, which 0 * NaN would let through), and the
 //     non-finite elements of the others, whose keys it lists: rows that do see such a
 //     key get its non-finite values added at the end, rows that do not stay clean.
@@ -49,8 +51,8 @@ constexpr int kRows = 128;  // query rows of a tile (TMEM lanes)
 constexpr int kKeys = 64;   // keys of a step
 constexpr int kUnit = 16;   // tokens per unit (one TMA box)
 constexpr int kUnits = kKeys / kUnit;
-constexpr int kThreads = 352;
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kGuardWarp = 10;
+constexpr int kThreads = 384;
+constexpr int kMmaWarp = 8, kLoadKWarp = 9, kLoadVWarp = 10, kGuardWarp = 11;
 constexpr int kRing = 8;  // step barriers per tile (>= K stages, >= V stages)
 constexpr uint32_t kTmemCols = 512;  // S/P of A (two buffers), of B, O of A, O of B
 constexpr float kLog2eP = 1.4426950408889634f;
@@ -223,26 +225,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     return wait_all(&step_done[x][u % kRing], (u / kRing) & 1);
   };
 
-  if (warp == kLoadWarp) {
-    // ---------------------------------------------------------------- loader
+  if (warp == kLoadKWarp || warp == kLoadVWarp) {
+    // ---------------------------------------------------------------- loaders
+    const bool is_k = warp == kLoadKWarp;
+    const CUtensorMap* map = is_k ? &kmap : &vmap;
+    const int stages = is_k ? C::KS : C::VS;
+    uint8_t* ring = is_k ? sK(0) : sV(0);
+    uint64_t* full = is_k ? k_full : v_full;
     const int32_t* table = a.block_tables + static_cast<int64_t>(w.row) * a.bt_stride;
     const int32_t block_units = a.block_size / kUnit;
     const int unit = lane % kUnits, half = lane / kUnits;  // this lane's box of a step
+    uint8_t* box = ring + half * C::HALF_BYTES + unit * 2048;
+    const int32_t head_row = h * a.num_blocks * a.block_size;
     // Pool row of this lane's unit of step j (-1: past the range or invalid).
     auto fetch = [&](int32_t j) -> int32_t {
       const int32_t x = (j0 + j) * kUnits + unit;
-      if (j >= n || x >= sd.units) return -1;
-      const int32_t tu = unit_pos(sd, x) / kUnit;
-      const int32_t ent = tu / block_units;
+      if (j >= n || x >= sd.units || half >= C::HALVES) return -1;
+      const int32_t tu = x < sd.sink_units ? x : x - sd.sink_units + sd.first_unit;
+      const int32_t ent = block_units == 1 ? tu : tu / block_units;
       const int32_t blk = __ldg(table + ent);
       if (blk < 0 || blk >= a.num_blocks) {
-        if (half == 0) set_status(a.status, kStatusBadBlock);
+        if (is_k && half == 0) set_status(a.status, kStatusBadBlock);
         return -1;
       }
-      return (h * a.num_blocks + blk) * a.block_size + (tu - ent * block_units) * kUnit;
+      return head_row + blk * a.block_size + (tu - ent * block_units) * kUnit;
     };
     int32_t y = fetch(0), y_next = fetch(1);
-    if (lane == 0) {
+    if (is_k && lane == 0) {
       const uint32_t rows = static_cast<uint32_t>(tt * a.groups);
       mbar_arrive_expect_tx(&q_full, sd.tiles() * C::HALVES * rows * 128u);
       for (int x = 0; x < sd.tiles(); ++x) {
@@ -253,38 +262,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-    auto load = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* full, int32_t row) {
-      const bool mine = row >= 0 && half < C::HALVES;
-      const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
-      if (lane == 0) mbar_arrive_expect_tx(full, boxes * 2048u);
-      __syncwarp();
-      if (mine) {
-        tma_load_2d(dst + half * C::HALF_BYTES + unit * 2048, map, full, half * 64, row);
-      }
-    };
+    // Step j - KS has read the K stage, step j - VS + 2 the V stage (of both tiles: B's
+    // commit follows A's products).
+    const int32_t lag = is_k ? 0 : 2;
     bool ok = true;
-    int32_t k_loads = 0, v_loads = 0;
+    int32_t loads = 0;
+    int stage = 0;
     for (int32_t j = 0; j < n; ++j) {
-      // Step j - KS has read the K stage, step j - VS + 2 the V stage (of both tiles:
-      // B's commit follows A's products).
-      if (j >= C::KS) ok = wait_step(1, j - C::KS);
+      if (j >= stages) ok = wait_step(1, j - stages + lag);
       if (!ok) break;
-      load(&kmap, sK(j % C::KS), &k_full[j % C::KS], y);
-      k_loads = j + 1;
-      if (j >= C::VS) ok = wait_step(1, j - C::VS + 2);
-      if (!ok) break;
-      load(&vmap, sV(j % C::VS), &v_full[j % C::VS], y);
-      v_loads = j + 1;
+      const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, y >= 0));
+      if (lane == 0) mbar_arrive_expect_tx(full + stage, boxes * 2048u);
+      __syncwarp();
+      if (y >= 0) tma_load_2d(box + stage * C::STAGE_BYTES, map, full + stage, half * 64, y);
+      loads = j + 1;
+      if (++stage == stages) stage = 0;
       y = y_next;
       y_next = fetch(j + 2);
     }
     // Drain: every load has landed before the CTA leaves its shared memory.
-    bool drained = wait_all(&q_full, 0);
-    for (int32_t j = max(0, k_loads - C::KS); j < k_loads; ++j) {
-      drained = wait_all(&k_full[j % C::KS], (j / C::KS) & 1) && drained;
-    }
-    for (int32_t j = max(0, v_loads - C::VS); j < v_loads; ++j) {
-      drained = wait_all(&v_full[j % C::VS], (j / C::VS) & 1) && drained;
+    bool drained = !is_k || wait_all(&q_full, 0);
+    for (int32_t j = max(0, loads - stages); j < loads; ++j) {
+      drained = wait_all(full + j % stages, (j / stages) & 1) && drained;
     }
     if ((!ok || !drained) && lane == 0) set_status(a.status, kStatusWaitTimeout);
   } else if (warp == kMmaWarp) {
