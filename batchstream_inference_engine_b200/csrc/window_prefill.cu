@@ -140,14 +140,47 @@ __device__ __forceinline__ int32_t step_ranges(int32_t steps, int32_t splits) {
   return most < splits ? most : splits;
 }
 
-// Linear item -> (sequence, tile pair, kv head): a chunk's last tiles, which see the
-// most keys, come first.
+// Linear item -> (sequence, tile pair, kv head), which also numbers the records.
 __device__ __forceinline__ void pair_of(const WindowArgs& a, int32_t item, int32_t& r,
                                         int32_t& tile, int32_t& h) {
   h = item % a.num_kv_heads;
   item /= a.num_kv_heads;
   r = item % a.num_rows;
   tile = a.qtiles - 1 - item / a.num_rows;
+}
+
+// Most sequences that every CTA ranks (one a thread).
+constexpr int kMaxRanked = kThreads;
+
+// The sequence, tile pair and kv head of launch index b: the sequences with the most
+// steps first, a sequence's last tiles, which see the most keys, ahead of its others.
+// A step range is the whole of a CTA's time, so the long ones must not start last.
+// All threads call it; `steps` and `pick` are shared memory.
+__device__ __forceinline__ void ranked_pair(const WindowArgs& a, int32_t b, int32_t (&steps)[kMaxRanked],
+                                            int32_t& pick, int32_t& r, int32_t& tile, int32_t& h) {
+  h = b % a.num_kv_heads;
+  b /= a.num_kv_heads;
+  tile = a.qtiles - 1 - b % a.qtiles;
+  r = b / a.qtiles;
+  if (a.num_rows == 1 || a.num_rows > kMaxRanked) return;
+  const int t = threadIdx.x;
+  int32_t mine = 0;
+  if (t < a.num_rows) {
+    const int32_t tokens = __ldg(a.cu_q + t + 1) - __ldg(a.cu_q + t);
+    // Keys that the chunk's last tile reads, near enough for an order.
+    if (tokens > 0) mine = min(__ldg(a.context_lens + t), a.window + a.tile_tokens);
+    steps[t] = mine;
+  }
+  __syncthreads();
+  if (t < a.num_rows) {
+    int32_t rank = 0;
+    for (int32_t i = 0; i < a.num_rows; ++i) {
+      rank += steps[i] > mine || (steps[i] == mine && i < t) ? 1 : 0;
+    }
+    if (rank == r) pick = t;  // the ranks are a permutation of the rows
+  }
+  __syncthreads();
+  r = pick;
 }
 
 // a * 0 + c on bf16 pairs.
@@ -177,9 +210,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   const int32_t tt = a.tile_tokens / 2;  // tokens of one tile
   const int32_t split = blockIdx.x % a.splits;
-  const int32_t item = blockIdx.x / a.splits;
+  __shared__ int32_t ranked[kMaxRanked], picked;
   int32_t r, tile, h;
-  pair_of(a, item, r, tile, h);
+  ranked_pair(a, blockIdx.x / a.splits, ranked, picked, r, tile, h);
+  // The item of its records (pair_of).
+  const int32_t item = ((a.qtiles - 1 - tile) * a.num_rows + r) * a.num_kv_heads + h;
   WindowTile w;
   if (!window_tile(a, r, tile, w, tid == 0 && tile == 0 && h == 0 && split == 0)) return;
   const Steps sd = steps_of(a, w, tt);
@@ -301,21 +336,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         static_cast<uint32_t>(umma_desc(smem_u32(sV(0)), C::HALF_BYTES, 1024));
     const uint32_t mine = elect_lane();  // issues every product
     bool ok = wait_all(&q_full, 0);
+    // Steps in which tile x has keys: the sinks' and [from[x], to[x]] (step_active).
+    const int32_t sink_steps = (sd.sink_units + kUnits - 1) / kUnits - j0;
+    const int32_t from[2] = {sd.a.first - j0, sd.b.first - j0};
+    const int32_t to[2] = {sd.a.last - j0, sd.b.used ? sd.b.last - j0 : -1};
     // By tile: whether it has a P V product yet, and the phase of each P buffer (bit).
+    // Ring positions and phases are carried along: this warp's own instructions,
+    // products apart, must stay well below a step's time.  (A warp per tile, the guard
+    // moved into V's loader to make room for it, measured 6 to 9% slower.)
     uint32_t started[2] = {0, 0}, phases[2] = {0, 0};
+    int ks = 0, vs = 0;
+    uint32_t k_phase = 0, v_phase = 0;
     for (int32_t u = 0; u < n + 2 && ok; ++u) {
       const int b = u & 1;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const TileSteps& ts = x == 0 ? sd.a : sd.b;
-        const bool pv = u > 1 && step_active(sd, ts, j0 + u - 2);
-        const bool qk = u < n && step_active(sd, ts, j0 + u);
-        const int32_t vs = (u - 2) % C::VS, ks = u % C::KS;
+        auto active = [&](int32_t j) { return j <= to[x] && (j >= from[x] || j < sink_steps); };
+        const bool pv = u > 1 && active(u - 2);
+        const bool qk = u < n && active(u);
+        // P last: K and V are there long before it.
+        if (qk) ok = wait_all(&k_full[ks], k_phase);
         if (pv) {
-          ok = wait_all(&p_full[x][b], (phases[x] >> b) & 1u) &&
-               wait_all(&v_ok[vs], ((u - 2) / C::VS) & 1);
+          ok = ok && wait_all(&v_ok[vs], v_phase);
+          ok = ok && wait_all(&p_full[x][b], (phases[x] >> b) & 1u);
         }
-        if (ok && qk) ok = wait_all(&k_full[ks], (u / C::KS) & 1);
         if (!ok) break;
         tc_fence_after();
         const uint32_t s_col = tmem + (2 * x + b) * kKeys;
@@ -338,9 +382,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           });
         }
         umma_commit_elect(mine, &step_done[x][u % kRing]);
-        __syncwarp();
+      }
+      if (++ks == C::KS) {
+        ks = 0;
+        k_phase ^= 1u;
+      }
+      if (u > 1 && ++vs == C::VS) {
+        vs = 0;
+        v_phase ^= 1u;
       }
     }
+    __syncwarp();
     umma_commit_elect(mine, &mma_done);
     const bool drained = wait_all(&mma_done, 0);
     if ((!ok || !drained) && lane == 0) set_status(a.status, kStatusWaitTimeout);
