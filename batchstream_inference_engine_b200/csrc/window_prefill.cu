@@ -130,6 +130,17 @@ __device__ __forceinline__ bool step_masked(const WindowArgs& a, const Steps& s,
   return u1 >= s.sink_units && unit_pos(s, max(u0, s.sink_units)) <= t.pos1 - a.window;
 }
 
+// Steps [lo, hi] of a tile that need no mask (every row sees every key): behind the
+// sinks, the units from the first that all windows hold whole to the last that ends at
+// or before the first row.
+__device__ __forceinline__ void plain_steps(const WindowArgs& a, const Steps& s,
+                                            const TileSteps& t, int32_t& lo, int32_t& hi) {
+  const int32_t out = t.pos1 - a.window;  // the last position that some row does not see
+  const int32_t whole = out < 0 ? 0 : out / kUnit + 1;
+  lo = (s.sink_units + max(whole - s.first_unit, 0) + kUnits - 1) / kUnits;
+  hi = (s.sink_units + (t.pos0 + 1) / kUnit - s.first_unit) / kUnits - 1;
+}
+
 __device__ __forceinline__ bool sees(const WindowArgs& a, int32_t qpos, int32_t pos) {
   return pos <= qpos && (pos < a.sinks || pos > qpos - a.window);
 }
@@ -488,16 +499,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float zscale = fabsf(a.scale) * kLog2eP;
     float m_used = -INFINITY, l_run = 0.f;
     int32_t done = 0;
+    int32_t plain_lo, plain_hi;
+    plain_steps(a, sd, ts, plain_lo, plain_hi);
     const bool a_first = step_active(sd, sd.a, j0);  // A has a step here, the first one
     bool ok = true;
     for (int32_t u = 0; u < n; ++u) {
       ok = wait_step(x, u);
       if (!ok) break;
-      if (!step_active(sd, ts, j0 + u)) continue;
+      const bool plain = j0 + u >= plain_lo && j0 + u <= plain_hi;
+      if (!plain && !step_active(sd, ts, j0 + u)) continue;
       tc_fence_after();
       const uint32_t s_addr = tmem + lane_base + (2 * x + (u & 1)) * kKeys;
       // Visible tokens of the step's units, 16 bits each (border steps only).
-      const bool border = step_masked(a, sd, ts, j0 + u);
+      const bool border = !plain && step_masked(a, sd, ts, j0 + u);
       uint32_t maps[2];
       if (border) {
         auto below = [](int32_t c) -> uint32_t {  // map of the first c tokens
