@@ -108,8 +108,8 @@ Tensor int32_list(const char* name, const char* arg, const Tensor& t, int64_t co
 
 // ------------------------------------------------------------------ status words
 
-// The status word of each (device, stream) lives in the workspaces that ops.py
-// keeps; their addresses are asked for once and forgotten whenever one moves.
+// The status word of each (device, stream) is a tensor that ops.py keeps and never
+// moves; its address is asked for once.
 struct StatusWord {
   int device;
   void* stream;
@@ -398,11 +398,6 @@ PyObject* set_status_source(PyObject* const* a) {
   Py_RETURN_NONE;
 }
 
-PyObject* forget_status(PyObject* const*) {
-  g_status.clear();
-  Py_RETURN_NONE;
-}
-
 // ------------------------------------------------------------------ module
 
 template <PyObject* (*Fn)(PyObject* const*), Py_ssize_t Count>
@@ -436,7 +431,6 @@ PyMethodDef g_methods[] = {
     method<rotary_append, 10>("rotary_append"),
     method<copy_blocks, 4>("copy_blocks"),
     method<set_status_source, 1>("set_status_source"),
-    method<forget_status, 0>("forget_status"),
     {nullptr, nullptr, 0, nullptr},
 };
 

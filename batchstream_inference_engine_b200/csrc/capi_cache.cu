@@ -453,7 +453,8 @@ int bs_window_prefill_attention_workspace_bytes(int64_t num_tokens, int64_t num_
                                                 int64_t block_size, int64_t max_blocks_per_seq,
                                                 int32_t dtype, int64_t window, int64_t sinks,
                                                 uint64_t* bytes_out) {
-  const WindowShape s{num_rows, num_tokens,   max_query_len, true,
+  // (A chunk cannot hold more than all tokens; a negative bound stays to be refused.)
+  const WindowShape s{num_rows, num_tokens, std::min(max_query_len, num_tokens), true,
                       num_heads, num_kv_heads, head_dim, block_size,
                       max_blocks_per_seq, window, sinks, dtype};
   return window_workspace(s, bytes_out);
@@ -489,7 +490,7 @@ int bs_window_prefill_attention(const void* query, int64_t query_token_stride, c
                                 int64_t sinks, void* output, int64_t output_token_stride,
                                 void* workspace, uint64_t workspace_bytes, uint32_t* status,
                                 void* stream) {
-  const WindowShape s{num_rows, num_tokens,   max_query_len, true,
+  const WindowShape s{num_rows, num_tokens, std::min(max_query_len, num_tokens), true,
                       num_heads, num_kv_heads, head_dim, block_size,
                       max_blocks_per_seq, window, sinks, dtype};
   const WindowCall c{query,        query_token_stride, cu_q,      context_lens, seq_rows,

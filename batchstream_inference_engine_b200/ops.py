@@ -51,6 +51,23 @@ def _require_cuda(name: str, *tensors: torch.Tensor) -> torch.device:
     return device
 
 
+class _StatusWords:
+    """One zero-filled status word per (device, stream) for the calls that keep no
+    workspace.  A word never moves: captured calls hold its address."""
+
+    def __init__(self):
+        self._lock = threading.Lock()
+        self._words: dict[tuple[int, int], torch.Tensor] = {}
+
+    def get(self, index: int, stream: int) -> torch.Tensor:
+        with self._lock:
+            word = self._words.get((index, stream))
+            if word is None:
+                word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+                self._words[index, stream] = word
+            return word
+
+
 class _Workspaces:
     """Zero-filled scratch buffers, one per (device, stream), grown on demand.
 
@@ -75,18 +92,26 @@ class _Workspaces:
                     fresh[:4].copy_(buf[:4])
                 buf = fresh
                 self._buffers[key] = buf
-                _native.forget_status()  # it may hold the old buffer's address
             return buf
 
 
 _workspaces = _Workspaces()
-_native.set_status_source(lambda index, stream: _workspaces.get(
-    torch.device("cuda", index), stream, 0).data_ptr())
+_status_words = _StatusWords()
+_native.set_status_source(lambda index, stream: _status_words.get(index, stream).data_ptr())
 
 
 def workspace_for(device: torch.device, nbytes: int) -> torch.Tensor:
     """The scratch buffer used for calls on the current stream of `device`."""
     return _workspaces.get(device, torch.cuda.current_stream(device).cuda_stream, nbytes)
+
+
+def status_words(device: torch.device) -> list[torch.Tensor]:
+    """The int32 words in which the calls on the current stream of `device` report
+    bad input: the workspace's, and the one of the calls without a workspace."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return [_workspaces.get(device, stream, 0)[:4].view(torch.int32),
+            _status_words.get(index, stream)]
 
 
 def take_status(device: torch.device | None = None) -> int:
@@ -98,7 +123,11 @@ def take_status(device: torch.device | None = None) -> int:
     device = device or torch.device("cuda", torch.cuda.current_device())
     stream = torch.cuda.current_stream(device).cuda_stream
     ws = _workspaces.get(device, stream, 0)
+    word = status_words(device)[1]
     bits = ctypes.c_uint32(0)
+    rc = lib().bs_take_status(word.data_ptr(), stream, ctypes.byref(bits))
+    if bits.value:  # reported by a call without a workspace; the other word's turn is next
+        check(rc)
     rc = lib().bs_take_status(ws.data_ptr(), stream, ctypes.byref(bits))
     if bits.value:
         # A launch that reported a problem may have left segment counters set:

@@ -321,6 +321,7 @@ class TorchModel:
             self.rope_frequencies, self.rope_amplitude = ops.rope_frequencies(
                 config.rotary_dim or config.head_dim, config.rope_theta, config.rope_scaling,
                 device=self.device)
+        self._bounded = bool(config.attention_window) or not config.rotary_from_tables
         self.max_position = max_position
         # Per-step accounting for benchmarks: forwards, tokens and rows
         # processed, attention FLOPs (QK^T + PV over visible keys), launches of
@@ -341,6 +342,7 @@ class TorchModel:
         self._graph_stream = None
         self._graph_pool = None
         self._graph_ws = None
+        self._graph_status = None  # status words of the capture stream
         self._hosts = None  # pinned buffers for pending token ids
         self._host_turn = 0
 
@@ -387,22 +389,24 @@ class TorchModel:
         """Copies `ids` to one of a few pinned buffers and records the event the
         host waits on; at most len(self._hosts) - 1 steps may be pending."""
         n = ids.numel()
-        if self._hosts is None or self._hosts[0].numel() < n + 2:
-            self._hosts = [torch.empty(max(n + 2, 1024), dtype=torch.int32, pin_memory=True)
+        if self._hosts is None or self._hosts[0].numel() < n + 4:
+            self._hosts = [torch.empty(max(n + 4, 1024), dtype=torch.int32, pin_memory=True)
                            for _ in range(3)]
         buf = self._hosts[self._host_turn]
         self._host_turn = (self._host_turn + 1) % len(self._hosts)
-        host, status = buf[:n], buf[n: n + 2]
+        host, status = buf[:n], buf[n: n + 4]
         host.copy_(ids, non_blocking=True)
-        # Kernels report bad input in the status word of their stream's
-        # workspace (eager calls: this stream; graph replays: the capture
-        # stream's): copied after the step, read with the ids.
-        status[0].copy_(ops.workspace_for(self.device, 0)[:4].view(torch.int32)[0],
-                        non_blocking=True)
-        if self._graph_ws is not None:
-            status[1].copy_(self._graph_ws[:4].view(torch.int32)[0], non_blocking=True)
-        else:
-            status[1].fill_(0)
+        # Kernels report bad input in the status words of their stream (eager
+        # calls: this stream; graph replays: the capture stream's): copied after
+        # the step, read with the ids.  Only a model with the operators that use
+        # the second word of a stream needs to look at it.
+        words = ops.status_words(self.device)
+        words += self._graph_status or []
+        if not self._bounded:
+            words = words[::2]
+        status.fill_(0)
+        for i, word in enumerate(words):
+            status[i: i + 1].copy_(word, non_blocking=True)
         self.stats["d2h_bytes"] += 4 * n
         event = torch.cuda.Event()
         event.record(torch.cuda.current_stream(self.device))
@@ -673,6 +677,7 @@ class TorchModel:
                 need = max(need, ops.prefill_workspace_bytes(
                     q, rows, q, c.num_heads, c.num_kv_heads, c.head_dim, block_size, self.dtype))
         self._graph_ws = ops.workspace_for(self.device, need)
+        self._graph_status = ops.status_words(self.device)
 
     @torch.inference_mode()
     def warm_graphs(self, pool: PagedKVPool) -> int:

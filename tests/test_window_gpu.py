@@ -189,6 +189,36 @@ def test_decode_large_batch_many_lengths():
     c.check(out)
 
 
+def test_decode_more_sequences_than_the_span_scan_stages():
+    # 5500 sequences: their lengths do not fit the stage memory, and there are more
+    # segments than resident CTAs.
+    g = torch.Generator().manual_seed(7)
+    lens = torch.randint(0, 60, (5500,), generator=g).tolist()
+    c = Paged(lens, [1] * 5500, 2, 1, 64, 16, torch.bfloat16, 20, 3, seed=7)
+    out = c.decode()
+    assert ops.take_status() == 0
+    c.check(out)
+
+
+def test_decode_output_may_be_the_query():
+    for dtype in (torch.bfloat16, torch.float32):
+        c = Paged([5000, 70, 3], [1] * 3, 14, 2, 64, 16, dtype, 4000, 4, seed=13)
+        want = c.decode()
+        q = c.q.to(DEV)
+        ops.window_attention_batched(q, c.k, c.v, c.table, c.len_d, c.scale, 4000, 4, out=q)
+        assert torch.equal(q, want)
+
+
+def test_decode_negative_and_zero_scale():
+    # softmax of zeros weights every visible key alike; a negative scale turns the
+    # order around.
+    for dtype in (torch.bfloat16, torch.float32):
+        for scale in (0.0, -0.3):
+            c = Paged([70, 300], [1, 1], 14, 2, 64, 16, dtype, 40, 5, seed=14)
+            c.scale = scale
+            c.check(c.decode())
+
+
 def test_decode_of_an_all_padding_batch_and_of_none():
     c = Paged([0, 0, 0], [1, 1, 1], 14, 2, 64, 16, torch.bfloat16, 40, 4)
     assert bool((c.decode() == SENTINEL).all())
@@ -400,6 +430,40 @@ def test_chunk_padding_rows_and_rows_past_the_last_chunk():
     assert torch.equal(out[: c.T], plain) and bool((out[c.T:] == SENTINEL).all())
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.3, 20.0])
+@pytest.mark.parametrize("dtype,head_dim", [(torch.bfloat16, 64), (torch.bfloat16, 128),
+                                            (torch.float32, 64)])
+def test_chunk_scales(scale, dtype, head_dim):
+    # 20 makes near one-hot rows whose maximum moves by far more than the rescaling
+    # slack from step to step.
+    news, priors = [150, 30], [300, 90]
+    c = Paged([p + n for p, n in zip(priors, news)], news, 8, 2, head_dim, 16, dtype, 200, 4,
+              seed=34)
+    c.scale = scale
+    out = c.chunks()
+    assert ops.take_status() == 0
+    c.check(out)
+
+
+def test_chunk_bound_far_above_the_tokens():
+    news, priors = [20, 150], [50, 0]
+    for dtype in (torch.bfloat16, torch.float32):
+        c = Paged([p + n for p, n in zip(priors, news)], news, 14, 2, 64, 16, dtype, 40, 4, seed=35)
+        assert torch.equal(c.chunks(max_query_len=1 << 30), c.chunks(max_query_len=170))
+
+
+@pytest.mark.parametrize("rows", [384, 385, 700])
+def test_chunk_many_sequences(rows):
+    # Up to 384 sequences are ranked inside every CTA, more run in order.
+    news = [1 + (7 * i) % 5 for i in range(rows)]
+    priors = [(37 * i) % 90 for i in range(rows)]
+    c = Paged([p + n for p, n in zip(priors, news)], news, 4, 2, 64, 16, torch.bfloat16, 40, 4,
+              seed=36)
+    out = c.chunks()
+    assert ops.take_status() == 0
+    c.check(out)
+
+
 def test_chunk_strided_query_and_output():
     news, priors = [20, 150], [50, 0]
     c = Paged([p + n for p, n in zip(priors, news)], news, 14, 2, 64, 16, torch.bfloat16, 40, 4,
@@ -475,6 +539,28 @@ def test_other_streams_and_two_calls_at_once():
         torch.cuda.synchronize()
         assert torch.equal(out_a, want_a) and torch.equal(twice, want_a)
         assert torch.equal(out_b, want_b)
+
+
+def test_a_captured_call_reports_after_the_workspace_has_grown():
+    c = Paged([70, 50], [1, 1], 14, 2, 64, 16, torch.bfloat16, 40, 5, seed=15)
+    q, out = c.q.to(DEV), torch.zeros(2, 14, 64, dtype=torch.bfloat16, device=DEV)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        ops.window_attention_batched(q, c.k, c.v, c.table, c.len_d, c.scale, 40, 5, out=out)
+        assert ops.take_status() == 0
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            ops.window_attention_batched(q, c.k, c.v, c.table, c.len_d, c.scale, 40, 5, out=out)
+        ops.workspace_for(torch.device("cuda", 0), 64 << 20)
+        c.len_d[1] = -1
+        graph.replay()
+        with pytest.raises(RuntimeError, match="context length"):
+            ops.take_status()
+        c.len_d[1] = 50
+        graph.replay()
+        assert ops.take_status() == 0
+        c.check(out)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
