@@ -11,9 +11,10 @@
 // computes key j's scores against the query rows (fp32 in shared memory, read as
 // broadcasts), the running softmax of a row comes from warp reductions, and the V
 // rows are weighted with lanes along head_dim.  No barrier until the four warps'
-// states are combined at the end.  Rows of more than 512 bytes leave V in the pool
-// (its copy would not fit), and rows that are not whole 16-byte pieces are read one
-// element at a time.
+// states are combined at the end.  Rows of more than 256 bytes copy V over K once the
+// scores are there: both would leave room for one CTA on an SM (fp32, d128, 200
+// sequences, window 2000: 140 us with both, 117 so; 47 sequences, window 900: 31 and
+// 33).  Rows that are not whole 16-byte pieces are read one element at a time.
 //
 // A weight of zero skips its V row, so NaN or infinities in a key that a row does
 // not see never reach that row.
@@ -60,21 +61,22 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Shared memory of one warp: 32 K rows, then 32 V rows where they fit; at the end its
-// state, GM rows of head_dim floats.  Lanes read K rows in parallel, so a pad of 16
-// bytes (one float in the element-wise form, which holds floats) moves consecutive
-// rows to different banks.
+// Shared memory of one warp: 32 K rows, then 32 V rows or the V rows in their place; at
+// the end its state, GM rows of head_dim floats.  Lanes read K rows in parallel, so a
+// pad of 16 bytes (one float in the element-wise form, which holds K as floats and
+// leaves V in the pool) moves consecutive rows to different banks.
 template <typename T, int GM, int DPL, bool VEC>
 struct Layout {
-  static constexpr bool kStageV = VEC && DPL * 32 * sizeof(T) <= 512;
+  static constexpr bool kVOverK = DPL * 32 * sizeof(T) > 256;
   __host__ __device__ static int k_row(int D) {
     return VEC ? D * static_cast<int>(sizeof(T)) + 16 : (D + 1) * 4;
   }
   __host__ __device__ static int v_row(int D) {
-    return kStageV ? D * static_cast<int>(sizeof(T)) : 0;
+    return kVOverK ? k_row(D) : D * static_cast<int>(sizeof(T));
   }
+  __host__ __device__ static int v_offset(int D) { return kVOverK ? 0 : 32 * k_row(D); }
   __host__ __device__ static int warp_bytes(int D) {
-    const int rows = 32 * (k_row(D) + v_row(D)), state = GM * D * 4;
+    const int rows = VEC ? v_offset(D) + 32 * v_row(D) : 32 * k_row(D), state = GM * D * 4;
     return ((rows > state ? rows : state) + 15) / 16 * 16;
   }
   __host__ __device__ static int q_bytes(int D) { return (GM * D * 4 + 15) / 16 * 16; }
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
   uint8_t* states = wsm + L_::q_bytes(D);
   const int warp_bytes = L_::warp_bytes(D), k_row = L_::k_row(D), v_row = L_::v_row(D);
   uint8_t* sK = states + warp * warp_bytes;
-  uint8_t* sV = sK + 32 * k_row;
+  uint8_t* sV = sK + L_::v_offset(D);
   float* probs = reinterpret_cast<float*>(states + kWarps * warp_bytes);
   float* sP = probs + warp * 32 * GM;
   float* sM = probs + kWarps * 32 * GM;
@@ -163,11 +165,11 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
       }
     }
     constexpr int kElems = 16 / sizeof(T);
-    if constexpr (VEC) {
-      // Copies of 16 bytes, consecutive lanes along a row; rows of no key stay as
-      // they are (their scores and weights are never used).
+    // Copies of 16 bytes, consecutive lanes along a row; rows of no key stay as they
+    // are (their scores and weights are never used).
+    auto copy_rows = [&](int first, int last) {  // 0: K, 1: V
       const int per_row = D / kElems;
-      for (int part = 0; part < (L_::kStageV ? 2 : 1); ++part) {
+      for (int part = first; part <= last; ++part) {
         const T* from = part == 0 ? kh : vh;
         uint8_t* to = part == 0 ? sK : sV;
         const int stride = part == 0 ? k_row : v_row;
@@ -180,7 +182,10 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
         }
         copy_commit();
       }
-      copy_wait<L_::kStageV ? 1 : 0>();
+    };
+    if constexpr (VEC) {
+      copy_rows(0, L_::kVOverK ? 0 : 1);
+      copy_wait<L_::kVOverK ? 0 : 1>();
     } else {
       for (int key = 0; key < 32; ++key) {
         const int64_t ko = __shfl_sync(0xffffffffu, off, key);
@@ -221,6 +226,10 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
         }
       }
     }
+    if constexpr (VEC && L_::kVOverK) {
+      __syncwarp();  // every lane has read its K row
+      copy_rows(1, 1);
+    }
 #pragma unroll
     for (int i = 0; i < GM; ++i) {
       if (i >= rows) {
@@ -243,19 +252,19 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
       for (int k = 0; k < DPL; ++k) o[i][k] *= corr;
       sP[lane * GM + i] = p;
     }
-    if constexpr (L_::kStageV) copy_wait<0>();
+    if constexpr (VEC) copy_wait<0>();
     __syncwarp();
     const uint32_t held = __ballot_sync(0xffffffffu, off >= 0);  // keys with a row
     const int nkeys = min(32, end - base);
 #pragma unroll 4
     for (int j = 0; j < nkeys; ++j) {
       if (!((held >> j) & 1u)) continue;
-      const int64_t vo = L_::kStageV ? 0 : __shfl_sync(0xffffffffu, off, j);
+      const int64_t vo = VEC ? 0 : __shfl_sync(0xffffffffu, off, j);
       float vv[DPL];
 #pragma unroll
       for (int k = 0; k < DPL; ++k) {
         const int d = lane + 32 * k;
-        if constexpr (L_::kStageV) {
+        if constexpr (VEC) {
           vv[k] = FULL || d < D ? to_float<T>(reinterpret_cast<const T*>(sV + j * v_row)[d]) : 0.f;
         } else {
           vv[k] = FULL || d < D ? to_float<T>(vh[vo + d]) : 0.f;
