@@ -202,8 +202,8 @@ int plan_mma_decode(const WindowShape& s, MmaDecodePlan* p) {
   return BS_OK;
 }
 
-// How the tensor-core prefill runs a call: one CTA per pair of 128-row query tiles,
-// kv head and range of key steps.
+// How the tensor-core prefill runs a call: one CTA per 128-row query tile, kv head and
+// range of key steps.
 struct MmaChunkPlan {
   int64_t tile_tokens, qtiles, items, splits, ml_offset, bytes;
 };
@@ -214,14 +214,14 @@ int plan_mma_chunks(const WindowShape& s, MmaChunkPlan* p) {
   int sms = 0;
   if (int rc = bsb::sm_count(&sms)) return rc;
   const int64_t groups = s.heads / s.kv_heads;
-  p->tile_tokens = 2 * (bsb::kWindowPairRows / 2 / groups);
+  p->tile_tokens = bsb::kWindowTileRows / groups;
   p->qtiles = (s.max_query_len + p->tile_tokens - 1) / p->tile_tokens;
   p->items = product(product(s.rows, p->qtiles), s.kv_heads);
   if (p->items < 0 || p->items > kInt32Max / bsb::kMaxWindowRanges / 8) {
     return fail(BS_ERR_UNSUPPORTED, "too many query tiles");
   }
-  // Pairs that can hold tokens (the others of a padded launch exit at once); one CTA
-  // runs per SM, so ranges are cut only as far as one wave of them goes.
+  // Tiles that can hold tokens (the others of a padded launch exit at once); two CTAs
+  // run on an SM, so ranges are cut only as far as one wave of them goes.
   const int64_t busy = std::max<int64_t>(
       1, std::min(s.rows * p->qtiles,
                   (s.tokens + p->tile_tokens - 1) / p->tile_tokens + s.rows) * s.kv_heads);
@@ -229,11 +229,11 @@ int plan_mma_chunks(const WindowShape& s, MmaChunkPlan* p) {
                                 std::min(s.window, kMaxContext) + std::min(s.sinks, kMaxContext) +
                                     p->tile_tokens + 32);
   const int64_t most = keys / (bsb::kWindowStepKeys * bsb::kMinWindowSteps);
-  const int64_t record = bsb::kWindowPairRows * (s.head_dim + 2) * 4;
+  const int64_t record = bsb::kWindowTileRows * (s.head_dim + 2) * 4;
   p->splits = std::max<int64_t>(
-      1, std::min(std::min<int64_t>(sms / busy, bsb::kMaxWindowRanges), most));
+      1, std::min(std::min<int64_t>(2ll * sms / busy, bsb::kMaxWindowRanges), most));
   while (p->splits > 1 && p->items * p->splits * record > kMaxRecordBytes) --p->splits;
-  p->ml_offset = p->items * p->splits * bsb::kWindowPairRows * s.head_dim;
+  p->ml_offset = p->items * p->splits * bsb::kWindowTileRows * s.head_dim;
   p->bytes = p->splits > 1 ? p->items * p->splits * record : 0;
   return BS_OK;
 }
@@ -349,7 +349,7 @@ int run_mma_chunks(const WindowShape& s, const WindowCall& c, bsb::WindowArgs& a
   const int64_t rows = s.kv_heads * c.num_blocks * s.block_size;
   const int64_t groups = s.heads / s.kv_heads;
   if (int rc = bsb::query_tensor_map(&qmap, c.query, s.tokens, c.q_stride, s.heads, s.head_dim,
-                                     groups, p.tile_tokens / 2)) {
+                                     groups, p.tile_tokens)) {
     return rc;
   }
   if (int rc = bsb::pool_tensor_map(&kmap, c.key_pool, rows, s.head_dim)) return rc;

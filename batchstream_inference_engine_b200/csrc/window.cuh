@@ -106,9 +106,9 @@ __host__ __device__ __forceinline__ int32_t window_range(int32_t count, int32_t 
 // Query rows (tokens x heads of one kv head) of a tile of the CUDA-core kernel.
 constexpr int kWindowSimtRows = 16;
 
-// Tensor-core chunks: rows of a record (two query tiles), the fewest steps of 64
-// keys in a range and the most ranges.
-constexpr int kWindowPairRows = 256;
+// Tensor-core chunks: rows of a query tile, the fewest steps of 64 keys in a range
+// and the most ranges.
+constexpr int kWindowTileRows = 128;
 constexpr int kWindowStepKeys = 64;
 constexpr int kMinWindowSteps = 4;
 constexpr int kMaxWindowRanges = 8;

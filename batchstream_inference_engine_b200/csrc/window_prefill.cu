@@ -2,44 +2,51 @@
 // cores (tcgen05 + TMEM): bf16, head_dim 64 or 128, block sizes that are multiples
 // of 16, up to 16 query heads per kv head.
 //
-// Query rows are packed: a tile's 128 rows are 128 / G consecutive tokens times the
-// G query heads of one kv head, so every K and V row that a CTA loads serves the
-// whole group, and the keys a tile reads beyond its window are those of a few
-// tokens (18 at G = 7) instead of 128.  One CTA takes two such tiles (A and B, the
-// tokens next to each other) over the same keys, in steps of 64 keys.
+// Query rows are packed: a CTA's tile of 128 rows is 128 / G consecutive tokens times
+// the G query heads of one kv head, so every K and V row that it loads serves the whole
+// group, and the keys it reads beyond its window are those of a few tokens (18 at G = 7)
+// instead of 128.
 //
 // The keys a CTA reads are 16-token units: the sink units, then the window's from
 // the first token any row sees to the last row's own.  A step is 4 units, each one
 // TMA box per K, V and 64 dims through the block table, so sink units and window
 // units share a step and nothing between them is touched.
 //
-// Roles (12 warps, one CTA per SM):
-//   * softmax A (warps 0-3) and B (warps 4-7), one thread per query row: S from
-//     TMEM, mask on border steps only, base-2 online softmax in fp32 whose maximum
-//     moves only when it grows by more than 2^8 (then O is rescaled in TMEM), P
-//     rounded to bf16 (the tensor cores' input) over the first half of S's columns;
-//   * MMA (warp 8): step t of a tile is O += P V of step t - 2 (P from TMEM), then
-//     S = Q K^T of step t over that P's columns (one thread's products execute in
-//     order), then one commit.  S has two buffers, so the scores of the next step are
-//     there when the softmax of this one ends: with one buffer of 128 keys it waited
-//     for both products, a third of each step;
-//   * loaders, of Q and K (warp 9) and of V (warp 10): a TMA box is only 16 rows, and
-//     issuing one takes a warp some 35 cycles, so one warp for both (16 boxes a step
-//     at head_dim 128) was what the steps waited for;
-//   * guard (warp 11): on border steps it zeroes the V rows that no row of the CTA
+// Roles (8 warps, two CTAs per SM):
+//   * softmax (warps 0-3), one thread per query row: S from TMEM, mask on border steps
+//     only, base-2 online softmax in fp32 whose maximum moves only when it grows by more
+//     than 2^8 (then O is rescaled in TMEM), P rounded to bf16 (the tensor cores' input)
+//     over the first half of S's columns;
+//   * MMA (warp 4): step t is O += P V of step t - 2 (P from TMEM), then S = Q K^T of
+//     step t over that P's columns (one thread's products execute in order), then one
+//     commit.  S has two buffers, so the scores of the next step are there when the
+//     softmax of this one ends;
+//   * loaders, of Q and K (warp 5) and of V (warp 6): a TMA box is only 16 rows, and
+//     issuing one takes a warp some 35 cycles;
+//   * guard (warp 7): on border steps it zeroes the V rows that no row of the CTA
 //     sees (never-loaded or stale memory, which 0 * NaN would let through), and the
 //     non-finite elements of the others, whose keys it lists: rows that do see such a
 //     key get its non-finite values added at the end, rows that do not stay clean.
 //
-// Bound: the exponentials (16 a clock and SM against 8192 tensor FLOP: 128 keys of
-// both tiles cost 2048 clocks of the special-function units, the products 1024 at
-// head_dim 64 and 2048 at 128).
+// A step of one tile takes 512 clocks of the special-function units (16 exponentials a
+// clock and SM) and 384 (head_dim 64) or 640 (128) of the tensor cores (a product of
+// 64 keys is bound by its operands in shared memory), but a softmax warp needs some
+// 1500 from scores to scores: its loads, maxima, exponentials and stores follow one
+// another.  Two CTAs to an SM overlap them, and one's start and end with the other's
+// steps.  Two tiles in one CTA over the same keys read half as much from L2, but start
+// and end together: 8 chunks of 512, d64, 14 heads, window 1024: 45.7 us so, 36.9 with
+// a tile each; 6 ragged chunks of 100 to 2048, d128, 28 heads, window 4096: 268 and
+// 243 us (990 TFLOP/s, 59% of the measured peak, with room for two stages only).  Over
+// 150 shapes the geometric mean fell by 8% (d64) and 11% (d128), the worst lost 10%.
+// Tried and slower: exponentials by the maximum of the steps before, checked afterwards
+// (more registers for a wait that the other CTA hides: 39.3 against 39.9 us, 254 and 257,
+// and slower for long chunks).
 //
-// A call with fewer CTAs than SMs cuts each tile pair's steps into ranges, whose
+// A call with fewer CTAs than two per SM cuts each tile's steps into ranges, whose
 // records window_prefill_merge_kernel joins in range order.
 //
 // Waits are bounded and their outcome made warp-uniform before warp-collective
-// instructions; the loader and the MMA warp drain what they started before TMEM is
+// instructions; the loaders and the MMA warp drain what they started before TMEM is
 // freed, also on the error path.
 #include "tcgen05.cuh"
 #include "window.cuh"
@@ -51,10 +58,10 @@ constexpr int kRows = 128;  // query rows of a tile (TMEM lanes)
 constexpr int kKeys = 64;   // keys of a step
 constexpr int kUnit = 16;   // tokens per unit (one TMA box)
 constexpr int kUnits = kKeys / kUnit;
-constexpr int kThreads = 384;
-constexpr int kMmaWarp = 8, kLoadKWarp = 9, kLoadVWarp = 10, kGuardWarp = 11;
-constexpr int kRing = 8;  // step barriers per tile (>= K stages, >= V stages)
-constexpr uint32_t kTmemCols = 512;  // S/P of A (two buffers), of B, O of A, O of B
+constexpr int kThreads = 256;
+constexpr int kMmaWarp = 4, kLoadKWarp = 5, kLoadVWarp = 6, kGuardWarp = 7;
+constexpr int kRing = 8;  // step barriers (>= K stages, >= V stages)
+constexpr uint32_t kTmemCols = 256;  // two S/P buffers, O
 constexpr float kLog2eP = 1.4426950408889634f;
 constexpr float kRescaleSlack = 8.f;
 constexpr int kMaxBad = 64;  // listed keys with non-finite V (more: all are looked at)
@@ -62,47 +69,32 @@ constexpr int kMaxBad = 64;  // listed keys with non-finite V (more: all are loo
 template <int D>
 struct Cfg {
   static constexpr int HALVES = D / 64;
-  static constexpr int KS = D == 64 ? 6 : 5;  // K stages
-  static constexpr int VS = D == 64 ? 6 : 4;  // V stages
+  // Stages of K and V: two CTAs share an SM's 227 KiB.
+  static constexpr int KS = D == 64 ? 5 : 2;
+  static constexpr int VS = D == 64 ? 5 : 2;
   static constexpr int Q_HALF_BYTES = kRows * 128;  // 64 dims of 128 rows
   static constexpr int Q_BYTES = HALVES * Q_HALF_BYTES;
   static constexpr int HALF_BYTES = kKeys * 128;
   static constexpr int STAGE_BYTES = HALVES * HALF_BYTES;
-  static constexpr int SMEM_BYTES = 2 * Q_BYTES + (KS + VS) * STAGE_BYTES;
-  static constexpr uint32_t O_COL = 256;
+  static constexpr int SMEM_BYTES = Q_BYTES + (KS + VS) * STAGE_BYTES;
+  static constexpr uint32_t O_COL = 2 * kKeys;  // behind the two S/P buffers
+  static_assert(O_COL + D <= kTmemCols, "TMEM columns");
   static_assert(KS <= kRing && VS <= kRing, "a step waiter could fall a whole ring behind");
 };
 
-// One tile's tokens and the steps that hold keys of its windows.  (Plain members and
-// selects: an array indexed by the tile would live in local memory, which this
-// kernel's shared memory leaves no L1 cache for.)
-struct TileSteps {
-  int32_t used;        // it holds tokens
-  int32_t pos0, pos1;  // first and last position of its tokens
-  int32_t first, last;
-};
-
-// The steps of a CTA's key range.
+// The units a tile reads.
 struct Steps {
   int32_t sink_units, first_unit, units;
-  TileSteps a, b;
-  __device__ __forceinline__ TileSteps tile(int x) const { return x == 0 ? a : b; }
-  __device__ __forceinline__ int32_t tiles() const { return b.used ? 2 : 1; }
+  int32_t pos0, pos1;  // first and last position of its tokens
 };
 
-__device__ __forceinline__ Steps steps_of(const WindowArgs& a, const WindowTile& w, int32_t tt) {
+__device__ __forceinline__ Steps steps_of(const WindowArgs& a, const WindowTile& w) {
   Steps s;
   s.first_unit = w.lo / kUnit;
   s.sink_units = min((a.sinks + kUnit - 1) / kUnit, s.first_unit);
-  const int32_t end = w.pos0 + w.ntok - 1;
-  s.units = s.sink_units + end / kUnit - s.first_unit + 1;
-  auto tile = [&](int32_t used, int32_t pos0, int32_t pos1) {
-    const int32_t lo = max(0, pos0 - a.window + 1);
-    return TileSteps{used, pos0, pos1, (s.sink_units + lo / kUnit - s.first_unit) / kUnits,
-                     (s.sink_units + pos1 / kUnit - s.first_unit) / kUnits};
-  };
-  s.a = tile(1, w.pos0, min(end, w.pos0 + tt - 1));
-  s.b = tile(w.ntok > tt ? 1 : 0, w.pos0 + tt, end);
+  s.pos0 = w.pos0;
+  s.pos1 = w.pos0 + w.ntok - 1;
+  s.units = s.sink_units + s.pos1 / kUnit - s.first_unit + 1;
   return s;
 }
 
@@ -115,44 +107,38 @@ __device__ __forceinline__ int32_t unit_pos(const Steps& s, int32_t x) {
   return (x < s.sink_units ? x : x - s.sink_units + s.first_unit) * kUnit;
 }
 
-// Whether a tile has keys in step j.
-__device__ __forceinline__ bool step_active(const Steps& s, const TileSteps& t, int32_t j) {
-  return t.used && j <= t.last && (j >= t.first || j * kUnits < s.sink_units);
-}
-
-// Whether some row of a tile does not see some key of step j.
-__device__ __forceinline__ bool step_masked(const WindowArgs& a, const Steps& s,
-                                            const TileSteps& t, int32_t j) {
+// Whether some row of the tile does not see some key of step j.
+__device__ __forceinline__ bool step_masked(const WindowArgs& a, const Steps& s, int32_t j) {
   const int32_t u0 = j * kUnits, u1 = u0 + kUnits - 1;
-  if (u1 >= s.units || unit_pos(s, u1) + kUnit - 1 > t.pos0) return true;
+  if (u1 >= s.units || unit_pos(s, u1) + kUnit - 1 > s.pos0) return true;
   if (u0 < s.sink_units && a.sinks < min(u1 + 1, s.sink_units) * kUnit) return true;
   // The step's first window unit against the last row's window.
-  return u1 >= s.sink_units && unit_pos(s, max(u0, s.sink_units)) <= t.pos1 - a.window;
+  return u1 >= s.sink_units && unit_pos(s, max(u0, s.sink_units)) <= s.pos1 - a.window;
 }
 
-// Steps [lo, hi] of a tile that need no mask (every row sees every key): behind the
+// Steps [lo, hi] that need no mask (every row sees every key): behind the
 // sinks, the units from the first that all windows hold whole to the last that ends at
 // or before the first row.
-__device__ __forceinline__ void plain_steps(const WindowArgs& a, const Steps& s,
-                                            const TileSteps& t, int32_t& lo, int32_t& hi) {
-  const int32_t out = t.pos1 - a.window;  // the last position that some row does not see
+__device__ __forceinline__ void plain_steps(const WindowArgs& a, const Steps& s, int32_t& lo,
+                                            int32_t& hi) {
+  const int32_t out = s.pos1 - a.window;  // the last position that some row does not see
   const int32_t whole = out < 0 ? 0 : out / kUnit + 1;
   lo = (s.sink_units + max(whole - s.first_unit, 0) + kUnits - 1) / kUnits;
-  hi = (s.sink_units + (t.pos0 + 1) / kUnit - s.first_unit) / kUnits - 1;
+  hi = (s.sink_units + (s.pos0 + 1) / kUnit - s.first_unit) / kUnits - 1;
 }
 
 __device__ __forceinline__ bool sees(const WindowArgs& a, int32_t qpos, int32_t pos) {
   return pos <= qpos && (pos < a.sinks || pos > qpos - a.window);
 }
 
-// Ranges a tile pair with `steps` steps is cut into.
+// Ranges a tile with `steps` steps is cut into.
 __device__ __forceinline__ int32_t step_ranges(int32_t steps, int32_t splits) {
   const int32_t most = (steps + kMinWindowSteps - 1) / kMinWindowSteps;
   return most < splits ? most : splits;
 }
 
-// Linear item -> (sequence, tile pair, kv head), which also numbers the records.
-__device__ __forceinline__ void pair_of(const WindowArgs& a, int32_t item, int32_t& r,
+// Linear item -> (sequence, tile, kv head), which also numbers the records.
+__device__ __forceinline__ void tile_of(const WindowArgs& a, int32_t item, int32_t& r,
                                         int32_t& tile, int32_t& h) {
   h = item % a.num_kv_heads;
   item /= a.num_kv_heads;
@@ -163,11 +149,11 @@ __device__ __forceinline__ void pair_of(const WindowArgs& a, int32_t item, int32
 // Most sequences that every CTA ranks (one a thread).
 constexpr int kMaxRanked = kThreads;
 
-// The sequence, tile pair and kv head of launch index b: the sequences with the most
+// The sequence, tile and kv head of launch index b: the sequences with the most
 // steps first, a sequence's last tiles, which see the most keys, ahead of its others.
 // A step range is the whole of a CTA's time, so the long ones must not start last.
 // All threads call it; `steps` and `pick` are shared memory.
-__device__ __forceinline__ void ranked_pair(const WindowArgs& a, int32_t b, int32_t (&steps)[kMaxRanked],
+__device__ __forceinline__ void ranked_tile(const WindowArgs& a, int32_t b, int32_t (&steps)[kMaxRanked],
                                             int32_t& pick, int32_t& r, int32_t& tile, int32_t& h) {
   h = b % a.num_kv_heads;
   b /= a.num_kv_heads;
@@ -202,33 +188,32 @@ __device__ __forceinline__ uint32_t fma_zero_bf16x2(uint32_t a, uint32_t c) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 2)
     window_prefill_kernel(const __grid_constant__ CUtensorMap qmap,
                           const __grid_constant__ CUtensorMap kmap,
                           const __grid_constant__ CUtensorMap vmap, const WindowArgs a) {
   using C = Cfg<D>;
   extern __shared__ __align__(1024) uint8_t smem[];  // 128-byte swizzle atoms
-  __shared__ uint64_t q_full, k_full[C::KS], v_full[C::VS], v_ok[C::VS], step_done[2][kRing],
-      p_full[2][2], a_ahead, mma_done;
+  __shared__ uint64_t q_full, k_full[C::KS], v_full[C::VS], v_ok[C::VS], step_done[kRing],
+      p_full[2], mma_done;
   __shared__ uint32_t tmem_base;
   __shared__ int32_t bad_count, bad_pos[kMaxBad];
 
-  auto sQ = [&](int x) { return smem + x * C::Q_BYTES; };
-  auto sK = [&](int st) { return smem + 2 * C::Q_BYTES + st * C::STAGE_BYTES; };
-  auto sV = [&](int st) { return smem + 2 * C::Q_BYTES + (C::KS + st) * C::STAGE_BYTES; };
+  uint8_t* const sQ = smem;
+  auto sK = [&](int st) { return smem + C::Q_BYTES + st * C::STAGE_BYTES; };
+  auto sV = [&](int st) { return smem + C::Q_BYTES + (C::KS + st) * C::STAGE_BYTES; };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   pdl_wait();
-  const int32_t tt = a.tile_tokens / 2;  // tokens of one tile
   const int32_t split = blockIdx.x % a.splits;
   __shared__ int32_t ranked[kMaxRanked], picked;
   int32_t r, tile, h;
-  ranked_pair(a, blockIdx.x / a.splits, ranked, picked, r, tile, h);
-  // The item of its records (pair_of).
+  ranked_tile(a, blockIdx.x / a.splits, ranked, picked, r, tile, h);
+  // The item of its records (tile_of).
   const int32_t item = ((a.qtiles - 1 - tile) * a.num_rows + r) * a.num_kv_heads + h;
   WindowTile w;
   if (!window_tile(a, r, tile, w, tid == 0 && tile == 0 && h == 0 && split == 0)) return;
-  const Steps sd = steps_of(a, w, tt);
+  const Steps sd = steps_of(a, w);
   const int32_t all = step_count(sd);
   const int32_t ranges = step_ranges(all, a.splits);
   if (split >= ranges) return;
@@ -242,11 +227,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&v_full[s], 1);
       mbar_init(&v_ok[s], 1);
     }
-    for (int x = 0; x < 2; ++x) {
-      for (int s = 0; s < kRing; ++s) mbar_init(&step_done[x][s], 1);
-      for (int b = 0; b < 2; ++b) mbar_init(&p_full[x][b], kRows);
-    }
-    mbar_init(&a_ahead, kRows);
+    for (int s = 0; s < kRing; ++s) mbar_init(&step_done[s], 1);
+    for (int b = 0; b < 2; ++b) mbar_init(&p_full[b], kRows);
     mbar_init(&mma_done, 1);
     fence_barrier_init();
     bad_count = 0;
@@ -265,11 +247,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto wait_all = [&](uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
   };
-  // Step u of tile x is done: P V of step u - 2 and S of step u.  Waiters take the
-  // steps in order and are never kRing behind (see the ring sizes).
-  auto wait_step = [&](int x, int u) {
-    return wait_all(&step_done[x][u % kRing], (u / kRing) & 1);
-  };
+  // Step u is done: P V of step u - 2 and S of step u.  Waiters take the steps in order
+  // and are never kRing behind (see the ring sizes).
+  auto wait_step = [&](int u) { return wait_all(&step_done[u % kRing], (u / kRing) & 1); };
 
   if (warp == kLoadKWarp || warp == kLoadVWarp) {
     // ---------------------------------------------------------------- loaders
@@ -298,24 +278,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     int32_t y = fetch(0), y_next = fetch(1);
     if (is_k && lane == 0) {
-      const uint32_t rows = static_cast<uint32_t>(tt * a.groups);
-      mbar_arrive_expect_tx(&q_full, sd.tiles() * C::HALVES * rows * 128u);
-      for (int x = 0; x < sd.tiles(); ++x) {
-        for (int hf = 0; hf < C::HALVES; ++hf) {
-          tma_load_3d(sQ(x) + hf * C::Q_HALF_BYTES, &qmap, &q_full, hf * 64, h * a.groups,
-                      w.tok0 + x * tt);
-        }
+      const uint32_t rows = static_cast<uint32_t>(a.tile_tokens * a.groups);
+      mbar_arrive_expect_tx(&q_full, C::HALVES * rows * 128u);
+      for (int hf = 0; hf < C::HALVES; ++hf) {
+        tma_load_3d(sQ + hf * C::Q_HALF_BYTES, &qmap, &q_full, hf * 64, h * a.groups, w.tok0);
       }
     }
     __syncwarp();
-    // Step j - KS has read the K stage, step j - VS + 2 the V stage (of both tiles: B's
-    // commit follows A's products).
+    // Step j - KS has read the K stage, step j - VS + 2 the V stage.
     const int32_t lag = is_k ? 0 : 2;
     bool ok = true;
     int32_t loads = 0;
     int stage = 0;
     for (int32_t j = 0; j < n; ++j) {
-      if (j >= stages) ok = wait_step(1, j - stages + lag);
+      if (j >= stages) ok = wait_step(j - stages + lag);
       if (!ok) break;
       const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, y >= 0));
       if (lane == 0) mbar_arrive_expect_tx(full + stage, boxes * 2048u);
@@ -336,9 +312,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------------------------------------------------------- MMA issuer
     constexpr uint32_t kIdescS = umma_idesc(128, kKeys, 0, 0);
     constexpr uint32_t kIdescO = umma_idesc(128, D, 0, 1);
-    constexpr uint32_t kQStep = C::Q_BYTES >> 4, kQHalf = C::Q_HALF_BYTES >> 4;
+    constexpr uint32_t kQHalf = C::Q_HALF_BYTES >> 4;
     constexpr uint32_t kStageStep = C::STAGE_BYTES >> 4, kHalf = C::HALF_BYTES >> 4;
-    const uint64_t desc_q = umma_desc(smem_u32(sQ(0)), 16, 1024);
+    const uint64_t desc_q = umma_desc(smem_u32(sQ), 16, 1024);
     const uint32_t hi = static_cast<uint32_t>(desc_q >> 32);  // of every operand
     const uint32_t q_lo = static_cast<uint32_t>(desc_q);
     const uint32_t k_lo = static_cast<uint32_t>(umma_desc(smem_u32(sK(0)), 16, 1024));
@@ -347,58 +323,44 @@ __global__ void __launch_bounds__(kThreads, 1)
         static_cast<uint32_t>(umma_desc(smem_u32(sV(0)), C::HALF_BYTES, 1024));
     const uint32_t mine = elect_lane();  // issues every product
     bool ok = wait_all(&q_full, 0);
-    // Steps in which tile x has keys: the sinks' and [from[x], to[x]] (step_active).
-    const int32_t sink_steps = (sd.sink_units + kUnits - 1) / kUnits - j0;
-    const int32_t from[2] = {sd.a.first - j0, sd.b.first - j0};
-    const int32_t to[2] = {sd.a.last - j0, sd.b.used ? sd.b.last - j0 : -1};
-    // By tile: whether it has a P V product yet, and the phase of each P buffer (bit).
-    // Ring positions and phases are carried along: this warp's own instructions,
-    // products apart, must stay well below a step's time.  (A warp per tile, the guard
-    // moved into V's loader to make room for it, measured 6 to 9% slower.)
-    uint32_t started[2] = {0, 0}, phases[2] = {0, 0};
+    // Ring positions and phases are carried along: this warp's own instructions, products
+    // apart, must stay well below a step's time.
     int ks = 0, vs = 0;
     uint32_t k_phase = 0, v_phase = 0;
     for (int32_t u = 0; u < n + 2 && ok; ++u) {
       const int b = u & 1;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        auto active = [&](int32_t j) { return j <= to[x] && (j >= from[x] || j < sink_steps); };
-        const bool pv = u > 1 && active(u - 2);
-        const bool qk = u < n && active(u);
-        // P last: K and V are there long before it.
-        if (qk) ok = wait_all(&k_full[ks], k_phase);
-        if (pv) {
-          ok = ok && wait_all(&v_ok[vs], v_phase);
-          ok = ok && wait_all(&p_full[x][b], (phases[x] >> b) & 1u);
-        }
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t s_col = tmem + (2 * x + b) * kKeys;
-        if (pv) {
-          const uint32_t v0 = v_lo + vs * kStageStep;
-          unroll<kKeys / 16>([&](auto k) {
-            // P: 8 columns per 16 keys; V: 16 rows of 128 bytes.
-            umma_f16_ts_elect<8 * k, 128 * k>(mine, tmem + C::O_COL + x * D, s_col, v0, hi,
-                                              kIdescO, k > 0 ? 1u : started[x]);
-          });
-          started[x] = 1u;
-          phases[x] ^= 1u << b;
-        }
-        if (qk) {
-          const uint32_t q0 = q_lo + x * kQStep, k0 = k_lo + ks * kStageStep;
-          unroll<D / 16>([&](auto k) {
-            // 32 bytes a slice of 16 dims.
-            umma_f16_elect<(k / 4) * kQHalf + 2 * (k % 4), (k / 4) * kHalf + 2 * (k % 4)>(
-                mine, s_col, q0, k0, hi, kIdescS, k > 0 ? 1u : 0u);
-          });
-        }
-        umma_commit_elect(mine, &step_done[x][u % kRing]);
+      const bool pv = u > 1, qk = u < n;
+      // P last: K and V are there long before it.
+      if (qk) ok = wait_all(&k_full[ks], k_phase);
+      if (pv) {
+        ok = ok && wait_all(&v_ok[vs], v_phase);
+        ok = ok && wait_all(&p_full[b], ((u >> 1) & 1) ^ 1);  // of step u - 2
       }
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t s_col = tmem + b * kKeys;
+      if (pv) {
+        const uint32_t v0 = v_lo + vs * kStageStep;
+        unroll<kKeys / 16>([&](auto k) {
+          // P: 8 columns per 16 keys; V: 16 rows of 128 bytes.
+          umma_f16_ts_elect<8 * k, 128 * k>(mine, tmem + C::O_COL, s_col, v0, hi, kIdescO,
+                                            k > 0 || u > 2 ? 1u : 0u);
+        });
+      }
+      if (qk) {
+        const uint32_t k0 = k_lo + ks * kStageStep;
+        unroll<D / 16>([&](auto k) {
+          // 32 bytes a slice of 16 dims.
+          umma_f16_elect<(k / 4) * kQHalf + 2 * (k % 4), (k / 4) * kHalf + 2 * (k % 4)>(
+              mine, s_col, q_lo, k0, hi, kIdescS, k > 0 ? 1u : 0u);
+        });
+      }
+      umma_commit_elect(mine, &step_done[u % kRing]);
       if (++ks == C::KS) {
         ks = 0;
         k_phase ^= 1u;
       }
-      if (u > 1 && ++vs == C::VS) {
+      if (pv && ++vs == C::VS) {
         vs = 0;
         v_phase ^= 1u;
       }
@@ -409,16 +371,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if ((!ok || !drained) && lane == 0) set_status(a.status, kStatusWaitTimeout);
   } else if (warp == kGuardWarp) {
     // ---------------------------------------------------------------- guard
-    const int32_t end = w.pos0 + w.ntok - 1;
     bool ok = true;
     for (int32_t j = 0; j < n; ++j) {
       const int vs = j % C::VS;
       ok = wait_all(&v_full[vs], (j / C::VS) & 1);
       if (!ok) break;
-      const bool border =
-          (step_active(sd, sd.a, j0 + j) && step_masked(a, sd, sd.a, j0 + j)) ||
-          (step_active(sd, sd.b, j0 + j) && step_masked(a, sd, sd.b, j0 + j));
-      if (border) {
+      if (step_masked(a, sd, j0 + j)) {
         auto position = [&](int row) {  // of the key of a V row
           return unit_pos(sd, (j0 + j) * kUnits + row / kUnit) + row % kUnit;
         };
@@ -427,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int g = 0; g < kKeys / 32; ++g) {
           const int row = g * 32 + lane;
           const int32_t pos = position(row);
-          const bool live = (j0 + j) * kUnits + row / kUnit < sd.units && pos <= end &&
+          const bool live = (j0 + j) * kUnits + row / kUnit < sd.units && pos <= sd.pos1 &&
                             (pos < a.sinks || pos >= w.lo);
           const uint32_t dead = __ballot_sync(0xffffffffu, !live);
           for (int q = 0; q < 8; ++q) {
@@ -488,30 +446,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok && lane == 0) set_status(a.status, kStatusWaitTimeout);
   } else {
     // ---------------------------------------------------------------- softmax
-    const int x = warp >> 2;
-    const TileSteps ts = sd.tile(x);
-    const int row = tid & (kRows - 1);
+    const int row = tid;
     const int32_t tok = row / a.groups, g = row - tok * a.groups;
-    const bool live = x * tt + tok < w.ntok && tok < tt;
-    const int32_t qpos = w.pos0 + x * tt + tok;
-    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t o_addr = tmem + lane_base + C::O_COL + x * D;
+    const bool live = tok < w.ntok;
+    const int32_t qpos = w.pos0 + tok;
+    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t o_addr = tmem + lane_base + C::O_COL;
     const float zscale = fabsf(a.scale) * kLog2eP;
     float m_used = -INFINITY, l_run = 0.f;
-    int32_t done = 0;
     int32_t plain_lo, plain_hi;
-    plain_steps(a, sd, ts, plain_lo, plain_hi);
-    const bool a_first = step_active(sd, sd.a, j0);  // A has a step here, the first one
+    plain_steps(a, sd, plain_lo, plain_hi);
     bool ok = true;
     for (int32_t u = 0; u < n; ++u) {
-      ok = wait_step(x, u);
+      ok = wait_step(u);
       if (!ok) break;
-      const bool plain = j0 + u >= plain_lo && j0 + u <= plain_hi;
-      if (!plain && !step_active(sd, ts, j0 + u)) continue;
       tc_fence_after();
-      const uint32_t s_addr = tmem + lane_base + (2 * x + (u & 1)) * kKeys;
+      const uint32_t s_addr = tmem + lane_base + (u & 1) * kKeys;
       // Visible tokens of the step's units, 16 bits each (border steps only).
-      const bool border = !plain && step_masked(a, sd, ts, j0 + u);
+      const bool border =
+          (j0 + u < plain_lo || j0 + u > plain_hi) && step_masked(a, sd, j0 + u);
       uint32_t maps[2];
       if (border) {
         auto below = [](int32_t c) -> uint32_t {  // map of the first c tokens
@@ -531,6 +484,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld32(s_addr, v[0]);
       tmem_ld32(s_addr + 32, v[1]);
       tmem_wait_ld();
+      tmem_settle(v[0]);
+      tmem_settle(v[1]);
       if (a.scale < 0.f) {  // turned around: the rest works with the scale's magnitude
 #pragma unroll
         for (int i = 0; i < 64; ++i) v[i / 32][i % 32] ^= 0x80000000u;
@@ -548,12 +503,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float m_step = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * zscale;
       const bool grow = live && m_step > m_used + kRescaleSlack;
-      if (done == 0) {
+      if (u == 0) {
         m_used = m_step;
       } else if (__any_sync(0xffffffffu, grow)) {
         // O may be rescaled once P V of the step before is done; rows that did not
         // grow keep theirs (factor 1).
-        ok = wait_step(x, u + 1);
+        ok = wait_step(u + 1);
         if (!ok) break;
         tc_fence_after();
         const float m_new = grow ? m_step : m_used;
@@ -563,18 +518,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t o[32];
           tmem_ld32(o_addr + c0, o);
           tmem_wait_ld();
+          tmem_settle(o);
 #pragma unroll
           for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
           tmem_st32(o_addr + c0, o);
         }
         l_run *= corr;
         m_used = m_new;
-      }
-      // B's first exponentials wait for A's, once: from then on one tile uses the
-      // special-function units while the other loads, reduces and stores.
-      if (x == 1 && done == 0 && a_first) {
-        ok = wait_all(&a_ahead, 0);
-        if (!ok) break;
       }
       const float m_base = m_used == -INFINITY ? 0.f : m_used;  // no -inf - -inf
       const float2 zs2 = make_float2(zscale, zscale), mm = make_float2(-m_base, -m_base);
@@ -593,35 +543,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_st32(s_addr, p);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&p_full[x][u & 1]);
-      if (x == 0 && done == 0) mbar_arrive(&a_ahead);
+      mbar_arrive(&p_full[u & 1]);
       l_run += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) +
                ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
-      ++done;
     }
     // The last P V is done (the steps in order, as everywhere).
-    if (ok) ok = wait_step(x, n) && wait_step(x, n + 1);
+    if (ok) ok = wait_step(n) && wait_step(n + 1);
     if (!ok) {
       if (lane == 0) set_status(a.status, kStatusWaitTimeout);
-    } else if (ts.used) {
+    } else {
       tc_fence_after();
       const bool split_up = ranges > 1;
       // Listed keys are complete: the guard arrived for every V that was used.
       const int32_t bad = bad_count;
-      const float scale = split_up || done == 0 ? 1.f : 1.f / l_run;
+      const float scale = split_up ? 1.f : 1.f / l_run;
       const int32_t* table = a.block_tables + static_cast<int64_t>(w.row) * a.bt_stride;
-      const int64_t rec_row = (static_cast<int64_t>(item) * a.splits + split) * 2 * kRows +
-                              x * kRows + row;
+      const int64_t rec_row = (static_cast<int64_t>(item) * a.splits + split) * kRows + row;
 #pragma unroll
       for (int c0 = 0; c0 < D; c0 += 32) {
         uint32_t v[32];
-        if (done > 0) {
-          tmem_ld32(o_addr + c0, v);
-          tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) v[c] = 0u;
-        }
+        tmem_ld32(o_addr + c0, v);
+        tmem_wait_ld();
+        tmem_settle(v);
 #pragma unroll
         for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * scale);
         if (bad > 0 && live) {
@@ -658,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
           __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) +
-                               static_cast<int64_t>(w.tok0 + x * tt + tok) * a.o_stride +
+                               static_cast<int64_t>(w.tok0 + tok) * a.o_stride +
                                static_cast<int64_t>(h * a.groups + g) * D + c0;
 #pragma unroll
           for (int c = 0; c < 32; c += 8) {
@@ -686,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the records of a tile pair's step ranges, in range order: eight threads a
+// Joins the records of a tile's step ranges, in range order: eight threads a
 // row, D / 8 columns each.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeRows = kMergeThreads / 8;
@@ -694,35 +637,33 @@ constexpr int kMergeRows = kMergeThreads / 8;
 template <int D>
 __global__ void __launch_bounds__(kMergeThreads) window_prefill_merge_kernel(const WindowArgs a) {
   pdl_wait();
-  constexpr int kParts = 2 * kRows / kMergeRows;  // CTAs per tile pair
+  constexpr int kParts = kRows / kMergeRows;  // CTAs per tile
   const int32_t item = blockIdx.x / kParts;
   int32_t r, tile, h;
-  pair_of(a, item, r, tile, h);
+  tile_of(a, item, r, tile, h);
   WindowTile w;
   if (!window_tile(a, r, tile, w, false)) return;
-  const int32_t tt = a.tile_tokens / 2;
-  const int32_t prow = (blockIdx.x % kParts) * kMergeRows + threadIdx.x / 8;
-  const int32_t x = prow / kRows, row = prow % kRows;
+  const int32_t row = (blockIdx.x % kParts) * kMergeRows + threadIdx.x / 8;
   const int32_t tok = row / a.groups, g = row - tok * a.groups;
-  if (tok >= tt || x * tt + tok >= w.ntok) return;
-  const Steps sd = steps_of(a, w, tt);
+  if (tok >= w.ntok) return;
+  const Steps sd = steps_of(a, w);
   const int32_t ranges = step_ranges(step_count(sd), a.splits);
   if (ranges <= 1) return;  // written by the kernel itself
   const int32_t c = (threadIdx.x % 8) * (D / 8);
-  const int64_t rec0 = static_cast<int64_t>(item) * a.splits * 2 * kRows + prow;
+  const int64_t rec0 = static_cast<int64_t>(item) * a.splits * kRows + row;
   const float* ml = a.records + a.rec_stride_ml;
   float M = -INFINITY;
-  for (int32_t s = 0; s < ranges; ++s) M = fmaxf(M, ml[(rec0 + s * 2 * kRows) * 2]);
+  for (int32_t s = 0; s < ranges; ++s) M = fmaxf(M, ml[(rec0 + s * kRows) * 2]);
   float L = 0.f, acc[D / 8];
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) acc[i] = 0.f;
 #pragma unroll 4
   for (int32_t s = 0; s < ranges; ++s) {
-    const float2 p = *reinterpret_cast<const float2*>(ml + (rec0 + s * 2 * kRows) * 2);
+    const float2 p = *reinterpret_cast<const float2*>(ml + (rec0 + s * kRows) * 2);
     if (p.x == -INFINITY) continue;  // no key of this row in the range
     const float f = fast_exp2(p.x - M);
     L += f * p.y;
-    const float4* o = reinterpret_cast<const float4*>(a.records + (rec0 + s * 2 * kRows) * D + c);
+    const float4* o = reinterpret_cast<const float4*>(a.records + (rec0 + s * kRows) * D + c);
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
       const float4 v = o[i];
@@ -734,7 +675,7 @@ __global__ void __launch_bounds__(kMergeThreads) window_prefill_merge_kernel(con
   }
   const float inv = 1.f / L;
   __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) +
-                       static_cast<int64_t>(w.tok0 + x * tt + tok) * a.o_stride +
+                       static_cast<int64_t>(w.tok0 + tok) * a.o_stride +
                        static_cast<int64_t>(h * a.groups + g) * D + c;
 #pragma unroll
   for (int i = 0; i < D / 8; i += 8) {
@@ -768,7 +709,7 @@ int launch_d(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& km
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, window_prefill_kernel<D>, qmap, kmap, vmap, a);
   if (e != cudaSuccess || a.splits == 1) return static_cast<int>(e);
-  cfg.gridDim = dim3(static_cast<unsigned>(items * (2 * kRows / kMergeRows)));
+  cfg.gridDim = dim3(static_cast<unsigned>(items * (kRows / kMergeRows)));
   cfg.blockDim = dim3(kMergeThreads);
   cfg.dynamicSmemBytes = 0;
   return static_cast<int>(cudaLaunchKernelEx(&cfg, window_prefill_merge_kernel<D>, a));
