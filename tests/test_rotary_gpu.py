@@ -234,3 +234,30 @@ def test_wrapper_refuses():
         with pytest.raises(RuntimeError):
             call(**kw)
     assert ops.take_status() == 0
+
+
+def test_query_out_must_not_overlap_qkv():
+    # q in place would be read by other threads after it was written.
+    c = Case(5, 14, 2, 64, 64, False, torch.bfloat16, torch.bfloat16)
+    rows = c.qkv.contiguous()
+    inside = rows.view(-1)[: 5 * 14 * 64].view(5, 14, 64)
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.rotary_append(rows, c.freq, c.pos, c.slots, c.k, c.v, 14, query_out=inside)
+
+
+@pytest.mark.parametrize("pool_dtype,head_dim", [(torch.bfloat16, 64), (torch.float32, 72)])
+def test_slots_past_32_bit_offsets(pool_dtype, head_dim):
+    # More than 2^31 elements a pool, the slots at its end; the same rows as in a small pool.
+    blocks = 1_100_000
+    c = Case(5, 14, 2, head_dim, head_dim, False, torch.bfloat16, pool_dtype)
+    assert 2 * blocks * 16 * head_dim > 2 ** 31
+    k = torch.zeros(2, blocks, 16, head_dim, dtype=pool_dtype, device=DEV)
+    v = torch.zeros_like(k)
+    small_k = torch.zeros(2, 8, 16, head_dim, dtype=pool_dtype, device=DEV)
+    small_v = torch.zeros_like(small_k)
+    slots = torch.tensor([0, 127, 5, 64, 126], dtype=torch.int32, device=DEV)
+    want = ops.rotary_append(c.qkv, c.freq, c.pos, slots, small_k, small_v, 14)
+    got = ops.rotary_append(c.qkv, c.freq, c.pos, slots + (blocks - 8) * 16, k, v, 14)
+    assert ops.take_status() == 0
+    assert torch.equal(got, want)
+    assert torch.equal(k[:, blocks - 8:], small_k) and torch.equal(v[:, blocks - 8:], small_v)

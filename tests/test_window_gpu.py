@@ -452,9 +452,9 @@ def test_chunk_bound_far_above_the_tokens():
         assert torch.equal(c.chunks(max_query_len=1 << 30), c.chunks(max_query_len=170))
 
 
-@pytest.mark.parametrize("rows", [384, 385, 700])
+@pytest.mark.parametrize("rows", [256, 257, 384, 385, 700])
 def test_chunk_many_sequences(rows):
-    # Up to 384 sequences are ranked inside every CTA, more run in order.
+    # Up to 256 sequences are ranked inside every CTA, more run in order.
     news = [1 + (7 * i) % 5 for i in range(rows)]
     priors = [(37 * i) % 90 for i in range(rows)]
     c = Paged([p + n for p, n in zip(priors, news)], news, 4, 2, 64, 16, torch.bfloat16, 40, 4,
@@ -462,6 +462,32 @@ def test_chunk_many_sequences(rows):
     out = c.chunks()
     assert ops.take_status() == 0
     c.check(out)
+
+
+@pytest.mark.parametrize("dtype,head_dim,blocks", [
+    (torch.bfloat16, 128, 600_000), (torch.bfloat16, 64, 1_200_000), (torch.float32, 80, 850_000)])
+def test_pool_past_32_bit_offsets(dtype, head_dim, blocks):
+    # More than 2^31 elements a pool, the sequences in the last blocks of the last head.
+    news, priors = [20, 150], [700, 0]
+    c = Paged([p + n for p, n in zip(priors, news)], news, 14, 2, head_dim, 16, dtype, 400, 4,
+              seed=38)
+    few = c.k.shape[1]
+    assert 2 * blocks * 16 * head_dim > 2 ** 31
+    for name in ("k", "v"):
+        small = getattr(c, name)
+        big = torch.zeros(2, blocks, 16, head_dim, dtype=dtype, device=DEV)
+        big[:, blocks - few:] = small
+        setattr(c, name, big)
+    c.table[c.table < few] += blocks - few
+    c.check(c.chunks())
+    one = Paged([720, 150], [1, 1], 14, 2, head_dim, 16, dtype, 400, 4, seed=39)
+    few = one.k.shape[1]
+    for name in ("k", "v"):
+        getattr(c, name)[:, blocks - few:] = getattr(one, name)
+        setattr(one, name, getattr(c, name))
+    one.table[one.table < few] += blocks - few
+    one.check(one.decode())
+    assert ops.take_status() == 0
 
 
 def test_chunk_strided_query_and_output():
