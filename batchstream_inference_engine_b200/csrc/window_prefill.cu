@@ -40,7 +40,8 @@
 // 150 shapes the geometric mean fell by 8% (d64) and 11% (d128), the worst lost 10%.
 // Tried and slower: exponentials by the maximum of the steps before, checked afterwards
 // (more registers for a wait that the other CTA hides: 39.3 against 39.9 us, 254 and 257,
-// and slower for long chunks).
+// and slower for long chunks); two threads a row, 32 keys each, that swap their maxima
+// (what a step costs whatever its keys is paid twice: 40.5 against 36.7, 269 and 243).
 //
 // A call with fewer CTAs than two per SM cuts each tile's steps into ranges, whose
 // records window_prefill_merge_kernel joins in range order.
