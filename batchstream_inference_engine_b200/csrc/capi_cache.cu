@@ -153,12 +153,13 @@ constexpr int64_t kMaxSegmentCtas = 8;
 
 // Whether clusters of c CTAs take the segments, the longest of `most` units, instead
 // of spans over the batch.  Clusters start and end sooner (no scan of the batch, no
-// merge launch), spans share ragged work out evenly.  Measured, clusters / spans in
-// us, d64, two kv heads, one sequence with a window of 64: 7.0 / 10.1, 4096: 14.8 /
-// 19.9; 64 sequences (c = 3), log-uniform lengths up to 4 windows of 1024 (6 units a
-// warp): 13.9 / 15.4, of 2048 (11): 19.2 / 16.7; 200 (c = 1), 256 (5): 11.6 / 14.7,
-// 1024 (17): 24.4 / 17.6; d128, 16 sequences (c = 4), 4096 (16): 18.1 / 24.4.
-bool clusters_win(int64_t c, int64_t most) { return most <= c * 4 * (c >= 4 ? 16 : 8); }
+// merge launch), spans share ragged work out evenly.  Measured, clusters / spans in us,
+// lengths log-uniform up to four windows; d64, 14 + 2 heads: one sequence, window 1024:
+// 4.1 / 7.5; 32 (c = 6), 4096 (11 units a warp): 16.0 / 22.0, 16384 (43): 38.8 / 26.0; 64
+// (c = 3), 1024 (6): 12.5 / 15.6, 2048 (11): 17.9 / 16.5; 200 (c = 1), 512 (8.5): 14.4 /
+// 15.6, 1024 (17): 23.0 / 17.5; d128, 28 + 4 heads, 32 (c = 2), 1024 (8.4): 16.6 / 19.4,
+// 2048 (16): 25.4 / 21.2.
+bool clusters_win(int64_t c, int64_t most) { return most <= c * 4 * (c >= 4 ? 16 : 9); }
 
 int plan_mma_decode(const WindowShape& s, MmaDecodePlan* p) {
   int sms = 0, dev = 0;

@@ -531,11 +531,17 @@ __device__ __forceinline__ Span compute_warp_spans_smem(const DecodeArgs& a, Sca
   return sp;
 }
 
+// Units a warp takes before a segment is shared by the CTAs of its cluster.  Windows of
+// 77 to 128 tokens (8 units on 4 warps), one sequence: 5.1 us in one CTA, 5.8 shared; of
+// 128 to 160 (12 units): 6.2 and 5.9; 64 sequences: 7.2 and 7.8, 8.7 and 7.6.
+constexpr int kAloneUnits = 2;
+
 // The span of a CTA of a segment's cluster (DecodeArgs::segment_ctas), in unit numbers
-// of its sequence alone.  All threads call it.
+// of its sequence alone, and the CTAs that share the segment: all, or the first.  nb is
+// 0 for a CTA without a part in it.  All threads call it.
 template <int NW>
 __device__ __forceinline__ Span segment_span(const DecodeArgs& a, WarpStarts& ws, int32_t& seq,
-                                             int32_t& h, int32_t& nb) {
+                                             int32_t& h, int32_t& nb, int32_t& ranks) {
   const int32_t seg = blockIdx.x / a.segment_ctas, rank = blockIdx.x % a.segment_ctas;
   seq = seg / a.num_kv_heads;
   h = seg % a.num_kv_heads;
@@ -554,9 +560,11 @@ __device__ __forceinline__ Span segment_span(const DecodeArgs& a, WarpStarts& ws
   Span sp{};
   const int64_t first = static_cast<int64_t>(h) * nb;
   sp.q = nb;
-  sp.r0 = first + static_cast<int64_t>(nb) * rank / a.segment_ctas;
-  sp.r1 = first + static_cast<int64_t>(nb) * (rank + 1) / a.segment_ctas;
+  ranks = nb <= kAloneUnits * NW ? 1 : a.segment_ctas;
+  sp.r0 = first + static_cast<int64_t>(nb) * rank / ranks;
+  sp.r1 = first + static_cast<int64_t>(nb) * (rank + 1) / ranks;
   sp.seq = seq;
+  if (rank >= ranks) nb = 0;
   return sp;
 }
 

@@ -26,17 +26,19 @@
 // is 16 tokens of the sequence's visible range (its sink units, then the window's),
 // masked by a 16-bit map, the block size any multiple of 16, and the scores are not
 // rounded to bf16 (the reference's rounding points belong to the full form only).
-// 256 sequences, 28 + 4 heads, d128, window 4096 (1.5 GB of keys and values): 243 us,
-// 94% of the measured copy rate; the CUDA-core kernel takes 3538.  64 sequences, d64,
-// window 1024 (10 MB): 14.8 us, where launch, table, first load and cluster exchange
-// follow one another.  Few segments are shared by clusters of CTAs that join through
-// distributed shared memory: one sequence of 77 tokens 7.0 us, by spans and their merge
-// 10.1.
+// 256 sequences, 28 + 4 heads, d128, window 4096 (1.5 GB of keys and values): 228 to
+// 244 us, 94 to 100% of the measured copy rate; the CUDA-core kernel takes 3538.  64
+// sequences, d64, window 1024 (10 MB): 12.7 us, where launch, table, loads, 6 units a
+// warp and the cluster's exchange follow one another.  Few segments are shared by
+// clusters of CTAs that join through distributed shared memory (join_segment): one
+// sequence of 77 tokens 5.1 us, by spans and their merge 10.1.  (A join whose reads
+// waited for one another, behind a chain of the warps' parts: 7.2 and 14.3.)
 #include "decode.cuh"
 
 namespace bsb {
 namespace {
 
+constexpr int kMaxRanks = 8;  // CTAs of a cluster
 constexpr int kBS = 16;  // tokens per block (fast path only)
 
 enum : int32_t { kFirst = 1, kLast = 2, kWhole = 4, kSlot1 = 8 };
@@ -76,6 +78,83 @@ struct Cfg {
   static_assert(STAGE_BYTES % 1024 == 0, "stages must stay 1024-byte aligned");
   static_assert(SLOT_FLOATS * 4 <= S * STAGE_BYTES, "slot 1 must fit in the stages");
 };
+
+// The end of a cluster's segment (DecodeArgs::segment_ctas): every warp with units has
+// left its part (O, maxima, sums) in its slot 0.  The CTA joins its warps' parts, all
+// threads at once, then the cluster's CTAs each join a share of the elements over all
+// CTAs' parts, in rank order.  Every read of a join is issued before the first is used:
+// one trip through distributed shared memory costs some 250 ns.
+template <typename C, int D>
+__device__ __forceinline__ void join_segment(const DecodeArgs& a, uint8_t* smem,
+                                             const int32_t (&slot_seq)[C::W][2], int32_t seq,
+                                             int32_t kvh, int32_t ranks) {
+  constexpr int W = C::W, kThreads = W * 32;
+  __shared__ float part_ml[2 * C::GROWS];
+  float* part = reinterpret_cast<float*>(smem);  // over the stages, whose copies are done
+  const int tid = threadIdx.x, G = a.groups;
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
+                       static_cast<int64_t>(seq) * a.o_stride_seq +
+                       static_cast<int64_t>(kvh) * G * D;
+  __syncthreads();
+  bool parked = ranks > 1;  // or one warp has written the output
+#pragma unroll
+  for (int w = 0; w < W; ++w) parked |= slot_seq[w][0] >= 0;
+  if (!parked) return;
+  for (int e = tid; e < G * D; e += kThreads) {
+    const int r = e / D;
+    float m[W], l[W], o[W], M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float* slot =
+          reinterpret_cast<const float*>(smem + W * C::S * C::STAGE_BYTES + w * C::SLOT0_BYTES);
+      const bool has = slot_seq[w][0] >= 0;
+      m[w] = has ? slot[G * D + r] : -INFINITY;
+      l[w] = has ? slot[G * D + G + r] : 0.f;
+      o[w] = has ? slot[e] : 0.f;
+      M = fmaxf(M, m[w]);
+    }
+    float L = 0.f, O = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = m[w] == -INFINITY ? 0.f : fast_exp2(m[w] - M);
+      L += f * l[w];
+      O += f * o[w];
+    }
+    if (ranks == 1) {
+      out[e] = __float2bfloat16_rn(O / L);
+    } else {
+      part[e] = O;
+      if (e % D == 0) {
+        part_ml[r] = M;
+        part_ml[C::GROWS + r] = L;
+      }
+    }
+  }
+  if (ranks == 1) return;
+  cluster_sync();
+  const int rank = blockIdx.x % a.segment_ctas;
+  for (int e = rank * kThreads + tid; e < G * D; e += ranks * kThreads) {
+    const int r = e / D;
+    float m[kMaxRanks], l[kMaxRanks], o[kMaxRanks], M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kMaxRanks; ++k) {
+      m[k] = k < ranks ? cluster_load(part_ml, r, k) : -INFINITY;
+      l[k] = k < ranks ? cluster_load(part_ml, C::GROWS + r, k) : 0.f;
+      o[k] = k < ranks ? cluster_load(part, e, k) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < kMaxRanks; ++k) M = fmaxf(M, m[k]);
+    float L = 0.f, O = 0.f;
+#pragma unroll
+    for (int k = 0; k < kMaxRanks; ++k) {
+      const float f = m[k] == -INFINITY ? 0.f : fast_exp2(m[k] - M);
+      L += f * l[k];
+      O += f * o[k];
+    }
+    out[e] = __float2bfloat16_rn(O / L);
+  }
+  cluster_sync();  // the others may still read this CTA's shared memory
+}
 
 template <int D, bool G16, bool WIN>
 __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
@@ -126,15 +205,15 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
   // The stages are free until the first copy: they hold the lengths and rows
   // for the span scan when they fit (one round of global loads).
   constexpr int kScratchInts = W * S * C::STAGE_BYTES / 4;
-  int32_t own_seq = 0, own_kvh = 0, own_units = 0;  // WIN: the cluster's segment
+  int32_t own_seq = 0, own_kvh = 0, own_units = 0, ranks = 1;  // WIN: the cluster's segment
   const bool clustered = WIN && a.segment_ctas > 0;
   const Span sp =
-      clustered ? segment_span<W>(a, starts, own_seq, own_kvh, own_units)
+      clustered ? segment_span<W>(a, starts, own_seq, own_kvh, own_units, ranks)
       : 2 * a.num_seqs <= kScratchInts
           ? compute_warp_spans_smem<W, WIN>(a, scan, starts, reinterpret_cast<int32_t*>(smem))
           : compute_warp_spans<W, WIN>(a, scan, starts);  // both sync the inits
   if (a.lens_ready && !early_loads) pdl_wait();  // query, pools from here on
-  if (clustered && own_units == 0) return;  // the whole cluster: nothing to read or write
+  if (clustered && own_units == 0) return;  // no part in a segment
   if (sp.r0 >= sp.r1 && !clustered) {
     if (a.tasks != nullptr && tid == 0) a.tasks[blockIdx.x].valid = 0;
     return;
@@ -242,7 +321,7 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
     const bool first = (cu == wr0) || (cb == 0);
     const bool last = (cu == wr1 - 1) || (cb == cnb - 1);
     const bool whole = seg_unit >= wr0 && seg_unit + cnb <= wr1 &&
-                       !(clustered && a.segment_ctas > 1);
+                       !(clustered && ranks > 1);
     if (lane == 0) {
       if (!valid && !dry) set_status(a.status, kStatusBadBlock);
       TileMeta& m = meta[warp][stage];
@@ -543,16 +622,12 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
     }
   }
 
-  // Clusters: the CTA's joined part (O, maxima, sums), read by the other CTAs; empty
-  // until its last warp fills it.  (Slot 0 of warp 0 is folded before that.)
-  __shared__ float part_ml[WIN ? 2 * C::GROWS : 1];
-  const bool joined = clustered && a.segment_ctas > 1;
-  if (joined && tid < C::GROWS) {
-    part_ml[tid] = -INFINITY;
-    part_ml[C::GROWS + tid] = 0.f;
+  if constexpr (WIN) {
+    if (clustered) {
+      join_segment<C, D>(a, smem, slot_seq, own_seq, own_kvh, ranks);
+      return;
+    }
   }
-  __shared__ int32_t part_slot;
-  if (WIN && tid == 0) part_slot = 0;
 
   // ---------------------------------------------------------------- CTA merge
   // A segment cut between warps is a chain: the last portion of the warp where
@@ -611,13 +686,7 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
     }
     const int64_t seg_unit = slot_unit[warp][k];
     const int32_t nb = slot_nb[warp][k];
-    if (joined) {
-      if (lane < G) {
-        part_ml[lane] = mine[G * D + lane];
-        part_ml[C::GROWS + lane] = mine[G * D + G + lane];
-      }
-      if (lane == 0) part_slot = static_cast<int32_t>(mine - reinterpret_cast<float*>(smem));
-    } else if (seg_unit >= sp.r0 && seg_unit + nb <= sp.r1) {
+    if (seg_unit >= sp.r0 && seg_unit + nb <= sp.r1) {
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
                            static_cast<int64_t>(seq) * a.o_stride_seq +
                            static_cast<int64_t>(kvh) * G * D;
@@ -653,36 +722,6 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
         fin_unit[idx] = seg_unit;
       }
     }
-  }
-  if (joined) {
-    // Each CTA of the cluster joins its share of the segment's elements from all
-    // parts, in rank order.  A part's place differs from CTA to CTA.
-    cluster_sync();
-    const uint32_t ranks = a.segment_ctas, rank = blockIdx.x % a.segment_ctas;
-    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
-                         static_cast<int64_t>(own_seq) * a.o_stride_seq +
-                         static_cast<int64_t>(own_kvh) * G * D;
-    for (int e = rank * (W * 32) + tid; e < G * D; e += ranks * (W * 32)) {
-      const int r = e / D;
-      float M = -INFINITY, m[8];
-#pragma unroll
-      for (uint32_t k = 0; k < 8; ++k) {
-        m[k] = k < ranks ? cluster_load(part_ml, r, k) : -INFINITY;
-        M = fmaxf(M, m[k]);
-      }
-      float L = 0.f, O = 0.f;
-#pragma unroll
-      for (uint32_t k = 0; k < 8; ++k) {
-        if (m[k] == -INFINITY) continue;  // an empty part
-        const float f = fast_exp2(m[k] - M);
-        const int at = __float_as_int(cluster_load(reinterpret_cast<float*>(&part_slot), 0, k));
-        L += f * cluster_load(part_ml, C::GROWS + r, k);
-        O += f * cluster_load(reinterpret_cast<float*>(smem), at + e, k);
-      }
-      out[e] = __float2bfloat16_rn(O / L);
-    }
-    cluster_sync();  // the others may still read this CTA's shared memory
-    return;
   }
   // Segments crossing CTAs for which this CTA came last: merge with all threads.
   // The stages and slots are free now and serve as scratch.
