@@ -108,9 +108,20 @@ int check_window_shape(const WindowShape& s) {
 constexpr int64_t kMaxSimtSplits = 64;
 constexpr int64_t kMinSimtKeys = 128;
 
+// Whether the ranges of a tile are a cluster whose CTAs join through distributed shared
+// memory, instead of leaving records for a second kernel: while all of them run at once
+// with some SMs to spare, for clusters to fit in.  Measured, clusters / records in us, fp32:
+// d64 (444 resident): 336 CTAs 14.6 / 20.9, 384: 15.6 / 20.5, 600 (a chunk): 106 / 86, 640:
+// 35.9 / 30.9; d128 (444): 448: 11.1 / 12.3, 576: 22.4 / 16.0; d256 (148): 112: 25.0 / 31.2,
+// 144: 41.6 / 33.4.
+bool simt_clusters_win(int64_t ctas, int64_t splits, int64_t resident) {
+  return splits > 1 && splits <= bsb::kMaxWindowCluster && ctas <= resident - resident / 8;
+}
+
 // How the CUDA-core kernel runs a call.
 struct SimtPlan {
   int64_t tile_tokens, qtiles, items, splits, rec_stride, bytes;
+  bool clustered;
 };
 
 int plan_simt(const WindowShape& s, SimtPlan* p) {
@@ -130,9 +141,13 @@ int plan_simt(const WindowShape& s, SimtPlan* p) {
   p->splits = std::max<int64_t>(
       1, std::min(std::min(want, kMaxSimtSplits), (keys + kMinSimtKeys - 1) / kMinSimtKeys));
   if (p->items * p->splits > kInt32Max) p->splits = 1;
+  const int64_t resident =
+      sms * bsb::window_simt_ctas_per_sm(s.dtype == BS_BF16, p->tile_tokens * groups > 8,
+                                         static_cast<int>(s.head_dim));
+  p->clustered = simt_clusters_win(p->items * p->splits, p->splits, resident);
   const int64_t gm = p->tile_tokens * groups <= 8 ? 8 : bsb::kWindowSimtRows;
   p->rec_stride = gm * s.head_dim + 2 * gm;
-  p->bytes = p->splits > 1 ? p->items * p->splits * p->rec_stride * 4 : 0;
+  p->bytes = p->splits > 1 && !p->clustered ? p->items * p->splits * p->rec_stride * 4 : 0;
   return BS_OK;
 }
 
@@ -422,6 +437,7 @@ int run_window(const WindowShape& s, const WindowCall& c) {
   a.tile_tokens = static_cast<int32_t>(p.tile_tokens);
   a.qtiles = static_cast<int32_t>(p.qtiles);
   a.splits = static_cast<int32_t>(p.splits);
+  a.clustered = p.clustered ? 1 : 0;
   a.records = static_cast<float*>(c.workspace);
   a.rec_stride = static_cast<int32_t>(p.rec_stride);
   const bool vec = (s.head_dim * dtype_size(s.dtype)) % 16 == 0 && aligned16(c.key_pool) &&
@@ -429,7 +445,7 @@ int run_window(const WindowShape& s, const WindowCall& c) {
   const int rc = bsb::launch_window_simt(a, s.dtype == BS_BF16, vec,
                                          static_cast<cudaStream_t>(c.stream));
   if (rc != 0) return cuda_fail(rc, "window attention launch");
-  bsb::add_kernel_launches(p.splits > 1 ? 2 : 1);
+  bsb::add_kernel_launches(p.splits > 1 && !p.clustered ? 2 : 1);
   return BS_OK;
 }
 

@@ -272,4 +272,21 @@ inline cudaError_t once_per_device(unsigned long long* done, SetFn&& set) {
   return e;
 }
 
+// Barrier of a cluster's CTAs (all their threads), ordering their shared memory.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Float `index` of shared array `p` in CTA `rank` of the cluster.
+__device__ __forceinline__ float cluster_load(const float* p, int index, uint32_t rank) {
+  uint32_t addr;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(addr)
+               : "r"(smem_u32(p + index)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 }  // namespace bsb

@@ -80,23 +80,6 @@ struct DecodeArgs {
   int32_t segment_ctas;
 };
 
-// Barrier of a cluster's CTAs (all their threads), ordering their shared memory.
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-// Float `index` of shared array `p` in CTA `rank` of the cluster.
-__device__ __forceinline__ float cluster_load(const float* p, int index, uint32_t rank) {
-  uint32_t addr;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-               : "=r"(addr)
-               : "r"(smem_u32(p + index)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-
 // Tokens per unit of the sliding-window variant (one tile of the tensor cores).
 constexpr int32_t kWindowUnit = 16;
 

@@ -39,6 +39,9 @@ struct WindowArgs {
   // than one, a CTA leaves a record (O unnormalised, then row maxima in base 2
   // and row sums) that a second kernel merges in range order.
   int32_t splits;
+  // CUDA cores: the ranges' CTAs are a cluster and join through distributed shared memory
+  // instead (no records, no second kernel).
+  int32_t clustered;
   float* records;
   int32_t rec_stride;
   // Tensor-core chunks: the (maximum, sum) pairs of every record row start this
@@ -105,6 +108,7 @@ __host__ __device__ __forceinline__ int32_t window_range(int32_t count, int32_t 
 
 // Query rows (tokens x heads of one kv head) of a tile of the CUDA-core kernel.
 constexpr int kWindowSimtRows = 16;
+constexpr int kMaxWindowCluster = 8;  // CTAs of a cluster
 
 // Tensor-core chunks: rows of a query tile, the fewest steps of 64 keys in a range
 // and the most ranges.
@@ -115,6 +119,8 @@ constexpr int kMaxWindowRanges = 8;
 
 int launch_window_prefill(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& kmap,
                           const CUtensorMap& vmap, cudaStream_t stream);
+// CTAs of the CUDA-core kernel that an SM holds; wide: more than 8 query rows a tile.
+int window_simt_ctas_per_sm(bool bf16, bool wide, int head_dim);
 int launch_window_simt(const WindowArgs& a, bool bf16, bool vec, cudaStream_t stream);
 
 }  // namespace bsb

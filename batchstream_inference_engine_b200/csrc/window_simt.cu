@@ -14,9 +14,11 @@
 // states are combined at the end.  Rows of more than 256 bytes copy V over K once the
 // scores are there: both would leave room for one CTA on an SM (fp32, d128, 200
 // sequences, window 2000: 140 us with both, 117 so; 47 sequences, window 900: 31 and
-// 33).  24 fp32 sequences of up to 4096 tokens, d64, window 777: 16.8 us, a chain of
-// table entry, rows, scores, V and merge with too few keys to hide it (one warp lane
-// loading its own key row instead: 68 us).  Rows that are not whole 16-byte pieces are read one element at a time.
+// 33).  24 fp32 sequences of up to 4096 tokens, d64, window 777: 12.1 us, a chain of
+// table entry, rows, scores, V and join with too few keys to hide it (one warp lane
+// loading its own key row instead: 68 us).  The ranges of a tile are a cluster that
+// joins through distributed shared memory while all CTAs run at once; more leave records
+// for a second kernel, which costs some 4 us.  Rows that are not whole 16-byte pieces are read one element at a time.
 //
 // A weight of zero skips its V row, so NaN or infinities in a key that a row does
 // not see never reach that row.
@@ -112,8 +114,10 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
   WindowTile w;
   if (!window_tile(a, r, tile, w, tid == 0 && tile == 0 && h == 0 && split == 0)) return;
   const int32_t per = window_range(w.count, a.splits);
-  if (static_cast<int64_t>(split) * per >= w.count) return;
-  const int32_t begin = split * per;
+  // (A cluster's CTA without keys stays: it joins, and the others read its empty part.)
+  if (!a.clustered && static_cast<int64_t>(split) * per >= w.count) return;
+  const int32_t begin =
+      static_cast<int32_t>(min(static_cast<int64_t>(split) * per, static_cast<int64_t>(w.count)));
   const int32_t end = w.count - begin < per ? w.count : begin + per;
 
   const int G = a.groups, D = FULL ? 32 * DPL : a.head_dim, bs = a.block_size;
@@ -311,7 +315,9 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
   __syncthreads();
   T* out = static_cast<T*>(a.out) + static_cast<int64_t>(w.tok0) * a.o_stride +
            static_cast<int64_t>(h) * G * D;
-  float* rec = a.splits > 1 ? a.records + static_cast<int64_t>(blockIdx.x) * a.rec_stride : nullptr;
+  // A cluster's CTA leaves its part where the query rows were, its maxima and sums where
+  // the weights were.
+  float* rec = a.clustered ? sQ : a.splits > 1 ? a.records + static_cast<int64_t>(blockIdx.x) * a.rec_stride : nullptr;
   for (int e = tid; e < rows * D; e += kThreads) {
     const int i = e / D;
     float M = -INFINITY;
@@ -328,14 +334,42 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
     if (rec != nullptr) {
       rec[e] = O;
       if (e - i * D == 0) {
-        rec[GM * D + i] = M;
-        rec[GM * D + GM + i] = L;
+        float* ml = a.clustered ? probs : rec + GM * D;
+        ml[i] = M;
+        ml[GM + i] = L;
       }
     } else {
       const int t = e / (G * D);
       out[static_cast<int64_t>(t) * a.o_stride + (e - t * G * D)] = of_float<T>(O / L);
     }
   }
+  if (!a.clustered) return;
+  // Every CTA joins a share of the elements, in range order; all reads of a join are
+  // issued before the first is used.
+  cluster_sync();
+  for (int e = split * kThreads + tid; e < rows * D; e += a.splits * kThreads) {
+    const int i = e / D;
+    float ms[kMaxWindowCluster], ls[kMaxWindowCluster], os[kMaxWindowCluster], M = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kMaxWindowCluster; ++x) {
+      ms[x] = x < a.splits ? cluster_load(probs, i, x) : -INFINITY;
+      ls[x] = x < a.splits ? cluster_load(probs, GM + i, x) : 0.f;
+      os[x] = x < a.splits ? cluster_load(sQ, e, x) : 0.f;
+    }
+#pragma unroll
+    for (int x = 0; x < kMaxWindowCluster; ++x) M = fmaxf(M, ms[x]);
+    const float mb = M == -INFINITY ? 0.f : M;
+    float L = 0.f, O = 0.f;
+#pragma unroll
+    for (int x = 0; x < kMaxWindowCluster; ++x) {
+      const float f = fast_exp2(ms[x] - mb);
+      L += ls[x] * f;
+      O += os[x] * f;
+    }
+    const int t = e / (G * D);
+    out[static_cast<int64_t>(t) * a.o_stride + (e - t * G * D)] = of_float<T>(O / L);
+  }
+  cluster_sync();  // the others may still read this CTA's shared memory
 }
 
 // Joins the records of a tile's key ranges, in range order.
@@ -385,7 +419,7 @@ int launch_one(const WindowArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return static_cast<int>(e);
   }
   const int64_t items = static_cast<int64_t>(a.num_rows) * a.qtiles * a.num_kv_heads;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
@@ -395,8 +429,14 @@ int launch_one(const WindowArgs& a, cudaStream_t stream) {
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (a.clustered) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.splits;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
   const int rc = static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, a));
-  if (rc != 0 || a.splits == 1) return rc;
+  if (rc != 0 || a.splits == 1 || a.clustered) return rc;
   cfg.gridDim = dim3(static_cast<unsigned>(items));
   cfg.dynamicSmemBytes = 0;
   return static_cast<int>(cudaLaunchKernelEx(&cfg, window_simt_merge_kernel<T, GM>, a));
@@ -425,7 +465,30 @@ int launch_rows(const WindowArgs& a, bool vec, cudaStream_t stream) {
              : launch_dims<T, kWindowSimtRows, false>(a, stream);
 }
 
+template <typename T, int GM, int DPL>
+int smem_bytes(int D) {
+  return D * sizeof(T) % 16 == 0 ? Layout<T, GM, DPL, true>::total(D)
+                                 : Layout<T, GM, DPL, false>::total(D);
+}
+
+template <typename T, int GM>
+int smem_bytes(int D) {
+  return D <= 32 ? smem_bytes<T, GM, 1>(D)
+         : D <= 64 ? smem_bytes<T, GM, 2>(D)
+         : D <= 128 ? smem_bytes<T, GM, 4>(D) : smem_bytes<T, GM, 8>(D);
+}
+
 }  // namespace
+
+int window_simt_ctas_per_sm(bool bf16, bool wide, int head_dim) {
+  constexpr int kSmem = 228 * 1024, kReserved = 1024, kByRegisters = 4;
+  const int bytes = bf16 ? (wide ? smem_bytes<__nv_bfloat16, kWindowSimtRows>(head_dim)
+                                 : smem_bytes<__nv_bfloat16, 8>(head_dim))
+                         : (wide ? smem_bytes<float, kWindowSimtRows>(head_dim)
+                                 : smem_bytes<float, 8>(head_dim));
+  const int by_smem = kSmem / (bytes + kReserved);
+  return by_smem < kByRegisters ? by_smem : kByRegisters;
+}
 
 int launch_window_simt(const WindowArgs& a, bool bf16, bool vec, cudaStream_t stream) {
   return bf16 ? launch_rows<__nv_bfloat16>(a, vec, stream) : launch_rows<float>(a, vec, stream);
