@@ -200,6 +200,21 @@ def test_decode_more_sequences_than_the_span_scan_stages():
     c.check(out)
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,head_dim", [
+    (torch.float32, 14, 2, 64), (torch.float32, 8, 2, 256), (torch.bfloat16, 16, 2, 80),
+    (torch.bfloat16, 14, 2, 64), (torch.bfloat16, 28, 4, 128)])
+@pytest.mark.parametrize("rows,window", [(3, 100), (8, 777), (24, 777), (64, 777), (64, 200)])
+def test_decode_by_clusters_and_by_records(dtype, heads, kv_heads, head_dim, rows, window):
+    # Batches on both sides of the rules that let a sequence's CTAs join in a cluster,
+    # of sequences on both sides of the sizes that one CTA takes alone, and empty ones.
+    lens = [(0, 1, 17, 64, 120, 128, 130, 145, 300, 900)[i % 10] + i // 10 for i in range(rows)]
+    c = Paged(lens, [1] * rows, heads, kv_heads, head_dim, 16, dtype, window, 4, seed=40)
+    out = c.decode()
+    assert ops.take_status() == 0
+    c.check(out)
+    assert torch.equal(out, c.decode())
+
+
 def test_decode_output_may_be_the_query():
     for dtype in (torch.bfloat16, torch.float32):
         c = Paged([5000, 70, 3], [1] * 3, 14, 2, 64, 16, dtype, 4000, 4, seed=13)
