@@ -57,8 +57,8 @@ struct DecodeArgs {
   // kernel launched just ahead of this one: the span search may then overlap it
   // (programmatic dependent launch); query and pools are read only after it.
   int32_t lens_ready;
-  // With lens_ready: the kernel just ahead wrote at most each sequence's last
-  // pool block, so other blocks and the query may be loaded before it ends.
+  // With lens_ready: the kernel just ahead wrote at most the query and each
+  // sequence's last pool block, so other blocks may be loaded before it ends.
   int32_t after_append;
   // [grid] merge tasks.  When set (tensor-core kernel), cut segments are merged
   // by decode_merge_kernel after the decode kernel instead of by the last CTA

@@ -261,7 +261,16 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
     const int32_t* table = a.block_tables + static_cast<int64_t>(row) * a.bt_stride;
     return (e0 + lane < a.max_blocks) ? __ldg(table + e0 + lane) : 0;
   };
-  auto issue = [&](int stage, bool dry) {
+  // Starts the copy of a segment's query rows into a stage (lane 0).
+  auto load_query = [&](int stage, int32_t seq, int32_t head) {
+    const __nv_bfloat16* qsrc = static_cast<const __nv_bfloat16*>(a.q) +
+                                static_cast<int64_t>(seq) * a.q_stride_seq +
+                                static_cast<int64_t>(head) * G * D;
+    bulk_load(wst + stage * C::STAGE_BYTES + 2 * C::BLOCK_BYTES, qsrc, G * D * 2u,
+              &full_bar[warp][stage]);
+  };
+  // `early`: ahead of pdl_wait(), with the query's bytes expected and not yet asked for.
+  auto issue = [&](int stage, bool dry, bool early) {
     // The window caches up to 32 entries of one table row, filled to the row's
     // width rather than this sequence's block count: sequences that share a row
     // (the tokens of a prefill chunk) have different lengths and reuse it.
@@ -359,12 +368,7 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
                            hf * 64, y, policy);
         }
       }
-      if (first) {
-        const __nv_bfloat16* qsrc = static_cast<const __nv_bfloat16*>(a.q) +
-                                    static_cast<int64_t>(ci) * a.q_stride_seq +
-                                    static_cast<int64_t>(ch) * G * D;
-        bulk_load(st + 2 * C::BLOCK_BYTES, qsrc, G * D * 2u, &full_bar[warp][stage]);
-      }
+      if (first && !early) load_query(stage, ci, ch);
     }
     if (!dry && !probe) armed |= 1u << stage;
     // Advance to the next unit.
@@ -392,11 +396,15 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
   int issued = 0;
   if (early_loads) {
     // Stages up to (not including) the first block that ends a segment: the
-    // append ahead may still be writing that one.
-    for (; issued < S && issued < ntiles && cb != cnb - 1; ++issued) issue(issued, false);
+    // append ahead may still be writing that one, and the query too (a rotary
+    // append writes both).  The loop stays within one segment, so the only query
+    // it leaves out is that of stage 0.
+    const int32_t q_seq = ci, q_head = ch;
+    for (; issued < S && issued < ntiles && cb != cnb - 1; ++issued) issue(issued, false, true);
     pdl_wait();
+    if (issued > 0 && lane == 0 && !probe) load_query(0, q_seq, q_head);
   }
-  for (; issued < S && issued < ntiles; ++issued) issue(issued, false);
+  for (; issued < S && issued < ntiles; ++issued) issue(issued, false, false);
 
   // ---------------------------------------------------------------- compute
   const int g = lane >> 2, t = lane & 3;
@@ -564,7 +572,7 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
     __syncwarp();
     if (it + S < ntiles) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      issue(stage, dry);
+      issue(stage, dry, false);
     }
 
     if (mt.flags & kLast) {

@@ -198,6 +198,30 @@ def test_fork_refuses_while_a_step_is_in_flight(exact_gemm):
     backend.fork_sequence(s, [4])
 
 
+@pytest.mark.parametrize("graphs", [False, True])
+def test_scaled_rotary_before_full_attention(exact_gemm, graphs, monkeypatch):
+    # Without a window the full decode follows the rotary append directly and starts
+    # ahead of its end: the same tokens as without that overlap.
+    config = dataclasses.replace(CONFIG, attention_window=0, attention_sinks=0)
+    weights = weights_of()
+    rng = np.random.default_rng(8)
+    specs = [(rng.integers(0, VOCAB, int(n)).tolist(), 24) for n in (300, 5, 90, 1, 200, 33, 64, 17)]
+    served = []
+    for overlap in (True, False):
+        if not overlap:
+            plain = ops.paged_attention_batched
+            monkeypatch.setattr(ops, "paged_attention_batched",
+                                lambda *a, **kw: plain(*a, **{**kw, "after_append": False}))
+        model = TorchModel(config, weights, device=DEV, dtype=torch.bfloat16, max_position=1024,
+                           step_graphs=graphs, max_graph_batch=16, max_graph_prefill=128)
+        backend = PagedBackend(model, num_blocks=128, block_size=16, prefill_chunk=96,
+                               vocab=NoEnd(), max_seqs=16)
+        requests = serve(backend, specs, 8, BlockBudget(128, 16))
+        assert not any(r.failed for r in requests)
+        served.append([r.tokens for r in requests])
+    assert served[0] == served[1]
+
+
 def test_default_rotary_over_frequencies_and_a_full_window(exact_gemm):
     # A window that covers the sequence and the plain frequencies in half layout:
     # linear scaling by 1 takes the new operators through the reference's model.

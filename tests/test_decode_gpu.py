@@ -326,6 +326,46 @@ def test_early_loads_after_an_append_give_the_same_bits():
         ops.paged_attention_batched(q, k2, v2, bt, lens_d, 0.125, after_append=True)
 
 
+def test_query_written_by_the_append_ahead_is_read_after_it():
+    # The rotary appends write the query and the new token's slot; the decode behind
+    # them may load other blocks early, never the query.  A different query in the same
+    # buffer each time, enough of them that the append is still running.
+    lens, tables, bt, _, k, v = ragged_batch(256, 14, 2, 64, torch.bfloat16, median=300, seed=14)
+    B = len(lens)
+    g = torch.Generator(device=DEV).manual_seed(6)
+    pos = torch.tensor([n - 1 for n in lens], dtype=torch.int32, device=DEV)
+    slots = torch.tensor([tables[i][(n - 1) // 16] * 16 + (n - 1) % 16
+                          for i, n in enumerate(lens)], dtype=torch.int32, device=DEV)
+    lens_d = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    angles = torch.rand((max(lens), 64), generator=g, device=DEV)
+    cos, sin = angles.cos().bfloat16(), angles.sin().bfloat16()
+    freq = ops.rope_frequencies(64, 1e4, {"type": "linear", "factor": 4.0}, device=DEV)[0]
+    rows = [torch.randn((B, 18 * 64), generator=g, device=DEV).bfloat16() for _ in range(6)]
+    q = torch.empty((B, 14, 64), dtype=torch.bfloat16, device=DEV)
+
+    def by_tables(qkv):
+        ops.rope_append(qkv, cos, sin, pos, slots, k, v, 14, query_out=q)
+
+    def by_frequencies(qkv):
+        ops.rotary_append(qkv, freq, pos, slots, k, v, 14, query_out=q)
+
+    for append in (by_tables, by_frequencies):
+        plain, early = [], []
+        for qkv in rows:
+            append(qkv)
+            torch.cuda.synchronize()
+            plain.append(ops.paged_attention_batched(q, k, v, bt, lens_d, 0.125))
+        torch.cuda.synchronize()
+        out = torch.empty((len(rows), B, 14, 64), dtype=torch.bfloat16, device=DEV)
+        for i, qkv in enumerate(rows):
+            append(qkv)
+            early.append(ops.paged_attention_batched(q, k, v, bt, lens_d, 0.125, out=out[i],
+                                                     lens_ready=True, after_append=True))
+        for a, b in zip(plain, early):
+            assert torch.equal(a, b)
+    assert ops.take_status() == 0
+
+
 def test_zero_length_rows_are_padding():
     lens, tables, bt, q, k, v = ragged_batch(8, 14, 2, 64, torch.bfloat16, median=150, seed=11)
     padded = torch.tensor(lens, dtype=torch.int32, device=DEV)
