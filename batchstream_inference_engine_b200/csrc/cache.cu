@@ -55,8 +55,8 @@ __global__ void __launch_bounds__(kMetaThreads)
   __shared__ int32_t cu[kMaxMetaRows + 1];
   __shared__ int32_t warp_tot[kMetaThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
 
   // Block-wide exclusive scan of n_new in chunks of kMetaThreads.
   int32_t carry = 0;
@@ -134,8 +134,8 @@ __global__ void __launch_bounds__(256)
                           int64_t v_stride, const int32_t* __restrict__ slots, int32_t T,
                           int32_t Hkv, int32_t D, Tpool* __restrict__ k_pool,
                           Tpool* __restrict__ v_pool, int64_t pool_slots, uint32_t* status) {
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   const int32_t vecs = D >> 3;
   const int64_t per_tensor = static_cast<int64_t>(T) * Hkv * vecs;
   const int64_t total = 2 * per_tensor;
@@ -185,8 +185,8 @@ __global__ void __launch_bounds__(256)
                              int64_t v_stride, const int32_t* __restrict__ slots, int32_t T,
                              int32_t Hkv, int32_t D, Tpool* __restrict__ k_pool,
                              Tpool* __restrict__ v_pool, int64_t pool_slots, uint32_t* status) {
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   const int64_t per_tensor = static_cast<int64_t>(T) * Hkv * D;
   for (int64_t idx = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
        idx < 2 * per_tensor; idx += static_cast<int64_t>(gridDim.x) * blockDim.x) {
@@ -226,8 +226,8 @@ __global__ void __launch_bounds__(64)
                          Tpool* __restrict__ k_pool, Tpool* __restrict__ v_pool,
                          int64_t pool_slots, int32_t* __restrict__ context_lens,
                          int32_t* __restrict__ slots, uint32_t* status) {
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   const int32_t r = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (r >= R) return;
@@ -377,8 +377,8 @@ __global__ void __launch_bounds__(256)
     expand_rows_kernel(const int32_t* __restrict__ cu_q, const int32_t* __restrict__ context_lens,
                        const int32_t* __restrict__ seq_rows, int32_t R, int32_t T,
                        int32_t* __restrict__ token_lens, int32_t* __restrict__ token_rows) {
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   const int32_t t = blockIdx.x * blockDim.x + threadIdx.x;
   if (t >= T) return;
   // Last row r with cu_q[r] <= t.

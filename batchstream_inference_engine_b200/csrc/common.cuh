@@ -245,7 +245,10 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
 // stream-serialization attribute may start while the previous kernel on its
 // stream is still running; pdl_wait() blocks until that kernel has finished and
 // its writes are visible (a no-op without the attribute).  pdl_trigger() lets
-// the next such kernel start early.
+// the next such kernel start early; a kernel calls it after its own pdl_wait(),
+// so that one which starts early, and reads what the kernel just ahead does not
+// write before it waits (the decode behind an append), finds all earlier kernels
+// finished.  Ahead of the wait only where the next kernel waits before it reads.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -197,11 +197,11 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
     fin_count = 0;
     task.valid = 0;
   }
-  pdl_trigger();  // the merge pass may launch now; it waits for this grid
   // lens_ready: the work split overlaps the kernel just ahead; after_append:
   // so do the first loads of blocks that kernel cannot have written.
   const bool early_loads = a.lens_ready && a.after_append;
   if (!a.lens_ready) pdl_wait();
+  pdl_trigger();  // ahead of the wait (lens_ready) only for the merge pass, which waits
   // The stages are free until the first copy: they hold the lengths and rows
   // for the span scan when they fit (one round of global loads).
   constexpr int kScratchInts = W * S * C::STAGE_BYTES / 4;

@@ -72,8 +72,8 @@ __global__ void __launch_bounds__(32 * kNormRowsPerCta)
                     const int32_t* __restrict__ index, int32_t x_rows, const T* __restrict__ w,
                     int32_t rows, int32_t hidden, float eps, T* __restrict__ out,
                     int64_t out_stride, T* sum_out, int64_t sum_stride, uint32_t* status) {
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   const int lane = threadIdx.x & 31;
   const int32_t r = blockIdx.x * kNormRowsPerCta + (threadIdx.x >> 5);
   if (r >= rows) return;
@@ -208,8 +208,8 @@ __global__ void __launch_bounds__(128)
                        const int32_t* __restrict__ slots, int32_t ntok, int32_t H, int32_t Hkv,
                        int32_t D, T* __restrict__ q_out, Tpool* __restrict__ k_pool,
                        Tpool* __restrict__ v_pool, int64_t pool_slots, uint32_t* status) {
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   const int32_t half = D >> 1;
   const int32_t r = blockIdx.x * blockDim.x + threadIdx.x;
   if (r >= (H + 2 * Hkv) * half) return;
@@ -267,8 +267,8 @@ __global__ void __launch_bounds__(128)
                            __nv_bfloat16* __restrict__ q_out, __nv_bfloat16* __restrict__ k_pool,
                            __nv_bfloat16* __restrict__ v_pool, int64_t pool_slots,
                            uint32_t* status) {
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   const int32_t half = D >> 1, chunks = half >> 3;
   const int32_t per_tok = (H + 2 * Hkv) * chunks;
   const int64_t idx = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -331,8 +331,8 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(128)
     silu_mul_kernel(const T* __restrict__ gate_up, int64_t stride, int32_t ntok, int32_t inter,
                     T* __restrict__ out) {
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   const int32_t c = (blockIdx.x * blockDim.x + threadIdx.x) * (VEC ? 8 : 1);
   if (c >= inter) return;
   for (int32_t t = blockIdx.y; t < ntok; t += gridDim.y) {
@@ -372,8 +372,8 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kArgmaxThreads)
     argmax_rows_kernel(const T* __restrict__ x, int64_t stride, int64_t cols,
                        int32_t* __restrict__ out) {
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   const T* row = x + static_cast<int64_t>(blockIdx.x) * stride;
   float best = -INFINITY;
   int64_t bi = cols;  // past every index: loses all ties

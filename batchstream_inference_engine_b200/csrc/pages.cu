@@ -64,8 +64,8 @@ constexpr int kRound = 4;  // segments a warp copies at a time
 
 template <typename V>
 __global__ void __launch_bounds__(kThreads) copy_blocks_kernel(const CopyArgs a) {
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   const int32_t i = static_cast<int32_t>(blockIdx.x / a.slices);
   const int32_t slice = static_cast<int32_t>(blockIdx.x % a.slices);
   const int32_t s = a.src[i], d = a.dst[i];

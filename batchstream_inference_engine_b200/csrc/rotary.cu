@@ -116,8 +116,8 @@ __device__ __forceinline__ void turn_pair(float& x, float& y, float2 cs) {
 template <typename T, typename Tpool, bool INTER>
 __global__ void __launch_bounds__(kThreads) rotary_append_vec_kernel(const RotaryArgs a) {
   extern __shared__ float2 turn[];
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   const int32_t t = blockIdx.x;
   const Token tok = begin_token<T>(a, t, turn);
   const T* row = static_cast<const T*>(a.qkv) + t * a.qkv_stride;
@@ -176,8 +176,8 @@ __global__ void __launch_bounds__(kThreads) rotary_append_vec_kernel(const Rotar
 template <typename T, typename Tpool, bool INTER>
 __global__ void __launch_bounds__(kThreads) rotary_append_kernel(const RotaryArgs a) {
   extern __shared__ float2 turn[];
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   const int32_t t = blockIdx.x;
   const int32_t half = a.rotary_dim >> 1;
   const Token tok = begin_token<T>(a, t, turn);

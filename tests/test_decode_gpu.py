@@ -366,6 +366,38 @@ def test_query_written_by_the_append_ahead_is_read_after_it():
     assert ops.take_status() == 0
 
 
+def test_early_loads_see_what_earlier_kernels_wrote():
+    # Block copies two kernels ahead of the decode: only the append lies between, and
+    # the decode's early loads read copied blocks.
+    lens, tables, bt, q, k, v = ragged_batch(64, 14, 2, 64, torch.bfloat16, median=300, seed=15)
+    B, nb = len(lens), k.size(1)
+    g = torch.Generator(device=DEV).manual_seed(7)
+    pools = [torch.randn((2, nb, 16, 64), generator=g, device=DEV).bfloat16() for _ in range(4)]
+    used = sorted({b for i, n in enumerate(lens) for b in tables[i][: -(-n // 16)]})
+    # A second half of the pool holds the blocks; copies bring them to their places.
+    big_k = torch.cat([torch.zeros_like(k), k], 1).contiguous()
+    big_v = torch.cat([torch.zeros_like(v), v], 1).contiguous()
+    dst = torch.tensor(used, dtype=torch.int32, device=DEV)
+    src = dst + nb
+    pos = torch.tensor([n - 1 for n in lens], dtype=torch.int32, device=DEV)
+    slots = torch.tensor([tables[i][(n - 1) // 16] * 16 + (n - 1) % 16
+                          for i, n in enumerate(lens)], dtype=torch.int32, device=DEV)
+    lens_d = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    freq = ops.rope_frequencies(64, 1e4, device=DEV)[0]
+    qkv = torch.randn((B, 18 * 64), generator=g, device=DEV).bfloat16()
+    for new_k, new_v in zip(pools[::2], pools[1::2]):
+        big_k[:, nb:], big_v[:, nb:] = new_k, new_v
+        torch.cuda.synchronize()
+        ops.copy_blocks(big_k, big_v, src, dst)
+        q = ops.rotary_append(qkv, freq, pos, slots, big_k, big_v, 14)
+        early = ops.paged_attention_batched(q, big_k, big_v, bt, lens_d, 0.125, lens_ready=True,
+                                            after_append=True)
+        torch.cuda.synchronize()
+        plain = ops.paged_attention_batched(q, big_k, big_v, bt, lens_d, 0.125)
+        assert torch.equal(early, plain)
+    assert ops.take_status() == 0
+
+
 def test_zero_length_rows_are_padding():
     lens, tables, bt, q, k, v = ragged_batch(8, 14, 2, 64, torch.bfloat16, median=150, seed=11)
     padded = torch.tensor(lens, dtype=torch.int32, device=DEV)
