@@ -805,6 +805,31 @@ int occupancy_one() {
 
 namespace {
 
+// The merge pass of either form: at most `grid` records per segment.
+int launch_merge(const DecodeArgs& a, int grid, cudaStream_t stream) {
+  const int smem = static_cast<int>((2 * static_cast<int64_t>(grid) * a.groups + 2 * a.groups) *
+                                    sizeof(float));
+  // Room for 16 heads a group and 700 CTAs; the grids hold at most three an SM.
+  constexpr int kMaxSmem = 90 * 1024;
+  static unsigned long long configured = 0;  // one bit per device
+  cudaError_t e = once_per_device(&configured, [] {
+    return cudaFuncSetAttribute(decode_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kMaxSmem);
+  });
+  if (e != cudaSuccess) return static_cast<int>(e);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_merge_kernel, a));
+}
+
 template <bool WIN>
 int launch_both(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap& vmap, int grid,
                 cudaStream_t stream) {
@@ -817,32 +842,7 @@ int launch_both(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap&
     rc = g16 ? launch_one<128, true, WIN>(a, kmap, vmap, grid, stream)
              : launch_one<128, false, WIN>(a, kmap, vmap, grid, stream);
   if (rc != 0 || a.tasks == nullptr) return rc;
-  // Merge pass: at most `grid` records per segment.
-  const int smem = static_cast<int>((2 * static_cast<int64_t>(grid) * a.groups + 2 * a.groups) *
-                                    sizeof(float));
-  // The attribute is per device: set it on the current one whenever the
-  // size grows past what that device was given.
-  static int configured_smem[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  if (dev >= 64 || smem > configured_smem[dev]) {
-    e = cudaFuncSetAttribute(decode_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             smem);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    if (dev < 64) configured_smem[dev] = smem;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_merge_kernel, a));
+  return launch_merge(a, grid, stream);
 }
 
 template <bool WIN>

@@ -17,6 +17,9 @@ terms cancelled), n visible keys and u = 2^-24:
 """
 
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -685,3 +688,41 @@ def test_wrappers_refuse():
     with pytest.raises(RuntimeError):
         ops.window_prefill_attention(q, c.k, c.v, c.table, c.cu, c.len_d, 0.125, 0, 40)
     assert ops.take_status() == 0
+
+
+MERGES = """
+import torch
+from batchstream_inference_engine_b200 import ops
+g = torch.Generator(device="cuda").manual_seed(0)
+pool = lambda nb: torch.randn((2, nb, 16, 64), generator=g, device="cuda").bfloat16()
+def call(rows, tokens, window, **kw):
+    k, v = pool(rows * tokens // 16), pool(rows * tokens // 16)
+    q = torch.randn((rows, 32, 64), generator=g, device="cuda").bfloat16()
+    bt = torch.arange(k.size(1), dtype=torch.int32, device="cuda").view(rows, -1)
+    lens = torch.full((rows,), tokens, dtype=torch.int32, device="cuda")
+    if window:
+        return lambda: ops.window_attention_batched(q, k, v, bt, lens, 0.125, window)
+    return lambda: ops.paged_attention_batched(q, k, v, bt, lens, 0.125, **kw)
+ORDERS = {
+    # The merge pass takes 56 KB of shared memory behind the large calls, 33 KB or less
+    # behind the small ones.
+    "full first": (call(40, 4096, 0), call(1, 16384, 8192)),
+    "window first": (call(40, 16384, 8192), call(1, 4096, 0, units_hint=512)),
+}
+large, small = ORDERS["%s"]
+first = large()
+small()
+again = large()
+assert torch.equal(first, again) and bool(first.isfinite().all())
+assert ops.take_status() == 0
+"""
+
+
+@pytest.mark.parametrize("order", ["full first", "window first"])
+def test_merge_passes_of_both_forms_in_one_process(order):
+    # A process of its own: what the first large call sets up must outlast a small call
+    # of the other form.
+    root = Path(__file__).resolve().parent.parent
+    done = subprocess.run([sys.executable, "-c", MERGES % order], cwd=root, capture_output=True,
+                          text=True, timeout=120)
+    assert done.returncode == 0, done.stderr[-2000:]
