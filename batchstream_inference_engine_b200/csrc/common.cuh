@@ -275,8 +275,10 @@ inline cudaError_t once_per_device(unsigned long long* done, SetFn&& set) {
   return e;
 }
 
-// Barrier of a cluster's CTAs (all their threads), ordering their shared memory.
+// Barrier of a cluster's CTAs (all their threads), ordering their shared memory.  It is
+// .aligned: the lanes of a warp, which may come from loops of different lengths, meet first.
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

@@ -260,6 +260,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     fence_barrier_init();
   }
   if (warp == 0) {
+    __syncwarp();  // thread 0 comes from the barriers' setup
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(&tmem_base)),
                  "r"(kTmemCols));
@@ -573,6 +574,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             *reinterpret_cast<uint4*>(dst + c0 + c) = w;
           }
         }
+        __syncwarp();  // rows past the chunk part from the others above
       }
     } else if (tid == 0) {
       set_status(a.status, kStatusWaitTimeout);
@@ -582,6 +584,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   if (warp == 0) {
     tc_fence_after();
+    __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(kTmemCols));
   }

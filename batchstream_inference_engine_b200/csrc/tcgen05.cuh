@@ -49,7 +49,10 @@ __device__ __forceinline__ void tc_fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
 
-// 32 consecutive TMEM columns of this thread's lane.
+// 32 consecutive TMEM columns of this thread's lane.  These instructions are .aligned:
+// all lanes execute them together.  Where the code before one may have diverged (rows
+// without a token, keys that only some rows see), nothing but a warp barrier or another
+// warp-wide .sync instruction promises that its lanes have met again.
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"

@@ -235,6 +235,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     bad_count = 0;
   }
   if (warp == 0) {
+    __syncwarp();  // thread 0 comes from the barriers' setup
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(&tmem_base)),
                  "r"(kTmemCols));
@@ -480,6 +481,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (ux >= sd.units || !live) map = 0;
           maps[un / 2] = un % 2 ? maps[un / 2] | (map << 16) : map;
         }
+        __syncwarp();  // ahead of .aligned loads
       }
       uint32_t v[2][32];
       tmem_ld32(s_addr, v[0]);
@@ -593,8 +595,9 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           }
         }
-        if (!live) continue;
-        if (split_up) {
+        if (!live) {
+          // Holds no token: nothing to store.
+        } else if (split_up) {
           float* dst = a.records + rec_row * D + c0;
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
@@ -614,6 +617,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             *reinterpret_cast<uint4*>(dst + c) = o;
           }
         }
+        __syncwarp();  // rows without a token, and those that see a listed key, part above
       }
       if (split_up && live) {
         float* ml = a.records + a.rec_stride_ml + rec_row * 2;
@@ -625,6 +629,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   if (warp == 0) {
     tc_fence_after();
+    __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(kTmemCols));
   }
