@@ -65,6 +65,7 @@ constexpr int kRing = 8;  // step barriers (>= K stages, >= V stages)
 constexpr uint32_t kTmemCols = 256;  // two S/P buffers, O
 constexpr float kLog2eP = 1.4426950408889634f;
 constexpr float kRescaleSlack = 8.f;
+constexpr float kFarMaximum = 1073741824.f;  // 2^30
 constexpr int kMaxBad = 64;  // listed keys with non-finite V (more: all are looked at)
 
 template <int D>
@@ -455,7 +456,17 @@ __global__ void __launch_bounds__(kThreads, 2)
     const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t o_addr = tmem + lane_base + C::O_COL;
     const float zscale = fabsf(a.scale) * kLog2eP;
-    float m_used = -INFINITY, l_run = 0.f;
+    // Exponents are scale * score - scale * raw_used, the largest score used so far.  That
+    // product is rounded and the fused step takes it from the exact one, which shifts all
+    // of a row's exponents alike, by up to 2^-24 of the product: harmless until 2^shift
+    // overflows.  From 2^30 on rows scale by the power of two below, which is exact:
+    // scores that differ at all are then 2^5 or more apart, so only the keys at the
+    // maximum count, as they do with the scale itself.
+    float raw_used = -INFINITY, zs = zscale, l_run = 0.f;
+    auto scale_of = [&](float top) {
+      return fabsf(top * zscale) < kFarMaximum || top == -INFINITY  // (-inf: no key yet)
+                 ? zscale : __uint_as_float(__float_as_uint(zscale) & 0x7f800000u);
+    };
     int32_t plain_lo, plain_hi;
     plain_steps(a, sd, plain_lo, plain_hi);
     bool ok = true;
@@ -504,18 +515,18 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int i = 0; i < 32; ++i) {  // three-input maxima
         mx[i & 3] = fmaxf(fmaxf(mx[i & 3], __uint_as_float(v[0][i])), __uint_as_float(v[1][i]));
       }
-      const float m_step = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * zscale;
-      const bool grow = live && m_step > m_used + kRescaleSlack;
+      const float raw = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      const bool grow = live && __fmul_rn(raw, zscale) > __fmul_rn(raw_used, zscale) + kRescaleSlack;
       if (u == 0) {
-        m_used = m_step;
+        raw_used = raw;
+        zs = scale_of(raw);
       } else if (__any_sync(0xffffffffu, grow)) {
         // O may be rescaled once P V of the step before is done; rows that did not
         // grow keep theirs (factor 1).
         ok = wait_step(u + 1);
         if (!ok) break;
         tc_fence_after();
-        const float m_new = grow ? m_step : m_used;
-        const float corr = grow ? fast_exp2(m_used - m_new) : 1.f;
+        const float corr = grow ? fast_exp2(__fmul_rn(raw_used, zscale) - __fmul_rn(raw, zscale)) : 1.f;
 #pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += 32) {
           uint32_t o[32];
@@ -527,10 +538,11 @@ __global__ void __launch_bounds__(kThreads, 2)
           tmem_st32(o_addr + c0, o);
         }
         l_run *= corr;
-        m_used = m_new;
+        raw_used = grow ? raw : raw_used;
+        zs = scale_of(raw_used);
       }
-      const float m_base = m_used == -INFINITY ? 0.f : m_used;  // no -inf - -inf
-      const float2 zs2 = make_float2(zscale, zscale), mm = make_float2(-m_base, -m_base);
+      const float m_base = raw_used == -INFINITY ? 0.f : raw_used * zs;  // no -inf - -inf
+      const float2 zs2 = make_float2(zs, zs), mm = make_float2(-m_base, -m_base);
       float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                        make_float2(0.f, 0.f)};
       uint32_t p[32];
@@ -621,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       if (split_up && live) {
         float* ml = a.records + a.rec_stride_ml + rec_row * 2;
-        *reinterpret_cast<float2*>(ml) = make_float2(m_used, l_run);
+        *reinterpret_cast<float2*>(ml) = make_float2(raw_used * zscale, l_run);
       }
     }
   }

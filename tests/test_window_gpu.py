@@ -726,3 +726,32 @@ def test_merge_passes_of_both_forms_in_one_process(order):
     done = subprocess.run([sys.executable, "-c", MERGES % order], cwd=root, capture_output=True,
                           text=True, timeout=120)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("length,new,heads,kv_heads,window,dtype", [
+    (300, 100, 14, 2, 120, torch.bfloat16), (478, 128, 2, 2, 351, torch.bfloat16),
+    (300, 1, 14, 2, 120, torch.bfloat16), (300, 20, 14, 2, 120, torch.float32)])
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("far", [-1e30, 1e30, -1e8, 3e37])
+def test_scores_far_from_zero(length, new, heads, kv_heads, window, dtype, head_dim, far):
+    # One dim of every key makes all scores of a row the same huge number (the query's
+    # other dims are 0): the output is the mean of the visible values.
+    c = Paged([length], [new], heads, kv_heads, head_dim, 16, dtype, window, 0, seed=8)
+    c.q[..., 0] = 1.0
+    c.q[..., 1:] = 0.0
+    keys = c.k.view(kv_heads, -1, head_dim)
+    keys[..., 0] = far
+    out = (c.decode if new == 1 else c.chunks)().double().cpu()
+    assert ops.take_status() == 0
+    G = heads // kv_heads
+    for t, p in enumerate(range(length - new, length)):
+        v = c.values[0][:, max(0, p - window + 1): p + 1].double()
+        mean, big = v.mean(1), v.abs().mean(1)
+        # The weights are alike, but not 1: the maximum they are taken from is a rounded
+        # product, up to 2^-24 of it off.  In bf16 each rounds by up to 2^-8 of itself.
+        tol = 2 * (v.size(1) + 64) * 2.0 ** -24 * big
+        if dtype == torch.bfloat16:
+            tol = tol + 2.0 ** -8 * big
+        tol = tol + torch.finfo(dtype).eps / 2 * (mean.abs() + tol)
+        err = (out[t] - mean.repeat_interleave(G, 0)).abs()
+        assert bool((err <= tol.repeat_interleave(G, 0)).all()), (t, float(err.max()))
