@@ -83,7 +83,9 @@ struct Cfg {
 // left its part (O, maxima, sums) in its slot 0.  The CTA joins its warps' parts, all
 // threads at once, then the cluster's CTAs each join a share of the elements over all
 // CTAs' parts, in rank order.  Every read of a join is issued before the first is used:
-// one trip through distributed shared memory costs some 250 ns.
+// one trip through distributed shared memory costs some 250 ns.  A part without a finite
+// score has the maximum -inf and weighs 0, but is not left out: if its scores are NaN,
+// so are its O and sums, and 0 * NaN brings that to the output.
 template <typename C, int D>
 __device__ __forceinline__ void join_segment(const DecodeArgs& a, uint8_t* smem,
                                              const int32_t (&slot_seq)[C::W][2], int32_t seq,
@@ -113,10 +115,11 @@ __device__ __forceinline__ void join_segment(const DecodeArgs& a, uint8_t* smem,
       o[w] = has ? slot[e] : 0.f;
       M = fmaxf(M, m[w]);
     }
+    const float base = M == -INFINITY ? 0.f : M;
     float L = 0.f, O = 0.f;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float f = m[w] == -INFINITY ? 0.f : fast_exp2(m[w] - M);
+      const float f = fast_exp2(m[w] - base);
       L += f * l[w];
       O += f * o[w];
     }
@@ -144,10 +147,11 @@ __device__ __forceinline__ void join_segment(const DecodeArgs& a, uint8_t* smem,
     }
 #pragma unroll
     for (int k = 0; k < kMaxRanks; ++k) M = fmaxf(M, m[k]);
+    const float base = M == -INFINITY ? 0.f : M;
     float L = 0.f, O = 0.f;
 #pragma unroll
     for (int k = 0; k < kMaxRanks; ++k) {
-      const float f = m[k] == -INFINITY ? 0.f : fast_exp2(m[k] - M);
+      const float f = fast_exp2(m[k] - base);
       L += f * l[k];
       O += f * o[k];
     }
@@ -674,8 +678,9 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
       if (lane < G) {
         const float ma = mine[G * D + lane], mb = other[G * D + lane];
         const float M = fmaxf(ma, mb);
-        fa = fast_exp2(ma - M);
-        fb = fast_exp2(mb - M);
+        const float base = M == -INFINITY ? 0.f : M;  // neither has a finite score
+        fa = fast_exp2(ma - base);
+        fb = fast_exp2(mb - base);
         mine[G * D + G + lane] = mine[G * D + G + lane] * fa + other[G * D + G + lane] * fb;
         mine[G * D + lane] = M;
       }

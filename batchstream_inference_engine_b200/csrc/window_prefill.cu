@@ -672,14 +672,15 @@ __global__ void __launch_bounds__(kMergeThreads) window_prefill_merge_kernel(con
   const float* ml = a.records + a.rec_stride_ml;
   float M = -INFINITY;
   for (int32_t s = 0; s < ranges; ++s) M = fmaxf(M, ml[(rec0 + s * kRows) * 2]);
+  const float base = M == -INFINITY ? 0.f : M;
   float L = 0.f, acc[D / 8];
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) acc[i] = 0.f;
 #pragma unroll 4
   for (int32_t s = 0; s < ranges; ++s) {
     const float2 p = *reinterpret_cast<const float2*>(ml + (rec0 + s * kRows) * 2);
-    if (p.x == -INFINITY) continue;  // no key of this row in the range
-    const float f = fast_exp2(p.x - M);
+    // A range without a finite score of this row weighs 0 (NaN scores: 0 * NaN).
+    const float f = fast_exp2(p.x - base);
     L += f * p.y;
     const float4* o = reinterpret_cast<const float4*>(a.records + (rec0 + s * kRows) * D + c);
 #pragma unroll

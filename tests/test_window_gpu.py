@@ -755,3 +755,43 @@ def test_scores_far_from_zero(length, new, heads, kv_heads, window, dtype, head_
         tol = tol + torch.finfo(dtype).eps / 2 * (mean.abs() + tol)
         err = (out[t] - mean.repeat_interleave(G, 0)).abs()
         assert bool((err <= tol.repeat_interleave(G, 0)).all()), (t, float(err.max()))
+
+
+# (context, new tokens, heads, kv heads, window, sequences, keys of a part): the joins of
+# four warps in one CTA, of 8 CTAs in a cluster, of spans over the batch, of the step
+# ranges of a chunk (256 keys each), and of the CUDA-core kernel's ranges.
+JOINS = [(49, 1, 14, 2, 64, 1, 1, torch.bfloat16), (1000, 1, 14, 2, 1024, 1, 120, torch.bfloat16),
+         (16000, 1, 14, 2, 16000, 1, 200, torch.bfloat16),
+         (900, 1, 14, 2, 1024, 200, 300, torch.bfloat16),
+         (478, 128, 2, 2, 351, 1, 256, torch.bfloat16), (700, 30, 14, 2, 600, 1, 256, torch.bfloat16),
+         (1000, 1, 14, 2, 1024, 1, 120, torch.float32), (700, 2, 14, 2, 600, 1, 256, torch.float32)]
+
+
+@pytest.mark.parametrize("length,new,heads,kv_heads,window,seqs,part,dtype", JOINS)
+@pytest.mark.parametrize("newest", [True, False])
+def test_parts_without_a_finite_score_are_joined(length, new, heads, kv_heads, window, seqs, part,
+                                                 dtype, newest):
+    # The newest (or the oldest visible) keys, whole parts of a join, score NaN or -inf.
+    c = Paged([length] * seqs, [new] * seqs, heads, kv_heads, 64, 16, dtype, window, 0, seed=7)
+    run = c.decode if new == 1 else c.chunks
+    c.q[..., 0] = c.q[..., 0].abs() + 0.5
+    first = max(0, length - new - window + 1)
+    at = range(length - part, length) if newest else range(first, first + part)
+    table = c.table.cpu()
+    slots = [int(table[r, p // 16]) * 16 + p % 16 for r in range(seqs) for p in at]
+    keys = c.k.view(kv_heads, -1, 64)
+    kept = keys[:, slots].clone()
+    got = {}
+    for value in (-math.inf, -1e30, math.nan):
+        keys[:, slots] = kept
+        keys[:, slots, 0] = value
+        got[value] = run()
+    assert ops.take_status() == 0
+    pos = [p for p in range(length - new, length)] * seqs
+    for t, p in enumerate(pos):
+        sees = [j for j in at if p - window < j <= p]
+        if sees:
+            assert got[math.nan][t].isnan().all(), t
+        if len(sees) < min(p + 1, window):  # another key is left
+            # Weights of 0 either way.
+            assert got[-1e30][t].isfinite().all() and torch.equal(got[-math.inf][t], got[-1e30][t]), t
