@@ -22,6 +22,7 @@ import subprocess
 import sys
 import sysconfig
 from concurrent.futures import ThreadPoolExecutor
+from importlib.metadata import version
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -29,6 +30,7 @@ CSRC = PACKAGE / "csrc"
 BUILD = PACKAGE / "_build"
 LIBRARY = PACKAGE / "libbatchstream_b200.so"
 BINDING = PACKAGE / "_native.so"
+BINDING_FOR = BUILD / "native_for.txt"  # what the extension was built against
 INCLUDE = PACKAGE.parent / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -87,10 +89,17 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     return LIBRARY
 
 
+def binding_against() -> str:
+    """The versions of Python and torch that the extension's binary interface is tied to."""
+    return f"{sys.implementation.cache_tag} torch {version('torch')}"
+
+
 def build_binding(force: bool = False) -> Path:
     """Compile (if stale) and return the path of the Python extension."""
     source = CSRC / "binding.cpp"
-    if not (force or _stale(BINDING, [source, INCLUDE / "batchstream_b200.h"])):
+    against = binding_against()
+    if not (force or _stale(BINDING, [source, INCLUDE / "batchstream_b200.h"])
+            or not BINDING_FOR.exists() or BINDING_FOR.read_text() != against):
         return BINDING
     compiler = shutil.which("g++")
     if compiler is None:
@@ -113,6 +122,7 @@ def build_binding(force: bool = False) -> Path:
     if proc.returncode != 0:
         raise RuntimeError(f"building {BINDING.name} failed:\n{proc.stderr}")
     tmp.replace(BINDING)
+    BINDING_FOR.write_text(against)
     return BINDING
 
 

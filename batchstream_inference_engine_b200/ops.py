@@ -8,6 +8,7 @@ surface as ``RuntimeError``, as the reference op raises them through
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import threading
@@ -20,8 +21,21 @@ from ._lib import BS_BF16, BS_F32, check, i64_array, lib
 try:
     from . import _native
 except ImportError as e:
-    raise ImportError("the _native extension is not built or does not load; run "
-                      "`python -m batchstream_inference_engine_b200.build`") from e
+
+    class _Missing:
+        """Stands for the extension where it is not built or does not load (it belongs to
+        one version of torch): the operators in it fail when called, the others do not
+        need it."""
+
+        def __init__(self, cause):
+            self._cause = cause
+
+        def __getattr__(self, name):
+            raise ImportError(f"{name}: the _native extension is not built or does not load; run "
+                              "`python -m batchstream_inference_engine_b200.build`"
+                              ) from self._cause
+
+    _native = _Missing(e)
 
 _DTYPES = {torch.bfloat16: BS_BF16, torch.float32: BS_F32}
 
@@ -97,7 +111,8 @@ class _Workspaces:
 
 _workspaces = _Workspaces()
 _status_words = _StatusWords()
-_native.set_status_source(lambda index, stream: _status_words.get(index, stream).data_ptr())
+with contextlib.suppress(ImportError):
+    _native.set_status_source(lambda index, stream: _status_words.get(index, stream).data_ptr())
 
 
 def workspace_for(device: torch.device, nbytes: int) -> torch.Tensor:
