@@ -11,13 +11,16 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
 #include <initializer_list>
+#include <map>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -145,6 +148,26 @@ struct Launch {
     status = status_word(device.index(), stream);
   }
 };
+
+// (bytes, device index): zero bytes for good, whatever the current stream records.  A
+// stream of its own fills them, waited for here; the allocator gives a captured stream's
+// pool to that stream alone.
+PyObject* zeros_apart(PyObject* const* a) {
+  const int64_t bytes = int_of(a[0]);
+  const auto device = static_cast<c10::DeviceIndex>(int_of(a[1]));
+  const c10::cuda::CUDAGuard guard(device);
+  const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+  static std::map<c10::DeviceIndex, cudaStream_t> streams;
+  cudaStream_t& stream = streams[device];
+  if (stream == nullptr) {
+    C10_CUDA_CHECK(cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking));
+  }
+  const c10::cuda::CUDAStreamGuard on(c10::cuda::getStreamFromExternal(stream, device));
+  const Tensor t = at::empty({bytes}, at::TensorOptions(at::kByte).device(at::kCUDA, device));
+  C10_CUDA_CHECK(cudaMemsetAsync(t.data_ptr(), 0, bytes, stream));
+  C10_CUDA_CHECK(cudaStreamSynchronize(stream));
+  return THPVariable_Wrap(t);
+}
 
 // Scratch of one call, from the stream-ordered allocator (inside a capture: from the
 // graph's own pool, so two graphs never share it).
@@ -431,6 +454,7 @@ PyMethodDef g_methods[] = {
     method<rotary_append, 10>("rotary_append"),
     method<copy_blocks, 4>("copy_blocks"),
     method<set_status_source, 1>("set_status_source"),
+    method<zeros_apart, 2>("zeros_apart"),
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -8,7 +8,6 @@ surface as ``RuntimeError``, as the reference op raises them through
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 import threading
@@ -18,23 +17,21 @@ import torch
 from . import _lib
 from ._lib import BS_BF16, BS_F32, check, i64_array, lib
 
+class _Missing:
+    """Stands for the extension where it is not built or does not load (it belongs to one
+    version of torch): the operators in it fail when called, the others do not need it."""
+
+    def __init__(self, cause):
+        self._cause = cause
+
+    def __getattr__(self, name):
+        raise ImportError(f"{name}: the _native extension is not built or does not load; run "
+                          "`python -m batchstream_inference_engine_b200.build`") from self._cause
+
+
 try:
     from . import _native
 except ImportError as e:
-
-    class _Missing:
-        """Stands for the extension where it is not built or does not load (it belongs to
-        one version of torch): the operators in it fail when called, the others do not
-        need it."""
-
-        def __init__(self, cause):
-            self._cause = cause
-
-        def __getattr__(self, name):
-            raise ImportError(f"{name}: the _native extension is not built or does not load; run "
-                              "`python -m batchstream_inference_engine_b200.build`"
-                              ) from self._cause
-
     _native = _Missing(e)
 
 _DTYPES = {torch.bfloat16: BS_BF16, torch.float32: BS_F32}
@@ -65,6 +62,18 @@ def _require_cuda(name: str, *tensors: torch.Tensor) -> torch.device:
     return device
 
 
+def _zeros(nbytes: int, device: torch.device) -> tuple[torch.Tensor, bool]:
+    """Zero bytes that outlive graphs, and whether the current stream is being captured.
+    Inside a capture torch.zeros would record its fill into the graph: nothing would be
+    zero before the first replay, and every replay would clear what is there."""
+    # (Not inference tensors, which a later call outside inference mode could not clear.)
+    with torch.cuda.device(device), torch.inference_mode(False):
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing and not isinstance(_native, _Missing):
+            return _native.zeros_apart(nbytes, torch.cuda.current_device()), True
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device), capturing
+
+
 class _StatusWords:
     """One zero-filled status word per (device, stream) for the calls that keep no
     workspace.  A word never moves: captured calls hold its address."""
@@ -77,7 +86,7 @@ class _StatusWords:
         with self._lock:
             word = self._words.get((index, stream))
             if word is None:
-                word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+                word = _zeros(4, torch.device("cuda", index))[0].view(torch.int32)
                 self._words[index, stream] = word
             return word
 
@@ -86,12 +95,14 @@ class _Workspaces:
     """Zero-filled scratch buffers, one per (device, stream), grown on demand.
 
     The kernels leave the counter region zero after every call, so a buffer is
-    zero-filled only when it is (re)allocated.
+    zero-filled only when it is (re)allocated.  Outgrown buffers stay: captured calls
+    hold their addresses, and report there.
     """
 
     def __init__(self):
         self._lock = threading.Lock()
         self._buffers: dict[tuple[int, int], torch.Tensor] = {}
+        self._outgrown: dict[tuple[int, int], list[torch.Tensor]] = {}
 
     def get(self, device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
         key = (device.index if device.index is not None else torch.cuda.current_device(), stream)
@@ -101,17 +112,24 @@ class _Workspaces:
                 size = max(nbytes, 1 << 20)
                 if buf is not None:
                     size = max(size, 2 * buf.numel())
-                fresh = torch.zeros(size, dtype=torch.uint8, device=device)
-                if buf is not None:  # keep status bits not yet taken
-                    fresh[:4].copy_(buf[:4])
+                fresh, capturing = _zeros(size, device)
+                if buf is not None:
+                    if not capturing:  # status bits not yet taken move along
+                        fresh[:4].copy_(buf[:4])
+                        buf[:4].zero_()
+                    self._outgrown.setdefault(key, []).append(buf)
                 buf = fresh
                 self._buffers[key] = buf
             return buf
 
+    def outgrown(self, device: torch.device, stream: int) -> list[torch.Tensor]:
+        key = (device.index if device.index is not None else torch.cuda.current_device(), stream)
+        return list(self._outgrown.get(key, ()))
+
 
 _workspaces = _Workspaces()
 _status_words = _StatusWords()
-with contextlib.suppress(ImportError):
+if not isinstance(_native, _Missing):
     _native.set_status_source(lambda index, stream: _status_words.get(index, stream).data_ptr())
 
 
@@ -133,7 +151,8 @@ def take_status(device: torch.device | None = None) -> int:
     """Synchronise the current stream and raise if a kernel set a status bit.
 
     Returns 0 when no bit was set (kernels never fault on bad tables, lengths or
-    slots; they record the problem here instead).
+    slots; they record the problem here instead).  A captured call reports, at every
+    replay, to the stream it was captured on: take that stream's status.
     """
     device = device or torch.device("cuda", torch.cuda.current_device())
     stream = torch.cuda.current_stream(device).cuda_stream
@@ -143,12 +162,13 @@ def take_status(device: torch.device | None = None) -> int:
     rc = lib().bs_take_status(word.data_ptr(), stream, ctypes.byref(bits))
     if bits.value:  # reported by a call without a workspace; the other word's turn is next
         check(rc)
-    rc = lib().bs_take_status(ws.data_ptr(), stream, ctypes.byref(bits))
-    if bits.value:
-        # A launch that reported a problem may have left segment counters set:
-        # clear them so that the next call on this workspace starts clean.
-        check(lib().bs_reset_workspace(ws.data_ptr(), stream))
-    check(rc)
+    for ws in (ws, *_workspaces.outgrown(device, stream)):
+        rc = lib().bs_take_status(ws.data_ptr(), stream, ctypes.byref(bits))
+        if bits.value:
+            # A launch that reported a problem may have left segment counters set:
+            # clear them so that the next call on this workspace starts clean.
+            check(lib().bs_reset_workspace(ws.data_ptr(), stream))
+        check(rc)
     return bits.value
 
 
