@@ -375,8 +375,9 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
       if (first && !early) load_query(stage, ci, ch);
     }
     if (!dry && !probe) armed |= 1u << stage;
-    // Advance to the next unit.
-    ++cu;
+    // Advance to the next unit.  (WIN: the last one looks no further, least of all a
+    // cluster's, whose next sequences are others' and in a padded batch all empty.)
+    if (++cu == wr1 && WIN) return;
     if (++cb == cnb) {
       cb = 0;
       if (++ch == Hkv) {
