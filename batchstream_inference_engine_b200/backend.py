@@ -170,6 +170,10 @@ class PagedBackend:
         outputs = {}
         for seq_id, sequence, row in launched.rows:
             if row is None or sequence.finished:
+                if sequence.feeds is launched:
+                    # The row that ran on past the end: its input, the ending token, is
+                    # cached, and its output is nobody's.
+                    sequence.next_token = sequence.feeds = None
                 continue
             token = tokens[row]
             if sequence.feeds is launched:

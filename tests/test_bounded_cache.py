@@ -325,6 +325,58 @@ def test_fork_sequence_composes_the_child_prompt():
     assert backend.blocks_in_use == 0
 
 
+class Ids:
+    """A launched step whose ids are known."""
+
+    def __init__(self, ids):
+        self._ids = ids
+
+    def ref(self, i):
+        return -1 - i
+
+    def result(self):
+        return self._ids
+
+
+def test_fork_of_a_sequence_that_ended_with_a_step_in_flight(monkeypatch):
+    # The pipelined loop launches one step past an end-of-generation token.
+    config = ModelConfig(**TINY)
+    model = TorchModel(config, random_weights(config, vocab_size=50, intermediate_size=16),
+                       device="cpu", dtype=torch.float32, max_position=64)
+    end = 49
+    answers = iter([[5], [end], [7]])
+
+    def launch_tokens(groups):
+        for tokens, cache in groups:
+            cache.reserve(len(tokens))
+            cache.advance(len(tokens))
+        return Ids(next(answers))
+
+    monkeypatch.setattr(model, "launch_tokens", launch_tokens)
+
+    class Vocab:
+        def is_end_of_generation(self, token):
+            return token == end
+
+    backend = PagedBackend(model, num_blocks=16, block_size=4, prefill_chunk=8, vocab=Vocab(),
+                           max_seqs=8)
+    s = backend.start_sequence([1, 2, 3])
+    first = backend.launch()
+    second = backend.launch()
+    backend.finish(first)
+    third = backend.launch()  # the host does not know yet that `end` was generated
+    assert backend.finish(second)[s].finished
+    with pytest.raises(RuntimeError, match="unfinished"):
+        backend.fork_sequence(s, [8, 9])
+    assert backend.finish(third) == {}
+    child = backend._sequences[backend.fork_sequence(s, [8, 9])]
+    # 1 2 3, 5 and the ending token are cached.
+    assert child.cache.length == 5 and list(child.pending) == [8, 9]
+    assert child.next_token is None
+    with pytest.raises(RuntimeError, match="finished"):
+        backend.fork_sequence(s, [])
+
+
 # ------------------------------------------------------------------ refusals of the C ABI
 
 
