@@ -360,7 +360,7 @@ def test_fork_of_a_sequence_that_ended_with_a_step_in_flight(monkeypatch):
 
     backend = PagedBackend(model, num_blocks=16, block_size=4, prefill_chunk=8, vocab=Vocab(),
                            max_seqs=8)
-    s = backend.start_sequence([1, 2, 3])
+    s = backend.start_sequence([1, 2])
     first = backend.launch()
     second = backend.launch()
     backend.finish(first)
@@ -370,8 +370,8 @@ def test_fork_of_a_sequence_that_ended_with_a_step_in_flight(monkeypatch):
         backend.fork_sequence(s, [8, 9])
     assert backend.finish(third) == {}
     child = backend._sequences[backend.fork_sequence(s, [8, 9])]
-    # 1 2 3, 5 and the ending token are cached.
-    assert child.cache.length == 5 and list(child.pending) == [8, 9]
+    # 1 2, 5 and the ending token are cached: a whole block, so that nothing is copied.
+    assert child.cache.length == 4 and list(child.pending) == [8, 9]
     assert child.next_token is None
     with pytest.raises(RuntimeError, match="finished"):
         backend.fork_sequence(s, [])
