@@ -125,14 +125,22 @@ class BlockAllocator:
         blocks are shared (neither sequence writes them again), and a last
         partial block is taken from the free list for the child.  Returns that
         block's (source, destination) copy, if any.  Takes nothing and raises
-        OutOfBlocks when no block or device table row is free."""
+        OutOfBlocks when no block or device table row is free.
+
+        A trimmed sequence is forked where its window ends, at its cached tokens:
+        earlier ones would look back on blocks that are gone.  A fork that ends among
+        those is refused."""
         table = self._tables[seq_id]
         if child_id in self._tables:
             raise ValueError(f"sequence {child_id} already exists")
         whole, tail = divmod(tokens, self._block_size)
         if tokens < 0 or whole + (tail > 0) > len(table):
             raise ValueError(f"sequence {seq_id} has no blocks for {tokens} tokens")
-        copied = tail > 0 and table[whole] != EMPTY_BLOCK
+        if (tokens < self._trimmed.get(seq_id, 0) * self._block_size
+                and EMPTY_BLOCK in table[: whole + (tail > 0)]):
+            raise ValueError(f"sequence {seq_id} has given up blocks that {tokens} tokens look "
+                             "back on")
+        copied = tail > 0
         if copied and not self._free:
             raise OutOfBlocks(f"forking sequence {seq_id} needs a block but none is free")
         if self.device_tables is not None:
@@ -150,8 +158,6 @@ class BlockAllocator:
         if copied:
             child.append(self._free.pop())
             pairs.append((table[whole], child[-1]))
-        elif tail:
-            child.append(EMPTY_BLOCK)
         self._tables[child_id] = child
         return pairs
 

@@ -106,6 +106,22 @@ def test_trimming_a_shared_block_keeps_it_for_the_other_sequence():
     assert sorted(a._free) == list(range(32)) and not a._refs and not a._trimmed
 
 
+def test_fork_refuses_tokens_whose_blocks_are_gone():
+    a = mirrored()
+    a.allocate(0, 30)
+    a.trim(0, 17, keep_first=4)  # blocks 1 to 3; block 4 holds token 17
+    for tokens in (5, 8, 13, 15):
+        with pytest.raises(ValueError):
+            a.fork(0, 1, tokens)
+    assert 1 not in a._tables and len(a._free_rows) == 5 and not a._refs
+    assert a.fork(0, 3, 4) == [] and a.block_table(3) == a.block_table(0)[:1]  # the sinks alone
+    assert a.fork(0, 1, 30) == [(a.block_table(0)[7], a.block_table(1)[7])]
+    assert a.block_table(1)[:7] == a.block_table(0)[:7]
+    a.trim(0, 1000)  # the partial last block too
+    with pytest.raises(ValueError):
+        a.fork(0, 2, 30)
+
+
 def test_compact_moves_the_highest_blocks_into_the_lowest_holes():
     a = mirrored(num_blocks=12)
     for s in range(3):
