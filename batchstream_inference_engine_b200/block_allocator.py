@@ -38,7 +38,8 @@ class BlockAllocator:
         self._free = list(range(num_blocks))
         self._tables: dict[int, list[int]] = {}
         self._refs: dict[int, int] = {}  # tables that hold a block, where more than one does
-        self._trimmed: dict[int, int] = {}  # entries below this were looked at by trim
+        self._trimmed: dict[int, int] = {}  # entries below this were given up by trim,
+        self._kept: dict[int, int] = {}  # down to this one (ahead of it are the sinks)
         self.num_blocks = num_blocks
         # Device mirror (optional).
         self._device = torch.device(device) if device is not None else None
@@ -99,6 +100,7 @@ class BlockAllocator:
         for block in self._tables.pop(seq_id):
             self._release(block)
         self._trimmed.pop(seq_id, None)
+        self._kept.pop(seq_id, None)
         row = self._rows.pop(seq_id, None)
         if row is not None:
             self._synced.pop(seq_id, None)
@@ -154,6 +156,7 @@ class BlockAllocator:
                 self._refs[block] = self._refs.get(block, 1) + 1
         if seq_id in self._trimmed:
             self._trimmed[child_id] = min(self._trimmed[seq_id], whole)
+            self._kept[child_id] = self._kept[seq_id]
         pairs = []
         if copied:
             child.append(self._free.pop())
@@ -168,13 +171,19 @@ class BlockAllocator:
         freed (a block that a fork still holds stays in use)."""
         table = self._tables[seq_id]
         end = min(first_token // self._block_size, len(table))
-        begin = max(self._trimmed.get(seq_id, 0), -(-keep_first // self._block_size))
+        keep = -(-max(keep_first, 0) // self._block_size)
+        if keep >= end:
+            return 0
+        low, high = self._kept.get(seq_id, keep), self._trimmed.get(seq_id, keep)  # given up
         freed = 0
-        for i in range(begin, end):
+        for i in (*range(keep, min(low, end)), *range(max(keep, high), end)):
             freed += self._release(table[i])
             table[i] = EMPTY_BLOCK
-        if end > begin:
-            self._trimmed[seq_id] = end
+        if keep > high:
+            low = keep
+        elif end >= low:
+            low = min(low, keep)
+        self._kept[seq_id], self._trimmed[seq_id] = low, max(high, end)
         return freed
 
     def compact(self) -> list[tuple[int, int]]:

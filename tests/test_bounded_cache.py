@@ -90,6 +90,33 @@ def test_trim_gives_up_the_blocks_between_sinks_and_window():
     assert sorted(a._free) == list(range(32))
 
 
+def test_trim_with_fewer_sinks_than_before():
+    a = mirrored()
+    a.allocate(0, 40)
+    table = list(a.block_table(0))
+    assert a.trim(0, 21, keep_first=9) == 2  # blocks 3 and 4
+    assert a.trim(0, 7, keep_first=4) == 0  # block 0 stays, block 1 holds token 7
+    assert a.trim(0, 8, keep_first=4) == 1
+    assert a.trim(0, 33, keep_first=0) == 5  # blocks 0, 2, 5, 6, 7
+    assert a.block_table(0) == [EMPTY_BLOCK] * 8 + table[8:]
+    a.free(0)
+    assert sorted(a._free) == list(range(32)) and not a._trimmed and not a._kept
+
+
+def test_trims_in_any_order_give_up_what_each_asks_for():
+    rng = random.Random(1)
+    for _ in range(300):
+        a = mirrored(num_blocks=16, block_size=3)
+        a.allocate(0, 48)
+        gone = set()
+        for _ in range(6):
+            first, keep = rng.randint(-3, 60), rng.randint(0, 30)
+            want = {i for i in range(16) if 3 * i + 3 <= first and 3 * i >= keep} - gone
+            assert a.trim(0, first, keep_first=keep) == len(want)
+            gone |= want
+            assert {i for i, b in enumerate(a.block_table(0)) if b == EMPTY_BLOCK} == gone
+
+
 def test_trimming_a_shared_block_keeps_it_for_the_other_sequence():
     a = mirrored()
     a.allocate(0, 16)
