@@ -184,6 +184,7 @@ class PagedKVPool:
         # reference) before the host has read it.  Rows: every live sequence,
         # plus the padding of a graph-captured step.
         self.last_ids = torch.zeros(max_seqs + 64, dtype=torch.int32, device=self.device)
+        self.copies = 0  # block copies issued: from the first on, steps look at their status
 
     @property
     def free_blocks(self) -> int:
@@ -223,6 +224,7 @@ class PagedKVPool:
             ends = torch.tensor(pairs, dtype=torch.int32).t().contiguous().pin_memory()
             src, dst = ends.to(self.device, non_blocking=True)
             ops.copy_blocks(self.keys, self.values, src, dst)
+            self.copies += 1
 
 
 class PagedKVCache:
@@ -383,9 +385,9 @@ class TorchModel:
         logits = self.forward_batch(groups)
         ids = ops.argmax_rows(logits)
         pool.last_ids[: ids.numel()].copy_(ids)
-        return self._pending(ids, list(range(len(groups))))
+        return self._pending(pool, ids, list(range(len(groups))))
 
-    def _pending(self, ids: torch.Tensor, index: list[int]) -> PendingTokens:
+    def _pending(self, pool: PagedKVPool, ids: torch.Tensor, index: list[int]) -> PendingTokens:
         """Copies `ids` to one of a few pinned buffers and records the event the
         host waits on; at most len(self._hosts) - 1 steps may be pending."""
         n = ids.numel()
@@ -398,11 +400,11 @@ class TorchModel:
         host.copy_(ids, non_blocking=True)
         # Kernels report bad input in the status words of their stream (eager
         # calls: this stream; graph replays: the capture stream's): copied after
-        # the step, read with the ids.  Only a model with the operators that use
-        # the second word of a stream needs to look at it.
+        # the step, read with the ids.  The second word of a stream is that of the
+        # operators of bounded caches, and of the pool's block copies.
         words = ops.status_words(self.device)
         words += self._graph_status or []
-        if not self._bounded:
+        if not self._bounded and not pool.copies:
             words = words[::2]
         status.fill_(0)
         for i, word in enumerate(words):
@@ -760,7 +762,7 @@ class TorchModel:
         st["attn_flops"] += self._attention_flops(starts, lengths)
         st["launches"] += graph_launches
         index = list(range(n_dec)) + list(range(B, B + len(groups) - n_dec))
-        return self._pending(ids, index)
+        return self._pending(pool, ids, index)
 
 
 def _powers_of_two(lo: int, limit: int) -> list[int]:

@@ -239,3 +239,26 @@ def test_default_rotary_over_frequencies_and_a_full_window(exact_gemm):
     # The table-driven embedding rounds cos and sin to bf16 (2^-9 of 1 each), so q and k
     # are off by up to 2^-8 of themselves; through 2 layers of scores and values.
     assert float((logits[0] - logits[1]).abs().max()) <= 0.05 * float(logits[1].abs().max())
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+def test_a_skipped_block_copy_fails_the_next_step_of_any_model(exact_gemm, graphs):
+    # Block copies report in the second status word, which a model without a window or
+    # another rotary form does not write otherwise.
+    config = ModelConfig(num_layers=2, hidden_size=256, num_heads=4, num_kv_heads=2,
+                         rope_theta=1e4, rms_norm_eps=1e-6)
+    model = TorchModel(config, weights_of(config), device=DEV, dtype=torch.bfloat16,
+                       max_position=256, step_graphs=graphs, max_graph_batch=4)
+    backend = PagedBackend(model, num_blocks=32, block_size=16, prefill_chunk=64, vocab=NoEnd(),
+                           max_seqs=4)
+    a = backend.start_sequence(list(range(1, 20)))
+    backend.step()
+    child = backend.fork_sequence(a, [5])
+    backend.step()
+    backend.step()
+    backend.pool._copy([(3, 4), (5, 4)])  # clashing pairs, as a broken allocator would give
+    with pytest.raises(RuntimeError, match="named by another pair"):
+        backend.step()
+    backend.step()
+    for s in (a, child):
+        backend.release_sequence(s)
