@@ -21,6 +21,7 @@ from itertools import count
 
 import torch
 
+from .serve import BlockBudget
 from .torch_model import PagedKVCache, PagedKVPool, TorchModel
 
 
@@ -70,12 +71,20 @@ class PagedBackend:
 
     ``num_blocks`` / ``block_size`` / ``prefill_chunk`` mean what they mean in
     the reference; ``max_seqs`` bounds the live sequences (device table rows).
+
+    With a sliding window a sequence holds only the blocks it still sees
+    (``sequence_blocks``) and may grow past the pool, up to the model's
+    ``max_position`` tokens: a table row keeps an entry for every block a sequence
+    ever had.  ``block_budget()`` admits requests by what they hold.
     """
 
     def __init__(self, model: TorchModel, num_blocks: int, block_size: int, prefill_chunk: int,
                  vocab=None, max_seqs: int = 256, pool_dtype: torch.dtype | None = None):
         self._model = model
-        max_blocks = min(num_blocks, -(-model.max_position // block_size))
+        max_blocks = -(-model.max_position // block_size)
+        if not model.config.attention_window:
+            max_blocks = min(num_blocks, max_blocks)
+        self._max_blocks = max_blocks
         self._pool = PagedKVPool(model.config, num_blocks, block_size, device=model.device,
                                  dtype=pool_dtype or model.dtype, max_seqs=max_seqs,
                                  max_blocks_per_seq=max_blocks)
@@ -92,6 +101,24 @@ class PagedBackend:
     @property
     def pool(self) -> PagedKVPool:
         return self._pool
+
+    @property
+    def sequence_blocks(self) -> int | None:
+        """The most blocks that a sequence holds at a time (None: as many as its tokens fill).
+
+        While a step adds n <= prefill_chunk tokens to L cached ones, these are the
+        sinks' and those of tokens L - window + 1 to L + n - 1, which begin anywhere in
+        their first block."""
+        config, size = self._model.config, self._pool.block_size
+        if not config.attention_window:
+            return None
+        seen = config.attention_window - 1 + max(self._prefill_chunk, 1)
+        return -(-config.attention_sinks // size) + (seen + 2 * size - 2) // size
+
+    def block_budget(self) -> BlockBudget:
+        """The admission budget of this backend's pool."""
+        return BlockBudget(self._num_blocks, self._pool.block_size, self.sequence_blocks,
+                           self._max_blocks * self._pool.block_size)
 
     def tokenize(self, text: str) -> list[int]:
         return self._vocab.tokenize(text)

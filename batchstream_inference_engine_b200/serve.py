@@ -24,18 +24,25 @@ from dataclasses import dataclass, field
 
 class BlockBudget:
     """src/server/kv_budget.py:1-36: capacity in blocks, requests reserve their
-    worst case rounded up to whole blocks."""
+    worst case rounded up to whole blocks.  ``sequence_blocks``: the most that one
+    sequence holds at a time (a sliding window gives blocks back); ``sequence_tokens``:
+    the longest sequence there can be (``PagedBackend.block_budget`` knows both)."""
 
-    def __init__(self, num_blocks: int, block_size: int):
+    def __init__(self, num_blocks: int, block_size: int, sequence_blocks: int | None = None,
+                 sequence_tokens: int | None = None):
         self._capacity = num_blocks
         self.available = num_blocks
         self._block_size = block_size
+        self._sequence_blocks = sequence_blocks
+        self._sequence_tokens = sequence_tokens
 
     def _blocks(self, tokens: int) -> int:
-        return -(-tokens // self._block_size)
+        blocks = -(-tokens // self._block_size)
+        return blocks if self._sequence_blocks is None else min(blocks, self._sequence_blocks)
 
     def fits_ever(self, tokens: int) -> bool:
-        return self._blocks(tokens) <= self._capacity
+        return (self._blocks(tokens) <= self._capacity
+                and (self._sequence_tokens is None or tokens <= self._sequence_tokens))
 
     def try_reserve(self, tokens: int) -> bool:
         blocks = self._blocks(tokens)

@@ -449,8 +449,7 @@ class TorchModel:
         lengths = [len(tokens) for tokens, _ in groups]
         T = sum(lengths)
         starts = [cache.length for _, cache in groups]
-        if max(s + n for s, n in zip(starts, lengths)) > self.max_position:
-            raise RuntimeError(f"positions beyond the rotary table ({self.max_position})")
+        self._check_positions(starts, lengths)
         rows = [alloc.row(cache.seq_id) for _, cache in groups]
         flat = [t for tokens, _ in groups for t in tokens]
         ends = [sum(lengths[: i + 1]) - 1 for i in range(R)]
@@ -498,6 +497,12 @@ class TorchModel:
         st["attn_flops"] += self._attention_flops(starts, lengths)
         st["launches"] += ops.kernel_launches() - launches
         return last
+
+    def _check_positions(self, starts, lengths) -> None:
+        # (Without tables the row of block-table entries is the only limit: the allocator's.)
+        if (self.config.rotary_from_tables
+                and max(s + n for s, n in zip(starts, lengths)) > self.max_position):
+            raise RuntimeError(f"positions beyond the rotary table ({self.max_position})")
 
     def _attend_tokens(self, q, kp, vp, tables, lens, rows, out) -> None:
         """One layer's attention of the rows that hold one new token each."""
@@ -743,8 +748,7 @@ class TorchModel:
         self.stats["h2d_bytes"] += 16 * alloc.sync_device()
         lengths = [len(tokens) for tokens, _ in groups]
         starts = [cache.length for _, cache in groups]
-        if max(s + n for s, n in zip(starts, lengths)) > self.max_position:
-            raise RuntimeError(f"positions beyond the rotary table ({self.max_position})")
+        self._check_positions(starts, lengths)
         n_dec = 0
         while n_dec < len(lengths) and lengths[n_dec] == 1:
             n_dec += 1

@@ -368,6 +368,60 @@ def test_fork_sequence_composes_the_child_prompt():
     assert backend.blocks_in_use == 0
 
 
+@pytest.mark.parametrize("window,sinks,block,chunk", [
+    (1, 0, 1, 1), (70, 5, 16, 32), (64, 16, 16, 16), (5, 33, 4, 9), (100, 0, 7, 1), (3, 2, 16, 40)])
+def test_sequence_blocks_bound_what_a_windowed_sequence_holds(window, sinks, block, chunk):
+    config = ModelConfig(**TINY, attention_window=window, attention_sinks=sinks)
+    model = TorchModel(config, random_weights(config, vocab_size=50, intermediate_size=16),
+                       device="cpu", dtype=torch.float32, max_position=4096)
+    backend = PagedBackend(model, num_blocks=400, block_size=block, prefill_chunk=chunk,
+                           max_seqs=64)
+    rng = random.Random(window)
+    most = 0
+    for seq in range(30):
+        cache = backend.pool.new_cache(seq)
+        cache.reserve(0)
+        while cache.length < 700:
+            n = rng.choice([1, rng.randint(1, chunk), chunk])
+            cache.reserve(n)
+            most = max(most, sum(b != EMPTY_BLOCK for b in backend.pool.block_table(seq)))
+            cache.advance(n)
+            backend.pool.trim(cache, window, sinks)
+        backend.pool.release(cache)
+    assert 0.9 * backend.sequence_blocks - 1 <= most <= backend.sequence_blocks
+    budget = backend.block_budget()
+    assert budget.fits_ever(4096 // block * block) and not budget.fits_ever(4096 + block)
+    budget.try_reserve(4000)
+    assert 400 - budget.available == min(-(-4000 // block), backend.sequence_blocks)
+    budget.try_reserve(1)
+    budget.release(4000)
+    assert budget.available == 399
+
+
+def test_without_a_window_the_budget_is_the_plain_one():
+    model = TorchModel(ModelConfig(**TINY), random_weights(ModelConfig(**TINY), vocab_size=50,
+                                                           intermediate_size=16),
+                       device="cpu", dtype=torch.float32, max_position=64)
+    backend = PagedBackend(model, num_blocks=10, block_size=4, prefill_chunk=8, max_seqs=8)
+    assert backend.sequence_blocks is None
+    budget = backend.block_budget()
+    assert budget.fits_ever(40) and not budget.fits_ever(41)
+    assert budget.try_reserve(37) and budget.available == 0
+
+
+def test_only_rotary_tables_limit_positions():
+    for kw, limited in (({}, True), ({"rope_scaling": {"type": "linear", "factor": 2.0}}, False)):
+        config = ModelConfig(**TINY, **kw)
+        model = TorchModel(config, random_weights(config, vocab_size=50, intermediate_size=16),
+                           device="cpu", dtype=torch.float32, max_position=64)
+        model._check_positions([60, 0], [4, 64])
+        if limited:
+            with pytest.raises(RuntimeError, match="rotary table"):
+                model._check_positions([0, 64], [1, 1])
+        else:
+            model._check_positions([0, 64], [1, 1])
+
+
 class Ids:
     """A launched step whose ids are known."""
 

@@ -262,3 +262,21 @@ def test_a_skipped_block_copy_fails_the_next_step_of_any_model(exact_gemm, graph
     backend.step()
     for s in (a, child):
         backend.release_sequence(s)
+
+
+@pytest.mark.parametrize("pipelined,graphs", [(False, False), (True, True)])
+def test_conversations_longer_than_the_pool(exact_gemm, pipelined, graphs):
+    # 20 blocks hold 320 tokens; each request runs to between 330 and 700.
+    weights = weights_of()
+    model = TorchModel(CONFIG, weights, device=DEV, dtype=torch.float32, max_position=1024,
+                       step_graphs=graphs, max_graph_batch=8, max_graph_prefill=64)
+    backend = PagedBackend(model, num_blocks=20, block_size=16, prefill_chunk=32, vocab=NoEnd(),
+                           max_seqs=4)
+    assert backend.sequence_blocks == 9  # one of the sinks, eight of 69 + 32 tokens
+    rng = np.random.default_rng(9)
+    specs = [(rng.integers(0, VOCAB, n).tolist(), m) for n, m in ((500, 200), (10, 400), (330, 3))]
+    requests = serve(backend, specs, 4, backend.block_budget(), pipelined=pipelined)
+    assert not any(r.failed for r in requests) and backend.blocks_in_use == 0
+    for (prompt, n), request in zip(specs, requests):
+        assert len(request.tokens) == n
+        check_generated(weights, prompt, request.tokens, torch.float32)
