@@ -41,6 +41,80 @@ from . import ops
 from .block_allocator import BlockAllocator
 
 
+# Keys of a checkpoint's config.json beyond the reference's six, in the names that
+# checkpoints use.  A form that this package does not have is refused, not ignored.
+
+
+def _checkpoint_window(config: dict) -> int:
+    """attention_window of a config.json: the layers all have it or none has."""
+    window = config.get("sliding_window")
+    layers = config["num_hidden_layers"]
+    kinds = config.get("layer_types")
+    if kinds is not None:
+        windowed = sum(kind == "sliding_attention" for kind in kinds)
+        if windowed + sum(kind == "full_attention" for kind in kinds) != layers:
+            raise ValueError(f"layer_types {kinds} are not full or sliding attention of all layers")
+    elif not window or not config.get("use_sliding_window", True):
+        windowed = 0
+    elif "use_sliding_window" in config:  # from the layer max_window_layers on
+        windowed = max(0, layers - config.get("max_window_layers", 0))
+    else:
+        windowed = layers
+    if windowed not in (0, layers):
+        raise ValueError(f"{windowed} of {layers} layers have a sliding window: all or none can")
+    if windowed and not (window and window > 0):
+        raise ValueError(f"sliding attention needs a positive sliding_window, not {window!r}")
+    return int(window) if windowed else 0
+
+
+def _checkpoint_rope(config: dict) -> dict:
+    both = [config[k] for k in ("rope_scaling", "rope_parameters") if config.get(k)]
+    if len(both) == 2 and both[0] != both[1]:
+        raise ValueError("rope_scaling and rope_parameters disagree")
+    return dict(both[0]) if both else {}
+
+
+def _checkpoint_rotary_dim(config: dict, head_dim: int) -> int:
+    """rotary_dim of a config.json (0: the whole head)."""
+    part = config.get("partial_rotary_factor") or _checkpoint_rope(config).get(
+        "partial_rotary_factor") or 1.0
+    dim = round(head_dim * part)
+    if not 0 < part <= 1 or dim < 2 or dim % 2 or abs(head_dim * part - dim) > 1e-6:
+        raise ValueError(f"partial_rotary_factor {part!r} of {head_dim} dims is not an even number")
+    return 0 if dim == head_dim else dim
+
+
+def _checkpoint_scaling(config: dict) -> dict | None:
+    """rope_scaling of a config.json, as ops.rope_frequencies takes it."""
+    rope = _checkpoint_rope(config)
+    kind = rope.pop("rope_type", None) or rope.get("type")
+    rope.pop("type", None)
+    for name in ("rope_theta", "partial_rotary_factor"):
+        value = rope.pop(name, None)
+        if value is not None and config.get(name, value) != value:
+            raise ValueError(f"{name} is given twice, as {config[name]!r} and {value!r}")
+    if kind in (None, "default") and not rope:
+        return None
+    length = rope.pop("original_max_position_embeddings", None)
+    if length is None:
+        length = config.get("max_position_embeddings")
+    if kind == "linear":
+        known, scaling = ("factor",), {}
+    elif kind == "yarn":
+        known = ("factor", "beta_fast", "beta_slow", "attention_factor")
+        scaling = {"original_max_position": length}
+    elif {"low_freq_factor", "high_freq_factor"} <= rope.keys():
+        kind, known = "banded", ("factor", "low_freq_factor", "high_freq_factor")
+        scaling = {"original_max_position": length}
+    else:
+        raise ValueError(f"rotary scaling {kind!r} is not supported")
+    if rope.pop("truncate", True) is not True or rope.keys() - set(known):
+        raise ValueError(f"{kind} rotary scaling with {sorted(rope.keys() - set(known))} or "
+                         "without truncation is not supported")
+    scaling |= {k: v for k, v in rope.items() if v is not None}
+    return {"type": kind, **scaling}
+
+
 @dataclass(frozen=True)
 class ModelConfig:
     """src/server/torch_model.py:13-36 (the same fields and head_dim rule)."""
@@ -64,14 +138,21 @@ class ModelConfig:
 
     @classmethod
     def from_file(cls, path: Path) -> "ModelConfig":
+        """The model of a checkpoint's config.json, with its sliding window, rotary scaling
+        ("linear", "yarn", or by low_freq_factor and high_freq_factor) and partial rotary
+        embedding; ValueError for forms of these that there are no kernels for."""
         config = json.loads(Path(path).read_text())
+        heads = config["num_attention_heads"]
         return cls(
             num_layers=config["num_hidden_layers"],
             hidden_size=config["hidden_size"],
-            num_heads=config["num_attention_heads"],
+            num_heads=heads,
             num_kv_heads=config["num_key_value_heads"],
             rope_theta=config["rope_theta"],
             rms_norm_eps=config["rms_norm_eps"],
+            attention_window=_checkpoint_window(config),
+            rotary_dim=_checkpoint_rotary_dim(config, config["hidden_size"] // heads),
+            rope_scaling=_checkpoint_scaling(config),
         )
 
     @property

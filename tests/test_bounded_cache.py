@@ -2,6 +2,7 @@
 allocator, rotary frequencies, the model's windows, and what the operators refuse."""
 
 import ctypes
+import json
 import math
 import random
 
@@ -318,6 +319,66 @@ def test_config_defaults_are_the_reference_model():
     assert not ModelConfig(**TINY, rope_interleaved=True).rotary_from_tables
     scaled = ModelConfig(**TINY, rope_scaling={"type": "linear", "factor": 2.0})
     assert not scaled.rotary_from_tables and isinstance(hash(scaled), int)
+
+
+CHECKPOINT = {"num_hidden_layers": 4, "hidden_size": 64, "num_attention_heads": 4,
+              "num_key_value_heads": 2, "rope_theta": 1e6, "rms_norm_eps": 1e-6,
+              "max_position_embeddings": 4096}
+YARN = {"type": "yarn", "factor": 4.0, "original_max_position_embeddings": 1024}
+
+
+@pytest.mark.parametrize("keys,fields", [
+    ({}, {}),
+    ({"sliding_window": 2048, "use_sliding_window": False, "max_window_layers": 2}, {}),
+    ({"sliding_window": None, "layer_types": ["full_attention"] * 4, "rope_scaling": None}, {}),
+    ({"sliding_window": 2048, "use_sliding_window": True, "max_window_layers": 4}, {}),
+    ({"sliding_window": 2048, "use_sliding_window": True, "max_window_layers": 0},
+     {"attention_window": 2048}),
+    ({"sliding_window": 2048}, {"attention_window": 2048}),
+    ({"sliding_window": 99, "layer_types": ["sliding_attention"] * 4}, {"attention_window": 99}),
+    ({"partial_rotary_factor": 0.5}, {"rotary_dim": 8}),
+    ({"rope_parameters": {"rope_type": "default", "rope_theta": 1e6,
+                          "partial_rotary_factor": 0.25}}, {"rotary_dim": 4}),
+    ({"rope_scaling": {"type": "linear", "factor": 2.0}},
+     {"rope_scaling": {"type": "linear", "factor": 2.0}}),
+    ({"rope_scaling": YARN},
+     {"rope_scaling": {"type": "yarn", "factor": 4.0, "original_max_position": 1024}}),
+    ({"rope_scaling": {"rope_type": "yarn", "factor": 4.0, "attention_factor": 1.0,
+                       "beta_fast": 16}},
+     {"rope_scaling": {"type": "yarn", "factor": 4.0, "attention_factor": 1.0, "beta_fast": 16,
+                       "original_max_position": 4096}}),
+    ({"rope_scaling": {"rope_type": "banded", "factor": 8.0, "low_freq_factor": 1.0,
+                       "high_freq_factor": 4.0, "original_max_position_embeddings": 512}},
+     {"rope_scaling": {"type": "banded", "factor": 8.0, "low_freq_factor": 1.0,
+                       "high_freq_factor": 4.0, "original_max_position": 512}}),
+])
+def test_checkpoints_reach_the_bounded_forms(tmp_path, keys, fields):
+    path = tmp_path / "config.json"
+    path.write_text(json.dumps(CHECKPOINT | keys))
+    config = ModelConfig.from_file(path)
+    plain = dict(num_layers=4, hidden_size=64, num_heads=4, num_kv_heads=2, rope_theta=1e6,
+                 rms_norm_eps=1e-6)
+    assert config == ModelConfig(**plain, **fields)
+    if config.rope_scaling:
+        ops.rope_frequencies(16, 1e6, config.rope_scaling, device="cpu")
+
+
+@pytest.mark.parametrize("keys", [
+    {"sliding_window": 2048, "use_sliding_window": True, "max_window_layers": 3},
+    {"sliding_window": 2048, "layer_types": ["sliding_attention", "full_attention"] * 2},
+    {"sliding_window": 2048, "layer_types": ["chunked_attention"] * 4},
+    {"layer_types": ["sliding_attention"] * 4}, {"partial_rotary_factor": 0.3},
+    {"partial_rotary_factor": 2.0}, {"rope_scaling": {"type": "dynamic", "factor": 2.0}},
+    {"rope_scaling": {"type": "default", "sections": [1, 2]}},
+    {"rope_scaling": dict(YARN, mscale=0.7)}, {"rope_scaling": dict(YARN, truncate=False)},
+    {"rope_scaling": YARN, "rope_parameters": {"rope_type": "default"}},
+    {"rope_parameters": {"rope_type": "default", "rope_theta": 5e5}},
+])
+def test_checkpoint_forms_without_a_kernel_are_refused(tmp_path, keys):
+    path = tmp_path / "config.json"
+    path.write_text(json.dumps(CHECKPOINT | keys))
+    with pytest.raises(ValueError):
+        ModelConfig.from_file(path)
 
 
 @pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (5, 2), (9, 30), (100, 3)])
