@@ -63,7 +63,8 @@ struct RotaryArgs {
 
 // Cos and sin of 2 pi turns for an fp64 turn count, |turns| <= 1/2.  fp32 outputs
 // take the fp64 functions (rounding the angle to fp32 alone would cost them 1.6
-// half steps); for bf16 outputs, 2^16 times coarser, the fp32 ones do.
+// half steps); for bf16 rows, 2^16 times coarser, the fp32 ones do (off by 2^-22 at most;
+// their k in a fp32 pool too: its digits beyond 2^-8 are not the model's).
 __device__ __forceinline__ float2 cos_sin(double turns, double amp, float) {
   double s, c;
   sincospi(2.0 * turns, &s, &c);

@@ -745,7 +745,12 @@ def window_attention_batched(query: torch.Tensor, key_pool: torch.Tensor, value_
     p = context_lens[b] - 1) sees key j only if j < sinks or j > p - window.
     Blocks outside are never read and may have been freed
     (``BlockAllocator.trim``).  A length of 0 marks a padding row, whose output
-    row is left as it was.  Scores stay in fp32.  ``out`` may be ``query`` itself.
+    row is left as it was.  ``out`` may be ``query`` itself.
+
+    Scores, maxima and sums stay in fp32.  In bf16 on the tensor cores (head_dim 64 or
+    128, blocks of a multiple of 16) each weight is rounded to bf16 before it multiplies
+    its value, by 2^-8 of itself at most; the sum that divides the output is of the
+    unrounded ones.  Elsewhere the weights are fp32.
     """
     return _native.window_attention_batched(query, key_pool, value_pool, block_tables,
                                             context_lens, scaling, window, sinks, seq_rows, out,
@@ -765,7 +770,8 @@ def window_prefill_attention(query: torch.Tensor, key_pool: torch.Tensor, value_
     sees are never read.  A context length of 0 marks a padding chunk; rows of
     ``out`` past the last chunk are left as they were.  A chunk longer than
     ``max_query_len`` or than its context, or outside the T rows, is reported
-    (``take_status``) and skipped.  ``out`` may be ``query`` itself.
+    (``take_status``) and skipped.  ``out`` may be ``query`` itself.  Precision as
+    ``window_attention_batched``.
     """
     return _native.window_prefill_attention(query, key_pool, value_pool, block_tables, cu_q,
                                             context_lens, scaling, max_query_len, window, sinks,
@@ -851,7 +857,9 @@ def rotary_append(qkv: torch.Tensor, frequencies: torch.Tensor, positions: torch
     2 * len(frequencies) dims of every q and k head turns by
     position * frequencies[i] (fp64, ``rope_frequencies``) and is multiplied by
     ``amplitude``; the other dims are copied.  Pairs are dims (i, i + half) or,
-    ``interleaved``, (2i, 2i + 1).  Computed in fp32 and rounded once.  A
+    ``interleaved``, (2i, 2i + 1).  Computed in fp32 and rounded once; cos and sin come
+    from the fp64 angle's rest below a half turn, for bf16 rows by the fp32 functions
+    (off by 2^-22 at most, where the rows themselves hold 2^-8; in a fp32 pool too).  A
     negative slot skips the row's K/V write; two rows must not share a slot.
     Returns q as [T, H, D].
     """
