@@ -109,13 +109,16 @@ constexpr int64_t kMaxSimtSplits = 64;
 constexpr int64_t kMinSimtKeys = 128;
 
 // Whether the ranges of a tile are a cluster whose CTAs join through distributed shared
-// memory, instead of leaving records for a second kernel: while all of them run at once
-// with some SMs to spare, for clusters to fit in.  Measured, clusters / records in us, fp32:
-// d64 (444 resident): 336 CTAs 14.6 / 20.9, 384: 15.6 / 20.5, 600 (a chunk): 106 / 86, 640:
-// 35.9 / 30.9; d128 (444): 448: 11.1 / 12.3, 576: 22.4 / 16.0; d256 (148): 112: 25.0 / 31.2,
-// 144: 41.6 / 33.4.
-bool simt_clusters_win(int64_t ctas, int64_t splits, int64_t resident) {
-  return splits > 1 && splits <= bsb::kMaxWindowCluster && ctas <= resident - resident / 8;
+// memory, instead of leaving records for a second kernel: while they take no more waves.
+// A cluster's CTAs start and end together, so fewer of them run at once (410 CTAs in
+// clusters of 5, 384 of 8, where 444 fit), and those without keys stay; records cost the
+// second kernel.  Measured, clusters / records in us, 444 at once; fp32, 7 heads of 64:
+// 384 CTAs (8 a cluster; 1 wave, 1) 16.0 / 24.1, 392 (2, 1) 28.1 / 24.1, 448 (2, 2) 29.5 /
+// 34.7, 410 (5; 1, 1) 16.2 / 20.5, 420 (2, 1) 26.7 / 20.5; 296 at once, 16 heads of 64:
+// 384 (8; 2, 2) 49.0 / 62.7, 560 (3, 2) 72.0 / 63.2, 390 (3, of which one without keys; 2,
+// 1) 49.8 / 33.1; heads of 128: 512 (2, 2) 67.5 / 93.9, 560 (3, 2) 97.3 / 95.5.
+bool simt_clusters_win(int64_t items, int64_t busy, int64_t clusters, int64_t resident) {
+  return clusters > 0 && (items + clusters - 1) / clusters <= (busy + resident - 1) / resident;
 }
 
 // How the CUDA-core kernel runs a call.
@@ -136,15 +139,25 @@ int plan_simt(const WindowShape& s, SimtPlan* p) {
   }
   const int64_t keys = std::min(s.max_blocks * s.block_size,
                                 std::min(s.window, kMaxContext) + std::min(s.sinks, kMaxContext) +
-                                    p->tile_tokens);
+                                    p->tile_tokens - 1);
   const int64_t want = p->items > 0 ? (4ll * sms + p->items - 1) / p->items : 1;
   p->splits = std::max<int64_t>(
       1, std::min(std::min(want, kMaxSimtSplits), (keys + kMinSimtKeys - 1) / kMinSimtKeys));
   if (p->items * p->splits > kInt32Max) p->splits = 1;
-  const int64_t resident =
-      sms * bsb::window_simt_ctas_per_sm(s.dtype == BS_BF16, p->tile_tokens * groups > 8,
-                                         static_cast<int>(s.head_dim));
-  p->clustered = simt_clusters_win(p->items * p->splits, p->splits, resident);
+  p->clustered = false;
+  if (p->splits > 1 && p->splits <= bsb::kMaxWindowCluster) {
+    const bool bf16 = s.dtype == BS_BF16, wide = p->tile_tokens * groups > 8;
+    const int head_dim = static_cast<int>(s.head_dim), cluster = static_cast<int>(p->splits);
+    const int ctas = bsb::window_simt_at_once(bf16, wide, head_dim, 1);
+    const int clusters = bsb::window_simt_at_once(bf16, wide, head_dim, cluster);
+    if (ctas <= 0 || clusters < 0) {
+      return fail(BS_ERR_CUDA, "occupancy query for window attention failed (%d, %d)", ctas,
+                  clusters);
+    }
+    const int64_t per = bsb::window_range(static_cast<int32_t>(keys), cluster);
+    const int64_t busy = p->items * ((keys + per - 1) / per);
+    p->clustered = simt_clusters_win(p->items, busy, clusters, static_cast<int64_t>(sms) * ctas);
+  }
   const int64_t gm = p->tile_tokens * groups <= 8 ? 8 : bsb::kWindowSimtRows;
   p->rec_stride = gm * s.head_dim + 2 * gm;
   p->bytes = p->splits > 1 && !p->clustered ? p->items * p->splits * p->rec_stride * 4 : 0;

@@ -123,8 +123,9 @@ constexpr int kMaxWindowRanges = 8;
 
 int launch_window_prefill(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& kmap,
                           const CUtensorMap& vmap, cudaStream_t stream);
-// CTAs of the CUDA-core kernel that an SM holds; wide: more than 8 query rows a tile.
-int window_simt_ctas_per_sm(bool bf16, bool wide, int head_dim);
+// What runs at once of the CUDA-core kernel: CTAs per SM (cluster 1), or clusters of so many
+// CTAs on the device (negative: a CUDA error); wide: more than 8 query rows a tile.
+int window_simt_at_once(bool bf16, bool wide, int head_dim, int cluster);
 int launch_window_simt(const WindowArgs& a, bool bf16, bool vec, cudaStream_t stream);
 
 }  // namespace bsb

@@ -22,6 +22,9 @@
 //
 // A weight of zero skips its V row, so NaN or infinities in a key that a row does
 // not see never reach that row.
+#include <mutex>
+#include <vector>
+
 #include "window.cuh"
 
 namespace bsb {
@@ -405,19 +408,24 @@ __global__ void __launch_bounds__(kThreads) window_simt_merge_kernel(const Windo
   }
 }
 
+// Shared memory for an instance's largest head_dim.
+template <typename T, int GM, int DPL, bool VEC, bool FULL>
+cudaError_t allow_smem() {
+  static unsigned long long configured = 0;  // one bit per device
+  return once_per_device(&configured, [] {
+    return cudaFuncSetAttribute(window_simt_kernel<T, GM, DPL, VEC, FULL>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                Layout<T, GM, DPL, VEC>::total(DPL * 32));
+  });
+}
+
 template <typename T, int GM, int DPL, bool VEC, bool FULL>
 int launch_one(const WindowArgs& a, cudaStream_t stream) {
   using L_ = Layout<T, GM, DPL, VEC>;
   const int smem = L_::total(a.head_dim);
   auto kernel = window_simt_kernel<T, GM, DPL, VEC, FULL>;
-  if (smem > 48 * 1024) {
-    static unsigned long long configured = 0;  // one bit per device
-    const cudaError_t e = once_per_device(&configured, [&] {
-      return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  L_::total(DPL * 32));
-    });
-    if (e != cudaSuccess) return static_cast<int>(e);
-  }
+  const cudaError_t e = allow_smem<T, GM, DPL, VEC, FULL>();
+  if (e != cudaSuccess) return static_cast<int>(e);
   const int64_t items = static_cast<int64_t>(a.num_rows) * a.qtiles * a.num_kv_heads;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -465,29 +473,69 @@ int launch_rows(const WindowArgs& a, bool vec, cudaStream_t stream) {
              : launch_dims<T, kWindowSimtRows, false>(a, stream);
 }
 
+// What the device runs at once of an instance: CTAs per SM (cluster 1), or clusters of
+// `cluster` CTAs on the whole device; or a CUDA error, negative.  Asked for once per
+// device and size.
+template <typename T, int GM, int DPL, bool VEC, bool FULL>
+int at_once(int D, int cluster) {
+  struct Known {
+    int device, D, cluster, count;
+  };
+  static std::mutex mutex;
+  static std::vector<Known> known;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return -static_cast<int>(e);
+  std::lock_guard<std::mutex> lock(mutex);
+  for (const Known& k : known) {
+    if (k.device == dev && k.D == D && k.cluster == cluster) return k.count;
+  }
+  using L_ = Layout<T, GM, DPL, VEC>;
+  auto kernel = window_simt_kernel<T, GM, DPL, VEC, FULL>;
+  e = allow_smem<T, GM, DPL, VEC, FULL>();
+  int count = 0;
+  if (e == cudaSuccess && cluster == 1) {
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&count, kernel, kThreads, L_::total(D));
+  } else if (e == cudaSuccess) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cluster);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = L_::total(D);
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&count, kernel, &cfg);
+  }
+  if (e != cudaSuccess) return -static_cast<int>(e);
+  known.push_back({dev, D, cluster, count});
+  return count;
+}
+
+// As the launch chooses, with aligned pools.
 template <typename T, int GM, int DPL>
-int smem_bytes(int D) {
-  return D * sizeof(T) % 16 == 0 ? Layout<T, GM, DPL, true>::total(D)
-                                 : Layout<T, GM, DPL, false>::total(D);
+int at_once_full(int D, int cluster) {
+  if (D * sizeof(T) % 16 != 0) return at_once<T, GM, DPL, false, false>(D, cluster);
+  return D == 32 * DPL ? at_once<T, GM, DPL, true, true>(D, cluster)
+                       : at_once<T, GM, DPL, true, false>(D, cluster);
 }
 
 template <typename T, int GM>
-int smem_bytes(int D) {
-  return D <= 32 ? smem_bytes<T, GM, 1>(D)
-         : D <= 64 ? smem_bytes<T, GM, 2>(D)
-         : D <= 128 ? smem_bytes<T, GM, 4>(D) : smem_bytes<T, GM, 8>(D);
+int at_once_dims(int D, int cluster) {
+  return D <= 32 ? at_once_full<T, GM, 1>(D, cluster)
+         : D <= 64 ? at_once_full<T, GM, 2>(D, cluster)
+         : D <= 128 ? at_once_full<T, GM, 4>(D, cluster) : at_once_full<T, GM, 8>(D, cluster);
 }
 
 }  // namespace
 
-int window_simt_ctas_per_sm(bool bf16, bool wide, int head_dim) {
-  constexpr int kSmem = 228 * 1024, kReserved = 1024, kByRegisters = 4;
-  const int bytes = bf16 ? (wide ? smem_bytes<__nv_bfloat16, kWindowSimtRows>(head_dim)
-                                 : smem_bytes<__nv_bfloat16, 8>(head_dim))
-                         : (wide ? smem_bytes<float, kWindowSimtRows>(head_dim)
-                                 : smem_bytes<float, 8>(head_dim));
-  const int by_smem = kSmem / (bytes + kReserved);
-  return by_smem < kByRegisters ? by_smem : kByRegisters;
+int window_simt_at_once(bool bf16, bool wide, int head_dim, int cluster) {
+  return bf16 ? (wide ? at_once_dims<__nv_bfloat16, kWindowSimtRows>(head_dim, cluster)
+                      : at_once_dims<__nv_bfloat16, 8>(head_dim, cluster))
+              : (wide ? at_once_dims<float, kWindowSimtRows>(head_dim, cluster)
+                      : at_once_dims<float, 8>(head_dim, cluster));
 }
 
 int launch_window_simt(const WindowArgs& a, bool bf16, bool vec, cudaStream_t stream) {

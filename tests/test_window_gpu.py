@@ -16,6 +16,7 @@ terms cancelled), n visible keys and u = 2^-24:
   * fp32: the division and the output's rounding, 2 u of the value.
 """
 
+import ctypes
 import math
 import subprocess
 import sys
@@ -24,7 +25,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from batchstream_inference_engine_b200 import ops
+from batchstream_inference_engine_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -795,3 +796,29 @@ def test_parts_without_a_finite_score_are_joined(length, new, heads, kv_heads, w
         if len(sees) < min(p + 1, window):  # another key is left
             # Weights of 0 either way.
             assert got[-1e30][t].isfinite().all() and torch.equal(got[-math.inf][t], got[-1e30][t]), t
+
+
+@pytest.mark.parametrize("dtype,heads,head_dim,block,window,clustered,records", [
+    # 444 CTAs run at once, or 48 clusters of 8, or 103 of 4.
+    (torch.bfloat16, 16, 64, 8, 1000, (48, 60), (52,)),
+    (torch.float32, 7, 48, 16, 1000, (48, 60), (52,)),
+    (torch.float32, 7, 48, 16, 500, (96, 115), (108,))])
+def test_clusters_while_they_take_no_more_waves(dtype, heads, head_dim, block, window, clustered,
+                                                records):
+    # Records need scratch, clusters do not.
+    def scratch(rows):
+        got = ctypes.c_uint64(0)
+        _lib.check(_lib.lib().bs_window_attention_batched_workspace_bytes(
+            rows, heads, 1, head_dim, block, 4096 // block, ops.dtype_code(dtype), window, 0,
+            ctypes.byref(got)))
+        return got.value
+
+    if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+        assert [scratch(n) for n in clustered] == [0] * len(clustered)
+        assert all(scratch(n) > 0 for n in records)
+    for rows in (*clustered, *records):
+        c = Paged([2 * window] * rows, [1] * rows, heads, 1, head_dim, block, dtype, window, 0,
+                  seed=rows)
+        out = c.decode()
+        assert ops.take_status() == 0
+        c.check(out)
