@@ -186,14 +186,19 @@ class BlockAllocator:
         self._kept[seq_id], self._trimmed[seq_id] = low, max(high, end)
         return freed
 
+    def moves(self) -> list[tuple[int, int]]:
+        """The (source, destination) copies that ``compact`` would return."""
+        used = sorted({b for table in self._tables.values() for b in table} - {EMPTY_BLOCK})
+        count = len(used)
+        return list(zip((b for b in used if b >= count),
+                        sorted(b for b in self._free if b < count)))
+
     def compact(self) -> list[tuple[int, int]]:
         """Renumbers the blocks in use to ids below their count: each block above
         takes the place of a free one below, the lowest first.  Returns the
         (source, destination) copies; no block is both."""
-        used = sorted({b for table in self._tables.values() for b in table} - {EMPTY_BLOCK})
-        count = len(used)
-        sources = [b for b in used if b >= count]
-        moved = dict(zip(sources, sorted(b for b in self._free if b < count)))
+        moved = dict(self.moves())
+        count = self.num_blocks - len(self._free)
         for seq_id, table in self._tables.items():
             if any(b in moved for b in table):
                 self._tables[seq_id][:] = [moved.get(b, b) for b in table]

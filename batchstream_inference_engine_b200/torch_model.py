@@ -283,7 +283,12 @@ class PagedKVPool:
     def fork(self, cache: "PagedKVCache", seq_id: int) -> "PagedKVCache":
         """A new sequence that starts with the tokens cached for `cache`: whole
         blocks are shared, a last partial one is copied (all layers, one launch)."""
-        self._copy(self.allocator.fork(cache.seq_id, seq_id, cache.length))
+        pairs = self.allocator.fork(cache.seq_id, seq_id, cache.length)
+        try:
+            self._copy(pairs)
+        except BaseException:  # nothing was copied: there is no child
+            self.allocator.free(seq_id)
+            raise
         child = self.new_cache(seq_id)
         child.length = cache.length
         return child
@@ -296,9 +301,8 @@ class PagedKVPool:
     def compact(self) -> int:
         """Moves the blocks in use to the lowest ids (all layers, one launch);
         returns how many moved."""
-        pairs = self.allocator.compact()
-        self._copy(pairs)
-        return len(pairs)
+        self._copy(self.allocator.moves())  # (raises before any block has a new id)
+        return len(self.allocator.compact())
 
     def _copy(self, pairs: list[tuple[int, int]]) -> None:
         if pairs:

@@ -535,6 +535,28 @@ def test_fork_of_a_sequence_that_ended_with_a_step_in_flight(monkeypatch):
         backend.fork_sequence(s, [])
 
 
+def test_forks_and_compactions_that_cannot_copy_change_nothing():
+    # A pool without a GPU has no kernel for its copies.
+    config = ModelConfig(**TINY)
+    model = TorchModel(config, random_weights(config, vocab_size=50, intermediate_size=16),
+                       device="cpu", dtype=torch.float32, max_position=64)
+    backend = PagedBackend(model, num_blocks=16, block_size=4, prefill_chunk=8, max_seqs=4)
+    pool = backend.pool
+    cache = pool.new_cache(100)
+    cache.reserve(6)
+    cache.advance(6)
+    alloc = pool.allocator
+    before = (dict(alloc._tables), sorted(alloc._free), list(alloc._free_rows), dict(alloc._refs))
+    with pytest.raises(RuntimeError):
+        pool.fork(cache, 101)
+    table = list(pool.block_table(100))
+    assert alloc.moves() and min(table) > 2
+    with pytest.raises(RuntimeError):
+        pool.compact()
+    after = (dict(alloc._tables), sorted(alloc._free), list(alloc._free_rows), dict(alloc._refs))
+    assert after == before and pool.block_table(100) == table
+
+
 # ------------------------------------------------------------------ refusals of the C ABI
 
 
