@@ -26,12 +26,13 @@
 // is 16 tokens of the sequence's visible range (its sink units, then the window's),
 // masked by a 16-bit map, the block size any multiple of 16, and the scores are not
 // rounded to bf16 (the reference's rounding points belong to the full form only).
-// 256 sequences, 28 + 4 heads, d128, window 4096 (1.5 GB of keys and values): 228 to
-// 244 us, 94 to 100% of the measured copy rate; the CUDA-core kernel takes 3538.  64
-// sequences, d64, window 1024 (10 MB): 12.7 us, where launch, table, loads, 6 units a
+// 256 sequences, 28 + 4 heads, d128, window 4096 (1.5 GB of keys and values): 240 to
+// 250 us, 92 to 96% of the measured copy rate (228 us in a chain of calls over the same
+// data); the CUDA-core kernel takes 3538.  64
+// sequences, d64, window 1024 (10 MB): 13.3 us, where launch, table, loads, 6 units a
 // warp and the cluster's exchange follow one another.  Few segments are shared by
 // clusters of CTAs that join through distributed shared memory (join_segment): one
-// sequence of 77 tokens 5.1 us, by spans and their merge 10.1.  (A join whose reads
+// sequence of 77 tokens 5.4 us, by spans and their merge 10.1.  (A join whose reads
 // waited for one another, behind a chain of the warps' parts: 7.2 and 14.3.)
 #include "decode.cuh"
 

@@ -16,11 +16,11 @@
 // in shared memory, for all its heads.
 //
 // Bound by memory, and for few tokens by the launch: 4096 tokens of 28 + 2 * 4 heads of
-// 128 (75.5 MB read and written, 64 rotary dims) take 12.4 us with the rows in L2 and
-// 14.8 without, one token 1.9 us in a graph.  All 64-bit functions instead of fp32 ones
+// 128 (75.5 MB read and written, 64 rotary dims) take 13.1 us with the rows in L2 and
+// 16.9 without, one token 2.3 us in a graph.  All 64-bit functions instead of fp32 ones
 // for bf16 outputs, one element a thread: 51 us.  Loading four units a thread before
-// storing any (16.8 us) or the row ahead of the positions (13.0) was slower: the CTAs
-// of an SM hide each other's latency already.
+// storing any (16.8 us, where one takes 12.4) or the row ahead of the positions (13.0) was
+// slower with the rows in L2: the CTAs of an SM hide each other's latency already.
 #include "common.cuh"
 
 namespace bsb {

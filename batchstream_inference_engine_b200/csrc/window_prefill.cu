@@ -35,9 +35,10 @@
 // steps.  Two tiles in one CTA over the same keys read half as much from L2, but start
 // and end together: 8 chunks of 512, d64, 14 heads, window 1024: 45.7 us so, 36.9 with
 // a tile each; 6 ragged chunks of 100 to 2048, d128, 28 heads, window 4096: 268 and
-// 243 us (990 TFLOP/s, 59% of what a plain matrix product reaches; two stages are
-// all that fits, and a third is worth 1%).  Over
-// 150 shapes the geometric mean fell by 8% (d64) and 11% (d128), the worst lost 10%.
+// 243 us.  As it is: 37.1 us, and 237 us with the keys in L2 (1015 TFLOP/s, 61% of what a
+// plain matrix product reaches), 279 without (52%).  Two stages of d128 are all that fits;
+// a third is worth 1%.  The d64 case has 464 tiles for 296 places: SMs are busy for 83% of
+// its time.
 // Tried and slower: exponentials by the maximum of the steps before, checked afterwards
 // (more registers for a wait that the other CTA hides: 39.3 against 39.9 us, 254 and 257,
 // and slower for long chunks); two threads a row, 32 keys each, that swap their maxima

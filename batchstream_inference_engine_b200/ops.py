@@ -789,7 +789,8 @@ def rope_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None,
     * "linear": f_i / factor (positions interpolated);
     * "ntk": theta grows by factor^(d / (d - 2)), so the slowest pair turns factor
       times slower and the fastest as before;
-    * "yarn": f_i where pair i turns more than ``beta_fast`` (32) times within
+    * "yarn" (Peng et al., "YaRN: Efficient Context Window Extension of Large Language
+      Models", 2023): f_i where pair i turns more than ``beta_fast`` (32) times within
       ``original_max_position``, f_i / factor below ``beta_slow`` (1) turns, and a
       linear ramp over the pairs between; amplitude 0.1 ln(factor) + 1, or
       ``attention_factor``;
