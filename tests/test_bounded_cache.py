@@ -335,6 +335,8 @@ YARN = {"type": "yarn", "factor": 4.0, "original_max_position_embeddings": 1024}
     ({"sliding_window": 2048, "use_sliding_window": True, "max_window_layers": 0},
      {"attention_window": 2048}),
     ({"sliding_window": 2048}, {"attention_window": 2048}),
+    ({"sliding_window": 2048, "use_sliding_window": True, "max_window_layers": None},
+     {"attention_window": 2048}),
     ({"sliding_window": 99, "layer_types": ["sliding_attention"] * 4}, {"attention_window": 99}),
     ({"partial_rotary_factor": 0.5}, {"rotary_dim": 8}),
     ({"rope_parameters": {"rope_type": "default", "rope_theta": 1e6,
