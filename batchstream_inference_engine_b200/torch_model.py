@@ -57,7 +57,7 @@ def _checkpoint_window(config: dict) -> int:
     elif not window or not config.get("use_sliding_window", True):
         windowed = 0
     elif "use_sliding_window" in config:  # from the layer max_window_layers on
-        windowed = max(0, layers - config.get("max_window_layers") or 0)
+        windowed = max(0, layers - (config.get("max_window_layers") or 0))
     else:
         windowed = layers
     if windowed not in (0, layers):
