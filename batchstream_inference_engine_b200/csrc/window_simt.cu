@@ -17,8 +17,8 @@
 // 33).  24 fp32 sequences of up to 4096 tokens, d64, window 777: 12.1 us, a chain of
 // table entry, rows, scores, V and join with too few keys to hide it (one warp lane
 // loading its own key row instead: 68 us).  The ranges of a tile are a cluster that
-// joins through distributed shared memory while all CTAs run at once; more leave records
-// for a second kernel, which costs some 4 us.  Rows that are not whole 16-byte pieces are read one element at a time.
+// joins through distributed shared memory while clusters take no more waves than single
+// CTAs would; else they leave records for a second kernel, which costs some 4 us.  Rows that are not whole 16-byte pieces are read one element at a time.
 //
 // A weight of zero skips its V row, so NaN or infinities in a key that a row does
 // not see never reach that row.
