@@ -43,6 +43,14 @@ EXPORTS = (
     "bs_window_prefill_attention_workspace_bytes",
     "bs_rotary_append",
     "bs_copy_blocks",
+    "bs_rotary_append_int4",
+    "bs_read_int4",
+    "bs_int4_attention_batched",
+    "bs_int4_attention_batched_workspace_bytes",
+    "bs_int4_prefill_attention",
+    "bs_int4_prefill_attention_workspace_bytes",
+    "bs_verify_drafts",
+    "bs_verify_drafts_workspace_bytes",
 )
 
 _i32, _i64, _u64, _p, _dbl = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_double
@@ -142,7 +150,24 @@ _SIGNATURES = {
     "bs_copy_blocks": (
         [_p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _p, _p], ctypes.c_int,
     ),
+    "bs_rotary_append_int4": (
+        [_p, _i64, _i32, _p, _i64, _i32, _dbl, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _i64,
+         _i64, _p, _p],
+        ctypes.c_int,
+    ),
+    "bs_read_int4": (
+        [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p], ctypes.c_int,
+    ),
+    "bs_verify_drafts": (
+        [_p, _i64, _i32, _i64, _i64, _p, _p, _i64, _p, _p, _dbl, _p, _i64, _i32, _p, _p, _p, _u64,
+         _p, _p],
+        ctypes.c_int,
+    ),
+    "bs_verify_drafts_workspace_bytes": ([_i64, _i64, _i32, ctypes.POINTER(_u64)], ctypes.c_int),
 }
+for _name in ("attention_batched", "attention_batched_workspace_bytes", "prefill_attention",
+              "prefill_attention_workspace_bytes"):
+    _SIGNATURES["bs_int4_" + _name] = _SIGNATURES["bs_window_" + _name]
 
 _lib: ctypes.CDLL | None = None
 

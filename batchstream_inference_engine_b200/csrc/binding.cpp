@@ -1,4 +1,5 @@
-// Python entry points of the bounded-cache operators (module _native).
+// Python entry points of the bounded-cache and 4-bit operators and of draft verification
+// (module _native).
 //
 // The calls last a few microseconds on the device, and a ctypes call with its checks
 // in Python takes 15 to 20 on the host: here the checks, the output and scratch
@@ -180,7 +181,21 @@ void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // ------------------------------------------------------------------ window attention
 
-// What both window attentions take: [T, H, D] queries over paged pools.
+// Bytes of a token and kv head in a 4-bit pool, and head_dim from them.
+int64_t int4_row(int64_t head_dim) { return head_dim / 2 + head_dim / 16; }
+
+int64_t int4_head_dim(const char* name, const Tensor& key_pool, const Tensor& value_pool) {
+  require(key_pool.dim() == 4 && value_pool.sizes() == key_pool.sizes() &&
+              key_pool.scalar_type() == at::kByte && value_pool.scalar_type() == at::kByte,
+          name, "4-bit pools must be uint8 [Hkv, NB, bs, 9 * D / 16] of one shape");
+  require(key_pool.size(3) > 0 && key_pool.size(3) % 18 == 0, name,
+          "4-bit pools must be uint8 [Hkv, NB, bs, 9 * D / 16], D a multiple of 32");
+  require(key_pool.is_contiguous() && value_pool.is_contiguous(), name, "pools must be contiguous");
+  return key_pool.size(3) / 9 * 16;
+}
+
+// What the window attentions and those over 4-bit pools take: [T, H, D] queries over paged
+// pools.
 struct WindowInputs {
   Tensor query, tables, out;
   bool own_out = false;  // allocated here
@@ -193,14 +208,21 @@ int64_t token_stride(const Tensor& t) { return std::max(t.stride(0), t.size(1) *
 
 WindowInputs window_inputs(const char* name, const Tensor& query, const Tensor& key_pool,
                            const Tensor& value_pool, const Tensor& block_tables,
-                           const std::optional<Tensor>& out, PyObject* max_blocks) {
-  require(query.dim() == 3 && key_pool.dim() == 4 && value_pool.sizes() == key_pool.sizes(), name,
-          "query must be [T, H, D] and the pools [Hkv, NB, bs, D]");
-  require(query.scalar_type() == key_pool.scalar_type() &&
-              value_pool.scalar_type() == key_pool.scalar_type(),
-          name, "query and pools must share a dtype");
-  require(key_pool.is_contiguous() && value_pool.is_contiguous(), name, "pools must be contiguous");
-  require(query.size(2) == key_pool.size(3), name, "query and pools disagree on head_dim");
+                           const std::optional<Tensor>& out, PyObject* max_blocks, bool int4) {
+  if (int4) {
+    const int64_t head_dim = int4_head_dim(name, key_pool, value_pool);
+    require(query.dim() == 3, name, "query must be [T, H, D]");
+    require(query.size(2) == head_dim, name, "query and pools disagree on head_dim");
+  } else {
+    require(query.dim() == 3 && key_pool.dim() == 4 && value_pool.sizes() == key_pool.sizes(), name,
+            "query must be [T, H, D] and the pools [Hkv, NB, bs, D]");
+    require(query.scalar_type() == key_pool.scalar_type() &&
+                value_pool.scalar_type() == key_pool.scalar_type(),
+            name, "query and pools must share a dtype");
+    require(key_pool.is_contiguous() && value_pool.is_contiguous(), name,
+            "pools must be contiguous");
+    require(query.size(2) == key_pool.size(3), name, "query and pools disagree on head_dim");
+  }
   require(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2, name,
           "block_tables must be int32 [rows, max_blocks]");
   WindowInputs w;
@@ -245,8 +267,12 @@ PyObject* result(const WindowInputs& w, PyObject* out) {
 
 // (query, key_pool, value_pool, block_tables, context_lens, scaling, window, sinks,
 //  seq_rows, out, max_blocks_per_seq)
-PyObject* window_attention_batched(PyObject* const* a) {
-  const char* name = "window_attention_batched";
+template <bool Int4>
+PyObject* attention_batched(PyObject* const* a) {
+  const char* name = Int4 ? "int4_attention_batched" : "window_attention_batched";
+  const auto workspace_bytes = Int4 ? &bs_int4_attention_batched_workspace_bytes
+                                    : &bs_window_attention_batched_workspace_bytes;
+  const auto attend = Int4 ? &bs_int4_attention_batched : &bs_window_attention_batched;
   const Tensor& query = tensor_of(a[0], name, "query");
   const Tensor& key_pool = tensor_of(a[1], name, "key_pool");
   const Tensor& value_pool = tensor_of(a[2], name, "value_pool");
@@ -258,15 +284,15 @@ PyObject* window_attention_batched(PyObject* const* a) {
   const std::optional<Tensor> out = optional_tensor(a[9], name, "out");
   const c10::Device device = cuda_device(name, {&query, &key_pool, &value_pool, &block_tables,
                                                 &context_lens, pointer(seq_rows), pointer(out)});
-  const WindowInputs w = window_inputs(name, query, key_pool, value_pool, block_tables, out, a[10]);
+  const WindowInputs w = window_inputs(name, query, key_pool, value_pool, block_tables, out, a[10],
+                                       Int4);
   const Tensor lens = int32_list(name, "context_lens", context_lens, w.T);
   const Tensor rows = seq_rows ? int32_list(name, "seq_rows", *seq_rows, w.T) : Tensor();
   const Launch launch(device);
   uint64_t need = 0;
-  check(bs_window_attention_batched_workspace_bytes(w.T, w.H, w.Hkv, w.D, w.bs, w.mb, w.code,
-                                                    window, sinks, &need));
+  check(workspace_bytes(w.T, w.H, w.Hkv, w.D, w.bs, w.mb, w.code, window, sinks, &need));
   const Tensor ws = scratch(need, device);
-  check(bs_window_attention_batched(
+  check(attend(
       w.query.data_ptr(), token_stride(w.query), key_pool.data_ptr(), value_pool.data_ptr(),
       static_cast<const int32_t*>(w.tables.data_ptr()), table_stride(w.tables), w.tables.size(0),
       static_cast<const int32_t*>(address(rows)), static_cast<const int32_t*>(lens.data_ptr()), w.T,
@@ -277,8 +303,12 @@ PyObject* window_attention_batched(PyObject* const* a) {
 
 // (query, key_pool, value_pool, block_tables, cu_q, context_lens, scaling,
 //  max_query_len, window, sinks, seq_rows, out, max_blocks_per_seq)
-PyObject* window_prefill_attention(PyObject* const* a) {
-  const char* name = "window_prefill_attention";
+template <bool Int4>
+PyObject* prefill_attention(PyObject* const* a) {
+  const char* name = Int4 ? "int4_prefill_attention" : "window_prefill_attention";
+  const auto workspace_bytes = Int4 ? &bs_int4_prefill_attention_workspace_bytes
+                                    : &bs_window_prefill_attention_workspace_bytes;
+  const auto attend = Int4 ? &bs_int4_prefill_attention : &bs_window_prefill_attention;
   const Tensor& query = tensor_of(a[0], name, "query");
   const Tensor& key_pool = tensor_of(a[1], name, "key_pool");
   const Tensor& value_pool = tensor_of(a[2], name, "value_pool");
@@ -292,17 +322,18 @@ PyObject* window_prefill_attention(PyObject* const* a) {
   const c10::Device device =
       cuda_device(name, {&query, &key_pool, &value_pool, &block_tables, &cu_q, &context_lens,
                          pointer(seq_rows), pointer(out)});
-  const WindowInputs w = window_inputs(name, query, key_pool, value_pool, block_tables, out, a[12]);
+  const WindowInputs w = window_inputs(name, query, key_pool, value_pool, block_tables, out, a[12],
+                                       Int4);
   const Tensor lens = int32_list(name, "context_lens", context_lens, 0);
   const int64_t R = lens.numel();
   const Tensor cu = int32_list(name, "cu_q", cu_q, R + 1);
   const Tensor rows = seq_rows ? int32_list(name, "seq_rows", *seq_rows, R) : Tensor();
   const Launch launch(device);
   uint64_t need = 0;
-  check(bs_window_prefill_attention_workspace_bytes(w.T, R, max_query_len, w.H, w.Hkv, w.D, w.bs,
-                                                    w.mb, w.code, window, sinks, &need));
+  check(workspace_bytes(w.T, R, max_query_len, w.H, w.Hkv, w.D, w.bs, w.mb, w.code, window, sinks,
+                        &need));
   const Tensor ws = scratch(need, device);
-  check(bs_window_prefill_attention(
+  check(attend(
       w.query.data_ptr(), token_stride(w.query), static_cast<const int32_t*>(cu.data_ptr()), R, w.T,
       max_query_len, static_cast<const int32_t*>(lens.data_ptr()),
       static_cast<const int32_t*>(address(rows)), key_pool.data_ptr(), value_pool.data_ptr(),
@@ -313,6 +344,16 @@ PyObject* window_prefill_attention(PyObject* const* a) {
 }
 
 // ------------------------------------------------------------------ rotary, copies
+
+PyObject* pair(const Tensor& x, const Tensor& y) {
+  PyObject* first = THPVariable_Wrap(x);
+  PyObject* second = first != nullptr ? THPVariable_Wrap(y) : nullptr;
+  PyObject* both = second != nullptr ? PyTuple_Pack(2, first, second) : nullptr;
+  Py_XDECREF(first);
+  Py_XDECREF(second);
+  if (both == nullptr) throw PythonError();
+  return both;
+}
 
 // Whether two tensors' memory overlaps (both with non-negative strides).
 bool overlap(const Tensor& a, const Tensor& b) {
@@ -329,8 +370,9 @@ bool overlap(const Tensor& a, const Tensor& b) {
 
 // (qkv, frequencies, positions, slot_mapping, key_pool, value_pool, num_heads,
 //  interleaved, amplitude, query_out)
-PyObject* rotary_append(PyObject* const* a) {
-  const char* name = "rotary_append";
+template <bool Int4>
+PyObject* append(PyObject* const* a) {
+  const char* name = Int4 ? "rotary_append_int4" : "rotary_append";
   const Tensor& qkv = tensor_of(a[0], name, "qkv");
   const Tensor& frequencies = tensor_of(a[1], name, "frequencies");
   const Tensor& positions = tensor_of(a[2], name, "positions");
@@ -343,11 +385,18 @@ PyObject* rotary_append(PyObject* const* a) {
   const std::optional<Tensor> query_out = optional_tensor(a[9], name, "query_out");
   const c10::Device device = cuda_device(name, {&qkv, &frequencies, &positions, &slot_mapping,
                                                 &key_pool, &value_pool, pointer(query_out)});
-  require(key_pool.dim() == 4 && value_pool.sizes() == key_pool.sizes() &&
-              value_pool.scalar_type() == key_pool.scalar_type(),
-          name, "the pools must be [Hkv, NB, bs, D] of one shape and dtype");
-  require(key_pool.is_contiguous() && value_pool.is_contiguous(), name, "pools must be contiguous");
-  const int64_t Hkv = key_pool.size(0), D = key_pool.size(3), T = positions.numel();
+  int64_t D;
+  if (Int4) {
+    D = int4_head_dim(name, key_pool, value_pool);
+  } else {
+    require(key_pool.dim() == 4 && value_pool.sizes() == key_pool.sizes() &&
+                value_pool.scalar_type() == key_pool.scalar_type(),
+            name, "the pools must be [Hkv, NB, bs, D] of one shape and dtype");
+    require(key_pool.is_contiguous() && value_pool.is_contiguous(), name,
+            "pools must be contiguous");
+    D = key_pool.size(3);
+  }
+  const int64_t Hkv = key_pool.size(0), T = positions.numel();
   const Tensor pos = int32_list(name, "positions", positions, T);
   const Tensor slots = int32_list(name, "slot_mapping", slot_mapping, T);
   require(frequencies.scalar_type() == at::kDouble && frequencies.dim() == 1, name,
@@ -368,10 +417,27 @@ PyObject* rotary_append(PyObject* const* a) {
     require(!overlap(*query_out, qkv), name, "query_out must not overlap qkv");
     q_out = *query_out;
   } else {
-    require(H > 0, name, "num_heads must be positive");
+    require(Int4 ? H >= 0 : H > 0, name,
+            Int4 ? "num_heads must not be negative" : "num_heads must be positive");
     q_out = at::empty({T, H, D}, qkv.options());
   }
   const Launch launch(device);
+  if (Int4) {
+    for (const Tensor* pool : {&key_pool, &value_pool}) {
+      require(!overlap(*pool, rows) && !overlap(*pool, q_out), name,
+              "the pools must not overlap qkv or query_out");
+    }
+    check(bs_rotary_append_int4(
+        rows.data_ptr(), std::max(rows.stride(0), width), dtype_code(qkv.scalar_type()),
+        static_cast<const double*>(freq.data_ptr()), 2 * freq.numel(), interleaved ? 1 : 0,
+        amplitude, static_cast<const int32_t*>(pos.data_ptr()),
+        static_cast<const int32_t*>(slots.data_ptr()), T, H, Hkv, D, q_out.data_ptr(),
+        key_pool.data_ptr(), value_pool.data_ptr(), key_pool.size(1), key_pool.size(2),
+        launch.status, launch.stream));
+    if (!query_out) return THPVariable_Wrap(q_out);
+    Py_INCREF(a[9]);
+    return a[9];
+  }
   check(bs_rotary_append(rows.data_ptr(), std::max(rows.stride(0), width),
                          dtype_code(qkv.scalar_type()),
                          static_cast<const double*>(freq.data_ptr()), 2 * freq.numel(),
@@ -386,7 +452,27 @@ PyObject* rotary_append(PyObject* const* a) {
   return a[9];
 }
 
-// (key_pool, value_pool, src, dst)
+// (key_pool, value_pool, slot_mapping)
+PyObject* read_int4(PyObject* const* a) {
+  const char* name = "read_int4";
+  const Tensor& key_pool = tensor_of(a[0], name, "key_pool");
+  const Tensor& value_pool = tensor_of(a[1], name, "value_pool");
+  const Tensor& slot_mapping = tensor_of(a[2], name, "slot_mapping");
+  const c10::Device device = cuda_device(name, {&key_pool, &value_pool, &slot_mapping});
+  const int64_t D = int4_head_dim(name, key_pool, value_pool), Hkv = key_pool.size(0);
+  const int64_t T = slot_mapping.numel();
+  const Tensor slots = int32_list(name, "slot_mapping", slot_mapping, T);
+  const Launch launch(device);
+  const auto options = at::TensorOptions(at::kBFloat16).device(device);
+  const Tensor k = at::empty({T, Hkv, D}, options), v = at::empty({T, Hkv, D}, options);
+  check(bs_read_int4(key_pool.data_ptr(), value_pool.data_ptr(),
+                     static_cast<const int32_t*>(slots.data_ptr()), T, Hkv, key_pool.size(1),
+                     key_pool.size(2), D, k.data_ptr(), v.data_ptr(), launch.status,
+                     launch.stream));
+  return pair(k, v);
+}
+
+// (key_pool, value_pool, src, dst).  4-bit pools are copied as pairs of bytes.
 PyObject* copy_blocks(PyObject* const* a) {
   const char* name = "copy_blocks";
   const Tensor& key_pool = tensor_of(a[0], name, "key_pool");
@@ -402,14 +488,78 @@ PyObject* copy_blocks(PyObject* const* a) {
   require(src.numel() == dst.numel(), name, "src and dst must have one entry per pair");
   const int64_t n = src.numel();
   const Tensor from = int32_list(name, "src", src, n), to = int32_list(name, "dst", dst, n);
+  const bool int4 = key_pool.scalar_type() == at::kByte;
+  require(!int4 || key_pool.size(dims - 1) % 18 == 0, name,
+          "4-bit pools must be uint8 [L, Hkv, NB, bs, 9 * D / 16], D a multiple of 32");
   const Launch launch(device);
   check(bs_copy_blocks(key_pool.data_ptr(), value_pool.data_ptr(),
-                       dtype_code(key_pool.scalar_type()), dims == 5 ? key_pool.size(0) : 1,
+                       int4 ? BS_BF16 : dtype_code(key_pool.scalar_type()),
+                       dims == 5 ? key_pool.size(0) : 1,
                        key_pool.size(dims - 4), key_pool.size(dims - 3), key_pool.size(dims - 2),
-                       key_pool.size(dims - 1), static_cast<const int32_t*>(from.data_ptr()),
+                       key_pool.size(dims - 1) / (int4 ? 2 : 1), static_cast<const int32_t*>(from.data_ptr()),
                        static_cast<const int32_t*>(to.data_ptr()), n, launch.status,
                        launch.stream));
   Py_RETURN_NONE;
+}
+
+// ------------------------------------------------------------------ drafts
+
+// (logits, draft_tokens, cu_rows, uniforms, temperature, draft_probs)
+PyObject* verify_drafts(PyObject* const* a) {
+  const char* name = "verify_drafts";
+  const Tensor& logits = tensor_of(a[0], name, "logits");
+  const Tensor& draft_tokens = tensor_of(a[1], name, "draft_tokens");
+  const Tensor& cu_rows = tensor_of(a[2], name, "cu_rows");
+  const Tensor& uniforms = tensor_of(a[3], name, "uniforms");
+  std::optional<Tensor> temperatures;
+  double temperature = 0.0;
+  if (THPVariable_Check(a[4])) {
+    temperatures = tensor_of(a[4], name, "temperature");
+  } else {
+    temperature = float_of(a[4]);
+  }
+  const std::optional<Tensor> draft_probs = optional_tensor(a[5], name, "draft_probs");
+  const c10::Device device = cuda_device(name, {&logits, &draft_tokens, &cu_rows, &uniforms,
+                                                pointer(temperatures), pointer(draft_probs)});
+  require(logits.dim() == 2, name, "logits must be [rows, vocab]");
+  const int64_t N = logits.size(0), V = logits.size(1);
+  auto rows_of = [&](const Tensor& t) {
+    return t.stride(1) == 1 && (N <= 1 || t.stride(0) >= V) ? t : t.contiguous();
+  };
+  auto floats = [&](const char* arg, const Tensor& t, int64_t count) {
+    if (t.scalar_type() != at::kFloat || t.dim() != 1 || t.numel() < count) {
+      refuse(string(name) + ": " + arg + " must be one-dimensional float32 with at least " +
+             std::to_string(count) + " entries");
+    }
+    return t.contiguous();
+  };
+  const Tensor l = rows_of(logits);
+  const Tensor tokens = int32_list(name, "draft_tokens", draft_tokens, N);
+  const Tensor cu = int32_list(name, "cu_rows", cu_rows, 1);
+  const int64_t B = cu.numel() - 1;
+  const Tensor u = floats("uniforms", uniforms, N);
+  const Tensor temps = temperatures ? floats("temperature", *temperatures, B) : Tensor();
+  Tensor probs;
+  if (draft_probs) {
+    require(draft_probs->dim() == 2 && draft_probs->sizes() == logits.sizes(), name,
+            "draft_probs must be [rows, vocab] like the logits");
+    probs = rows_of(*draft_probs);
+  }
+  const Launch launch(device);
+  uint64_t need = 0;
+  check(bs_verify_drafts_workspace_bytes(N, V, dtype_code(logits.scalar_type()), &need));
+  const Tensor ws = scratch(need, device);
+  const auto options = at::TensorOptions(at::kInt).device(device);
+  const Tensor out = at::empty({N}, options), accepted = at::empty({B}, options);
+  check(bs_verify_drafts(
+      l.data_ptr(), std::max(l.stride(0), V), dtype_code(logits.scalar_type()), N, V,
+      static_cast<const int32_t*>(tokens.data_ptr()), static_cast<const int32_t*>(cu.data_ptr()), B,
+      static_cast<const float*>(u.data_ptr()), static_cast<const float*>(address(temps)),
+      temperature, address(probs), probs.defined() ? std::max(probs.stride(0), V) : 0,
+      probs.defined() ? dtype_code(probs.scalar_type()) : 0, static_cast<int32_t*>(out.data_ptr()),
+      static_cast<int32_t*>(accepted.data_ptr()), address(ws), need, launch.status,
+      launch.stream));
+  return pair(out, accepted);
 }
 
 // (callable(device index, stream handle) -> address of the status word)
@@ -449,9 +599,14 @@ PyMethodDef method(const char* name) {
 }
 
 PyMethodDef g_methods[] = {
-    method<window_attention_batched, 11>("window_attention_batched"),
-    method<window_prefill_attention, 13>("window_prefill_attention"),
-    method<rotary_append, 10>("rotary_append"),
+    method<attention_batched<false>, 11>("window_attention_batched"),
+    method<prefill_attention<false>, 13>("window_prefill_attention"),
+    method<append<false>, 10>("rotary_append"),
+    method<attention_batched<true>, 11>("int4_attention_batched"),
+    method<prefill_attention<true>, 13>("int4_prefill_attention"),
+    method<append<true>, 10>("rotary_append_int4"),
+    method<read_int4, 3>("read_int4"),
+    method<verify_drafts, 6>("verify_drafts"),
     method<copy_blocks, 4>("copy_blocks"),
     method<set_status_source, 1>("set_status_source"),
     method<zeros_apart, 2>("zeros_apart"),

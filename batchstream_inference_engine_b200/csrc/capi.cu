@@ -1046,6 +1046,7 @@ int bs_take_status(void* workspace, void* stream, uint32_t* status_out) {
   if (bits & BS_STATUS_BAD_POSITION) msg += " position outside the rotary tables;";
   if (bits & BS_STATUS_BAD_INDEX) msg += " gathered row index out of range;";
   if (bits & BS_STATUS_BAD_COPY) msg += " block copied to is named by another pair;";
+  if (bits & BS_STATUS_BAD_VALUE) msg += " value not finite or too large;";
   g_error = msg;
   return BS_ERR_DEVICE;
 }

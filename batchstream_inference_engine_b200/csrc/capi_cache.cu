@@ -1,6 +1,7 @@
 // C ABI of the operators that keep a conversation's cache bounded: attention over
 // a sliding window with sink tokens, rotary embedding with the K/V append from
-// frequencies, and block copies (declared in include/batchstream_b200.h).
+// frequencies, block copies, and the same attention and append over a cache of 4 bits
+// (declared in include/batchstream_b200.h).
 //
 // Validation, messages and launch rules as in capi.cu: a malformed call is an
 // error code plus a message, launches go on the caller's stream, nothing here
@@ -16,6 +17,7 @@
 
 #include "../../include/batchstream_b200.h"
 #include "decode.cuh"
+#include "int4.cuh"
 #include "window.cuh"
 
 namespace bsb {
@@ -36,6 +38,14 @@ int launch_rotary_append(const void* qkv, int64_t qkv_stride, bool bf16, const d
 int launch_copy_blocks(void* k_pool, void* v_pool, const int32_t* src, const int32_t* dst,
                        int32_t n, int32_t num_blocks, int64_t rows, int64_t block_bytes, int align,
                        int sms, uint32_t* status, cudaStream_t stream);
+int launch_int4_append(const void* qkv, int64_t qkv_stride, bool bf16, const double* freq,
+                       int32_t rotary_dim, bool interleaved, double amp, const int32_t* pos,
+                       const int32_t* slots, int32_t ntok, int32_t H, int32_t Hkv, int32_t D,
+                       void* q_out, void* k_pool, void* v_pool, int32_t num_blocks,
+                       int32_t block_size, bool vec, uint32_t* status, cudaStream_t stream);
+int launch_int4_read(const void* k_pool, const void* v_pool, const int32_t* slots, int64_t ntok,
+                     int32_t Hkv, int32_t D, int32_t num_blocks, int32_t block_size, void* k_out,
+                     void* v_out, int sms, uint32_t* status, cudaStream_t stream);
 }  // namespace bsb
 
 namespace {
@@ -66,6 +76,19 @@ constexpr int64_t kMaxGroups = 16;
 constexpr int64_t kMaxContext = 1ll << 30;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Codes of 4-bit pools are read and written as 32-bit words.
+bool int4_aligned(const void* k, const void* v) {
+  return ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 3u) == 0;
+}
+// Head sizes and block sizes of 4-bit pools: whole groups, blocks of whole words.
+int check_int4_block(int64_t head_dim, int64_t block_size) {
+  BS_CHECK(head_dim % bsb::kInt4Group == 0, "head_dim must be a multiple of 32");
+  BS_CHECK(head_dim / bsb::kInt4Group % 2 == 0 || block_size % 2 == 0,
+           "block_size must be even for a head_dim that is not a multiple of 64");
+  return BS_OK;
+}
+// The window of a call in which 0 means every token (others stay as they are, to be checked).
+int64_t window_of(int64_t window) { return window == 0 ? kMaxContext : window; }
 int dtype_size(int32_t dtype) { return dtype == BS_BF16 ? 2 : 4; }
 
 // a * b, or -1 when it does not fit (both non-negative).
@@ -80,6 +103,7 @@ struct WindowShape {
   bool chunks;                          // chunks of tokens (else one token per row)
   int64_t heads, kv_heads, head_dim, block_size, max_blocks, window, sinks;
   int32_t dtype;
+  bool int4;  // the pools are 4-bit ones
 };
 
 int check_window_shape(const WindowShape& s) {
@@ -95,6 +119,9 @@ int check_window_shape(const WindowShape& s) {
   if (s.head_dim > kMaxHeadDim || s.heads / s.kv_heads > kMaxGroups || s.kv_heads > kInt32Max) {
     return fail(BS_ERR_UNSUPPORTED, "head_dim <= %lld and groups <= %lld are supported",
                 static_cast<long long>(kMaxHeadDim), static_cast<long long>(kMaxGroups));
+  }
+  if (s.int4) {
+    if (int rc = check_int4_block(s.head_dim, s.block_size)) return rc;
   }
   const int64_t context = product(s.max_blocks, s.block_size);
   if (context < 0 || context > kMaxContext) {
@@ -148,8 +175,8 @@ int plan_simt(const WindowShape& s, SimtPlan* p) {
   if (p->splits > 1 && p->splits <= bsb::kMaxWindowCluster) {
     const bool bf16 = s.dtype == BS_BF16, wide = p->tile_tokens * groups > 8;
     const int head_dim = static_cast<int>(s.head_dim), cluster = static_cast<int>(p->splits);
-    const int ctas = bsb::window_simt_at_once(bf16, wide, head_dim, 1);
-    const int clusters = bsb::window_simt_at_once(bf16, wide, head_dim, cluster);
+    const int ctas = bsb::window_simt_at_once(bf16, s.int4, wide, head_dim, 1);
+    const int clusters = bsb::window_simt_at_once(bf16, s.int4, wide, head_dim, cluster);
     if (ctas <= 0 || clusters < 0) {
       return fail(BS_ERR_CUDA, "occupancy query for window attention failed (%d, %d)", ctas,
                   clusters);
@@ -167,7 +194,7 @@ int plan_simt(const WindowShape& s, SimtPlan* p) {
 // Shapes the tensor-core kernels take (with 16-byte aligned pools and queries, and
 // outputs that their stores can address; see mma_pointers).
 bool mma_shape(const WindowShape& s) {
-  return s.dtype == BS_BF16 && s.block_size % 16 == 0 && (s.head_dim == 64 || s.head_dim == 128);
+  return !s.int4 && s.dtype == BS_BF16 && s.block_size % 16 == 0 && (s.head_dim == 64 || s.head_dim == 128);
 }
 
 // How the tensor-core decode runs a call: a cluster of segment_ctas CTAs per
@@ -405,7 +432,9 @@ int run_window(const WindowShape& s, const WindowCall& c) {
   BS_CHECK(c.num_blocks > 0, "sizes must be positive");
   BS_CHECK(c.q_stride >= s.heads * s.head_dim && c.o_stride >= s.heads * s.head_dim,
            "token strides must cover heads * head_dim");
-  const int64_t pool_rows = product(product(s.kv_heads, c.num_blocks), s.block_size);
+  // (Rows are tensor-map coordinates; of 4-bit pools only a head's are counted.)
+  const int64_t pool_rows =
+      product(product(s.int4 ? 1 : s.kv_heads, c.num_blocks), s.block_size);
   if (pool_rows < 0 || pool_rows > kInt32Max) {
     return fail(BS_ERR_UNSUPPORTED, "pool has more than 2^31 rows");
   }
@@ -423,6 +452,7 @@ int run_window(const WindowShape& s, const WindowCall& c) {
   a.o_stride = c.o_stride;
   a.k_pool = c.key_pool;
   a.v_pool = c.value_pool;
+  a.int4 = s.int4 ? 1 : 0;
   a.block_tables = c.block_tables;
   a.bt_stride = c.table_stride;
   a.bt_rows = static_cast<int32_t>(c.table_rows);
@@ -447,6 +477,9 @@ int run_window(const WindowShape& s, const WindowCall& c) {
   // magnitude to scale by.
   if (mma && a.scale != 0.f && std::isfinite(a.scale)) return run_mma_chunks(s, c, a);
 
+  if (s.int4) {
+    BS_CHECK(int4_aligned(c.key_pool, c.value_pool), "4-bit pools must be 4-byte aligned");
+  }
   SimtPlan p;
   if (int rc = plan_simt(s, &p)) return rc;
   if (int rc = check_workspace(c, p.bytes)) return rc;
@@ -531,6 +564,139 @@ int bs_window_prefill_attention(const void* query, int64_t query_token_stride, c
                      num_blocks,   scaling,          output,     output_token_stride, workspace,
                      workspace_bytes, status,        stream};
   return run_window(s, c);
+}
+
+int bs_int4_attention_batched_workspace_bytes(int64_t num_seqs, int64_t num_heads,
+                                              int64_t num_kv_heads, int64_t head_dim,
+                                              int64_t block_size, int64_t max_blocks_per_seq,
+                                              int32_t dtype, int64_t window, int64_t sinks,
+                                              uint64_t* bytes_out) {
+  const WindowShape s{num_seqs, num_seqs,   1,          false,
+                      num_heads, num_kv_heads, head_dim, block_size,
+                      max_blocks_per_seq, window_of(window), sinks, dtype, true};
+  return window_workspace(s, bytes_out);
+}
+
+int bs_int4_prefill_attention_workspace_bytes(int64_t num_tokens, int64_t num_rows,
+                                              int64_t max_query_len, int64_t num_heads,
+                                              int64_t num_kv_heads, int64_t head_dim,
+                                              int64_t block_size, int64_t max_blocks_per_seq,
+                                              int32_t dtype, int64_t window, int64_t sinks,
+                                              uint64_t* bytes_out) {
+  const WindowShape s{num_rows, num_tokens, std::min(max_query_len, num_tokens), true,
+                      num_heads, num_kv_heads, head_dim, block_size,
+                      max_blocks_per_seq, window_of(window), sinks, dtype, true};
+  return window_workspace(s, bytes_out);
+}
+
+int bs_int4_attention_batched(const void* query, int64_t query_seq_stride, const void* key_pool,
+                              const void* value_pool, const int32_t* block_tables,
+                              int64_t table_stride, int64_t table_rows, const int32_t* seq_rows,
+                              const int32_t* context_lens, int64_t num_seqs, int64_t num_heads,
+                              int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                              int64_t num_blocks, int64_t max_blocks_per_seq, int32_t dtype,
+                              double scaling, int64_t window, int64_t sinks, void* output,
+                              int64_t output_seq_stride, void* workspace,
+                              uint64_t workspace_bytes, uint32_t* status, void* stream) {
+  const WindowShape s{num_seqs, num_seqs,   1,          false,
+                      num_heads, num_kv_heads, head_dim, block_size,
+                      max_blocks_per_seq, window_of(window), sinks, dtype, true};
+  const WindowCall c{query,        query_seq_stride, nullptr,    context_lens, seq_rows,
+                     key_pool,     value_pool,       block_tables, table_stride, table_rows,
+                     num_blocks,   scaling,          output,     output_seq_stride, workspace,
+                     workspace_bytes, status,        stream};
+  return run_window(s, c);
+}
+
+int bs_int4_prefill_attention(const void* query, int64_t query_token_stride, const int32_t* cu_q,
+                              int64_t num_rows, int64_t num_tokens, int64_t max_query_len,
+                              const int32_t* context_lens, const int32_t* seq_rows,
+                              const void* key_pool, const void* value_pool,
+                              const int32_t* block_tables, int64_t table_stride,
+                              int64_t table_rows, int64_t max_blocks_per_seq, int64_t num_heads,
+                              int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                              int64_t num_blocks, int32_t dtype, double scaling, int64_t window,
+                              int64_t sinks, void* output, int64_t output_token_stride,
+                              void* workspace, uint64_t workspace_bytes, uint32_t* status,
+                              void* stream) {
+  const WindowShape s{num_rows, num_tokens, std::min(max_query_len, num_tokens), true,
+                      num_heads, num_kv_heads, head_dim, block_size,
+                      max_blocks_per_seq, window_of(window), sinks, dtype, true};
+  const WindowCall c{query,        query_token_stride, cu_q,      context_lens, seq_rows,
+                     key_pool,     value_pool,       block_tables, table_stride, table_rows,
+                     num_blocks,   scaling,          output,     output_token_stride, workspace,
+                     workspace_bytes, status,        stream};
+  return run_window(s, c);
+}
+
+int bs_rotary_append_int4(const void* qkv, int64_t qkv_row_stride, int32_t dtype,
+                          const double* frequencies, int64_t rotary_dim, int32_t interleaved,
+                          double amplitude, const int32_t* positions, const int32_t* slot_mapping,
+                          int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads,
+                          int64_t head_dim, void* query_out, void* key_pool, void* value_pool,
+                          int64_t num_blocks, int64_t block_size, uint32_t* status, void* stream) {
+  BS_CHECK(dtype == BS_BF16 || dtype == BS_F32, "dtype must be bfloat16 or float32");
+  BS_CHECK(num_tokens >= 0 && num_tokens <= kInt32Max, "num_tokens out of range");
+  BS_CHECK(num_heads >= 0 && num_kv_heads > 0 && head_dim > 0, "sizes must be positive");
+  BS_CHECK(rotary_dim >= 0 && rotary_dim % 2 == 0 && rotary_dim <= head_dim,
+           "rotary_dim must be even and in [0, head_dim]");
+  BS_CHECK(std::isfinite(amplitude), "amplitude must be finite");
+  BS_CHECK(num_blocks > 0 && block_size > 0, "sizes must be positive");
+  if (int rc = check_int4_block(head_dim, block_size)) return rc;
+  if (head_dim > 1024 || num_heads > 65536 || num_kv_heads > 65536) {
+    return fail(BS_ERR_UNSUPPORTED, "head_dim <= 1024 and at most 65536 heads are supported");
+  }
+  BS_CHECK(qkv_row_stride >= (num_heads + 2 * num_kv_heads) * head_dim,
+           "qkv rows must hold q, k and v");
+  const int64_t slots = product(num_blocks, block_size);
+  if (slots < 0 || slots > kInt32Max) return fail(BS_ERR_UNSUPPORTED, "pool too large");
+  if (num_tokens == 0) return BS_OK;
+  BS_CHECK(qkv && (rotary_dim == 0 || (frequencies && positions)) && slot_mapping &&
+               (num_heads == 0 || query_out) && key_pool && value_pool,
+           "null pointer argument");
+  BS_CHECK(int4_aligned(key_pool, value_pool), "4-bit pools must be 4-byte aligned");
+  // (Rows of 8 dims: all heads begin on 16 bytes when the first does.)
+  const bool vec = (rotary_dim == 0 || rotary_dim % (interleaved ? 8 : 16) == 0) &&
+                   qkv_row_stride % 8 == 0 && aligned16(qkv) && aligned16(query_out);
+  const int rc = bsb::launch_int4_append(
+      qkv, qkv_row_stride, dtype == BS_BF16, frequencies, static_cast<int32_t>(rotary_dim),
+      interleaved != 0, amplitude, positions, slot_mapping, static_cast<int32_t>(num_tokens),
+      static_cast<int32_t>(num_heads), static_cast<int32_t>(num_kv_heads),
+      static_cast<int32_t>(head_dim), query_out, key_pool, value_pool,
+      static_cast<int32_t>(num_blocks), static_cast<int32_t>(block_size), vec, status,
+      static_cast<cudaStream_t>(stream));
+  if (rc != 0) return cuda_fail(rc, "rotary_append_int4 launch");
+  bsb::add_kernel_launches(1);
+  return BS_OK;
+}
+
+int bs_read_int4(const void* key_pool, const void* value_pool, const int32_t* slot_mapping,
+                 int64_t num_tokens, int64_t num_kv_heads, int64_t num_blocks, int64_t block_size,
+                 int64_t head_dim, void* key_out, void* value_out, uint32_t* status,
+                 void* stream) {
+  BS_CHECK(num_tokens >= 0 && num_tokens <= kInt32Max, "num_tokens out of range");
+  BS_CHECK(num_kv_heads > 0 && num_kv_heads <= kInt32Max && num_blocks > 0 && block_size > 0,
+           "sizes must be positive");
+  BS_CHECK(head_dim > 0, "sizes must be positive");
+  if (int rc = check_int4_block(head_dim, block_size)) return rc;
+  const int64_t slots = product(num_blocks, block_size);
+  if (slots < 0 || slots > kInt32Max || head_dim > 1024) {
+    return fail(BS_ERR_UNSUPPORTED, "pool too large");
+  }
+  if (num_tokens == 0) return BS_OK;
+  BS_CHECK(key_pool && value_pool && slot_mapping && key_out && value_out, "null pointer argument");
+  BS_CHECK(int4_aligned(key_pool, value_pool), "4-bit pools must be 4-byte aligned");
+  BS_CHECK(aligned16(key_out) && aligned16(value_out), "outputs must be 16-byte aligned");
+  int sms = 0;
+  if (int rc = bsb::sm_count(&sms)) return rc;
+  const int rc = bsb::launch_int4_read(
+      key_pool, value_pool, slot_mapping, num_tokens, static_cast<int32_t>(num_kv_heads),
+      static_cast<int32_t>(head_dim), static_cast<int32_t>(num_blocks),
+      static_cast<int32_t>(block_size), key_out, value_out, sms, status,
+      static_cast<cudaStream_t>(stream));
+  if (rc != 0) return cuda_fail(rc, "read_int4 launch");
+  bsb::add_kernel_launches(1);
+  return BS_OK;
 }
 
 int bs_rotary_append(const void* qkv, int64_t qkv_row_stride, int32_t dtype,

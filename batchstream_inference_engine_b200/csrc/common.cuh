@@ -28,6 +28,7 @@ enum : uint32_t {
   kStatusBadPosition = 1u << 5,  // position outside the rotary tables
   kStatusBadIndex = 1u << 6,     // gathered row index outside its tensor
   kStatusBadCopy = 1u << 7,      // block copy whose destination another pair names
+  kStatusBadValue = 1u << 8,     // value that the operator cannot hold or weigh
 };
 
 constexpr uint32_t kSpinLimit = 1u << 26;

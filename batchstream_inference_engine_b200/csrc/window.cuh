@@ -23,6 +23,7 @@ struct WindowArgs {
   int64_t o_stride;
   const void* k_pool;  // [Hkv, NB, bs, D] contiguous
   const void* v_pool;
+  int32_t int4;  // the pools are 4-bit ones (int4.cuh)
   const int32_t* block_tables;
   int64_t bt_stride;
   int32_t bt_rows, max_blocks;
@@ -125,7 +126,7 @@ int launch_window_prefill(const WindowArgs& a, const CUtensorMap& qmap, const CU
                           const CUtensorMap& vmap, cudaStream_t stream);
 // What runs at once of the CUDA-core kernel: CTAs per SM (cluster 1), or clusters of so many
 // CTAs on the device (negative: a CUDA error); wide: more than 8 query rows a tile.
-int window_simt_at_once(bool bf16, bool wide, int head_dim, int cluster);
+int window_simt_at_once(bool bf16, bool int4, bool wide, int head_dim, int cluster);
 int launch_window_simt(const WindowArgs& a, bool bf16, bool vec, cudaStream_t stream);
 
 }  // namespace bsb

@@ -25,6 +25,7 @@
 #include <mutex>
 #include <vector>
 
+#include "int4.cuh"
 #include "window.cuh"
 
 namespace bsb {
@@ -103,9 +104,10 @@ __device__ __forceinline__ void window_item(const WindowArgs& a, int64_t item, i
 }
 
 // GM: query rows held per CTA; DPL: head dims per lane; VEC: 16-byte K rows; FULL:
-// head_dim is exactly 32 DPL (its loops then have compile-time bounds).
-template <typename T, int GM, int DPL, bool VEC, bool FULL>
+// head_dim is exactly 32 DPL (its loops then have compile-time bounds); Q4: 4-bit pools.
+template <typename T, int GM, int DPL, bool VEC, bool FULL, bool Q4>
 __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs a) {
+  static_assert(!Q4 || (!VEC && !FULL), "4-bit rows are held as floats");
   using L_ = Layout<T, GM, DPL, VEC>;
   extern __shared__ __align__(16) uint8_t wsm[];
   pdl_wait();
@@ -163,12 +165,19 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
     // Lane j's key of the group: its position and its row's offset (-1: none).
     const int32_t v = base + lane;
     int32_t pos = 0;
-    int64_t off = -1;
+    int64_t off = -1, scales = 0;  // Q4: bytes, of the row's codes and scales
     if (v < end) {
       pos = window_key(w, v);
       const int32_t blk = __ldg(table + pos / bs);
       if (blk >= 0 && blk < a.num_blocks) {
-        off = (static_cast<int64_t>(blk) * bs + pos % bs) * D;
+        if constexpr (Q4) {
+          off = (static_cast<int64_t>(h) * a.num_blocks + blk) * bs * int4_row_bytes(D);
+          scales = off + static_cast<int64_t>(bs) * int4_code_bytes(D) +
+                   (pos % bs) * int4_scale_bytes(D);
+          off += (pos % bs) * int4_code_bytes(D);
+        } else {
+          off = (static_cast<int64_t>(blk) * bs + pos % bs) * D;
+        }
       } else {
         set_status(a.status, kStatusBadBlock);
       }
@@ -192,7 +201,29 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
         copy_commit();
       }
     };
-    if constexpr (VEC) {
+    // A pool's rows as floats, a lane taking 8 dims at a time.
+    auto widen_rows = [&](const void* pool) {
+      const int per_row = D >> 3;
+      const uint8_t* bytes = static_cast<const uint8_t*>(pool);
+#pragma unroll 4
+      for (int it = 0; it < per_row; ++it) {
+        const int idx = it * 32 + lane;
+        const int key = idx / per_row, c = idx - key * per_row;
+        const int64_t ko = __shfl_sync(0xffffffffu, off, key);
+        const int64_t so = __shfl_sync(0xffffffffu, scales, key);
+        if (ko < 0) continue;
+        float f[8];
+        int4_floats(__ldg(reinterpret_cast<const uint32_t*>(bytes + ko) + c),
+                    int4_scale_float(__ldg(reinterpret_cast<const uint16_t*>(bytes + so) + (c >> 2))),
+                    f);
+        float* dst = reinterpret_cast<float*>(sK + key * k_row) + 8 * c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dst[i] = f[i];
+      }
+    };
+    if constexpr (Q4) {
+      widen_rows(a.k_pool);
+    } else if constexpr (VEC) {
       copy_rows(0, L_::kVOverK ? 0 : 1);
       copy_wait<L_::kVOverK ? 0 : 1>();
     } else {
@@ -239,6 +270,10 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
       __syncwarp();  // every lane has read its K row
       copy_rows(1, 1);
     }
+    if constexpr (Q4) {
+      __syncwarp();  // every lane has read its K row
+      widen_rows(a.v_pool);
+    }
 #pragma unroll
     for (int i = 0; i < GM; ++i) {
       if (i >= rows) {
@@ -268,12 +303,14 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
 #pragma unroll 4
     for (int j = 0; j < nkeys; ++j) {
       if (!((held >> j) & 1u)) continue;
-      const int64_t vo = VEC ? 0 : __shfl_sync(0xffffffffu, off, j);
+      const int64_t vo = VEC || Q4 ? 0 : __shfl_sync(0xffffffffu, off, j);
       float vv[DPL];
 #pragma unroll
       for (int k = 0; k < DPL; ++k) {
         const int d = lane + 32 * k;
-        if constexpr (VEC) {
+        if constexpr (Q4) {
+          vv[k] = d < D ? reinterpret_cast<const float*>(sK + j * k_row)[d] : 0.f;
+        } else if constexpr (VEC) {
           vv[k] = FULL || d < D ? to_float<T>(reinterpret_cast<const T*>(sV + j * v_row)[d]) : 0.f;
         } else {
           vv[k] = FULL || d < D ? to_float<T>(vh[vo + d]) : 0.f;
@@ -409,22 +446,22 @@ __global__ void __launch_bounds__(kThreads) window_simt_merge_kernel(const Windo
 }
 
 // Shared memory for an instance's largest head_dim.
-template <typename T, int GM, int DPL, bool VEC, bool FULL>
+template <typename T, int GM, int DPL, bool VEC, bool FULL, bool Q4>
 cudaError_t allow_smem() {
   static unsigned long long configured = 0;  // one bit per device
   return once_per_device(&configured, [] {
-    return cudaFuncSetAttribute(window_simt_kernel<T, GM, DPL, VEC, FULL>,
+    return cudaFuncSetAttribute(window_simt_kernel<T, GM, DPL, VEC, FULL, Q4>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 Layout<T, GM, DPL, VEC>::total(DPL * 32));
   });
 }
 
-template <typename T, int GM, int DPL, bool VEC, bool FULL>
+template <typename T, int GM, int DPL, bool VEC, bool FULL, bool Q4 = false>
 int launch_one(const WindowArgs& a, cudaStream_t stream) {
   using L_ = Layout<T, GM, DPL, VEC>;
   const int smem = L_::total(a.head_dim);
-  auto kernel = window_simt_kernel<T, GM, DPL, VEC, FULL>;
-  const cudaError_t e = allow_smem<T, GM, DPL, VEC, FULL>();
+  auto kernel = window_simt_kernel<T, GM, DPL, VEC, FULL, Q4>;
+  const cudaError_t e = allow_smem<T, GM, DPL, VEC, FULL, Q4>();
   if (e != cudaSuccess) return static_cast<int>(e);
   const int64_t items = static_cast<int64_t>(a.num_rows) * a.qtiles * a.num_kv_heads;
   cudaLaunchAttribute attr[2];
@@ -456,6 +493,14 @@ int launch_full(const WindowArgs& a, cudaStream_t stream) {
   return launch_one<T, GM, DPL, VEC, false>(a, stream);
 }
 
+template <typename T, int GM>
+int launch_q4(const WindowArgs& a, cudaStream_t stream) {
+  if (a.head_dim <= 32) return launch_one<T, GM, 1, false, false, true>(a, stream);
+  if (a.head_dim <= 64) return launch_one<T, GM, 2, false, false, true>(a, stream);
+  if (a.head_dim <= 128) return launch_one<T, GM, 4, false, false, true>(a, stream);
+  return launch_one<T, GM, 8, false, false, true>(a, stream);
+}
+
 template <typename T, int GM, bool VEC>
 int launch_dims(const WindowArgs& a, cudaStream_t stream) {
   if (a.head_dim <= 32) return launch_full<T, GM, 1, VEC>(a, stream);
@@ -466,7 +511,9 @@ int launch_dims(const WindowArgs& a, cudaStream_t stream) {
 
 template <typename T>
 int launch_rows(const WindowArgs& a, bool vec, cudaStream_t stream) {
-  if (a.tile_tokens * a.groups <= 8) {
+  const bool wide = a.tile_tokens * a.groups > 8;
+  if (a.int4) return wide ? launch_q4<T, kWindowSimtRows>(a, stream) : launch_q4<T, 8>(a, stream);
+  if (!wide) {
     return vec ? launch_dims<T, 8, true>(a, stream) : launch_dims<T, 8, false>(a, stream);
   }
   return vec ? launch_dims<T, kWindowSimtRows, true>(a, stream)
@@ -476,7 +523,7 @@ int launch_rows(const WindowArgs& a, bool vec, cudaStream_t stream) {
 // What the device runs at once of an instance: CTAs per SM (cluster 1), or clusters of
 // `cluster` CTAs on the whole device; or a CUDA error, negative.  Asked for once per
 // device and size.
-template <typename T, int GM, int DPL, bool VEC, bool FULL>
+template <typename T, int GM, int DPL, bool VEC, bool FULL, bool Q4 = false>
 int at_once(int D, int cluster) {
   struct Known {
     int device, D, cluster, count;
@@ -491,8 +538,8 @@ int at_once(int D, int cluster) {
     if (k.device == dev && k.D == D && k.cluster == cluster) return k.count;
   }
   using L_ = Layout<T, GM, DPL, VEC>;
-  auto kernel = window_simt_kernel<T, GM, DPL, VEC, FULL>;
-  e = allow_smem<T, GM, DPL, VEC, FULL>();
+  auto kernel = window_simt_kernel<T, GM, DPL, VEC, FULL, Q4>;
+  e = allow_smem<T, GM, DPL, VEC, FULL, Q4>();
   int count = 0;
   if (e == cudaSuccess && cluster == 1) {
     e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&count, kernel, kThreads, L_::total(D));
@@ -516,26 +563,28 @@ int at_once(int D, int cluster) {
 
 // As the launch chooses, with aligned pools.
 template <typename T, int GM, int DPL>
-int at_once_full(int D, int cluster) {
+int at_once_full(int D, int cluster, bool int4) {
+  if (int4) return at_once<T, GM, DPL, false, false, true>(D, cluster);
   if (D * sizeof(T) % 16 != 0) return at_once<T, GM, DPL, false, false>(D, cluster);
   return D == 32 * DPL ? at_once<T, GM, DPL, true, true>(D, cluster)
                        : at_once<T, GM, DPL, true, false>(D, cluster);
 }
 
 template <typename T, int GM>
-int at_once_dims(int D, int cluster) {
-  return D <= 32 ? at_once_full<T, GM, 1>(D, cluster)
-         : D <= 64 ? at_once_full<T, GM, 2>(D, cluster)
-         : D <= 128 ? at_once_full<T, GM, 4>(D, cluster) : at_once_full<T, GM, 8>(D, cluster);
+int at_once_dims(int D, int cluster, bool int4) {
+  return D <= 32 ? at_once_full<T, GM, 1>(D, cluster, int4)
+         : D <= 64 ? at_once_full<T, GM, 2>(D, cluster, int4)
+         : D <= 128 ? at_once_full<T, GM, 4>(D, cluster, int4)
+                    : at_once_full<T, GM, 8>(D, cluster, int4);
 }
 
 }  // namespace
 
-int window_simt_at_once(bool bf16, bool wide, int head_dim, int cluster) {
-  return bf16 ? (wide ? at_once_dims<__nv_bfloat16, kWindowSimtRows>(head_dim, cluster)
-                      : at_once_dims<__nv_bfloat16, 8>(head_dim, cluster))
-              : (wide ? at_once_dims<float, kWindowSimtRows>(head_dim, cluster)
-                      : at_once_dims<float, 8>(head_dim, cluster));
+int window_simt_at_once(bool bf16, bool int4, bool wide, int head_dim, int cluster) {
+  return bf16 ? (wide ? at_once_dims<__nv_bfloat16, kWindowSimtRows>(head_dim, cluster, int4)
+                      : at_once_dims<__nv_bfloat16, 8>(head_dim, cluster, int4))
+              : (wide ? at_once_dims<float, kWindowSimtRows>(head_dim, cluster, int4)
+                      : at_once_dims<float, 8>(head_dim, cluster, int4));
 }
 
 int launch_window_simt(const WindowArgs& a, bool bf16, bool vec, cudaStream_t stream) {

@@ -647,6 +647,12 @@ __all__ = [
     "rope_frequencies",
     "rotary_append",
     "copy_blocks",
+    "int4_pool_shape",
+    "rotary_append_int4",
+    "read_int4",
+    "int4_attention_batched",
+    "int4_prefill_attention",
+    "verify_drafts",
     "take_status",
     "status_words",
     "kernel_launches",
@@ -872,11 +878,117 @@ def copy_blocks(key_pool: torch.Tensor, value_pool: torch.Tensor, src: torch.Ten
                 dst: torch.Tensor) -> None:
     """Copies block src[i] to block dst[i], K and V, in every layer and kv head.
 
-    Pools [L, Hkv, NB, bs, D] (or one layer's [Hkv, NB, bs, D]); src and dst int32
-    on the device.  All pairs happen at once: a pair whose destination another
+    Pools [L, Hkv, NB, bs, D] (or one layer's [Hkv, NB, bs, D]), or 4-bit ones
+    (``int4_pool_shape``); src and dst int32 on the device.  All pairs happen at once: a pair whose destination another
     pair names too, as source or destination, is reported (``take_status``) and
     skipped, and so is one outside the pool.  Negative ends are padding.  (Every
     pair is looked up among all others on the device: n pairs cost n^2 lookups, small
     against the copies for thousands of pairs.)
     """
     _native.copy_blocks(key_pool, value_pool, src, dst)
+
+
+# ------------------------------------------------------------------ the 4-bit cache
+
+
+def int4_pool_shape(num_kv_heads: int, num_blocks: int, block_size: int,
+                    head_dim: int) -> tuple[int, int, int, int]:
+    """Shape of one layer's 4-bit key or value pool, uint8 [Hkv, NB, bs, 9 * D / 16].
+
+    32 consecutive dims of a token and head share a scale s of at most 4 significant bits;
+    a code n = 0 .. 15 stands for s * (n - 8), which is exactly a bf16 number: 4.5 bits a
+    dim.  A block holds the codes of its tokens, then their scales
+    (``include/batchstream_b200.h`` has the layout).  head_dim must be a multiple of 32, and
+    block_size even where head_dim is not a multiple of 64.
+    """
+    if head_dim <= 0 or head_dim % 32:
+        raise RuntimeError("head_dim of a 4-bit pool must be a multiple of 32")
+    if head_dim % 64 and block_size % 2:
+        raise RuntimeError("block_size must be even for a head_dim that is not a multiple of 64")
+    return num_kv_heads, num_blocks, block_size, head_dim // 2 + head_dim // 16
+
+
+def rotary_append_int4(qkv: torch.Tensor, frequencies: torch.Tensor, positions: torch.Tensor,
+                       slot_mapping: torch.Tensor, key_pool: torch.Tensor,
+                       value_pool: torch.Tensor, num_heads: int, interleaved: bool = False,
+                       amplitude: float = 1.0, query_out: torch.Tensor | None = None
+                       ) -> torch.Tensor:
+    """``rotary_append`` into 4-bit pools (``int4_pool_shape``), in one launch.
+
+    Without frequencies (an empty tensor) nothing turns; with num_heads 0 the rows are
+    [k heads | v heads].  What is stored of 32 dims: s = -x / 8 for the element x of the
+    largest magnitude (the negative one of two), the magnitude rounded up to 4 bits, and
+    codes rint(x / s) + 8, at most 15.  Elements are off by |s| / 2 at most, those beyond
+    7.5 |s| on the other side than x by |s|.  Rotated keys are formed in fp64 and rounded
+    only here.  Groups below 2^-100 are stored as zeros, and so are groups with an
+    element that is not finite or 2^120 or more, which are reported (``take_status``).
+    Returns q as [T, H, D].
+    """
+    return _native.rotary_append_int4(qkv, frequencies, positions, slot_mapping, key_pool,
+                                      value_pool, num_heads, interleaved, amplitude, query_out)
+
+
+def read_int4(key_pool: torch.Tensor, value_pool: torch.Tensor,
+              slot_mapping: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of 4-bit pools as the bf16 numbers that they stand for: (keys, values), each
+    [T, Hkv, D], of the slots in int32 ``slot_mapping``.  Rows of negative slots are zeros."""
+    return _native.read_int4(key_pool, value_pool, slot_mapping)
+
+
+def int4_attention_batched(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
+                           block_tables: torch.Tensor, context_lens: torch.Tensor,
+                           scaling: float, window: int = 0, sinks: int = 0,
+                           seq_rows: torch.Tensor | None = None,
+                           out: torch.Tensor | None = None,
+                           max_blocks_per_seq: int | None = None) -> torch.Tensor:
+    """``window_attention_batched`` over 4-bit pools (``int4_pool_shape``); window 0 sees
+    every token.  The result is that of the bf16 pools which hold the same numbers, with
+    the same precision; head_dim up to 256.
+    """
+    return _native.int4_attention_batched(query, key_pool, value_pool, block_tables, context_lens,
+                                          scaling, window, sinks, seq_rows, out,
+                                          max_blocks_per_seq)
+
+
+def int4_prefill_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
+                           block_tables: torch.Tensor, cu_q: torch.Tensor,
+                           context_lens: torch.Tensor, scaling: float, max_query_len: int,
+                           window: int = 0, sinks: int = 0,
+                           seq_rows: torch.Tensor | None = None,
+                           out: torch.Tensor | None = None,
+                           max_blocks_per_seq: int | None = None) -> torch.Tensor:
+    """``window_prefill_attention`` over 4-bit pools; window 0 sees every token.  Short
+    chunks too: the few drafted tokens of many sequences at once."""
+    return _native.int4_prefill_attention(query, key_pool, value_pool, block_tables, cu_q,
+                                          context_lens, scaling, max_query_len, window, sinks,
+                                          seq_rows, out, max_blocks_per_seq)
+
+
+# ------------------------------------------------------------------ drafted tokens
+
+
+def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, cu_rows: torch.Tensor,
+                  uniforms: torch.Tensor, temperature: float | torch.Tensor = 1.0,
+                  draft_probs: torch.Tensor | None = None
+                  ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Verifies drafted tokens against the target's distribution, from given random numbers.
+
+    Sequence b has rows cu_rows[b] .. cu_rows[b + 1] - 1 of ``logits`` [N, vocab] (bf16 or
+    fp32): one for each of its drafts, and one for the token behind them.  draft_tokens
+    int32 [N] holds the draft that each row has the distribution of (a sequence's last
+    entry is not looked at); draft_probs [N, vocab] (bf16 or fp32) what they were drawn from,
+    None for drafts that were certain (looked up, or a greedy draft model's); uniforms fp32
+    [N] numbers in [0, 1).  With p = softmax(logits / temperature), a draft x is accepted
+    if u q(x) < p(x); at the first that is not, a token is drawn from max(p - q, 0) (from p
+    without x where drafts are certain, from p where nothing is left), behind the last one
+    from p, with the u of the sequence's last row.  So the tokens are distributed as the
+    target's own.  ``temperature`` (a number, or fp32 [B]) 0 accepts what the largest logit
+    (the first, as ``argmax_rows``) would have been, and ends with it.
+
+    Returns int32 (tokens [N], accepted [B]): at each sequence's rows its accepted drafts,
+    the token after them, then -1s (also at rows of no sequence); and how many drafts were
+    accepted.  A sequence without rows is padding.  Bad row offsets, drafts outside the
+    vocabulary, rows without a finite maximum and bad temperatures are reported
+    (``take_status``); the latter two take the largest logit.
+    """
+    return _native.verify_drafts(logits, draft_tokens, cu_rows, uniforms, temperature, draft_probs)

@@ -54,6 +54,7 @@ enum bs_error {
 #define BS_STATUS_BAD_POSITION 0x20u
 #define BS_STATUS_BAD_INDEX 0x40u
 #define BS_STATUS_BAD_COPY 0x80u
+#define BS_STATUS_BAD_VALUE 0x100u
 
 /* Message of the last failing call on this thread ("" if none). */
 const char* bs_last_error(void);
@@ -407,6 +408,113 @@ int bs_copy_blocks(void* key_pool, void* value_pool, int32_t pool_dtype, int64_t
                    int64_t num_kv_heads, int64_t num_blocks, int64_t block_size, int64_t head_dim,
                    const int32_t* src, const int32_t* dst, int64_t num_pairs, uint32_t* status,
                    void* stream);
+
+/*
+ * The 4-bit cache (no counterpart in the reference).  Pools are bytes
+ * [num_kv_heads, num_blocks, block_size, 9 * head_dim / 16], contiguous, 4-byte aligned:
+ * a block holds block_size * head_dim / 2 bytes of codes, then block_size * head_dim / 32
+ * bf16 scales.  32 consecutive dims of a token share the scale s, a bf16 number of at most
+ * 4 significant bits; code n = 0 .. 15 stands for s * (n - 8), which is exactly a bf16
+ * number.  Of 8 dims in a little-endian 32-bit word, dim 2i is nibble i and dim 2i + 1
+ * nibble i + 4.  head_dim is a multiple of 32; block_size is even where head_dim is not a
+ * multiple of 64.
+ *
+ * bs_rotary_append_int4: bs_rotary_append into such pools.  rotary_dim may be 0 (nothing
+ * turns; frequencies and positions are not read), num_heads too (rows [k heads | v heads]).
+ * What is stored of the rotated key and of the value: s = -x / 8 for the group's element x
+ * of the largest magnitude (the negative one of two), the magnitude rounded up to 4 bits,
+ * and n = rint(x / s) + 8, at most 15; the rotated key is formed in fp64 and rounded only
+ * here.  Elements are off by |s| / 2 at most, those beyond 7.5 |s| on the other side than
+ * x by |s|.  Groups below 2^-100 are zeros; a group with an element of 2^120 or more, or
+ * not finite, is zeros and sets BS_STATUS_BAD_VALUE.
+ *
+ * bs_read_int4: rows back as bf16 [num_tokens, num_kv_heads, head_dim] (16-byte aligned);
+ * rows with a negative slot, or with one past the pool (reported), are zeros.
+ *
+ * bs_int4_attention_batched, bs_int4_prefill_attention: bs_window_attention_batched and
+ * bs_window_prefill_attention over such pools, with their workspaces; window 0 means every
+ * token.  head_dim up to 256.  On the tensor cores (bf16, head_dim 64 or 128, block sizes
+ * that are multiples of 16) keys and values enter the products as the bf16 numbers that
+ * the codes stand for.
+ */
+int bs_rotary_append_int4(const void* qkv, int64_t qkv_row_stride, int32_t dtype,
+                          const double* frequencies, int64_t rotary_dim, int32_t interleaved,
+                          double amplitude, const int32_t* positions, const int32_t* slot_mapping,
+                          int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads,
+                          int64_t head_dim, void* query_out, void* key_pool, void* value_pool,
+                          int64_t num_blocks, int64_t block_size, uint32_t* status, void* stream);
+int bs_read_int4(const void* key_pool, const void* value_pool, const int32_t* slot_mapping,
+                 int64_t num_tokens, int64_t num_kv_heads, int64_t num_blocks, int64_t block_size,
+                 int64_t head_dim, void* key_out, void* value_out, uint32_t* status,
+                 void* stream);
+int bs_int4_attention_batched(const void* query, int64_t query_seq_stride, const void* key_pool,
+                              const void* value_pool, const int32_t* block_tables,
+                              int64_t table_stride, int64_t table_rows, const int32_t* seq_rows,
+                              const int32_t* context_lens, int64_t num_seqs, int64_t num_heads,
+                              int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                              int64_t num_blocks, int64_t max_blocks_per_seq, int32_t dtype,
+                              double scaling, int64_t window, int64_t sinks, void* output,
+                              int64_t output_seq_stride, void* workspace,
+                              uint64_t workspace_bytes, uint32_t* status, void* stream);
+int bs_int4_attention_batched_workspace_bytes(int64_t num_seqs, int64_t num_heads,
+                                              int64_t num_kv_heads, int64_t head_dim,
+                                              int64_t block_size, int64_t max_blocks_per_seq,
+                                              int32_t dtype, int64_t window, int64_t sinks,
+                                              uint64_t* bytes_out);
+int bs_int4_prefill_attention(const void* query, int64_t query_token_stride, const int32_t* cu_q,
+                              int64_t num_rows, int64_t num_tokens, int64_t max_query_len,
+                              const int32_t* context_lens, const int32_t* seq_rows,
+                              const void* key_pool, const void* value_pool,
+                              const int32_t* block_tables, int64_t table_stride,
+                              int64_t table_rows, int64_t max_blocks_per_seq, int64_t num_heads,
+                              int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                              int64_t num_blocks, int32_t dtype, double scaling, int64_t window,
+                              int64_t sinks, void* output, int64_t output_token_stride,
+                              void* workspace, uint64_t workspace_bytes, uint32_t* status,
+                              void* stream);
+int bs_int4_prefill_attention_workspace_bytes(int64_t num_tokens, int64_t num_rows,
+                                              int64_t max_query_len, int64_t num_heads,
+                                              int64_t num_kv_heads, int64_t head_dim,
+                                              int64_t block_size, int64_t max_blocks_per_seq,
+                                              int32_t dtype, int64_t window, int64_t sinks,
+                                              uint64_t* bytes_out);
+
+/*
+ * Verification of drafted tokens against the target's distribution, from given random
+ * numbers (no counterpart in the reference, which takes one token a step).  Sequence b has
+ * the rows cu_rows[b] .. cu_rows[b + 1] - 1 of `logits` [num_rows, vocab]: one for each of
+ * its drafts, and one for the token behind them.  draft_tokens[r] is the draft that row r
+ * has the distribution of (a sequence's last entry is not looked at); draft_probs [num_rows,
+ * vocab], or NULL for drafts that were certain, is what they were drawn from.  With
+ * p_r = softmax(logits_r / temperature):
+ *   - draft x of row r is accepted if uniforms[r] * q_r(x) < p_r(x);
+ *   - at the first row whose draft is not accepted, a token is drawn with the weights
+ *     max(p - q, 0) (p without x where drafts are certain; p itself where nothing is left,
+ *     or x where x has all the weight), with all accepted from p of the last row: the first
+ *     token at which the running sum of the weights, in fp64, exceeds uniforms[last row]
+ *     times their sum.
+ * temperatures[b] (or `temperature` for all, where it is NULL) of 0 accepts and takes the
+ * first largest logit instead, as bs_argmax_rows does.
+ *
+ * tokens_out[num_rows] holds, at each sequence's rows, its accepted drafts, the token after
+ * them, and -1s (as at rows of no sequence); accepted_out[b] counts the accepted drafts.  A
+ * sequence without rows is padding.  cu_rows that run backwards or past num_rows
+ * (BS_STATUS_BAD_LENGTH) accept nothing and write no token; a draft outside the vocabulary
+ * (BS_STATUS_BAD_INDEX) is not accepted; where a row that decides has no finite maximum or
+ * the temperature is negative or not finite (BS_STATUS_BAD_VALUE) the largest logit is taken.
+ *
+ * `workspace`: scratch of the queried size, 16-byte aligned, its contents irrelevant, one
+ * per call in flight.
+ */
+int bs_verify_drafts(const void* logits, int64_t logits_row_stride, int32_t dtype,
+                     int64_t num_rows, int64_t vocab, const int32_t* draft_tokens,
+                     const int32_t* cu_rows, int64_t num_seqs, const float* uniforms,
+                     const float* temperatures, double temperature, const void* draft_probs,
+                     int64_t probs_row_stride, int32_t probs_dtype, int32_t* tokens_out,
+                     int32_t* accepted_out, void* workspace, uint64_t workspace_bytes,
+                     uint32_t* status, void* stream);
+int bs_verify_drafts_workspace_bytes(int64_t num_rows, int64_t vocab, int32_t dtype,
+                                     uint64_t* bytes_out);
 
 /*
  * Waits for `stream`, then reads and clears the status word at the start of a
