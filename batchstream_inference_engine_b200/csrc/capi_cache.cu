@@ -194,7 +194,7 @@ int plan_simt(const WindowShape& s, SimtPlan* p) {
 // Shapes the tensor-core kernels take (with 16-byte aligned pools and queries, and
 // outputs that their stores can address; see mma_pointers).
 bool mma_shape(const WindowShape& s) {
-  return !s.int4 && s.dtype == BS_BF16 && s.block_size % 16 == 0 && (s.head_dim == 64 || s.head_dim == 128);
+  return s.dtype == BS_BF16 && s.block_size % 16 == 0 && (s.head_dim == 64 || s.head_dim == 128);
 }
 
 // How the tensor-core decode runs a call: a cluster of segment_ctas CTAs per
@@ -222,13 +222,15 @@ int plan_mma_decode(const WindowShape& s, MmaDecodePlan* p) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   const int64_t groups = s.heads / s.kv_heads;
-  // Resident CTAs per SM by device, [head_dim 128][more than 8 heads a group].
-  static std::atomic<int> per_sm[64][2][2];
-  std::atomic<int>* known = dev < 64 ? &per_sm[dev][s.head_dim == 128][groups > 8] : nullptr;
+  // Resident CTAs per SM by device, [4-bit pools][head_dim 128][more than 8 heads a group].
+  static std::atomic<int> per_sm[64][2][2][2];
+  std::atomic<int>* known =
+      dev < 64 ? &per_sm[dev][s.int4][s.head_dim == 128][groups > 8] : nullptr;
   int ctas = known != nullptr ? known->load() : 0;
   if (ctas == 0) {
-    ctas = bsb::window_decode_mma_ctas_per_sm(static_cast<int>(s.head_dim),
-                                              static_cast<int>(groups));
+    const auto ctas_per_sm =
+        s.int4 ? bsb::decode_int4_ctas_per_sm : bsb::window_decode_mma_ctas_per_sm;
+    ctas = ctas_per_sm(static_cast<int>(s.head_dim), static_cast<int>(groups));
     if (ctas <= 0) return fail(BS_ERR_CUDA, "occupancy query for window decode failed (%d)", ctas);
     if (known != nullptr) known->store(ctas);
   }
@@ -304,11 +306,11 @@ int window_workspace(const WindowShape& s, uint64_t* bytes_out) {
   SimtPlan p;
   if (int rc = plan_simt(s, &p)) return rc;
   int64_t need = p.bytes;
-  if (mma_shape(s) && s.chunks) {
+  if (mma_shape(s) && s.chunks && !s.int4) {
     MmaChunkPlan m;
     if (int rc = plan_mma_chunks(s, &m)) return rc;
     need = std::max(need, m.bytes);
-  } else if (mma_shape(s)) {
+  } else if (mma_shape(s) && !s.chunks) {
     MmaDecodePlan m;
     if (int rc = plan_mma_decode(s, &m)) return rc;
     need = std::max(need, m.bytes);
@@ -358,9 +360,11 @@ int run_mma_decode(const WindowShape& s, const WindowCall& c) {
   if (int rc = plan_mma_decode(s, &p)) return rc;
   if (int rc = check_workspace(c, p.bytes)) return rc;
   CUtensorMap kmap, vmap;
-  const int64_t rows = s.kv_heads * c.num_blocks * s.block_size;
-  if (int rc = bsb::pool_tensor_map(&kmap, c.key_pool, rows, s.head_dim)) return rc;
-  if (int rc = bsb::pool_tensor_map(&vmap, c.value_pool, rows, s.head_dim)) return rc;
+  if (!s.int4) {
+    const int64_t rows = s.kv_heads * c.num_blocks * s.block_size;
+    if (int rc = bsb::pool_tensor_map(&kmap, c.key_pool, rows, s.head_dim)) return rc;
+    if (int rc = bsb::pool_tensor_map(&vmap, c.value_pool, rows, s.head_dim)) return rc;
+  }
   bsb::DecodeArgs a{};
   a.q = c.query;
   a.q_stride_seq = c.q_stride;
@@ -392,9 +396,14 @@ int run_mma_decode(const WindowShape& s, const WindowCall& c) {
   a.window = static_cast<int32_t>(std::min(s.window, kMaxContext));
   a.sinks = static_cast<int32_t>(std::min(s.sinks, kMaxContext));
   a.block_units = static_cast<int32_t>(s.block_size / bsb::kWindowUnit);
-  bsb::apply_wait_probe(a);
-  const int rc = bsb::launch_window_decode_mma(a, kmap, vmap, static_cast<int>(p.grid),
-                                               static_cast<cudaStream_t>(c.stream));
+  const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
+  int rc;
+  if (s.int4) {
+    rc = bsb::launch_decode_int4(a, static_cast<int>(p.grid), stream);
+  } else {
+    bsb::apply_wait_probe(a);
+    rc = bsb::launch_window_decode_mma(a, kmap, vmap, static_cast<int>(p.grid), stream);
+  }
   if (rc != 0) return cuda_fail(rc, "window decode launch");
   bsb::add_kernel_launches(p.segment_ctas > 0 ? 1 : 2);  // the decode and its merge pass
   return BS_OK;
@@ -475,7 +484,7 @@ int run_window(const WindowShape& s, const WindowCall& c) {
   a.status = c.status;
   // The tensor-core prefill compares scores before it scales them: it needs a
   // magnitude to scale by.
-  if (mma && a.scale != 0.f && std::isfinite(a.scale)) return run_mma_chunks(s, c, a);
+  if (mma && !s.int4 && a.scale != 0.f && std::isfinite(a.scale)) return run_mma_chunks(s, c, a);
 
   if (s.int4) {
     BS_CHECK(int4_aligned(c.key_pool, c.value_pool), "4-bit pools must be 4-byte aligned");

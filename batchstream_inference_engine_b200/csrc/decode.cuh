@@ -698,6 +698,9 @@ int decode_mma_ctas_per_sm(int head_dim, int groups);
 int launch_window_decode_mma(const DecodeArgs& a, const CUtensorMap& kmap,
                              const CUtensorMap& vmap, int grid, cudaStream_t stream);
 int window_decode_mma_ctas_per_sm(int head_dim, int groups);
+// The same over 4-bit pools (decode_int4.cu).
+int launch_decode_int4(const DecodeArgs& a, int grid, cudaStream_t stream);
+int decode_int4_ctas_per_sm(int head_dim, int groups);
 int launch_decode_simt(const DecodeArgs& a, int dtype_is_bf16, int grid, cudaStream_t stream);
 int decode_simt_ctas_per_sm(int head_dim, int groups, int dtype_is_bf16);
 

@@ -34,12 +34,11 @@
 // clusters of CTAs that join through distributed shared memory (join_segment): one
 // sequence of 77 tokens 5.4 us, by spans and their merge 10.1.  (A join whose reads
 // waited for one another, behind a chain of the warps' parts: 7.2 and 14.3.)
-#include "decode.cuh"
+#include "decode_join.cuh"
 
 namespace bsb {
 namespace {
 
-constexpr int kMaxRanks = 8;  // CTAs of a cluster
 constexpr int kBS = 16;  // tokens per block (fast path only)
 
 enum : int32_t { kFirst = 1, kLast = 2, kWhole = 4, kSlot1 = 8 };
@@ -80,87 +79,6 @@ struct Cfg {
   static_assert(SLOT_FLOATS * 4 <= S * STAGE_BYTES, "slot 1 must fit in the stages");
 };
 
-// The end of a cluster's segment (DecodeArgs::segment_ctas): every warp with units has
-// left its part (O, maxima, sums) in its slot 0.  The CTA joins its warps' parts, all
-// threads at once, then the cluster's CTAs each join a share of the elements over all
-// CTAs' parts, in rank order.  Every read of a join is issued before the first is used:
-// one trip through distributed shared memory costs some 250 ns.  A part without a finite
-// score has the maximum -inf and weighs 0, but is not left out: if its scores are NaN,
-// so are its O and sums, and 0 * NaN brings that to the output.
-template <typename C, int D>
-__device__ __forceinline__ void join_segment(const DecodeArgs& a, uint8_t* smem,
-                                             const int32_t (&slot_seq)[C::W][2], int32_t seq,
-                                             int32_t kvh, int32_t ranks) {
-  constexpr int W = C::W, kThreads = W * 32;
-  __shared__ float part_ml[2 * C::GROWS];
-  float* part = reinterpret_cast<float*>(smem);  // over the stages, whose copies are done
-  const int tid = threadIdx.x, G = a.groups;
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
-                       static_cast<int64_t>(seq) * a.o_stride_seq +
-                       static_cast<int64_t>(kvh) * G * D;
-  __syncthreads();
-  bool parked = ranks > 1;  // or one warp has written the output
-#pragma unroll
-  for (int w = 0; w < W; ++w) parked |= slot_seq[w][0] >= 0;
-  if (!parked) return;
-  for (int e = tid; e < G * D; e += kThreads) {
-    const int r = e / D;
-    float m[W], l[W], o[W], M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float* slot =
-          reinterpret_cast<const float*>(smem + W * C::S * C::STAGE_BYTES + w * C::SLOT0_BYTES);
-      const bool has = slot_seq[w][0] >= 0;
-      m[w] = has ? slot[G * D + r] : -INFINITY;
-      l[w] = has ? slot[G * D + G + r] : 0.f;
-      o[w] = has ? slot[e] : 0.f;
-      M = fmaxf(M, m[w]);
-    }
-    const float base = M == -INFINITY ? 0.f : M;
-    float L = 0.f, O = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float f = fast_exp2(m[w] - base);
-      L += f * l[w];
-      O += f * o[w];
-    }
-    if (ranks == 1) {
-      out[e] = __float2bfloat16_rn(O / L);
-    } else {
-      part[e] = O;
-      if (e % D == 0) {
-        part_ml[r] = M;
-        part_ml[C::GROWS + r] = L;
-      }
-    }
-  }
-  if (ranks == 1) return;
-  cluster_sync();
-  const int rank = blockIdx.x % a.segment_ctas;
-  for (int e = rank * kThreads + tid; e < G * D; e += ranks * kThreads) {
-    const int r = e / D;
-    float m[kMaxRanks], l[kMaxRanks], o[kMaxRanks], M = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kMaxRanks; ++k) {
-      m[k] = k < ranks ? cluster_load(part_ml, r, k) : -INFINITY;
-      l[k] = k < ranks ? cluster_load(part_ml, C::GROWS + r, k) : 0.f;
-      o[k] = k < ranks ? cluster_load(part, e, k) : 0.f;
-    }
-#pragma unroll
-    for (int k = 0; k < kMaxRanks; ++k) M = fmaxf(M, m[k]);
-    const float base = M == -INFINITY ? 0.f : M;
-    float L = 0.f, O = 0.f;
-#pragma unroll
-    for (int k = 0; k < kMaxRanks; ++k) {
-      const float f = fast_exp2(m[k] - base);
-      L += f * l[k];
-      O += f * o[k];
-    }
-    out[e] = __float2bfloat16_rn(O / L);
-  }
-  cluster_sync();  // the others may still read this CTA's shared memory
-}
-
 template <int D, bool G16, bool WIN>
 __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
     decode_mma_kernel(const __grid_constant__ CUtensorMap kmap,
@@ -172,8 +90,7 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
   __shared__ TileMeta meta[W][S];
   __shared__ ScanSmem scan;
   __shared__ WarpStarts starts;
-  __shared__ int32_t slot_seq[W][2], slot_kvh[W][2], slot_nb[W][2];
-  __shared__ int64_t slot_unit[W][2];
+  __shared__ WarpSlots<W> slots;
   // Segments whose last record this CTA wrote: merged by the whole CTA.
   __shared__ int32_t fin_count;
   __shared__ MergeTask task;  // the cut segment this CTA finishes (tasks mode)
@@ -184,10 +101,6 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
   uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto stages_of = [&](int w) { return smem + w * S * C::STAGE_BYTES; };
-  auto slot_of = [&](int w, int k) {
-    return reinterpret_cast<float*>(k == 0 ? smem + W * S * C::STAGE_BYTES + w * C::SLOT0_BYTES
-                                           : stages_of(w));
-  };
   uint8_t* wst = stages_of(warp);
 
   if (tid == 0) {
@@ -197,7 +110,7 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
   }
-  if (tid < W * 2) slot_seq[tid / 2][tid % 2] = -1;
+  if (tid < W * 2) slots.seq[tid / 2][tid % 2] = -1;
   if (tid == 0) {
     fin_count = 0;
     task.valid = 0;
@@ -610,7 +523,7 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
       } else {
         // A cut portion: park it in slot 0 (first portion) or slot 1 (last).
         const int k = (mt.flags & kSlot1) ? 1 : 0;
-        float* slot = slot_of(warp, k);
+        float* slot = warp_slot<C>(smem, warp, k);
 #pragma unroll
         for (int hr = 0; hr < (G16 ? 2 : 1); ++hr) {
           const int r = g + 8 * hr;
@@ -627,10 +540,10 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
           }
         }
         if (lane == 0) {
-          slot_seq[warp][k] = mt.seq;
-          slot_kvh[warp][k] = mt.kvh;
-          slot_nb[warp][k] = mt.nb;
-          slot_unit[warp][k] = mt.seg_unit;
+          slots.seq[warp][k] = mt.seq;
+          slots.kvh[warp][k] = mt.kvh;
+          slots.nb[warp][k] = mt.nb;
+          slots.unit[warp][k] = mt.seg_unit;
         }
       }
     }
@@ -638,95 +551,17 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
 
   if constexpr (WIN) {
     if (clustered) {
-      join_segment<C, D>(a, smem, slot_seq, own_seq, own_kvh, ranks);
+      join_segment<C, D>(a, smem, slots, own_seq, own_kvh, ranks);
       return;
     }
   }
 
   // ---------------------------------------------------------------- CTA merge
-  // A segment cut between warps is a chain: the last portion of the warp where
-  // it starts, the only portion of warps inside it, the first portion of the
-  // warp where it ends.  The chain's tail (no later non-empty warp continues the
-  // segment) folds the earlier slots into its own and finishes the segment.
-  __syncthreads();
-  auto warp_empty = [&](int w) {
-    return sp.r0 + spanw * (w + 1) / W == sp.r0 + spanw * w / W;
-  };
-  auto holds = [&](int w, int k, int32_t seq, int32_t kvh) {
-    return slot_seq[w][k] == seq && slot_kvh[w][k] == kvh;
-  };
-  for (int k = 0; k < 2; ++k) {
-    const int32_t seq = slot_seq[warp][k];
-    if (seq < 0) continue;
-    const int32_t kvh = slot_kvh[warp][k];
-    bool tail = true;
-    if (k == 1 || slot_seq[warp][1] < 0) {
-      for (int w2 = warp + 1; w2 < W; ++w2) {
-        if (warp_empty(w2)) continue;
-        tail = !holds(w2, 0, seq, kvh);
-        break;
-      }
-    }
-    if (!tail) continue;
-    float* mine = slot_of(warp, k);
-    for (int w2 = warp - 1; w2 >= 0; --w2) {
-      if (warp_empty(w2)) continue;
-      const int k2 = holds(w2, 1, seq, kvh) ? 1 : (holds(w2, 0, seq, kvh) ? 0 : -1);
-      if (k2 < 0) break;
-      const float* other = slot_of(w2, k2);
-      // Row factors once (lane r < G), then one FMA pair per element; a row
-      // spans D >= 64 elements, so elements e = lane + 32j share row (32j) / D.
-      float fa = 0.f, fb = 0.f;
-      if (lane < G) {
-        const float ma = mine[G * D + lane], mb = other[G * D + lane];
-        const float M = fmaxf(ma, mb);
-        const float base = M == -INFINITY ? 0.f : M;  // neither has a finite score
-        fa = fast_exp2(ma - base);
-        fb = fast_exp2(mb - base);
-        mine[G * D + G + lane] = mine[G * D + G + lane] * fa + other[G * D + G + lane] * fb;
-        mine[G * D + lane] = M;
-      }
-      // Compile-time bounds (rows padded to GROWS): the loads of all elements
-      // issue back to back instead of one dependent step at a time.
-#pragma unroll
-      for (int j = 0; j < C::GROWS * D / 32; ++j) {
-        const int r = (32 * j) / D;
-        const float a0 = __shfl_sync(0xffffffffu, fa, r);
-        const float b0 = __shfl_sync(0xffffffffu, fb, r);
-        const int e = lane + 32 * j;
-        if (r < G) mine[e] = mine[e] * a0 + other[e] * b0;
-      }
-      __syncwarp();
-      if (k2 == 1) break;  // the chain starts in that warp
-    }
-    const int64_t seg_unit = slot_unit[warp][k];
-    const int32_t nb = slot_nb[warp][k];
-    if (seg_unit >= sp.r0 && seg_unit + nb <= sp.r1) {
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
-                           static_cast<int64_t>(seq) * a.o_stride_seq +
-                           static_cast<int64_t>(kvh) * G * D;
-      const float inv_l = lane < G ? 1.f / mine[G * D + G + lane] : 0.f;
-#pragma unroll
-      for (int j = 0; j < C::GROWS * D / 32; ++j) {
-        const int r = (32 * j) / D;
-        const float inv = __shfl_sync(0xffffffffu, inv_l, r);
-        const int e = lane + 32 * j;
-        if (r < G) out[e] = __float2bfloat16_rn(mine[e] * inv);
-      }
-    } else if (a.tasks != nullptr) {
-      // Cut across CTAs: leave this CTA's record; the segment is merged after
-      // the kernel, listed by the CTA that holds its last unit.
-      warp_store_record_fixed<C::GROWS, D>(a, sp, seg_unit, mine, mine + G * D,
-                                           mine + G * D + G, lane);
-      if (lane == 0 && seg_unit < sp.r0 && seg_unit + nb <= sp.r1) {
-        task.seg_unit = seg_unit;
-        task.q = sp.q;
-        task.rem = sp.rem;
-        task.seq = seq;
-        task.kvh = kvh;
-        task.nb = nb;
-        task.valid = 1;
-      }
+  fold_slots<C, D>(a, smem, sp, spanw, slots, [&](int32_t seq, int32_t kvh, int64_t seg_unit,
+                                                  int32_t nb, const float* mine) {
+    if (a.tasks != nullptr) {
+      // Leave this CTA's record; the segment is merged after the kernel.
+      record_cut<C, D>(a, sp, seq, kvh, seg_unit, nb, mine, task);
     } else if (warp_write_record(a, sp, seq, kvh, seg_unit, nb, mine, mine + G * D,
                                  mine + G * D + G, lane)) {
       if (lane == 0) {
@@ -737,7 +572,7 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
         fin_unit[idx] = seg_unit;
       }
     }
-  }
+  });
   // Segments crossing CTAs for which this CTA came last: merge with all threads.
   // The stages and slots are free now and serve as scratch.
   __syncthreads();
@@ -810,10 +645,8 @@ int occupancy_one() {
 
 }  // namespace
 
-namespace {
-
-// The merge pass of either form: at most `grid` records per segment.
-int launch_merge(const DecodeArgs& a, int grid, cudaStream_t stream) {
+// The merge pass of every form: at most `grid` records per segment.
+int launch_decode_merge(const DecodeArgs& a, int grid, cudaStream_t stream) {
   const int smem = static_cast<int>((2 * static_cast<int64_t>(grid) * a.groups + 2 * a.groups) *
                                     sizeof(float));
   // Room for 16 heads a group and 700 CTAs; the grids hold at most three an SM.
@@ -837,6 +670,8 @@ int launch_merge(const DecodeArgs& a, int grid, cudaStream_t stream) {
   return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_merge_kernel, a));
 }
 
+namespace {
+
 template <bool WIN>
 int launch_both(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap& vmap, int grid,
                 cudaStream_t stream) {
@@ -849,7 +684,7 @@ int launch_both(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap&
     rc = g16 ? launch_one<128, true, WIN>(a, kmap, vmap, grid, stream)
              : launch_one<128, false, WIN>(a, kmap, vmap, grid, stream);
   if (rc != 0 || a.tasks == nullptr) return rc;
-  return launch_merge(a, grid, stream);
+  return launch_decode_merge(a, grid, stream);
 }
 
 template <bool WIN>
