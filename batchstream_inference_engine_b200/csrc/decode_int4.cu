@@ -4,71 +4,112 @@
 //
 // The batch's units of 16 tokens are shared out as in decode_mma.cu: equal spans over the
 // batch, or clusters per segment for few segments, with the same joins (decode_join.cuh).  A
-// warp works through its span on its own, in steps of up to UNITS units of one segment; its
-// lanes copy a step's codes and scales into a ring of S stages (cp.async, 16 bytes a lane),
-// with the table entries of the step after it already on their way.
+// warp works through its span on its own, a unit at a time; its lanes copy a unit's codes and
+// scales into a ring of S stages (cp.async, 16 bytes a lane), with the table entries of up to
+// 32 units in a register of each lane and those of the next already on their way.
 //
 // The codes never pass through shared memory as bf16: they become the products' operands in
 // registers, in the order in which the products take them,
-//     S = Q K^T    Q the rows (16, the group's heads), K's codes the columns' operand: a lane
-//                  takes the same quarter of the dims of one key per 8 keys, whatever their
-//                  groups, and the query's fragments are laid out alike;
-//     O^T = V^T P^T    V^T the rows' operand: one ldmatrix.trans brings a lane the codes of 4
-//                  dims for two neighbouring keys in one register, so a shift and a mask leave
-//                  the pair of one dim; P^T is S's accumulator as it is.
-// A register of two values costs a shift (three of four), a mask and a fused multiply-add, 11
-// instructions for 8 elements; all else together is less.  Stages are swizzled so that
-// neither operand's loads meet in a bank.
+//     S^T = K Q^T    K the rows' operand (16 keys): a lane takes the same quarter of the dims
+//                    of two keys, whatever their groups, and the query's fragments are laid
+//                    out alike;
+//     O^T = V^T P^T  V^T the rows' operand: one ldmatrix.trans brings a lane the codes of 4
+//                    dims for two neighbouring keys in one register, so a shift and a mask
+//                    leave the pair of one dim; P^T is S^T, its 8 x 8 tiles transposed.
+// So no row of either product is padding for up to 8 heads, and the softmax's factors belong
+// to O's columns as they are.  A register of two values costs a shift (three of four), a mask
+// and a fused multiply-add, 11 instructions for 8 elements; all else together is less.  Stages
+// are swizzled so that neither operand's loads meet in a bank.
+//
+// Scores are weighed against a maximum that moves only when one is more than 2^8 above it
+// (then all lanes find the new one and O is scaled): most units need no reduction.
 #include "decode_join.cuh"
 #include "int4.cuh"
 
 namespace bsb {
 namespace {
 
-enum : int32_t { kFirst = 1, kLast = 2, kWhole = 4, kSlot1 = 8, kCount = 16 };  // units from bit 4
+// Of a step (4 bits): there is one; a portion's first or last one; it has all its units and
+// their tokens are all visible.
+enum : uint32_t { kFirst = 1, kLast = 2, kFull = 4, kStep = 8 };
+// Of a portion: the segment is all the warp's; it goes to slot 1.
+enum : int32_t { kWhole = 1, kSlot1 = 2 };
+constexpr float kSlack = 8.f;  // how far above the maximum a score may be, base 2
+constexpr float kNoScore = -3.402823466e38f;  // the maximum before any score: no finite one is below
 
 template <int D, bool G16>
 struct Cfg {
-  static constexpr int W = 4;      // warps per CTA
-  static constexpr int S = 2;      // stages per warp
-  static constexpr int UNITS = 2;  // units of a step
-  static constexpr int MIN_CTAS = 3;
+  static constexpr int W = 4;                    // warps per CTA
+  static constexpr int U = 2;                    // units of a step
+  static constexpr int S = D == 64 ? 4 : 3;      // stages per warp, a step each
+  static constexpr int MIN_CTAS = D == 64 ? (G16 ? 3 : 4) : (G16 ? 2 : 3);
   static constexpr int GROWS = G16 ? 16 : 8;
   static constexpr int CODE_BYTES = kWindowUnit * D / 2;  // of a unit, K or V
   static constexpr int SCALE_BYTES = kWindowUnit * D / 16;
-  static constexpr int Q_BYTES = GROWS * D * 2;
-  // K codes | V codes | K scales | V scales, each of all units; the query.
-  static constexpr int V_OFF = UNITS * CODE_BYTES;
-  static constexpr int KS_OFF = 2 * UNITS * CODE_BYTES;
-  static constexpr int VS_OFF = KS_OFF + UNITS * SCALE_BYTES;
-  static constexpr int Q_OFF = VS_OFF + UNITS * SCALE_BYTES;
-  static constexpr int STAGE_BYTES = Q_OFF + Q_BYTES;
+  // A unit in a stage: K codes | V codes | K scales | V scales.
+  static constexpr int KS_OFF = 2 * CODE_BYTES;
+  static constexpr int VS_OFF = KS_OFF + SCALE_BYTES;
+  static constexpr int UNIT_BYTES = VS_OFF + SCALE_BYTES;
+  static constexpr int STAGE_BYTES = U * UNIT_BYTES;
   static constexpr int SLOT_FLOATS = GROWS * D + 2 * GROWS;
   static constexpr int SLOT0_BYTES = (SLOT_FLOATS * 4 + 127) / 128 * 128;
   static constexpr int SMEM_BYTES = W * S * STAGE_BYTES + W * SLOT0_BYTES;
   static_assert(STAGE_BYTES % 128 == 0, "stages stay 128-byte aligned");
   static_assert(SLOT_FLOATS * 4 <= S * STAGE_BYTES, "slot 1 must fit in the stages");
+  static_assert(S <= 8, "a stage has 4 bits of the flags");
 };
 
-// What a stage holds.
-template <int UNITS>
-struct StepMeta {
+// Whose a run of units is.
+struct Owner {
   int32_t seq, kvh, nb, flags;
   int64_t seg_unit;
-  int32_t map[UNITS];  // visible tokens of each unit
+};
+
+// What a stage holds: the visible tokens of a step that does not show them all (16 bits a
+// unit), and whose it is of a portion's first and last ones.
+struct StepMeta {
+  uint32_t map;
+  Owner owner;
+};
+
+// Up to 32 consecutive units of a segment, one per lane.
+struct Run {
+  int32_t n;
+  uint32_t flags;  // kFirst, kLast: a portion's first, its last units
+  int32_t blk;       // this lane's: block-table entry, unit of its block, visible tokens
+  int32_t in_block, map;
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
+// The 8 x 8 tile of 16-bit elements that a warp holds, a row to four lanes, transposed.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// D = A * B, as mma_bf16_16816.
+__device__ __forceinline__ void mma_zero_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                               uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 template <int D, bool G16>
 __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kernel(const DecodeArgs a) {
   using C = Cfg<D, G16>;
-  constexpr int W = C::W, S = C::S, UNITS = C::UNITS;
+  constexpr int W = C::W, S = C::S, U = C::U;
   constexpr int NG = D / kInt4Group;  // groups of a row
+  constexpr int NQ = G16 ? 2 : 1;     // tiles of 8 query heads
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ StepMeta<UNITS> meta[W][S];
+  __shared__ StepMeta meta[W][S];
+  __shared__ Owner owners[W][2];  // of the current run and the one behind it
   __shared__ ScanSmem scan;
   __shared__ WarpStarts starts;
   __shared__ WarpSlots<W> slots;
@@ -100,107 +141,62 @@ __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kern
   const int64_t wr0 = sp.r0 + spanw * warp / W;
   const int64_t wr1 = sp.r0 + spanw * (warp + 1) / W;
 
-  // ---------------------------------------------------------------- issue cursor
-  // The next step: its sequence, kv head and first unit.  All lanes keep identical copies.
+  // ---------------------------------------------------------------- fetch cursor
+  // The next run's sequence, kv head and first unit.  All lanes keep identical copies.
   int32_t ci = starts.seq[warp];
   int64_t cprefix = starts.prefix[warp];
   int32_t clen = 0, crow = 0, cnb = 0, ch = 0, cb = 0;
   int32_t nxt_len = 0, nxt_row = 0;
-  int64_t cu = wr0;
-  WindowUnits cw{};
-  if (wr1 > wr0) {
+  int32_t togo = static_cast<int32_t>(wr1 - wr0);  // units that are not in a run yet
+  bool begins = true;                              // the next run is its portion's first
+  int parity = 0;
+  if (togo > 0) {
     cnb = units_of<true>(a, starts.len[warp], starts.row[warp], clen, crow);
-    cw = window_units(a, clen);
     const int64_t rel = wr0 - cprefix * Hkv;
     ch = static_cast<int32_t>(rel / cnb);
     cb = static_cast<int32_t>(rel % cnb);
     nxt_len = starts.nlen[warp];
     nxt_row = starts.nrow[warp];
   }
-  const int64_t block_bytes = static_cast<int64_t>(a.block_size) * int4_row_bytes(D);
-  const int32_t scales_at = a.block_size * int4_code_bytes(D);  // of a block
-
-  // The step prepared last: lane u < UNITS has unit u's token unit and table entry.
-  int32_t step_units = 0, step_tu = 0, step_blk = -1;
-  auto prepare = [&]() {
-    step_units = static_cast<int32_t>(min(static_cast<int64_t>(min(UNITS, cnb - cb)), wr1 - cu));
-    if (step_units <= 0) {
-      step_units = 0;
-      return;
+  // Loads the next run's table entries and moves the cursor past it.
+  auto fetch = [&]() {
+    Run r{};
+    r.n = min(min(32, cnb - cb), togo);
+    if (r.n <= 0) {
+      r.n = 0;
+      return r;
     }
-    if (lane < step_units) {
-      const int32_t x = cb + lane;
-      step_tu = x < cw.sink_units ? x : x - cw.sink_units + cw.first_unit;
-      step_blk = __ldg(a.block_tables + static_cast<int64_t>(crow) * a.bt_stride +
-                       (a.block_units == 1 ? step_tu : step_tu / a.block_units));
+    const WindowUnits cw = window_units(a, clen);
+    const int32_t x = cb + lane;
+    const int32_t tu = x < cw.sink_units ? x : x - cw.sink_units + cw.first_unit;
+    r.blk = -1;
+    if (lane < r.n) {
+      const int32_t ent = a.block_units == 1 ? tu : tu / a.block_units;
+      r.in_block = tu - ent * a.block_units;
+      r.blk = __ldg(a.block_tables + static_cast<int64_t>(crow) * a.bt_stride + ent);
     }
-  };
-  // Starts the prepared step's copies into a stage and prepares the one after.
-  auto issue = [&](int stage) {
-    if (step_units == 0) return;
-    const int32_t n = step_units;
-    const uint32_t dst = smem_u32(wst + stage * C::STAGE_BYTES);
-    const int64_t seg_unit = cprefix * Hkv + static_cast<int64_t>(ch) * cnb;
-    const bool first = cu == wr0 || cb == 0;
-    StepMeta<UNITS>& m = meta[warp][stage];
+    const int32_t tok0 = tu * kWindowUnit, lo = clen - a.window;
+    auto below = [](int32_t c) {  // map of a unit's first c tokens
+      return c >= kWindowUnit ? 0xffff : c <= 0 ? 0 : (1 << c) - 1;
+    };
+    r.map = below(clen - tok0) & (~below(lo - tok0) | below(a.sinks - tok0));
+    togo -= r.n;
+    cb += r.n;
+    const bool ends = togo == 0 || cb == cnb;
+    r.flags = (begins ? kFirst : 0u) | (ends ? kLast : 0u);
     if (lane == 0) {
-      const bool last = cu + n == wr1 || cb + n == cnb;
-      const bool whole = seg_unit >= wr0 && seg_unit + cnb <= wr1 && !(clustered && ranks > 1);
-      m.seq = ci;
-      m.kvh = ch;
-      m.nb = cnb;
-      m.seg_unit = seg_unit;
-      m.flags = (first ? kFirst : 0) | (last ? kLast : 0) | (whole ? kWhole : 0) |
-                (seg_unit > wr0 ? kSlot1 : 0) | n * kCount;
+      const int64_t seg_unit = cprefix * Hkv + static_cast<int64_t>(ch) * cnb;
+      Owner& w = owners[warp][parity];
+      w.seq = ci;
+      w.kvh = ch;
+      w.nb = cnb;
+      w.seg_unit = seg_unit;
+      w.flags = (seg_unit >= wr0 && seg_unit + cnb <= wr1 && !(clustered && ranks > 1) ? kWhole : 0) |
+                (seg_unit > wr0 ? kSlot1 : 0);
     }
-    if (lane < n) {
-      const bool valid = step_blk >= 0 && step_blk < a.num_blocks;
-      if (!valid) set_status(a.status, kStatusBadBlock);
-      const int32_t tok0 = step_tu * kWindowUnit, lo = clen - a.window;
-      auto below = [](int32_t c) {  // map of a unit's first c tokens
-        return c >= kWindowUnit ? 0xffff : c <= 0 ? 0 : (1 << c) - 1;
-      };
-      m.map[lane] = valid ? below(clen - tok0) & (~below(lo - tok0) | below(a.sinks - tok0)) : 0;
-      if (!valid) step_blk = -1;
-    }
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int32_t blk = __shfl_sync(0xffffffffu, step_blk, u);
-      const int32_t tu = __shfl_sync(0xffffffffu, step_tu, u);
-      if (u >= n || blk < 0) continue;
-      const int32_t tok = a.block_units == 1 ? 0 : tu % a.block_units * kWindowUnit;
-      const int64_t block =
-          (static_cast<int64_t>(ch) * a.num_blocks + blk) * block_bytes;
-      const uint8_t* k = static_cast<const uint8_t*>(a.k_pool) + block;
-      const uint8_t* v = static_cast<const uint8_t*>(a.v_pool) + block;
-      // 16-byte piece c of row r lies at piece c ^ f(r) of its row: 8 rows of one piece, and 8
-      // neighbouring pieces, are then in different banks.
-#pragma unroll
-      for (int i = 0; i < C::CODE_BYTES / 512; ++i) {
-        const int id = lane + 32 * i;
-        const int r = id / (D / 32), c = id % (D / 32);
-        const uint32_t at = r * (D / 2) + ((D == 128 ? c ^ ((r >> 1) & 3) : c ^ ((r >> 2) & 1)) << 4);
-        const int32_t from = tok * int4_code_bytes(D) + id * 16;
-        copy16(dst + u * C::CODE_BYTES + at, k + from);
-        copy16(dst + C::V_OFF + u * C::CODE_BYTES + at, v + from);
-      }
-      constexpr int kPieces = C::SCALE_BYTES / 16;
-      if (lane < 2 * kPieces) {
-        const int c = lane % kPieces;
-        copy16(dst + (lane < kPieces ? C::KS_OFF : C::VS_OFF) + u * C::SCALE_BYTES + c * 16,
-               (lane < kPieces ? k : v) + scales_at + tok * int4_scale_bytes(D) + c * 16);
-      }
-    }
-    if (first) {
-      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) +
-                               static_cast<int64_t>(ci) * a.q_stride_seq +
-                               static_cast<int64_t>(ch) * G * D;
-      for (int e = lane; e < G * D / 8; e += 32) copy16(dst + C::Q_OFF + e * 16, q + e * 8);
-    }
-    // On to the next step.
-    cu += n;
-    cb += n;
-    if (cu < wr1 && cb == cnb) {
+    parity ^= 1;
+    begins = ends;
+    if (togo > 0 && cb == cnb) {
       cb = 0;
       if (++ch == Hkv) {
         ch = 0;
@@ -211,274 +207,371 @@ __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kern
           ++ci;
           cnb = ci < a.num_seqs ? seq_units<true>(a, ci, clen, crow, false) : 1;
         }
-        cw = window_units(a, max(clen, 0));
         if (ci + 1 < a.num_seqs) {
           nxt_len = __ldg(a.context_lens + ci + 1);
           nxt_row = a.seq_rows != nullptr ? __ldg(a.seq_rows + ci + 1) : ci + 1;
         }
       }
     }
-    prepare();
+    return r;
   };
 
-  prepare();
+  // ---------------------------------------------------------------- issue
+  const int32_t block_bytes = a.block_size * int4_row_bytes(D);  // fits (host)
+  const int32_t scales_at = a.block_size * int4_code_bytes(D);   // of a block
+  const int64_t head_bytes = static_cast<int64_t>(a.num_blocks) * block_bytes;
+  // This lane's pieces of a unit: where they are in a block and in a stage.  16-byte piece c
+  // of row r lies at piece c ^ f(r) of its row: 8 rows of one piece, and 8 neighbouring
+  // pieces, are then in different banks.
+  const int lr = lane / (D / 32), lc = lane % (D / 32);
+  const uint32_t piece_at =
+      lr * (D / 2) + ((D == 128 ? lc ^ ((lr >> 1) & 3) : lc ^ ((lr >> 2) & 1)) << 4);
+  constexpr int kScalePieces = C::SCALE_BYTES / 16;
+  const uint8_t* const k_codes = static_cast<const uint8_t*>(a.k_pool) + lane * 16;
+  const uint8_t* const v_codes = static_cast<const uint8_t*>(a.v_pool) + lane * 16;
+  const uint8_t* const scales = static_cast<const uint8_t*>(lane < kScalePieces ? a.k_pool : a.v_pool) +
+                                scales_at + (lane % kScalePieces) * 16;  // K's lanes, V's lanes
+
+  Run cur = fetch(), nxt{};
+  int32_t idx = 0;     // next unit of the current run: it and the one behind it are a step
+  uint32_t full = 0;   // its units whose tokens are all visible
+  int64_t head_at = 0;
+  const Owner* owner = nullptr;
+  auto begin_run = [&]() {
+    if (cur.n == 0) return;
+    const bool valid = cur.blk >= 0 && cur.blk < a.num_blocks;
+    if (lane < cur.n && !valid) set_status(a.status, kStatusBadBlock);
+    if (!valid) cur.blk = cur.map = 0;  // any block will do: none of its tokens counts
+    full = __ballot_sync(0xffffffffu, lane < cur.n && cur.map == 0xffff);
+    owner = &owners[warp][parity ^ 1];
+    const int32_t kvh = owner->kvh;
+    head_at = kvh * head_bytes;
+    if (cur.flags & kFirst) {  // the query will be wanted: into L1
+      const char* q = reinterpret_cast<const char*>(
+          static_cast<const __nv_bfloat16*>(a.q) +
+          static_cast<int64_t>(owner->seq) * a.q_stride_seq + static_cast<int64_t>(kvh) * G * D);
+      if (lane * 128 < G * D * 2) asm volatile("prefetch.global.L1 [%0];" ::"l"(q + lane * 128));
+    }
+    idx = 0;
+    nxt = fetch();
+  };
+  __syncwarp();
+  begin_run();
+  // Starts the next step's copies into the stage at `dst` and returns its flags.
+  auto issue = [&](uint32_t dst, int stage) -> uint32_t {
+    uint32_t flags = 0;
+    if (cur.n != 0) {
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    issue(s);
+      for (int u = 0; u < U; ++u) {
+        const int from = min(idx + u, cur.n - 1);  // (a step past the end repeats the last unit)
+        const int32_t blk = __shfl_sync(0xffffffffu, cur.blk, from);
+        int64_t at = head_at + static_cast<int64_t>(blk) * block_bytes, scales_from = at;
+        if (a.block_units != 1) {
+          const int32_t tok = __shfl_sync(0xffffffffu, cur.in_block, from) * kWindowUnit;
+          at += tok * int4_code_bytes(D);
+          scales_from += tok * int4_scale_bytes(D);
+        }
+        const uint8_t* k = k_codes + at;
+        const uint8_t* v = v_codes + at;
+        const uint32_t to = dst + u * C::UNIT_BYTES;
+#pragma unroll
+        for (int i = 0; i < C::CODE_BYTES / 512; ++i) {  // (8 rows on: the same swizzle)
+          copy16(to + piece_at + i * 512, k + i * 512);
+          copy16(to + piece_at + C::CODE_BYTES + i * 512, v + i * 512);
+        }
+        if (lane < 2 * kScalePieces) copy16(to + lane * 16 + C::KS_OFF, scales + scales_from);
+      }
+      const uint32_t every = (1u << U) - 1u;
+      flags = kStep | (((full >> idx) & every) == every ? kFull : 0u);
+      if (idx == 0) flags |= cur.flags & kFirst;
+      if (idx + U >= cur.n) flags |= cur.flags & kLast;
+      if (flags != (kStep | kFull)) {
+        uint32_t seen = __shfl_sync(0xffffffffu, cur.map, idx);
+        const uint32_t second = __shfl_sync(0xffffffffu, cur.map, idx + 1);
+        if (idx + 1 < cur.n) seen |= second << 16;
+        if (lane == 0) {
+          StepMeta& m = meta[warp][stage];
+          m.map = seen;
+          if (flags & (kFirst | kLast)) m.owner = *owner;
+        }
+        __syncwarp();  // the owner has been read
+      }
+      idx += U;
+      if (idx >= cur.n) {
+        cur = nxt;
+        begin_run();
+      }
+    }
     asm volatile("cp.async.commit_group;" ::: "memory");
-  }
+    return flags;
+  };
 
   // ---------------------------------------------------------------- compute
   const int g = lane >> 2, t = lane & 3;
-  constexpr int WORDS = D / 32;  // words of codes a lane takes of a key
-  uint32_t qa[WORDS][4], qb[G16 ? WORDS : 1][4];  // query rows g, g + 8
-  float o[NG][2][4], o2[G16 ? NG : 1][2][4];      // O^T of query columns 0 .. 7, 8 .. 15
-  float m2[2] = {-INFINITY, -INFINITY}, lsum[2] = {0.f, 0.f};
+  constexpr int WORDS = D / 32;     // words of codes a lane takes of a key
+  uint32_t qf[NQ][WORDS][4];        // query rows g, g + 8: lane t's quarter of the dims
+  float o[NQ][NG][2][4];            // O^T, columns 2t, 2t + 1 (+ 8)
+  float m2[NQ][2], lsum[NQ][2];     // of the same columns
   const float zscale = a.scale * kLog2e;
-  int32_t left = static_cast<int32_t>(wr1 - wr0);
+  const uint32_t ring = smem_u32(wst);
+  uint32_t queue = 0;  // flags of the steps in the stages, the oldest in the lowest bits
+  // Of a unit's part of a stage, this lane's: K codes, K scale, V codes (as ldmatrix wants
+  // them), V scales.
+  const uint32_t k_at = g * (D / 2) + (D == 128 ? (t ^ ((g >> 1) & 3)) << 4
+                                                : (((t >> 1) ^ ((g >> 2) & 1)) << 4) + (t & 1) * 8);
+  const uint32_t ks_at = C::KS_OFF + (g * NG + (D == 128 ? t : t >> 1)) * 2;
+  const int vr = 8 * ((lane >> 3) & 1) + (lane & 7);
+  const uint32_t v_at = C::CODE_BYTES + vr * (D / 2) +
+                        (((lane >> 4) ^ (D == 128 ? (vr >> 1) & 3 : (vr >> 2) & 1)) << 4);
+  const uint32_t vs_at = C::VS_OFF + 2 * t * (NG * 2);
 
-  for (int stage = 0; left > 0; stage = stage + 1 == S ? 0 : stage + 1) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
-    __syncwarp();
-    const StepMeta<UNITS>& mt = meta[warp][stage];
-    const int32_t flags = mt.flags, n = flags / kCount;
-    const uint8_t* st = wst + stage * C::STAGE_BYTES;
-    const uint32_t base = smem_u32(st);
-    left -= n;
-    if (flags & kFirst) {
-      m2[0] = m2[1] = -INFINITY;
-      lsum[0] = lsum[1] = 0.f;
+  // The first S turns only fill the stages.
+  int stage = 0;
+#pragma unroll 1
+  for (int it = -S;; it = min(it + 1, 0)) {
+    const uint32_t base = ring + stage * C::STAGE_BYTES;
+    if (it >= 0) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+      __syncwarp();
+      const uint32_t flags = queue & 15u;
+      if (flags == 0) break;
+      const StepMeta& mt = meta[warp][stage];
+      float bias[U][2];  // of keys g, g + 8 of each unit: -inf where the token is not seen
 #pragma unroll
-      for (int q = 0; q < NG; ++q) {
+      for (int u = 0; u < U; ++u) bias[u][0] = bias[u][1] = 0.f;
+      if (flags != (kStep | kFull)) {
+        if (flags & kFirst) {
+          const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) +
+                                   static_cast<int64_t>(mt.owner.seq) * a.q_stride_seq +
+                                   static_cast<int64_t>(mt.owner.kvh) * G * D + t * (D / 4);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+          for (int h = 0; h < NQ; ++h) {
+            m2[h][0] = m2[h][1] = kNoScore;
+            lsum[h][0] = lsum[h][1] = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            o[q][j][e] = 0.f;
-            if (G16) o2[q][j][e] = 0.f;
+            for (int x = 0; x < NG; ++x) {
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[h][x][j][e] = 0.f;
+              }
+            }
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) {
+              uint4 x = make_uint4(0u, 0u, 0u, 0u);
+              if (g + 8 * h < G) x = *reinterpret_cast<const uint4*>(q + (g + 8 * h) * D + w * 8);
+              qf[h][w][0] = x.x;
+              qf[h][w][1] = x.y;
+              qf[h][w][2] = x.z;
+              qf[h][w][3] = x.w;
+            }
           }
         }
-      }
-      // Lane t's dims: a quarter of the row's.
+        if (!(flags & kFull)) {
+          // Unseen tokens: their codes may be stale, their scales NaN; with scales of 0 they
+          // are 0.
+          const uint32_t seen = mt.map;
 #pragma unroll
-      for (int w = 0; w < WORDS; ++w) {
-        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-        const uint4* src = reinterpret_cast<const uint4*>(st + C::Q_OFF) + t * WORDS + w;
-        const uint4 x = g < G ? src[g * (D / 8)] : zero;
-        qa[w][0] = x.x; qa[w][1] = x.y; qa[w][2] = x.z; qa[w][3] = x.w;
-        if (G16) {
-          const uint4 y = g + 8 < G ? src[(g + 8) * (D / 8)] : zero;
-          qb[w][0] = y.x; qb[w][1] = y.y; qb[w][2] = y.z; qb[w][3] = y.w;
+          for (int u = 0; u < U; ++u) {
+            uint16_t* scale = reinterpret_cast<uint16_t*>(wst + stage * C::STAGE_BYTES +
+                                                          u * C::UNIT_BYTES + C::KS_OFF);
+            for (int e = lane; e < 2 * kWindowUnit * NG; e += 32) {
+              if (!((seen >> (16 * u + e / NG % kWindowUnit)) & 1)) scale[e] = 0;
+            }
+            if (!((seen >> (16 * u + g)) & 1)) bias[u][0] = -INFINITY;
+            if (!((seen >> (16 * u + g + 8)) & 1)) bias[u][1] = -INFINITY;
+          }
+          __syncwarp();
         }
       }
-    }
-    // S = Q K^T, 8 keys at a time.
-    float s[2 * UNITS][4];
-    bool all = true;
+      // S^T = K Q^T: keys g and g + 8 of each unit, in two chains.
+      float s[U][NQ][4];
+      float above = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
+      for (int u = 0; u < U; ++u) {
+        const uint32_t unit = base + u * C::UNIT_BYTES;
+        uint32_t kw[2][WORDS], ks[2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float(&acc)[4] = s[2 * u + j];
-        acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
-        if (u >= n) continue;
-        const int r = 8 * j + g;
-        const uint32_t row = base + u * C::CODE_BYTES + r * (D / 2);
-        uint32_t w[WORDS], group;
-        if constexpr (D == 128) {
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(row + ((t ^ ((r >> 1) & 3)) << 4)));
-          group = t;
-        } else {
-          asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
-                       : "=r"(w[0]), "=r"(w[1])
-                       : "r"(row + (((t >> 1) ^ ((r >> 2) & 1)) << 4) + (t & 1) * 8));
-          group = t >> 1;
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t from = unit + k_at + r * 8 * (D / 2);  // (key g + 8 has key g's swizzle)
+          if constexpr (D == 128) {
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(kw[r][0]), "=r"(kw[r][1]), "=r"(kw[r][2]), "=r"(kw[r][3])
+                         : "r"(from));
+          } else {
+            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
+                         : "=r"(kw[r][0]), "=r"(kw[r][1])
+                         : "r"(from));
+          }
+          uint16_t bits;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(unit + ks_at + r * 8 * NG * 2));
+          ks[r] = __byte_perm(bits, 0, 0x1010);
         }
-        const uint32_t bits = *reinterpret_cast<const uint16_t*>(
-            st + C::KS_OFF + u * C::SCALE_BYTES + (r * NG + group) * 2);
-        const uint32_t scale = bits | (bits << 16), shift = int4_shift(scale);
+        float s2[NQ][4];
+        const uint32_t shift[2] = {int4_shift(ks[0]), int4_shift(ks[1])};
 #pragma unroll
         for (int i = 0; i < WORDS; ++i) {
-          uint32_t v[4];
-          int4_values(w[i], scale, shift, v);
-          const uint32_t a0[4] = {qa[i][0], G16 ? qb[G16 ? i : 0][0] : 0u, qa[i][1],
-                                  G16 ? qb[G16 ? i : 0][1] : 0u};
-          const uint32_t a1[4] = {qa[i][2], G16 ? qb[G16 ? i : 0][2] : 0u, qa[i][3],
-                                  G16 ? qb[G16 ? i : 0][3] : 0u};
-          mma_bf16_16816(acc, a0, v[0], v[1]);
-          mma_bf16_16816(acc, a1, v[2], v[3]);
+          uint32_t x[4], y[4];
+          int4_values(kw[0][i], ks[0], shift[0], x);
+          int4_values(kw[1][i], ks[1], shift[1], y);
+          const uint32_t k0[4] = {x[0], y[0], x[1], y[1]}, k1[4] = {x[2], y[2], x[3], y[3]};
+#pragma unroll
+          for (int h = 0; h < NQ; ++h) {
+            if (i == 0) {
+              mma_zero_16816(s[u][h], k0, qf[h][i][0], qf[h][i][1]);
+              mma_zero_16816(s2[h], k1, qf[h][i][2], qf[h][i][3]);
+            } else {
+              mma_bf16_16816(s[u][h], k0, qf[h][i][0], qf[h][i][1]);
+              mma_bf16_16816(s2[h], k1, qf[h][i][2], qf[h][i][3]);
+            }
+          }
+        }
+        // Scores in base 2 of keys g (e 0, 1) and g + 8 (e 2, 3).  (The product is rounded
+        // before the maximum is taken from it: huge scores that are equal stay equal.)
+#pragma unroll
+        for (int h = 0; h < NQ; ++h) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[u][h][e] = __fmaf_rn(s[u][h][e] + s2[h][e], zscale, bias[u][e >> 1]);
+          }
+          above = fmaxf(above, fmaxf(fmaxf(s[u][h][0], s[u][h][2]) - m2[h][0],
+                                     fmaxf(s[u][h][1], s[u][h][3]) - m2[h][1]));
         }
       }
-      all = all && u < n && mt.map[u] == 0xffff;
-    }
-    // Scores in base 2; unseen tokens -inf.
-    float mx[2] = {-INFINITY, -INFINITY};
+      if (__any_sync(0xffffffffu, above > kSlack)) {
 #pragma unroll
-    for (int x = 0; x < 2 * UNITS; ++x) {
-      const int32_t map = all ? 0xffff : x / 2 < n ? mt.map[x / 2] : 0;
+        for (int h = 0; h < NQ; ++h) {
 #pragma unroll
-      for (int e = 0; e < (G16 ? 4 : 2); ++e) {
-        float v = __fmul_rn(s[x][e], zscale);
-        if (!all && !((map >> (8 * (x & 1) + 2 * t + (e & 1))) & 1)) v = -INFINITY;
-        s[x][e] = v;
-        mx[e >> 1] = fmaxf(mx[e >> 1], v);
-      }
-    }
-    float corr[2] = {1.f, 1.f};
+          for (int c = 0; c < 2; ++c) {
+            float m = m2[h][c];
 #pragma unroll
-    for (int hr = 0; hr < (G16 ? 2 : 1); ++hr) {
-      float m = mx[hr];
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      const float mtop = fmaxf(m2[hr], m);
-      const float mnew = mtop == -INFINITY ? 0.f : mtop;  // no token yet (no -inf - -inf)
-      corr[hr] = fast_exp2(m2[hr] - mnew);
-      m2[hr] = mtop;
-      float ps = 0.f;
+            for (int u = 0; u < U; ++u) m = fmaxf(m, fmaxf(s[u][h][c], s[u][h][c + 2]));
 #pragma unroll
-      for (int x = 0; x < 2 * UNITS; ++x) {
-        const float p0 = fast_exp2(s[x][2 * hr] - mnew), p1 = fast_exp2(s[x][2 * hr + 1] - mnew);
-        s[x][2 * hr] = p0;
-        s[x][2 * hr + 1] = p1;
-        ps += p0 + p1;
-      }
-      lsum[hr] = lsum[hr] * corr[hr] + ps;
-    }
-    // The rows' factors belong to this lane's columns 2t, 2t + 1.
-    if (__any_sync(0xffffffffu, corr[0] != 1.f || (G16 && corr[1] != 1.f))) {
+            for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+            const float corr = fast_exp2(m2[h][c] - m);
+            m2[h][c] = m;
+            lsum[h][c] *= corr;
 #pragma unroll
-      for (int hr = 0; hr < (G16 ? 2 : 1); ++hr) {
-        const float f0 = __shfl_sync(0xffffffffu, corr[hr], 8 * t);
-        const float f1 = __shfl_sync(0xffffffffu, corr[hr], 8 * t + 4);
+            for (int x = 0; x < NG; ++x) {
 #pragma unroll
-        for (int q = 0; q < NG; ++q) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float(&acc)[4] = hr == 0 ? o[q][j] : o2[G16 ? q : 0][j];
-            acc[0] *= f0;
-            acc[1] *= f1;
-            acc[2] *= f0;
-            acc[3] *= f1;
+              for (int j = 0; j < 2; ++j) {
+                o[h][x][j][c] *= corr;
+                o[h][x][j][c + 2] *= corr;
+              }
+            }
           }
         }
       }
-    }
-    // O^T += V^T P^T, 16 keys at a time.
+      // O^T += V^T P^T.
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      if (u >= n) continue;
-      const uint32_t p0 = pack_bf16x2(s[2 * u][0], s[2 * u][1]);
-      const uint32_t p1 = pack_bf16x2(s[2 * u + 1][0], s[2 * u + 1][1]);
-      const uint32_t p2 = G16 ? pack_bf16x2(s[2 * u][2], s[2 * u][3]) : 0u;
-      const uint32_t p3 = G16 ? pack_bf16x2(s[2 * u + 1][2], s[2 * u + 1][3]) : 0u;
-      // Scales of keys 2t, 2t + 1 and 2t + 8, 2t + 9, pairs of groups in a register.
-      const uint32_t* sv =
-          reinterpret_cast<const uint32_t*>(st + C::VS_OFF + u * C::SCALE_BYTES);
-      uint32_t keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;
-      if (!all) {  // scales of unseen tokens become 0: their codes may be stale, scales NaN
-        const int32_t map = mt.map[u];
-        auto pair = [&](int tok) {
-          return (((map >> tok) & 1) ? 0x0000ffffu : 0u) |
-                 (((map >> (tok + 1)) & 1) ? 0xffff0000u : 0u);
-        };
-        keep_lo = pair(2 * t);
-        keep_hi = pair(2 * t + 8);
-      }
-      uint32_t sc[4][NG / 2];
+      for (int u = 0; u < U; ++u) {
+        const uint32_t unit = base + u * C::UNIT_BYTES;
+        // The codes of V; the scales of keys 2t, 2t + 1 and 2t + 8, 2t + 9, pairs of groups in
+        // a register.
+        uint32_t sc[4][NG / 2], vc[NG / 2][4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int key = 2 * t + (k & 1) + 8 * (k >> 1);
+        for (int q = 0; q < NG / 2; ++q) {  // (pieces 2 and 3 are 0 and 1 with one bit turned)
+          ldmatrix_x4_trans(unit + (v_at ^ (32 * q)), vc[q][0], vc[q][1], vc[q][2], vc[q][3]);
+        }
 #pragma unroll
-        for (int i = 0; i < NG / 2; ++i) sc[k][i] = sv[key * (NG / 2) + i];
-      }
-      const int r = 8 * ((lane >> 3) & 1) + (lane & 7);
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t from = unit + vs_at + ((k & 1) + 8 * (k >> 1)) * (NG * 2);
+          if constexpr (NG == 4) {
+            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
+                         : "=r"(sc[k][0]), "=r"(sc[k][1])
+                         : "r"(from));
+          } else {
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sc[k][0]) : "r"(from));
+          }
+        }
+        uint32_t p[NQ][2];  // P^T: query column g, keys 2t, 2t + 1 and 2t + 8, 2t + 9
 #pragma unroll
-      for (int q0 = 0; q0 < NG; q0 += 2) {
-        const int q = q0 + (lane >> 4);  // the group whose row this lane points at
-        const uint32_t piece = D == 128 ? q ^ ((r >> 1) & 3) : q ^ ((r >> 2) & 1);
-        uint32_t c[4];
-        ldmatrix_x4_trans(base + C::V_OFF + u * C::CODE_BYTES + r * (D / 2) + (piece << 4), c[0],
-                          c[1], c[2], c[3]);
+        for (int h = 0; h < NQ; ++h) {
+          float e[4];
 #pragma unroll
-        for (int qq = 0; qq < 2; ++qq) {
-          const uint32_t sel = qq == 0 ? 0x5410 : 0x7632;
-          const uint32_t s_lo = __byte_perm(sc[0][q0 / 2], sc[1][q0 / 2], sel) & keep_lo;
-          const uint32_t s_hi = __byte_perm(sc[2][q0 / 2], sc[3][q0 / 2], sel) & keep_hi;
+          for (int c = 0; c < 2; ++c) {
+            e[c] = fast_exp2(s[u][h][c] - m2[h][c]);
+            e[c + 2] = fast_exp2(s[u][h][c + 2] - m2[h][c]);
+            lsum[h][c] += e[c] + e[c + 2];
+          }
+          p[h][0] = transpose_8x8(pack_bf16x2(e[0], e[1]));
+          p[h][1] = transpose_8x8(pack_bf16x2(e[2], e[3]));
+        }
+#pragma unroll
+        for (int q = 0; q < NG; ++q) {
+          const uint32_t sel = q % 2 == 0 ? 0x5410 : 0x7632;
+          const uint32_t s_lo = __byte_perm(sc[0][q / 2], sc[1][q / 2], sel);
+          const uint32_t s_hi = __byte_perm(sc[2][q / 2], sc[3][q / 2], sel);
           uint32_t lo[4], hi[4];  // dim i of the lane's four, keys (2t, 2t + 1), (2t + 8, 2t + 9)
-          int4_values(c[2 * qq], s_lo, int4_shift(s_lo), lo);
-          int4_values(c[2 * qq + 1], s_hi, int4_shift(s_hi), hi);
+          int4_values(vc[q / 2][2 * (q % 2)], s_lo, int4_shift(s_lo), lo);
+          int4_values(vc[q / 2][2 * (q % 2) + 1], s_hi, int4_shift(s_hi), hi);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const uint32_t av[4] = {lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1]};
-            mma_bf16_16816(o[q0 + qq][j], av, p0, p1);
-            if (G16) mma_bf16_16816(o2[G16 ? q0 + qq : 0][j], av, p2, p3);
+#pragma unroll
+            for (int h = 0; h < NQ; ++h) mma_bf16_16816(o[h][q][j], av, p[h][0], p[h][1]);
+          }
+        }
+      }
+
+      if (flags & kLast) {
+        const int32_t seq = mt.owner.seq, kvh = mt.owner.kvh;
+        const bool whole = (mt.owner.flags & kWhole) != 0;
+        const int slot_of = (mt.owner.flags & kSlot1) ? 1 : 0;
+        float* slot = warp_slot<C>(smem, warp, slot_of);
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
+                             static_cast<int64_t>(seq) * a.o_stride_seq +
+                             static_cast<int64_t>(kvh) * G * D;
+        if (lane == 0 && !whole) {
+          slots.seq[warp][slot_of] = seq;
+          slots.kvh[warp][slot_of] = kvh;
+          slots.nb[warp][slot_of] = mt.owner.nb;
+          slots.unit[warp][slot_of] = mt.owner.seg_unit;
+        }
+        __syncwarp();  // (slot 1 lies over the stages: their last reads are done)
+        // Neighbouring lanes (g, g ^ 1) hold the dims 2k and 2k + 1: each takes both dims of one
+        // of the two query rows.
+        const int odd = g & 1;
+#pragma unroll
+        for (int h = 0; h < NQ; ++h) {
+          float l[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            l[c] = lsum[h][c];
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], x);
+          }
+          const int row = 8 * h + 2 * t + odd;
+          const float inv = whole ? 1.f / (odd ? l[1] : l[0]) : 1.f;
+#pragma unroll
+          for (int q = 0; q < NG; ++q) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float(&acc)[4] = o[h][q][i / 2];
+              const float x0 = acc[2 * (i & 1)], x1 = acc[2 * (i & 1) + 1];  // rows 2t, 2t + 1
+              const float got = __shfl_xor_sync(0xffffffffu, odd ? x0 : x1, 4);
+              const float lo = (odd ? got : x0) * inv, hi = (odd ? x1 : got) * inv;
+              const int dim = 32 * q + 8 * (g >> 1) + 2 * i;
+              if (row < G) {
+                if (whole) {
+                  *reinterpret_cast<uint32_t*>(out + row * D + dim) = pack_bf16x2(lo, hi);
+                } else {
+                  *reinterpret_cast<float2*>(slot + row * D + dim) = make_float2(lo, hi);
+                }
+              }
+            }
+          }
+          if (!whole && g < 2 && row < G) {  // (g is odd here where the row is)
+            slot[G * D + row] = odd ? m2[h][1] : m2[h][0];
+            slot[G * D + G + row] = odd ? l[1] : l[0];
           }
         }
       }
     }
     // The stage has been read: refill it with the step S positions ahead.
     __syncwarp();
-    const int32_t seq = mt.seq, kvh = mt.kvh, nb = mt.nb;
-    const int64_t seg_unit = mt.seg_unit;
-    __syncwarp();
-    issue(stage);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-
-    if (flags & kLast) {
-      float lrow[2];
-#pragma unroll
-      for (int hr = 0; hr < 2; ++hr) {
-        float l = lsum[hr];
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        lrow[hr] = l;
-      }
-      const bool whole = (flags & kWhole) != 0;
-      const int slot_of = (flags & kSlot1) ? 1 : 0;
-      float* slot = warp_slot<C>(smem, warp, slot_of);
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
-                           static_cast<int64_t>(seq) * a.o_stride_seq +
-                           static_cast<int64_t>(kvh) * G * D;
-      // Neighbouring lanes (g, g ^ 1) hold the dims 2k and 2k + 1: each takes both dims of one
-      // of the two query rows.
-      const int odd = g & 1;
-#pragma unroll
-      for (int hr = 0; hr < (G16 ? 2 : 1); ++hr) {
-        const int row = 8 * hr + 2 * t + odd;
-        const float inv = whole ? 1.f / __shfl_sync(0xffffffffu, lrow[hr], 8 * t + 4 * odd) : 1.f;
-#pragma unroll
-        for (int q = 0; q < NG; ++q) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float(&acc)[4] = hr == 0 ? o[q][i / 2] : o2[G16 ? q : 0][i / 2];
-            const float x0 = acc[2 * (i & 1)], x1 = acc[2 * (i & 1) + 1];  // rows 2t, 2t + 1
-            const float got = __shfl_xor_sync(0xffffffffu, odd ? x0 : x1, 4);
-            const float lo = (odd ? got : x0) * inv, hi = (odd ? x1 : got) * inv;
-            const int dim = 32 * q + 8 * (g >> 1) + 2 * i;
-            if (row < G) {
-              if (whole) {
-                *reinterpret_cast<uint32_t*>(out + row * D + dim) = pack_bf16x2(lo, hi);
-              } else {
-                *reinterpret_cast<float2*>(slot + row * D + dim) = make_float2(lo, hi);
-              }
-            }
-          }
-        }
-        if (!whole && t == 0 && 8 * hr + g < G) {
-          slot[G * D + 8 * hr + g] = m2[hr];
-          slot[G * D + G + 8 * hr + g] = lrow[hr];
-        }
-      }
-      if (!whole && lane == 0) {
-        slots.seq[warp][slot_of] = seq;
-        slots.kvh[warp][slot_of] = kvh;
-        slots.nb[warp][slot_of] = nb;
-        slots.unit[warp][slot_of] = seg_unit;
-      }
-      __syncwarp();
-    }
+    queue = (queue >> 4) | (issue(base, stage) << (4 * (S - 1)));
+    stage = stage + 1 == S ? 0 : stage + 1;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 

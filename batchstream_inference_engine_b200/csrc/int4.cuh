@@ -43,7 +43,9 @@ __device__ __forceinline__ uint32_t int4_shift(uint32_t scale) {
   return d;
 }
 __device__ __forceinline__ uint32_t int4_raw(uint32_t w, int i) {  // 128 + n of dims 2i, 2i + 1
-  return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+  uint32_t d;  // (one instruction; with two immediates the compiler makes it two)
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(w >> (4 * i)), "r"(0x000f000fu), "r"(0x43004300u));
+  return d;
 }
 __device__ __forceinline__ void int4_values(uint32_t w, uint32_t scale, uint32_t shift,
                                             uint32_t (&v)[4]) {
