@@ -306,11 +306,11 @@ int window_workspace(const WindowShape& s, uint64_t* bytes_out) {
   SimtPlan p;
   if (int rc = plan_simt(s, &p)) return rc;
   int64_t need = p.bytes;
-  if (mma_shape(s) && s.chunks && !s.int4) {
+  if (mma_shape(s) && s.chunks) {
     MmaChunkPlan m;
     if (int rc = plan_mma_chunks(s, &m)) return rc;
     need = std::max(need, m.bytes);
-  } else if (mma_shape(s) && !s.chunks) {
+  } else if (mma_shape(s)) {
     MmaDecodePlan m;
     if (int rc = plan_mma_decode(s, &m)) return rc;
     need = std::max(need, m.bytes);
@@ -420,8 +420,12 @@ int run_mma_chunks(const WindowShape& s, const WindowCall& c, bsb::WindowArgs& a
                                      groups, p.tile_tokens)) {
     return rc;
   }
-  if (int rc = bsb::pool_tensor_map(&kmap, c.key_pool, rows, s.head_dim)) return rc;
-  if (int rc = bsb::pool_tensor_map(&vmap, c.value_pool, rows, s.head_dim)) return rc;
+  if (s.int4) {
+    kmap = vmap = qmap;  // not used
+  } else {
+    if (int rc = bsb::pool_tensor_map(&kmap, c.key_pool, rows, s.head_dim)) return rc;
+    if (int rc = bsb::pool_tensor_map(&vmap, c.value_pool, rows, s.head_dim)) return rc;
+  }
   a.tile_tokens = static_cast<int32_t>(p.tile_tokens);
   a.qtiles = static_cast<int32_t>(p.qtiles);
   a.splits = static_cast<int32_t>(p.splits);
@@ -484,7 +488,7 @@ int run_window(const WindowShape& s, const WindowCall& c) {
   a.status = c.status;
   // The tensor-core prefill compares scores before it scales them: it needs a
   // magnitude to scale by.
-  if (mma && !s.int4 && a.scale != 0.f && std::isfinite(a.scale)) return run_mma_chunks(s, c, a);
+  if (mma && a.scale != 0.f && std::isfinite(a.scale)) return run_mma_chunks(s, c, a);
 
   if (s.int4) {
     BS_CHECK(int4_aligned(c.key_pool, c.value_pool), "4-bit pools must be 4-byte aligned");

@@ -47,9 +47,15 @@
 // A call with fewer CTAs than two per SM cuts each tile's steps into ranges, whose
 // records window_prefill_merge_kernel joins in range order.
 //
+// Over 4-bit pools (Q4) warps 5 to 7 write the operands that TMA would bring: each takes
+// every third unit of 16 tokens, of K of one step, then of V of the step before, a lane 32
+// dims of a token at a time, whose codes and scale it loaded a unit ahead.  What no row of the
+// CTA sees gets a scale of 0; appended values are finite, so there is nothing to guard.
+//
 // Waits are bounded and their outcome made warp-uniform before warp-collective
 // instructions; the loaders and the MMA warp drain what they started before TMEM is
 // freed, also on the error path.
+#include "int4.cuh"
 #include "tcgen05.cuh"
 #include "window.cuh"
 
@@ -190,7 +196,7 @@ __device__ __forceinline__ uint32_t fma_zero_bf16x2(uint32_t a, uint32_t c) {
   return d;
 }
 
-template <int D>
+template <int D, bool Q4>
 __global__ void __launch_bounds__(kThreads, 2)
     window_prefill_kernel(const __grid_constant__ CUtensorMap qmap,
                           const __grid_constant__ CUtensorMap kmap,
@@ -225,10 +231,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (tid == 0) {
     mbar_init(&q_full, 1);
-    for (int s = 0; s < C::KS; ++s) mbar_init(&k_full[s], 1);
+    // (4-bit: one arrival for each unit written.)
+    for (int s = 0; s < C::KS; ++s) mbar_init(&k_full[s], Q4 ? kUnits : 1);
     for (int s = 0; s < C::VS; ++s) {
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_ok[s], 1);
+      mbar_init(&v_ok[s], Q4 ? kUnits : 1);
     }
     for (int s = 0; s < kRing; ++s) mbar_init(&step_done[s], 1);
     for (int b = 0; b < 2; ++b) mbar_init(&p_full[b], kRows);
@@ -255,7 +262,127 @@ __global__ void __launch_bounds__(kThreads, 2)
   // and are never kRing behind (see the ring sizes).
   auto wait_step = [&](int u) { return wait_all(&step_done[u % kRing], (u / kRing) & 1); };
 
-  if (warp == kLoadKWarp || warp == kLoadVWarp) {
+  if (Q4 && warp >= kLoadKWarp) {
+    // ---------------------------------------------------------------- 4-bit K and V
+    if (warp == kLoadKWarp) {
+      if (lane == 0) {
+        const uint32_t rows = static_cast<uint32_t>(a.tile_tokens * a.groups);
+        mbar_arrive_expect_tx(&q_full, C::HALVES * rows * 128u);
+        for (int hf = 0; hf < C::HALVES; ++hf) {
+          tma_load_3d(sQ + hf * C::Q_HALF_BYTES, &qmap, &q_full, hf * 64, h * a.groups, w.tok0);
+        }
+      }
+      __syncwarp();
+    }
+    constexpr int NG = D / kInt4Group, ROWS = 32 / NG, PARTS = kUnit / ROWS;  // rows a load
+    const int32_t* table = a.block_tables + static_cast<int64_t>(w.row) * a.bt_stride;
+    const int32_t block_units = a.block_size / kUnit;
+    const int64_t block_bytes = static_cast<int64_t>(a.block_size) * int4_row_bytes(D);
+    const int64_t head_at = static_cast<int64_t>(h) * a.num_blocks * block_bytes;
+    const int row = lane / NG, group = lane % NG;  // this lane's token (of ROWS) and dims
+    // Its four 16-byte pieces of a row of 64 dims are at `piece` ^ i: the lanes of groups 2 and
+    // 3 take their words in another order than those of 0 and 1, whose banks they share.
+    const uint32_t piece = ((group & 1) * 4) ^ (group & 2) ^ (row & 7);
+    const uint32_t row_at = (group >> 1) * C::HALF_BYTES + row * 128;
+    // Units in the order K(0), K(1), V(0), K(2), V(1), ..: a step's scores come first.
+    struct Unit {
+      int32_t j, un;  // step, unit of the step; j < 0: none
+      bool is_v;
+    };
+    auto unit_of = [&](int32_t m) {
+      const int32_t part = m / kUnits;
+      Unit u;
+      u.un = m % kUnits;
+      u.is_v = part > 0 && part % 2 == 0;
+      u.j = u.is_v ? part / 2 - 1 : (part + 1) / 2;
+      if (u.j >= n) u.j = -1;
+      return u;
+    };
+    // Token unit of a unit of the range, or -1.
+    auto token_unit = [&](const Unit& u) -> int32_t {
+      const int32_t x = (j0 + u.j) * kUnits + u.un;
+      if (u.j < 0 || x >= sd.units) return -1;
+      return x < sd.sink_units ? x : x - sd.sink_units + sd.first_unit;
+    };
+    auto entry = [&](int32_t m) -> int32_t {
+      const int32_t tu = token_unit(unit_of(m));
+      return tu < 0 ? -1 : __ldg(table + (block_units == 1 ? tu : tu / block_units));
+    };
+    struct Codes {
+      uint4 words[PARTS];
+      uint32_t scale[PARTS];
+    };
+    auto load = [&](int32_t m, int32_t blk) {
+      Codes c;
+      const Unit u = unit_of(m);
+      const int32_t tu = token_unit(u);
+      const bool valid = tu >= 0 && blk >= 0 && blk < a.num_blocks;
+      if (tu >= 0 && !valid && !u.is_v && lane == 0) set_status(a.status, kStatusBadBlock);
+      const uint8_t* block = static_cast<const uint8_t*>(u.is_v ? a.v_pool : a.k_pool) + head_at +
+                             blk * block_bytes;
+      const int32_t first = tu % block_units * kUnit;
+      const int32_t pos0 = tu * kUnit;
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) {
+        const int32_t r = row + p * ROWS, pos = pos0 + r;
+        c.words[p] = make_uint4(0u, 0u, 0u, 0u);
+        c.scale[p] = 0u;
+        if (valid) {
+          c.words[p] = __ldg(reinterpret_cast<const uint4*>(
+              block + (first + r) * int4_code_bytes(D) + group * 16));
+          // Rows that nobody sees may hold anything: their values are 0.
+          if (pos <= sd.pos1 && (pos < a.sinks || pos >= w.lo)) {
+            c.scale[p] = __ldg(reinterpret_cast<const uint16_t*>(
+                block + a.block_size * int4_code_bytes(D) + (first + r) * int4_scale_bytes(D)) + group);
+          }
+        }
+      }
+      return c;
+    };
+    constexpr int kWriters = 3;
+    const int32_t total = kUnits * (2 * n + 1);
+    int32_t m = warp - kLoadKWarp;
+    Codes now = load(m, entry(m)), then;
+    int32_t ent = entry(m + kWriters);
+    bool ok = true;
+    for (; m < total; m += kWriters) {
+      then = load(m + kWriters, ent);
+      ent = entry(m + 2 * kWriters);
+      const Unit u = unit_of(m);
+      if (u.j >= 0) {
+        // Step j - KS has read the K stage, step j - VS + 2 the V stage.
+        const int32_t free_at = u.is_v ? u.j - C::VS + 2 : u.j - C::KS;
+        if (u.j >= (u.is_v ? C::VS : C::KS)) ok = wait_step(free_at);
+        if (!ok) break;
+        const int stage = u.is_v ? u.j % C::VS : u.j % C::KS;
+        uint8_t* to = (u.is_v ? sV(stage) : sK(stage)) + u.un * kUnit * 128 + row_at;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          uint32_t words[4] = {now.words[p].x, now.words[p].y, now.words[p].z, now.words[p].w};
+          if (group & 2) {
+            words[0] = now.words[p].z;
+            words[1] = now.words[p].w;
+            words[2] = now.words[p].x;
+            words[3] = now.words[p].y;
+          }
+          const uint32_t scale = now.scale[p] | (now.scale[p] << 16), shift = int4_shift(scale);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t v[4];
+            int4_values(words[i], scale, shift, v);
+            *reinterpret_cast<uint4*>(to + p * ROWS * 128 + ((piece ^ i) << 4)) =
+                make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(u.is_v ? &v_ok[stage] : &k_full[stage]);
+      }
+      now = then;
+    }
+    const bool drained = warp != kLoadKWarp || wait_all(&q_full, 0);
+    if ((!ok || !drained) && lane == 0) set_status(a.status, kStatusWaitTimeout);
+  } else if (warp == kLoadKWarp || warp == kLoadVWarp) {
     // ---------------------------------------------------------------- loaders
     const bool is_k = warp == kLoadKWarp;
     const CUtensorMap* map = is_k ? &kmap : &vmap;
@@ -706,13 +833,13 @@ __global__ void __launch_bounds__(kMergeThreads) window_prefill_merge_kernel(con
   }
 }
 
-template <int D>
+template <int D, bool Q4>
 int launch_d(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& kmap,
              const CUtensorMap& vmap, cudaStream_t stream) {
   using C = Cfg<D>;
   static unsigned long long configured = 0;  // one bit per device
   cudaError_t e = once_per_device(&configured, [] {
-    return cudaFuncSetAttribute(window_prefill_kernel<D>,
+    return cudaFuncSetAttribute(window_prefill_kernel<D, Q4>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   });
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -727,7 +854,7 @@ int launch_d(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& km
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, window_prefill_kernel<D>, qmap, kmap, vmap, a);
+  e = cudaLaunchKernelEx(&cfg, window_prefill_kernel<D, Q4>, qmap, kmap, vmap, a);
   if (e != cudaSuccess || a.splits == 1) return static_cast<int>(e);
   cfg.gridDim = dim3(static_cast<unsigned>(items * (kRows / kMergeRows)));
   cfg.blockDim = dim3(kMergeThreads);
@@ -739,8 +866,12 @@ int launch_d(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& km
 
 int launch_window_prefill(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& kmap,
                           const CUtensorMap& vmap, cudaStream_t stream) {
-  return a.head_dim == 64 ? launch_d<64>(a, qmap, kmap, vmap, stream)
-                          : launch_d<128>(a, qmap, kmap, vmap, stream);
+  if (a.int4) {  // (kmap and vmap are not used)
+    return a.head_dim == 64 ? launch_d<64, true>(a, qmap, kmap, vmap, stream)
+                            : launch_d<128, true>(a, qmap, kmap, vmap, stream);
+  }
+  return a.head_dim == 64 ? launch_d<64, false>(a, qmap, kmap, vmap, stream)
+                          : launch_d<128, false>(a, qmap, kmap, vmap, stream);
 }
 
 }  // namespace bsb
