@@ -48,8 +48,8 @@
 // records window_prefill_merge_kernel joins in range order.
 //
 // Over 4-bit pools (Q4) warps 5 to 7 write the operands that TMA would bring: each takes
-// every third unit of 16 tokens, of K of one step, then of V of the step before, a lane 32
-// dims of a token at a time, whose codes and scale it loaded a unit ahead.  What no row of the
+// every third half tile of 32 keys, of K of one step, then of V of the step before, a lane
+// 32 dims of a token at a time, whose codes and scale it loaded two half tiles ahead.  What no row of the
 // CTA sees gets a scale of 0; appended values are finite, so there is nothing to guard.
 //
 // Waits are bounded and their outcome made warp-uniform before warp-collective
@@ -231,11 +231,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (tid == 0) {
     mbar_init(&q_full, 1);
-    // (4-bit: one arrival for each unit written.)
-    for (int s = 0; s < C::KS; ++s) mbar_init(&k_full[s], Q4 ? kUnits : 1);
+    // (4-bit: an arrival for each half tile written.)
+    for (int s = 0; s < C::KS; ++s) mbar_init(&k_full[s], Q4 ? 2 : 1);
     for (int s = 0; s < C::VS; ++s) {
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_ok[s], Q4 ? kUnits : 1);
+      mbar_init(&v_ok[s], Q4 ? 2 : 1);
     }
     for (int s = 0; s < kRing; ++s) mbar_init(&step_done[s], 1);
     for (int b = 0; b < 2; ++b) mbar_init(&p_full[b], kRows);
@@ -275,6 +275,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncwarp();
     }
     constexpr int NG = D / kInt4Group, ROWS = 32 / NG, PARTS = kUnit / ROWS;  // rows a load
+    constexpr int kWriters = 3;
     const int32_t* table = a.block_tables + static_cast<int64_t>(w.row) * a.bt_stride;
     const int32_t block_units = a.block_size / kUnit;
     const int64_t block_bytes = static_cast<int64_t>(a.block_size) * int4_row_bytes(D);
@@ -284,101 +285,131 @@ __global__ void __launch_bounds__(kThreads, 2)
     // 3 take their words in another order than those of 0 and 1, whose banks they share.
     const uint32_t piece = ((group & 1) * 4) ^ (group & 2) ^ (row & 7);
     const uint32_t row_at = (group >> 1) * C::HALF_BYTES + row * 128;
-    // Units in the order K(0), K(1), V(0), K(2), V(1), ..: a step's scores come first.
-    struct Unit {
-      int32_t j, un;  // step, unit of the step; j < 0: none
-      bool is_v;
-    };
-    auto unit_of = [&](int32_t m) {
-      const int32_t part = m / kUnits;
-      Unit u;
-      u.un = m % kUnits;
-      u.is_v = part > 0 && part % 2 == 0;
-      u.j = u.is_v ? part / 2 - 1 : (part + 1) / 2;
-      if (u.j >= n) u.j = -1;
-      return u;
-    };
-    // Token unit of a unit of the range, or -1.
-    auto token_unit = [&](const Unit& u) -> int32_t {
-      const int32_t x = (j0 + u.j) * kUnits + u.un;
-      if (u.j < 0 || x >= sd.units) return -1;
+    // Half tiles of 32 keys in the order K(0), V(-1), K(1), V(0), K(2), V(1), ..: half
+    // tile i is half i & 1 of K(i / 4) or, with bit 1, of V(i / 4 - 1).
+    auto step_of = [&](int32_t i) { return (i >> 2) - ((i >> 1) & 1); };
+    auto token_unit = [&](int32_t x) {  // of unit x of the range
       return x < sd.sink_units ? x : x - sd.sink_units + sd.first_unit;
     };
-    auto entry = [&](int32_t m) -> int32_t {
-      const int32_t tu = token_unit(unit_of(m));
-      return tu < 0 ? -1 : __ldg(table + (block_units == 1 ? tu : tu / block_units));
-    };
-    struct Codes {
-      uint4 words[PARTS];
-      uint32_t scale[PARTS];
-    };
-    auto load = [&](int32_t m, int32_t blk) {
-      Codes c;
-      const Unit u = unit_of(m);
-      const int32_t tu = token_unit(u);
-      const bool valid = tu >= 0 && blk >= 0 && blk < a.num_blocks;
-      if (tu >= 0 && !valid && !u.is_v && lane == 0) set_status(a.status, kStatusBadBlock);
-      const uint8_t* block = static_cast<const uint8_t*>(u.is_v ? a.v_pool : a.k_pool) + head_at +
-                             blk * block_bytes;
-      const int32_t first = tu % block_units * kUnit;
-      const int32_t pos0 = tu * kUnit;
+    // Table entries of a half tile's two units (-1: past the range).
+    auto entries = [&](int32_t i, int32_t (&blk)[2]) {
+      const int32_t j = step_of(i), x0 = (j0 + j) * kUnits + 2 * (i & 1);
 #pragma unroll
-      for (int p = 0; p < PARTS; ++p) {
-        const int32_t r = row + p * ROWS, pos = pos0 + r;
-        c.words[p] = make_uint4(0u, 0u, 0u, 0u);
-        c.scale[p] = 0u;
-        if (valid) {
-          c.words[p] = __ldg(reinterpret_cast<const uint4*>(
-              block + (first + r) * int4_code_bytes(D) + group * 16));
-          // Rows that nobody sees may hold anything: their values are 0.
-          if (pos <= sd.pos1 && (pos < a.sinks || pos >= w.lo)) {
-            c.scale[p] = __ldg(reinterpret_cast<const uint16_t*>(
-                block + a.block_size * int4_code_bytes(D) + (first + r) * int4_scale_bytes(D)) + group);
-          }
+      for (int e = 0; e < 2; ++e) {
+        blk[e] = -1;
+        if (j >= 0 && j < n && x0 + e < sd.units) {
+          const int32_t tu = token_unit(x0 + e);
+          blk[e] = __ldg(table + (block_units == 1 ? tu : tu / block_units));
         }
       }
-      return c;
     };
-    constexpr int kWriters = 3;
-    const int32_t total = kUnits * (2 * n + 1);
-    int32_t m = warp - kLoadKWarp;
-    Codes now = load(m, entry(m)), then;
-    int32_t ent = entry(m + kWriters);
-    bool ok = true;
-    for (; m < total; m += kWriters) {
-      then = load(m + kWriters, ent);
-      ent = entry(m + 2 * kWriters);
-      const Unit u = unit_of(m);
-      if (u.j >= 0) {
-        // Step j - KS has read the K stage, step j - VS + 2 the V stage.
-        const int32_t free_at = u.is_v ? u.j - C::VS + 2 : u.j - C::KS;
-        if (u.j >= (u.is_v ? C::VS : C::KS)) ok = wait_step(free_at);
-        if (!ok) break;
-        const int stage = u.is_v ? u.j % C::VS : u.j % C::KS;
-        uint8_t* to = (u.is_v ? sV(stage) : sK(stage)) + u.un * kUnit * 128 + row_at;
+    struct Codes {
+      uint4 words[2][PARTS];
+      uint32_t scale[2][PARTS];
+    };
+    int32_t plain_lo, plain_hi;
+    plain_steps(a, sd, plain_lo, plain_hi);
+    const int32_t codes_lane = row * int4_code_bytes(D) + group * 16;
+    const int32_t scales_lane = a.block_size * int4_code_bytes(D) + row * int4_scale_bytes(D) + group * 2;
+    auto load = [&](int32_t i, const int32_t (&blk)[2], Codes& c) {
+      const int32_t j = step_of(i), x0 = (j0 + j) * kUnits + 2 * (i & 1);
+      const bool is_v = (i & 2) != 0;
+      const uint8_t* pool = static_cast<const uint8_t*>(is_v ? a.v_pool : a.k_pool) + head_at;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const bool valid = blk[e] >= 0 && blk[e] < a.num_blocks;
+        if (!valid) {
+          if (lane == 0 && !is_v && j >= 0 && j < n && x0 + e < sd.units) {
+            set_status(a.status, kStatusBadBlock);
+          }
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) {
+            c.words[e][p] = make_uint4(0u, 0u, 0u, 0u);
+            c.scale[e][p] = 0u;
+          }
+          continue;
+        }
+        const uint8_t* codes = pool + blk[e] * block_bytes + codes_lane;
+        const uint8_t* scales = pool + blk[e] * block_bytes + scales_lane;
+        if (block_units != 1) {
+          const int32_t first = token_unit(x0 + e) % block_units * kUnit;
+          codes += first * int4_code_bytes(D);
+          scales += first * int4_scale_bytes(D);
+        }
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-          uint32_t words[4] = {now.words[p].x, now.words[p].y, now.words[p].z, now.words[p].w};
-          if (group & 2) {
-            words[0] = now.words[p].z;
-            words[1] = now.words[p].w;
-            words[2] = now.words[p].x;
-            words[3] = now.words[p].y;
-          }
-          const uint32_t scale = now.scale[p] | (now.scale[p] << 16), shift = int4_shift(scale);
+          c.words[e][p] = __ldg(reinterpret_cast<const uint4*>(codes + p * ROWS * int4_code_bytes(D)));
+          c.scale[e][p] = __ldg(reinterpret_cast<const uint16_t*>(scales + p * ROWS * int4_scale_bytes(D)));
+        }
+      }
+    };
+    // Codes are loaded kAhead of this warp's half tiles ahead, table entries one more.
+    constexpr int kAhead = 2;
+    Codes codes[kAhead];
+    int32_t i = warp - kLoadKWarp, blk[2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t v[4];
-            int4_values(words[i], scale, shift, v);
-            *reinterpret_cast<uint4*>(to + p * ROWS * 128 + ((piece ^ i) << 4)) =
-                make_uint4(v[0], v[1], v[2], v[3]);
+    for (int x = 0; x < kAhead; ++x) {
+      entries(i + x * kWriters, blk);
+      load(i + x * kWriters, blk, codes[x]);
+    }
+    entries(i + kAhead * kWriters, blk);
+    bool ok = true;
+    auto turn = [&](Codes& c) {
+      const bool is_v = (i & 2) != 0;
+      const int32_t j = step_of(i);
+      if (j >= 0 && j < n) {
+        // Step j - KS has read the K stage, step j - VS + 2 the V stage.
+        if (j >= (is_v ? C::VS : C::KS)) ok = wait_step(is_v ? j - C::VS + 2 : j - C::KS);
+        if (!ok) return;
+        const int stage = is_v ? j % C::VS : j % C::KS;
+        uint8_t* to = (is_v ? sV(stage) : sK(stage)) + (i & 1) * 32 * 128 + row_at;
+        if (j0 + j < plain_lo || j0 + j > plain_hi) {
+          // Rows that nobody sees may hold anything: their values are 0.  (Here, not where the
+          // codes are loaded, which would wait for them.)
+          const int32_t x0 = (j0 + j) * kUnits + 2 * (i & 1);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int32_t pos = token_unit(x0 + e) * kUnit + row;
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+              const int32_t at = pos + p * ROWS;
+              if (at > sd.pos1 || (at >= a.sinks && at < w.lo)) c.scale[e][p] = 0u;
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) {
+            const uint4 raw = c.words[e][p];
+            const bool turned = (group & 2) != 0;
+            const uint32_t words[4] = {turned ? raw.z : raw.x, turned ? raw.w : raw.y,
+                                       turned ? raw.x : raw.z, turned ? raw.y : raw.w};
+            const uint32_t scale = __byte_perm(c.scale[e][p], 0, 0x1010);
+            const uint32_t shift = int4_shift(scale);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t v[4];
+              int4_values(words[k], scale, shift, v);
+              *reinterpret_cast<uint4*>(to + (e * kUnit + p * ROWS) * 128 + ((piece ^ k) << 4)) =
+                  make_uint4(v[0], v[1], v[2], v[3]);
+            }
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(u.is_v ? &v_ok[stage] : &k_full[stage]);
+        if (lane == 0) mbar_arrive(is_v ? &v_ok[stage] : &k_full[stage]);
       }
-      now = then;
+      i += kWriters;
+      load(i + (kAhead - 1) * kWriters, blk, c);
+      entries(i + kAhead * kWriters, blk);
+    };
+    const int32_t end = 4 * (n + 1);
+    while (ok && i < end) {
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        if (ok && i < end) turn(codes[x]);
+      }
     }
     const bool drained = warp != kLoadKWarp || wait_all(&q_full, 0);
     if ((!ok || !drained) && lane == 0) set_status(a.status, kStatusWaitTimeout);
