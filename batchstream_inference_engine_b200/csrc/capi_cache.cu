@@ -194,6 +194,8 @@ int plan_simt(const WindowShape& s, SimtPlan* p) {
 // Shapes the tensor-core kernels take (with 16-byte aligned pools and queries, and
 // outputs that their stores can address; see mma_pointers).
 bool mma_shape(const WindowShape& s) {
+  // (The bytes of a 4-bit block are counted in 32 bits.)
+  if (s.int4 && s.block_size > (1 << 23)) return false;
   return s.dtype == BS_BF16 && s.block_size % 16 == 0 && (s.head_dim == 64 || s.head_dim == 128);
 }
 

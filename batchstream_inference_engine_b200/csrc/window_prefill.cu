@@ -278,50 +278,61 @@ __global__ void __launch_bounds__(kThreads, 2)
     constexpr int kWriters = 3;
     const int32_t* table = a.block_tables + static_cast<int64_t>(w.row) * a.bt_stride;
     const int32_t block_units = a.block_size / kUnit;
-    const int64_t block_bytes = static_cast<int64_t>(a.block_size) * int4_row_bytes(D);
-    const int64_t head_at = static_cast<int64_t>(h) * a.num_blocks * block_bytes;
-    const int row = lane / NG, group = lane % NG;  // this lane's token (of ROWS) and dims
-    // Its four 16-byte pieces of a row of 64 dims are at `piece` ^ i: the lanes of groups 2 and
-    // 3 take their words in another order than those of 0 and 1, whose banks they share.
-    const uint32_t piece = ((group & 1) * 4) ^ (group & 2) ^ (row & 7);
-    const uint32_t row_at = (group >> 1) * C::HALF_BYTES + row * 128;
+    const int32_t block_bytes = a.block_size * int4_row_bytes(D);  // fits (host)
+    // This lane's token (of ROWS) and dims.  Neighbouring lanes have neighbouring tokens: their
+    // 16-byte pieces of a step's row of 64 dims, at `piece` ^ k, are then in different banks.
+    const int row = lane % ROWS, group = lane / ROWS;
+    const uint32_t piece = ((group & 1) * 4) ^ (row & 7);
+    const uint32_t ring = smem_u32(sK(0)) + (group >> 1) * C::HALF_BYTES + row * 128;
+    const int64_t head_at = static_cast<int64_t>(h) * a.num_blocks * block_bytes +
+                            row * int4_code_bytes(D) + group * 16;
+    const uint8_t* const k_codes = static_cast<const uint8_t*>(a.k_pool) + head_at;
+    const uint8_t* const v_codes = static_cast<const uint8_t*>(a.v_pool) + head_at;
+    const int32_t to_scales = a.block_size * int4_code_bytes(D) + row * int4_scale_bytes(D) +
+                              group * 2 - row * int4_code_bytes(D) - group * 16;
     // Half tiles of 32 keys in the order K(0), V(-1), K(1), V(0), K(2), V(1), ..: half
     // tile i is half i & 1 of K(i / 4) or, with bit 1, of V(i / 4 - 1).
     auto step_of = [&](int32_t i) { return (i >> 2) - ((i >> 1) & 1); };
     auto token_unit = [&](int32_t x) {  // of unit x of the range
       return x < sd.sink_units ? x : x - sd.sink_units + sd.first_unit;
     };
-    // Table entries of a half tile's two units (-1: past the range).
-    auto entries = [&](int32_t i, int32_t (&blk)[2]) {
-      const int32_t j = step_of(i), x0 = (j0 + j) * kUnits + 2 * (i & 1);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        blk[e] = -1;
-        if (j >= 0 && j < n && x0 + e < sd.units) {
-          const int32_t tu = token_unit(x0 + e);
-          blk[e] = __ldg(table + (block_units == 1 ? tu : tu / block_units));
-        }
+    // Table entries of units 32 q .. 32 q + 31 of the CTA's steps, a lane each, for an even and
+    // an odd q (-1: past the range).  Window q + 1 is loaded when K is 16 units into window q, which
+    // V, at most 8 behind it, has entered by then.
+    const int32_t unit0 = j0 * kUnits, units = min(n * kUnits, sd.units - unit0);
+    int32_t even = -1, odd = -1, windows = 0;
+    auto load_entries = [&]() {
+      const int32_t x = 32 * windows + lane;
+      int32_t blk = -1;
+      if (x < units) {
+        const int32_t tu = token_unit(unit0 + x);
+        blk = __ldg(table + (block_units == 1 ? tu : tu / block_units));
+      }
+      if (windows++ & 1) {
+        odd = blk;
+      } else {
+        even = blk;
       }
     };
+    load_entries();
+    load_entries();
     struct Codes {
       uint4 words[2][PARTS];
       uint32_t scale[2][PARTS];
     };
     int32_t plain_lo, plain_hi;
     plain_steps(a, sd, plain_lo, plain_hi);
-    const int32_t codes_lane = row * int4_code_bytes(D) + group * 16;
-    const int32_t scales_lane = a.block_size * int4_code_bytes(D) + row * int4_scale_bytes(D) + group * 2;
-    auto load = [&](int32_t i, const int32_t (&blk)[2], Codes& c) {
-      const int32_t j = step_of(i), x0 = (j0 + j) * kUnits + 2 * (i & 1);
+    auto load = [&](int32_t i, Codes& c) {
+      const int32_t j = step_of(i), x0 = j * kUnits + 2 * (i & 1);
+      if (j < 0 || x0 >= n * kUnits) return;
       const bool is_v = (i & 2) != 0;
-      const uint8_t* pool = static_cast<const uint8_t*>(is_v ? a.v_pool : a.k_pool) + head_at;
+      if (x0 + 16 >= 32 * windows) load_entries();
+      const int32_t win = (x0 & 32) != 0 ? odd : even;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const bool valid = blk[e] >= 0 && blk[e] < a.num_blocks;
-        if (!valid) {
-          if (lane == 0 && !is_v && j >= 0 && j < n && x0 + e < sd.units) {
-            set_status(a.status, kStatusBadBlock);
-          }
+        const int32_t blk = __shfl_sync(0xffffffffu, win, (x0 + e) & 31);
+        if (static_cast<uint32_t>(blk) >= static_cast<uint32_t>(a.num_blocks)) {
+          if (lane == 0 && !is_v && x0 + e < units) set_status(a.status, kStatusBadBlock);
 #pragma unroll
           for (int p = 0; p < PARTS; ++p) {
             c.words[e][p] = make_uint4(0u, 0u, 0u, 0u);
@@ -329,10 +340,10 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
           continue;
         }
-        const uint8_t* codes = pool + blk[e] * block_bytes + codes_lane;
-        const uint8_t* scales = pool + blk[e] * block_bytes + scales_lane;
+        const uint8_t* codes = (is_v ? v_codes : k_codes) + static_cast<int64_t>(blk) * block_bytes;
+        const uint8_t* scales = codes + to_scales;
         if (block_units != 1) {
-          const int32_t first = token_unit(x0 + e) % block_units * kUnit;
+          const int32_t first = token_unit(unit0 + x0 + e) % block_units * kUnit;
           codes += first * int4_code_bytes(D);
           scales += first * int4_scale_bytes(D);
         }
@@ -343,16 +354,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
     };
-    // Codes are loaded kAhead of this warp's half tiles ahead, table entries one more.
+    // Codes are loaded kAhead of this warp's half tiles ahead.
     constexpr int kAhead = 2;
     Codes codes[kAhead];
-    int32_t i = warp - kLoadKWarp, blk[2];
+    int32_t i = warp - kLoadKWarp;
 #pragma unroll
-    for (int x = 0; x < kAhead; ++x) {
-      entries(i + x * kWriters, blk);
-      load(i + x * kWriters, blk, codes[x]);
-    }
-    entries(i + kAhead * kWriters, blk);
+    for (int x = 0; x < kAhead; ++x) load(i + x * kWriters, codes[x]);
     bool ok = true;
     auto turn = [&](Codes& c) {
       const bool is_v = (i & 2) != 0;
@@ -362,7 +369,6 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (j >= (is_v ? C::VS : C::KS)) ok = wait_step(is_v ? j - C::VS + 2 : j - C::KS);
         if (!ok) return;
         const int stage = is_v ? j % C::VS : j % C::KS;
-        uint8_t* to = (is_v ? sV(stage) : sK(stage)) + (i & 1) * 32 * 128 + row_at;
         if (j0 + j < plain_lo || j0 + j > plain_hi) {
           // Rows that nobody sees may hold anything: their values are 0.  (Here, not where the
           // codes are loaded, which would wait for them.)
@@ -377,22 +383,26 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           }
         }
+        const uint32_t to = ring + ((is_v ? C::KS : 0) + stage) * C::STAGE_BYTES + (i & 1) * 32 * 128;
+        uint32_t at[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) at[k] = to + ((piece ^ k) << 4);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
           for (int p = 0; p < PARTS; ++p) {
-            const uint4 raw = c.words[e][p];
-            const bool turned = (group & 2) != 0;
-            const uint32_t words[4] = {turned ? raw.z : raw.x, turned ? raw.w : raw.y,
-                                       turned ? raw.x : raw.z, turned ? raw.y : raw.w};
+            const uint32_t words[4] = {c.words[e][p].x, c.words[e][p].y, c.words[e][p].z,
+                                       c.words[e][p].w};
             const uint32_t scale = __byte_perm(c.scale[e][p], 0, 0x1010);
             const uint32_t shift = int4_shift(scale);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               uint32_t v[4];
               int4_values(words[k], scale, shift, v);
-              *reinterpret_cast<uint4*>(to + (e * kUnit + p * ROWS) * 128 + ((piece ^ k) << 4)) =
-                  make_uint4(v[0], v[1], v[2], v[3]);
+              asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(
+                               at[k] + (e * kUnit + p * ROWS) * 128),
+                           "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+                           : "memory");
             }
           }
         }
@@ -401,8 +411,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (lane == 0) mbar_arrive(is_v ? &v_ok[stage] : &k_full[stage]);
       }
       i += kWriters;
-      load(i + (kAhead - 1) * kWriters, blk, c);
-      entries(i + kAhead * kWriters, blk);
+      load(i + (kAhead - 1) * kWriters, c);
     };
     const int32_t end = 4 * (n + 1);
     while (ok && i < end) {
