@@ -265,7 +265,7 @@ int plan_mma_decode(const WindowShape& s, MmaDecodePlan* p) {
 // How the tensor-core prefill runs a call: one CTA per 128-row query tile, kv head and
 // range of key steps.
 struct MmaChunkPlan {
-  int64_t tile_tokens, qtiles, items, splits, ml_offset, bytes;
+  int64_t tile_rows, tile_tokens, qtiles, items, splits, ml_offset, bytes;
 };
 
 constexpr int64_t kMaxRecordBytes = 64ll << 20;
@@ -274,7 +274,12 @@ int plan_mma_chunks(const WindowShape& s, MmaChunkPlan* p) {
   int sms = 0;
   if (int rc = bsb::sm_count(&sms)) return rc;
   const int64_t groups = s.heads / s.kv_heads;
-  p->tile_tokens = bsb::kWindowTileRows / groups;
+  // Over 4-bit pools two tiles share K and V, which are costly to write, where a chunk has
+  // rows for both; then one CTA runs on an SM, else two.
+  const bool both = s.int4 && s.max_query_len > bsb::kWindowTileRows / groups;
+  const int64_t resident = (both ? 1 : 2) * static_cast<int64_t>(sms);
+  p->tile_rows = (both ? 2 : 1) * bsb::kWindowTileRows;
+  p->tile_tokens = p->tile_rows / groups;
   p->qtiles = (s.max_query_len + p->tile_tokens - 1) / p->tile_tokens;
   p->items = product(product(s.rows, p->qtiles), s.kv_heads);
   if (p->items < 0 || p->items > kInt32Max / bsb::kMaxWindowRanges / 8) {
@@ -292,11 +297,11 @@ int plan_mma_chunks(const WindowShape& s, MmaChunkPlan* p) {
                                 std::min(s.window, kMaxContext) + std::min(s.sinks, kMaxContext) +
                                     p->tile_tokens + 32);
   const int64_t most = keys / (bsb::kWindowStepKeys * bsb::kMinWindowSteps);
-  const int64_t record = bsb::kWindowTileRows * (s.head_dim + 2) * 4;
+  const int64_t record = p->tile_rows * (s.head_dim + 2) * 4;
   p->splits = std::max<int64_t>(
-      1, std::min(std::min<int64_t>(2ll * sms / busy, bsb::kMaxWindowRanges), most));
+      1, std::min(std::min<int64_t>(resident / busy, bsb::kMaxWindowRanges), most));
   while (p->splits > 1 && p->items * p->splits * record > kMaxRecordBytes) --p->splits;
-  p->ml_offset = p->items * p->splits * bsb::kWindowTileRows * s.head_dim;
+  p->ml_offset = p->items * p->splits * p->tile_rows * s.head_dim;
   p->bytes = p->splits > 1 ? p->items * p->splits * record : 0;
   return BS_OK;
 }
@@ -428,6 +433,7 @@ int run_mma_chunks(const WindowShape& s, const WindowCall& c, bsb::WindowArgs& a
     if (int rc = bsb::pool_tensor_map(&kmap, c.key_pool, rows, s.head_dim)) return rc;
     if (int rc = bsb::pool_tensor_map(&vmap, c.value_pool, rows, s.head_dim)) return rc;
   }
+  a.tile_rows = static_cast<int32_t>(p.tile_rows);
   a.tile_tokens = static_cast<int32_t>(p.tile_tokens);
   a.qtiles = static_cast<int32_t>(p.qtiles);
   a.splits = static_cast<int32_t>(p.splits);

@@ -34,8 +34,9 @@ struct WindowArgs {
   int32_t num_heads, num_kv_heads, groups, head_dim, block_size, num_blocks;
   int32_t window, sinks;
   float scale;
-  // Query tiles of tile_tokens tokens per sequence (1 without cu_q).
-  int32_t tile_tokens, qtiles;
+  // Query tiles of tile_tokens tokens per sequence (1 without cu_q); tensor-core chunks: of
+  // tile_rows rows.
+  int32_t tile_tokens, qtiles, tile_rows;
   // A tile's keys are cut into up to `splits` ranges, one CTA each; with more
   // than one, a CTA leaves a record (O unnormalised, then row maxima in base 2
   // and row sums) that a second kernel merges in range order.
@@ -111,7 +112,8 @@ __host__ __device__ __forceinline__ int32_t window_range(int32_t count, int32_t 
 constexpr int kWindowSimtRows = 16;
 constexpr int kMaxWindowCluster = 8;  // CTAs of a cluster
 
-// Tensor-core chunks: rows of a query tile, the fewest steps of 64 keys in a range
+// Tensor-core chunks: rows of a query tile (4-bit pools: of a CTA's tiles, one or two), the
+// fewest steps of 64 keys in a range
 // and the most ranges.
 constexpr int kWindowTileRows = 128;
 constexpr int kWindowStepKeys = 64;

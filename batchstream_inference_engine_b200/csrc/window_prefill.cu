@@ -66,28 +66,33 @@ constexpr int kRows = 128;  // query rows of a tile (TMEM lanes)
 constexpr int kKeys = 64;   // keys of a step
 constexpr int kUnit = 16;   // tokens per unit (one TMA box)
 constexpr int kUnits = kKeys / kUnit;
-constexpr int kThreads = 256;
-constexpr int kMmaWarp = 4, kLoadKWarp = 5, kLoadVWarp = 6, kGuardWarp = 7;
 constexpr int kRing = 8;  // step barriers (>= K stages, >= V stages)
-constexpr uint32_t kTmemCols = 256;  // two S/P buffers, O
+constexpr uint32_t kTileCols = 256;  // TMEM columns of a tile: two S/P buffers, O
 constexpr float kLog2eP = 1.4426950408889634f;
 constexpr float kRescaleSlack = 8.f;
 constexpr float kFarMaximum = 1073741824.f;  // 2^30
 constexpr int kMaxBad = 64;  // listed keys with non-finite V (more: all are looked at)
 
-template <int D>
+// TILES query tiles share a CTA's K and V: one (two CTAs per SM, 8 warps each) or, over
+// 4-bit pools, two (one CTA per SM, 16 warps).
+template <int D, int TILES>
 struct Cfg {
+  static constexpr int ROWS = TILES * kRows;
+  static constexpr int MMA_WARP = 4 * TILES, LOAD_K_WARP = MMA_WARP + 1;
+  static constexpr int LOAD_V_WARP = MMA_WARP + 2, GUARD_WARP = MMA_WARP + 3;
+  static constexpr int THREADS = 256 * TILES, MIN_CTAS = 3 - TILES;
+  static constexpr int WRITERS = THREADS / 32 - LOAD_K_WARP;  // of K and V from 4-bit pools
   static constexpr int HALVES = D / 64;
-  // Stages of K and V: two CTAs share an SM's 227 KiB.
-  static constexpr int KS = D == 64 ? 5 : 2;
-  static constexpr int VS = D == 64 ? 5 : 2;
-  static constexpr int Q_HALF_BYTES = kRows * 128;  // 64 dims of 128 rows
+  // Stages of K and V: the CTAs of an SM share its 227 KiB.
+  static constexpr int KS = TILES == 2 ? (D == 64 ? 6 : 4) : (D == 64 ? 5 : 2);
+  static constexpr int VS = KS;
+  static constexpr int Q_HALF_BYTES = ROWS * 128;  // 64 dims of the rows
   static constexpr int Q_BYTES = HALVES * Q_HALF_BYTES;
   static constexpr int HALF_BYTES = kKeys * 128;
   static constexpr int STAGE_BYTES = HALVES * HALF_BYTES;
   static constexpr int SMEM_BYTES = Q_BYTES + (KS + VS) * STAGE_BYTES;
   static constexpr uint32_t O_COL = 2 * kKeys;  // behind the two S/P buffers
-  static_assert(O_COL + D <= kTmemCols, "TMEM columns");
+  static_assert(O_COL + D <= kTileCols, "TMEM columns");
   static_assert(KS <= kRing && VS <= kRing, "a step waiter could fall a whole ring behind");
 };
 
@@ -156,7 +161,7 @@ __device__ __forceinline__ void tile_of(const WindowArgs& a, int32_t item, int32
 }
 
 // Most sequences that every CTA ranks (one a thread).
-constexpr int kMaxRanked = kThreads;
+constexpr int kMaxRanked = 256;
 
 // The sequence, tile and kv head of launch index b: the sequences with the most
 // steps first, a sequence's last tiles, which see the most keys, ahead of its others.
@@ -196,15 +201,18 @@ __device__ __forceinline__ uint32_t fma_zero_bf16x2(uint32_t a, uint32_t c) {
   return d;
 }
 
-template <int D, bool Q4>
-__global__ void __launch_bounds__(kThreads, 2)
+template <int D, bool Q4, int TILES>
+__global__ void __launch_bounds__((Cfg<D, TILES>::THREADS), (Cfg<D, TILES>::MIN_CTAS))
     window_prefill_kernel(const __grid_constant__ CUtensorMap qmap,
                           const __grid_constant__ CUtensorMap kmap,
                           const __grid_constant__ CUtensorMap vmap, const WindowArgs a) {
-  using C = Cfg<D>;
+  static_assert(Q4 || TILES == 1, "the loaders and the guard are for one tile");
+  using C = Cfg<D, TILES>;
+  constexpr int kMmaWarp = C::MMA_WARP, kLoadKWarp = C::LOAD_K_WARP;
+  constexpr int kLoadVWarp = C::LOAD_V_WARP, kGuardWarp = C::GUARD_WARP;
   extern __shared__ __align__(1024) uint8_t smem[];  // 128-byte swizzle atoms
-  __shared__ uint64_t q_full, k_full[C::KS], v_full[C::VS], v_ok[C::VS], step_done[kRing],
-      p_full[2], mma_done;
+  __shared__ uint64_t q_full, k_full[C::KS], v_full[C::VS], v_ok[C::VS], step_done[TILES][kRing],
+      p_full[TILES][2], mma_done;
   __shared__ uint32_t tmem_base;
   __shared__ int32_t bad_count, bad_pos[kMaxBad];
 
@@ -237,8 +245,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(&v_full[s], 1);
       mbar_init(&v_ok[s], Q4 ? 2 : 1);
     }
-    for (int s = 0; s < kRing; ++s) mbar_init(&step_done[s], 1);
-    for (int b = 0; b < 2; ++b) mbar_init(&p_full[b], kRows);
+    for (int x = 0; x < TILES; ++x) {
+      for (int s = 0; s < kRing; ++s) mbar_init(&step_done[x][s], 1);
+      for (int b = 0; b < 2; ++b) mbar_init(&p_full[x][b], kRows);
+    }
     mbar_init(&mma_done, 1);
     fence_barrier_init();
     bad_count = 0;
@@ -247,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncwarp();  // thread 0 comes from the barriers' setup
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(&tmem_base)),
-                 "r"(kTmemCols));
+                 "r"(TILES * kTileCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tc_fence_before();
@@ -258,9 +268,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   auto wait_all = [&](uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
   };
-  // Step u is done: P V of step u - 2 and S of step u.  Waiters take the steps in order
-  // and are never kRing behind (see the ring sizes).
-  auto wait_step = [&](int u) { return wait_all(&step_done[u % kRing], (u / kRing) & 1); };
+  // Step u of a tile is done: P V of step u - 2 and S of step u (of the tiles before it too:
+  // they are issued first).  Waiters take the steps in order and are never kRing behind (see
+  // the ring sizes).
+  auto wait_step = [&](int u, int of = TILES - 1) {
+    return wait_all(&step_done[of][u % kRing], (u / kRing) & 1);
+  };
 
   if (Q4 && warp >= kLoadKWarp) {
     // ---------------------------------------------------------------- 4-bit K and V
@@ -275,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncwarp();
     }
     constexpr int NG = D / kInt4Group, ROWS = 32 / NG, PARTS = kUnit / ROWS;  // rows a load
-    constexpr int kWriters = 3;
+    constexpr int kWriters = C::WRITERS;
     const int32_t* table = a.block_tables + static_cast<int64_t>(w.row) * a.bt_stride;
     const int32_t block_units = a.block_size / kUnit;
     const int32_t block_bytes = a.block_size * int4_row_bytes(D);  // fits (host)
@@ -503,30 +516,33 @@ __global__ void __launch_bounds__(kThreads, 2)
       const bool pv = u > 1, qk = u < n;
       // P last: K and V are there long before it.
       if (qk) ok = wait_all(&k_full[ks], k_phase);
-      if (pv) {
-        ok = ok && wait_all(&v_ok[vs], v_phase);
-        ok = ok && wait_all(&p_full[b], ((u >> 1) & 1) ^ 1);  // of step u - 2
+      if (pv) ok = ok && wait_all(&v_ok[vs], v_phase);
+      if (!ok) break;
+#pragma unroll
+      for (int x = 0; x < TILES; ++x) {
+        if (pv) ok = wait_all(&p_full[x][b], ((u >> 1) & 1) ^ 1);  // of step u - 2
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t cols = tmem + x * kTileCols, s_col = cols + b * kKeys;
+        if (pv) {
+          const uint32_t v0 = v_lo + vs * kStageStep;
+          unroll<kKeys / 16>([&](auto k) {
+            // P: 8 columns per 16 keys; V: 16 rows of 128 bytes.
+            umma_f16_ts_elect<8 * k, 128 * k>(mine, cols + C::O_COL, s_col, v0, hi, kIdescO,
+                                              k > 0 || u > 2 ? 1u : 0u);
+          });
+        }
+        if (qk) {
+          const uint32_t q0 = q_lo + x * (kRows * 128 >> 4), k0 = k_lo + ks * kStageStep;
+          unroll<D / 16>([&](auto k) {
+            // 32 bytes a slice of 16 dims.
+            umma_f16_elect<(k / 4) * kQHalf + 2 * (k % 4), (k / 4) * kHalf + 2 * (k % 4)>(
+                mine, s_col, q0, k0, hi, kIdescS, k > 0 ? 1u : 0u);
+          });
+        }
+        umma_commit_elect(mine, &step_done[x][u % kRing]);
       }
       if (!ok) break;
-      tc_fence_after();
-      const uint32_t s_col = tmem + b * kKeys;
-      if (pv) {
-        const uint32_t v0 = v_lo + vs * kStageStep;
-        unroll<kKeys / 16>([&](auto k) {
-          // P: 8 columns per 16 keys; V: 16 rows of 128 bytes.
-          umma_f16_ts_elect<8 * k, 128 * k>(mine, tmem + C::O_COL, s_col, v0, hi, kIdescO,
-                                            k > 0 || u > 2 ? 1u : 0u);
-        });
-      }
-      if (qk) {
-        const uint32_t k0 = k_lo + ks * kStageStep;
-        unroll<D / 16>([&](auto k) {
-          // 32 bytes a slice of 16 dims.
-          umma_f16_elect<(k / 4) * kQHalf + 2 * (k % 4), (k / 4) * kHalf + 2 * (k % 4)>(
-              mine, s_col, q_lo, k0, hi, kIdescS, k > 0 ? 1u : 0u);
-        });
-      }
-      umma_commit_elect(mine, &step_done[u % kRing]);
       if (++ks == C::KS) {
         ks = 0;
         k_phase ^= 1u;
@@ -617,11 +633,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (!ok && lane == 0) set_status(a.status, kStatusWaitTimeout);
   } else {
     // ---------------------------------------------------------------- softmax
-    const int row = tid;
+    const int row = tid, own = warp / 4;  // row of the CTA's tiles; its tile
     const int32_t tok = row / a.groups, g = row - tok * a.groups;
     const bool live = tok < w.ntok;
     const int32_t qpos = w.pos0 + tok;
-    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t lane_base = (static_cast<uint32_t>(warp % 4 * 32) << 16) + own * kTileCols;
     const uint32_t o_addr = tmem + lane_base + C::O_COL;
     const float zscale = fabsf(a.scale) * kLog2eP;
     // Exponents are scale * score - scale * raw_used, the largest score used so far.  That
@@ -639,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     plain_steps(a, sd, plain_lo, plain_hi);
     bool ok = true;
     for (int32_t u = 0; u < n; ++u) {
-      ok = wait_step(u);
+      ok = wait_step(u, own);
       if (!ok) break;
       tc_fence_after();
       const uint32_t s_addr = tmem + lane_base + (u & 1) * kKeys;
@@ -691,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       } else if (__any_sync(0xffffffffu, grow)) {
         // O may be rescaled once P V of the step before is done; rows that did not
         // grow keep theirs (factor 1).
-        ok = wait_step(u + 1);
+        ok = wait_step(u + 1, own);
         if (!ok) break;
         tc_fence_after();
         const float corr = grow ? fast_exp2(__fmul_rn(raw_used, zscale) - __fmul_rn(raw, zscale)) : 1.f;
@@ -726,12 +742,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       tmem_st32(s_addr, p);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&p_full[u & 1]);
+      mbar_arrive(&p_full[own][u & 1]);
       l_run += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) +
                ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
     }
     // The last P V is done (the steps in order, as everywhere).
-    if (ok) ok = wait_step(n) && wait_step(n + 1);
+    if (ok) ok = wait_step(n, own) && wait_step(n + 1, own);
     if (!ok) {
       if (lane == 0) set_status(a.status, kStatusWaitTimeout);
     } else {
@@ -741,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int32_t bad = bad_count;
       const float scale = split_up ? 1.f : 1.f / l_run;
       const int32_t* table = a.block_tables + static_cast<int64_t>(w.row) * a.bt_stride;
-      const int64_t rec_row = (static_cast<int64_t>(item) * a.splits + split) * kRows + row;
+      const int64_t rec_row = (static_cast<int64_t>(item) * a.splits + split) * C::ROWS + row;
 #pragma unroll
       for (int c0 = 0; c0 < D; c0 += 32) {
         uint32_t v[32];
@@ -811,7 +827,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     tc_fence_after();
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                 "r"(kTmemCols));
+                 "r"(TILES * kTileCols));
   }
 }
 
@@ -823,34 +839,34 @@ constexpr int kMergeRows = kMergeThreads / 8;
 template <int D>
 __global__ void __launch_bounds__(kMergeThreads) window_prefill_merge_kernel(const WindowArgs a) {
   pdl_wait();
-  constexpr int kParts = kRows / kMergeRows;  // CTAs per tile
-  const int32_t item = blockIdx.x / kParts;
+  const int parts = a.tile_rows / kMergeRows;  // CTAs per tile
+  const int32_t item = blockIdx.x / parts;
   int32_t r, tile, h;
   tile_of(a, item, r, tile, h);
   WindowTile w;
   if (!window_tile(a, r, tile, w, false)) return;
-  const int32_t row = (blockIdx.x % kParts) * kMergeRows + threadIdx.x / 8;
+  const int32_t row = (blockIdx.x % parts) * kMergeRows + threadIdx.x / 8;
   const int32_t tok = row / a.groups, g = row - tok * a.groups;
   if (tok >= w.ntok) return;
   const Steps sd = steps_of(a, w);
   const int32_t ranges = step_ranges(step_count(sd), a.splits);
   if (ranges <= 1) return;  // written by the kernel itself
   const int32_t c = (threadIdx.x % 8) * (D / 8);
-  const int64_t rec0 = static_cast<int64_t>(item) * a.splits * kRows + row;
+  const int64_t rec0 = static_cast<int64_t>(item) * a.splits * a.tile_rows + row;
   const float* ml = a.records + a.rec_stride_ml;
   float M = -INFINITY;
-  for (int32_t s = 0; s < ranges; ++s) M = fmaxf(M, ml[(rec0 + s * kRows) * 2]);
+  for (int32_t s = 0; s < ranges; ++s) M = fmaxf(M, ml[(rec0 + s * a.tile_rows) * 2]);
   const float base = M == -INFINITY ? 0.f : M;
   float L = 0.f, acc[D / 8];
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) acc[i] = 0.f;
 #pragma unroll 4
   for (int32_t s = 0; s < ranges; ++s) {
-    const float2 p = *reinterpret_cast<const float2*>(ml + (rec0 + s * kRows) * 2);
+    const float2 p = *reinterpret_cast<const float2*>(ml + (rec0 + s * a.tile_rows) * 2);
     // A range without a finite score of this row weighs 0 (NaN scores: 0 * NaN).
     const float f = fast_exp2(p.x - base);
     L += f * p.y;
-    const float4* o = reinterpret_cast<const float4*>(a.records + (rec0 + s * kRows) * D + c);
+    const float4* o = reinterpret_cast<const float4*>(a.records + (rec0 + s * a.tile_rows) * D + c);
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
       const float4 v = o[i];
@@ -873,13 +889,13 @@ __global__ void __launch_bounds__(kMergeThreads) window_prefill_merge_kernel(con
   }
 }
 
-template <int D, bool Q4>
+template <int D, bool Q4, int TILES>
 int launch_d(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& kmap,
              const CUtensorMap& vmap, cudaStream_t stream) {
-  using C = Cfg<D>;
+  using C = Cfg<D, TILES>;
   static unsigned long long configured = 0;  // one bit per device
   cudaError_t e = once_per_device(&configured, [] {
-    return cudaFuncSetAttribute(window_prefill_kernel<D, Q4>,
+    return cudaFuncSetAttribute(window_prefill_kernel<D, Q4, TILES>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   });
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -889,14 +905,14 @@ int launch_d(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& km
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(items * a.splits));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM_BYTES;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, window_prefill_kernel<D, Q4>, qmap, kmap, vmap, a);
+  e = cudaLaunchKernelEx(&cfg, window_prefill_kernel<D, Q4, TILES>, qmap, kmap, vmap, a);
   if (e != cudaSuccess || a.splits == 1) return static_cast<int>(e);
-  cfg.gridDim = dim3(static_cast<unsigned>(items * (kRows / kMergeRows)));
+  cfg.gridDim = dim3(static_cast<unsigned>(items * (C::ROWS / kMergeRows)));
   cfg.blockDim = dim3(kMergeThreads);
   cfg.dynamicSmemBytes = 0;
   return static_cast<int>(cudaLaunchKernelEx(&cfg, window_prefill_merge_kernel<D>, a));
@@ -906,12 +922,16 @@ int launch_d(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& km
 
 int launch_window_prefill(const WindowArgs& a, const CUtensorMap& qmap, const CUtensorMap& kmap,
                           const CUtensorMap& vmap, cudaStream_t stream) {
-  if (a.int4) {  // (kmap and vmap are not used)
-    return a.head_dim == 64 ? launch_d<64, true>(a, qmap, kmap, vmap, stream)
-                            : launch_d<128, true>(a, qmap, kmap, vmap, stream);
+  if (a.int4 && a.tile_rows == 2 * kRows) {  // (kmap and vmap are not used)
+    return a.head_dim == 64 ? launch_d<64, true, 2>(a, qmap, kmap, vmap, stream)
+                            : launch_d<128, true, 2>(a, qmap, kmap, vmap, stream);
   }
-  return a.head_dim == 64 ? launch_d<64, false>(a, qmap, kmap, vmap, stream)
-                          : launch_d<128, false>(a, qmap, kmap, vmap, stream);
+  if (a.int4) {
+    return a.head_dim == 64 ? launch_d<64, true, 1>(a, qmap, kmap, vmap, stream)
+                            : launch_d<128, true, 1>(a, qmap, kmap, vmap, stream);
+  }
+  return a.head_dim == 64 ? launch_d<64, false, 1>(a, qmap, kmap, vmap, stream)
+                          : launch_d<128, false, 1>(a, qmap, kmap, vmap, stream);
 }
 
 }  // namespace bsb
