@@ -297,9 +297,13 @@ int plan_mma_chunks(const WindowShape& s, MmaChunkPlan* p) {
                                 std::min(s.window, kMaxContext) + std::min(s.sinks, kMaxContext) +
                                     p->tile_tokens + 32);
   const int64_t most = keys / (bsb::kWindowStepKeys * bsb::kMinWindowSteps);
+  // (4-bit chunks of one tile: as far as more than one wave goes.  64 chunks of 5 behind up to
+  // 8192 tokens, us with 1 / 2 / 3 ranges: d64 (128 tiles) -- / 99 / 74, d128 (256) 217 / 139 /
+  // 156; of two tiles the rule above holds: 8 of 128, d64, with 2 / 3: 27 / 37.)
+  const int64_t want = s.int4 && !both ? (resident + busy - 1) / busy : resident / busy;
   const int64_t record = p->tile_rows * (s.head_dim + 2) * 4;
   p->splits = std::max<int64_t>(
-      1, std::min(std::min<int64_t>(resident / busy, bsb::kMaxWindowRanges), most));
+      1, std::min(std::min<int64_t>(want, bsb::kMaxWindowRanges), most));
   while (p->splits > 1 && p->items * p->splits * record > kMaxRecordBytes) --p->splits;
   p->ml_offset = p->items * p->splits * p->tile_rows * s.head_dim;
   p->bytes = p->splits > 1 ? p->items * p->splits * record : 0;

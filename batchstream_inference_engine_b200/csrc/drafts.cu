@@ -15,7 +15,8 @@
 // draft_verify_kernel, a cluster per sequence, joins them, finds the row that ends the
 // step and draws from it alone, in fp64: the sums run over the whole vocabulary, and where
 // its tokens weigh 1e-5 each, an error of 1e-7 in the sum ahead of one moves one draw in a
-// hundred to its neighbour.
+// hundred to its neighbour.  Each warp sums a range of the row in blocks of 256 tokens and
+// keeps the sums of up to 64 parts of it, so that the draw walks one part again.
 #include "common.cuh"
 #include "drafts.cuh"
 
@@ -25,6 +26,9 @@ namespace {
 constexpr float kLog2eF = 1.4426950408889634f;
 constexpr int kStatThreads = 256;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kBlock = 256;  // tokens a warp weighs at a time
+constexpr int kParts = 64;   // of a warp's range, most
+constexpr int kKept = 32;    // rows of a sequence whose maximum is kept
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -80,60 +84,77 @@ __global__ void __launch_bounds__(kStatThreads) draft_stats_kernel(const DraftAr
       s_temp = a.temperature != nullptr ? a.temperature[b] : a.temperature_all;
     }
   }
-  // The first maximum.
+  // The maximum (fmaxf passes over NaN, which the sum finds).
   float top = -INFINITY;
-  int32_t arg = 0x7fffffff;
 #pragma unroll
   for (int k = 0; k < LOADS; ++k) {
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      const int32_t j = first + (k * kStatThreads + tid) * VE + i;
-      if (j >= 0 && j < a.vocab && ahead(v[k][i], j, top, arg)) {
-        top = v[k][i];
-        arg = j;
-      }
-    }
+    for (int i = 0; i < VE; i += 2) top = fmaxf(top, fmaxf(v[k][i], v[k][i + 1]));
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float t2 = __shfl_xor_sync(0xffffffffu, top, o);
-    const int32_t a2 = __shfl_xor_sync(0xffffffffu, arg, o);
-    if (ahead(t2, a2, top, arg)) {
-      top = t2;
-      arg = a2;
-    }
-  }
-  if (lane == 0) {
-    s_max[warp] = top;
-    s_arg[warp] = arg;
-  }
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) s_max[warp] = top;
   __syncthreads();
   if (s_seq < 0) {  // a row of no sequence
     if (piece == 0 && tid == 0) a.tokens[row] = -1;
     return;
   }
 #pragma unroll
-  for (int w = 0; w < kStatThreads / 32; ++w) {
-    if (ahead(s_max[w], s_arg[w], top, arg)) {
-      top = s_max[w];
-      arg = s_arg[w];
-    }
-  }
-  float sum = 0.f;
-  if (samples(s_temp) && top > -INFINITY && top < INFINITY) {
-    const float scale = fminf(kLog2eF / s_temp, 3e38f);
+  for (int w = 0; w < kStatThreads / 32; ++w) top = fmaxf(top, s_max[w]);
+  // The sum of exponentials where it is wanted, else only whether there is a NaN.
+  const bool finite = top > -INFINITY && top < INFINITY, weigh = samples(s_temp) && finite;
+  const float scale = weigh ? fminf(kLog2eF / s_temp, 3e38f) : 0.f;
+  float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  const float2 minus_top = make_float2(finite ? -top : 0.f, finite ? -top : 0.f);
+  const float2 scale2 = make_float2(scale, scale);
+  float sum;
+  if (weigh) {
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
 #pragma unroll
-      for (int i = 0; i < VE; ++i) sum += fast_exp2((v[k][i] - top) * scale);
+      for (int i = 0; i < VE; i += 2) {
+        const float2 z = __fmul2_rn(__fadd2_rn(make_float2(v[k][i], v[k][i + 1]), minus_top), scale2);
+        sums[i / 2 & 1] = __fadd2_rn(sums[i / 2 & 1], make_float2(fast_exp2(z.x), fast_exp2(z.y)));
+      }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) s_sum[warp] = sum;
-    __syncthreads();
+    sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+  } else {
     sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kStatThreads / 32; ++w) sum += s_sum[w];
+    for (int k = 0; k < LOADS; ++k) {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        if (v[k][i] != v[k][i]) sum = __int_as_float(0x7fffffff);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kStatThreads / 32; ++w) sum += s_sum[w];
+  // The first index of the maximum, NaN before all else, where the row may be decided by it.
+  const bool has_nan = sum != sum;
+  int32_t arg = 0x7fffffff;
+  if (!weigh || has_nan) {
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        const int32_t j = first + (k * kStatThreads + tid) * VE + i;
+        const bool hit = has_nan ? v[k][i] != v[k][i] : v[k][i] == top;
+        if (hit && j >= 0 && j < a.vocab) arg = min(arg, j);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) arg = min(arg, __shfl_xor_sync(0xffffffffu, arg, o));
+    if (lane == 0) s_arg[warp] = arg;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kStatThreads / 32; ++w) arg = min(arg, s_arg[w]);
+    if (has_nan) top = __int_as_float(0x7fffffff);
   }
   if (tid == 0) {
     a.records[static_cast<int64_t>(row) * a.pieces + piece] =
@@ -150,13 +171,14 @@ struct RowStats {
 __device__ __forceinline__ RowStats join_row(const DraftArgs& a, int32_t row, float temperature,
                                              int lane) {
   const float4* rec = a.records + static_cast<int64_t>(row) * a.pieces;
-  RowStats s{-INFINITY, 0.f, 0x7fffffff};
-  for (int32_t c = lane; c < a.pieces; c += 32) {
+  const float4 none = make_float4(-INFINITY, 0.f, __int_as_float(0x7fffffff), 0.f);
+  const float4 mine = lane < a.pieces ? __ldcg(rec + lane) : none;  // all there is, for most
+  RowStats s{mine.x, 0.f, __float_as_int(mine.z)};
+  for (int32_t c = lane + 32; c < a.pieces; c += 32) {
     const float4 r = __ldcg(rec + c);
-    const int32_t arg = __float_as_int(r.z);
-    if (ahead(r.x, arg, s.top, s.arg)) {
+    if (ahead(r.x, __float_as_int(r.z), s.top, s.arg)) {
       s.top = r.x;
-      s.arg = arg;
+      s.arg = __float_as_int(r.z);
     }
   }
 #pragma unroll
@@ -170,7 +192,8 @@ __device__ __forceinline__ RowStats join_row(const DraftArgs& a, int32_t row, fl
   }
   if (samples(temperature) && s.top > -INFINITY && s.top < INFINITY) {
     const float scale = fminf(kLog2eF / temperature, 3e38f);
-    for (int32_t c = lane; c < a.pieces; c += 32) {
+    if (mine.y > 0.f) s.sum = mine.y * fast_exp2((mine.x - s.top) * scale);
+    for (int32_t c = lane + 32; c < a.pieces; c += 32) {
       const float4 r = __ldcg(rec + c);
       if (r.y > 0.f) s.sum += r.y * fast_exp2((r.x - s.top) * scale);
     }
@@ -188,27 +211,46 @@ __device__ __forceinline__ double cluster_load64(const double* p, uint32_t rank)
   return v;
 }
 
-// Inclusive sums of the CTA's threads, in thread order.  All threads call it.
-__device__ __forceinline__ double block_scan(double v, double (&totals)[kWarps]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double n = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += n;
-  }
-  __syncthreads();  // the last use of totals
-  if (lane == 31) totals[warp] = v;
-  __syncthreads();
-  double before = 0.0;
-  for (int w = 0; w < warp; ++w) before += totals[w];
-  return before + v;
+// A logit's bits as the double of that value (of 0: 2^-127, which no sum notices; infinities
+// and NaN become large numbers).  Whole-number instructions: the fp64 units are what bounds the
+// draw.
+__device__ __forceinline__ double widen(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return __hiloint2double(static_cast<int32_t>((((u & 0x7fffffffu) >> 3) + (896u << 20)) |
+                                               (u & 0x80000000u)),
+                          static_cast<int32_t>(u << 29));
 }
 
+// exp(d / T) for d <= 0: 2^(k / 64) from a table times the series of e^(r ln 2 / 64) for the
+// rest, |r| <= 1/2, whose next term is below 2^-44 of it.  The constants live in registers (as
+// immediates each takes two moves at every use).
+struct Weigher {
+  const double* table;
+  double per_t, round, c4, c3, c2, c1;
+  __device__ __forceinline__ Weigher(const double* t, float temperature) : table(t) {
+    constexpr double kC = 0.010830424696249145;  // ln 2 / 64
+    per_t = 64.0 * 1.4426950408889634 / static_cast<double>(temperature);
+    round = 6755399441055744.0;  // 1.5 * 2^52: a sum's low bits are the nearest whole number
+    c4 = kC * kC * kC * kC / 24.0;
+    c3 = kC * kC * kC / 6.0;
+    c2 = kC * kC / 2.0;
+    c1 = kC;
+    asm volatile("" : "+d"(round), "+d"(c4), "+d"(c3), "+d"(c2), "+d"(c1));
+  }
+  __device__ __forceinline__ double operator()(double d) const {
+    const double t = fma(d, per_t, round);
+    const int32_t k = __double2loint(t);
+    const double r = fma(d, per_t, round - t);
+    const double e = fma(fma(fma(fma(r, c4, c3), r, c2), r, c1), r, 1.0) * table[k & 63];
+    return __hiloint2double(__double2hiint(e) + ((k >> 6) << 20), __double2loint(e));
+  }
+};
+
 template <typename T, typename Q>
-__global__ void __launch_bounds__(kThreads) draft_verify_kernel(const DraftArgs a) {
-  __shared__ int32_t s_first, s_arg;
-  __shared__ float s_top;
-  __shared__ double s_totals[kWarps], s_incl[kThreads], s_part;
+__global__ void __launch_bounds__(kThreads, 2) draft_verify_kernel(const DraftArgs a) {
+  __shared__ int32_t s_first, s_arg[kKept];
+  __shared__ float s_top[kKept];
+  __shared__ double s_exp2[64], s_parts[kWarps][kParts], s_warps[kWarps], s_all;
   pdl_wait();
   const int32_t b = blockIdx.x / a.ranks, rank = blockIdx.x % a.ranks;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -227,40 +269,56 @@ __global__ void __launch_bounds__(kThreads) draft_verify_kernel(const DraftArgs 
   }
   const float temperature = a.temperature != nullptr ? a.temperature[b] : a.temperature_all;
   const bool sampled = samples(temperature);
-  const double inv_t = sampled ? 1.0 / static_cast<double>(temperature) : 0.0;
+  if (tid < 64) s_exp2[tid] = exp2(tid / 64.0);
+  const Weigher weight(s_exp2, sampled ? temperature : 1.f);
+  // Below this the weight is 0 (2^-1000).
+  const float least = sampled ? -1000.f * 0.69314718f * temperature : 0.f;
   const T* logits = static_cast<const T*>(a.logits);
   const Q* probs = static_cast<const Q*>(a.draft_probs);
   if (tid == 0) s_first = n - 1;
   __syncthreads();
-  // The first draft that is not accepted.
-  for (int32_t i = warp; i < n - 1; i += kWarps) {
+  // The first draft that is not accepted; and what its row, or the last, ends with.
+  for (int32_t i = warp; i < n; i += kWarps) {
     const int32_t r = r0 + i, x = a.draft_tokens[r];
+    const bool draft = i < n - 1, known = x >= 0 && x < a.vocab;
+    float l = 0.f, q = 1.f, u = 0.f;
+    if (draft && known && sampled) {
+      l = to_float(logits[r * a.logits_stride + x]);
+      if (probs != nullptr) q = to_float(probs[r * a.probs_stride + x]);
+      u = a.uniforms[r];
+    }
     const RowStats s = join_row(a, r, temperature, lane);
-    if (lane == 0) {
+    if (lane == 0 && i < kKept) {
+      s_top[i] = s.top;
+      s_arg[i] = s.arg;
+    }
+    if (lane == 0 && draft) {
       bool take = false;
-      if (x < 0 || x >= a.vocab) {
+      if (!known) {
         set_status(a.status, kStatusBadIndex);
       } else if (!sampled) {
         take = x == s.arg;
-      } else if (s.top > -INFINITY && s.top < INFINITY) {
-        const double l = static_cast<double>(to_float(logits[r * a.logits_stride + x]));
-        const double p = exp((l - static_cast<double>(s.top)) * inv_t) / static_cast<double>(s.sum);
-        const double q =
-            probs != nullptr ? static_cast<double>(to_float(probs[r * a.probs_stride + x])) : 1.0;
-        take = static_cast<double>(a.uniforms[r]) * q < p;
+      } else if (s.top > -INFINITY && s.top < INFINITY && l - s.top > least) {
+        const double p = weight(widen(l) - widen(s.top)) / static_cast<double>(s.sum);
+        take = static_cast<double>(u) * static_cast<double>(q) < p;
       }
       if (!take) atomicMin(&s_first, i);
     }
   }
   __syncthreads();
   const int32_t taken = s_first, row = r0 + taken;
-  if (warp == 0) {
-    const RowStats s = join_row(a, row, temperature, lane);
-    if (lane == 0) {
-      s_top = s.top;
-      s_arg = s.arg;
+  if (taken >= kKept) {
+    if (warp == 0) {
+      const RowStats s = join_row(a, row, temperature, lane);
+      if (lane == 0) {
+        s_top[0] = s.top;
+        s_arg[0] = s.arg;
+      }
     }
+    __syncthreads();
   }
+  const float top = s_top[taken < kKept ? taken : 0];
+  const int32_t arg = s_arg[taken < kKept ? taken : 0];
   if (rank == 0) {
     for (int32_t i = tid; i < n; i += kThreads) {
       if (i != taken) a.tokens[r0 + i] = i < taken ? a.draft_tokens[r0 + i] : -1;
@@ -270,71 +328,108 @@ __global__ void __launch_bounds__(kThreads) draft_verify_kernel(const DraftArgs 
       if (!sampled && temperature != 0.f) set_status(a.status, kStatusBadValue);
     }
   }
-  __syncthreads();
-  const float top = s_top;
   const bool weighable = top > -INFINITY && top < INFINITY;
   if (!sampled || !weighable) {
     if (rank == 0 && tid == 0) {
-      a.tokens[row] = s_arg;
+      a.tokens[row] = arg;
       if (sampled) set_status(a.status, kStatusBadValue);
     }
     return;
   }
 
-  // The draw: this CTA's share of the vocabulary, a run of it to each thread.
+  // The draw: this CTA's share of the vocabulary, a range of it to each warp, lanes along it.
   const T* lrow = logits + row * a.logits_stride;
   const bool rejected = taken < n - 1;
   const int32_t x = rejected ? a.draft_tokens[row] : -1;
   const bool certain = rejected && probs == nullptr;
   const Q* qrow = rejected && !certain ? probs + row * a.probs_stride : nullptr;
-  const int32_t share = (a.vocab + a.ranks - 1) / a.ranks, run = (share + kThreads - 1) / kThreads;
-  const int32_t end = min(a.vocab, (rank + 1) * share);
-  const int32_t j0 = min(end, rank * share + tid * run), j1 = min(end, j0 + run);
-  const double top64 = static_cast<double>(top);
-  auto weight = [&](int32_t j) -> double {  // of p, not normalised
-    const float l = to_float(lrow[j]);
-    return l == -INFINITY || (certain && j == x) ? 0.0 : exp((static_cast<double>(l) - top64) * inv_t);
-  };
+  const int32_t blocks = (a.vocab + kBlock - 1) / kBlock;  // of the row
+  const int32_t all_warps = a.ranks * kWarps, me = rank * kWarps + warp;
+  const int32_t b0 = static_cast<int32_t>(static_cast<int64_t>(blocks) * me / all_warps);
+  const int32_t b1 = static_cast<int32_t>(static_cast<int64_t>(blocks) * (me + 1) / all_warps);
+  const int32_t per = (b1 - b0 + kParts - 1) / kParts;  // blocks of a part
+  const double top64 = widen(top);
   double inv_z = 0.0;
-  auto rest = [&](int32_t j) -> double {  // of p - q
-    const double d = weight(j) * inv_z - static_cast<double>(to_float(qrow[j]));
-    return d > 0.0 ? d : 0.0;
+  // A block's logits and draft probabilities, i of token 32 i + lane; their weights.
+  struct Block {
+    float l[kBlock / 32], q[kBlock / 32];
   };
-  // Sums of the CTAs ahead and of all, from this CTA's inclusive sums.
-  auto join = [&](double mine, double& before, double& all) {
-    const double incl = block_scan(mine, s_totals);
-    s_incl[tid] = incl;
-    if (tid == kThreads - 1) s_part = incl;
+  auto fetch = [&](int32_t block, bool rest, Block& b) {
+#pragma unroll
+    for (int i = 0; i < kBlock / 32; ++i) {
+      const int32_t j = block * kBlock + 32 * i + lane;
+      const bool there = j < a.vocab && !(certain && j == x);
+      b.l[i] = there ? to_float(lrow[j]) : -INFINITY;
+      b.q[i] = there && rest ? to_float(qrow[j]) : 0.f;
+    }
+  };
+  auto weigh = [&](const Block& b, bool rest, double (&w)[kBlock / 32]) {
+#pragma unroll
+    for (int i = 0; i < kBlock / 32; ++i) {
+      w[i] = weight(widen(b.l[i]) - top64);
+      if (rest) w[i] = fma(w[i], inv_z, -widen(b.q[i]));
+      // Nothing below `least` (or masked), nor where q is larger (of the high word: neither
+      // negative nor NaN).
+      const bool keep = b.l[i] - top > least && static_cast<uint32_t>(__double2hiint(w[i])) < 0x7ff00000u;
+      w[i] = __hiloint2double(keep ? __double2hiint(w[i]) : 0, keep ? __double2loint(w[i]) : 0);
+    }
+  };
+  // Sums of the weights of this warp's parts and of its range; then of the ranges ahead of it,
+  // of those ahead of the next, and of all (each range ends exactly where the next begins:
+  // the sums are formed in the same order).
+  auto add_up = [&](bool rest, double& before, double& before_next, double& all) {
+    double range = 0.0;
+    Block ahead_block;
+    if (b0 < b1) fetch(b0, rest, ahead_block);
+    for (int32_t p = 0, block = b0; block < b1; ++p) {
+      double sum = 0.0;
+      for (const int32_t end = min(block + per, b1); block < end; ++block) {
+        const Block now = ahead_block;
+        if (block + 1 < b1) fetch(block + 1, rest, ahead_block);
+        double w[kBlock / 32];
+        weigh(now, rest, w);
+        sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      range += sum;
+      if (lane == 0) s_parts[warp][p] = sum;
+    }
+    if (lane == 0) s_warps[warp] = range;
+    __syncthreads();
+    if (tid == 0) {
+      double t = 0.0;
+      for (int w = 0; w < kWarps; ++w) t += s_warps[w];
+      s_all = t;
+    }
     if (a.ranks > 1) {
       cluster_sync();
     } else {
       __syncthreads();
     }
-    before = all = 0.0;
+    double ctas = 0.0, warps = 0.0;
+    all = 0.0;
     for (int32_t k = 0; k < a.ranks; ++k) {
-      if (k == rank) before = all;
-      all += a.ranks > 1 ? cluster_load64(&s_part, k) : s_part;
+      if (k == rank) ctas = all;
+      all += a.ranks > 1 ? cluster_load64(&s_all, k) : s_all;
     }
-    if (a.ranks > 1) cluster_sync();  // s_part may be written again
-  };
-  double sum = 0.0, before, all;
-  for (int32_t j = j0; j < j1; ++j) sum += weight(j);
-  join(sum, before, all);
-  bool use_rest = false;
-  if (qrow != nullptr) {
-    inv_z = 1.0 / all;
-    const double p_sum = sum, p_before = before, p_all = all;
-    sum = 0.0;
-    for (int32_t j = j0; j < j1; ++j) sum += rest(j);
-    join(sum, before, all);
-    use_rest = all > 0.0;
-    if (!use_rest) {  // nothing is left: p itself
-      before = p_before;
-      all = p_all;
-      const double incl = block_scan(p_sum, s_totals);
-      s_incl[tid] = incl;
+    for (int w = 0; w < warp; ++w) warps += s_warps[w];
+    before = ctas + warps;
+    before_next = ctas + (warps + s_warps[warp]);
+    if (a.ranks > 1) {
+      cluster_sync();  // the sums may be written again
+    } else {
       __syncthreads();
     }
+  };
+  double before, before_next, all;
+  bool rest = qrow != nullptr;
+  add_up(false, before, before_next, all);
+  if (rest) {
+    inv_z = 1.0 / all;
+    add_up(true, before, before_next, all);
+    rest = all > 0.0;
+    if (!rest) add_up(false, before, before_next, all);  // nothing is left: p itself
   }
   if (!(all > 0.0)) {  // a certain draft that has all the weight
     if (rank == 0 && tid == 0) a.tokens[row] = x;
@@ -343,34 +438,60 @@ __global__ void __launch_bounds__(kThreads) draft_verify_kernel(const DraftArgs 
   double target = static_cast<double>(a.uniforms[r1 - 1]) * all;
   if (!(target < all)) target = all * (1.0 - 1.1102230246251565e-16);
   if (target < 0.0) target = 0.0;
-  // The thread whose run holds the token; its warp walks the run.
-  const double ahead_of = before + (tid > 0 ? s_incl[tid - 1] : 0.0);
-  const bool holds = ahead_of <= target && target < before + s_incl[tid];
-  const uint32_t who = __ballot_sync(0xffffffffu, holds);
-  if (who == 0) return;
-  const int src = __ffs(who) - 1;
-  const int32_t k0 = __shfl_sync(0xffffffffu, j0, src), k1 = __shfl_sync(0xffffffffu, j1, src);
-  double base = __shfl_sync(0xffffffffu, ahead_of, src);
-  int32_t last = -1;  // last token of any weight, should the run's sums fall short
-  for (int32_t k = k0; k < k1; k += 32) {
-    const int32_t j = k + lane;
-    const double own = j < k1 ? (use_rest ? rest(j) : weight(j)) : 0.0;
-    double incl = own;
+  // The warp whose range holds the token: every range ends where the next begins.
+  if (!(before <= target && target < before_next)) return;
+  // Its part.
+  double sums[kParts / 32], incl[kParts / 32], carry = 0.0;
+  int32_t part = -1, last = -1;
+#pragma unroll
+  for (int k = 0; k < kParts / 32; ++k) {
+    const int32_t p = 32 * k + lane;
+    sums[k] = p * per < b1 - b0 ? s_parts[warp][p] : 0.0;
+    incl[k] = sums[k];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const double v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
+      const double v = __shfl_up_sync(0xffffffffu, incl[k], o);
+      if (lane >= o) incl[k] += v;
     }
-    const uint32_t over = __ballot_sync(0xffffffffu, own > 0.0 && base + incl > target);
-    if (over != 0) {
-      last = k + __ffs(over) - 1;
-      break;
-    }
-    const uint32_t some = __ballot_sync(0xffffffffu, own > 0.0);
-    if (some != 0) last = k + 31 - __clz(some);
-    base += __shfl_sync(0xffffffffu, incl, 31);
+    incl[k] += carry;
+    carry = __shfl_sync(0xffffffffu, incl[k], 31);
+    const uint32_t some = __ballot_sync(0xffffffffu, sums[k] > 0.0);
+    const uint32_t over = __ballot_sync(0xffffffffu, sums[k] > 0.0 && before + incl[k] > target);
+    if (part < 0 && over != 0) part = 32 * k + __ffs(over) - 1;
+    if (some != 0) last = 32 * k + 31 - __clz(some);
   }
-  if (lane == 0) a.tokens[row] = last;
+  if (part < 0) part = last;  // (the parts' sums fell short of the range's)
+  double ahead_of = before;
+#pragma unroll
+  for (int k = 0; k < kParts / 32; ++k) {
+    const double v = __shfl_sync(0xffffffffu, incl[k] - sums[k], part & 31);
+    if (part / 32 == k) ahead_of += v;
+  }
+  int32_t token = -1;  // the last of any weight, should the part's sums fall short
+  for (int32_t block = b0 + part * per, end = min(block + per, b1); block < end; ++block) {
+    Block now;
+    fetch(block, rest, now);
+    double w[kBlock / 32];
+    weigh(now, rest, w);
+#pragma unroll
+    for (int i = 0; i < kBlock / 32; ++i) {
+      double sum = w[i];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      const uint32_t some = __ballot_sync(0xffffffffu, w[i] > 0.0);
+      const uint32_t over = __ballot_sync(0xffffffffu, w[i] > 0.0 && ahead_of + sum > target);
+      if (over != 0) {
+        if (lane == 0) a.tokens[row] = block * kBlock + 32 * i + __ffs(over) - 1;
+        return;
+      }
+      if (some != 0) token = block * kBlock + 32 * i + 31 - __clz(some);
+      ahead_of += __shfl_sync(0xffffffffu, sum, 31);
+    }
+  }
+  if (lane == 0) a.tokens[row] = token;
 }
 
 template <typename T, typename Q>
