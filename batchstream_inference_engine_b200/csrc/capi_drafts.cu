@@ -37,8 +37,8 @@ constexpr int64_t kInt32Max = 2147483647ll;
 
 // Pieces of a row: as many as it has when it begins at the end of a 16-byte unit.
 int64_t pieces_of(int64_t vocab, int32_t dtype) {
-  const int64_t shift = dtype == BS_BF16 ? 7 : 3;
-  return (vocab + shift + bsb::kDraftPiece - 1) / bsb::kDraftPiece;
+  const int64_t size = dtype == BS_BF16 ? 2 : 4, shift = 16 / size - 1;
+  return ((vocab + shift) * size + bsb::kDraftPieceBytes - 1) / bsb::kDraftPieceBytes;
 }
 
 int check_sizes(int64_t num_rows, int64_t vocab, int32_t dtype) {
@@ -106,10 +106,10 @@ int bs_verify_drafts(const void* logits, int64_t logits_row_stride, int32_t dtyp
   a.num_seqs = static_cast<int32_t>(num_seqs);
   a.vocab = static_cast<int32_t>(vocab);
   a.pieces = static_cast<int32_t>(pieces_of(vocab, dtype));
-  // CTAs that draw a sequence's token: two per SM over the batch, 4096 tokens each.
+  // CTAs that draw a sequence's token: one per SM over the batch, 4096 tokens each at least.
   a.ranks = static_cast<int32_t>(std::max<int64_t>(
       1, std::min({int64_t{bsb::kMaxDraftRanks},
-                   num_seqs > 0 ? int64_t{2} * sms / num_seqs : int64_t{1}, (vocab + 4095) / 4096})));
+                   num_seqs > 0 ? int64_t{sms} / num_seqs : int64_t{1}, (vocab + 4095) / 4096})));
   a.records = static_cast<float4*>(workspace);
   a.tokens = tokens_out;
   a.accepted = accepted_out;

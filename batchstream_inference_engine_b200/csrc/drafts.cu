@@ -46,10 +46,49 @@ __device__ __forceinline__ bool samples(float temperature) {
   return temperature > 0.f && temperature < INFINITY;
 }
 
+// N elements of a row as they lie in memory, in 32-bit words.
+template <typename T, int N>
+struct Raw {
+  static constexpr int PER = 4 / sizeof(T), WORDS = N / PER;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (PER == 1) return __uint_as_float(w[i]);
+    return __uint_as_float(i % 2 == 0 ? w[i / 2] << 16 : w[i / 2] & 0xffff0000u);
+  }
+  __device__ __forceinline__ void load(const T* p) {  // on 16 bytes
+#pragma unroll
+    for (int k = 0; k < WORDS; k += 4) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + k / 4);
+      w[k] = v.x;
+      w[k + 1] = v.y;
+      w[k + 2] = v.z;
+      w[k + 3] = v.w;
+    }
+  }
+  // Elements j .. j + N - 1 of a row, `out` where the row does not go or at `skip`.
+  __device__ __forceinline__ void load(const T* row, int32_t j, int32_t end, float out,
+                                       int32_t skip = -1) {
+#pragma unroll
+    for (int k = 0; k < WORDS; ++k) {
+      float e[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int32_t at = j + k * PER + i;
+        e[i] = at >= 0 && at < end && at != skip ? to_float(row[at]) : out;
+      }
+      if constexpr (PER == 1) {
+        w[k] = __float_as_uint(e[0]);
+      } else {
+        w[k] = (__float_as_uint(e[0]) >> 16) | (__float_as_uint(e[1]) & 0xffff0000u);
+      }
+    }
+  }
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kStatThreads) draft_stats_kernel(const DraftArgs a) {
+__global__ void __launch_bounds__(kStatThreads, 6) draft_stats_kernel(const DraftArgs a) {
   constexpr int VE = 16 / sizeof(T);  // elements of a 16-byte load
-  constexpr int LOADS = kDraftPiece / (kStatThreads * VE);
+  constexpr int LOADS = draft_piece<T>() / (kStatThreads * VE);
   __shared__ float s_max[kStatThreads / 32], s_sum[kStatThreads / 32], s_temp;
   __shared__ int32_t s_arg[kStatThreads / 32], s_seq;
   pdl_wait();
@@ -57,27 +96,21 @@ __global__ void __launch_bounds__(kStatThreads) draft_stats_kernel(const DraftAr
   const int32_t row = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) s_seq = -1;
-  __syncthreads();
-  // The row's 16-byte pieces, as memory is aligned: element j is `shift` + j of them.
+  // The row's 16-byte units, as memory is aligned: element j is `shift` + j of them.
   const T* logits = static_cast<const T*>(a.logits) + row * a.logits_stride;
   const int32_t shift = static_cast<int32_t>((reinterpret_cast<uintptr_t>(logits) & 15u) / sizeof(T));
-  const int32_t first = piece * kDraftPiece - shift;
-  float v[LOADS][VE];
+  const int32_t first = piece * draft_piece<T>() - shift + tid * VE;
+  Raw<T, VE> v[LOADS];
 #pragma unroll
   for (int k = 0; k < LOADS; ++k) {
-    const int32_t j = first + (k * kStatThreads + tid) * VE;
+    const int32_t j = first + k * kStatThreads * VE;
     if (j >= 0 && j + VE <= a.vocab) {
-      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(logits + j));
-      const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) v[k][i] = to_float(e[i]);
+      v[k].load(logits + j);
     } else {
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        v[k][i] = j + i >= 0 && j + i < a.vocab ? to_float(logits[j + i]) : -INFINITY;
-      }
+      v[k].load(logits, j, a.vocab, -INFINITY);
     }
   }
+  __syncthreads();
   for (int32_t b = tid; b < a.num_seqs; b += kStatThreads) {
     if (a.cu_rows[b] <= row && row < a.cu_rows[b + 1]) {
       s_seq = b;
@@ -89,7 +122,7 @@ __global__ void __launch_bounds__(kStatThreads) draft_stats_kernel(const DraftAr
 #pragma unroll
   for (int k = 0; k < LOADS; ++k) {
 #pragma unroll
-    for (int i = 0; i < VE; i += 2) top = fmaxf(top, fmaxf(v[k][i], v[k][i + 1]));
+    for (int i = 0; i < VE; i += 2) top = fmaxf(top, fmaxf(v[k].at(i), v[k].at(i + 1)));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -103,28 +136,27 @@ __global__ void __launch_bounds__(kStatThreads) draft_stats_kernel(const DraftAr
   for (int w = 0; w < kStatThreads / 32; ++w) top = fmaxf(top, s_max[w]);
   // The sum of exponentials where it is wanted, else only whether there is a NaN.
   const bool finite = top > -INFINITY && top < INFINITY, weigh = samples(s_temp) && finite;
-  const float scale = weigh ? fminf(kLog2eF / s_temp, 3e38f) : 0.f;
-  float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-  const float2 minus_top = make_float2(finite ? -top : 0.f, finite ? -top : 0.f);
-  const float2 scale2 = make_float2(scale, scale);
-  float sum;
+  float sum = 0.f;
   if (weigh) {
+    const float scale = fminf(kLog2eF / s_temp, 3e38f);
+    const float2 scale2 = make_float2(scale, scale), minus_top = make_float2(-top, -top);
+    float2 sums = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
 #pragma unroll
       for (int i = 0; i < VE; i += 2) {
-        const float2 z = __fmul2_rn(__fadd2_rn(make_float2(v[k][i], v[k][i + 1]), minus_top), scale2);
-        sums[i / 2 & 1] = __fadd2_rn(sums[i / 2 & 1], make_float2(fast_exp2(z.x), fast_exp2(z.y)));
+        const float2 z =
+            __fmul2_rn(__fadd2_rn(make_float2(v[k].at(i), v[k].at(i + 1)), minus_top), scale2);
+        sums = __fadd2_rn(sums, make_float2(fast_exp2(z.x), fast_exp2(z.y)));
       }
     }
-    sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+    sum = sums.x + sums.y;
   } else {
-    sum = 0.f;
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        if (v[k][i] != v[k][i]) sum = __int_as_float(0x7fffffff);
+        if (v[k].at(i) != v[k].at(i)) sum = __int_as_float(0x7fffffff);
       }
     }
   }
@@ -143,9 +175,9 @@ __global__ void __launch_bounds__(kStatThreads) draft_stats_kernel(const DraftAr
     for (int k = 0; k < LOADS; ++k) {
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        const int32_t j = first + (k * kStatThreads + tid) * VE + i;
-        const bool hit = has_nan ? v[k][i] != v[k][i] : v[k][i] == top;
-        if (hit && j >= 0 && j < a.vocab) arg = min(arg, j);
+        const int32_t j = first + k * kStatThreads * VE + i;
+        const float e = v[k].at(i);
+        if ((has_nan ? e != e : e == top) && j >= 0 && j < a.vocab) arg = min(arg, j);
       }
     }
 #pragma unroll
@@ -211,17 +243,26 @@ __device__ __forceinline__ double cluster_load64(const double* p, uint32_t rank)
   return v;
 }
 
-// A logit's bits as the double of that value (of 0: 2^-127, which no sum notices; infinities
-// and NaN become large numbers).  Whole-number instructions: the fp64 units are what bounds the
-// draw.
+// The double of a float that is not negative (of 0: 2^-127, which no sum notices; infinities
+// and NaN become large numbers).  Whole-number instructions: the fp64 units are what bounds
+// the draw.
 __device__ __forceinline__ double widen(float v) {
   const uint32_t u = __float_as_uint(v);
-  return __hiloint2double(static_cast<int32_t>((((u & 0x7fffffffu) >> 3) + (896u << 20)) |
-                                               (u & 0x80000000u)),
+  return __hiloint2double(static_cast<int32_t>((u >> 3) + (896u << 20)),
                           static_cast<int32_t>(u << 29));
 }
 
-// exp(d / T) for d <= 0: 2^(k / 64) from a table times the series of e^(r ln 2 / 64) for the
+// How far a logit lies below the largest, in fp64.  Of bf16 logits the fp32 difference is
+// exact, but for logits 2^16 times smaller than the largest: off by 2^-24 of that one at most,
+// which moves the weights of the few that there are by less than the sums can show.
+__device__ __forceinline__ double distance(__nv_bfloat16, float top, float l) {
+  return widen(top - l);
+}
+__device__ __forceinline__ double distance(float, float top, float l) {
+  return static_cast<double>(top) - static_cast<double>(l);
+}
+
+// exp(-d / T) for d >= 0: 2^(k / 64) from a table times the series of e^(r ln 2 / 64) for the
 // rest, |r| <= 1/2, whose next term is below 2^-44 of it.  The constants live in registers (as
 // immediates each takes two moves at every use).
 struct Weigher {
@@ -229,7 +270,7 @@ struct Weigher {
   double per_t, round, c4, c3, c2, c1;
   __device__ __forceinline__ Weigher(const double* t, float temperature) : table(t) {
     constexpr double kC = 0.010830424696249145;  // ln 2 / 64
-    per_t = 64.0 * 1.4426950408889634 / static_cast<double>(temperature);
+    per_t = -64.0 * 1.4426950408889634 / static_cast<double>(temperature);
     round = 6755399441055744.0;  // 1.5 * 2^52: a sum's low bits are the nearest whole number
     c4 = kC * kC * kC * kC / 24.0;
     c3 = kC * kC * kC / 6.0;
@@ -247,7 +288,7 @@ struct Weigher {
 };
 
 template <typename T, typename Q>
-__global__ void __launch_bounds__(kThreads, 2) draft_verify_kernel(const DraftArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) draft_verify_kernel(const DraftArgs a) {
   __shared__ int32_t s_first, s_arg[kKept];
   __shared__ float s_top[kKept];
   __shared__ double s_exp2[64], s_parts[kWarps][kParts], s_warps[kWarps], s_all;
@@ -271,8 +312,8 @@ __global__ void __launch_bounds__(kThreads, 2) draft_verify_kernel(const DraftAr
   const bool sampled = samples(temperature);
   if (tid < 64) s_exp2[tid] = exp2(tid / 64.0);
   const Weigher weight(s_exp2, sampled ? temperature : 1.f);
-  // Below this the weight is 0 (2^-1000).
-  const float least = sampled ? -1000.f * 0.69314718f * temperature : 0.f;
+  // From this distance on the weight is 0 (2^-1000).
+  const float most = sampled ? 1000.f * 0.69314718f * temperature : 0.f;
   const T* logits = static_cast<const T*>(a.logits);
   const Q* probs = static_cast<const Q*>(a.draft_probs);
   if (tid == 0) s_first = n - 1;
@@ -298,8 +339,9 @@ __global__ void __launch_bounds__(kThreads, 2) draft_verify_kernel(const DraftAr
         set_status(a.status, kStatusBadIndex);
       } else if (!sampled) {
         take = x == s.arg;
-      } else if (s.top > -INFINITY && s.top < INFINITY && l - s.top > least) {
-        const double p = weight(widen(l) - widen(s.top)) / static_cast<double>(s.sum);
+      } else if (s.top > -INFINITY && s.top < INFINITY && s.top - l < most) {
+        const double p = weight(static_cast<double>(s.top) - static_cast<double>(l)) /
+                         static_cast<double>(s.sum);
         take = static_cast<double>(u) * static_cast<double>(q) < p;
       }
       if (!take) atomicMin(&s_first, i);
@@ -343,34 +385,41 @@ __global__ void __launch_bounds__(kThreads, 2) draft_verify_kernel(const DraftAr
   const int32_t x = rejected ? a.draft_tokens[row] : -1;
   const bool certain = rejected && probs == nullptr;
   const Q* qrow = rejected && !certain ? probs + row * a.probs_stride : nullptr;
-  const int32_t blocks = (a.vocab + kBlock - 1) / kBlock;  // of the row
+  // 16-byte loads of 8 tokens a lane: blocks begin where the row's 16-byte units do, `shift`
+  // tokens ahead of it, if the draft probabilities' units are the same.
+  const int32_t shift = static_cast<int32_t>((reinterpret_cast<uintptr_t>(lrow) & 15u) / sizeof(T));
+  const bool wide = qrow == nullptr || ((reinterpret_cast<uintptr_t>(qrow) - shift * sizeof(Q)) & 15u) == 0;
+  const int32_t blocks = (a.vocab + shift + kBlock - 1) / kBlock;  // of the row
   const int32_t all_warps = a.ranks * kWarps, me = rank * kWarps + warp;
   const int32_t b0 = static_cast<int32_t>(static_cast<int64_t>(blocks) * me / all_warps);
   const int32_t b1 = static_cast<int32_t>(static_cast<int64_t>(blocks) * (me + 1) / all_warps);
   const int32_t per = (b1 - b0 + kParts - 1) / kParts;  // blocks of a part
-  const double top64 = widen(top);
   double inv_z = 0.0;
-  // A block's logits and draft probabilities, i of token 32 i + lane; their weights.
+  // A block's logits and draft probabilities, a lane's 8 tokens; their weights.
   struct Block {
-    float l[kBlock / 32], q[kBlock / 32];
+    Raw<T, 8> l;
+    Raw<Q, 8> q;
   };
   auto fetch = [&](int32_t block, bool rest, Block& b) {
-#pragma unroll
-    for (int i = 0; i < kBlock / 32; ++i) {
-      const int32_t j = block * kBlock + 32 * i + lane;
-      const bool there = j < a.vocab && !(certain && j == x);
-      b.l[i] = there ? to_float(lrow[j]) : -INFINITY;
-      b.q[i] = there && rest ? to_float(qrow[j]) : 0.f;
+    const int32_t j0 = block * kBlock - shift, j = j0 + lane * 8;
+    if (wide && j0 >= 0 && j0 + kBlock <= a.vocab && !(certain && x >= j0 && x < j0 + kBlock)) {
+      b.l.load(lrow + j);
+      if (rest) b.q.load(qrow + j);
+    } else {
+      b.l.load(lrow, j, a.vocab, -INFINITY, certain ? x : -1);
+      if (rest) b.q.load(qrow, j, a.vocab, 0.f);
     }
   };
-  auto weigh = [&](const Block& b, bool rest, double (&w)[kBlock / 32]) {
+  auto weigh = [&](const Block& b, bool rest, double (&w)[8]) {
 #pragma unroll
-    for (int i = 0; i < kBlock / 32; ++i) {
-      w[i] = weight(widen(b.l[i]) - top64);
-      if (rest) w[i] = fma(w[i], inv_z, -widen(b.q[i]));
-      // Nothing below `least` (or masked), nor where q is larger (of the high word: neither
-      // negative nor NaN).
-      const bool keep = b.l[i] - top > least && static_cast<uint32_t>(__double2hiint(w[i])) < 0x7ff00000u;
+    for (int i = 0; i < 8; ++i) {
+      const float l = b.l.at(i);
+      bool keep = top - l < most;
+      w[i] = weight(distance(T(), top, l));
+      if (rest) {  // where p is above q (of the high word: neither negative nor NaN)
+        w[i] = fma(w[i], inv_z, -widen(fabsf(b.q.at(i))));
+        keep = keep && static_cast<uint32_t>(__double2hiint(w[i])) < 0x7ff00000u;
+      }
       w[i] = __hiloint2double(keep ? __double2hiint(w[i]) : 0, keep ? __double2loint(w[i]) : 0);
     }
   };
@@ -386,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 2) draft_verify_kernel(const DraftAr
       for (const int32_t end = min(block + per, b1); block < end; ++block) {
         const Block now = ahead_block;
         if (block + 1 < b1) fetch(block + 1, rest, ahead_block);
-        double w[kBlock / 32];
+        double w[8];
         weigh(now, rest, w);
         sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
       }
@@ -471,25 +520,38 @@ __global__ void __launch_bounds__(kThreads, 2) draft_verify_kernel(const DraftAr
   for (int32_t block = b0 + part * per, end = min(block + per, b1); block < end; ++block) {
     Block now;
     fetch(block, rest, now);
-    double w[kBlock / 32];
+    double w[8], own = 0.0;
     weigh(now, rest, w);
 #pragma unroll
-    for (int i = 0; i < kBlock / 32; ++i) {
-      double sum = w[i];
+    for (int i = 0; i < 8; ++i) own += w[i];
+    double sum = own;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-      }
-      const uint32_t some = __ballot_sync(0xffffffffu, w[i] > 0.0);
-      const uint32_t over = __ballot_sync(0xffffffffu, w[i] > 0.0 && ahead_of + sum > target);
-      if (over != 0) {
-        if (lane == 0) a.tokens[row] = block * kBlock + 32 * i + __ffs(over) - 1;
-        return;
-      }
-      if (some != 0) token = block * kBlock + 32 * i + 31 - __clz(some);
-      ahead_of += __shfl_sync(0xffffffffu, sum, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const double v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
     }
+    // A lane's tokens: the first past the target, and the last of any weight.
+    double run = ahead_of + (sum - own);
+    int32_t hit = -1, some = -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      run += w[i];
+      if (w[i] > 0.0) {
+        some = i;
+        if (hit < 0 && run > target) hit = i;
+      }
+    }
+    const uint32_t over = __ballot_sync(0xffffffffu, hit >= 0);
+    if (over != 0) {
+      if (lane == __ffs(over) - 1) a.tokens[row] = block * kBlock - shift + lane * 8 + hit;
+      return;
+    }
+    const uint32_t any = __ballot_sync(0xffffffffu, some >= 0);
+    if (any != 0) {
+      const int src = 31 - __clz(any);
+      token = block * kBlock - shift + src * 8 + __shfl_sync(0xffffffffu, some, src);
+    }
+    ahead_of += __shfl_sync(0xffffffffu, sum, 31);
   }
   if (lane == 0) a.tokens[row] = token;
 }

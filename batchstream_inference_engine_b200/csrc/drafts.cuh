@@ -6,8 +6,12 @@
 
 namespace bsb {
 
-// Elements of a row that one CTA of the first pass takes.
-constexpr int kDraftPiece = 8192;
+// Bytes of a row that one CTA of the first pass takes, and elements.
+constexpr int kDraftPieceBytes = 16384;
+template <typename T>
+__host__ __device__ constexpr int draft_piece() {
+  return kDraftPieceBytes / static_cast<int>(sizeof(T));
+}
 constexpr int kMaxDraftRanks = 8;  // CTAs of a sequence's cluster
 
 struct DraftArgs {
