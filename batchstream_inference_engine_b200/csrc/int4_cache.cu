@@ -39,98 +39,133 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162f
 __device__ __forceinline__ void store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// Dims d .. d + 7 of a head and their partners' values: x, and y of the same pairs.  The
-// sign of the sine's term: -1 for a pair's first dim, 1 for its second, 0 past the rotary
-// dims.
-template <typename T, bool INTER, bool VEC>
-__device__ __forceinline__ void load_pairs(const AppendArgs& a, const T* head, int32_t d,
-                                           float (&x)[8], float (&y)[8]) {
+// Cos and sin of a token's pairs, times amp, as fp64 and rounded to fp32.
+struct Turns {
+  double2* exact;
+  float2* rounded;
+};
+
+// Dims d .. d + 7 of a head turned by the angles of their pairs: F is double (keys) or float
+// (queries).  VEC: the 8 dims lie on 16 bytes and are all a pair's first dims, all its second
+// (half layout), or whole pairs, or all past the rotary dims.
+template <typename T, bool INTER, bool VEC, typename F, typename F2>
+__device__ __forceinline__ void turned(const AppendArgs& a, const T* head, int32_t d,
+                                       const F2* turn, F (&out)[8]) {
   const int32_t half = a.rotary_dim >> 1;
+  float x[8], y[8];
   if constexpr (VEC) {
     load8(head + d, x);
+    if (d >= a.rotary_dim) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) out[j] = static_cast<F>(x[j]);
+      return;
+    }
     if constexpr (INTER) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = x[j ^ 1];
-    } else if (d < a.rotary_dim) {
-      load8(head + (d < half ? d + half : d - half), y);
+      for (int j = 0; j < 8; j += 2) {
+        const F2 cs = turn[(d + j) >> 1];
+        const F u = static_cast<F>(x[j]), v = static_cast<F>(x[j + 1]);
+        out[j] = fma(u, cs.x, -(v * cs.y));
+        out[j + 1] = fma(v, cs.x, u * cs.y);
+      }
+    } else {
+      const bool second = d >= half;
+      load8(head + (second ? d - half : d + half), y);
+      const F2* cs = turn + (second ? d - half : d);
+      const F sign = second ? F(1) : F(-1);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        out[j] = fma(static_cast<F>(x[j]), cs[j].x, sign * (static_cast<F>(y[j]) * cs[j].y));
+      }
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int32_t e = d + j;
-      x[j] = to_float(head[e]);
-      y[j] = 0.f;
-      if (e < a.rotary_dim) y[j] = to_float(head[INTER ? e ^ 1 : e < half ? e + half : e - half]);
+      const F u = static_cast<F>(to_float(head[e]));
+      if (e >= a.rotary_dim) {
+        out[j] = u;
+        continue;
+      }
+      const bool second = INTER ? (e & 1) != 0 : e >= half;
+      const F v = static_cast<F>(to_float(head[INTER ? e ^ 1 : second ? e - half : e + half]));
+      const F2 cs = turn[INTER ? e >> 1 : second ? e - half : e];
+      const F w = v * cs.y;
+      out[j] = fma(u, cs.x, second ? w : -w);
     }
   }
 }
 
-// Pair index of dim e, and whether it is the pair's second dim.
-template <bool INTER>
-__device__ __forceinline__ int32_t pair_of(int32_t e, int32_t half, bool& second) {
-  second = INTER ? (e & 1) != 0 : e >= half;
-  return INTER ? e >> 1 : second ? e - half : e;
-}
+// The magnitude of v rounded up to fp32.
+__device__ __forceinline__ float magnitude(float v) { return fabsf(v); }
+__device__ __forceinline__ float magnitude(double v) { return __double2float_ru(fabs(v)); }
+__device__ __forceinline__ bool negative(float v) { return __float_as_int(v) < 0; }
+__device__ __forceinline__ bool negative(double v) { return __double2hiint(v) < 0; }
 
 // 8 elements of a group that this thread and its three neighbours hold: writes the group's
 // share of codes and, on its first thread, the scale.  All 32 lanes call it.  Exact borders:
 // the fp32 quotient's code is corrected by the remainder x - s n, which is exact.
-template <typename V>
-__device__ __forceinline__ void quantise(const V (&x)[8], bool mine, int quad, uint32_t* codes,
+template <typename F>
+__device__ __forceinline__ void quantise(const F (&x)[8], bool mine, int quad, uint32_t* codes,
                                          uint16_t* scale, uint32_t* status) {
   // Largest elements of either side, rounded up to fp32 (which the 4-bit rounding up does not
-  // notice); NaN as infinity.
-  float hi = 0.f, lo = 0.f;
+  // notice) and compared by their bits, in which NaN is the largest.
+  float size[8];
+  uint32_t hi = 0, lo = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    float up, down;
-    if constexpr (sizeof(V) == 8) {
-      up = __double2float_ru(x[j]);
-      down = __double2float_ru(-x[j]);
+    size[j] = magnitude(x[j]);
+    const uint32_t bits = __float_as_uint(size[j]);
+    if (negative(x[j])) {
+      lo = max(lo, bits);
     } else {
-      up = x[j];
-      down = -x[j];
+      hi = max(hi, bits);
     }
-    if (!(x[j] == x[j])) up = down = INFINITY;
-    hi = fmaxf(hi, up);
-    lo = fmaxf(lo, down);
   }
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    lo = fmaxf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, o));
   }
-  const float top = fmaxf(hi, lo);
+  const uint32_t top = max(hi, lo);
   float s = 0.f;
-  if (top >= kHuge) {  // (infinity too)
+  if (top >= __float_as_uint(kHuge)) {  // (infinity and NaN too)
     if (mine && quad == 0) set_status(status, kStatusBadValue);
-  } else if (top >= kTiny) {
-    s = __uint_as_float((__float_as_uint(top * 0.125f) + 0xfffffu) & 0xfff00000u);
+  } else if (top >= __float_as_uint(kTiny)) {
+    s = __uint_as_float((__float_as_uint(__uint_as_float(top) * 0.125f) + 0xfffffu) & 0xfff00000u);
     if (lo < hi) s = -s;
   }
-  const float inv = s == 0.f ? 0.f : 1.f / s, limit = fabsf(s) * 0.5f;
-  uint32_t word = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float n = s == 0.f ? 0.f : rintf(static_cast<float>(x[j]) * inv);
-    const V rest = s == 0.f ? V(0) : fma(V(-n), V(s), x[j]);
-    const V far = rest < V(0) ? -rest : rest;
-    const bool odd = (static_cast<int>(n) & 1) != 0;
-    if (far > V(limit) || (far == V(limit) && odd)) n += (rest < V(0)) == (s < 0.f) ? 1.f : -1.f;
-    const int code = max(0, min(15, static_cast<int>(n) + 8));
-    word |= static_cast<uint32_t>(code) << (4 * ((j >> 1) + 4 * (j & 1)));
-  }
   if (!mine) return;
+  uint32_t word = 0x88888888u;  // zeros
+  if (s != 0.f) {
+    const float inv = 1.f / fabsf(s), limit = fabsf(s) * 0.5f;
+    word = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      // Of magnitudes; the sign comes last.
+      float n = rintf(size[j] * inv);
+      const F rest = fma(F(-n), F(fabsf(s)), x[j] < F(0) ? -x[j] : x[j]);
+      const F far = rest < F(0) ? -rest : rest;
+      if (far > F(limit) || (far == F(limit) && (static_cast<int>(n) & 1) != 0)) {
+        n += rest < F(0) ? -1.f : 1.f;
+      }
+      const int m = static_cast<int>(n), code = (negative(x[j]) != (s < 0.f) ? -m : m) + 8;
+      word |= static_cast<uint32_t>(min(15, code)) << (4 * ((j >> 1) + 4 * (j & 1)));
+    }
+  }
   *codes = word;
   if (quad == 0) *scale = static_cast<uint16_t>(__float_as_uint(s) >> 16);
 }
 
-template <typename T, bool INTER, bool VEC>
+// DIM: head_dim, or 0 for any.
+template <typename T, bool INTER, bool VEC, int DIM>
 __global__ void __launch_bounds__(kThreads) int4_append_kernel(const AppendArgs a) {
-  extern __shared__ double2 turn[];  // cos, sin of the pairs, times amp
+  extern __shared__ double2 shared_turns[];
   pdl_wait();
   pdl_trigger();
   const int32_t t = blockIdx.x;
+  const int32_t half = a.rotary_dim >> 1;
+  const Turns turn{shared_turns, reinterpret_cast<float2*>(shared_turns + half)};
   const int32_t slot = a.slots[t], p = a.rotary_dim > 0 ? a.pos[t] : 0;
   const bool bad_slot = slot >= a.num_blocks * a.block_size;  // fits in int32 (host)
   const bool rotate = p >= 0, append = slot >= 0 && !bad_slot;
@@ -138,36 +173,27 @@ __global__ void __launch_bounds__(kThreads) int4_append_kernel(const AppendArgs 
     if (p < 0) set_status(a.status, kStatusBadPosition);
     if (bad_slot) set_status(a.status, kStatusBadSlot);
   }
-  const int32_t half = a.rotary_dim >> 1;
   if (rotate) {
     for (int32_t i = threadIdx.x; i < half; i += kThreads) {
       const double turns = static_cast<double>(p) * a.freq[i] * kTurnsPerRad;
       double s, c;
       sincospi(2.0 * (turns - rint(turns)), &s, &c);
-      turn[i] = make_double2(c * a.amp, s * a.amp);
+      c *= a.amp;
+      s *= a.amp;
+      turn.exact[i] = make_double2(c, s);
+      turn.rounded[i] = make_float2(static_cast<float>(c), static_cast<float>(s));
     }
   }
   __syncthreads();
   const T* row = static_cast<const T*>(a.qkv) + t * a.qkv_stride;
-  const int32_t D = a.D, per = D >> 3;  // units of 8 dims a head
+  const int32_t D = DIM > 0 ? DIM : a.D, per = D >> 3;  // units of 8 dims a head
 
   if (rotate) {
     T* q_row = static_cast<T*>(a.q_out) + static_cast<int64_t>(t) * a.H * D;
     for (int32_t u = threadIdx.x; u < a.H * per; u += kThreads) {
       const int32_t h = u / per, d = (u - h * per) * 8;
-      float x[8], y[8];
-      load_pairs<T, INTER, VEC>(a, row + h * D, d, x, y);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (d + j < a.rotary_dim) {
-          bool second;
-          const double2 cs = turn[pair_of<INTER>(d + j, half, second)];
-          const float c = static_cast<float>(cs.x), s = static_cast<float>(cs.y);
-          y[j] = second ? fmaf(x[j], c, y[j] * s) : fmaf(x[j], c, -(y[j] * s));
-        } else {
-          y[j] = x[j];
-        }
-      }
+      float y[8];
+      turned<T, INTER, VEC>(a, row + h * D, d, turn.rounded, y);
       if constexpr (VEC) {
         store8(q_row + h * D + d, y);
       } else {
@@ -180,33 +206,36 @@ __global__ void __launch_bounds__(kThreads) int4_append_kernel(const AppendArgs 
 
   const int32_t blk = slot / a.block_size, off = slot - blk * a.block_size;
   const int64_t block_bytes = static_cast<int64_t>(a.block_size) * int4_row_bytes(D);
-  const int32_t units = 2 * a.Hkv * per;  // k heads, then v heads
-  for (int32_t u0 = threadIdx.x & ~31; u0 < units; u0 += kThreads) {
-    const int32_t u = min(u0 + static_cast<int32_t>(threadIdx.x & 31), units - 1);
-    const int32_t hh = u / per, d = (u - hh * per) * 8;
-    const bool is_v = hh >= a.Hkv;
-    const bool mine = u0 + static_cast<int32_t>(threadIdx.x & 31) < units && (is_v || rotate);
-    const T* head = row + (a.H + hh) * D;
-    float x[8], y[8];
-    load_pairs<T, INTER, VEC>(a, head, d, x, y);
-    uint8_t* block = (is_v ? a.v_pool : a.k_pool) +
-                     (static_cast<int64_t>(is_v ? hh - a.Hkv : hh) * a.num_blocks + blk) * block_bytes;
-    uint32_t* codes =
-        reinterpret_cast<uint32_t*>(block + off * int4_code_bytes(D) + (d >> 1));
-    uint16_t* scale = reinterpret_cast<uint16_t*>(block + a.block_size * int4_code_bytes(D) +
-                                                  off * int4_scale_bytes(D)) + d / kInt4Group;
-    double v[8];
+  const int32_t units = a.Hkv * per;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = static_cast<double>(x[j]);
-      if (!is_v && rotate && d + j < a.rotary_dim) {
-        bool second;
-        const double2 cs = turn[pair_of<INTER>(d + j, half, second)];
-        const double w = static_cast<double>(y[j]) * cs.y;
-        v[j] = second ? fma(v[j], cs.x, w) : fma(v[j], cs.x, -w);
+  for (int part = 0; part < 2; ++part) {  // k heads, v heads
+    const T* heads = row + (a.H + part * a.Hkv) * D;
+    uint8_t* pool = part == 0 ? a.k_pool : a.v_pool;
+    // (Keys from the first warp on, values from the last down: few heads keep all warps busy.)
+    const int32_t first = part == 0 ? threadIdx.x : kThreads - 32 - (threadIdx.x & ~31) + (threadIdx.x & 31);
+    for (int32_t u0 = first & ~31; u0 < units; u0 += kThreads) {
+      const int32_t own = u0 + static_cast<int32_t>(threadIdx.x & 31), u = min(own, units - 1);
+      const int32_t hh = u / per, d = (u - hh * per) * 8;
+      uint8_t* block = pool + (static_cast<int64_t>(hh) * a.num_blocks + blk) * block_bytes;
+      uint32_t* codes = reinterpret_cast<uint32_t*>(block + off * int4_code_bytes(D) + (d >> 1));
+      uint16_t* scale = reinterpret_cast<uint16_t*>(block + a.block_size * int4_code_bytes(D) +
+                                                    off * int4_scale_bytes(D)) + d / kInt4Group;
+      const int quad = threadIdx.x & 3;
+      if (part == 0 && a.rotary_dim > 0) {
+        double v[8];
+        turned<T, INTER, VEC>(a, heads + hh * D, d, turn.exact, v);
+        quantise(v, own < units && rotate, quad, codes, scale, a.status);
+      } else {
+        float v[8];
+        if constexpr (VEC) {
+          load8(heads + hh * D + d, v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = to_float(heads[hh * D + d + j]);
+        }
+        quantise(v, own < units, quad, codes, scale, a.status);
       }
     }
-    quantise(v, mine, threadIdx.x & 3, codes, scale, a.status);
   }
 }
 
@@ -266,14 +295,20 @@ int launch_append_t(const AppendArgs& a, int32_t ntok, bool interleaved, bool ve
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ntok);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(double2) * (a.rotary_dim / 2);
+  cfg.dynamicSmemBytes = (sizeof(double2) + sizeof(float2)) * (a.rotary_dim / 2);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  auto kernel = vec ? (interleaved ? int4_append_kernel<T, true, true>
-                                   : int4_append_kernel<T, false, true>)
-                    : (interleaved ? int4_append_kernel<T, true, false>
-                                   : int4_append_kernel<T, false, false>);
+  auto kernel = int4_append_kernel<T, false, false, 0>;
+  if (!vec) {
+    if (interleaved) kernel = int4_append_kernel<T, true, false, 0>;
+  } else if (a.D == 64) {
+    kernel = interleaved ? int4_append_kernel<T, true, true, 64> : int4_append_kernel<T, false, true, 64>;
+  } else if (a.D == 128) {
+    kernel = interleaved ? int4_append_kernel<T, true, true, 128> : int4_append_kernel<T, false, true, 128>;
+  } else {
+    kernel = interleaved ? int4_append_kernel<T, true, true, 0> : int4_append_kernel<T, false, true, 0>;
+  }
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, a));
 }
 
