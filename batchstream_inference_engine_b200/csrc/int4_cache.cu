@@ -164,6 +164,13 @@ __global__ void __launch_bounds__(kThreads) int4_append_kernel(const AppendArgs 
   pdl_wait();
   pdl_trigger();
   const int32_t t = blockIdx.x;
+  const T* row = static_cast<const T*>(a.qkv) + t * a.qkv_stride;
+  const int32_t D = DIM > 0 ? DIM : a.D, per = D >> 3;  // units of 8 dims a head
+  // The token's row will be wanted once its angles are there.
+  for (int64_t at = threadIdx.x * 128ll; at < (a.H + 2 * a.Hkv) * D * static_cast<int64_t>(sizeof(T));
+       at += kThreads * 128) {
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(reinterpret_cast<const char*>(row) + at));
+  }
   const int32_t half = a.rotary_dim >> 1;
   const Turns turn{shared_turns, reinterpret_cast<float2*>(shared_turns + half)};
   const int32_t slot = a.slots[t], p = a.rotary_dim > 0 ? a.pos[t] : 0;
@@ -184,36 +191,16 @@ __global__ void __launch_bounds__(kThreads) int4_append_kernel(const AppendArgs 
       turn.rounded[i] = make_float2(static_cast<float>(c), static_cast<float>(s));
     }
   }
-  __syncthreads();
-  const T* row = static_cast<const T*>(a.qkv) + t * a.qkv_stride;
-  const int32_t D = DIM > 0 ? DIM : a.D, per = D >> 3;  // units of 8 dims a head
-
-  if (rotate) {
-    T* q_row = static_cast<T*>(a.q_out) + static_cast<int64_t>(t) * a.H * D;
-    for (int32_t u = threadIdx.x; u < a.H * per; u += kThreads) {
-      const int32_t h = u / per, d = (u - h * per) * 8;
-      float y[8];
-      turned<T, INTER, VEC>(a, row + h * D, d, turn.rounded, y);
-      if constexpr (VEC) {
-        store8(q_row + h * D + d, y);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) store(q_row + h * D + d + j, y[j]);
-      }
-    }
-  }
-  if (!append) return;
-
-  const int32_t blk = slot / a.block_size, off = slot - blk * a.block_size;
+  const int32_t at = append ? slot : 0, blk = at / a.block_size, off = at - blk * a.block_size;
   const int64_t block_bytes = static_cast<int64_t>(a.block_size) * int4_row_bytes(D);
   const int32_t units = a.Hkv * per;
-#pragma unroll
-  for (int part = 0; part < 2; ++part) {  // k heads, v heads
-    const T* heads = row + (a.H + part * a.Hkv) * D;
-    uint8_t* pool = part == 0 ? a.k_pool : a.v_pool;
-    // (Keys from the first warp on, values from the last down: few heads keep all warps busy.)
-    const int32_t first = part == 0 ? threadIdx.x : kThreads - 32 - (threadIdx.x & ~31) + (threadIdx.x & 31);
-    for (int32_t u0 = first & ~31; u0 < units; u0 += kThreads) {
+  auto store_heads = [&](bool keys) {
+    const T* heads = row + (a.H + (keys ? 0 : a.Hkv)) * D;
+    uint8_t* pool = keys ? a.k_pool : a.v_pool;
+    // Values from the last warp down: they are there before the angles, which the first warps
+    // work on.
+    const int32_t first = keys ? threadIdx.x & ~31 : kThreads - 32 - (threadIdx.x & ~31);
+    for (int32_t u0 = first; u0 < units; u0 += kThreads) {
       const int32_t own = u0 + static_cast<int32_t>(threadIdx.x & 31), u = min(own, units - 1);
       const int32_t hh = u / per, d = (u - hh * per) * 8;
       uint8_t* block = pool + (static_cast<int64_t>(hh) * a.num_blocks + blk) * block_bytes;
@@ -221,7 +208,7 @@ __global__ void __launch_bounds__(kThreads) int4_append_kernel(const AppendArgs 
       uint16_t* scale = reinterpret_cast<uint16_t*>(block + a.block_size * int4_code_bytes(D) +
                                                     off * int4_scale_bytes(D)) + d / kInt4Group;
       const int quad = threadIdx.x & 3;
-      if (part == 0 && a.rotary_dim > 0) {
+      if (keys && a.rotary_dim > 0) {
         double v[8];
         turned<T, INTER, VEC>(a, heads + hh * D, d, turn.exact, v);
         quantise(v, own < units && rotate, quad, codes, scale, a.status);
@@ -234,6 +221,24 @@ __global__ void __launch_bounds__(kThreads) int4_append_kernel(const AppendArgs 
           for (int j = 0; j < 8; ++j) v[j] = to_float(heads[hh * D + d + j]);
         }
         quantise(v, own < units, quad, codes, scale, a.status);
+      }
+    }
+  };
+  if (append) store_heads(false);
+  __syncthreads();
+  if (append) store_heads(true);
+  if (rotate) {
+    T* q_row = static_cast<T*>(a.q_out) + static_cast<int64_t>(t) * a.H * D;
+    // (From the last thread down: the first have the keys.)
+    for (int32_t u = kThreads - 1 - threadIdx.x; u < a.H * per; u += kThreads) {
+      const int32_t h = u / per, d = (u - h * per) * 8;
+      float y[8];
+      turned<T, INTER, VEC>(a, row + h * D, d, turn.rounded, y);
+      if constexpr (VEC) {
+        store8(q_row + h * D + d, y);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) store(q_row + h * D + d + j, y[j]);
       }
     }
   }
