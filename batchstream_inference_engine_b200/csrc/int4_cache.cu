@@ -138,18 +138,20 @@ __device__ __forceinline__ void quantise(const F (&x)[8], bool mine, int quad, u
   if (!mine) return;
   uint32_t word = 0x88888888u;  // zeros
   if (s != 0.f) {
-    const float inv = 1.f / fabsf(s), limit = fabsf(s) * 0.5f;
+    float inv;  // (near enough: the remainder tells)
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(fabsf(s)));
+    const float limit = fabsf(s) * 0.5f;
     word = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      // Of magnitudes; the sign comes last.
-      float n = rintf(size[j] * inv);
-      const F rest = fma(F(-n), F(fabsf(s)), x[j] < F(0) ? -x[j] : x[j]);
+      // Of magnitudes; the sign comes last.  A sum with 1.5 * 2^23 has the nearest whole number
+      // in its low bits.
+      const float near = fmaf(size[j], inv, 12582912.f);
+      int m = __float_as_int(near) - 0x4b400000;
+      const F rest = fma(F(12582912.f - near), F(fabsf(s)), x[j] < F(0) ? -x[j] : x[j]);
       const F far = rest < F(0) ? -rest : rest;
-      if (far > F(limit) || (far == F(limit) && (static_cast<int>(n) & 1) != 0)) {
-        n += rest < F(0) ? -1.f : 1.f;
-      }
-      const int m = static_cast<int>(n), code = (negative(x[j]) != (s < 0.f) ? -m : m) + 8;
+      if (far > F(limit) || (far == F(limit) && (m & 1) != 0)) m += rest < F(0) ? -1 : 1;
+      const int code = (negative(x[j]) != (s < 0.f) ? -m : m) + 8;
       word |= static_cast<uint32_t>(min(15, code)) << (4 * ((j >> 1) + 4 * (j & 1)));
     }
   }
@@ -230,15 +232,44 @@ __global__ void __launch_bounds__(kThreads) int4_append_kernel(const AppendArgs 
   if (rotate) {
     T* q_row = static_cast<T*>(a.q_out) + static_cast<int64_t>(t) * a.H * D;
     // (From the last thread down: the first have the keys.)
-    for (int32_t u = kThreads - 1 - threadIdx.x; u < a.H * per; u += kThreads) {
-      const int32_t h = u / per, d = (u - h * per) * 8;
-      float y[8];
-      turned<T, INTER, VEC>(a, row + h * D, d, turn.rounded, y);
-      if constexpr (VEC) {
-        store8(q_row + h * D + d, y);
-      } else {
+    const int32_t me = kThreads - 1 - static_cast<int32_t>(threadIdx.x);
+    if constexpr (VEC && !INTER) {
+      // 8 pairs at a time: dims d and those half the rotary dims on; then the dims behind.
+      const int32_t pairs = half >> 3, rest = (D - a.rotary_dim) >> 3;
+      for (int32_t u = me; u < a.H * pairs; u += kThreads) {
+        const int32_t h = u / pairs, d = (u - h * pairs) * 8;
+        const T* src = row + h * D + d;
+        T* dst = q_row + h * D + d;
+        float x[8], y[8];
+        load8(src, x);
+        load8(src + half, y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) store(q_row + h * D + d + j, y[j]);
+        for (int j = 0; j < 8; ++j) {
+          const float2 cs = turn.rounded[d + j];
+          const float v = fmaf(x[j], cs.x, -(y[j] * cs.y));
+          y[j] = fmaf(y[j], cs.x, x[j] * cs.y);
+          x[j] = v;
+        }
+        store8(dst, x);
+        store8(dst + half, y);
+      }
+      for (int32_t u = me; u < a.H * rest; u += kThreads) {
+        const int32_t h = u / rest, e = h * D + a.rotary_dim + (u - h * rest) * 8;
+        float x[8];
+        load8(row + e, x);
+        store8(q_row + e, x);
+      }
+    } else {
+      for (int32_t u = me; u < a.H * per; u += kThreads) {
+        const int32_t h = u / per, d = (u - h * per) * 8;
+        float y[8];
+        turned<T, INTER, VEC>(a, row + h * D, d, turn.rounded, y);
+        if constexpr (VEC) {
+          store8(q_row + h * D + d, y);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) store(q_row + h * D + d + j, y[j]);
+        }
       }
     }
   }
