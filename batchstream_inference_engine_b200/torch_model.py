@@ -246,13 +246,18 @@ class PagedKVPool:
     """Device-resident K/V pool [layers, kv_heads, blocks, block_size, head_dim]
     with the reference's allocator and a device mirror of its block tables
     (src/server/torch_model.py:115-137).  ``dtype`` is bf16 as in the reference;
-    fp32 pools serve fp32 parity runs."""
+    fp32 pools serve fp32 parity runs, and torch.uint8 makes 4-bit pools
+    (``ops.int4_pool_shape``), which hold 3.5 times as many tokens as bf16 ones."""
 
     def __init__(self, config: ModelConfig, num_blocks: int, block_size: int,
                  device: torch.device | str = "cuda", dtype: torch.dtype = torch.bfloat16,
                  max_seqs: int = 256, max_blocks_per_seq: int | None = None):
         self.device = torch.device(device)
+        self.int4 = dtype == torch.uint8
         shape = (config.num_layers, config.num_kv_heads, num_blocks, block_size, config.head_dim)
+        if self.int4:
+            shape = (config.num_layers, *ops.int4_pool_shape(config.num_kv_heads, num_blocks,
+                                                             block_size, config.head_dim))
         self.keys = torch.zeros(shape, dtype=dtype, device=self.device)
         self.values = torch.zeros(shape, dtype=dtype, device=self.device)
         self.block_size = block_size
@@ -395,7 +400,8 @@ class TorchModel:
         # Rotary tables exactly as the reference makes them (fp32 angles on the
         # CPU, cos/sin rounded to bf16, torch_model.py:199-200, 289-292), built
         # once for every position and gathered per step on the device.
-        # Other rotary forms go from frequencies instead (ops.rotary_append).
+        # Other rotary forms go from frequencies instead (ops.rotary_append), and so does every
+        # form into 4-bit pools (_frequencies).
         if config.rotary_from_tables:
             steps = torch.arange(0, config.head_dim, 2, dtype=torch.float)
             inverse_frequencies = 1.0 / (config.rope_theta ** (steps / config.head_dim))
@@ -404,10 +410,9 @@ class TorchModel:
             angles = torch.cat((frequencies, frequencies), dim=-1)
             self.cos = angles.cos().to(torch.bfloat16).to(device=self.device, dtype=dtype)
             self.sin = angles.sin().to(torch.bfloat16).to(device=self.device, dtype=dtype)
-        else:
-            self.rope_frequencies, self.rope_amplitude = ops.rope_frequencies(
-                config.rotary_dim or config.head_dim, config.rope_theta, config.rope_scaling,
-                device=self.device)
+        self.rope_frequencies = None
+        if not config.rotary_from_tables:
+            self._frequencies()
         self._bounded = bool(config.attention_window) or not config.rotary_from_tables
         self.max_position = max_position
         # Per-step accounting for benchmarks: forwards, tokens and rows
@@ -438,6 +443,14 @@ class TorchModel:
         model_dir = Path(model_dir)
         config = ModelConfig.from_file(model_dir / "config.json")
         return cls(config, load_safetensors(model_dir / "model.safetensors"), device, dtype)
+
+    def _frequencies(self) -> torch.Tensor:
+        """Rotary frequencies on the device, made once; sets rope_amplitude too."""
+        if self.rope_frequencies is None:
+            c = self.config
+            self.rope_frequencies, self.rope_amplitude = ops.rope_frequencies(
+                c.rotary_dim or c.head_dim, c.rope_theta, c.rope_scaling, device=self.device)
+        return self.rope_frequencies
 
     # ---------------------------------------------------------------- public
 
@@ -472,6 +485,43 @@ class TorchModel:
         pool.last_ids[: ids.numel()].copy_(ids)
         return self._pending(pool, ids, list(range(len(groups))))
 
+    @torch.inference_mode()
+    def verify_tokens(self, groups: list[tuple[list[int], PagedKVCache]],
+                      temperature: float | torch.Tensor = 0.0,
+                      uniforms: torch.Tensor | None = None,
+                      draft_probs: torch.Tensor | None = None) -> list[list[int]]:
+        """A step that verifies drafted tokens (``ops.verify_drafts``): each group's tokens are
+        its next input token and the drafts behind it.  Returns, for each group, the drafts
+        that were accepted and the token after them; the cache then holds the input token
+        and the accepted drafts.  With temperature 0 these are the tokens that as many
+        greedy steps would give.  ``uniforms`` (fp32, one per input token) is needed for
+        other temperatures (a number, or one per group on the device); ``draft_probs``
+        [input tokens, vocab] holds, in the row of the token ahead of each draft, what it was
+        drawn from (None: drafts were certain)."""
+        if any(t < 0 for tokens, _ in groups for t in tokens):
+            raise RuntimeError("verify_tokens: token references cannot be verified")
+        pool = groups[0][1]._pool
+        lengths = [len(tokens) for tokens, _ in groups]
+        T = sum(lengths)
+        if uniforms is None:
+            if torch.is_tensor(temperature) or temperature != 0.0:
+                raise RuntimeError("verify_tokens: a temperature needs uniforms")
+            uniforms = torch.zeros(T, device=self.device)
+        logits = F.linear(self._hidden(groups, list(range(T))), self.embed)
+        offsets = [0]
+        for n in lengths:
+            offsets.append(offsets[-1] + n)
+        staged = self._stage(offsets + [t for tokens, _ in groups for t in (*tokens[1:], 0)])
+        out, accepted = ops.verify_drafts(logits, staged[len(offsets):], staged[: len(offsets)],
+                                          uniforms, temperature, draft_probs)
+        host = torch.cat([out, accepted]).tolist()
+        self._raise_status()
+        self.stats["d2h_bytes"] += 4 * len(host)
+        taken = host[T:]
+        self._advance(pool, [(tokens[: 1 + n], cache)
+                             for (tokens, cache), n in zip(groups, taken)])
+        return [host[at: at + n + 1] for at, n in zip(offsets, taken)]
+
     def _pending(self, pool: PagedKVPool, ids: torch.Tensor, index: list[int]) -> PendingTokens:
         """Copies `ids` to one of a few pinned buffers and records the event the
         host waits on; at most len(self._hosts) - 1 steps may be pending."""
@@ -486,10 +536,10 @@ class TorchModel:
         # Kernels report bad input in the status words of their stream (eager
         # calls: this stream; graph replays: the capture stream's): copied after
         # the step, read with the ids.  The second word of a stream is that of the
-        # operators of bounded caches, and of the pool's block copies.
+        # operators of bounded and 4-bit caches, and of the pool's block copies.
         words = ops.status_words(self.device)
         words += self._graph_status or []
-        if not self._bounded and not pool.copies:
+        if not self._bounded and not pool.copies and not pool.int4:
             words = words[::2]
         status.fill_(0)
         for i, word in enumerate(words):
@@ -523,7 +573,19 @@ class TorchModel:
         return staged
 
     def _last_hidden(self, groups) -> torch.Tensor:
-        config = self.config
+        """The final-normed hidden states of each group's last token, whose tokens are cached
+        from here on."""
+        ends, at = [], -1
+        for tokens, _ in groups:
+            at += len(tokens)
+            ends.append(at)
+        last = self._hidden(groups, ends)
+        self._advance(groups[0][1]._pool, groups)
+        return last
+
+    def _hidden(self, groups, ends: list[int]) -> torch.Tensor:
+        """The final-normed hidden states of the tokens `ends` of the groups', all in a row.
+        The tokens' keys and values are written, but not yet counted as cached."""
         pool = groups[0][1]._pool
         for tokens, cache in groups:
             cache.reserve(len(tokens))
@@ -537,28 +599,26 @@ class TorchModel:
         self._check_positions(starts, lengths)
         rows = [alloc.row(cache.seq_id) for _, cache in groups]
         flat = [t for tokens, _ in groups for t in tokens]
-        ends = [sum(lengths[: i + 1]) - 1 for i in range(R)]
+        E = len(ends)
         # Context lengths after the step are known here: the decode kernel gets
         # them as final at launch (lens_ready) and partitions its work while the
         # K/V write before it is still running.
         after = [st + n for st, n in zip(starts, lengths)]
         staged = self._stage(rows + starts + lengths + ends + after + flat)
-        rows_d, start_d, n_d, ends_d, ctx_d, tokens_d = (
-            staged[:R], staged[R:2 * R], staged[2 * R:3 * R], staged[3 * R:4 * R],
-            staged[4 * R:5 * R], staged[5 * R:])
+        rows_d, start_d, n_d, ends_d, ctx_d, tokens_d = staged.split([R, R, R, E, R, T])
         # Leading single-token rows run through the batched decode kernel, the
         # rest (prompt chunks) through the chunked-prefill kernel.
         n_dec = 0
         while n_dec < R and lengths[n_dec] == 1:
             n_dec += 1
-        if n_dec == R:
+        if n_dec == R and not pool.int4:
             # One token per row: positions are the start positions; one locate
             # launch gives the slots.
             positions = start_d
             _, slots = ops.decode_append(None, None, pool.keys[0], pool.values[0],
                                          alloc.device_tables, start_d, seq_rows=rows_d)
             cu_q = ctx = None
-        else:
+        else:  # (4-bit pools too: decode_append checks its pools)
             cu_q, positions, slots, ctx = ops.step_metadata(
                 alloc.device_tables, start_d, n_d, T, pool.block_size, pool.num_blocks,
                 seq_rows=rows_d)
@@ -574,7 +634,6 @@ class TorchModel:
                                     max_chunk, rows_d[n_dec:], attended[n_dec:])
 
         last = self._layers(pool, self._resolve(pool, tokens_d), positions, slots, ends_d, attend)
-        self._advance(pool, groups)
         st = self.stats
         st["steps"] += 1
         st["tokens"] += T
@@ -592,7 +651,11 @@ class TorchModel:
     def _attend_tokens(self, q, kp, vp, tables, lens, rows, out) -> None:
         """One layer's attention of the rows that hold one new token each."""
         c = self.config
-        if c.attention_window:
+        if kp.dtype == torch.uint8:
+            ops.int4_attention_batched(q, kp, vp, tables, lens, c.head_dim ** -0.5,
+                                       c.attention_window, c.attention_sinks, seq_rows=rows,
+                                       out=out)
+        elif c.attention_window:
             ops.window_attention_batched(q, kp, vp, tables, lens, c.head_dim ** -0.5,
                                          c.attention_window, c.attention_sinks, seq_rows=rows,
                                          out=out)
@@ -604,7 +667,11 @@ class TorchModel:
     def _attend_chunks(self, q, kp, vp, tables, cu_q, lens, max_query_len, rows, out) -> None:
         """One layer's attention of the prompt chunks."""
         c = self.config
-        if c.attention_window:
+        if kp.dtype == torch.uint8:
+            ops.int4_prefill_attention(q, kp, vp, tables, cu_q, lens, c.head_dim ** -0.5,
+                                       max_query_len, c.attention_window, c.attention_sinks,
+                                       seq_rows=rows, out=out)
+        elif c.attention_window:
             ops.window_prefill_attention(q, kp, vp, tables, cu_q, lens, c.head_dim ** -0.5,
                                          max_query_len, c.attention_window, c.attention_sinks,
                                          seq_rows=rows, out=out)
@@ -662,7 +729,11 @@ class TorchModel:
                 normed = ops.rms_norm(hidden, lw["ln1"], eps, add=delta, sum_out=hidden)
             qkv = F.linear(normed, lw["qkv_w"], lw["qkv_b"])
             kp, vp = pool.keys[layer], pool.values[layer]
-            if config.rotary_from_tables:
+            if pool.int4:
+                ops.rotary_append_int4(qkv, self._frequencies(), positions, slots, kp, vp, H,
+                                       interleaved=config.rope_interleaved,
+                                       amplitude=self.rope_amplitude, query_out=q)
+            elif config.rotary_from_tables:
                 ops.rope_append(qkv, self.cos, self.sin, positions, slots, kp, vp, H, query_out=q)
             else:
                 ops.rotary_append(qkv, self.rope_frequencies, positions, slots, kp, vp, H,
