@@ -218,31 +218,33 @@ constexpr int64_t kMaxSegmentCtas = 8;
 // 2048 (16): 25.4 / 21.2.
 bool clusters_win(int64_t c, int64_t most) { return most <= c * 4 * (c >= 4 ? 16 : 9); }
 
-int plan_mma_decode(const WindowShape& s, MmaDecodePlan* p) {
+// `seqs` sequences of `rows` query rows a kv head, of `tokens` query tokens each.
+int plan_mma_decode(const WindowShape& s, int64_t seqs, int64_t rows, int64_t tokens,
+                    MmaDecodePlan* p) {
   int sms = 0, dev = 0;
   if (int rc = bsb::sm_count(&sms)) return rc;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-  const int64_t groups = s.heads / s.kv_heads;
-  // Resident CTAs per SM by device, [4-bit pools][head_dim 128][more than 8 heads a group].
-  static std::atomic<int> per_sm[64][2][2][2];
+  // Resident CTAs per SM by device, [bf16 pools, 4-bit ones, those with chunks][head_dim
+  // 128][more than 8 rows].
+  static std::atomic<int> per_sm[64][3][2][2];
   std::atomic<int>* known =
-      dev < 64 ? &per_sm[dev][s.int4][s.head_dim == 128][groups > 8] : nullptr;
+      dev < 64 ? &per_sm[dev][s.int4 ? 1 + s.chunks : 0][s.head_dim == 128][rows > 8] : nullptr;
   int ctas = known != nullptr ? known->load() : 0;
   if (ctas == 0) {
-    const auto ctas_per_sm =
-        s.int4 ? bsb::decode_int4_ctas_per_sm : bsb::window_decode_mma_ctas_per_sm;
-    ctas = ctas_per_sm(static_cast<int>(s.head_dim), static_cast<int>(groups));
+    const int dim = static_cast<int>(s.head_dim), r = static_cast<int>(rows);
+    ctas = s.int4 ? bsb::decode_int4_ctas_per_sm(dim, r, s.chunks)
+                  : bsb::window_decode_mma_ctas_per_sm(dim, r);
     if (ctas <= 0) return fail(BS_ERR_CUDA, "occupancy query for window decode failed (%d)", ctas);
     if (known != nullptr) known->store(ctas);
   }
   // Units the batch can hold: a window of n tokens touches n / 16 + 1 of them.
   // Fewer than one unit a warp would only add records to merge.
   const int64_t unit = bsb::kWindowUnit;
-  const int64_t seen = (std::min(s.window, kMaxContext) + unit - 1) / unit + 1 +
+  const int64_t seen = (std::min(s.window, kMaxContext) + tokens - 1 + unit - 1) / unit + 1 +
                        (std::min(s.sinks, kMaxContext) + unit - 1) / unit;
   const int64_t most = std::min(seen, s.max_blocks * s.block_size / unit);
-  const int64_t resident = static_cast<int64_t>(sms) * ctas, segments = s.rows * s.kv_heads;
+  const int64_t resident = static_cast<int64_t>(sms) * ctas, segments = seqs * s.kv_heads;
   p->segment_ctas = 0;
   if (segments > 0 && segments <= resident) {
     const int64_t c = std::min({kMaxSegmentCtas, std::max<int64_t>(resident / segments, 1),
@@ -254,11 +256,34 @@ int plan_mma_decode(const WindowShape& s, MmaDecodePlan* p) {
       return BS_OK;
     }
   }
-  const int64_t units = s.rows * s.kv_heads * most;
+  const int64_t units = segments * most;
   p->grid = std::max<int64_t>(1, std::min(resident, (units + 3) / 4));
-  p->rec_stride = bsb::decode_record_stride(groups, s.head_dim);
+  p->rec_stride = bsb::decode_record_stride(rows, s.head_dim);
   p->tasks_offset = (2 * p->grid * p->rec_stride * 4 + 255) / 256 * 256;
   p->bytes = p->tasks_offset + p->grid * static_cast<int64_t>(sizeof(bsb::MergeTask));
+  return BS_OK;
+}
+
+// How the tensor-core decode runs short chunks over 4-bit pools: a chunk is a sequence with
+// as many times the heads as it may have tokens.
+struct ShortChunkPlan {
+  int64_t lists_offset, bytes;
+  MmaDecodePlan decode;
+};
+
+// Whether it runs them: up to two tiles of 8 rows.  FIGURES
+bool short_chunks(const WindowShape& s) {
+  return s.int4 && s.chunks && mma_shape(s) && s.max_query_len > 0 &&
+         s.max_query_len <= bsb::kShortChunkRows / (s.heads / s.kv_heads);
+}
+
+int plan_short_chunks(const WindowShape& s, ShortChunkPlan* p) {
+  if (int rc = plan_mma_decode(s, s.rows, s.max_query_len * (s.heads / s.kv_heads),
+                               s.max_query_len, &p->decode)) {
+    return rc;
+  }
+  p->lists_offset = (p->decode.bytes + 255) / 256 * 256;
+  p->bytes = p->lists_offset + s.rows * 16;
   return BS_OK;
 }
 
@@ -321,9 +346,14 @@ int window_workspace(const WindowShape& s, uint64_t* bytes_out) {
     MmaChunkPlan m;
     if (int rc = plan_mma_chunks(s, &m)) return rc;
     need = std::max(need, m.bytes);
+    if (short_chunks(s)) {
+      ShortChunkPlan c;
+      if (int rc = plan_short_chunks(s, &c)) return rc;
+      need = std::max(need, c.bytes);
+    }
   } else if (mma_shape(s)) {
     MmaDecodePlan m;
-    if (int rc = plan_mma_decode(s, &m)) return rc;
+    if (int rc = plan_mma_decode(s, s.rows, s.heads / s.kv_heads, 1, &m)) return rc;
     need = std::max(need, m.bytes);
   }
   *bytes_out = static_cast<uint64_t>(need);
@@ -366,16 +396,8 @@ bool mma_pointers(const WindowCall& c) {
          aligned16(c.output) && c.q_stride % 8 == 0 && c.o_stride % 8 == 0;
 }
 
-int run_mma_decode(const WindowShape& s, const WindowCall& c) {
-  MmaDecodePlan p;
-  if (int rc = plan_mma_decode(s, &p)) return rc;
-  if (int rc = check_workspace(c, p.bytes)) return rc;
-  CUtensorMap kmap, vmap;
-  if (!s.int4) {
-    const int64_t rows = s.kv_heads * c.num_blocks * s.block_size;
-    if (int rc = bsb::pool_tensor_map(&kmap, c.key_pool, rows, s.head_dim)) return rc;
-    if (int rc = bsb::pool_tensor_map(&vmap, c.value_pool, rows, s.head_dim)) return rc;
-  }
+// The arguments of the tensor-core decode that are alike for single tokens and chunks.
+bsb::DecodeArgs decode_args(const WindowShape& s, const WindowCall& c, const MmaDecodePlan& p) {
   bsb::DecodeArgs a{};
   a.q = c.query;
   a.q_stride_seq = c.q_stride;
@@ -407,6 +429,20 @@ int run_mma_decode(const WindowShape& s, const WindowCall& c) {
   a.window = static_cast<int32_t>(std::min(s.window, kMaxContext));
   a.sinks = static_cast<int32_t>(std::min(s.sinks, kMaxContext));
   a.block_units = static_cast<int32_t>(s.block_size / bsb::kWindowUnit);
+  return a;
+}
+
+int run_mma_decode(const WindowShape& s, const WindowCall& c) {
+  MmaDecodePlan p;
+  if (int rc = plan_mma_decode(s, s.rows, s.heads / s.kv_heads, 1, &p)) return rc;
+  if (int rc = check_workspace(c, p.bytes)) return rc;
+  CUtensorMap kmap, vmap;
+  if (!s.int4) {
+    const int64_t rows = s.kv_heads * c.num_blocks * s.block_size;
+    if (int rc = bsb::pool_tensor_map(&kmap, c.key_pool, rows, s.head_dim)) return rc;
+    if (int rc = bsb::pool_tensor_map(&vmap, c.value_pool, rows, s.head_dim)) return rc;
+  }
+  bsb::DecodeArgs a = decode_args(s, c, p);
   const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
   int rc;
   if (s.int4) {
@@ -417,6 +453,32 @@ int run_mma_decode(const WindowShape& s, const WindowCall& c) {
   }
   if (rc != 0) return cuda_fail(rc, "window decode launch");
   bsb::add_kernel_launches(p.segment_ctas > 0 ? 1 : 2);  // the decode and its merge pass
+  return BS_OK;
+}
+
+int run_short_chunks(const WindowShape& s, const WindowCall& c, bsb::WindowArgs& w) {
+  ShortChunkPlan p;
+  if (int rc = plan_short_chunks(s, &p)) return rc;
+  if (int rc = check_workspace(c, p.bytes)) return rc;
+  int2* rows = reinterpret_cast<int2*>(static_cast<uint8_t*>(c.workspace) + p.lists_offset);
+  int32_t* lens = reinterpret_cast<int32_t*>(rows + s.rows);
+  int32_t* table_rows = lens + s.rows;
+  w.tile_tokens = w.max_query_len;
+  const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
+  if (int rc = bsb::launch_chunk_rows(w, rows, lens, table_rows, stream)) {
+    return cuda_fail(rc, "chunk list launch");
+  }
+  bsb::DecodeArgs a = decode_args(s, c, p.decode);
+  a.context_lens = lens;
+  a.seq_rows = table_rows;
+  a.chunk_rows = rows;
+  a.chunk_heads = a.groups;
+  a.groups *= w.max_query_len;
+  a.chunk_window = a.window;
+  a.window += w.max_query_len - 1;
+  const int rc = bsb::launch_decode_int4(a, static_cast<int>(p.decode.grid), stream);
+  if (rc != 0) return cuda_fail(rc, "short chunk launch");
+  bsb::add_kernel_launches(p.decode.segment_ctas > 0 ? 2 : 3);
   return BS_OK;
 }
 
@@ -498,6 +560,7 @@ int run_window(const WindowShape& s, const WindowCall& c) {
   a.sinks = static_cast<int32_t>(std::min(s.sinks, kMaxContext));
   a.scale = static_cast<float>(c.scaling);
   a.status = c.status;
+  if (mma && short_chunks(s)) return run_short_chunks(s, c, a);
   // The tensor-core prefill compares scores before it scales them: it needs a
   // magnitude to scale by.
   if (mma && a.scale != 0.f && std::isfinite(a.scale)) return run_mma_chunks(s, c, a);

@@ -78,6 +78,40 @@ struct DecodeArgs {
   // segment_ctas: sequence and kv head as b / Hkv, b % Hkv), which join their parts
   // through distributed shared memory: no spans over the batch, no merge pass.
   int32_t segment_ctas;
+  // Short chunks (decode_int4.cu): chunk_rows is each sequence's first query token and their
+  // count, its length what the last of them sees; `groups` counts the rows of as many tokens
+  // as the longest chunk may have, chunk_heads query heads each.  chunk_window is the window
+  // of a token, `window` that of all of them, by which units are found.
+  const int2* chunk_rows;
+  int32_t chunk_heads, chunk_window;
+};
+
+// The output rows of a segment.
+template <bool CHUNK>
+struct OutRows {
+  int64_t at, stride;  // elements: of its first row; between tokens
+  int32_t heads, rows;
+  __device__ __forceinline__ OutRows(const DecodeArgs& a, int32_t seq, int32_t kvh) {
+    if constexpr (CHUNK) {
+      const int2 tokens = __ldg(a.chunk_rows + seq);
+      stride = a.o_stride_seq;
+      heads = a.chunk_heads;
+      rows = tokens.y * heads;
+      at = tokens.x * stride + static_cast<int64_t>(kvh) * heads * a.head_dim;
+    } else {
+      rows = a.groups;
+      at = static_cast<int64_t>(seq) * a.o_stride_seq +
+           static_cast<int64_t>(kvh) * a.groups * a.head_dim;
+    }
+  }
+  __device__ __forceinline__ int64_t row(int32_t r, int32_t dim) const {
+    if constexpr (CHUNK) {
+      const int32_t token = r / heads;
+      return at + token * stride + (r - token * heads) * dim;
+    } else {
+      return at + r * dim;
+    }
+  }
 };
 
 // Tokens per unit of the sliding-window variant (one tile of the tensor cores).
@@ -611,7 +645,7 @@ __device__ __forceinline__ bool warp_write_record(const DecodeArgs& a, const Spa
 // for 2 * n * G + 2 * G floats.  Row weights are computed once per record, then
 // the O rows stream in as float4 loads that do not depend on one another.
 // Must be called by all threads of the CTA (it synchronises them).
-template <typename OutT>
+template <typename OutT, bool CHUNK = false>
 __device__ void cta_merge_records(const DecodeArgs& a, const Span& sp, int32_t seq, int32_t kvh,
                                   int64_t seg_unit, int32_t nb, float* scratch) {
   const int G = a.groups, D = a.head_dim;
@@ -658,10 +692,10 @@ __device__ void cta_merge_records(const DecodeArgs& a, const Span& sp, int32_t s
     rowInvL[tid] = 1.f / L;
   }
   __syncthreads();
-  OutT* out = static_cast<OutT*>(a.out) + static_cast<int64_t>(seq) * a.o_stride_seq +
-              static_cast<int64_t>(kvh) * G * D;
+  const OutRows<CHUNK> to(a, seq, kvh);
   for (int e4 = tid; e4 < E4; e4 += nthr) {
     const int r = (e4 * 4) / D;
+    if (CHUNK && r >= to.rows) break;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c0 = 0; c0 < n; c0 += kBatch) {
       if (e4 != tid || c0 != 0) {  // else: prefetched above
@@ -682,10 +716,11 @@ __device__ void cta_merge_records(const DecodeArgs& a, const Span& sp, int32_t s
       }
     }
     const float inv = rowInvL[r];
-    store_out<OutT>(out + 4 * e4 + 0, acc.x * inv);
-    store_out<OutT>(out + 4 * e4 + 1, acc.y * inv);
-    store_out<OutT>(out + 4 * e4 + 2, acc.z * inv);
-    store_out<OutT>(out + 4 * e4 + 3, acc.w * inv);
+    OutT* out = static_cast<OutT*>(a.out) + to.row(r, D) + (e4 * 4 - r * D);
+    store_out<OutT>(out + 0, acc.x * inv);
+    store_out<OutT>(out + 1, acc.y * inv);
+    store_out<OutT>(out + 2, acc.z * inv);
+    store_out<OutT>(out + 3, acc.w * inv);
   }
   __syncthreads();  // scratch may be reused
 }
@@ -700,7 +735,9 @@ int launch_window_decode_mma(const DecodeArgs& a, const CUtensorMap& kmap,
 int window_decode_mma_ctas_per_sm(int head_dim, int groups);
 // The same over 4-bit pools (decode_int4.cu).
 int launch_decode_int4(const DecodeArgs& a, int grid, cudaStream_t stream);
-int decode_int4_ctas_per_sm(int head_dim, int groups);
+// `rows` query rows of a segment, of one token or (chunks) several.
+constexpr int kShortChunkRows = 16;
+int decode_int4_ctas_per_sm(int head_dim, int rows, bool chunks);
 int launch_decode_simt(const DecodeArgs& a, int dtype_is_bf16, int grid, cudaStream_t stream);
 int decode_simt_ctas_per_sm(int head_dim, int groups, int dtype_is_bf16);
 

@@ -23,8 +23,11 @@
 //
 // Scores are weighed against a maximum that moves only when one is more than 2^8 above it
 // (then all lanes find the new one and O is scaled): most units need no reduction.
+#include <type_traits>
+
 #include "decode_join.cuh"
 #include "int4.cuh"
+#include "window.cuh"
 
 namespace bsb {
 namespace {
@@ -37,13 +40,15 @@ enum : int32_t { kWhole = 1, kSlot1 = 2 };
 constexpr float kSlack = 8.f;  // how far above the maximum a score may be, base 2
 constexpr float kNoScore = -3.402823466e38f;  // the maximum before any score: no finite one is below
 
-template <int D, bool G16>
+// NQ tiles of 8 query rows, one or two; CHUNK_: rows of several tokens.
+template <int D, int NQ, bool CHUNK_>
 struct Cfg {
+  static constexpr bool CHUNK = CHUNK_;
   static constexpr int W = 4;                    // warps per CTA
   static constexpr int U = 2;                    // units of a step
   static constexpr int S = D == 64 ? 4 : 3;      // stages per warp, a step each
-  static constexpr int MIN_CTAS = D == 64 ? (G16 ? 3 : 4) : (G16 ? 2 : 3);
-  static constexpr int GROWS = G16 ? 16 : 8;
+  static constexpr int MIN_CTAS = D == 64 ? 5 - NQ : 4 - NQ;
+  static constexpr int GROWS = 8 * NQ;
   static constexpr int CODE_BYTES = kWindowUnit * D / 2;  // of a unit, K or V
   static constexpr int SCALE_BYTES = kWindowUnit * D / 16;
   // A unit in a stage: K codes | V codes | K scales | V scales.
@@ -65,11 +70,21 @@ struct Owner {
   int64_t seg_unit;
 };
 
+// Of chunks also: its length, first query token and tokens.
+struct ChunkOwner : Owner {
+  int32_t len, tok0, tokens;
+};
+
 // What a stage holds: the visible tokens of a step that does not show them all (16 bits a
 // unit), and whose it is of a portion's first and last ones.
 struct StepMeta {
   uint32_t map;
   Owner owner;
+};
+struct ChunkMeta {
+  uint32_t map;
+  int32_t first[2];  // positions of the units' first tokens
+  ChunkOwner owner;
 };
 
 // Up to 32 consecutive units of a segment, one per lane.
@@ -78,6 +93,7 @@ struct Run {
   uint32_t flags;  // kFirst, kLast: a portion's first, its last units
   int32_t blk;       // this lane's: block-table entry, unit of its block, visible tokens
   int32_t in_block, map;
+  int32_t first;  // chunks: position of its first token
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -101,15 +117,17 @@ __device__ __forceinline__ void mma_zero_16816(float (&d)[4], const uint32_t (&a
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-template <int D, bool G16>
-__global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kernel(const DecodeArgs a) {
-  using C = Cfg<D, G16>;
+template <int D, int NQ, bool CHUNK>
+__global__ void __launch_bounds__(128, (Cfg<D, NQ, CHUNK>::MIN_CTAS))
+    decode_int4_kernel(const DecodeArgs a) {
+  using C = Cfg<D, NQ, CHUNK>;
+  using Whose = std::conditional_t<CHUNK, ChunkOwner, Owner>;
+  using Meta = std::conditional_t<CHUNK, ChunkMeta, StepMeta>;
   constexpr int W = C::W, S = C::S, U = C::U;
   constexpr int NG = D / kInt4Group;  // groups of a row
-  constexpr int NQ = G16 ? 2 : 1;     // tiles of 8 query heads
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ StepMeta meta[W][S];
-  __shared__ Owner owners[W][2];  // of the current run and the one behind it
+  __shared__ Meta meta[W][S];
+  __shared__ Whose owners[W][2];  // of the current run and the one behind it
   __shared__ ScanSmem scan;
   __shared__ WarpStarts starts;
   __shared__ WarpSlots<W> slots;
@@ -135,7 +153,7 @@ __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kern
     return;
   }
 
-  const int G = a.groups;
+  const int G = a.groups, heads = CHUNK ? a.chunk_heads : G;
   const int64_t Hkv = a.num_kv_heads;
   const int64_t spanw = sp.r1 - sp.r0;
   const int64_t wr0 = sp.r0 + spanw * warp / W;
@@ -175,24 +193,40 @@ __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kern
       r.in_block = tu - ent * a.block_units;
       r.blk = __ldg(a.block_tables + static_cast<int64_t>(crow) * a.bt_stride + ent);
     }
-    const int32_t tok0 = tu * kWindowUnit, lo = clen - a.window;
+    const int32_t tok0 = tu * kWindowUnit;
+    int2 tokens{};
+    if constexpr (CHUNK) tokens = __ldg(a.chunk_rows + ci);
+    // What the last token sees, or any of them.
+    const int32_t lo = CHUNK ? clen - a.chunk_window - (tokens.y - 1) : clen - a.window;
     auto below = [](int32_t c) {  // map of a unit's first c tokens
       return c >= kWindowUnit ? 0xffff : c <= 0 ? 0 : (1 << c) - 1;
     };
     r.map = below(clen - tok0) & (~below(lo - tok0) | below(a.sinks - tok0));
+    if constexpr (CHUNK) {  // (bit 16: all of them see all of it)
+      r.first = tok0;
+      if (tok0 + kWindowUnit <= clen - (tokens.y - 1) &&
+          (tok0 >= clen - a.chunk_window || tok0 + kWindowUnit <= a.sinks)) {
+        r.map |= 0x10000;
+      }
+    }
     togo -= r.n;
     cb += r.n;
     const bool ends = togo == 0 || cb == cnb;
     r.flags = (begins ? kFirst : 0u) | (ends ? kLast : 0u);
     if (lane == 0) {
       const int64_t seg_unit = cprefix * Hkv + static_cast<int64_t>(ch) * cnb;
-      Owner& w = owners[warp][parity];
+      Whose& w = owners[warp][parity];
       w.seq = ci;
       w.kvh = ch;
       w.nb = cnb;
       w.seg_unit = seg_unit;
       w.flags = (seg_unit >= wr0 && seg_unit + cnb <= wr1 && !(clustered && ranks > 1) ? kWhole : 0) |
                 (seg_unit > wr0 ? kSlot1 : 0);
+      if constexpr (CHUNK) {
+        w.len = clen;
+        w.tok0 = tokens.x;
+        w.tokens = tokens.y;
+      }
     }
     parity ^= 1;
     begins = ends;
@@ -236,21 +270,30 @@ __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kern
   int32_t idx = 0;     // next unit of the current run: it and the one behind it are a step
   uint32_t full = 0;   // its units whose tokens are all visible
   int64_t head_at = 0;
-  const Owner* owner = nullptr;
+  const Whose* owner = nullptr;
   auto begin_run = [&]() {
     if (cur.n == 0) return;
     const bool valid = cur.blk >= 0 && cur.blk < a.num_blocks;
-    if (lane < cur.n && !valid) set_status(a.status, kStatusBadBlock);
+    // (Units that the window of a longer group would reach may have no block any more.)
+    if (lane < cur.n && !valid && (!CHUNK || cur.map != 0)) set_status(a.status, kStatusBadBlock);
     if (!valid) cur.blk = cur.map = 0;  // any block will do: none of its tokens counts
-    full = __ballot_sync(0xffffffffu, lane < cur.n && cur.map == 0xffff);
+    full = __ballot_sync(0xffffffffu, lane < cur.n && cur.map == (CHUNK ? 0x1ffff : 0xffff));
     owner = &owners[warp][parity ^ 1];
     const int32_t kvh = owner->kvh;
     head_at = kvh * head_bytes;
     if (cur.flags & kFirst) {  // the query will be wanted: into L1
-      const char* q = reinterpret_cast<const char*>(
-          static_cast<const __nv_bfloat16*>(a.q) +
-          static_cast<int64_t>(owner->seq) * a.q_stride_seq + static_cast<int64_t>(kvh) * G * D);
-      if (lane * 128 < G * D * 2) asm volatile("prefetch.global.L1 [%0];" ::"l"(q + lane * 128));
+      int32_t first = owner->seq, tokens = 1;
+      if constexpr (CHUNK) {
+        first = owner->tok0;
+        tokens = owner->tokens;
+      }
+      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + first * a.q_stride_seq +
+                               static_cast<int64_t>(kvh) * heads * D + lane * 64;
+      for (int32_t j = 0; j < tokens; ++j) {
+        if (lane * 64 < heads * D) {
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(q + j * a.q_stride_seq));
+        }
+      }
     }
     idx = 0;
     nxt = fetch();
@@ -288,11 +331,21 @@ __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kern
       if (flags != (kStep | kFull)) {
         uint32_t seen = __shfl_sync(0xffffffffu, cur.map, idx);
         const uint32_t second = __shfl_sync(0xffffffffu, cur.map, idx + 1);
+        if constexpr (CHUNK) seen &= 0xffffu;
         if (idx + 1 < cur.n) seen |= second << 16;
+        int32_t first[2];
+        if constexpr (CHUNK) {
+          first[0] = __shfl_sync(0xffffffffu, cur.first, idx);
+          first[1] = __shfl_sync(0xffffffffu, cur.first, idx + 1);
+        }
         if (lane == 0) {
-          StepMeta& m = meta[warp][stage];
+          Meta& m = meta[warp][stage];
           m.map = seen;
-          if (flags & (kFirst | kLast)) m.owner = *owner;
+          if (CHUNK || (flags & (kFirst | kLast))) m.owner = *owner;
+          if constexpr (CHUNK) {
+            m.first[0] = first[0];
+            m.first[1] = first[1];
+          }
         }
         __syncwarp();  // the owner has been read
       }
@@ -335,15 +388,20 @@ __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kern
       __syncwarp();
       const uint32_t flags = queue & 15u;
       if (flags == 0) break;
-      const StepMeta& mt = meta[warp][stage];
+      const Meta& mt = meta[warp][stage];
       float bias[U][2];  // of keys g, g + 8 of each unit: -inf where the token is not seen
 #pragma unroll
       for (int u = 0; u < U; ++u) bias[u][0] = bias[u][1] = 0.f;
       if (flags != (kStep | kFull)) {
         if (flags & kFirst) {
+          int32_t first = mt.owner.seq, rows = G;
+          if constexpr (CHUNK) {
+            first = mt.owner.tok0;
+            rows = mt.owner.tokens * heads;
+          }
           const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) +
-                                   static_cast<int64_t>(mt.owner.seq) * a.q_stride_seq +
-                                   static_cast<int64_t>(mt.owner.kvh) * G * D + t * (D / 4);
+                                   first * a.q_stride_seq +
+                                   static_cast<int64_t>(mt.owner.kvh) * heads * D + t * (D / 4);
 #pragma unroll
           for (int h = 0; h < NQ; ++h) {
             m2[h][0] = m2[h][1] = kNoScore;
@@ -356,10 +414,13 @@ __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kern
                 for (int e = 0; e < 4; ++e) o[h][x][j][e] = 0.f;
               }
             }
+            const int32_t row = g + 8 * h, token = CHUNK ? row / heads : 0;
+            const __nv_bfloat16* from =
+                q + token * (CHUNK ? a.q_stride_seq : 0) + (row - token * heads) * D;
 #pragma unroll
             for (int w = 0; w < WORDS; ++w) {
               uint4 x = make_uint4(0u, 0u, 0u, 0u);
-              if (g + 8 * h < G) x = *reinterpret_cast<const uint4*>(q + (g + 8 * h) * D + w * 8);
+              if (row < rows) x = *reinterpret_cast<const uint4*>(from + w * 8);
               qf[h][w][0] = x.x;
               qf[h][w][1] = x.y;
               qf[h][w][2] = x.z;
@@ -386,7 +447,6 @@ __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kern
       }
       // S^T = K Q^T: keys g and g + 8 of each unit, in two chains.
       float s[U][NQ][4];
-      float above = -INFINITY;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const uint32_t unit = base + u * C::UNIT_BYTES;
@@ -434,6 +494,31 @@ __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kern
           for (int e = 0; e < 4; ++e) {
             s[u][h][e] = __fmaf_rn(s[u][h][e] + s2[h][e], zscale, bias[u][e >> 1]);
           }
+        }
+      }
+      if constexpr (CHUNK) {
+        if (!(flags & kFull)) {  // the rows' own limits
+#pragma unroll
+          for (int h = 0; h < NQ; ++h) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int32_t at = mt.owner.len - mt.owner.tokens + (8 * h + 2 * t + c) / heads;
+#pragma unroll
+              for (int k = 0; k < 2 * U; ++k) {
+                const int32_t key = mt.first[k / 2] + g + 8 * (k % 2);
+                if (key > at || (key >= a.sinks && key <= at - a.chunk_window)) {
+                  s[k / 2][h][c + 2 * (k % 2)] = -INFINITY;
+                }
+              }
+            }
+          }
+        }
+      }
+      float above = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < NQ; ++h) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
           above = fmaxf(above, fmaxf(fmaxf(s[u][h][0], s[u][h][2]) - m2[h][0],
                                      fmaxf(s[u][h][1], s[u][h][3]) - m2[h][1]));
         }
@@ -519,9 +604,7 @@ __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kern
         const bool whole = (mt.owner.flags & kWhole) != 0;
         const int slot_of = (mt.owner.flags & kSlot1) ? 1 : 0;
         float* slot = warp_slot<C>(smem, warp, slot_of);
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
-                             static_cast<int64_t>(seq) * a.o_stride_seq +
-                             static_cast<int64_t>(kvh) * G * D;
+        const OutRows<CHUNK> to(a, seq, kvh);
         if (lane == 0 && !whole) {
           slots.seq[warp][slot_of] = seq;
           slots.kvh[warp][slot_of] = kvh;
@@ -543,6 +626,7 @@ __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kern
           }
           const int row = 8 * h + 2 * t + odd;
           const float inv = whole ? 1.f / (odd ? l[1] : l[0]) : 1.f;
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + to.row(row, D);
 #pragma unroll
           for (int q = 0; q < NG; ++q) {
 #pragma unroll
@@ -552,12 +636,10 @@ __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kern
               const float got = __shfl_xor_sync(0xffffffffu, odd ? x0 : x1, 4);
               const float lo = (odd ? got : x0) * inv, hi = (odd ? x1 : got) * inv;
               const int dim = 32 * q + 8 * (g >> 1) + 2 * i;
-              if (row < G) {
-                if (whole) {
-                  *reinterpret_cast<uint32_t*>(out + row * D + dim) = pack_bf16x2(lo, hi);
-                } else {
-                  *reinterpret_cast<float2*>(slot + row * D + dim) = make_float2(lo, hi);
-                }
+              if (whole && row < to.rows) {
+                *reinterpret_cast<uint32_t*>(out + dim) = pack_bf16x2(lo, hi);
+              } else if (!whole && row < G) {
+                *reinterpret_cast<float2*>(slot + row * D + dim) = make_float2(lo, hi);
               }
             }
           }
@@ -587,20 +669,20 @@ __global__ void __launch_bounds__(128, (Cfg<D, G16>::MIN_CTAS)) decode_int4_kern
   if (tid == 0) a.tasks[blockIdx.x] = task;
 }
 
-template <int D, bool G16>
+template <int D, int NQ, bool CHUNK>
 cudaError_t allow_smem() {
   static unsigned long long configured = 0;  // one bit per device
   return once_per_device(&configured, [] {
-    return cudaFuncSetAttribute(decode_int4_kernel<D, G16>,
+    return cudaFuncSetAttribute(decode_int4_kernel<D, NQ, CHUNK>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                Cfg<D, G16>::SMEM_BYTES);
+                                Cfg<D, NQ, CHUNK>::SMEM_BYTES);
   });
 }
 
-template <int D, bool G16>
+template <int D, int NQ, bool CHUNK>
 int launch_one(const DecodeArgs& a, int grid, cudaStream_t stream) {
-  using C = Cfg<D, G16>;
-  cudaError_t e = allow_smem<D, G16>();
+  using C = Cfg<D, NQ, CHUNK>;
+  cudaError_t e = allow_smem<D, NQ, CHUNK>();
   if (e != cudaSuccess) return static_cast<int>(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
@@ -618,39 +700,78 @@ int launch_one(const DecodeArgs& a, int grid, cudaStream_t stream) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
   }
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_int4_kernel<D, G16>, a));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_int4_kernel<D, NQ, CHUNK>, a));
 }
 
-template <int D, bool G16>
+template <int D, int NQ, bool CHUNK>
 int occupancy_one() {
-  using C = Cfg<D, G16>;
+  using C = Cfg<D, NQ, CHUNK>;
   int n = 0;
-  cudaError_t e = allow_smem<D, G16>();
+  cudaError_t e = allow_smem<D, NQ, CHUNK>();
   if (e == cudaSuccess) {
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_int4_kernel<D, G16>, C::W * 32,
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_int4_kernel<D, NQ, CHUNK>, C::W * 32,
                                                       C::SMEM_BYTES);
   }
   return e != cudaSuccess ? -static_cast<int>(e) : n;
 }
 
+template <int D, bool CHUNK>
+int launch_rows(const DecodeArgs& a, int grid, cudaStream_t stream) {
+  return a.groups > 8 ? launch_one<D, 2, CHUNK>(a, grid, stream)
+                      : launch_one<D, 1, CHUNK>(a, grid, stream);
+}
+
+template <int D, bool CHUNK>
+int occupancy_rows(int rows) {
+  return rows > 8 ? occupancy_one<D, 2, CHUNK>() : occupancy_one<D, 1, CHUNK>();
+}
+
+// Short chunks as sequences of the kernel above; without tokens, of length 0.
+__global__ void __launch_bounds__(128) chunk_rows_kernel(const WindowArgs a, int2* rows,
+                                                         int32_t* lens, int32_t* table_rows) {
+  pdl_wait();
+  pdl_trigger();
+  const int32_t b = blockIdx.x * blockDim.x + threadIdx.x;
+  if (b >= a.num_rows) return;
+  WindowTile w{};
+  const bool any = window_tile(a, b, 0, w, true);
+  rows[b] = any ? make_int2(w.tok0, w.ntok) : make_int2(0, 0);
+  lens[b] = any ? w.pos0 + w.ntok : 0;
+  table_rows[b] = any ? w.row : 0;
+}
+
 }  // namespace
 
 int launch_decode_int4(const DecodeArgs& a, int grid, cudaStream_t stream) {
-  const bool g16 = a.groups > 8;
   int rc;
-  if (a.head_dim == 64) {
-    rc = g16 ? launch_one<64, true>(a, grid, stream) : launch_one<64, false>(a, grid, stream);
+  if (a.chunk_rows != nullptr) {
+    rc = a.head_dim == 64 ? launch_rows<64, true>(a, grid, stream)
+                          : launch_rows<128, true>(a, grid, stream);
   } else {
-    rc = g16 ? launch_one<128, true>(a, grid, stream) : launch_one<128, false>(a, grid, stream);
+    rc = a.head_dim == 64 ? launch_rows<64, false>(a, grid, stream)
+                          : launch_rows<128, false>(a, grid, stream);
   }
   if (rc != 0 || a.tasks == nullptr) return rc;
   return launch_decode_merge(a, grid, stream);
 }
 
-int decode_int4_ctas_per_sm(int head_dim, int groups) {
-  const bool g16 = groups > 8;
-  if (head_dim == 64) return g16 ? occupancy_one<64, true>() : occupancy_one<64, false>();
-  return g16 ? occupancy_one<128, true>() : occupancy_one<128, false>();
+int decode_int4_ctas_per_sm(int head_dim, int rows, bool chunks) {
+  if (chunks) return head_dim == 64 ? occupancy_rows<64, true>(rows) : occupancy_rows<128, true>(rows);
+  return head_dim == 64 ? occupancy_rows<64, false>(rows) : occupancy_rows<128, false>(rows);
+}
+
+int launch_chunk_rows(const WindowArgs& a, int2* rows, int32_t* lens, int32_t* table_rows,
+                      cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((a.num_rows + 127) / 128);
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, chunk_rows_kernel, a, rows, lens, table_rows));
 }
 
 }  // namespace bsb

@@ -2,7 +2,8 @@
 // worked on come together.  Shared by the tensor-core kernels over bf16 and 4-bit pools.
 //
 // C is the kernel's configuration: W warps with S stages of STAGE_BYTES each at the start of
-// shared memory, then W slots of SLOT0_BYTES; GROWS query rows.  A warp leaves a part (O
+// shared memory, then W slots of SLOT0_BYTES; GROWS query rows, of one token or, for short
+// chunks (CHUNK), several.  A warp leaves a part (O
 // unnormalised [G][D], then row maxima in base 2 and row sums) in its slot 0, its last part
 // in slot 1, which lies over its stages.
 #pragma once
@@ -41,9 +42,8 @@ __device__ __forceinline__ void join_segment(const DecodeArgs& a, uint8_t* smem,
   __shared__ float part_ml[2 * C::GROWS];
   float* part = reinterpret_cast<float*>(smem);  // over the stages, whose copies are done
   const int tid = threadIdx.x, G = a.groups;
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
-                       static_cast<int64_t>(seq) * a.o_stride_seq +
-                       static_cast<int64_t>(kvh) * G * D;
+  const OutRows<C::CHUNK> to(a, seq, kvh);
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out);
   __syncthreads();
   bool parked = ranks > 1;  // or one warp has written the output
 #pragma unroll
@@ -70,7 +70,7 @@ __device__ __forceinline__ void join_segment(const DecodeArgs& a, uint8_t* smem,
       O += f * o[w];
     }
     if (ranks == 1) {
-      out[e] = __float2bfloat16_rn(O / L);
+      if (!C::CHUNK || r < to.rows) out[to.row(r, D) + e - r * D] = __float2bfloat16_rn(O / L);
     } else {
       part[e] = O;
       if (e % D == 0) {
@@ -101,7 +101,7 @@ __device__ __forceinline__ void join_segment(const DecodeArgs& a, uint8_t* smem,
       L += f * l[k];
       O += f * o[k];
     }
-    out[e] = __float2bfloat16_rn(O / L);
+    if (!C::CHUNK || r < to.rows) out[to.row(r, D) + e - r * D] = __float2bfloat16_rn(O / L);
   }
   cluster_sync();  // the others may still read this CTA's shared memory
 }
@@ -172,16 +172,15 @@ __device__ __forceinline__ void fold_slots(const DecodeArgs& a, uint8_t* smem, c
     const int64_t seg_unit = slots.unit[warp][k];
     const int32_t nb = slots.nb[warp][k];
     if (seg_unit >= sp.r0 && seg_unit + nb <= sp.r1) {
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
-                           static_cast<int64_t>(seq) * a.o_stride_seq +
-                           static_cast<int64_t>(kvh) * G * D;
+      const OutRows<C::CHUNK> to(a, seq, kvh);
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out);
       const float inv_l = lane < G ? 1.f / mine[G * D + G + lane] : 0.f;
 #pragma unroll
       for (int j = 0; j < C::GROWS * D / 32; ++j) {
         const int r = (32 * j) / D;
         const float inv = __shfl_sync(0xffffffffu, inv_l, r);
         const int e = lane + 32 * j;
-        if (r < G) out[e] = __float2bfloat16_rn(mine[e] * inv);
+        if (r < to.rows) out[to.row(r, D) + e - r * D] = __float2bfloat16_rn(mine[e] * inv);
       }
     } else {
       cut(seq, kvh, seg_unit, nb, mine);

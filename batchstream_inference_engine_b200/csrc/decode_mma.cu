@@ -55,6 +55,7 @@ struct TileMeta {
 
 template <int D, bool G16>
 struct Cfg {
+  static constexpr bool CHUNK = false;
   static constexpr int W = 4;                  // warps per CTA
   // Stages per warp: two at either head_dim.  Deeper rings only lengthen the
   // DRAM queues (12 warps x 2 stages x 4 KiB per SM already cover bandwidth x
@@ -619,6 +620,7 @@ int launch_one(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap& 
 // Merges, after the decode kernel, the cut segments its CTAs listed: one CTA
 // per decode CTA, all threads on the records of one segment.
 // Three CTAs per SM: as many as the decode kernel's grid holds, all in one wave.
+template <bool CHUNK>
 __global__ void __launch_bounds__(128, 3) decode_merge_kernel(const DecodeArgs a) {
   extern __shared__ float merge_scratch[];
   pdl_wait();
@@ -627,7 +629,32 @@ __global__ void __launch_bounds__(128, 3) decode_merge_kernel(const DecodeArgs a
   Span sp{};
   sp.q = t.q;
   sp.rem = t.rem;
-  cta_merge_records<__nv_bfloat16>(a, sp, t.seq, t.kvh, t.seg_unit, t.nb, merge_scratch);
+  cta_merge_records<__nv_bfloat16, CHUNK>(a, sp, t.seq, t.kvh, t.seg_unit, t.nb, merge_scratch);
+}
+
+template <bool CHUNK>
+int launch_merge(const DecodeArgs& a, int grid, cudaStream_t stream) {
+  const int smem = static_cast<int>((2 * static_cast<int64_t>(grid) * a.groups + 2 * a.groups) *
+                                    sizeof(float));
+  // Room for 16 rows and 700 CTAs; the grids hold at most four an SM.
+  constexpr int kMaxSmem = 90 * 1024;
+  static unsigned long long configured = 0;  // one bit per device
+  cudaError_t e = once_per_device(&configured, [] {
+    return cudaFuncSetAttribute(decode_merge_kernel<CHUNK>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+  });
+  if (e != cudaSuccess) return static_cast<int>(e);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_merge_kernel<CHUNK>, a));
 }
 
 template <int D, bool G16, bool WIN>
@@ -647,27 +674,8 @@ int occupancy_one() {
 
 // The merge pass of every form: at most `grid` records per segment.
 int launch_decode_merge(const DecodeArgs& a, int grid, cudaStream_t stream) {
-  const int smem = static_cast<int>((2 * static_cast<int64_t>(grid) * a.groups + 2 * a.groups) *
-                                    sizeof(float));
-  // Room for 16 heads a group and 700 CTAs; the grids hold at most three an SM.
-  constexpr int kMaxSmem = 90 * 1024;
-  static unsigned long long configured = 0;  // one bit per device
-  cudaError_t e = once_per_device(&configured, [] {
-    return cudaFuncSetAttribute(decode_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kMaxSmem);
-  });
-  if (e != cudaSuccess) return static_cast<int>(e);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_merge_kernel, a));
+  return a.chunk_rows != nullptr ? launch_merge<true>(a, grid, stream)
+                                 : launch_merge<false>(a, grid, stream);
 }
 
 namespace {

@@ -129,6 +129,10 @@ int launch_window_prefill(const WindowArgs& a, const CUtensorMap& qmap, const CU
 // What runs at once of the CUDA-core kernel: CTAs per SM (cluster 1), or clusters of so many
 // CTAs on the device (negative: a CUDA error); wide: more than 8 query rows a tile.
 int window_simt_at_once(bool bf16, bool int4, bool wide, int head_dim, int cluster);
+// Short chunks over 4-bit pools (decode_int4.cu): every chunk's first query token and count,
+// length and table row.
+int launch_chunk_rows(const WindowArgs& a, int2* rows, int32_t* lens, int32_t* table_rows,
+                      cudaStream_t stream);
 int launch_window_simt(const WindowArgs& a, bool bf16, bool vec, cudaStream_t stream);
 
 }  // namespace bsb

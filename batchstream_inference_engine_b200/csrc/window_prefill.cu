@@ -653,10 +653,15 @@ __global__ void __launch_bounds__((Cfg<D, TILES>::THREADS), (Cfg<D, TILES>::MIN_
     };
     int32_t plain_lo, plain_hi;
     plain_steps(a, sd, plain_lo, plain_hi);
+    const bool any_live = __any_sync(0xffffffffu, live);
     bool ok = true;
     for (int32_t u = 0; u < n; ++u) {
       ok = wait_step(u, own);
       if (!ok) break;
+      if (!any_live) {  // nothing reads what comes of these rows
+        mbar_arrive(&p_full[own][u & 1]);
+        continue;
+      }
       tc_fence_after();
       const uint32_t s_addr = tmem + lane_base + (u & 1) * kKeys;
       // Visible tokens of the step's units, 16 bits each (border steps only).

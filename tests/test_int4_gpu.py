@@ -590,6 +590,142 @@ def test_chunk_reports_bad_input_and_spares_the_others(change, message, head_dim
     assert torch.equal(out[keep.to(DEV)], good[keep.to(DEV)])
 
 
+# Chunks of a few tokens (the decode kernel's form of several tokens a row).
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (4, 2), (6, 2), (5, 1), (7, 1), (16, 2), (11, 1),
+                                            (16, 1)])
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("longest", [2, 3, 5, 8, 13])
+def test_short_chunks(heads, kv_heads, head_dim, longest):
+    # Ends before, at and behind the borders of 16 and 32 keys, chunks longer than what is behind
+    # them, and a long sequence that several warps and CTAs share.
+    priors = [0, 1, 10, 14, 15, 16, 30, 31, 33, 61, 128, 5000, 700]
+    news = [1 + (3 * i + longest - 1) % longest for i in range(len(priors))]
+    c = Packed([p + n for p, n in zip(priors, news)], news, heads, kv_heads, head_dim, 16,
+               torch.bfloat16, 1 << 40, 0, seed=heads + longest)
+    out = c.chunks()
+    assert ops.take_status() == 0
+    c.check(out)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (2, 17), (15, 0), (16, 16), (17, 33),
+                                          (64, 3), (200, 1 << 40), (200, 5), (4000, 1)])
+@pytest.mark.parametrize("heads,kv_heads,head_dim,block", [(14, 2, 64, 16), (8, 2, 128, 32)])
+def test_short_chunk_windows(window, sinks, heads, kv_heads, head_dim, block):
+    news = [5, 3, 1, 5, 4, 5, 2]
+    priors = [500, 0, 13, 194, 3000, 40, 5000]
+    c = Packed([p + n for p, n in zip(priors, news)], news, heads, kv_heads, head_dim, block,
+               torch.bfloat16, window, sinks, seed=sinks % 1000)
+    out = c.chunks()
+    assert ops.take_status() == 0
+    c.check(out)
+
+
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(14, 2, 64), (28, 4, 128)])
+@pytest.mark.parametrize("rows,longest,window", [(1, 4, 100), (1, 5, 1 << 40), (6, 5, 777),
+                                                 (40, 7, 1 << 40), (300, 2, 64)])
+def test_short_chunks_by_clusters_and_by_records(heads, kv_heads, head_dim, rows, longest, window):
+    news = [1 + (5 * i + longest - 1) % longest for i in range(rows)]
+    priors = [(997 * i + 2000) % 3000 for i in range(rows)]
+    c = Packed([p + n for p, n in zip(priors, news)], news, heads, kv_heads, head_dim, 16,
+               torch.bfloat16, window, 3, seed=rows)
+    out = c.chunks()
+    assert ops.take_status() == 0
+    c.check(out)
+    for _ in range(3):
+        assert torch.equal(c.chunks(), out)
+
+
+def test_short_chunks_of_more_sequences_than_the_span_scan_stages():
+    rows = 9000
+    news = [1 + (7 * i) % 3 for i in range(rows)]
+    priors = [(37 * i) % 40 for i in range(rows)]
+    c = Packed([p + n for p, n in zip(priors, news)], news, 2, 1, 64, 16, torch.bfloat16, 1 << 40, 0,
+               seed=37)
+    out = c.chunks()
+    assert ops.take_status() == 0
+    c.check(out)
+
+
+def test_short_chunk_padding_and_strides():
+    news, priors = [2, 0, 5, 1], [50, 10, 300, 0]
+    c = Packed([p + n for p, n in zip(priors, news)], news, 14, 2, 64, 16, torch.bfloat16, 1 << 40,
+               0, seed=31)
+    plain = c.chunks()
+    c.check(plain)
+    T = c.T + 9
+    wide = torch.randn(T, 14 * 64 + 24, device=DEV).bfloat16()
+    q = wide[:, 8:-16].unflatten(1, (14, 64))
+    q[: c.T] = c.q.to(DEV)
+    cu = torch.cat([c.cu, c.cu[-1:], c.cu[-1:] + 4])
+    ctx = torch.cat([c.len_d, torch.zeros(2, dtype=torch.int32, device=DEV)])
+    rows = torch.tensor([0, 1, 2, 3, 0, 77], dtype=torch.int32, device=DEV)
+    room = torch.full((T, 16 * 64), SENTINEL, dtype=torch.bfloat16, device=DEV)
+    out = room[:, : 14 * 64].unflatten(1, (14, 64))
+    ops.int4_prefill_attention(q, c.k, c.v, c.table, cu, ctx, c.scale, 8, seq_rows=rows, out=out)
+    assert ops.take_status() == 0
+    assert torch.equal(out[: c.T], plain) and bool((out[c.T:] == SENTINEL).all())
+    assert bool((room[:, 14 * 64:] == SENTINEL).all())
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 20.0])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_short_chunk_scales(scale, head_dim):
+    news, priors = [5, 3], [300, 90]
+    c = Packed([p + n for p, n in zip(priors, news)], news, 8, 2, head_dim, 16, torch.bfloat16, 200,
+               4, seed=34)
+    c.scale = scale
+    out = c.chunks()
+    assert ops.take_status() == 0
+    c.check(out)
+
+
+@pytest.mark.parametrize("change,message", [
+    ("block", "block table"), ("context", "context length"), ("table", "context length"),
+    ("row", "sequence row"), ("long", "context length"), ("outside", "context length"),
+    ("backwards", "context length"),
+])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_short_chunk_reports_bad_input_and_spares_the_others(change, message, head_dim):
+    news, priors = [4, 3, 5], [60, 70, 10]
+    c = Packed([p + n for p, n in zip(priors, news)], news, 14, 2, head_dim, 16, torch.bfloat16, 40,
+               5, seed=33)
+    ref, tol = c.reference()
+    good = c.chunks()
+    rows = torch.arange(3, dtype=torch.int32, device=DEV)
+    kw, skipped = {}, slice(4, 7)
+    if change == "block":
+        c.table[1, 4] = -1
+    elif change == "context":
+        c.len_d[1] = 2
+    elif change == "table":
+        c.len_d[1] = c.table.size(1) * 16 + 1
+    elif change == "row":
+        rows[1] = -1
+    else:
+        skipped = slice(7, 12)
+        if change == "long":
+            kw["max_query_len"] = 4  # the last chunk holds 5
+        elif change == "outside":
+            c.cu[3] = 13  # one token past the query's rows
+            c.len_d[2] += 1
+            kw["max_query_len"] = 6
+        else:
+            c.cu[3] = 6  # ends before it begins
+    out = c.chunks(seq_rows=rows, **kw)
+    with pytest.raises(RuntimeError, match=message):
+        ops.take_status()
+    if change != "block":
+        assert bool((out[skipped] == SENTINEL).all())
+    spared = [t for t in range(12) if not skipped.start <= t < skipped.stop]
+    # (Another max_query_len may cut a chunk and share its keys out differently: the same sums in
+    # another order, each within the tolerance of the reference.)
+    if "max_query_len" not in kw:
+        assert torch.equal(out[spared], good[spared])
+    assert bool(((out.double().cpu() - ref).abs() <= tol)[spared].all())
+
+
 @pytest.mark.parametrize("dtype,head_dim,blocks", [
     (torch.bfloat16, 128, 1_000_000), (torch.bfloat16, 64, 2_000_000), (torch.float32, 96, 1_300_000)])
 def test_pool_past_32_bit_offsets(dtype, head_dim, blocks):
