@@ -396,6 +396,8 @@ bool mma_pointers(const WindowCall& c) {
          aligned16(c.output) && c.q_stride % 8 == 0 && c.o_stride % 8 == 0;
 }
 
+constexpr int kInt4SpanShift = 4;
+
 // The arguments of the tensor-core decode that are alike for single tokens and chunks.
 bsb::DecodeArgs decode_args(const WindowShape& s, const WindowCall& c, const MmaDecodePlan& p) {
   bsb::DecodeArgs a{};
@@ -429,6 +431,7 @@ bsb::DecodeArgs decode_args(const WindowShape& s, const WindowCall& c, const Mma
   a.window = static_cast<int32_t>(std::min(s.window, kMaxContext));
   a.sinks = static_cast<int32_t>(std::min(s.sinks, kMaxContext));
   a.block_units = static_cast<int32_t>(s.block_size / bsb::kWindowUnit);
+  a.span_shift = s.int4 ? kInt4SpanShift : 0;
   return a;
 }
 

@@ -78,6 +78,8 @@ struct DecodeArgs {
   // segment_ctas: sequence and kv head as b / Hkv, b % Hkv), which join their parts
   // through distributed shared memory: no spans over the batch, no merge pass.
   int32_t segment_ctas;
+  // Spans over the batch: only as many CTAs share it as have 2^span_shift units each (0: all).
+  int32_t span_shift;
   // Short chunks (decode_int4.cu): chunk_rows is each sequence's first query token and their
   // count, its length what the last of them sees; `groups` counts the rows of as many tokens
   // as the longest chunk may have, chunk_heads query heads each.  chunk_window is the window
@@ -208,6 +210,20 @@ __device__ __forceinline__ int64_t span_owner(int64_t u, int64_t q, int64_t rem)
   return u < head ? u / (q + 1) : rem + (u - head) / q;
 }
 
+// This CTA's share of sp.W units.
+__device__ __forceinline__ void share_units(const DecodeArgs& a, Span& sp) {
+  const int64_t c = blockIdx.x;
+  int64_t C = gridDim.x;
+  if (a.span_shift > 0) {
+    const int64_t most = sp.W >> a.span_shift;
+    C = most < 1 ? 1 : most < C ? most : C;
+  }
+  sp.q = sp.W / C;
+  sp.rem = sp.W % C;
+  sp.r0 = c < C ? span_begin(c, sp.q, sp.rem) : sp.W;
+  sp.r1 = c < C ? sp.r0 + sp.q + (c < sp.rem ? 1 : 0) : sp.W;
+}
+
 // Record slot of CTA c for the segment starting at unit U: slot 0 is the
 // segment the span starts in, slot 1 the one it ends in.
 __device__ __forceinline__ int64_t record_index(int64_t c, int64_t U, int64_t q, int64_t rem) {
@@ -239,7 +255,7 @@ __device__ __forceinline__ Span compute_span(const DecodeArgs& a, ScanSmem& sm,
                                              bool find_start = true) {
   const int tid = threadIdx.x, nthr = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int nwarps = (nthr + 31) >> 5;
-  const int64_t C = gridDim.x, c = blockIdx.x;
+  const int64_t c = blockIdx.x;
   const int32_t B = a.num_seqs;
   Span sp;
 
@@ -262,10 +278,7 @@ __device__ __forceinline__ Span compute_span(const DecodeArgs& a, ScanSmem& sm,
   __syncthreads();
   const int64_t Hkv = a.num_kv_heads;
   sp.W = sm.total * Hkv;
-  sp.q = sp.W / C;
-  sp.rem = sp.W % C;
-  sp.r0 = span_begin(c, sp.q, sp.rem);
-  sp.r1 = sp.r0 + sp.q + (c < sp.rem ? 1 : 0);
+  share_units(a, sp);
   sp.seq = -1;
   sp.prefix = 0;
   if (sp.r0 >= sp.r1 || !find_start) return sp;
@@ -481,7 +494,7 @@ __device__ __forceinline__ Span compute_warp_spans_smem(const DecodeArgs& a, Sca
   static_assert(NW <= 8, "at most 8 warp spans");
   const int tid = threadIdx.x, nthr = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int nwarps = (nthr + 31) >> 5;
-  const int64_t C = gridDim.x, c = blockIdx.x;
+  const int64_t c = blockIdx.x;
   const int32_t B = a.num_seqs;
   const int64_t Hkv = a.num_kv_heads;
   int32_t* lens = scratch;
@@ -510,10 +523,7 @@ __device__ __forceinline__ Span compute_warp_spans_smem(const DecodeArgs& a, Sca
   }
   Span sp;
   sp.W = total * Hkv;
-  sp.q = sp.W / C;
-  sp.rem = sp.W % C;
-  sp.r0 = span_begin(c, sp.q, sp.rem);
-  sp.r1 = sp.r0 + sp.q + (c < sp.rem ? 1 : 0);
+  share_units(a, sp);
   sp.seq = -1;
   sp.prefix = 0;
   if (sp.r0 < sp.r1 && local > 0) {
@@ -645,7 +655,7 @@ __device__ __forceinline__ bool warp_write_record(const DecodeArgs& a, const Spa
 // for 2 * n * G + 2 * G floats.  Row weights are computed once per record, then
 // the O rows stream in as float4 loads that do not depend on one another.
 // Must be called by all threads of the CTA (it synchronises them).
-template <typename OutT, bool CHUNK = false>
+template <typename OutT>
 __device__ void cta_merge_records(const DecodeArgs& a, const Span& sp, int32_t seq, int32_t kvh,
                                   int64_t seg_unit, int32_t nb, float* scratch) {
   const int G = a.groups, D = a.head_dim;
@@ -692,10 +702,10 @@ __device__ void cta_merge_records(const DecodeArgs& a, const Span& sp, int32_t s
     rowInvL[tid] = 1.f / L;
   }
   __syncthreads();
-  const OutRows<CHUNK> to(a, seq, kvh);
+  OutT* out = static_cast<OutT*>(a.out) + static_cast<int64_t>(seq) * a.o_stride_seq +
+              static_cast<int64_t>(kvh) * G * D;
   for (int e4 = tid; e4 < E4; e4 += nthr) {
     const int r = (e4 * 4) / D;
-    if (CHUNK && r >= to.rows) break;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c0 = 0; c0 < n; c0 += kBatch) {
       if (e4 != tid || c0 != 0) {  // else: prefetched above
@@ -716,11 +726,10 @@ __device__ void cta_merge_records(const DecodeArgs& a, const Span& sp, int32_t s
       }
     }
     const float inv = rowInvL[r];
-    OutT* out = static_cast<OutT*>(a.out) + to.row(r, D) + (e4 * 4 - r * D);
-    store_out<OutT>(out + 0, acc.x * inv);
-    store_out<OutT>(out + 1, acc.y * inv);
-    store_out<OutT>(out + 2, acc.z * inv);
-    store_out<OutT>(out + 3, acc.w * inv);
+    store_out<OutT>(out + 4 * e4 + 0, acc.x * inv);
+    store_out<OutT>(out + 4 * e4 + 1, acc.y * inv);
+    store_out<OutT>(out + 4 * e4 + 2, acc.z * inv);
+    store_out<OutT>(out + 4 * e4 + 3, acc.w * inv);
   }
   __syncthreads();  // scratch may be reused
 }

@@ -716,14 +716,125 @@ int occupancy_one() {
 }
 
 template <int D, bool CHUNK>
-int launch_rows(const DecodeArgs& a, int grid, cudaStream_t stream) {
-  return a.groups > 8 ? launch_one<D, 2, CHUNK>(a, grid, stream)
-                      : launch_one<D, 1, CHUNK>(a, grid, stream);
+int occupancy_rows(int rows) {
+  return rows > 8 ? occupancy_one<D, 2, CHUNK>() : occupancy_one<D, 1, CHUNK>();
+}
+
+// Joins, behind the decode kernel, the records of the segments that are cut across CTAs: one
+// CTA for each of its CTAs (`tasks`).  A warp takes a row's maximum, weights and sum, then the
+// threads share the records out, a 16-byte piece of the rows each, kBatch loads at a time.
+constexpr int kMergeThreads = 256;
+template <int D, bool CHUNK>
+__global__ void __launch_bounds__(kMergeThreads, 3) merge_int4_kernel(const DecodeArgs a) {
+  constexpr int kBatch = 8, kWarps = kMergeThreads / 32;
+  extern __shared__ float weights[];  // [records][rows]
+  __shared__ float inverse[kShortChunkRows];
+  __shared__ float4 sums[kMergeThreads];
+  pdl_wait();
+  const MergeTask t = a.tasks[blockIdx.x];
+  if (!t.valid) return;
+  const int G = a.groups, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t first = span_owner(t.seg_unit, t.q, t.rem);
+  const int n = static_cast<int>(span_owner(t.seg_unit + t.nb - 1, t.q, t.rem) - first + 1);
+  // (Behind its first CTA the segment is what a span begins with.)
+  const float* rec0 = a.partials + record_index(first, t.seg_unit, t.q, t.rem) * a.rec_stride;
+  const float* rest = a.partials + first * 2 * a.rec_stride;
+  auto record = [&](int c) { return c == 0 ? rec0 : rest + static_cast<int64_t>(2 * c) * a.rec_stride; };
+  const int pieces = G * D / 4, width = (pieces + 31) / 32 * 32;
+  const int sets = width >= kMergeThreads ? 1 : kMergeThreads / width;
+  const int set = tid / width, own = tid - set * width;  // (set >= sets: no part)
+  float4 v[kBatch];
+  auto fetch = [&](int piece, int c0) {  // pieces of the set's next records
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int c = c0 + u * sets;
+      if (c < n) v[u] = __ldcg(reinterpret_cast<const float4*>(record(c)) + piece);
+    }
+  };
+  if (set < sets && own < pieces) fetch(own, set);  // with the maxima and sums: one trip
+  for (int r = warp; r < G; r += kWarps) {
+    float m = -INFINITY, l = 0.f;
+    for (int c = lane; c < n; c += 32) {
+      const float x = __ldcg(record(c) + G * D + r);
+      weights[c * G + r] = x;
+      m = fmaxf(m, x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int c = lane; c < n; c += 32) {
+      const float w = fast_exp2(weights[c * G + r] - m);
+      weights[c * G + r] = w;
+      l += w * __ldcg(record(c) + G * D + G + r);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) inverse[r] = 1.f / l;
+  }
+  __syncthreads();
+  const OutRows<CHUNK> to(a, t.seq, t.kvh);
+  for (int p0 = 0; p0 < pieces; p0 += kMergeThreads) {  // (more than one turn: one set)
+    const int piece = p0 + own, r = piece * 4 / D;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (set < sets && piece < pieces) {
+      for (int c0 = set; c0 < n; c0 += kBatch * sets) {
+        if (p0 != 0 || c0 != set) fetch(piece, c0);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int c = c0 + u * sets;
+          if (c < n) {
+            const float w = weights[c * G + r];
+            acc.x += w * v[u].x;
+            acc.y += w * v[u].y;
+            acc.z += w * v[u].z;
+            acc.w += w * v[u].w;
+          }
+        }
+      }
+    }
+    if (sets > 1) {
+      sums[tid] = acc;
+      __syncthreads();
+      if (set == 0) {
+        for (int k = 1; k < sets; ++k) {
+          const float4 x = sums[k * width + own];
+          acc.x += x.x;
+          acc.y += x.y;
+          acc.z += x.z;
+          acc.w += x.w;
+        }
+      }
+    }
+    if (set == 0 && piece < pieces && r < to.rows) {
+      const float inv = inverse[r];
+      const uint2 o = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv),
+                                 pack_bf16x2(acc.z * inv, acc.w * inv));
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + to.row(r, D) + piece * 4 -
+                                r * D) = o;
+    }
+  }
 }
 
 template <int D, bool CHUNK>
-int occupancy_rows(int rows) {
-  return rows > 8 ? occupancy_one<D, 2, CHUNK>() : occupancy_one<D, 1, CHUNK>();
+int launch_merge(const DecodeArgs& a, int grid, cudaStream_t stream) {
+  // Room for the weights of 16 rows and 700 CTAs; the grids hold at most four an SM.
+  constexpr int kMaxSmem = 45 * 1024;
+  static unsigned long long configured = 0;  // one bit per device
+  cudaError_t e = once_per_device(&configured, [] {
+    return cudaFuncSetAttribute(merge_int4_kernel<D, CHUNK>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+  });
+  if (e != cudaSuccess) return static_cast<int>(e);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kMergeThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(grid) * a.groups * sizeof(float);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, merge_int4_kernel<D, CHUNK>, a));
 }
 
 // Short chunks as sequences of the kernel above; without tokens, of length 0.
@@ -740,19 +851,22 @@ __global__ void __launch_bounds__(128) chunk_rows_kernel(const WindowArgs a, int
   table_rows[b] = any ? w.row : 0;
 }
 
+template <int D, bool CHUNK>
+int launch_rows(const DecodeArgs& a, int grid, cudaStream_t stream) {
+  const int rc = a.groups > 8 ? launch_one<D, 2, CHUNK>(a, grid, stream)
+                              : launch_one<D, 1, CHUNK>(a, grid, stream);
+  return rc != 0 || a.tasks == nullptr ? rc : launch_merge<D, CHUNK>(a, grid, stream);
+}
+
 }  // namespace
 
 int launch_decode_int4(const DecodeArgs& a, int grid, cudaStream_t stream) {
-  int rc;
   if (a.chunk_rows != nullptr) {
-    rc = a.head_dim == 64 ? launch_rows<64, true>(a, grid, stream)
-                          : launch_rows<128, true>(a, grid, stream);
-  } else {
-    rc = a.head_dim == 64 ? launch_rows<64, false>(a, grid, stream)
-                          : launch_rows<128, false>(a, grid, stream);
+    return a.head_dim == 64 ? launch_rows<64, true>(a, grid, stream)
+                            : launch_rows<128, true>(a, grid, stream);
   }
-  if (rc != 0 || a.tasks == nullptr) return rc;
-  return launch_decode_merge(a, grid, stream);
+  return a.head_dim == 64 ? launch_rows<64, false>(a, grid, stream)
+                          : launch_rows<128, false>(a, grid, stream);
 }
 
 int decode_int4_ctas_per_sm(int head_dim, int rows, bool chunks) {

@@ -207,8 +207,4 @@ __device__ __forceinline__ void record_cut(const DecodeArgs& a, const Span& sp, 
   }
 }
 
-// The merge pass of the segments that a launch of `grid` CTAs listed in a.tasks
-// (decode_mma.cu).
-int launch_decode_merge(const DecodeArgs& a, int grid, cudaStream_t stream);
-
 }  // namespace bsb

@@ -620,7 +620,6 @@ int launch_one(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap& 
 // Merges, after the decode kernel, the cut segments its CTAs listed: one CTA
 // per decode CTA, all threads on the records of one segment.
 // Three CTAs per SM: as many as the decode kernel's grid holds, all in one wave.
-template <bool CHUNK>
 __global__ void __launch_bounds__(128, 3) decode_merge_kernel(const DecodeArgs a) {
   extern __shared__ float merge_scratch[];
   pdl_wait();
@@ -629,32 +628,7 @@ __global__ void __launch_bounds__(128, 3) decode_merge_kernel(const DecodeArgs a
   Span sp{};
   sp.q = t.q;
   sp.rem = t.rem;
-  cta_merge_records<__nv_bfloat16, CHUNK>(a, sp, t.seq, t.kvh, t.seg_unit, t.nb, merge_scratch);
-}
-
-template <bool CHUNK>
-int launch_merge(const DecodeArgs& a, int grid, cudaStream_t stream) {
-  const int smem = static_cast<int>((2 * static_cast<int64_t>(grid) * a.groups + 2 * a.groups) *
-                                    sizeof(float));
-  // Room for 16 rows and 700 CTAs; the grids hold at most four an SM.
-  constexpr int kMaxSmem = 90 * 1024;
-  static unsigned long long configured = 0;  // one bit per device
-  cudaError_t e = once_per_device(&configured, [] {
-    return cudaFuncSetAttribute(decode_merge_kernel<CHUNK>,
-                                cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
-  });
-  if (e != cudaSuccess) return static_cast<int>(e);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_merge_kernel<CHUNK>, a));
+  cta_merge_records<__nv_bfloat16>(a, sp, t.seq, t.kvh, t.seg_unit, t.nb, merge_scratch);
 }
 
 template <int D, bool G16, bool WIN>
@@ -670,15 +644,30 @@ int occupancy_one() {
   return n;
 }
 
-}  // namespace
-
 // The merge pass of every form: at most `grid` records per segment.
-int launch_decode_merge(const DecodeArgs& a, int grid, cudaStream_t stream) {
-  return a.chunk_rows != nullptr ? launch_merge<true>(a, grid, stream)
-                                 : launch_merge<false>(a, grid, stream);
+int launch_merge(const DecodeArgs& a, int grid, cudaStream_t stream) {
+  const int smem = static_cast<int>((2 * static_cast<int64_t>(grid) * a.groups + 2 * a.groups) *
+                                    sizeof(float));
+  // Room for 16 heads a group and 700 CTAs; the grids hold at most three an SM.
+  constexpr int kMaxSmem = 90 * 1024;
+  static unsigned long long configured = 0;  // one bit per device
+  cudaError_t e = once_per_device(&configured, [] {
+    return cudaFuncSetAttribute(decode_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kMaxSmem);
+  });
+  if (e != cudaSuccess) return static_cast<int>(e);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_merge_kernel, a));
 }
-
-namespace {
 
 template <bool WIN>
 int launch_both(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap& vmap, int grid,
@@ -692,7 +681,7 @@ int launch_both(const DecodeArgs& a, const CUtensorMap& kmap, const CUtensorMap&
     rc = g16 ? launch_one<128, true, WIN>(a, kmap, vmap, grid, stream)
              : launch_one<128, false, WIN>(a, kmap, vmap, grid, stream);
   if (rc != 0 || a.tasks == nullptr) return rc;
-  return launch_decode_merge(a, grid, stream);
+  return launch_merge(a, grid, stream);
 }
 
 template <bool WIN>
