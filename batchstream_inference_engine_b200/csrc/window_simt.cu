@@ -20,9 +20,16 @@
 // joins through distributed shared memory while clusters take no more waves than single
 // CTAs would; else they leave records for a second kernel, which costs some 4 us.  Rows that are not whole 16-byte pieces are read one element at a time.
 //
+// Over 4-bit pools a group's codes are turned into floats on their way to shared memory, K's,
+// then V's in their place: an element costs some three instructions there, next to its four
+// to eight products.  Loads of eight rows' pieces are issued together and scores read 16 bytes:
+// 24 fp32 sequences of 1 to 4096 tokens, d64, whole context: 47 us (one element at a time: 68);
+// with 16 heads a group 94 (227).
+//
 // A weight of zero skips its V row, so NaN or infinities in a key that a row does
 // not see never reach that row.
 #include <mutex>
+#include <type_traits>
 #include <vector>
 
 #include "int4.cuh"
@@ -72,12 +79,13 @@ __device__ __forceinline__ void copy_wait() {
 // Shared memory of one warp: 32 K rows, then 32 V rows or the V rows in their place; at
 // the end its state, GM rows of head_dim floats.  Lanes read K rows in parallel, so a
 // pad of 16 bytes (one float in the element-wise form, which holds K as floats and
-// leaves V in the pool) moves consecutive rows to different banks.
-template <typename T, int GM, int DPL, bool VEC>
+// leaves V in the pool) moves consecutive rows to different banks.  Rows of 4-bit pools
+// are floats, V in K's place.
+template <typename T, int GM, int DPL, bool VEC, bool Q4>
 struct Layout {
   static constexpr bool kVOverK = DPL * 32 * sizeof(T) > 256;
   __host__ __device__ static int k_row(int D) {
-    return VEC ? D * static_cast<int>(sizeof(T)) + 16 : (D + 1) * 4;
+    return Q4 ? D * 4 + 16 : VEC ? D * static_cast<int>(sizeof(T)) + 16 : (D + 1) * 4;
   }
   __host__ __device__ static int v_row(int D) {
     return kVOverK ? k_row(D) : D * static_cast<int>(sizeof(T));
@@ -107,8 +115,8 @@ __device__ __forceinline__ void window_item(const WindowArgs& a, int64_t item, i
 // head_dim is exactly 32 DPL (its loops then have compile-time bounds); Q4: 4-bit pools.
 template <typename T, int GM, int DPL, bool VEC, bool FULL, bool Q4>
 __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs a) {
-  static_assert(!Q4 || (!VEC && !FULL), "4-bit rows are held as floats");
-  using L_ = Layout<T, GM, DPL, VEC>;
+  static_assert(!Q4 || !VEC, "4-bit rows are held as floats");
+  using L_ = Layout<T, GM, DPL, VEC, Q4>;
   extern __shared__ __align__(16) uint8_t wsm[];
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -201,24 +209,35 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
         copy_commit();
       }
     };
-    // A pool's rows as floats, a lane taking 8 dims at a time.
+    // A pool's rows as floats, a lane taking 8 dims at a time, of 4 or 8 rows at once.
     auto widen_rows = [&](const void* pool) {
-      const int per_row = D >> 3;
+      const int per_row = D >> 3;  // a multiple of 4
       const uint8_t* bytes = static_cast<const uint8_t*>(pool);
-#pragma unroll 4
-      for (int it = 0; it < per_row; ++it) {
-        const int idx = it * 32 + lane;
-        const int key = idx / per_row, c = idx - key * per_row;
-        const int64_t ko = __shfl_sync(0xffffffffu, off, key);
-        const int64_t so = __shfl_sync(0xffffffffu, scales, key);
-        if (ko < 0) continue;
-        float f[8];
-        int4_floats(__ldg(reinterpret_cast<const uint32_t*>(bytes + ko) + c),
-                    int4_scale_float(__ldg(reinterpret_cast<const uint16_t*>(bytes + so) + (c >> 2))),
-                    f);
-        float* dst = reinterpret_cast<float*>(sK + key * k_row) + 8 * c;
+      constexpr int kAtOnce = FULL && DPL > 1 ? 8 : 4;
+      for (int it = 0; it < per_row; it += kAtOnce) {
+        uint32_t words[kAtOnce];
+        uint16_t scale[kAtOnce];
+        int to[kAtOnce];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dst[i] = f[i];
+        for (int k = 0; k < kAtOnce; ++k) {
+          const int idx = (it + k) * 32 + lane;
+          const int key = idx / per_row, c = idx - key * per_row;
+          const int64_t ko = __shfl_sync(0xffffffffu, off, key);
+          const int64_t so = __shfl_sync(0xffffffffu, scales, key);
+          to[k] = ko < 0 ? -1 : key * k_row + 32 * c;
+          if (ko < 0) continue;
+          words[k] = __ldg(reinterpret_cast<const uint32_t*>(bytes + ko) + c);
+          scale[k] = __ldg(reinterpret_cast<const uint16_t*>(bytes + so) + (c >> 2));
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          if (to[k] < 0) continue;
+          float f[8];
+          int4_floats(words[k], int4_scale_float(scale[k]), f);
+          float4* dst = reinterpret_cast<float4*>(sK + to[k]);
+          dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+          dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+        }
       }
     };
     if constexpr (Q4) {
@@ -238,17 +257,19 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
     float s[GM];
 #pragma unroll
     for (int i = 0; i < GM; ++i) s[i] = 0.f;
-    if constexpr (VEC) {
-      const T* krow = reinterpret_cast<const T*>(sK + lane * k_row);
+    if constexpr (VEC || Q4) {
+      using Held = std::conditional_t<Q4, float, T>;
+      constexpr int kHeld = 16 / sizeof(Held);
+      const Held* krow = reinterpret_cast<const Held*>(sK + lane * k_row);
 #pragma unroll 4
-      for (int d = 0; d < D; d += kElems) {
-        float k[kElems];
+      for (int d = 0; d < D; d += kHeld) {
+        float k[kHeld];
         widen16(krow + d, k);
 #pragma unroll
         for (int i = 0; i < GM; ++i) {
           if (i < rows) {
 #pragma unroll
-            for (int x = 0; x < kElems; x += 4) {
+            for (int x = 0; x < kHeld; x += 4) {
               const float4 q4 = *reinterpret_cast<const float4*>(sQ + i * D + d + x);
               s[i] = fmaf(q4.x, k[x], fmaf(q4.y, k[x + 1],
                                            fmaf(q4.z, k[x + 2], fmaf(q4.w, k[x + 3], s[i]))));
@@ -452,13 +473,13 @@ cudaError_t allow_smem() {
   return once_per_device(&configured, [] {
     return cudaFuncSetAttribute(window_simt_kernel<T, GM, DPL, VEC, FULL, Q4>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                Layout<T, GM, DPL, VEC>::total(DPL * 32));
+                                Layout<T, GM, DPL, VEC, Q4>::total(DPL * 32));
   });
 }
 
 template <typename T, int GM, int DPL, bool VEC, bool FULL, bool Q4 = false>
 int launch_one(const WindowArgs& a, cudaStream_t stream) {
-  using L_ = Layout<T, GM, DPL, VEC>;
+  using L_ = Layout<T, GM, DPL, VEC, Q4>;
   const int smem = L_::total(a.head_dim);
   auto kernel = window_simt_kernel<T, GM, DPL, VEC, FULL, Q4>;
   const cudaError_t e = allow_smem<T, GM, DPL, VEC, FULL, Q4>();
@@ -495,9 +516,10 @@ int launch_full(const WindowArgs& a, cudaStream_t stream) {
 
 template <typename T, int GM>
 int launch_q4(const WindowArgs& a, cudaStream_t stream) {
-  if (a.head_dim <= 32) return launch_one<T, GM, 1, false, false, true>(a, stream);
-  if (a.head_dim <= 64) return launch_one<T, GM, 2, false, false, true>(a, stream);
-  if (a.head_dim <= 128) return launch_one<T, GM, 4, false, false, true>(a, stream);
+  if (a.head_dim == 32) return launch_one<T, GM, 1, false, true, true>(a, stream);
+  if (a.head_dim == 64) return launch_one<T, GM, 2, false, true, true>(a, stream);
+  if (a.head_dim == 128) return launch_one<T, GM, 4, false, true, true>(a, stream);
+  if (a.head_dim < 128) return launch_one<T, GM, 4, false, false, true>(a, stream);
   return launch_one<T, GM, 8, false, false, true>(a, stream);
 }
 
@@ -537,7 +559,7 @@ int at_once(int D, int cluster) {
   for (const Known& k : known) {
     if (k.device == dev && k.D == D && k.cluster == cluster) return k.count;
   }
-  using L_ = Layout<T, GM, DPL, VEC>;
+  using L_ = Layout<T, GM, DPL, VEC, Q4>;
   auto kernel = window_simt_kernel<T, GM, DPL, VEC, FULL, Q4>;
   e = allow_smem<T, GM, DPL, VEC, FULL, Q4>();
   int count = 0;
@@ -564,7 +586,12 @@ int at_once(int D, int cluster) {
 // As the launch chooses, with aligned pools.
 template <typename T, int GM, int DPL>
 int at_once_full(int D, int cluster, bool int4) {
-  if (int4) return at_once<T, GM, DPL, false, false, true>(D, cluster);
+  if (int4) {
+    if constexpr (DPL >= 4) {
+      if (D != 128) return at_once<T, GM, DPL, false, false, true>(D, cluster);
+    }
+    if constexpr (DPL <= 4) return at_once<T, GM, DPL, false, true, true>(D, cluster);
+  }
   if (D * sizeof(T) % 16 != 0) return at_once<T, GM, DPL, false, false>(D, cluster);
   return D == 32 * DPL ? at_once<T, GM, DPL, true, true>(D, cluster)
                        : at_once<T, GM, DPL, true, false>(D, cluster);
