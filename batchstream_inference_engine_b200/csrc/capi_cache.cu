@@ -271,7 +271,12 @@ struct ShortChunkPlan {
   MmaDecodePlan decode;
 };
 
-// Whether it runs them: up to two tiles of 8 rows.  FIGURES
+// Whether it runs them: up to two tiles of 8 rows.  us so / by the kernel of the long ones, chunks
+// of 2 (14 + 2 heads) or 4 (32 + 8): 64 of them behind up to 8192, d64, 51 / 74 and 115 / 182;
+// d128, 4 tokens, 174 / 225; 8 behind up to 4096 18 / 24, 31 / 37; a lone one behind 2500 16 /
+// 14.  Three tiles lose: 64 chunks of 3 (14 + 2 heads of 64) 67 / 74, 200 of them behind up to
+// 2000 64 / 53, at d128 163 / 134; and so do two turns of two tiles (32 + 8 heads, 8 tokens: 306 /
+// 222).
 bool short_chunks(const WindowShape& s) {
   return s.int4 && s.chunks && mma_shape(s) && s.max_query_len > 0 &&
          s.max_query_len <= bsb::kShortChunkRows / (s.heads / s.kv_heads);
@@ -300,7 +305,9 @@ int plan_mma_chunks(const WindowShape& s, MmaChunkPlan* p) {
   if (int rc = bsb::sm_count(&sms)) return rc;
   const int64_t groups = s.heads / s.kv_heads;
   // Over 4-bit pools two tiles share K and V, which are costly to write, where a chunk has
-  // rows for both; then one CTA runs on an SM, else two.
+  // rows for both; then one CTA runs on an SM, else two.  us with one / two: 8 chunks of 512, d64
+  // 92 / 86; 6 ragged ones of 100 to 2048, d128, 965 / 793; a lone one of 2048, d128, 66 / 55;
+  // 24 of 128, d64, 174 / 150.
   const bool both = s.int4 && s.max_query_len > bsb::kWindowTileRows / groups;
   const int64_t resident = (both ? 1 : 2) * static_cast<int64_t>(sms);
   p->tile_rows = (both ? 2 : 1) * bsb::kWindowTileRows;
@@ -322,10 +329,15 @@ int plan_mma_chunks(const WindowShape& s, MmaChunkPlan* p) {
                                 std::min(s.window, kMaxContext) + std::min(s.sinks, kMaxContext) +
                                     p->tile_tokens + 32);
   const int64_t most = keys / (bsb::kWindowStepKeys * bsb::kMinWindowSteps);
-  // (4-bit chunks of one tile: as far as more than one wave goes.  64 chunks of 5 behind up to
-  // 8192 tokens, us with 1 / 2 / 3 ranges: d64 (128 tiles) -- / 99 / 74, d128 (256) 217 / 139 /
-  // 156; of two tiles the rule above holds: 8 of 128, d64, with 2 / 3: 27 / 37.)
-  const int64_t want = s.int4 && !both ? (resident + busy - 1) / busy : resident / busy;
+  // Over 4-bit pools as far as more than one wave goes, but for a lone chunk, whose tiles are as
+  // long as one another: a range costs less next to the values it has to turn, and sequences of
+  // different lengths fill the places better.  us behind up to 8192 tokens, one wave at most /
+  // more: 16 chunks of 128, d64 (128 pairs of tiles on 148 places) 145 / 94; 8 of 300 (144) 147 /
+  // 90; 8 of 128, d128 (128) 162 / 102; 64 of 5, d64 (128 tiles on 296) 99 / 74; a lone one of
+  // 1000, d128 (112) 39 / 49.  Two waves where one is full already gain for some and lose for
+  // others: 40 of 64 (160 pairs) 150 / 104, 8 of 512 behind none (240) 33 / 47.
+  const int64_t want =
+      s.int4 && (!both || s.rows > 1) ? (resident + busy - 1) / busy : resident / busy;
   const int64_t record = p->tile_rows * (s.head_dim + 2) * 4;
   p->splits = std::max<int64_t>(
       1, std::min(std::min<int64_t>(want, bsb::kMaxWindowRanges), most));
@@ -396,6 +408,9 @@ bool mma_pointers(const WindowCall& c) {
          aligned16(c.output) && c.q_stride % 8 == 0 && c.o_stride % 8 == 0;
 }
 
+// Spans of 16 units or more: a sequence's records are joined by one CTA.  us with no bound / 8 /
+// 16 / 32 units, 14 + 2 heads of 64: one sequence of 32768 64 / 41 / 29 / 25, 64 of 1 to 16384
+// (log-uniform) 33 / 33 / 33 / 31, 200 of 1 to 4096 31 / 31 / 31 / 35.
 constexpr int kInt4SpanShift = 4;
 
 // The arguments of the tensor-core decode that are alike for single tokens and chunks.

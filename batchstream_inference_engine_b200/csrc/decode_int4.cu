@@ -45,9 +45,11 @@ template <int D, int NQ, bool CHUNK_>
 struct Cfg {
   static constexpr bool CHUNK = CHUNK_;
   static constexpr int W = 4;                    // warps per CTA
-  static constexpr int U = 2;                    // units of a step
+  static constexpr int U = 2;                    // units of a step (with one: 51 for 49 us, 100 for 96)
   static constexpr int S = D == 64 ? 4 : 3;      // stages per warp, a step each
-  static constexpr int MIN_CTAS = D == 64 ? 5 - NQ : 4 - NQ;
+  // CTAs per SM.  us with one more / these / one fewer, 256 sequences of 2048, d64, one tile of
+  // rows: 49 / 45 / --, two: 55 / 53 / --; d128, one: (spills) / 96 / 98, two: -- / 121 / 123.
+  static constexpr int MIN_CTAS = 4 - NQ;
   static constexpr int GROWS = 8 * NQ;
   static constexpr int CODE_BYTES = kWindowUnit * D / 2;  // of a unit, K or V
   static constexpr int SCALE_BYTES = kWindowUnit * D / 16;
