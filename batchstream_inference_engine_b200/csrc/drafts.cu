@@ -17,6 +17,13 @@
 // its tokens weigh 1e-5 each, an error of 1e-7 in the sum ahead of one moves one draw in a
 // hundred to its neighbour.  Each warp sums a range of the row in blocks of 256 tokens and
 // keeps the sums of up to 64 parts of it, so that the draw walks one part again.
+//
+// 64 sequences with four drafts each from a small model, 151936 bf16 logits: 72 us (floor 15),
+// 28 of them the first pass, 3.5 TB/s, bound by issuing and by CTAs that each hold one piece
+// (2.4 instructions a clock and SM, DRAM 42% busy); the rest is the draw, two passes over a row's
+// weights, some 20 instructions a token (2.4 a clock and SM, fp64 units 28% busy).  One sequence:
+// 13 us; 200 ragged ones, 32003 fp32 logits: 54 (floor 16).  Not kept: 768 or 1024 threads a
+// drawing CTA, four or eight CTAs an SM in the first pass (within 3%).
 #include "common.cuh"
 #include "drafts.cuh"
 

@@ -7,6 +7,12 @@
 //
 // A thread takes 8 dims at a time, four of them a group, which finds its extremes with
 // shuffles.  One CTA per token.
+//
+// 4096 tokens, 28 + 2 x 4 heads of 128, all turned: 24 us, then a read of all rows (6), 2.9
+// TB/s of what the append reads and writes.  What bounds it is latency: the position, the
+// slot, the row, the angles' fp64 sine and cosine and the group's extremes follow one
+// another (2.0 instructions a clock and SM).  96 or 64
+// threads a CTA take the same, 192 2 us more, 288 12.
 #include "int4.cuh"
 
 namespace bsb {
