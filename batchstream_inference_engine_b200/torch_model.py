@@ -498,8 +498,14 @@ class TorchModel:
         other temperatures (a number, or one per group on the device); ``draft_probs``
         [input tokens, vocab] holds, in the row of the token ahead of each draft, what it was
         drawn from (None: drafts were certain)."""
+        if not groups:
+            return []
+        if any(not tokens for tokens, _ in groups):
+            raise RuntimeError("verify_tokens: a group needs its input token")
         if any(t < 0 for tokens, _ in groups for t in tokens):
             raise RuntimeError("verify_tokens: token references cannot be verified")
+        if len({id(cache) for _, cache in groups}) < len(groups):
+            raise RuntimeError("verify_tokens: a sequence can be in one group only")
         pool = groups[0][1]._pool
         lengths = [len(tokens) for tokens, _ in groups]
         T = sum(lengths)

@@ -250,6 +250,13 @@ def test_model_refuses():
         model.verify_tokens([([1, 2], cache)], temperature=0.5)
     with pytest.raises(RuntimeError, match="references"):
         model.verify_tokens([([-1, 2], cache)])
+    with pytest.raises(RuntimeError, match="input token"):
+        model.verify_tokens([([1], pool.new_cache(1)), ([], cache)])
+    with pytest.raises(RuntimeError, match="one group"):
+        model.verify_tokens([([1, 2], cache), ([3], cache)])
+    with pytest.raises(RuntimeError, match="index"):
+        model.verify_tokens([([1, 1 << 20], cache)])
+    assert model.verify_tokens([]) == []
     assert cache.length == 0
     odd = dataclasses.replace(CONFIG, hidden_size=160, num_heads=4, num_kv_heads=2)
     with pytest.raises(RuntimeError, match="multiple of 32"):
