@@ -61,7 +61,7 @@ template <int D, int NQ, bool CHUNK_>
 struct Cfg {
   static constexpr bool CHUNK = CHUNK_;
   static constexpr int W = 4;                    // warps per CTA
-  static constexpr int U = 2;                    // units of a step (with one: 51 for 49 us, 100 for 96)
+  static constexpr int U = 2;                    // units of a step (with one: 72 for 66, 289 for 268 us)
   static constexpr int S = D == 64 ? 4 : 3;      // stages per warp, a step each
   // CTAs per SM.  us with one more / these / one fewer, 256 sequences of 2048, d64, one tile of
   // rows: 49 / 45 / --, two: 55 / 53 / --; d128, one: (spills) / 96 / 98, two: -- / 121 / 123.

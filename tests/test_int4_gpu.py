@@ -669,6 +669,28 @@ def test_short_chunk_padding_and_strides():
     assert bool((room[:, 14 * 64:] == SENTINEL).all())
 
 
+@pytest.mark.parametrize("far", [-1e30, 1e30, 2e35])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_short_chunk_scores_far_from_zero(head_dim, far):
+    test_scores_far_from_zero(2, head_dim, far)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("head_dim,priors", [(64, [300, 20]), (128, [300, 20]), (64, [5000, 9])])
+def test_short_chunk_rows_of_non_finite_queries_stay_alone(head_dim, priors, bad):
+    c = Packed([p + 2 for p in priors], [2] * 2, 14, 2, head_dim, 16, torch.bfloat16, 1 << 40, 0,
+               seed=35)
+    want = c.chunks()
+    c.check(want)
+    c.q[1, 3, 5] = bad
+    out = c.chunks()
+    assert ops.take_status() == 0
+    assert not bool(out[1, 3].isfinite().all())
+    keep = torch.ones(4, 14, dtype=torch.bool)
+    keep[1, 3] = False
+    assert torch.equal(out[keep.to(DEV)], want[keep.to(DEV)])
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 20.0])
 @pytest.mark.parametrize("head_dim", [64, 128])
 def test_short_chunk_scales(scale, head_dim):
@@ -840,6 +862,45 @@ def test_captured_calls_share_no_scratch(dtype):
             assert torch.equal(out, want)
             out.zero_()
         torch.cuda.synchronize()
+    assert ops.take_status() == 0
+
+
+def test_captured_short_chunks_share_no_scratch_and_follow_their_inputs():
+    # Few and many chunks (clusters, spans), replayed on two streams at once; then the first chunk
+    # of each becomes padding, which leaves its rows as they were and moves nothing else.
+    cases = [Packed([p + 2 for p in priors], [2] * len(priors), 14, 2, 64, 16, torch.bfloat16,
+                    1 << 40, 0, seed=s)
+             for s, priors in ((57, [100, 40, 9]), (58, [1000 + 7 * i for i in range(90)]),
+                               (59, [3000 + 11 * i for i in range(70)]))]
+    runs = []
+    for c in cases:
+        want = c.chunks()
+        c.check(want)
+        q, out = c.q.to(DEV), torch.zeros_like(want)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.int4_prefill_attention(q, c.k, c.v, c.table, c.cu, c.len_d, c.scale, 2, out=out)
+        runs.append((graph, q, out, want, torch.cuda.Stream()))
+    for turn in range(6):
+        for c, (graph, _, out, _, s) in zip(cases, runs):
+            if turn == 3:
+                c.len_d[0] = 0
+            torch.cuda.synchronize()
+            with torch.cuda.stream(s):
+                out.fill_(SENTINEL)
+        for graph, _, _, _, s in runs:
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for c, (_, q, out, want, _) in zip(cases, runs):
+            if turn < 3:
+                assert torch.equal(out, want)
+                continue
+            # (The spans are others now: the same sums in another order.)
+            assert bool((out[:2] == SENTINEL).all())
+            ref, tol = c.reference()
+            assert bool(((out.double().cpu() - ref).abs() <= tol)[2:].all())
     assert ops.take_status() == 0
 
 
