@@ -216,7 +216,15 @@ constexpr int64_t kMaxSegmentCtas = 8;
 // (c = 3), 1024 (6): 12.5 / 15.6, 2048 (11): 17.9 / 16.5; 200 (c = 1), 512 (8.5): 14.4 /
 // 15.6, 1024 (17): 23.0 / 17.5; d128, 28 + 4 heads, 32 (c = 2), 1024 (8.4): 16.6 / 19.4,
 // 2048 (16): 25.4 / 21.2.
-bool clusters_win(int64_t c, int64_t most) { return most <= c * 4 * (c >= 4 ? 16 : 9); }
+// Over 4-bit pools a unit is cheap next to a scan and a merge; spans / clusters, all sequences of
+// one length (or log-uniform up to it): d64, 14 + 2 heads: 200 of 1024 (c = 1, 16 units a warp)
+// 30.8 / 20.5 (22.5 / 16.4), of 2048 (32) 38.9 / 30.7 (24.6 / 22.5), 64 of 4096 (c = 3, 21) 32.8 /
+// 26.6 (22.5 / 20.5), of 16384 (85) -- (26.7 / 43.0); 4 of 16384 (c = 8, 32) 26.6 / 22.5, of 32768
+// (64) 30.7 / 34.8; d128, 28 + 4 heads: 100 of 1024 (c = 1, 16) 41.0 / 28.7, 32 of 8192 (c = 3, 43)
+// 59.4 / 57.3 (34.8 / 38.9).
+bool clusters_win(int64_t c, int64_t most, bool int4) {
+  return most <= c * 4 * (int4 ? (c >= 4 ? 40 : 32) : (c >= 4 ? 16 : 9));
+}
 
 // `seqs` sequences of `rows` query rows a kv head, of `tokens` query tokens each.
 int plan_mma_decode(const WindowShape& s, int64_t seqs, int64_t rows, int64_t tokens,
@@ -249,7 +257,7 @@ int plan_mma_decode(const WindowShape& s, int64_t seqs, int64_t rows, int64_t to
   if (segments > 0 && segments <= resident) {
     const int64_t c = std::min({kMaxSegmentCtas, std::max<int64_t>(resident / segments, 1),
                                 std::max<int64_t>((most + 3) / 4, 1)});
-    if (clusters_win(c, most)) {
+    if (clusters_win(c, most, s.int4)) {
       p->segment_ctas = c;
       p->grid = segments * c;
       p->rec_stride = p->tasks_offset = p->bytes = 0;

@@ -309,6 +309,21 @@ def test_decode_long_rows_are_split_and_joined(dtype, head_dim, lens):
         assert torch.equal(c.decode(), out)
 
 
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(14, 2, 64), (28, 4, 128), (16, 1, 64)])
+@pytest.mark.parametrize("lens,new", [([30000], 1), ([25000, 3, 700], 1), ([30000, 40], 2),
+                                      ([300 + 9 * i for i in range(250)], 2)])
+def test_rows_cut_across_spans_of_the_batch(heads, kv_heads, head_dim, lens, new):
+    if new * heads // kv_heads > 16:
+        new = 1
+    c = Packed(lens, [new] * len(lens), heads, kv_heads, head_dim, 16, torch.bfloat16, 1 << 40, 0,
+               seed=13)
+    run = c.decode if new == 1 else c.chunks
+    out = run()
+    assert ops.take_status() == 0
+    c.check(out)
+    assert torch.equal(run(), out)
+
+
 @pytest.mark.parametrize("heads,kv_heads,head_dim", [(14, 2, 64), (28, 4, 128), (16, 1, 128)])
 @pytest.mark.parametrize("window", [1 << 40, 256])
 def test_decode_large_batch_many_lengths(heads, kv_heads, head_dim, window):
