@@ -280,8 +280,8 @@ struct ShortChunkPlan {
 };
 
 // Whether it runs them: up to two tiles of 8 rows.  us so / by the kernel of the long ones, chunks
-// of 2 (14 + 2 heads) or 4 (32 + 8): 64 of them behind up to 8192, d64, 51 / 74 and 115 / 182;
-// d128, 4 tokens, 174 / 225; 8 behind up to 4096 18 / 24, 31 / 37; a lone one behind 2500 16 /
+// of 2 (14 + 2 heads) or 4 (32 + 8): 64 of them behind up to 8192, d64, 49 / 74 and 119 / 182;
+// d128, 4 tokens, 172 / 225; 8 behind up to 4096 16 / 24, 29 / 37; a lone one behind 2500 14 /
 // 14.  Three tiles lose: 64 chunks of 3 (14 + 2 heads of 64) 67 / 74, 200 of them behind up to
 // 2000 64 / 53, at d128 163 / 134; and so do two turns of two tiles (32 + 8 heads, 8 tokens: 306 /
 // 222).
