@@ -504,6 +504,8 @@ class TorchModel:
             raise RuntimeError("verify_tokens: a group needs its input token")
         if any(t < 0 for tokens, _ in groups for t in tokens):
             raise RuntimeError("verify_tokens: token references cannot be verified")
+        if any(t >= self.embed.size(0) for tokens, _ in groups for t in tokens):
+            raise RuntimeError("verify_tokens: a token index is outside the vocabulary")
         if len({id(cache) for _, cache in groups}) < len(groups):
             raise RuntimeError("verify_tokens: a sequence can be in one group only")
         pool = groups[0][1]._pool

@@ -255,9 +255,9 @@ def test_model_refuses():
     with pytest.raises(RuntimeError, match="one group"):
         model.verify_tokens([([1, 2], cache), ([3], cache)])
     with pytest.raises(RuntimeError, match="index"):
-        model.verify_tokens([([1, 1 << 20], cache)])
+        model.verify_tokens([([1, VOCAB], cache)])
     assert model.verify_tokens([]) == []
-    assert cache.length == 0
+    assert cache.length == 0 and ops.take_status() == 0
     odd = dataclasses.replace(CONFIG, hidden_size=160, num_heads=4, num_kv_heads=2)
     with pytest.raises(RuntimeError, match="multiple of 32"):
         PagedKVPool(odd, 8, 16, device=DEV, dtype=torch.uint8)
