@@ -222,12 +222,13 @@ class PagedBackend:
         drafts gives one output, as in ``step``.  With temperature 0 the outputs are
         ``step``'s; else they are distributed as the model's samples at that temperature,
         by random numbers from ``generator`` (on the model's device).  Prompts wait for
-        ``step``; a launched step must be finished first."""
+        ``step``; a launched step must be finished first.  Drafts behind one that would end
+        the generation are not looked at."""
         batch = []
         for seq_id, tokens in self._generating_inputs():
             if self._sequences[seq_id].feeds is not None:
                 raise RuntimeError(f"sequence {seq_id} has an unfinished step")
-            batch.append((seq_id, tokens + list(drafts.get(seq_id, ()))))
+            batch.append((seq_id, tokens + self._up_to_end(drafts.get(seq_id, ()))))
         if not batch:
             return {}
         uniforms = None
@@ -238,13 +239,15 @@ class PagedBackend:
             [(tokens, self._sequences[s].cache) for s, tokens in batch], temperature, uniforms)
         outputs = {}
         for (seq_id, _), tokens in zip(batch, results):
-            sequence, outputs[seq_id] = self._sequences[seq_id], []
-            for token in tokens:
-                sequence.next_token = token
-                sequence.finished = self._vocab.is_end_of_generation(token)
-                outputs[seq_id].append(StepOutput(token, sequence.finished))
-                if sequence.finished:
-                    break
+            sequence = self._sequences[seq_id]
+            sequence.next_token = tokens[-1]
+            # Of the drafts that hold only the last may end the generation.  It is cached then:
+            # the token behind it is nobody's, and a fork has nothing to feed again.
+            if len(tokens) > 1 and self._vocab.is_end_of_generation(tokens[-2]):
+                tokens, sequence.next_token = tokens[:-1], None
+            sequence.finished = self._vocab.is_end_of_generation(tokens[-1])
+            outputs[seq_id] = [StepOutput(token, False) for token in tokens[:-1]]
+            outputs[seq_id].append(StepOutput(tokens[-1], sequence.finished))
         return outputs
 
     def release_sequence(self, seq_id: int) -> None:
@@ -252,6 +255,15 @@ class PagedBackend:
 
     def close(self) -> None:
         pass
+
+    def _up_to_end(self, drafts) -> list[int]:
+        """Drafts as far as the first that would end the generation."""
+        tokens = []
+        for token in drafts:
+            tokens.append(token)
+            if self._vocab.is_end_of_generation(token):
+                break
+        return tokens
 
     def _generating_inputs(self) -> list[tuple[int, list[int]]]:
         return [
