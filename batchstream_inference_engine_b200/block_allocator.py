@@ -10,10 +10,10 @@ every table into an int32 tensor ``[max_seqs, max_blocks_per_seq]`` on the GPU
 from device memory; only new table entries cross PCIe, batched into one copy per
 ``sync_device()``.
 
-Three operations go beyond the reference: ``fork`` starts a sequence from the
+Four operations go beyond the reference: ``fork`` starts a sequence from the
 cached tokens of another (whole blocks are shared and reference-counted, the last
 partial one is copied), ``trim`` frees the blocks that a sliding window has left
-behind, and ``compact`` renumbers the blocks in use to the lowest ids.  ``fork``
+behind, ``shrink`` those behind a sequence's tokens, and ``compact`` renumbers the blocks in use to the lowest ids.  ``fork``
 and ``compact`` return the (source, destination) block copies that the caller owes
 the pool (``ops.copy_blocks``) before the next step.
 """
@@ -184,6 +184,24 @@ class BlockAllocator:
         elif end >= low:
             low = min(low, keep)
         self._kept[seq_id], self._trimmed[seq_id] = low, max(high, end)
+        return freed
+
+    def held_blocks(self, seq_id: int) -> int:
+        """Entries of seq_id's table (0 for a sequence without one)."""
+        return len(self._tables.get(seq_id, ()))
+
+    def shrink(self, seq_id: int, total_tokens: int) -> int:
+        """Gives up the blocks of seq_id behind its first `total_tokens` tokens, the last one
+        first (as ``allocate`` took them).  Returns how many that freed."""
+        table = self._tables.get(seq_id, [])
+        keep, freed = -(-total_tokens // self._block_size), 0
+        while len(table) > keep:
+            freed += self._release(table.pop())
+        if seq_id in self._synced:
+            self._synced[seq_id] = min(self._synced[seq_id], len(table))
+        if seq_id in self._trimmed:
+            self._trimmed[seq_id] = min(self._trimmed[seq_id], len(table))
+            self._kept[seq_id] = min(self._kept[seq_id], len(table))
         return freed
 
     def moves(self) -> list[tuple[int, int]]:

@@ -493,11 +493,11 @@ class TorchModel:
         """A step that verifies drafted tokens (``ops.verify_drafts``): each group's tokens are
         its next input token and the drafts behind it.  Returns, for each group, the drafts
         that were accepted and the token after them; the cache then holds the input token
-        and the accepted drafts.  With temperature 0 these are the tokens that as many
-        greedy steps would give.  ``uniforms`` (fp32, one per input token) is needed for
-        other temperatures (a number, or one per group on the device); ``draft_probs``
-        [input tokens, vocab] holds, in the row of the token ahead of each draft, what it was
-        drawn from (None: drafts were certain)."""
+        and the accepted drafts, and blocks taken for the others are free again.  With
+        temperature 0 these are the tokens that as many greedy steps would give.  ``uniforms``
+        (fp32, one per input token) is needed for other temperatures (a number, or one per
+        group on the device); ``draft_probs`` [input tokens, vocab] holds, in the row of the
+        token ahead of each draft, what it was drawn from (None: drafts were certain)."""
         if not groups:
             return []
         if any(not tokens for tokens, _ in groups):
@@ -515,6 +515,16 @@ class TorchModel:
             if torch.is_tensor(temperature) or temperature != 0.0:
                 raise RuntimeError("verify_tokens: a temperature needs uniforms")
             uniforms = torch.zeros(T, device=self.device)
+        held = [pool.allocator.held_blocks(cache.seq_id) for _, cache in groups]
+        try:
+            return self._verify(pool, groups, lengths, temperature, uniforms, draft_probs)
+        finally:
+            # The blocks of drafts that did not hold, or of a step that could not run.
+            for (_, cache), blocks in zip(reversed(groups), reversed(held)):
+                pool.allocator.shrink(cache.seq_id, max(cache.length, blocks * pool.block_size))
+
+    def _verify(self, pool, groups, lengths, temperature, uniforms, draft_probs) -> list[list[int]]:
+        T = sum(lengths)
         logits = F.linear(self._hidden(groups, list(range(T))), self.embed)
         offsets = [0]
         for n in lengths:

@@ -4,10 +4,13 @@ stand-in for the model that keeps the text in the cache's slots."""
 import pytest
 import torch
 
+from batchstream_inference_engine_b200 import torch_model
 from batchstream_inference_engine_b200.backend import PagedBackend
-from batchstream_inference_engine_b200.torch_model import ModelConfig, TorchModel, random_weights
+from batchstream_inference_engine_b200.block_allocator import OutOfBlocks
+from batchstream_inference_engine_b200.torch_model import (ModelConfig, PagedKVPool, TorchModel,
+                                                          random_weights)
 
-from .test_bounded_cache import TINY
+from .test_bounded_cache import TINY, mirrored
 
 END = 49
 PROMPT = [1, 2, 3, 4]
@@ -95,3 +98,97 @@ def test_a_sequence_that_a_drafted_step_ended_is_forked_as_after_plain_steps(mon
     assert backend.draft_step({}) == {} and backend.text(s) == text
     with pytest.raises(RuntimeError, match="finished"):
         backend.fork_sequence(s, [])
+
+
+def host_model(monkeypatch, accept, **config):
+    """A model whose step runs on the host, without its layers: sequences accept as many
+    drafts as `accept` says, one entry a group."""
+    config = ModelConfig(**TINY, **config)
+    model = TorchModel(config, random_weights(config, vocab_size=50, intermediate_size=16),
+                       device="cpu", dtype=torch.float32, max_position=64)
+    monkeypatch.setattr(model, "_stage", lambda values: torch.tensor(values, dtype=torch.int32))
+    monkeypatch.setattr(model, "_raise_status", lambda: None)
+    monkeypatch.setattr(model, "_layers", lambda pool, tokens, positions, slots, last, attend:
+                        torch.zeros(last.numel(), config.hidden_size))
+    monkeypatch.setattr(torch_model.ops, "step_metadata", lambda *a, **kw: (torch.zeros(9),) * 4)
+
+    def verify_drafts(logits, tokens, cu, uniforms, temperature, probs):
+        out = torch.full((tokens.numel(),), -1, dtype=torch.int32)
+        for b, n in enumerate(accept):
+            out[cu[b]: cu[b] + n] = tokens[cu[b]: cu[b] + n]
+            out[cu[b] + n] = 7
+        return out, torch.tensor(accept, dtype=torch.int32)
+
+    monkeypatch.setattr(torch_model.ops, "verify_drafts", verify_drafts)
+    return model
+
+
+def test_blocks_of_rejected_drafts_are_given_back(monkeypatch):
+    model = host_model(monkeypatch, [1, 0, 5])
+    pool = PagedKVPool(model.config, 40, 2, device="cpu", dtype=torch.float32, max_seqs=4)
+    caches = [pool.new_cache(i) for i in range(3)]
+    for cache, n in zip(caches, (3, 4, 1)):
+        cache.reserve(n)
+        cache.advance(n)
+    caches[2].reserve(11)  # what a caller holds ahead of its tokens stays
+    pool.allocator.sync_device()
+    free, held = pool.free_blocks, [list(pool.block_table(i)) for i in range(3)]
+    got = model.verify_tokens([([1, 2, 3, 4, 5], caches[0]), ([1, 2, 3, 4], caches[1]),
+                               ([1, 2, 3, 4, 5, 6], caches[2])])
+    assert got == [[2, 7], [7], [2, 3, 4, 5, 6, 7]]
+    assert [c.length for c in caches] == [5, 5, 7]
+    tables = [pool.block_table(i) for i in range(3)]
+    assert [len(t) for t in tables] == [3, 3, 6] and tables[2] == held[2]
+    assert pool.free_blocks == free - 2  # as plain steps of 2, 1 and 6 tokens would leave
+    assert tables[0][:2] == held[0] and tables[1][:2] == held[1]
+    assert sorted(pool.allocator._free + sum(tables, [])) == list(range(40))
+    # The device mirror learns of the blocks that come in their place.
+    for cache in caches[:2]:
+        cache.reserve(6)
+    pool.allocator.sync_device()
+    for i in range(2):
+        table = pool.block_table(i)
+        row = pool.allocator.device_tables[pool.allocator.row(i)]
+        assert row[: len(table)].tolist() == table
+
+
+def test_a_drafted_step_that_cannot_run_gives_back_what_it_took(monkeypatch):
+    model = host_model(monkeypatch, [0, 0])
+    pool = PagedKVPool(model.config, 8, 2, device="cpu", dtype=torch.float32, max_seqs=4)
+    caches = [pool.new_cache(i) for i in range(2)]
+    for cache in caches:
+        cache.reserve(2)
+        cache.advance(2)
+    free = list(pool.allocator._free)
+    with pytest.raises(OutOfBlocks):
+        model.verify_tokens([([1, 2, 3, 4, 5], caches[0]), ([1] * 9, caches[1])])
+    assert [c.length for c in caches] == [2, 2] and pool.allocator._free == free
+    pool = PagedKVPool(model.config, 40, 2, device="cpu", dtype=torch.float32, max_seqs=4)
+    cache = pool.new_cache(0)
+    cache.reserve(62)
+    cache.advance(62)
+    free = list(pool.allocator._free)
+    with pytest.raises(RuntimeError, match="rotary table"):
+        model.verify_tokens([([1, 2, 3], cache)])
+    assert cache.length == 62 and pool.allocator._free == free
+
+
+def test_shrink_gives_up_the_last_blocks():
+    a = mirrored(num_blocks=8)
+    a.allocate(0, 20)
+    a.fork(0, 1, 8)
+    a.sync_device()
+    table = list(a.block_table(0))
+    assert a.shrink(0, 20) == 0 and a.shrink(0, 17) == 0 and a.shrink(0, 16) == 1
+    assert a.block_table(0) == table[:4] and a._free[-1] == table[4]
+    assert a.shrink(0, 1) == 2  # the shared one of the three stays in use
+    assert a.block_table(0) == table[:1] and a.block_table(1) == table[:2]
+    a.allocate(0, 20)
+    a.sync_device()
+    assert a.device_tables[a.row(0), :5].tolist() == a.block_table(0)
+    assert a.shrink(7, 0) == 0  # (unknown: nothing to give up)
+    a.trim(0, 13)
+    assert a.block_table(0)[:3] == [-1] * 3
+    assert a.shrink(0, 8) == 2 and a.block_table(0) == [-1] * 2
+    a.allocate(0, 16)
+    assert a.trim(0, 16) == 2 and a.block_table(0) == [-1] * 4

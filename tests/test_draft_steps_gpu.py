@@ -8,7 +8,9 @@ import torch
 from batchstream_inference_engine_b200 import ops
 from batchstream_inference_engine_b200.backend import PagedBackend
 
-from .test_int4_engine_gpu import backend_of, check_generated, generate, prompts
+from .test_bounded_engine_gpu import VOCAB
+from .test_int4_engine_gpu import (CONFIG, WINDOWED, backend_of, check_generated, generate,
+                                  prompts)
 
 pytestmark = pytest.mark.gpu
 
@@ -58,4 +60,42 @@ def test_forks_of_sequences_that_a_drafted_step_ended(pool, behind):
             if pool == torch.uint8:
                 check_generated(backend, child, check, more, torch.float32)
         assert pool == torch.uint8 or runs[0] == runs[1]
+    assert ops.take_status() == 0
+
+
+def held_after(length, window, sinks, size=16):
+    """Blocks that a sequence of so many cached tokens holds after plain steps."""
+    gone = max(0, length - window + 1) // size - -(-sinks // size) if window else 0
+    return -(-length // size) - max(0, gone)
+
+
+@pytest.mark.parametrize("config", [CONFIG, WINDOWED])
+@pytest.mark.parametrize("pool", [torch.float32, torch.uint8])
+def test_rejected_drafts_leave_what_plain_steps_leave(config, pool):
+    # Chunks whose rejected end reaches into a new block, past the border where the window
+    # gives one up.
+    texts = prompts((130, 20))
+    _, want = generate(backend_of(config, pool=pool), texts, 80)
+    backend = backend_of(config, pool=pool)
+    ids, out = generate(backend, texts, 1)
+    turn = rejected = 0
+    while min(len(v) for v in out.values()) < 60:
+        drafts = {}
+        for i in ids:
+            drafts[i] = want[i][len(out[i]): len(out[i]) + turn % 4]
+            drafts[i] += [(t + 1) % VOCAB for t in want[i][len(out[i]) + len(drafts[i]):][:20 - turn % 7]]
+        for i, steps in backend.draft_step(drafts).items():
+            tokens = [o.token for o in steps]
+            assert tokens[:-1] == drafts[i][: len(tokens) - 1]
+            rejected += len(drafts[i]) + 1 - len(tokens)
+            out[i] += tokens
+        lengths = [backend._sequences[i].cache.length for i in ids]
+        assert lengths == [len(t) + len(out[i]) - 1 for t, i in zip(texts, ids)]
+        assert backend.blocks_in_use == sum(
+            held_after(n, config.attention_window, config.attention_sinks) for n in lengths)
+        turn += 1
+    assert rejected > 100
+    if pool == torch.float32:
+        for i in ids:
+            assert out[i][:80] == want[i][: len(out[i])]
     assert ops.take_status() == 0
