@@ -222,8 +222,13 @@ class PagedBackend:
         drafts gives one output, as in ``step``.  With temperature 0 the outputs are
         ``step``'s; else they are distributed as the model's samples at that temperature,
         by random numbers from ``generator`` (on the model's device).  Prompts wait for
-        ``step``; a launched step must be finished first.  Drafts behind one that would end
-        the generation are not looked at."""
+        ``step``; a launched step must be finished first.
+
+        Drafts behind one that would end the generation are not looked at, nor are those past
+        the last position, or for whose tokens no block is free once every sequence has one
+        for its next token: a step that runs without drafts runs with them, and behind it a
+        sequence holds the blocks of its cached tokens, as after plain steps.  What a request
+        may still generate is the caller's to know: outputs past that count against the pool."""
         batch = []
         for seq_id, tokens in self._generating_inputs():
             if self._sequences[seq_id].feeds is not None:
@@ -231,6 +236,7 @@ class PagedBackend:
             batch.append((seq_id, tokens + self._up_to_end(drafts.get(seq_id, ()))))
         if not batch:
             return {}
+        batch = self._with_room(batch)
         uniforms = None
         if temperature != 0.0:
             uniforms = torch.rand(sum(len(tokens) for _, tokens in batch), generator=generator,
@@ -264,6 +270,24 @@ class PagedBackend:
             if self._vocab.is_end_of_generation(token):
                 break
         return tokens
+
+    def _with_room(self, batch) -> list[tuple[int, list[int]]]:
+        """The batch with as many drafts of each sequence, in turn, as positions and blocks are
+        left for."""
+        pool, size = self._pool, self._pool.block_size
+        last = min(self._model.max_position, self._max_blocks * size)
+        lengths = [self._sequences[s].cache.length for s, _ in batch]
+        own = [max(pool.allocator.held_blocks(s), -(-(n + 1) // size))
+               for (s, _), n in zip(batch, lengths)]  # blocks, the next token's with them
+        free = pool.free_blocks - sum(
+            n - pool.allocator.held_blocks(s) for (s, _), n in zip(batch, own))
+        cut = []
+        for (seq_id, tokens), length, blocks in zip(batch, lengths, own):
+            room = min(last, (blocks + max(free, 0)) * size) - length
+            tokens = tokens[: max(room, 1)]
+            free -= max(0, -(-(length + len(tokens)) // size) - blocks)
+            cut.append((seq_id, tokens))
+        return cut
 
     def _generating_inputs(self) -> list[tuple[int, list[int]]]:
         return [

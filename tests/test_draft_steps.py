@@ -28,7 +28,7 @@ class Backend(PagedBackend):
         config = ModelConfig(**TINY, **config)
         model = TorchModel(config, random_weights(config, vocab_size=50, intermediate_size=16),
                            device="cpu", dtype=torch.float32, max_position=max_position)
-        super().__init__(model, num_blocks, block_size, 64, vocab=Vocab(), max_seqs=8)
+        super().__init__(model, num_blocks, block_size, 100, vocab=Vocab(), max_seqs=8)
         self.follow, self.slots = follow, {}
         monkeypatch.setattr(model, "next_tokens", None)
         monkeypatch.setattr(model, "launch_tokens", self._launch_tokens)
@@ -192,3 +192,67 @@ def test_shrink_gives_up_the_last_blocks():
     assert a.shrink(0, 8) == 2 and a.block_table(0) == [-1] * 2
     a.allocate(0, 16)
     assert a.trim(0, 16) == 2 and a.block_table(0) == [-1] * 4
+
+
+def started(backend, *lengths):
+    """Sequences that have generated a token behind prompts of so many tokens."""
+    ids = [backend.start_sequence(backend.follow[:n]) for n in lengths]
+    assert set(backend.step()) == set(ids)
+    return ids
+
+
+def test_drafts_stop_at_the_last_position(monkeypatch):
+    backend = Backend([t % 40 for t in range(80)], monkeypatch, num_blocks=80)
+    near, far = started(backend, 60, 5)
+    seen = []
+    verify = backend._model.verify_tokens
+
+    def verify_tokens(groups, *args):
+        seen.append([len(tokens) for tokens, _ in groups])
+        backend._model._check_positions([c.length for _, c in groups], seen[-1])
+        return verify(groups, *args)
+
+    monkeypatch.setattr(backend._model, "verify_tokens", verify_tokens)
+    follow = backend.follow
+    got = backend.draft_step({near: follow[61:70], far: follow[6:15]})
+    # 60 tokens are cached: the step holds four more, and the other sequence all of its.
+    assert seen == [[4, 10]]
+    assert [len(got[near]), len(got[far])] == [4, 10]
+    assert [o.token for o in got[far]] == follow[6:16]
+
+
+@pytest.mark.parametrize("free", [0, 1, 2, 3, 5, 50])
+def test_drafts_take_the_blocks_that_the_steps_tokens_leave(monkeypatch, free):
+    # Blocks of two tokens: the first sequence needs one for its own next token, the second
+    # has room for one draft, the third needs one too.
+    backend = Backend([t % 40 for t in range(80)], monkeypatch, block_size=2)
+    a, b, c = started(backend, 8, 7, 6)
+    taken = backend.pool.new_cache(99)
+    taken.reserve(2 * max(0, backend.pool.free_blocks - 2 - free))
+    drafts = {a: [1] * 5, b: [1] * 5, c: [1] * 5}
+    seen = []
+    verify = backend._model.verify_tokens
+
+    def verify_tokens(groups, *args):
+        seen.append([len(tokens) - 1 for tokens, _ in groups])
+        for tokens, cache in groups:
+            cache.reserve(len(tokens))
+        return verify(groups, *args)
+
+    monkeypatch.setattr(backend._model, "verify_tokens", verify_tokens)
+    got = backend.draft_step(drafts)
+    assert all(len(got[i]) >= 1 for i in (a, b, c))
+    # Each is given what is left in turn: one draft in its own block, two a block from there on
+    # (b's own block is the one its next token begins).
+    want = {0: [1, 0, 1], 1: [3, 0, 1], 2: [5, 0, 1], 3: [5, 2, 1], 5: [5, 5, 1], 50: [5, 5, 5]}
+    assert seen == [want[free]]
+
+
+def test_a_step_without_room_for_its_own_tokens_is_refused_as_a_plain_one(monkeypatch):
+    backend = Backend([t % 40 for t in range(80)], monkeypatch, num_blocks=20, block_size=2)
+    a, = started(backend, 8)
+    taken = backend.pool.new_cache(99)
+    taken.reserve(2 * backend.pool.free_blocks)
+    for step in (backend.step, lambda: backend.draft_step({a: [1, 2]})):
+        with pytest.raises(OutOfBlocks):
+            step()

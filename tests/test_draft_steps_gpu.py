@@ -99,3 +99,26 @@ def test_rejected_drafts_leave_what_plain_steps_leave(config, pool):
         for i in ids:
             assert out[i][:80] == want[i][: len(out[i])]
     assert ops.take_status() == 0
+
+
+@pytest.mark.parametrize("pool", [torch.float32, torch.uint8])
+def test_drafts_in_a_pool_that_the_outputs_fill(pool):
+    # As many blocks as 40 tokens each need: with 30 drafts each, every step runs.
+    texts = prompts()
+    blocks = sum(-(-(len(t) + 40) // 16) for t in texts)
+    _, want = generate(backend_of(pool=pool), texts, 80)
+    backend = backend_of(pool=pool, blocks=blocks)
+    ids, out = generate(backend, texts, 1)
+    while any(len(v) < 40 for v in out.values()):
+        # (A request generates 40 tokens, so its drafts are no more than are left.)
+        drafts = {i: want[i][len(out[i]):][: min(30, 39 - len(out[i]))] for i in ids}
+        drafts[ids[0]] = [(t + 1) % VOCAB for t in drafts[ids[0]]]  # none of them holds
+        for i, steps in backend.draft_step(drafts).items():
+            out[i] += [o.token for o in steps]
+            if len(out[i]) >= 40:
+                backend.release_sequence(i)
+                ids = [j for j in ids if j != i]
+    assert backend.blocks_in_use == 0 and not ids
+    if pool == torch.float32:
+        assert all(out[i] == want[i][:40] for i in out)
+    assert ops.take_status() == 0
