@@ -48,9 +48,10 @@ __device__ __forceinline__ bool ahead(float a, int32_t i, float b, int32_t j) {
   return a > b || (a == b && i < j);
 }
 
-// 1 / T as a factor of base-2 exponents; 0 stands for taking the largest logit.
+// Whether a temperature weighs tokens: from the smallest normal number on (log2(e) / T is then
+// finite in fp32).  0 and those below take the largest logit.
 __device__ __forceinline__ bool samples(float temperature) {
-  return temperature > 0.f && temperature < INFINITY;
+  return temperature >= 1.17549435e-38f && temperature < INFINITY;
 }
 
 // N elements of a row as they lie in memory, in 32-bit words.
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(kStatThreads, 6) draft_stats_kernel(const Draf
   const bool finite = top > -INFINITY && top < INFINITY, weigh = samples(s_temp) && finite;
   float sum = 0.f;
   if (weigh) {
-    const float scale = fminf(kLog2eF / s_temp, 3e38f);
+    const float scale = kLog2eF / s_temp;
     const float2 scale2 = make_float2(scale, scale), minus_top = make_float2(-top, -top);
     float2 sums = make_float2(0.f, 0.f);
 #pragma unroll
@@ -230,7 +231,7 @@ __device__ __forceinline__ RowStats join_row(const DraftArgs& a, int32_t row, fl
     }
   }
   if (samples(temperature) && s.top > -INFINITY && s.top < INFINITY) {
-    const float scale = fminf(kLog2eF / temperature, 3e38f);
+    const float scale = kLog2eF / temperature;
     if (mine.y > 0.f) s.sum = mine.y * fast_exp2((mine.x - s.top) * scale);
     for (int32_t c = lane + 32; c < a.pieces; c += 32) {
       const float4 r = __ldcg(rec + c);
@@ -250,40 +251,44 @@ __device__ __forceinline__ double cluster_load64(const double* p, uint32_t rank)
   return v;
 }
 
-// The double of a float that is not negative (of 0: 2^-127, which no sum notices; infinities
-// and NaN become large numbers).  Whole-number instructions: the fp64 units are what bounds
-// the draw.
+// The double of a float that is 0 or a positive normal number (of 0: 2^-127; infinities and NaN
+// become large numbers).  Whole-number instructions: the fp64 units are what bounds the draw.
 __device__ __forceinline__ double widen(float v) {
   const uint32_t u = __float_as_uint(v);
   return __hiloint2double(static_cast<int32_t>((u >> 3) + (896u << 20)),
                           static_cast<int32_t>(u << 29));
 }
 
-// How far a logit lies below the largest, in fp64.  Of bf16 logits the fp32 difference is
-// exact, but for logits 2^16 times smaller than the largest: off by 2^-24 of that one at most,
-// which moves the weights of the few that there are by less than the sums can show.
-__device__ __forceinline__ double distance(__nv_bfloat16, float top, float l) {
-  return widen(top - l);
-}
-__device__ __forceinline__ double distance(float, float top, float l) {
-  return static_cast<double>(top) - static_cast<double>(l);
-}
-
-// exp(-d / T) for d >= 0: 2^(k / 64) from a table times the series of e^(r ln 2 / 64) for the
-// rest, |r| <= 1/2, whose next term is below 2^-44 of it.  The constants live in registers (as
-// immediates each takes two moves at every use).
+// Weights exp((l - top) / T) of logits of type L: 2^(k / 64) from a table times the series of
+// e^(r ln 2 / 64) for the rest, |r| <= 1/2, whose next term is below 2^-44 of it.  The
+// constants live in registers (as immediates each takes two moves at every use).
+template <typename L>
 struct Weigher {
+  // Distances and T in units of 2^-66 where T is small: 0, which widen takes for 2^-127, then is
+  // below 2^-60 of T, and subnormal differences are normal numbers.
+  static constexpr bool kSmallUnits = sizeof(L) == 2;
   const double* table;
+  float units;
   double per_t, round, c4, c3, c2, c1;
   __device__ __forceinline__ Weigher(const double* t, float temperature) : table(t) {
     constexpr double kC = 0.010830424696249145;  // ln 2 / 64
-    per_t = -64.0 * 1.4426950408889634 / static_cast<double>(temperature);
+    units = kSmallUnits && temperature < 8.6736174e-19f /* 2^-60 */ ? 7.378697629e19f : 1.f;
+    per_t = -64.0 * 1.4426950408889634 / (static_cast<double>(temperature) * units);
     round = 6755399441055744.0;  // 1.5 * 2^52: a sum's low bits are the nearest whole number
     c4 = kC * kC * kC * kC / 24.0;
     c3 = kC * kC * kC / 6.0;
     c2 = kC * kC / 2.0;
     c1 = kC;
     asm volatile("" : "+d"(round), "+d"(c4), "+d"(c3), "+d"(c2), "+d"(c1));
+  }
+  __device__ __forceinline__ double exact_distance(float top, float l) const {
+    return (static_cast<double>(top) - static_cast<double>(l)) * units;
+  }
+  // Of bf16 logits the fp32 difference is exact, but for logits 2^16 times smaller than the
+  // largest: off by 2^-24 of that one at most, which moves the weights of the few that there are by
+  // less than the sums can show.
+  __device__ __forceinline__ double distance(float top, float l) const {
+    return kSmallUnits ? widen((top - l) * units) : exact_distance(top, l);
   }
   __device__ __forceinline__ double operator()(double d) const {
     const double t = fma(d, per_t, round);
@@ -318,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) draft_verify_kernel(const DraftAr
   const float temperature = a.temperature != nullptr ? a.temperature[b] : a.temperature_all;
   const bool sampled = samples(temperature);
   if (tid < 64) s_exp2[tid] = exp2(tid / 64.0);
-  const Weigher weight(s_exp2, sampled ? temperature : 1.f);
+  const Weigher<T> weight(s_exp2, sampled ? temperature : 1.f);
   // From this distance on the weight is 0 (2^-1000).
   const float most = sampled ? 1000.f * 0.69314718f * temperature : 0.f;
   const T* logits = static_cast<const T*>(a.logits);
@@ -347,8 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) draft_verify_kernel(const DraftAr
       } else if (!sampled) {
         take = x == s.arg;
       } else if (s.top > -INFINITY && s.top < INFINITY && s.top - l < most) {
-        const double p = weight(static_cast<double>(s.top) - static_cast<double>(l)) /
-                         static_cast<double>(s.sum);
+        const double p = weight(weight.exact_distance(s.top, l)) / static_cast<double>(s.sum);
         take = static_cast<double>(u) * static_cast<double>(q) < p;
       }
       if (!take) atomicMin(&s_first, i);
@@ -374,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) draft_verify_kernel(const DraftAr
     }
     if (tid == 0) {
       a.accepted[b] = taken;
-      if (!sampled && temperature != 0.f) set_status(a.status, kStatusBadValue);
+      if (!(temperature >= 0.f && temperature < INFINITY)) set_status(a.status, kStatusBadValue);
     }
   }
   const bool weighable = top > -INFINITY && top < INFINITY;
@@ -422,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1) draft_verify_kernel(const DraftAr
     for (int i = 0; i < 8; ++i) {
       const float l = b.l.at(i);
       bool keep = top - l < most;
-      w[i] = weight(distance(T(), top, l));
+      w[i] = weight(weight.distance(top, l));
       if (rest) {  // where p is above q (of the high word: neither negative nor NaN)
         w[i] = fma(w[i], inv_z, -widen(fabsf(b.q.at(i))));
         keep = keep && static_cast<uint32_t>(__double2hiint(w[i])) < 0x7ff00000u;

@@ -982,8 +982,9 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, cu_rows: tor
     if u q(x) < p(x); at the first that is not, a token is drawn from max(p - q, 0) (from p
     without x where drafts are certain, from p where nothing is left), behind the last one
     from p, with the u of the sequence's last row.  So the tokens are distributed as the
-    target's own.  ``temperature`` (a number, or fp32 [B]) 0 accepts what the largest logit
-    (the first, as ``argmax_rows``) would have been, and ends with it.
+    target's own.  ``temperature`` (a number, or fp32 [B]) 0, or below the smallest normal fp32
+    number, accepts what the largest logit (the first, as ``argmax_rows``) would have been,
+    and ends with it.
 
     Returns int32 (tokens [N], accepted [B]): at each sequence's rows its accepted drafts,
     the token after them, then -1s (also at rows of no sequence); and how many drafts were

@@ -493,8 +493,9 @@ int bs_int4_prefill_attention_workspace_bytes(int64_t num_tokens, int64_t num_ro
  *     or x where x has all the weight), with all accepted from p of the last row: the first
  *     token at which the running sum of the weights, in fp64, exceeds uniforms[last row]
  *     times their sum.
- * temperatures[b] (or `temperature` for all, where it is NULL) of 0 accepts and takes the
- * first largest logit instead, as bs_argmax_rows does.
+ * temperatures[b] (or `temperature` for all, where it is NULL) of 0, or below the smallest
+ * normal fp32 number, accepts and takes the first largest logit instead, as bs_argmax_rows
+ * does.
  *
  * tokens_out[num_rows] holds, at each sequence's rows, its accepted drafts, the token after
  * them, and -1s (as at rows of no sequence); accepted_out[b] counts the accepted drafts.  A
