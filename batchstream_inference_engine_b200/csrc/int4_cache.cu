@@ -115,7 +115,8 @@ template <typename F>
 __device__ __forceinline__ void quantise(const F (&x)[8], bool mine, int quad, uint32_t* codes,
                                          uint16_t* scale, uint32_t* status) {
   // Largest elements of either side, rounded up to fp32 (which the 4-bit rounding up does not
-  // notice) and compared by their bits, in which NaN is the largest.
+  // notice) and compared by their bits, in which NaN is the largest.  Where those are equal, or
+  // at a limit, the elements themselves are compared.
   float size[8];
   uint32_t hi = 0, lo = 0;
 #pragma unroll
@@ -133,13 +134,36 @@ __device__ __forceinline__ void quantise(const F (&x)[8], bool mine, int quad, u
     hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, o));
   }
-  const uint32_t top = max(hi, lo);
+  const uint32_t top = max(hi, lo), huge = __float_as_uint(kHuge), tiny = __float_as_uint(kTiny);
+  bool too_large = top >= huge, held = top >= tiny, mirrored = lo < hi;
+  if constexpr (sizeof(F) == 8) {
+    if (__any_sync(0xffffffffu, hi == lo || top == huge || top == tiny)) {
+      double above = 0.0, below = 0.0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (negative(x[j])) {
+          below = fmax(below, -x[j]);
+        } else {
+          above = fmax(above, x[j]);
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        above = fmax(above, __shfl_xor_sync(0xffffffffu, above, o));
+        below = fmax(below, __shfl_xor_sync(0xffffffffu, below, o));
+      }
+      const double most = fmax(above, below);
+      too_large = top > huge || most >= kHuge;  // (NaN is in `top` alone)
+      held = most >= kTiny;
+      mirrored = below < above;
+    }
+  }
   float s = 0.f;
-  if (top >= __float_as_uint(kHuge)) {  // (infinity and NaN too)
+  if (too_large) {  // (infinity and NaN too)
     if (mine && quad == 0) set_status(status, kStatusBadValue);
-  } else if (top >= __float_as_uint(kTiny)) {
+  } else if (held) {
     s = __uint_as_float((__float_as_uint(__uint_as_float(top) * 0.125f) + 0xfffffu) & 0xfff00000u);
-    if (lo < hi) s = -s;
+    if (mirrored) s = -s;
   }
   if (!mine) return;
   uint32_t word = 0x88888888u;  // zeros
