@@ -95,7 +95,7 @@ struct OutRows {
   int32_t heads, rows;
   __device__ __forceinline__ OutRows(const DecodeArgs& a, int32_t seq, int32_t kvh) {
     if constexpr (CHUNK) {
-      const int2 tokens = __ldg(a.chunk_rows + seq);
+      const int2 tokens = coherent_load(a.chunk_rows + seq);
       stride = a.o_stride_seq;
       heads = a.chunk_heads;
       rows = tokens.y * heads;
@@ -189,8 +189,8 @@ __device__ __forceinline__ int32_t seq_units_raw(const DecodeArgs& a, int32_t ra
 template <bool WIN = false>
 __device__ __forceinline__ int32_t seq_units(const DecodeArgs& a, int32_t i, int32_t& len,
                                              int32_t& row, bool report) {
-  return seq_units_raw<WIN>(a, __ldg(a.context_lens + i),
-                       a.seq_rows != nullptr ? __ldg(a.seq_rows + i) : i, len, row, report);
+  return seq_units_raw<WIN>(a, coherent_load(a.context_lens + i),
+                       a.seq_rows != nullptr ? coherent_load(a.seq_rows + i) : i, len, row, report);
 }
 
 struct Span {
@@ -470,10 +470,10 @@ __device__ __forceinline__ Span compute_warp_spans(const DecodeArgs& a, ScanSmem
   }
   if (tid < NW && ws.seq[tid] >= 0) {
     const int32_t i = ws.seq[tid];
-    ws.len[tid] = __ldg(a.context_lens + i);
-    ws.row[tid] = a.seq_rows != nullptr ? __ldg(a.seq_rows + i) : i;
-    ws.nlen[tid] = i + 1 < B ? __ldg(a.context_lens + i + 1) : 0;
-    ws.nrow[tid] = i + 1 < B ? (a.seq_rows != nullptr ? __ldg(a.seq_rows + i + 1) : i + 1) : 0;
+    ws.len[tid] = coherent_load(a.context_lens + i);
+    ws.row[tid] = a.seq_rows != nullptr ? coherent_load(a.seq_rows + i) : i;
+    ws.nlen[tid] = i + 1 < B ? coherent_load(a.context_lens + i + 1) : 0;
+    ws.nrow[tid] = i + 1 < B ? (a.seq_rows != nullptr ? coherent_load(a.seq_rows + i + 1) : i + 1) : 0;
   }
   __syncthreads();
   sp.seq = ws.seq[0];
@@ -505,8 +505,8 @@ __device__ __forceinline__ Span compute_warp_spans_smem(const DecodeArgs& a, Sca
   for (int32_t k = 0; k < per; ++k) {
     const int32_t i = i0 + k;
     if (i >= B) break;
-    const int32_t len = __ldg(a.context_lens + i);
-    const int32_t row = a.seq_rows != nullptr ? __ldg(a.seq_rows + i) : i;
+    const int32_t len = coherent_load(a.context_lens + i);
+    const int32_t row = a.seq_rows != nullptr ? coherent_load(a.seq_rows + i) : i;
     lens[i] = len;
     rows[i] = row;
     int32_t l2, r2;

@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(128, (Cfg<D, NQ, CHUNK>::MIN_CTAS))
     }
     const int32_t tok0 = tu * kWindowUnit;
     int2 tokens{};
-    if constexpr (CHUNK) tokens = __ldg(a.chunk_rows + ci);
+    if constexpr (CHUNK) tokens = coherent_load(a.chunk_rows + ci);
     // What the last token sees, or any of them.
     const int32_t lo = CHUNK ? clen - a.chunk_window - (tokens.y - 1) : clen - a.window;
     auto below = [](int32_t c) {  // map of a unit's first c tokens
@@ -260,8 +260,8 @@ __global__ void __launch_bounds__(128, (Cfg<D, NQ, CHUNK>::MIN_CTAS))
           cnb = ci < a.num_seqs ? seq_units<true>(a, ci, clen, crow, false) : 1;
         }
         if (ci + 1 < a.num_seqs) {
-          nxt_len = __ldg(a.context_lens + ci + 1);
-          nxt_row = a.seq_rows != nullptr ? __ldg(a.seq_rows + ci + 1) : ci + 1;
+          nxt_len = coherent_load(a.context_lens + ci + 1);
+          nxt_row = a.seq_rows != nullptr ? coherent_load(a.seq_rows + ci + 1) : ci + 1;
         }
       }
     }

@@ -306,8 +306,8 @@ __global__ void __maxnreg__((Cfg<D, G16>::MAX_REGS))
         }
         if constexpr (WIN) cw = window_units(a, max(clen, 0));
         if (ci + 1 < a.num_seqs) {
-          nxt_len = __ldg(a.context_lens + ci + 1);
-          nxt_row = a.seq_rows != nullptr ? __ldg(a.seq_rows + ci + 1) : ci + 1;
+          nxt_len = coherent_load(a.context_lens + ci + 1);
+          nxt_row = a.seq_rows != nullptr ? coherent_load(a.seq_rows + ci + 1) : ci + 1;
         }
       }
     }

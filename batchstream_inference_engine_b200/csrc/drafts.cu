@@ -66,7 +66,7 @@ struct Raw {
   __device__ __forceinline__ void load(const T* p) {  // on 16 bytes
 #pragma unroll
     for (int k = 0; k < WORDS; k += 4) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + k / 4);
+      const uint4 v = coherent_load(reinterpret_cast<const uint4*>(p) + k / 4);
       w[k] = v.x;
       w[k + 1] = v.y;
       w[k + 2] = v.z;

@@ -68,14 +68,14 @@ struct WindowTile {
 // was), or an invalid row, reported when `report`.
 __device__ __forceinline__ bool window_tile(const WindowArgs& a, int32_t r, int32_t tile,
                                             WindowTile& w, bool report) {
-  const int32_t ctx = __ldg(a.context_lens + r);
+  const int32_t ctx = coherent_load(a.context_lens + r);
   int32_t tok0 = r, n = 1;
   if (a.cu_q != nullptr) {
-    tok0 = __ldg(a.cu_q + r);
-    n = __ldg(a.cu_q + r + 1) - tok0;
+    tok0 = coherent_load(a.cu_q + r);
+    n = coherent_load(a.cu_q + r + 1) - tok0;
   }
   if (ctx == 0 || n == 0) return false;
-  w.row = a.seq_rows != nullptr ? __ldg(a.seq_rows + r) : r;
+  w.row = a.seq_rows != nullptr ? coherent_load(a.seq_rows + r) : r;
   if (w.row < 0 || w.row >= a.bt_rows) {
     if (report) set_status(a.status, kStatusBadRow);
     return false;

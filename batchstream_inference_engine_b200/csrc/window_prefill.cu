@@ -185,9 +185,9 @@ __device__ __forceinline__ void ranked_tile(const WindowArgs& a, int32_t b, int3
   const int t = threadIdx.x;
   int32_t mine = 0;
   if (t < a.num_rows) {
-    const int32_t tokens = __ldg(a.cu_q + t + 1) - __ldg(a.cu_q + t);
+    const int32_t tokens = coherent_load(a.cu_q + t + 1) - coherent_load(a.cu_q + t);
     // Keys that the chunk's last tile reads, near enough for an order.
-    if (tokens > 0) mine = min(__ldg(a.context_lens + t), a.window + a.tile_tokens);
+    if (tokens > 0) mine = min(coherent_load(a.context_lens + t), a.window + a.tile_tokens);
     steps[t] = mine;
   }
   __syncthreads();
@@ -370,8 +370,10 @@ __global__ void __launch_bounds__((Cfg<D, TILES>::THREADS), (Cfg<D, TILES>::MIN_
         }
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-          c.words[e][p] = __ldg(reinterpret_cast<const uint4*>(codes + p * ROWS * int4_code_bytes(D)));
-          c.scale[e][p] = __ldg(reinterpret_cast<const uint16_t*>(scales + p * ROWS * int4_scale_bytes(D)));
+          c.words[e][p] =
+              coherent_load(reinterpret_cast<const uint4*>(codes + p * ROWS * int4_code_bytes(D)));
+          c.scale[e][p] = coherent_load(
+              reinterpret_cast<const uint16_t*>(scales + p * ROWS * int4_scale_bytes(D)));
         }
       }
     };

@@ -226,8 +226,8 @@ __global__ void __launch_bounds__(kThreads) window_simt_kernel(const WindowArgs 
           const int64_t so = __shfl_sync(0xffffffffu, scales, key);
           to[k] = ko < 0 ? -1 : key * k_row + 32 * c;
           if (ko < 0) continue;
-          words[k] = __ldg(reinterpret_cast<const uint32_t*>(bytes + ko) + c);
-          scale[k] = __ldg(reinterpret_cast<const uint16_t*>(bytes + so) + (c >> 2));
+          words[k] = coherent_load(reinterpret_cast<const uint32_t*>(bytes + ko) + c);
+          scale[k] = coherent_load(reinterpret_cast<const uint16_t*>(bytes + so) + (c >> 2));
         }
 #pragma unroll
         for (int k = 0; k < kAtOnce; ++k) {
