@@ -31,6 +31,7 @@ from __future__ import annotations
 
 import json
 import struct
+import weakref
 from dataclasses import dataclass, field
 from pathlib import Path
 
@@ -430,7 +431,8 @@ class TorchModel:
         self.max_graph_batch = max_graph_batch
         self.max_graph_prefill = max_graph_prefill
         self.max_graph_chunks = max_graph_chunks
-        self._graphs: dict[tuple, tuple] = {}
+        # A pool's graphs, by shape, for as long as there is the pool whose memory they name.
+        self._graphs: weakref.WeakKeyDictionary[PagedKVPool, dict] = weakref.WeakKeyDictionary()
         self._graph_stream = None
         self._graph_pool = None
         self._graph_ws = None
@@ -871,9 +873,15 @@ class TorchModel:
             (b, rows, q) for b in decode for rows in _powers_of_two(1, self.max_graph_chunks)
             for q in _powers_of_two(64, self.max_graph_prefill)]
         for key in keys:
-            if (id(pool),) + key not in self._graphs:
-                self._capture(pool, key)
+            self._graph(pool, key)
         return len(keys)
+
+    def _graph(self, pool: PagedKVPool, key) -> tuple:
+        """The captured step of this shape on `pool` (captured now if it is the first)."""
+        graphs = self._graphs.setdefault(pool, {})
+        if key not in graphs:
+            graphs[key] = self._capture(pool, key)
+        return graphs[key]
 
     def _capture(self, pool: PagedKVPool, key):
         if self._graph_stream is None:
@@ -905,17 +913,12 @@ class TorchModel:
                 raise RuntimeError("the graph workspace moved during capture")
             ops.take_status(self.device)
         torch.cuda.current_stream(self.device).wait_stream(stream)
-        entry = (inputs, graph, ids, launches)
-        self._graphs[(id(pool),) + key] = entry
-        return entry
+        return inputs, graph, ids, launches
 
     def _graph_step(self, groups, key) -> PendingTokens:
         config = self.config
         pool = groups[0][1]._pool
-        entry = self._graphs.get((id(pool),) + key)
-        if entry is None:
-            entry = self._capture(pool, key)
-        inputs, graph, ids, graph_launches = entry
+        inputs, graph, ids, graph_launches = self._graph(pool, key)
         for tokens, cache in groups:
             cache.reserve(len(tokens))
         alloc = pool.allocator
