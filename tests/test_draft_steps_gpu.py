@@ -9,7 +9,7 @@ from batchstream_inference_engine_b200 import ops
 from batchstream_inference_engine_b200.backend import PagedBackend
 
 from .test_bounded_engine_gpu import VOCAB
-from .test_int4_engine_gpu import (CONFIG, WINDOWED, backend_of, check_generated, generate,
+from .test_int4_engine_gpu import (CONFIG, DEV, WINDOWED, backend_of, check_generated, generate,
                                   prompts)
 
 pytestmark = pytest.mark.gpu
@@ -122,3 +122,57 @@ def test_drafts_in_a_pool_that_the_outputs_fill(pool):
     if pool == torch.float32:
         assert all(out[i] == want[i][:40] for i in out)
     assert ops.take_status() == 0
+
+
+@torch.inference_mode()
+def step_logits(model, groups):
+    """The logits of every token of a step, which counts none of them as cached."""
+    hidden = model._hidden(groups, list(range(sum(len(tokens) for tokens, _ in groups))))
+    return torch.nn.functional.linear(hidden, model.embed)
+
+
+@pytest.mark.parametrize("pool", [torch.float32, torch.uint8])
+def test_verify_tokens_with_draft_probabilities(pool):
+    # The model's step with probabilities gives what verify_drafts gives of the same step's
+    # logits; temperatures by sequence, greedy among them.
+    texts = prompts((50, 7, 33))
+    backend = backend_of(pool=pool)
+    model = backend._model
+    ids, out = generate(backend, texts, 1)
+    g = torch.Generator().manual_seed(11)
+    accepted = rejected = 0
+    for turn in range(8):
+        caches = [backend._sequences[i].cache for i in ids]
+        lengths = [c.length for c in caches]
+        n = [int(torch.randint(0, 5, (1,), generator=g)) for _ in ids]
+        T = sum(n) + len(ids)
+        groups, at = [], [0]
+        for i, k, cache in zip(ids, n, caches):
+            groups.append([out[i][-1], *torch.randint(0, VOCAB, (k,), generator=g).tolist()])
+            at.append(at[-1] + k + 1)
+        # Every other turn's first drafts come from a sharper target: most of them hold.
+        probs = torch.softmax(step_logits(model, list(zip(groups, caches))).float() * 3, -1)
+        for b, tokens in enumerate(groups):
+            for k in range(len(tokens) - 1):
+                if turn % 2 == 0 and k == 0:
+                    tokens[1] = int(torch.multinomial(probs[at[b]].cpu(), 1, generator=g))
+        groups = list(zip(groups, caches))
+        logits = step_logits(model, groups)
+        uniforms = torch.rand(T, generator=g).to(DEV)
+        temperature = torch.tensor([0.9, 0.0, 1.4], device=DEV)
+        drafts = [t for tokens, _ in groups for t in (*tokens[1:], 0)]
+        want, taken = ops.verify_drafts(
+            logits, torch.tensor(drafts, dtype=torch.int32, device=DEV),
+            torch.tensor(at, dtype=torch.int32, device=DEV), uniforms, temperature, probs)
+        got = model.verify_tokens(groups, temperature, uniforms, probs)
+        for b, tokens in enumerate(got):
+            k = int(taken[b])
+            assert tokens == want[at[b]: at[b] + k + 1].tolist()
+            assert caches[b].length == lengths[b] + k + 1
+            out[ids[b]] += tokens
+            accepted += k
+            rejected += n[b] - k
+    assert accepted > 3 and rejected > 3 and ops.take_status() == 0
+    with pytest.raises(RuntimeError, match="draft_probs"):
+        model.verify_tokens(groups, temperature, uniforms, probs[:, :-1])
+    assert [c.length for c in caches] == [len(t) + len(out[i]) - 1 for t, i in zip(texts, ids)]
