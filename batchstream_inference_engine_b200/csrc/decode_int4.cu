@@ -32,11 +32,13 @@
 // row by row.  chunk_rows_kernel lists them ahead.
 //
 // 256 sequences of 512 to 32768 tokens (log-uniform), 28 + 4 heads of 128, 1.05 GB of codes and
-// scales: 279 us, 3.8 TB/s, 57% of a plain copy's rate.  What bounds it is issuing: 340
-// instructions for 16 tokens of 128 dims, half of them what turns codes into operands, 2.2 a
-// clock and SM, DRAM 40% busy.  64 sequences of 1 to 16384, 14 + 2 heads of 64: 24 us (floor
-// 1.9): launch, search of the spans, table entries, codes and joins follow one another for 2
-// to 4 units a warp.  One sequence of 77: 5.4 us.  The pools as bf16 (window attention's
+// scales: 280 us, 3.8 TB/s, 57% of a plain copy's rate.  What bounds it is latency inside a
+// warp: codes, operands, scores, weights and second product follow one another, 340
+// instructions for 16 tokens of 128 dims, half of them what turns codes into operands, and
+// three warps a scheduler issue 2.2 of 4 a clock and SM (DRAM 40% busy).  64 sequences of 1 to
+// 16384, 14 + 2 heads of 64: 24 us (floor 1.9): launch, search of the spans, table entries,
+// codes and joins follow one another for 5.9 units a warp (10426 on 444 CTAs), and the
+// merge behind them.  One sequence of 77: 5.4 us.  The pools as bf16 (window attention's
 // decode): 43 us for 64 of 1 to 8192 at d64, 37 here; at d128 111 and 68.
 // Not kept: a join by all threads of CTAs that hold one segment only (the same time).
 #include <type_traits>

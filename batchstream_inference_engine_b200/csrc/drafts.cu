@@ -11,18 +11,24 @@
 // exceeds u times their sum, u of the sequence's last row.  T = 0 takes the largest logit.
 //
 // draft_stats_kernel reads every logit once: a CTA holds a piece of a row in registers and
-// leaves its maximum, the sum of its exponentials and the first index of the maximum.
+// leaves its maximum, the sum of its exponentials and the first index of the maximum.  That
+// sum, of the acceptance, is fp32: where 2^17 tokens weigh 2^-17 each, an exponent is off by
+// 3.5 * 2^-24 of 17 (the difference, log2(e) / T, their product), ex2 by 2^-22 and the sums by
+// some 30 roundings: 2^-17 of the sum at most.  In fp64 a pass over every row would cost what
+// one of the draw's costs over a row of each sequence.
+//
 // draft_verify_kernel, a cluster per sequence, joins them, finds the row that ends the
 // step and draws from it alone, in fp64: the sums run over the whole vocabulary, and where
 // its tokens weigh 1e-5 each, an error of 1e-7 in the sum ahead of one moves one draw in a
 // hundred to its neighbour.  Each warp sums a range of the row in blocks of 256 tokens and
 // keeps the sums of up to 64 parts of it, so that the draw walks one part again.
 //
-// 64 sequences with four drafts each from a small model, 151936 bf16 logits: 72 us (floor 15),
-// 28 of them the first pass, 3.5 TB/s, bound by issuing and by CTAs that each hold one piece
-// (2.4 instructions a clock and SM, DRAM 42% busy); the rest is the draw, two passes over a row's
-// weights, some 20 instructions a token (2.4 a clock and SM, fp64 units 28% busy).  One sequence:
-// 13 us; 200 ragged ones, 32003 fp32 logits: 54 (floor 16).  Not kept: 768 or 1024 threads a
+// 64 sequences with four drafts each from a small model, 151936 bf16 logits: 73 us (floor 15),
+// 28 of them the first pass, 3.5 TB/s, bound by the latency of CTAs that each load one piece, then
+// work on it (2.4 of 4 instructions a clock and SM, DRAM 42% busy); the rest is the draw, two passes
+// over a row's weights, some 20 instructions a token, on 128 of 148 SMs with 16 warps each: latency
+// again (2.4 of 4, fp64 units 28% busy).  One sequence: 13 us; 200 ragged ones, 32003 fp32
+// logits: 55 (floor 16).  Not kept: 768 or 1024 threads a
 // drawing CTA, four or eight CTAs an SM in the first pass (within 3%).
 #include "common.cuh"
 #include "drafts.cuh"

@@ -989,7 +989,13 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, cu_rows: tor
     Returns int32 (tokens [N], accepted [B]): at each sequence's rows its accepted drafts,
     the token after them, then -1s (also at rows of no sequence); and how many drafts were
     accepted.  A sequence without rows is padding.  Bad row offsets, drafts outside the
-    vocabulary, rows without a finite maximum and bad temperatures are reported
-    (``take_status``); the latter two take the largest logit.
+    vocabulary, deciding rows without a finite maximum at a temperature that is not 0, and
+    bad temperatures are reported (``take_status``); the latter two take the largest logit.
+    At temperature 0 a NaN counts as the largest, as in ``argmax_rows``, and nothing is
+    reported.
+
+    The draw's weights and sums are fp64.  p(x) of the acceptance is an fp64 weight over an
+    fp32 sum of fp32 exponentials, so a draft nearer to its border than 2^-17 of p(x) may
+    fall on either side.
     """
     return _native.verify_drafts(logits, draft_tokens, cu_rows, uniforms, temperature, draft_probs)

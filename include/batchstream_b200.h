@@ -495,14 +495,16 @@ int bs_int4_prefill_attention_workspace_bytes(int64_t num_tokens, int64_t num_ro
  *     times their sum.
  * temperatures[b] (or `temperature` for all, where it is NULL) of 0, or below the smallest
  * normal fp32 number, accepts and takes the first largest logit instead, as bs_argmax_rows
- * does.
+ * does (a NaN counts as the largest, and is not reported).  p_r(x) of an acceptance is an
+ * fp64 weight over an fp32 sum of fp32 exponentials: off by 2^-17 of it at most.
  *
  * tokens_out[num_rows] holds, at each sequence's rows, its accepted drafts, the token after
  * them, and -1s (as at rows of no sequence); accepted_out[b] counts the accepted drafts.  A
  * sequence without rows is padding.  cu_rows that run backwards or past num_rows
  * (BS_STATUS_BAD_LENGTH) accept nothing and write no token; a draft outside the vocabulary
- * (BS_STATUS_BAD_INDEX) is not accepted; where a row that decides has no finite maximum or
- * the temperature is negative or not finite (BS_STATUS_BAD_VALUE) the largest logit is taken.
+ * (BS_STATUS_BAD_INDEX) is not accepted; where a row that decides by sampling has no finite
+ * maximum, or the temperature is negative or not finite (BS_STATUS_BAD_VALUE), the largest
+ * logit is taken.
  *
  * `workspace`: scratch of the queried size, 16-byte aligned, its contents irrelevant, one
  * per call in flight.
