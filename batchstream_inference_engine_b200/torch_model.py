@@ -886,6 +886,7 @@ class TorchModel:
     def _capture(self, pool: PagedKVPool, key):
         if self._graph_stream is None:
             self._graph_stream = torch.cuda.Stream(self.device)
+        if not any(self._graphs.values()):  # the memory that graphs share goes with the last one
             self._graph_pool = torch.cuda.graph_pool_handle()
         stream = self._graph_stream
         stream.wait_stream(torch.cuda.current_stream(self.device))
